@@ -37,6 +37,7 @@ extern "C" {
 #define B200Q_F32 0
 #define B200Q_F16 1
 #define B200Q_BF16 2
+#define B200Q_E4M3 3   /* FP8 E4M3 codes: pages of a key-value cache only */
 
 typedef void* b200q_stream_t;
 
@@ -408,6 +409,85 @@ int b200q_fp8_attention(const void* q, const void* k, const void* v, int dtype, 
  * and V slices of a QKV projection in one pass.  c1, c2, c3 >= 0, multiples of 16; x 32-byte aligned. */
 int b200q_amax_columns(const void* x, int dtype, int64_t rows, int64_t c1, int64_t c2, int64_t c3, float* amax_out,
                        b200q_stream_t stream);
+
+/* ------------------------------------------------------------------ paged key-value cache
+ * What a decoder keeps of the tokens it has seen, and the attention of the tokens that follow.  No counterpart in the
+ * reference's quantized-linear path.
+ *
+ * K and V live in pages of `page_size` rows of D elements per kv head.  Element (page, head, row, i) of K lies at
+ * k_pages + page * k_strides[0] + head * k_strides[1] + row * k_strides[2] + i (elements), so a pool may be stored
+ * [pages, heads, rows, D] or [pages, rows, heads, D].  Token t of sequence b is row t % page_size of page
+ * block_table[b * table_stride + t / page_size].  `lens[b]` tokens of sequence b are in the cache, the newest included.
+ * A length beyond the table's width is cut to it, a negative one is zero; a table entry outside [0, num_pages) stands for
+ * rows that are not there: they are not read, not written and not attended to.
+ *   dtype       B200Q_F16, B200Q_BF16, or B200Q_E4M3: codes of x / scale with scale = amax / 448 (zero -> 1)
+ *   k_amax,     B200Q_E4M3 only: the calibrated abs-max of K and V on the device, amax_numel = 1 (all heads) or
+ *   v_amax      `heads` (one per kv head)
+ * D a multiple of 16 up to 128; pages 16-byte aligned, strides multiples of 16 bytes. */
+typedef struct b200q_paged_cache {
+  void* k_pages;
+  void* v_pages;
+  int32_t dtype;
+  int32_t page_size;
+  int64_t num_pages, heads, D;
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  const float* k_amax;
+  const float* v_amax;
+  int64_t amax_numel;
+} b200q_paged_cache;
+
+/* The rows of T new tokens into their pages: k, v [T, heads, D] (dtype B200Q_F16 or B200Q_BF16; the pages' own unless
+ * those hold codes), strides: token and head of k, then of v (elements, multiples of 16 bytes, D contiguous).  The tokens
+ * of sequence b are rows cu_new[b] .. cu_new[b + 1] of k and v (cu_new[0] = 0, cu_new[B] = T, ascending) and the LAST of
+ * its lens[b]; cu_new NULL: one token of every sequence, T = B. */
+int b200q_paged_append(const void* k, const void* v, int dtype, const int64_t* strides, int64_t T, const int32_t* cu_new,
+                       const b200q_paged_cache* cache, const int32_t* block_table, int64_t table_stride,
+                       int64_t table_width, const int32_t* lens, int64_t B, b200q_stream_t stream);
+
+/* Attention of one new token of every sequence over its cache: out [B, Hq, D] (contiguous, q's dtype), q [B, Hq, D] with
+ * strides q_strides (batch, head; multiples of 16 bytes), dtype B200Q_F16 or B200Q_BF16 (the pages' own unless those hold
+ * codes).  Query head h reads kv head h / (Hq / heads).  The token at position p = lens[b] - 1 sees the keys j <= p with
+ * j > p - window or j < sinks (window <= 0: all of them).
+ *   P = softmax(q K^T * scale) in fp32, out = P V; a sequence without keys gets zeros.
+ * weights (may be NULL): fp32 [B, heads, weights_len], contiguous; weights[b, h, j] += the sum of P over the query heads of
+ * kv head h, for keys j < weights_len that are seen.
+ * workspace: b200q_paged_attention_workspace_bytes() bytes, 16-byte aligned, zero the first time it is used and left zero
+ * where it has to be; calls sharing one must not overlap.  scratch (with weights only):
+ * b200q_paged_attention_scratch_bytes(B, Hq, weights_len) bytes, any content. */
+size_t b200q_paged_attention_workspace_bytes(void);
+size_t b200q_paged_attention_scratch_bytes(int64_t B, int64_t Hq, int64_t weights_len);
+int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, const b200q_paged_cache* cache,
+                          const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* lens,
+                          int64_t B, int64_t Hq, float scale, int64_t window, int64_t sinks, void* out, float* weights,
+                          int64_t weights_len, void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes,
+                          b200q_stream_t stream);
+
+/* Which keys stay, and their rows moved to fresh pages.  Of a sequence's n = lens[b] tokens each kv head keeps
+ * min(n, keep): the first `sinks`, the last `recent`, and of the others those of the largest weights[b, h, :] (fp32
+ * [B, heads, weights_len], contiguous; equal ones: the lower token; NaN counts as -inf).  sinks + recent <= keep.
+ * Their rows go, in the order of the tokens, to rows 0, 1, .. of the pages out_table[b * out_stride + ..]; these pages
+ * must not hold rows that the call reads.  Pages may be shared between sequences on the reading side.
+ *   kept         int32 [B, heads, keep]: the tokens kept, ascending, -1 beyond the last
+ *   new_lens     int32 [B]: min(n, keep)
+ *   new_weights  fp32 [B, heads, weights_len]: the kept weights in the same order, zero beyond; not `weights` itself
+ * weights_len >= keep, and a sequence has at most weights_len tokens (a longer one is cut to it). */
+int b200q_paged_evict(const b200q_paged_cache* cache, const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                      const int32_t* lens, const float* weights, int64_t weights_len, const int32_t* out_table,
+                      int64_t out_stride, int64_t out_width, int64_t B, int64_t keep, int64_t recent, int64_t sinks,
+                      int32_t* kept, int32_t* new_lens, float* new_weights, b200q_stream_t stream);
+
+/* Causal attention with a sliding window and sinks over contiguous K and V: q [B, Hq, Sq, D], k and v [B, Hkv, Sk, D] of one
+ * dtype (B200Q_F16 or B200Q_BF16), out [B, Hq, Sq, D]; strides: batch, head, row of q, then of k, then of v, out_strides
+ * those of out (elements, multiples of 16 bytes, D contiguous).  Sequence b has q_lens[b] queries and k_lens[b] keys (NULL:
+ * Sq and Sk); its query i stands at position p = i + k_lens[b] - q_lens[b] and sees the keys 0 <= j <= p with j > p - window
+ * or j < sinks (window <= 0: all of them).  P = softmax(q k^T * scale) in fp32, out = P V; rows that see no key and rows
+ * beyond q_lens[b] get zeros.  What lies in masked rows of k and v, infinities and NaN included, does not matter.
+ * Hq % Hkv == 0, D a multiple of 16 up to 128, B * Hq <= 65535. */
+int b200q_window_attention(const void* q, const void* k, const void* v, int dtype, const int64_t* strides, void* out,
+                           const int64_t* out_strides, const int32_t* q_lens, const int32_t* k_lens, int64_t B, int64_t Hq,
+                           int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, float scale, int64_t window, int64_t sinks,
+                           b200q_stream_t stream);
 
 /* ------------------------------------------------------------------ glue of the decoder linear stack
  * The benchmark workloads wrap the quantized linears in a Llama-shaped decoder layer

@@ -58,6 +58,12 @@ SIGNATURES = {
     "b200q_fp8_attention": (_c.c_int, [_p, _p, _p, _c.c_int, _p, _p, _p, _p, _p, _p, _p, _c.c_size_t, _i64, _i64, _i64, _i64, _i64, _i64, _c.c_float, _c.c_int, _p]),
     "b200q_fp8_attention_quantize": (_c.c_int, [_p, _p, _p, _c.c_int, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
     "b200q_amax_columns": (_c.c_int, [_p, _c.c_int, _i64, _i64, _i64, _i64, _p, _p]),
+    "b200q_paged_append": (_c.c_int, [_p, _p, _c.c_int, _p, _i64, _p, _p, _p, _i64, _i64, _p, _i64, _p]),
+    "b200q_paged_attention_workspace_bytes": (_c.c_size_t, []),
+    "b200q_paged_attention_scratch_bytes": (_c.c_size_t, [_i64, _i64, _i64]),
+    "b200q_paged_attention": (_c.c_int, [_p, _c.c_int, _p, _p, _p, _i64, _i64, _p, _i64, _i64, _c.c_float, _i64, _i64, _p, _p, _i64, _p, _c.c_size_t, _p, _c.c_size_t, _p]),
+    "b200q_paged_evict": (_c.c_int, [_p, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p]),
+    "b200q_window_attention": (_c.c_int, [_p, _p, _p, _c.c_int, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _c.c_float, _i64, _i64, _p]),
     "b200q_rms_norm": (_c.c_int, [_p, _p, _p, _i64, _i64, _c.c_float, _p]),
     "b200q_add_rms_norm_fp8_quantize": (_c.c_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _c.c_float, _p]),
     "b200q_silu_mul": (_c.c_int, [_p, _p, _i64, _i64, _p]),
@@ -88,6 +94,12 @@ def cfg_ref(tile_n: int = 0, static_weights: bool = False, peer_wait_ms: int = 0
 class Peers(ctypes.Structure):
     """struct b200q_peers of include/b200q.h."""
     _fields_ = [("rank", _c.c_int32), ("world", _c.c_int32), ("recv", _p * 8), ("out", _p * 8), ("flags", _p * 8)]
+
+
+class PagedCache(ctypes.Structure):
+    """struct b200q_paged_cache of include/b200q.h."""
+    _fields_ = [("k_pages", _p), ("v_pages", _p), ("dtype", _c.c_int32), ("page_size", _c.c_int32), ("num_pages", _i64), ("heads", _i64), ("D", _i64),
+                ("k_strides", _i64 * 3), ("v_strides", _i64 * 3), ("k_amax", _p), ("v_amax", _p), ("amax_numel", _i64)]
 
 
 class GatherPeers(ctypes.Structure):

@@ -1,0 +1,185 @@
+"""Causal attention with a sliding window and sinks against a 64-bit restatement; the bounds are those of
+tests/test_gpu_paged_cache.py: one rounding of the result, one of P to 16 bits, 32-bit sums."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def reference(q, k, v, window, sinks, nq, nk, scale=None):
+    """(out, sum P |V|) in 64 bits; rows that see nothing are zero."""
+    b, hq, sq, d = q.shape
+    g = hq // k.shape[1]
+    out, mass = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(2))
+    for i in range(b):
+        at = torch.arange(nq[i], device="cuda")[:, None] + nk[i] - nq[i]
+        j = torch.arange(nk[i], device="cuda")
+        seen = j <= at
+        if window > 0:
+            seen = seen & ((j > at - window) | (j < sinks))
+        for h in range(hq):
+            kk, vv = k[i, h // g, :nk[i]].double(), v[i, h // g, :nk[i]].double()
+            s = (q[i, h, :nq[i]].double() @ kk.T) * (1 / math.sqrt(d) if scale is None else scale)
+            p = torch.softmax(s.masked_fill(~seen, -math.inf), -1).nan_to_num(0.0) if nk[i] else s
+            out[i, h, :nq[i]], mass[i, h, :nq[i]] = p @ vv, p @ vv.abs()
+    return out, mass
+
+
+def check(out, ref, mass):
+    u = U[out.dtype]
+    tol = u * ref.abs() + (u + 2.0 ** -13) * mass + 1e-30
+    off = (out.double() - ref).abs()
+    assert torch.isfinite(out.float()).all()
+    assert (off <= tol).all(), (off / tol).max().item()
+
+
+def inputs(g, b, hq, hkv, sq, sk, d, dt, token_major):
+    def make(h, s):
+        if token_major:
+            return torch.randn(b, s, h + 1, d, device="cuda", generator=g).to(dt)[:, :, :h].transpose(1, 2)
+        return torch.randn(b, h, s, d, device="cuda", generator=g).to(dt)
+    return make(hq, sq), make(hkv, sk), make(hkv, sk)
+
+
+SHAPES = [
+    # b, hq, hkv, sq, sk, d, window, sinks
+    (1, 1, 1, 1, 1, 64, 0, 0),
+    (1, 2, 1, 1, 300, 128, 0, 0),
+    (2, 4, 2, 17, 17, 16, 0, 0),
+    (1, 4, 4, 127, 127, 128, 0, 0),
+    (1, 4, 2, 128, 128, 128, 0, 0),
+    (1, 4, 2, 129, 129, 64, 0, 0),
+    (2, 6, 2, 257, 400, 80, 0, 0),
+    (2, 6, 2, 300, 200, 96, 0, 0),          # more queries than keys: the first rows see nothing
+    (1, 2, 2, 5, 0, 64, 0, 0),
+    (1, 8, 1, 700, 1200, 128, 0, 0),
+    (1, 2, 1, 513, 513, 128, 1, 0),
+    (1, 2, 1, 513, 513, 128, 64, 0),
+    (2, 2, 1, 513, 900, 112, 128, 4),
+    (1, 2, 1, 1025, 1025, 128, 200, 130),
+    (1, 2, 1, 1025, 1025, 48, 300, 5000),   # sinks cover everything
+    (1, 2, 1, 100, 100, 32, 5000, 3),       # window covers everything
+    (1, 2, 2, 2048, 2048, 128, 100, 1),
+    (3, 2, 1, 61, 1999, 128, 1024, 4),
+    (1, 40, 8, 333, 333, 64, 77, 2),
+    (1, 2, 1, 4097, 4097, 128, 0, 0),
+]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("token_major", [False, True])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_window_attention(b200, shape, token_major, dt):
+    b, hq, hkv, sq, sk, d, window, sinks = shape
+    g = torch.Generator(device="cuda").manual_seed(sq + sk + d)
+    q, k, v = inputs(g, b, hq, hkv, sq, sk, d, dt, token_major)
+    out = b200.window_attention(q, k, v, window=window, sinks=sinks)
+    assert out.shape == q.shape and out.dtype == dt
+    if token_major and sq > 1 and hq > 1:
+        assert out.transpose(1, 2).is_contiguous()
+    ref, mass = reference(q, k, v, window, sinks, [sq] * b, [sk] * b)
+    check(out, ref, mass)
+    assert torch.equal(out, b200.window_attention(q, k, v, window=window, sinks=sinks))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 3)])
+def test_ragged_lengths_with_anything_beyond_them(b200, dt, window, sinks):
+    b, hq, hkv, s, d = 7, 4, 2, 400, 80
+    g = torch.Generator(device="cuda").manual_seed(11)
+    q, k, v = inputs(g, b, hq, hkv, s, s + 50, d, dt, True)
+    nq, nk = [400, 1, 0, 129, 128, 300, 40], [450, 51, 30, 129, 400, 100, 0]
+    for i in range(b):
+        for t, n in ((q, nq), (k, nk), (v, nk)):
+            t[i, :, n[i]:] = float("nan")
+        v[i, :, nk[i]::3] = float("inf")
+    lens = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (nq, nk)]
+    out = b200.window_attention(q, k, v, window=window, sinks=sinks, q_lens=lens[0], k_lens=lens[1])
+    ref, mass = reference(q, k, v, window, sinks, nq, nk)
+    check(out, ref, mass)
+    wild = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([9999] * b, [-5] * b)]
+    assert not b200.window_attention(q, k, v, q_lens=wild[0], k_lens=wild[1]).any()      # cut to the tensors; no keys
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 2)])
+def test_masked_keys_do_not_matter(b200, bad, window, sinks):
+    """A key or value that is not finite shows in the rows that see it, and in no other."""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    q, k, v = inputs(g, 1, 4, 2, 500, 500, 64, torch.bfloat16, False)
+    at = 201
+    seen = torch.arange(500, device="cuda") >= at
+    if window > 0:
+        seen &= torch.arange(500, device="cuda") < at + window
+    clean = b200.window_attention(q, k, v, window=window, sinks=sinks)
+    v2 = v.clone()
+    v2[0, 0, at] = bad
+    out = b200.window_attention(q, k, v2, window=window, sinks=sinks)
+    ref, mass = reference(q, k, v, window, sinks, [500], [500])
+    check(out[:, :2, ~seen], ref[:, :2, ~seen], mass[:, :2, ~seen])
+    assert not torch.isfinite(out[:, :2, seen].float()).any() and torch.equal(out[:, 2:], clean[:, 2:])
+    k2 = k.clone()
+    k2[0, 0, at] = bad
+    out = b200.window_attention(q, k2, v, window=window, sinks=sinks)
+    check(out[:, :2, ~seen], ref[:, :2, ~seen], mass[:, :2, ~seen])
+    assert torch.equal(out[:, 2:], clean[:, 2:])
+
+
+def test_logits_of_every_size(b200):
+    """A maximum that keeps rising along the keys, and logits of some hundreds: the running maximum is followed."""
+    g = torch.Generator(device="cuda").manual_seed(13)
+    q, k, v = inputs(g, 1, 2, 1, 700, 700, 128, torch.bfloat16, False)
+    ramp = torch.linspace(0.01, 8.0, 700, device="cuda")[:, None]
+    for f in (ramp, ramp.flip(0), 20.0, 1e-4):
+        kk = (k.float() * f).bfloat16()
+        qq = (q.float().abs() + 0.25).bfloat16()
+        kk = torch.where(kk < 0, kk * 0.5, kk)
+        scale = 0.25
+        out = b200.window_attention(qq, kk, v, scale=scale)
+        ref, mass = reference(qq, kk, v, 0, 0, [700], [700], scale=scale)
+        size = (qq.float().abs() @ kk.float().abs().transpose(2, 3)).amax() * scale
+        u = 2.0 ** -8
+        tol = u * ref.abs() + (u + 2.0 ** -13 + 2.0 ** -22 * size.item()) * mass + 1e-30   # a logit of size s is off by 2^-24 s and a sum's rounding
+        assert ((out.double() - ref).abs() <= tol).all()
+
+
+def test_streams_and_graphs(b200):
+    g = torch.Generator(device="cuda").manual_seed(14)
+    q, k, v = inputs(g, 2, 4, 2, 300, 300, 128, torch.bfloat16, True)
+    here = b200.window_attention(q, k, v, window=64, sinks=2)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        there = b200.window_attention(q, k, v, window=64, sinks=2)
+    torch.cuda.current_stream().wait_stream(st)
+    assert torch.equal(here, there)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = b200.window_attention(q, k, v, window=64, sinks=2)
+    q.normal_(generator=g)
+    graph.replay()
+    ref, mass = reference(q, k, v, 64, 2, [300] * 2, [300] * 2)
+    check(out, ref, mass)
+
+
+def test_one_token_agrees_with_the_paged_form(b200):
+    """The last row of a window over contiguous keys is the single-token form over pages of the same keys."""
+    g = torch.Generator(device="cuda").manual_seed(15)
+    n, rows, d = 700, 16, 128
+    q, k, v = inputs(g, 1, 8, 2, n, n, d, torch.bfloat16, False)
+    pages = -(-n // rows)
+    kp, vp = (torch.zeros(pages, 2, rows, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    table = torch.randperm(pages, device="cuda", generator=g).to(torch.int32)[None]
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    b200.paged_append(k[0].transpose(0, 1), v[0].transpose(0, 1), kp, vp, table, lens, cu)
+    for window, sinks in ((0, 0), (256, 4)):
+        one = b200.paged_attention(q[:, :, -1], kp, vp, table, lens, window=window, sinks=sinks)
+        all_ = b200.window_attention(q, k, v, window=window, sinks=sinks)
+        ref, mass = reference(q[:, :, -1:], k, v, window, sinks, [1], [n])
+        check(one[:, :, None], ref, mass)
+        check(all_[:, :, -1:], ref, mass)
