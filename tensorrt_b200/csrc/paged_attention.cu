@@ -1,4 +1,26 @@
 // Attention of one new token of every sequence over its pages of the key-value cache.
+//
+//   x_j = (q . k_j) * scale,  out = sum_j exp(x_j - m) v_j / sum_j exp(x_j - m),  m = max_j x_j
+//
+// over the keys j that the token sees, in one pass with a running maximum and sum.  Every K and V row is read once and takes
+// part in 4 * D operations per query head, so the memory binds the kernel, whatever the group: what has to be found is enough
+// bytes in flight on every SM, and work of the same size for each of them.
+//
+// Work.  An item is a sequence, a kv head and up to 16 of its query heads; its keys are tiles of 64.  The tiles of all items
+// stand in one line, which the resident CTAs cut into equal pieces (the lengths are on the device, so every CTA adds them up
+// for itself).  A CTA that ends inside an item leaves its part (maximum, sum, unnormalised result, 32 bits) in the workspace; the
+// CTA that arrives last joins the parts in the order of the keys, so that results do not depend on who is last.
+//
+// A warp takes 16 of a tile's 64 keys through a ring of its own in shared memory, filled by asynchronous copies of 16 bytes, and
+// has its own maximum, sum and result; nothing but the end of an item makes warps wait for one another.  The products run on
+// mma.sync with the query heads as its 16 rows: at 16 rows a tensor-memory accumulator has nothing to gain here (the products need
+// a fifth of the mma.sync rate), and the fragments let 8-bit codes be widened in registers, between shared memory and the product.
+//
+// Rounding.  Products are summed in 32 bits, the softmax is 32-bit.  P is rounded to the 16-bit type of V's operand for the second
+// product: an error of one rounding of each term, of the size of the result's own.  8-bit K and V are exact in fp16; bf16
+// queries in front of them are scaled by a power of two into fp16's range, which loses nothing above 2^-38 of the largest.
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace b200q {
@@ -6,96 +28,561 @@ namespace {
 
 using paged::Cache;
 
+constexpr int kThreads = 128, kWarps = 4, kRows = 16, kTile = 64, kKeys = 16;   // kKeys: of one warp
+constexpr int kMaxCtas = 1024;                                                 // resident at once, on any part
+
 struct DecodeParams {
   Cache c;
+  int page_shift;            // log2 of the page size, or -1
   const char* q;
   int64_t q_batch, q_head;   // bytes
   void* out;
-  float* weights;
-  int64_t weights_len;
-  int Hq, group;
+  float* logits;             // with weights: [B, Hq, logits_stride], by the place among the keys seen
+  float* lse;                // [B, Hq]
+  int64_t logits_stride, weights_len;
+  int B, Hq, group, blocks, rows;   // `blocks` of up to `rows` query heads per kv head
   float scale;
   int64_t window, sinks;
+  unsigned* tickets;         // [kMaxCtas], zero between calls
+  float* parts;              // [kMaxCtas][2][kPart]
 };
 
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, float* f) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  f[0] = __uint_as_float(u.x << 16), f[1] = __uint_as_float(u.x & 0xffff0000u);
-  f[2] = __uint_as_float(u.y << 16), f[3] = __uint_as_float(u.y & 0xffff0000u);
+constexpr int kPart = kRows * paged::kMaxD + 2 * kRows;   // result rows, maxima, sums
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+// 16 bytes to shared memory, zeros where `there` is false.
+__device__ __forceinline__ void copy16(uint32_t dst, const char* src, bool there) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void load4(const __half* p, float* f) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-  f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
 }
-__device__ __forceinline__ void load4(const uint8_t* p, float* f) {
-  const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
-  const float2 a = e4m3x2_to_f32x2(u & 0xffffu), b = e4m3x2_to_f32x2(u >> 16);
-  f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ void ldmatrix_trans(uint32_t a, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+template <bool HALF>
+__device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (HALF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool HALF>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if constexpr (HALF) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t codes_f16x2(uint32_t v) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(v)));
+  return h;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
 
-// One CTA per sequence and kv head, one query head after the other; a warp takes every fourth key, a lane four elements of a row.
-template <typename T, typename KV>
-__global__ void __launch_bounds__(128) decode_kernel(const __grid_constant__ DecodeParams p) {
-  __shared__ float sm[4], sl[4], so[4][paged::kMaxD];
-  const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// The keys that the newest token of a sequence sees: `seen` of them, the first `sinks` in place, the others `gap` further on.
+struct Seen {
+  int seen, sinks, gap;
+  __device__ __forceinline__ int token(int i) const { return i < sinks ? i : i + gap; }
+  __device__ __forceinline__ int tiles() const { return seen > 0 ? (seen + kTile - 1) / kTile : 1; }   // 1: somebody writes the zeros
+};
+__device__ __forceinline__ Seen keys_seen(const DecodeParams& p, int b) {
   const int n = paged::cached_tokens(p.c, b, 0x7fffffff);
   const int first = p.window > 0 && n > p.window ? static_cast<int>(n - p.window) : 0;
-  const int sinks = static_cast<int>(min(p.sinks, static_cast<int64_t>(first))), gap = first - sinks, seen = n - gap;
-  const int32_t* line = p.c.table + b * p.c.table_stride;
-  const bool mine = lane * 4 < p.c.D;
-  const float ks = p.c.codes ? paged::head_scale(p.c.k_amax, p.c.amax_stride, h) : 1.0f;
-  const float vs = p.c.codes ? paged::head_scale(p.c.v_amax, p.c.amax_stride, h) : 1.0f;
-  for (int g = 0; g < p.group; ++g) {
-    const int hq = h * p.group + g;
-    float q[4] = {}, o[4] = {}, m = -INFINITY, l = 0.0f;
-    bool any = false;
-    if (mine) load4(reinterpret_cast<const T*>(p.q + b * p.q_batch + hq * p.q_head) + lane * 4, q);
-    auto logit = [&](int i, int* page, int* row) {
-      const int t = i < sinks ? i : i + gap;
-      *page = paged::page_of(line, t, p.c), *row = t % p.c.page_size;
-      float k[4] = {}, s = 0.0f;
-      if (*page >= 0 && mine) load4(reinterpret_cast<const KV*>(paged::row_at(p.c.k, *page, h, *row)) + lane * 4, k);
-      for (int e = 0; e < 4; ++e) s += q[e] * k[e];
-      for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-      return s * (ks * p.scale);
-    };
-    for (int i = warp; i < seen; i += 4) {
-      int page, row;
-      const float s = logit(i, &page, &row);
-      if (page < 0) continue;
-      any = true;
-      const float mn = fmaxf(m, s), safe = mn == -INFINITY ? 0.0f : mn, f = expf(m - safe), e = expf(s - safe);
-      float v[4] = {};
-      if (mine) load4(reinterpret_cast<const KV*>(paged::row_at(p.c.v, page, h, row)) + lane * 4, v);
-      for (int x = 0; x < 4; ++x) o[x] = o[x] * f + e * v[x];
-      l = l * f + e, m = mn;
+  const int sinks = p.sinks < first ? static_cast<int>(p.sinks) : first;
+  return Seen{n - (first - sinks), sinks, first - sinks};
+}
+
+// Layout of one warp's stage: 16 rows of K, then 16 of V, 16-byte chunks swizzled so that the reads below meet no bank twice.
+template <bool CODES, int DPAD>
+struct Stage {
+  static constexpr int kRowBytes = DPAD * (CODES ? 1 : 2);
+  static constexpr int kChunks = kRowBytes / 16;
+  static constexpr int kBytes = 2 * kKeys * kRowBytes;
+  static constexpr int kDepth = kBytes >= 8192 ? 3 : (kBytes >= 4096 ? 6 : 8);
+  __device__ static __forceinline__ int k_chunk(int key, int c) { return kRowBytes == 64 ? c : c ^ ((key & 1) << 2); }
+  __device__ static __forceinline__ int v_chunk(int key, int c) {
+    if (!CODES) return c ^ (key & 7);
+    return kRowBytes == 64 ? c ^ ((key >> 1) & 3) : c ^ (((key >> 1) & 3) << 1);
+  }
+};
+
+// The piece of the line of tiles that CTA c of `ctas` takes.
+__device__ __forceinline__ int64_t piece(int64_t tiles, int c, int ctas) { return tiles * c / ctas; }
+
+// Adds up the tiles of all sequences and finds the one that holds tile `piece(total, cta)`; all threads take part.
+__device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, int ctas, int* b_out, int64_t* before_out) {
+  __shared__ int64_t sums[kWarps];
+  __shared__ int64_t found[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t per = static_cast<int64_t>(p.c.heads) * p.blocks;
+  int64_t total = 0, inclusive = 0, mine = 0;
+  auto scan = [&](int64_t v) {                        // inclusive over the CTA; returns the sum
+    int64_t s = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += o;
     }
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
-    for (int x = 0; x < 4; ++x) if (mine) so[warp][lane * 4 + x] = o[x];
-    any = __syncthreads_or(any);
-    float top = sm[0], total = 0.0f;
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, sm[w]);
-    if (top == -INFINITY) top = 0.0f;
-    for (int w = 0; w < 4; ++w) total += sl[w] * expf(sm[w] - top);
-    for (int d = threadIdx.x; d < p.c.D; d += 128) {
-      float acc = 0.0f;
-      for (int w = 0; w < 4; ++w) acc += so[w][d] * expf(sm[w] - top);
-      const float r = !any ? 0.0f : acc * vs / total;
-      static_cast<T*>(p.out)[(static_cast<int64_t>(b) * p.Hq + hq) * p.c.D + d] = static_cast<T>(r);
+    if (lane == 31) sums[warp] = s;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) s += sums[w];
+      all += sums[w];
     }
-    if (p.weights != nullptr) {
-      float* w = p.weights + (static_cast<int64_t>(b) * p.c.heads + h) * p.weights_len;
-      for (int i = warp; i < seen; i += 4) {
-        int page, row;
-        const float s = logit(i, &page, &row);
-        const int t = i < sinks ? i : i + gap;
-        if (lane == 0 && page >= 0 && t < p.weights_len) w[t] += expf(s - top) / total;
-      }
+    __syncthreads();
+    inclusive = s;
+    return all;
+  };
+  for (int base = 0; base < p.B; base += kThreads) {
+    mine = base + tid < p.B ? keys_seen(p, base + tid).tiles() * per : 0;
+    total += scan(mine);
+  }
+  const int64_t want = piece(total, cta, ctas);
+  if (p.B <= kThreads) {
+    if (want >= inclusive - mine && want < inclusive) found[0] = tid, found[1] = inclusive - mine;
+    __syncthreads();
+  } else {
+    int64_t before = 0;
+    for (int base = 0; base < p.B; base += kThreads) {
+      mine = base + tid < p.B ? keys_seen(p, base + tid).tiles() * per : 0;
+      const int64_t all = scan(mine);
+      if (want >= before + inclusive - mine && want < before + inclusive) found[0] = base + tid, found[1] = before + inclusive - mine;
+      before += all;
+      if (before > want) break;
     }
     __syncthreads();
   }
+  *b_out = static_cast<int>(found[0]);
+  *before_out = found[1];
+  return total;
 }
+
+template <typename T, bool CODES, int DPAD>
+__global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant__ DecodeParams p) {
+  using S = Stage<CODES, DPAD>;
+  constexpr bool kHalf = CODES || std::is_same<T, __half>::value;
+  constexpr int kSteps = DPAD / 16, kOut = DPAD / 8;
+  extern __shared__ __align__(128) char smem[];
+  __shared__ float row_max[kWarps][kRows], row_sum[kWarps][kRows];
+  __shared__ int last_one;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int cta = blockIdx.x, ctas = gridDim.x;
+  char* const ring = smem + warp * S::kDepth * S::kBytes;
+  const uint32_t ring_u32 = smem_u32(ring);
+  pdl_launch_dependents();
+  pdl_wait();
+
+  int b;
+  int64_t before;
+  const int64_t total = find_start(p, cta, ctas, &b, &before);
+  int64_t at = piece(total, cta, ctas);
+  const int64_t first_tile = at, end = piece(total, cta + 1, ctas);
+  while (at < end) {
+    // ------------------------------------------------------------- the item
+    Seen see = keys_seen(p, b);
+    const int tiles = see.tiles();
+    const int64_t item = (at - before) / tiles;       // kv head and block of query heads, within the sequence
+    if (item >= static_cast<int64_t>(p.c.heads) * p.blocks) {
+      before += static_cast<int64_t>(tiles) * p.c.heads * p.blocks;
+      ++b;
+      continue;
+    }
+    const int h = static_cast<int>(item / p.blocks), block = static_cast<int>(item % p.blocks);
+    const int64_t item_start = before + item * tiles, item_end = item_start + tiles;
+    const int tile0 = static_cast<int>(at - item_start), tile1 = static_cast<int>((end < item_end ? end : item_end) - item_start);
+    const int head0 = h * p.group + block * p.rows, rows = min(p.rows, p.group - block * p.rows);
+    const int32_t* line = p.c.table + b * p.c.table_stride;
+    const char* kbase = p.c.k.base + h * p.c.k.head;
+    const char* vbase = p.c.v.base + h * p.c.v.head;
+
+    // ------------------------------------------------------------- copies of a warp's 16 keys of a tile
+    auto find_page = [&](int tile) {                  // lane: page of key lane % 16, -1 where there is none; row within it
+      const int i = tile * kTile + warp * kKeys + (lane & 15);
+      int page = -1, row = 0;
+      if (tile < tile1 && i < see.seen) {
+        const int token = see.token(i), n = p.page_shift >= 0 ? token >> p.page_shift : token / p.c.page_size;
+        asm volatile("ld.global.b32 %0, [%1];" : "=r"(page) : "l"(line + n) : "memory");
+        row = token - n * p.c.page_size;
+      }
+      return make_int2(page, row);
+    };
+    auto issue = [&](int slot, int2 where) {
+      const int page = static_cast<unsigned>(where.x) < static_cast<unsigned>(p.c.num_pages) ? where.x : -1;
+      constexpr int kLanes = S::kChunks < 8 ? S::kChunks : 8, kPer = 32 / kLanes;     // lanes to a row, rows to an instruction
+      const uint32_t kdst = ring_u32 + slot * S::kBytes, vdst = kdst + kKeys * S::kRowBytes;
+#pragma unroll
+      for (int j = 0; j < kKeys / kPer; ++j) {
+        const int key = j * kPer + lane / kLanes;
+        const int pg = __shfl_sync(0xffffffffu, page, key), row = __shfl_sync(0xffffffffu, where.y, key);
+        const int64_t safe = pg < 0 ? 0 : pg;
+        const char* ks = kbase + safe * p.c.k.page + row * p.c.k.row;
+        const char* vs = vbase + safe * p.c.v.page + row * p.c.v.row;
+#pragma unroll
+        for (int c0 = 0; c0 < S::kChunks; c0 += kLanes) {
+          const int c = c0 + lane % kLanes;
+          const bool inside = c * 16 < p.c.D * (CODES ? 1 : 2);
+          const int src = inside ? c * 16 : 0;
+          copy16(kdst + key * S::kRowBytes + S::k_chunk(key, c) * 16, ks + src, pg >= 0 && inside);
+          copy16(vdst + key * S::kRowBytes + S::v_chunk(key, c) * 16, vs + src, pg >= 0 && inside);
+        }
+      }
+      copy_commit();
+      return __ballot_sync(0xffffffffu, page >= 0 && lane < 16);
+    };
+    uint32_t there[S::kDepth];                         // which of the 16 keys of a stage exist
+    int2 ahead = find_page(tile0);
+#pragma unroll
+    for (int s = 0; s < S::kDepth - 1; ++s) {
+      const int2 now = ahead;
+      ahead = find_page(tile0 + s + 1);
+      there[s] = issue(s, now);
+    }
+
+    // ------------------------------------------------------------- queries: rows g and g + 8, the elements that this lane's K chunks meet
+    uint32_t q[kSteps][4];
+    float unit[2] = {1.0f, 1.0f};
+    {
+      const char* base = p.q + b * p.q_batch + head0 * p.q_head;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = g + 8 * r;
+        const char* src = base + row * p.q_head;
+        uint32_t w[2 * kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps / 2; ++i) {          // 8 elements each
+          const int e = CODES ? (i / 2) * 64 + t * 16 + (i % 2) * 8 : i * 32 + t * 8;
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (row < rows && e < p.c.D) u = ld_128(src + e * 2);
+          w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+        }
+        if constexpr (CODES && !std::is_same<T, __half>::value) {
+          float top = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 2 * kSteps; ++i)
+            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+          top = quad_max(top);
+          // 2^(13 - exponent): the largest lands in [2^13, 2^14); zero, infinity and NaN stay as they are
+          const int e = static_cast<int>(__float_as_uint(top) >> 23);
+          float f = 1.0f;
+          if (top != 0.0f && e < 255) {
+            const int s = min(140 - max(e, 1), 124);
+            f = __uint_as_float(static_cast<uint32_t>(max(s, -125) + 127) << 23);
+          }
+          unit[r] = 1.0f / f;
+#pragma unroll
+          for (int i = 0; i < 2 * kSteps; ++i)
+            w[i] = pack16<true>(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
+        }
+        // step s of the product takes words 2 s and 2 s + 1
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) q[s][r] = w[2 * s], q[s][2 + r] = w[2 * s + 1];
+      }
+    }
+    const float k_scale = CODES ? paged::head_scale(p.c.k_amax, p.c.amax_stride, h) : 1.0f;
+    const float v_scale = CODES ? paged::head_scale(p.c.v_amax, p.c.amax_stride, h) : 1.0f;
+    const float log2_scale = p.scale * k_scale * 1.4426950408889634f;
+    const float sl[2] = {log2_scale * unit[0], log2_scale * unit[1]};
+
+    // ------------------------------------------------------------- the keys
+    float o[kOut][4];
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    bool any = false;
+    for (int tile = tile0; tile < tile1;) {
+#pragma unroll
+      for (int s = 0; s < S::kDepth; ++s) {
+        if (tile < tile1) {
+          copy_wait<S::kDepth - 2>();
+          __syncwarp();
+          const uint32_t ks = ring_u32 + s * S::kBytes, vs = ks + kKeys * S::kRowBytes, keys = there[s];
+          any = any || keys != 0;
+          float x[2][4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+            const int key = n * 8 + g;
+            if constexpr (CODES) {
+#pragma unroll
+              for (int i = 0; i < kSteps / 4; ++i) {
+                const uint4 u = lds128(ks + key * S::kRowBytes + S::k_chunk(key, i * 4 + t) * 16);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mma<kHalf>(x[n], q[i * 4 + e], codes_f16x2(w[e]), codes_f16x2(w[e] >> 16));
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < kSteps / 2; ++i) {
+                const uint4 u = lds128(ks + key * S::kRowBytes + S::k_chunk(key, i * 4 + t) * 16);
+                mma<kHalf>(x[n], q[i * 2], u.x, u.y);
+                mma<kHalf>(x[n], q[i * 2 + 1], u.z, u.w);
+              }
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[n][e] *= sl[e >> 1];
+              if (!((keys >> (n * 8 + t * 2 + (e & 1))) & 1)) x[n][e] = -INFINITY;
+            }
+          if (p.logits != nullptr) {
+            const int i0 = tile * kTile + warp * kKeys + t * 2;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              if (g + 8 * r >= rows) continue;
+              float* dst = p.logits + (static_cast<int64_t>(b) * p.Hq + head0 + g + 8 * r) * p.logits_stride;
+#pragma unroll
+              for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int i = i0 + n * 8 + e;
+                  if (i < see.seen && see.token(i) < p.weights_len) dst[i] = x[n][2 * r + e];
+                }
+            }
+          }
+          float mx[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) mx[r] = fmaxf(m[r], quad_max(fmaxf(fmaxf(x[0][2 * r], x[0][2 * r + 1]), fmaxf(x[1][2 * r], x[1][2 * r + 1]))));
+          if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float f = mx[r] == -INFINITY ? 1.0f : exp2_fast(m[r] - mx[r]);
+              l[r] *= f;
+#pragma unroll
+              for (int i = 0; i < kOut; ++i) o[i][2 * r] *= f, o[i][2 * r + 1] *= f;
+              m[r] = mx[r];
+            }
+          }
+          const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[n][e] = exp2_fast(x[n][e] - base[e >> 1]);
+              l[e >> 1] += x[n][e];
+            }
+          const uint32_t a[4] = {pack16<kHalf>(x[0][0], x[0][1]), pack16<kHalf>(x[0][2], x[0][3]), pack16<kHalf>(x[1][0], x[1][1]),
+                                 pack16<kHalf>(x[1][2], x[1][3])};
+          if constexpr (CODES) {
+            constexpr int kWords = DPAD / 32;           // of the row pieces that this lane widens
+            uint32_t w[4][kWords];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int key = t * 2 + (k & 1) + (k >> 1) * 8;
+              if constexpr (DPAD == 128) {
+                const uint4 u = lds128(vs + key * S::kRowBytes + S::v_chunk(key, g) * 16);
+                w[k][0] = u.x, w[k][1] = u.y, w[k][2] = u.z, w[k][3] = u.w;
+              } else {
+                const uint2 u = lds64(vs + key * S::kRowBytes + S::v_chunk(key, g >> 1) * 16 + (g & 1) * 8);
+                w[k][0] = u.x, w[k][1] = u.y;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+              const uint32_t lo0 = __byte_perm(w[0][i], w[1][i], 0x5140), hi0 = __byte_perm(w[0][i], w[1][i], 0x7362);
+              const uint32_t lo1 = __byte_perm(w[2][i], w[3][i], 0x5140), hi1 = __byte_perm(w[2][i], w[3][i], 0x7362);
+              mma<kHalf>(o[4 * i], a, codes_f16x2(lo0), codes_f16x2(lo1));
+              mma<kHalf>(o[4 * i + 1], a, codes_f16x2(lo0 >> 16), codes_f16x2(lo1 >> 16));
+              mma<kHalf>(o[4 * i + 2], a, codes_f16x2(hi0), codes_f16x2(hi1));
+              mma<kHalf>(o[4 * i + 3], a, codes_f16x2(hi0 >> 16), codes_f16x2(hi1 >> 16));
+            }
+          } else {
+            const int key = (lane & 7) + (lane & 8);
+#pragma unroll
+            for (int i = 0; i < kOut; i += 2) {
+              uint32_t r[4];
+              ldmatrix_trans(vs + key * S::kRowBytes + S::v_chunk(key, i + (lane >> 4)) * 16, r);
+              mma<kHalf>(o[i], a, r[0], r[1]);
+              mma<kHalf>(o[i + 1], a, r[2], r[3]);
+            }
+          }
+          __syncwarp();
+          const int2 now = ahead;
+          ahead = find_page(tile + S::kDepth);
+          there[(s + S::kDepth - 1) % S::kDepth] = issue((s + S::kDepth - 1) % S::kDepth, now);
+          ++tile;
+        }
+      }
+    }
+    copy_wait<0>();
+    __syncwarp();
+
+    // ------------------------------------------------------------- the four warps' parts together
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if (t == 0) row_max[warp][g + 8 * r] = m[r], row_sum[warp][g + 8 * r] = any ? l[r] : -1.0f;   // -1: no key at all
+    }
+    float* mine = reinterpret_cast<float*>(ring);     // 16 rows of DPAD: the ring is empty
+#pragma unroll
+    for (int i = 0; i < kOut; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = t * 2 + (e & 1), d = CODES ? n * (DPAD / 8) + i : i * 8 + n;
+        mine[(g + 8 * (e >> 1)) * DPAD + d] = o[i][e];
+      }
+    __syncthreads();
+    const bool whole = tile0 == 0 && tile1 == tiles;
+    // CTAs that share the item: c0 .. c1, those with a piece of it; the counter of the one that begins it
+    const int c0 = static_cast<int>(((item_start + 1) * ctas - 1) / total), c1 = static_cast<int>((item_end * ctas - 1) / total);
+    float* part = p.parts + (static_cast<int64_t>(cta) * 2 + (at == first_tile ? 0 : 1)) * kPart;
+    constexpr int kQuads = DPAD / 4;
+    for (int i = tid; i < rows * kQuads; i += kThreads) {
+      const int row = i / kQuads, d = (i % kQuads) * 4;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, row_max[w][row]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f, acc[4] = {};
+      bool has = false;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (row_sum[w][row] < 0.0f) continue;
+        has = true;
+        const float f = exp2_fast(row_max[w][row] - base);
+        sum += row_sum[w][row] * f;
+        const float4 v = *reinterpret_cast<const float4*>(smem + w * S::kDepth * S::kBytes + (row * DPAD + d) * 4);
+        acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
+      }
+      if (whole) {
+        if (d < p.c.D) {
+          const float f = v_scale / sum;
+          T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.Hq + head0 + row) * p.c.D + d;
+          uint2 r = make_uint2(0, 0);
+          if (has) {
+            r.x = pack16<std::is_same<T, __half>::value>(acc[0] * f, acc[1] * f);
+            r.y = pack16<std::is_same<T, __half>::value>(acc[2] * f, acc[3] * f);
+          }
+          *reinterpret_cast<uint2*>(dst) = r;
+        }
+        if (d == 0 && p.lse != nullptr) p.lse[static_cast<int64_t>(b) * p.Hq + head0 + row] = has ? base + log2f(sum) : 0.0f;
+      } else {
+        *reinterpret_cast<float4*>(part + row * DPAD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        if (d == 0) part[kRows * DPAD + row] = top, part[kRows * DPAD + kRows + row] = has ? sum : -1.0f;
+      }
+    }
+    // ------------------------------------------------------------- the CTAs' parts together, by the one that comes last
+    if (!whole) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const unsigned n = static_cast<unsigned>(total >= ctas ? c1 - c0 + 1 : tiles);
+        const unsigned order = atomicAdd(p.tickets + c0, 1u);
+        last_one = order == n - 1;
+        if (last_one) p.tickets[c0] = 0;
+      }
+      __syncthreads();
+      if (last_one) {
+        __threadfence();
+        const bool second = piece(total, c0, ctas) < item_start;     // the item is not the first that CTA c0 worked on
+        for (int i = tid; i < rows * kQuads; i += kThreads) {
+          const int row = i / kQuads, d = (i % kQuads) * 4;
+          float top = -INFINITY, sum = 0.0f, acc[4] = {};
+          bool has = false;
+          for (int c = c0; c <= c1; ++c) {
+            if (total < ctas && piece(total, c, ctas) == piece(total, c + 1, ctas)) continue;
+            const float* src = p.parts + (static_cast<int64_t>(c) * 2 + (c == c0 && second ? 1 : 0)) * kPart;
+            const float pm = __ldcg(src + kRows * DPAD + row), ps = __ldcg(src + kRows * DPAD + kRows + row);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(src + row * DPAD + d));
+            if (ps < 0.0f) continue;
+            has = true;
+            const float now = fmaxf(top, pm), base = now == -INFINITY ? 0.0f : now, f0 = exp2_fast(top - base), f1 = exp2_fast(pm - base);
+            sum = sum * f0 + ps * f1;
+            acc[0] = acc[0] * f0 + v.x * f1, acc[1] = acc[1] * f0 + v.y * f1, acc[2] = acc[2] * f0 + v.z * f1, acc[3] = acc[3] * f0 + v.w * f1;
+            top = now;
+          }
+          if (d < p.c.D) {
+            const float f = v_scale / sum;
+            T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.Hq + head0 + row) * p.c.D + d;
+            uint2 r = make_uint2(0, 0);
+            if (has) {
+              r.x = pack16<std::is_same<T, __half>::value>(acc[0] * f, acc[1] * f);
+              r.y = pack16<std::is_same<T, __half>::value>(acc[2] * f, acc[3] * f);
+            }
+            *reinterpret_cast<uint2*>(dst) = r;
+          }
+          if (d == 0 && p.lse != nullptr)
+            p.lse[static_cast<int64_t>(b) * p.Hq + head0 + row] = has ? (top == -INFINITY ? 0.0f : top) + log2f(sum) : 0.0f;
+        }
+      }
+    }
+    __syncthreads();
+    at += tile1 - tile0;
+  }
+}
+
+// weights[b, h, token] += sum over the query heads of P, from the logits that the kernel above left and their normalisers.
+__global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ DecodeParams p, float* weights) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.z, h = blockIdx.y;
+  const Seen see = keys_seen(p, b);
+  const int64_t first = static_cast<int64_t>(b) * p.Hq + h * p.group;
+  float* w = weights + (static_cast<int64_t>(b) * p.c.heads + h) * p.weights_len;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < see.seen; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int token = see.token(static_cast<int>(i));
+    if (token >= p.weights_len) return;
+    float sum = 0.0f;
+    for (int g = 0; g < p.group; ++g) sum += exp2_fast(p.logits[(first + g) * p.logits_stride + i] - p.lse[first + g]);
+    w[token] += sum;
+  }
+}
+
+template <typename T, bool CODES, int DPAD>
+int launch_decode(const DecodeParams& p, int64_t most_tiles, cudaStream_t st) {
+  using S = Stage<CODES, DPAD>;
+  constexpr int kSmem = kWarps * S::kDepth * S::kBytes;
+  static_assert(S::kDepth * S::kBytes >= kRows * DPAD * 4, "a warp's result takes its ring");
+  auto kernel = decode_kernel<T, CODES, DPAD>;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return B200Q_ERR_CUDA;
+  static std::atomic<int> resident[64];                // CTAs that one SM holds; 0: not asked yet
+  int per_sm = dev >= 0 && dev < 64 ? resident[dev].load(std::memory_order_relaxed) : 0;
+  if (per_sm == 0) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return B200Q_ERR_CUDA;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, kSmem) != cudaSuccess || per_sm < 1) return B200Q_ERR_CUDA;
+    if (dev >= 0 && dev < 64) resident[dev].store(per_sm, std::memory_order_relaxed);
+  }
+  int64_t ctas = static_cast<int64_t>(per_sm) * sm_count();
+  ctas = ctas < kMaxCtas ? ctas : kMaxCtas;
+  ctas = ctas < most_tiles ? ctas : most_tiles;
+  if (launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), kSmem, st, p) != cudaSuccess) return B200Q_ERR_CUDA;
+  return check_launch();
+}
+
+template <typename T, bool CODES>
+int launch_decode_d(const DecodeParams& p, int64_t most_tiles, cudaStream_t st) {
+  return p.c.D <= 64 ? launch_decode<T, CODES, 64>(p, most_tiles, st) : launch_decode<T, CODES, 128>(p, most_tiles, st);
+}
+
+int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
 
 }  // namespace
 }  // namespace b200q
@@ -104,8 +591,12 @@ using namespace b200q;
 
 extern "C" {
 
-size_t b200q_paged_attention_workspace_bytes(void) { return 16; }
-size_t b200q_paged_attention_scratch_bytes(int64_t, int64_t, int64_t) { return 16; }
+size_t b200q_paged_attention_workspace_bytes(void) { return kMaxCtas * sizeof(unsigned) + static_cast<size_t>(kMaxCtas) * 2 * kPart * sizeof(float); }
+
+size_t b200q_paged_attention_scratch_bytes(int64_t B, int64_t Hq, int64_t weights_len) {
+  if (B <= 0 || Hq <= 0 || weights_len < 0) return 16;
+  return static_cast<size_t>(B * Hq) * (round4(weights_len) + 1) * sizeof(float) + 16;
+}
 
 int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, const b200q_paged_cache* cache, const int32_t* block_table,
                           int64_t table_stride, int64_t table_width, const int32_t* lens, int64_t B, int64_t Hq, float scale,
@@ -115,27 +606,43 @@ int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, co
   if (int rc = paged::make_cache(&p.c, cache, dtype, block_table, table_stride, table_width, lens, B)) return rc;
   if (Hq <= 0 || Hq > 65535 || Hq % p.c.heads != 0 || sinks < 0 || !(scale == scale) || B > 65535) return B200Q_ERR_INVALID;
   if (B == 0) return B200Q_OK;
-  if (q == nullptr || q_strides == nullptr || out == nullptr || (weights != nullptr && weights_len < 0)) return B200Q_ERR_INVALID;
+  if (q == nullptr || q_strides == nullptr || out == nullptr || (weights != nullptr && (weights_len < 0 || weights_len > 0x7fffff00LL)))
+    return B200Q_ERR_INVALID;
   if (!aligned(q, 16) || !aligned(out, 16) || !paged::strides_ok(q_strides, 2, 8)) return B200Q_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < b200q_paged_attention_workspace_bytes()) return B200Q_ERR_WORKSPACE;
   if (weights != nullptr && (scratch == nullptr || scratch_bytes < b200q_paged_attention_scratch_bytes(B, Hq, weights_len))) return B200Q_ERR_WORKSPACE;
   if (!aligned(workspace, 16) || !aligned(scratch, 16)) return B200Q_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
+  p.page_shift = -1;
+  if ((p.c.page_size & (p.c.page_size - 1)) == 0)
+    for (p.page_shift = 0; (1 << p.page_shift) < p.c.page_size;) ++p.page_shift;
   p.q = static_cast<const char*>(q);
   p.q_batch = q_strides[0] * 2, p.q_head = q_strides[1] * 2;
   p.out = out;
-  p.weights = weights;
-  p.weights_len = weights_len;
-  p.Hq = static_cast<int>(Hq), p.group = static_cast<int>(Hq / p.c.heads);
+  p.B = static_cast<int>(B), p.Hq = static_cast<int>(Hq), p.group = static_cast<int>(Hq / p.c.heads);
+  p.blocks = (p.group + kRows - 1) / kRows;
+  p.rows = (p.group + p.blocks - 1) / p.blocks;
+  p.blocks = (p.group + p.rows - 1) / p.rows;
   p.scale = scale;
   p.window = window, p.sinks = sinks;
-  const dim3 grid(p.c.heads, static_cast<unsigned>(B));
-  const auto st = static_cast<cudaStream_t>(stream);
-  if (dtype == B200Q_BF16) {
-    if (p.c.codes) decode_kernel<__nv_bfloat16, uint8_t><<<grid, 128, 0, st>>>(p); else decode_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 128, 0, st>>>(p);
-  } else {
-    if (p.c.codes) decode_kernel<__half, uint8_t><<<grid, 128, 0, st>>>(p); else decode_kernel<__half, __half><<<grid, 128, 0, st>>>(p);
+  p.tickets = static_cast<unsigned*>(workspace);
+  p.parts = reinterpret_cast<float*>(p.tickets + kMaxCtas);
+  if (weights != nullptr && weights_len > 0) {
+    p.logits_stride = round4(weights_len);
+    p.weights_len = weights_len;
+    p.logits = static_cast<float*>(scratch);
+    p.lse = p.logits + B * Hq * p.logits_stride;
   }
+  // the longest sequence that the table can hold: no more CTAs than tiles
+  const int64_t most = window > 0 && sinks < (1LL << 40) && window < (1LL << 40) && window + sinks < p.c.capacity ? window + sinks : p.c.capacity;
+  const int64_t tiles = (most > 0 ? (most + kTile - 1) / kTile : 1) * B * p.c.heads * p.blocks;
+  const auto st = static_cast<cudaStream_t>(stream);
+  const int rc = dtype == B200Q_BF16 ? (p.c.codes ? launch_decode_d<__nv_bfloat16, true>(p, tiles, st) : launch_decode_d<__nv_bfloat16, false>(p, tiles, st))
+                                     : (p.c.codes ? launch_decode_d<__half, true>(p, tiles, st) : launch_decode_d<__half, false>(p, tiles, st));
+  if (rc != B200Q_OK || p.logits == nullptr) return rc;
+  const int64_t keys = most < weights_len ? most : weights_len, chunks = (keys + 255) / 256;
+  const dim3 grid(static_cast<unsigned>(chunks < 1 ? 1 : (chunks < 65535 ? chunks : 65535)), static_cast<unsigned>(p.c.heads), static_cast<unsigned>(B));
+  if (launch_pdl(weights_kernel, grid, dim3(256), 0, st, p, weights) != cudaSuccess) return B200Q_ERR_CUDA;
   return check_launch();
 }
 
