@@ -13,8 +13,10 @@
 //
 // A warp takes 16 of a tile's 64 keys through a ring of its own in shared memory, filled by asynchronous copies of 16 bytes, and
 // has its own maximum, sum and result; nothing but the end of an item makes warps wait for one another.  The products run on
-// mma.sync with the query heads as its 16 rows: at 16 rows a tensor-memory accumulator has nothing to gain here (the products need
-// a fifth of the mma.sync rate), and the fragments let 8-bit codes be widened in registers, between shared memory and the product.
+// mma.sync with K and V^T as the 16-row operand and 8 or 16 query heads as the columns, S^T = K Q^T and O^T = V^T P^T: with so few
+// columns a tensor-memory accumulator has nothing to gain (the products need a tenth of the mma.sync rate), and register fragments
+// let 8-bit codes be widened between shared memory and the product.  P^T turns from the result of one product into the operand
+// of the next by an 8 x 8 transpose among the lanes.
 //
 // Rounding.  Products are summed in 32 bits, the softmax is 32-bit.  P is rounded to the 16-bit type of V's operand for the second
 // product: an error of one rounding of each term, of the size of the result's own.  8-bit K and V are exact in fp16; bf16
@@ -28,7 +30,7 @@ namespace {
 
 using paged::Cache;
 
-constexpr int kThreads = 128, kWarps = 4, kRows = 16, kTile = 64, kKeys = 16;   // kKeys: of one warp
+constexpr int kThreads = 128, kWarps = 4, kRows = 16, kTile = 64, kKeys = 16;   // kRows: most query heads of an item; kKeys: of one warp
 constexpr int kMaxCtas = 1024;                                                 // resident at once, on any part
 
 struct DecodeParams {
@@ -101,6 +103,22 @@ __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
+// over the lanes that share a place in their quads
+__device__ __forceinline__ float column_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 4);
+  v += __shfl_xor_sync(0xffffffffu, v, 8);
+  return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 
 // The keys that the newest token of a sequence sees: `seen` of them, the first `sinks` in place, the others `gap` further on.
 struct Seen {
@@ -116,12 +134,13 @@ __device__ __forceinline__ Seen keys_seen(const DecodeParams& p, int b) {
 }
 
 // Layout of one warp's stage: 16 rows of K, then 16 of V, 16-byte chunks swizzled so that the reads below meet no bank twice.
-template <bool CODES, int DPAD>
+template <bool CODES, int DPAD, int BLOCKS8>
 struct Stage {
   static constexpr int kRowBytes = DPAD * (CODES ? 1 : 2);
   static constexpr int kChunks = kRowBytes / 16;
   static constexpr int kBytes = 2 * kKeys * kRowBytes;
-  static constexpr int kDepth = kBytes >= 8192 ? 3 : (kBytes >= 4096 ? 6 : 8);
+  static constexpr int kPerSm = kBytes >= 8192 || BLOCKS8 == 2 ? 2 : 3;           // CTAs that share an SM
+  static constexpr int kDepth = kBytes >= 8192 ? 3 : (kBytes >= 4096 ? (kPerSm == 3 ? 4 : 6) : 8);
   __device__ static __forceinline__ int k_chunk(int key, int c) { return kRowBytes == 64 ? c : c ^ ((key & 1) << 2); }
   __device__ static __forceinline__ int v_chunk(int key, int c) {
     if (!CODES) return c ^ (key & 7);
@@ -182,11 +201,12 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
   return total;
 }
 
-template <typename T, bool CODES, int DPAD>
-__global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant__ DecodeParams p) {
-  using S = Stage<CODES, DPAD>;
+// BLOCKS8: query heads of an item in blocks of 8.
+template <typename T, bool CODES, int DPAD, int BLOCKS8>
+__global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm) decode_kernel(const __grid_constant__ DecodeParams p) {
+  using S = Stage<CODES, DPAD, BLOCKS8>;
   constexpr bool kHalf = CODES || std::is_same<T, __half>::value;
-  constexpr int kSteps = DPAD / 16, kOut = DPAD / 8;
+  constexpr int kSteps = DPAD / 16;
   extern __shared__ __align__(128) char smem[];
   __shared__ float row_max[kWarps][kRows], row_sum[kWarps][kRows];
   __shared__ int last_one;
@@ -263,16 +283,16 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
       there[s] = issue(s, now);
     }
 
-    // ------------------------------------------------------------- queries: rows g and g + 8, the elements that this lane's K chunks meet
-    uint32_t q[kSteps][4];
-    float unit[2] = {1.0f, 1.0f};
+    // ------------------------------------------------------------- queries: head g of each block, the elements that this lane's K chunks meet
+    uint32_t q[BLOCKS8][kSteps][2];
+    float unit[BLOCKS8];
     {
       const char* base = p.q + b * p.q_batch + head0 * p.q_head;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
+      for (int r = 0; r < BLOCKS8; ++r) {
         const int row = g + 8 * r;
         const char* src = base + row * p.q_head;
-        uint32_t w[2 * kSteps];
+        uint32_t* w = &q[r][0][0];                      // step s of the product takes words 2 s and 2 s + 1
 #pragma unroll
         for (int i = 0; i < kSteps / 2; ++i) {          // 8 elements each
           const int e = CODES ? (i / 2) * 64 + t * 16 + (i % 2) * 8 : i * 32 + t * 8;
@@ -280,6 +300,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
           if (row < rows && e < p.c.D) u = ld_128(src + e * 2);
           w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
         }
+        unit[r] = 1.0f;
         if constexpr (CODES && !std::is_same<T, __half>::value) {
           float top = 0.0f;
 #pragma unroll
@@ -298,21 +319,26 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
           for (int i = 0; i < 2 * kSteps; ++i)
             w[i] = pack16<true>(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
         }
-        // step s of the product takes words 2 s and 2 s + 1
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) q[s][r] = w[2 * s], q[s][2 + r] = w[2 * s + 1];
       }
     }
     const float k_scale = CODES ? paged::head_scale(p.c.k_amax, p.c.amax_stride, h) : 1.0f;
     const float v_scale = CODES ? paged::head_scale(p.c.v_amax, p.c.amax_stride, h) : 1.0f;
     const float log2_scale = p.scale * k_scale * 1.4426950408889634f;
-    const float sl[2] = {log2_scale * unit[0], log2_scale * unit[1]};
+    float sl[BLOCKS8][2];                               // of heads 2 t and 2 t + 1, the columns of this lane's products
+#pragma unroll
+    for (int r = 0; r < BLOCKS8; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) sl[r][e] = log2_scale * __shfl_sync(0xffffffffu, unit[r], (2 * t + e) * 4);
 
     // ------------------------------------------------------------- the keys
-    float o[kOut][4];
+    float o[BLOCKS8][kSteps][4];                        // O^T: rows of 16 elements, heads 2 t and 2 t + 1
+    float m[BLOCKS8][2], l[BLOCKS8][2];
 #pragma unroll
-    for (int i = 0; i < kOut; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    for (int r = 0; r < BLOCKS8; ++r) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.0f;
+      m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.0f;
+    }
     bool any = false;
     for (int tile = tile0; tile < tile1;) {
 #pragma unroll
@@ -322,73 +348,59 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
           __syncwarp();
           const uint32_t ks = ring_u32 + s * S::kBytes, vs = ks + kKeys * S::kRowBytes, keys = there[s];
           any = any || keys != 0;
-          float x[2][4];
+          // S^T: keys g and g + 8, heads 2 t and 2 t + 1; two chains of sums, the products of one wait for each other
+          float x[BLOCKS8][4], y[BLOCKS8][4];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
-            const int key = n * 8 + g;
+          for (int r = 0; r < BLOCKS8; ++r) x[r][0] = x[r][1] = x[r][2] = x[r][3] = y[r][0] = y[r][1] = y[r][2] = y[r][3] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kSteps / (CODES ? 4 : 2); ++i) {
+            const uint4 u = lds128(ks + g * S::kRowBytes + S::k_chunk(g, i * 4 + t) * 16);
+            const uint4 v = lds128(ks + (g + 8) * S::kRowBytes + S::k_chunk(g + 8, i * 4 + t) * 16);
             if constexpr (CODES) {
+              const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (int i = 0; i < kSteps / 4; ++i) {
-                const uint4 u = lds128(ks + key * S::kRowBytes + S::k_chunk(key, i * 4 + t) * 16);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t a[4] = {codes_f16x2(uw[e]), codes_f16x2(vw[e]), codes_f16x2(uw[e] >> 16), codes_f16x2(vw[e] >> 16)};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mma<kHalf>(x[n], q[i * 4 + e], codes_f16x2(w[e]), codes_f16x2(w[e] >> 16));
+                for (int r = 0; r < BLOCKS8; ++r) mma<kHalf>(e & 1 ? y[r] : x[r], a, q[r][i * 4 + e][0], q[r][i * 4 + e][1]);
               }
             } else {
+              const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
 #pragma unroll
-              for (int i = 0; i < kSteps / 2; ++i) {
-                const uint4 u = lds128(ks + key * S::kRowBytes + S::k_chunk(key, i * 4 + t) * 16);
-                mma<kHalf>(x[n], q[i * 2], u.x, u.y);
-                mma<kHalf>(x[n], q[i * 2 + 1], u.z, u.w);
+              for (int r = 0; r < BLOCKS8; ++r) {
+                mma<kHalf>(x[r], a0, q[r][i * 2][0], q[r][i * 2][1]);
+                mma<kHalf>(y[r], a1, q[r][i * 2 + 1][0], q[r][i * 2 + 1][1]);
               }
             }
           }
+          const bool there0 = (keys >> g) & 1, there1 = (keys >> (g + 8)) & 1;
+          uint32_t pt[BLOCKS8][2];
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int r = 0; r < BLOCKS8; ++r) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[n][e] *= sl[e >> 1];
-              if (!((keys >> (n * 8 + t * 2 + (e & 1))) & 1)) x[n][e] = -INFINITY;
+            for (int e = 0; e < 4; ++e) x[r][e] = (e < 2 ? there0 : there1) ? (x[r][e] + y[r][e]) * sl[r][e & 1] : -INFINITY;
+            if (p.logits != nullptr) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int i = tile * kTile + warp * kKeys + g + 8 * (e >> 1), row = 8 * r + 2 * t + (e & 1);
+                if (row < rows && i < see.seen && see.token(i) < p.weights_len)
+                  p.logits[(static_cast<int64_t>(b) * p.Hq + head0 + row) * p.logits_stride + i] = x[r][e];
+              }
             }
-          if (p.logits != nullptr) {
-            const int i0 = tile * kTile + warp * kKeys + t * 2;
+            const float m0 = fmaxf(m[r][0], column_max(fmaxf(x[r][0], x[r][2]))), m1 = fmaxf(m[r][1], column_max(fmaxf(x[r][1], x[r][3])));
+            if (__any_sync(0xffffffffu, m0 > m[r][0] || m1 > m[r][1])) {
+              const float f0 = m0 == -INFINITY ? 1.0f : exp2_fast(m[r][0] - m0), f1 = m1 == -INFINITY ? 1.0f : exp2_fast(m[r][1] - m1);
+              l[r][0] *= f0, l[r][1] *= f1, m[r][0] = m0, m[r][1] = m1;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              if (g + 8 * r >= rows) continue;
-              float* dst = p.logits + (static_cast<int64_t>(b) * p.Hq + head0 + g + 8 * r) * p.logits_stride;
-#pragma unroll
-              for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int i = i0 + n * 8 + e;
-                  if (i < see.seen && see.token(i) < p.weights_len) dst[i] = x[n][2 * r + e];
-                }
+              for (int i = 0; i < kSteps; ++i) o[r][i][0] *= f0, o[r][i][1] *= f1, o[r][i][2] *= f0, o[r][i][3] *= f1;
             }
+            const float base0 = m0 == -INFINITY ? 0.0f : m0, base1 = m1 == -INFINITY ? 0.0f : m1;
+            x[r][0] = exp2_fast(x[r][0] - base0), x[r][1] = exp2_fast(x[r][1] - base1);
+            x[r][2] = exp2_fast(x[r][2] - base0), x[r][3] = exp2_fast(x[r][3] - base1);
+            l[r][0] += x[r][0] + x[r][2], l[r][1] += x[r][1] + x[r][3];
+            pt[r][0] = transpose8x8(pack16<kHalf>(x[r][0], x[r][1]));
+            pt[r][1] = transpose8x8(pack16<kHalf>(x[r][2], x[r][3]));
           }
-          float mx[2];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) mx[r] = fmaxf(m[r], quad_max(fmaxf(fmaxf(x[0][2 * r], x[0][2 * r + 1]), fmaxf(x[1][2 * r], x[1][2 * r + 1]))));
-          if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const float f = mx[r] == -INFINITY ? 1.0f : exp2_fast(m[r] - mx[r]);
-              l[r] *= f;
-#pragma unroll
-              for (int i = 0; i < kOut; ++i) o[i][2 * r] *= f, o[i][2 * r + 1] *= f;
-              m[r] = mx[r];
-            }
-          }
-          const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[n][e] = exp2_fast(x[n][e] - base[e >> 1]);
-              l[e >> 1] += x[n][e];
-            }
-          const uint32_t a[4] = {pack16<kHalf>(x[0][0], x[0][1]), pack16<kHalf>(x[0][2], x[0][3]), pack16<kHalf>(x[1][0], x[1][1]),
-                                 pack16<kHalf>(x[1][2], x[1][3])};
           if constexpr (CODES) {
             constexpr int kWords = DPAD / 32;           // of the row pieces that this lane widens
             uint32_t w[4][kWords];
@@ -407,19 +419,22 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
             for (int i = 0; i < kWords; ++i) {
               const uint32_t lo0 = __byte_perm(w[0][i], w[1][i], 0x5140), hi0 = __byte_perm(w[0][i], w[1][i], 0x7362);
               const uint32_t lo1 = __byte_perm(w[2][i], w[3][i], 0x5140), hi1 = __byte_perm(w[2][i], w[3][i], 0x7362);
-              mma<kHalf>(o[4 * i], a, codes_f16x2(lo0), codes_f16x2(lo1));
-              mma<kHalf>(o[4 * i + 1], a, codes_f16x2(lo0 >> 16), codes_f16x2(lo1 >> 16));
-              mma<kHalf>(o[4 * i + 2], a, codes_f16x2(hi0), codes_f16x2(hi1));
-              mma<kHalf>(o[4 * i + 3], a, codes_f16x2(hi0 >> 16), codes_f16x2(hi1 >> 16));
+              const uint32_t a0[4] = {codes_f16x2(lo0), codes_f16x2(lo0 >> 16), codes_f16x2(lo1), codes_f16x2(lo1 >> 16)};
+              const uint32_t a1[4] = {codes_f16x2(hi0), codes_f16x2(hi0 >> 16), codes_f16x2(hi1), codes_f16x2(hi1 >> 16)};
+#pragma unroll
+              for (int r = 0; r < BLOCKS8; ++r) {
+                mma<kHalf>(o[r][2 * i], a0, pt[r][0], pt[r][1]);
+                mma<kHalf>(o[r][2 * i + 1], a1, pt[r][0], pt[r][1]);
+              }
             }
           } else {
-            const int key = (lane & 7) + (lane & 8);
+            const int key = (lane & 7) + ((lane >> 4) & 1) * 8;
 #pragma unroll
-            for (int i = 0; i < kOut; i += 2) {
-              uint32_t r[4];
-              ldmatrix_trans(vs + key * S::kRowBytes + S::v_chunk(key, i + (lane >> 4)) * 16, r);
-              mma<kHalf>(o[i], a, r[0], r[1]);
-              mma<kHalf>(o[i + 1], a, r[2], r[3]);
+            for (int i = 0; i < kSteps; ++i) {
+              uint32_t a[4];
+              ldmatrix_trans(vs + key * S::kRowBytes + S::v_chunk(key, 2 * i + ((lane >> 3) & 1)) * 16, a);
+#pragma unroll
+              for (int r = 0; r < BLOCKS8; ++r) mma<kHalf>(o[r][i], a, pt[r][0], pt[r][1]);
             }
           }
           __syncwarp();
@@ -434,19 +449,19 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
     __syncwarp();
 
     // ------------------------------------------------------------- the four warps' parts together
+    float* mine = reinterpret_cast<float*>(ring);     // rows of DPAD: the ring is empty
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (t == 0) row_max[warp][g + 8 * r] = m[r], row_sum[warp][g + 8 * r] = any ? l[r] : -1.0f;   // -1: no key at all
-    }
-    float* mine = reinterpret_cast<float*>(ring);     // 16 rows of DPAD: the ring is empty
+    for (int r = 0; r < BLOCKS8; ++r)
 #pragma unroll
-    for (int i = 0; i < kOut; ++i)
+      for (int e = 0; e < 2; ++e) {
+        const int row = 8 * r + 2 * t + e;
+        const float sum = column_sum(l[r][e]);
+        if (g == 0) row_max[warp][row] = m[r][e], row_sum[warp][row] = any ? sum : -1.0f;   // -1: no key at all
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int n = t * 2 + (e & 1), d = CODES ? n * (DPAD / 8) + i : i * 8 + n;
-        mine[(g + 8 * (e >> 1)) * DPAD + d] = o[i][e];
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            mine[row * DPAD + (CODES ? g * (DPAD / 8) + 2 * i + half : 16 * i + 8 * half + g)] = o[r][i][2 * half + e];
       }
     __syncthreads();
     const bool whole = tile0 == 0 && tile1 == tiles;
@@ -506,17 +521,32 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
           const int row = i / kQuads, d = (i % kQuads) * 4;
           float top = -INFINITY, sum = 0.0f, acc[4] = {};
           bool has = false;
-          for (int c = c0; c <= c1; ++c) {
-            if (total < ctas && piece(total, c, ctas) == piece(total, c + 1, ctas)) continue;
-            const float* src = p.parts + (static_cast<int64_t>(c) * 2 + (c == c0 && second ? 1 : 0)) * kPart;
-            const float pm = __ldcg(src + kRows * DPAD + row), ps = __ldcg(src + kRows * DPAD + kRows + row);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(src + row * DPAD + d));
-            if (ps < 0.0f) continue;
-            has = true;
-            const float now = fmaxf(top, pm), base = now == -INFINITY ? 0.0f : now, f0 = exp2_fast(top - base), f1 = exp2_fast(pm - base);
-            sum = sum * f0 + ps * f1;
-            acc[0] = acc[0] * f0 + v.x * f1, acc[1] = acc[1] * f0 + v.y * f1, acc[2] = acc[2] * f0 + v.z * f1, acc[3] = acc[3] * f0 + v.w * f1;
-            top = now;
+          constexpr int kAtOnce = 4;
+          int c = c0;
+          while (c <= c1) {
+            float pm[kAtOnce], ps[kAtOnce];
+            float4 v[kAtOnce];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {        // the loads first: they do not wait for one another
+              if (total < ctas)
+                while (c <= c1 && piece(total, c, ctas) == piece(total, c + 1, ctas)) ++c;
+              ps[k] = -1.0f;
+              if (c > c1) continue;
+              const float* src = p.parts + (static_cast<int64_t>(c) * 2 + (c == c0 && second ? 1 : 0)) * kPart;
+              pm[k] = __ldcg(src + kRows * DPAD + row), ps[k] = __ldcg(src + kRows * DPAD + kRows + row);
+              v[k] = __ldcg(reinterpret_cast<const float4*>(src + row * DPAD + d));
+              ++c;
+            }
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+              if (ps[k] < 0.0f) continue;
+              has = true;
+              const float now = fmaxf(top, pm[k]), base = now == -INFINITY ? 0.0f : now, f0 = exp2_fast(top - base), f1 = exp2_fast(pm[k] - base);
+              sum = sum * f0 + ps[k] * f1;
+              acc[0] = acc[0] * f0 + v[k].x * f1, acc[1] = acc[1] * f0 + v[k].y * f1;
+              acc[2] = acc[2] * f0 + v[k].z * f1, acc[3] = acc[3] * f0 + v[k].w * f1;
+              top = now;
+            }
           }
           if (d < p.c.D) {
             const float f = v_scale / sum;
@@ -555,12 +585,12 @@ __global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ De
   }
 }
 
-template <typename T, bool CODES, int DPAD>
+template <typename T, bool CODES, int DPAD, int BLOCKS8>
 int launch_decode(const DecodeParams& p, int64_t most_tiles, cudaStream_t st) {
-  using S = Stage<CODES, DPAD>;
+  using S = Stage<CODES, DPAD, BLOCKS8>;
   constexpr int kSmem = kWarps * S::kDepth * S::kBytes;
-  static_assert(S::kDepth * S::kBytes >= kRows * DPAD * 4, "a warp's result takes its ring");
-  auto kernel = decode_kernel<T, CODES, DPAD>;
+  static_assert(S::kDepth * S::kBytes >= 8 * BLOCKS8 * DPAD * 4, "a warp's result takes its ring");
+  auto kernel = decode_kernel<T, CODES, DPAD, BLOCKS8>;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return B200Q_ERR_CUDA;
   static std::atomic<int> resident[64];                // CTAs that one SM holds; 0: not asked yet
@@ -579,7 +609,8 @@ int launch_decode(const DecodeParams& p, int64_t most_tiles, cudaStream_t st) {
 
 template <typename T, bool CODES>
 int launch_decode_d(const DecodeParams& p, int64_t most_tiles, cudaStream_t st) {
-  return p.c.D <= 64 ? launch_decode<T, CODES, 64>(p, most_tiles, st) : launch_decode<T, CODES, 128>(p, most_tiles, st);
+  if (p.rows <= 8) return p.c.D <= 64 ? launch_decode<T, CODES, 64, 1>(p, most_tiles, st) : launch_decode<T, CODES, 128, 1>(p, most_tiles, st);
+  return p.c.D <= 64 ? launch_decode<T, CODES, 64, 2>(p, most_tiles, st) : launch_decode<T, CODES, 128, 2>(p, most_tiles, st);
 }
 
 int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
