@@ -635,7 +635,7 @@ int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, co
                           size_t workspace_bytes, void* scratch, size_t scratch_bytes, b200q_stream_t stream) {
   DecodeParams p{};
   if (int rc = paged::make_cache(&p.c, cache, dtype, block_table, table_stride, table_width, lens, B)) return rc;
-  if (Hq <= 0 || Hq > 65535 || Hq % p.c.heads != 0 || sinks < 0 || !(scale == scale) || B > 65535) return B200Q_ERR_INVALID;
+  if (Hq <= 0 || Hq > 65535 || Hq % p.c.heads != 0 || sinks < 0 || !(scale >= 0.0f) || B > 65535) return B200Q_ERR_INVALID;
   if (B == 0) return B200Q_OK;
   if (q == nullptr || q_strides == nullptr || out == nullptr || (weights != nullptr && (weights_len < 0 || weights_len > 0x7fffff00LL)))
     return B200Q_ERR_INVALID;

@@ -1,8 +1,38 @@
 // Causal attention with a sliding window and sinks over contiguous K and V.
+//
+//   x_ij = (q_i . k_j) * scale over the keys j that row i sees: j <= p_i with j > p_i - window or j < sinks
+//   out_i = sum_j exp(x_ij - m_i) v_j / sum_j exp(x_ij - m_i)
+//
+// 4 D operations a pair of row and key that see each other, and one exponential: for D = 128 the tensor cores and the special-function
+// units of an SM need the same time (a tile of 128 rows and 128 keys is 1024 clocks of both), so the two have to run under each
+// other all the time.
+//
+// A CTA, one to an SM, holds two tiles of 128 query rows: of two heads that share their K and V where the group is even, of one head
+// otherwise; with few queries a tile holds the rows of several heads.  One warp loads (TMA; Q once, then K and V tiles of 128
+// keys through a ring), one issues tcgen05.mma (S = Q K^T into tensor memory, O += P V with P read from tensor memory), and four
+// warps for each query tile run its softmax, one thread to a row, so that maximum and sum need no exchange: while one tile is in its softmax
+// the tensor cores work on the other.  P takes the place of the S it came from.  Only key tiles that some row of the CTA
+// sees are visited, and a query tile passes over those that none of its own rows sees; the comparisons of the mask
+// run on tiles at an edge of it.
+//
+// The running maximum is followed lazily: O and the sum stay referred to an older maximum while the new one is at most 2^8 times
+// larger, which 32-bit sums and the exponent range of both 16-bit types hold without loss; so the rescaling of O in tensor memory is
+// rare.  Rounding: S, the softmax, O and the sums are 32-bit; P is rounded to 16 bits for the second product, an error of one rounding
+// of each term, of the size of the result's own.
+//
+// A masked key has P = 0, and 0 times an infinity or a NaN of its V row would be a NaN: rows whose result is not finite are computed
+// again, by one warp each, over the keys that they see.  That costs nothing where all is finite.
+#include <cuda.h>
+
 #include "common.cuh"
+#include "gemm_host.cuh"
+#include "tcgen05.cuh"
 
 namespace b200q {
 namespace {
+
+constexpr int kTileRows = 128, kTileKeys = 128, kThreads = 320, kTmemCols = 512;
+constexpr float kLazy = 8.0f;   // log2 of how far the reference may lie below the maximum
 
 struct WindowParams {
   const char* q;
@@ -12,10 +42,18 @@ struct WindowParams {
   int64_t q_s[3], k_s[3], v_s[3], o_s[3];   // batch, head, row; elements
   const int32_t* q_lens;
   const int32_t* k_lens;
-  int Hq, group, Sq, Sk, D;
+  int Hq, Hkv, group, Sq, Sk, D;
   float scale;
-  int64_t window, sinks;
+  int window, sinks;         // window 0: none
+  int rp, nh;                // rows of one head and heads in a query tile, rp * nh = 128
+  int pair_heads;            // the second query tile: the next heads (1) or the next rows (0)
+  int units;                 // CTAs that share a kv head and rows
+  int q_blocks;
+  int B;
+  int* status;
 };
+
+__device__ __forceinline__ void timed_out(int* status, int where) { atomicCAS(status, 0, where); }
 
 __device__ __forceinline__ int length_of(const int32_t* lens, int b, int most) {
   if (lens == nullptr) return most;
@@ -24,9 +62,48 @@ __device__ __forceinline__ int length_of(const int32_t* lens, int b, int most) {
   return min(max(n, 0), most);
 }
 
+// 4-D tiled load into this CTA's shared memory, completion on this CTA's own barrier.
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int32_t x, int32_t y, int32_t z, int32_t w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(ptx::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(ptx::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+// kind::f16, fp32 accumulator; format 0 = fp16, 1 = bf16 for both operands; B K-major or N-major
+__device__ __forceinline__ uint32_t idesc_16(int format, int m, int n, int b_n_major) {
+  return (1u << 4) | (static_cast<uint32_t>(format) << 7) | (static_cast<uint32_t>(format) << 10) | (static_cast<uint32_t>(b_n_major) << 16) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, float* f) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  uint2 u;
+  asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(p) : "memory");
   if constexpr (std::is_same<T, __half>::value) {
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
     f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
@@ -36,13 +113,61 @@ __device__ __forceinline__ void load4(const T* p, float* f) {
   }
 }
 
-// One warp per query row, a lane four elements of a row, one key after the other.
+// What a CTA works on.
+struct Work {
+  int b, kv_head, nq, off;                  // off: position of query 0
+  int head[2], q0[2], lowest[2], highest[2];  // per query tile: first head, first query, positions of its rows (highest < 0: none)
+  int sink_tiles, first, tiles;             // key tiles 0 .. sink_tiles - 1, then first, first + 1, ..
+  __device__ __forceinline__ int tile(int j) const { return j < sink_tiles ? j : first + j - sink_tiles; }
+  __device__ __forceinline__ bool needs(const WindowParams& p, int s, int t) const {
+    const int k0 = t * kTileKeys;
+    return k0 <= highest[s] && (p.window == 0 || k0 + kTileKeys - 1 > lowest[s] - p.window || k0 < p.sinks);
+  }
+};
+
+__device__ __forceinline__ Work work_of(const WindowParams& p) {
+  Work w;
+  const int per_row_block = p.B * p.Hkv * p.units;
+  // the last queries first: they see most
+  const int block = p.q_blocks - 1 - static_cast<int>(blockIdx.x) / per_row_block, at = static_cast<int>(blockIdx.x) % per_row_block;
+  const int unit = at % p.units;
+  w.kv_head = at / p.units % p.Hkv;
+  w.b = at / p.units / p.Hkv;
+  w.nq = length_of(p.q_lens, w.b, p.Sq);
+  const int nk = length_of(p.k_lens, w.b, p.Sk);
+  w.off = nk - w.nq;
+  int low = 0x7fffffff, high = -1;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    w.head[s] = w.kv_head * p.group + (p.pair_heads ? 2 * unit + s : unit) * p.nh;
+    w.q0[s] = p.pair_heads ? block * p.rp : (2 * block + s) * p.rp;
+    w.lowest[s] = max(w.q0[s] + w.off, 0);
+    w.highest[s] = w.q0[s] < w.nq ? min(w.q0[s] + p.rp, w.nq) - 1 + w.off : -1;
+    if (w.highest[s] >= 0) low = min(low, w.lowest[s]), high = max(high, w.highest[s]);
+  }
+  w.sink_tiles = w.first = w.tiles = 0;
+  if (high >= 0) {
+    if (p.window > 0) {
+      w.first = max(0, low - p.window + 1) / kTileKeys;
+      w.sink_tiles = min((min(p.sinks, high + 1) + kTileKeys - 1) / kTileKeys, w.first);
+    }
+    w.tiles = w.sink_tiles + high / kTileKeys - w.first + 1;
+  }
+  return w;
+}
+
+template <int DPAD>
+struct Layout {
+  static constexpr int kBoxes = DPAD / 64, kBoxBytes = 128 * 128, kTileBytes = kBoxes * kBoxBytes;
+  static constexpr int kStages = DPAD == 128 ? 5 : 8;
+  static constexpr int kBars = 2 * kStages + 1 + 6 + 1;
+  static constexpr int kSmem = 1024 + (2 + kStages) * kTileBytes + kBars * 8 + 16;
+};
+
+// One row over the keys that it sees, by one warp, four elements a lane: for rows that a masked key spoiled.
 template <typename T>
-__global__ void __launch_bounds__(128) window_kernel(const __grid_constant__ WindowParams p) {
-  const int lane = threadIdx.x & 31, row = blockIdx.x * 4 + (threadIdx.x >> 5), b = blockIdx.y / p.Hq, h = blockIdx.y % p.Hq;
-  if (row >= p.Sq) return;
-  const int nq = length_of(p.q_lens, b, p.Sq), nk = length_of(p.k_lens, b, p.Sk);
-  const int at = row < nq ? row + nk - nq : -1;
+__device__ __noinline__ void row_again(const WindowParams& p, int b, int h, int row, int at) {
+  const int lane = threadIdx.x & 31;
   const bool mine = lane * 4 < p.D;
   const T* k = reinterpret_cast<const T*>(p.k) + b * p.k_s[0] + h / p.group * p.k_s[1] + lane * 4;
   const T* v = reinterpret_cast<const T*>(p.v) + b * p.v_s[0] + h / p.group * p.v_s[1] + lane * 4;
@@ -50,7 +175,7 @@ __global__ void __launch_bounds__(128) window_kernel(const __grid_constant__ Win
   if (mine) load4(reinterpret_cast<const T*>(p.q) + b * p.q_s[0] + h * p.q_s[1] + row * p.q_s[2] + lane * 4, q);
   for (int j = 0; j <= at; ++j) {
     if (p.window > 0 && j >= p.sinks && at - j >= p.window) {
-      j = static_cast<int>(at - p.window);
+      j = at - p.window;
       continue;
     }
     float x[4] = {}, y[4] = {}, s = 0.0f;
@@ -62,9 +187,302 @@ __global__ void __launch_bounds__(128) window_kernel(const __grid_constant__ Win
     for (int i = 0; i < 4; ++i) o[i] = o[i] * f + e * y[i];
     l = l * f + e, m = mn;
   }
-  T* out = reinterpret_cast<T*>(p.out) + b * p.o_s[0] + h * p.o_s[1] + row * p.o_s[2] + lane * 4;
-  if (mine)
-    for (int i = 0; i < 4; ++i) out[i] = static_cast<T>(at < 0 ? 0.0f : o[i] / l);
+  if (mine) {
+    const uint2 r = make_uint2(pack16<T>(o[0] / l, o[1] / l), pack16<T>(o[2] / l, o[3] / l));
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + b * p.o_s[0] + h * p.o_s[1] + row * p.o_s[2] + lane * 4) = r;
+  }
+}
+
+template <typename T, int DPAD>
+__global__ void __launch_bounds__(kThreads, 1)
+window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+              const __grid_constant__ WindowParams p) {
+  using L = Layout<DPAD>;
+  extern __shared__ char smem_raw[];
+  char* const base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
+  char* const sq = base;
+  char* const ring = base + 2 * L::kTileBytes;
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(ring + L::kStages * L::kTileBytes);
+  uint64_t* const full = bars;
+  uint64_t* const empty = bars + L::kStages;
+  uint64_t* const q_full = empty + L::kStages;
+  uint64_t* const s_full = q_full + 1;
+  uint64_t* const p_full = s_full + 2;
+  uint64_t* const o_full = p_full + 2;
+  uint64_t* const done = o_full + 2;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == 8) {
+    ptx::tmem_alloc<1>(tmem_slot, kTmemCols);
+    ptx::tmem_relinquish<1>();
+  } else if (threadIdx.x == 0) {
+    for (int i = 0; i < 2 * L::kStages + 1; ++i) ptx::mbar_init(bars + i, 1);
+    for (int s = 0; s < 2; ++s) ptx::mbar_init(s_full + s, 1), ptx::mbar_init(p_full + s, 4), ptx::mbar_init(o_full + s, 1);
+    ptx::mbar_init(done, 1);
+    ptx::fence_barrier_init();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();
+  const Work w = work_of(p);
+
+  if (warp == 9) {
+    // ------------------------------------------------------------- loads
+    if (lane == 0 && w.tiles > 0) {
+      ptx::mbar_arrive_expect_tx(q_full, 2 * L::kTileBytes);
+      for (int s = 0; s < 2; ++s)
+        for (int x = 0; x < L::kBoxes; ++x) tma_load_4d(sq + s * L::kTileBytes + x * L::kBoxBytes, &tq, q_full, x * 64, w.q0[s], w.head[s], w.b);
+      int st = 0, issued = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int j = 0; j < w.tiles && ok; ++j) {
+        const int row = w.tile(j) * kTileKeys;
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!ptx::mbar_wait(empty + st, ph ^ 1u)) {
+            timed_out(p.status, 80);
+            ok = false;
+            break;
+          }
+          ptx::mbar_arrive_expect_tx(full + st, L::kTileBytes);
+          for (int x = 0; x < L::kBoxes; ++x)
+            tma_load_4d(ring + st * L::kTileBytes + x * L::kBoxBytes, kv == 0 ? &tk : &tv, full + st, x * 64, row, w.kv_head, w.b);
+          ++issued;
+          if (++st == L::kStages) st = 0, ph ^= 1u;
+        }
+      }
+      // no copy may be under way when the CTA ends, whatever became of its readers
+      if (!ptx::mbar_wait(q_full, 0)) timed_out(p.status, 81);
+      for (int i = max(0, issued - L::kStages); i < issued; ++i)
+        if (!ptx::mbar_wait(full + i % L::kStages, (i / L::kStages) & 1)) timed_out(p.status, 81);
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------- products
+    if (lane == 0 && w.tiles > 0) {
+      constexpr int kFormat = std::is_same<T, __half>::value ? 0 : 1;
+      const uint32_t id_s = idesc_16(kFormat, 128, kTileKeys, 0), id_o = idesc_16(kFormat, 128, p.D, 1);
+      const int steps = p.D / 16;
+      // V as the second operand: rows of 64 elements of D, 8 keys to 1024 bytes, the next 64 elements a box further on
+      constexpr uint32_t kHiV = (1024u >> 4) | (1u << 14) | (2u << 29);
+      constexpr uint32_t kLeadV = (L::kBoxBytes >> 4) << 16;
+      bool ok = ptx::mbar_wait(q_full, 0);
+      if (!ok) timed_out(p.status, 82);
+      uint32_t p_phase[2] = {0, 0};
+      bool waiting[2] = {false, false}, begun[2] = {false, false};   // a P that is to be multiplied; O holds something
+      int v_stage = 0;                                               // of the key tile before
+      for (int j = 0; j <= w.tiles && ok; ++j) {
+        const int k_load = 2 * j, k_stage = k_load % L::kStages;
+        const bool more = j < w.tiles;
+        const int t = more ? w.tile(j) : 0;
+        bool k_here = false, v_here = false;
+        for (int s = 0; s < 2 && ok; ++s) {
+          if (waiting[s]) {
+            if (!v_here) {
+              const int v_load = 2 * j - 1;
+              v_stage = v_load % L::kStages;
+              ok = ptx::mbar_wait(full + v_stage, (v_load / L::kStages) & 1);
+              v_here = true;
+            }
+            ok = ok && ptx::mbar_wait(p_full + s, p_phase[s]);
+            if (!ok) {
+              timed_out(p.status, 83);
+              break;
+            }
+            p_phase[s] ^= 1u;
+            ptx::tc_fence_after();
+            const uint32_t lo = ((ptx::smem_u32(ring + v_stage * L::kTileBytes) >> 4) & 0x3fffu) | kLeadV;
+#pragma unroll
+            for (int k = 0; k < kTileKeys / 16; ++k)
+              mma_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, ptx::desc_join(lo + k * (2048 >> 4), kHiV), id_o, begun[s] || k > 0);
+            begun[s] = true;
+            waiting[s] = false;
+          }
+          if (more && w.needs(p, s, t)) {
+            if (!k_here) {
+              ok = ptx::mbar_wait(full + k_stage, (k_load / L::kStages) & 1);
+              k_here = true;
+              if (!ok) {
+                timed_out(p.status, 84);
+                break;
+              }
+              ptx::tc_fence_after();
+            }
+            const uint32_t a = ptx::desc_lo_sw128(ptx::smem_u32(sq + s * L::kTileBytes)), b = ptx::desc_lo_sw128(ptx::smem_u32(ring + k_stage * L::kTileBytes));
+            for (int k = 0; k < steps; ++k) {
+              const uint32_t at = ((k >> 2) * L::kBoxBytes + (k & 3) * 32) >> 4;
+              mma_ss(tmem + s * 128, ptx::desc_join(a + at, ptx::kDescHiSw128), ptx::desc_join(b + at, ptx::kDescHiSw128), id_s, k > 0);
+            }
+            ptx::tc_commit<1>(s_full + s);
+            waiting[s] = true;
+          }
+        }
+        // a stage is given back only once its copy has arrived, read or not
+        if (ok && more && !k_here) ok = ptx::mbar_wait(full + k_stage, (k_load / L::kStages) & 1);
+        if (ok && j > 0 && !v_here) ok = ptx::mbar_wait(full + (k_load - 1) % L::kStages, ((k_load - 1) / L::kStages) & 1);
+        if (!ok) {
+          timed_out(p.status, 84);
+          break;
+        }
+        if (j > 0) ptx::tc_commit<1>(empty + (2 * j - 1) % L::kStages);     // V of the tile before
+        if (more) ptx::tc_commit<1>(empty + k_stage);
+      }
+      for (int s = 0; s < 2; ++s) ptx::tc_commit<1>(o_full + s);
+      ptx::tc_commit<1>(done);
+      if (!ptx::mbar_wait(done, 0)) timed_out(p.status, 85);
+    }
+  } else {
+    // ------------------------------------------------------------- softmax of query tile s, one thread to a row
+    const int s = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;     // this warp's 32 lanes of tensor memory
+    const uint32_t ts = tmem + s * 128 + lanes, to = tmem + 256 + s * 128 + lanes;
+    const int h = w.head[s] + r / p.rp, i = w.q0[s] + r % p.rp;
+    const int at = i < w.nq ? i + w.off : -1;                         // position; < 0: sees nothing
+    const float sl = fmaxf(p.scale * 1.4426950408889634f, 1e-30f);    // 0 times a masked -inf would be NaN
+    const uint64_t sl2 = pack2(sl, sl);
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true, begun = false;
+    uint32_t phase = 0;
+    for (int j = 0; j < w.tiles && ok; ++j) {
+      const int t = w.tile(j), k0 = t * kTileKeys;
+      if (!w.needs(p, s, t)) continue;
+      ok = ptx::mbar_wait(s_full + s, phase);
+      if (!ok) {
+        timed_out(p.status, 86);
+        break;
+      }
+      phase ^= 1u;
+      ptx::tc_fence_after();
+      uint32_t x[kTileKeys];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32(ts + c * 32, x + c * 32);
+      ptx::tmem_ld_wait();
+      const bool inside = k0 + kTileKeys - 1 <= w.lowest[s] && w.q0[s] + p.rp <= w.nq && w.q0[s] + w.off >= 0 &&
+                          (p.window == 0 || k0 > w.highest[s] - p.window || k0 + kTileKeys <= p.sinks);
+      if (!inside) {
+        const int last = at - k0, first = p.window > 0 ? last - p.window : -1, sinks = p.sinks - k0;
+#pragma unroll
+        for (int c = 0; c < kTileKeys; ++c)
+          if (c > last || (c <= first && c >= sinks)) x[c] = 0xff800000u;
+      }
+      float top[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) top[c] = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[4 + c]));
+#pragma unroll
+      for (int c = 8; c < kTileKeys; c += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(__uint_as_float(x[c + e]), __uint_as_float(x[c + 4 + e])));
+      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      if (!begun) {
+        m = mx;
+        begun = true;
+      } else if (__any_sync(0xffffffffu, (mx - m) * sl > kLazy)) {
+        // O is complete up to the tile before: its product was issued in front of the S that has just arrived
+        const float now = fmaxf(m, mx), f = now == -INFINITY ? 1.0f : exp2_fast((m - now) * sl);
+        m = now;
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < DPAD / 32; ++c) {
+          uint32_t o[32];
+          ptx::tmem_ld_32x32(to + c * 32, o);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          ptx::tmem_st_32x32_x16(to + c * 32, o);
+          ptx::tmem_st_32x32_x16(to + c * 32 + 16, o + 16);
+        }
+      }
+      const float back = m == -INFINITY ? 0.0f : -m * sl;
+      const uint64_t back2 = pack2(back, back);
+      uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll
+      for (int c = 0; c < kTileKeys; c += 32) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float2 a = unpack2(fma2(pack2(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 1])), sl2, back2));
+          const float2 b = unpack2(fma2(pack2(__uint_as_float(x[c + e + 2]), __uint_as_float(x[c + e + 3])), sl2, back2));
+          const float e0 = exp2_fast(a.x), e1 = exp2_fast(a.y), e2 = exp2_fast(b.x), e3 = exp2_fast(b.y);
+          sum0 = add2(sum0, pack2(e0, e1));
+          sum1 = add2(sum1, pack2(e2, e3));
+          pk[e / 2] = pack16<T>(e0, e1);
+          pk[e / 2 + 1] = pack16<T>(e2, e3);
+        }
+        ptx::tmem_st_32x32_x16(ts + c / 2, pk);
+      }
+      const float2 s0 = unpack2(sum0), s1 = unpack2(sum1);
+      l += (s0.x + s0.y) + (s1.x + s1.y);
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(p_full + s);
+    }
+    if (ok && w.tiles > 0 && !ptx::mbar_wait(o_full + s, 0)) {
+      timed_out(p.status, 87);
+      ok = false;
+    }
+    if (ok) {
+      ptx::tc_fence_after();
+      const float f = 1.0f / l;
+      float probe = 0.0f;
+      T* dst = reinterpret_cast<T*>(p.out) + w.b * p.o_s[0] + h * p.o_s[1] + static_cast<int64_t>(i) * p.o_s[2];
+#pragma unroll
+      for (int c = 0; c < DPAD / 32; ++c) {
+        uint32_t o[32];
+        if (begun) {
+          ptx::tmem_ld_32x32(to + c * 32, o);
+          ptx::tmem_ld_wait();
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          if (c * 32 + e >= p.D || i >= p.Sq) continue;
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (at >= 0) {
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(o[e + k]) * f, probe = fmaf(y[k], 0.0f, probe);
+            u = make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
+          }
+          *reinterpret_cast<uint4*>(dst + c * 32 + e) = u;
+        }
+      }
+      for (unsigned bad = __ballot_sync(0xffffffffu, probe != probe); bad; bad &= bad - 1) {
+        const int who = __ffs(bad) - 1;
+        row_again<T>(p, w.b, __shfl_sync(0xffffffffu, h, who), __shfl_sync(0xffffffffu, i, who), __shfl_sync(0xffffffffu, at, who));
+      }
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<1>(tmem, kTmemCols);
+  }
+}
+
+// [D, rows, heads, batches] of 16-bit elements -> boxes of 64 x box_rows x box_heads, 128-byte swizzle, zeros out of bounds
+int make_map(CUtensorMap* map, const void* base, int dtype, int64_t D, int64_t rows, int64_t heads, int64_t B, const int64_t* s, int box_rows, int box_heads) {
+  gemm::EncodeTiledFn fn = gemm::encode_tiled();
+  if (fn == nullptr) return B200Q_ERR_CUDA;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(B)};
+  // where there is one only, any stride will do
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(rows > 1 ? 2 * s[2] : 2 * D), static_cast<cuuint64_t>(heads > 1 ? 2 * s[1] : 2 * D),
+                                 static_cast<cuuint64_t>(B > 1 ? 2 * s[0] : 2 * D)};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(box_heads), 1};
+  const cuuint32_t unit[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, dtype == B200Q_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides,
+                        box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B200Q_OK : B200Q_ERR_CUDA;
+}
+
+template <typename T, int DPAD>
+int launch_window(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const WindowParams& p, unsigned ctas, cudaStream_t st) {
+  auto kernel = window_kernel<T, DPAD>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DPAD>::kSmem) != cudaSuccess) return B200Q_ERR_CUDA;
+  if (launch_pdl(kernel, dim3(ctas), dim3(kThreads), Layout<DPAD>::kSmem, st, tq, tk, tv, p) != cudaSuccess) return B200Q_ERR_CUDA;
+  return check_launch();
 }
 
 }  // namespace
@@ -78,14 +496,15 @@ int b200q_window_attention(const void* q, const void* k, const void* v, int dtyp
                            const int32_t* q_lens, const int32_t* k_lens, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D,
                            float scale, int64_t window, int64_t sinks, b200q_stream_t stream) {
   if (dtype != B200Q_F16 && dtype != B200Q_BF16) return B200Q_ERR_INVALID;
-  if (B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Sq < 0 || Sk < 0 || Sq > 0x7fffff00LL || Sk > 0x7fffff00LL || D <= 0 || D > 128 ||
-      D % 16 != 0 || sinks < 0 || !(scale == scale) || B > 65535 || B * Hq > 65535)
+  if (B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Sq < 0 || Sk < 0 || Sq > 0x3fffff00LL || Sk > 0x3fffff00LL || D <= 0 || D > 128 ||
+      D % 16 != 0 || sinks < 0 || !(scale >= 0.0f) || B > 65535 || B * Hq > 65535)
     return B200Q_ERR_INVALID;
   if (B == 0 || Sq == 0) return B200Q_OK;
   if (q == nullptr || out == nullptr || strides == nullptr || out_strides == nullptr || (Sk > 0 && (k == nullptr || v == nullptr))) return B200Q_ERR_INVALID;
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16)) return B200Q_ERR_ALIGN;
+  const int64_t sizes[9] = {B, Hq, Sq, B, Hkv, Sk, B, Hkv, Sk};
   for (int i = 0; i < 9; ++i)
-    if (strides[i] < 0 || strides[i] % 8 != 0) return B200Q_ERR_ALIGN;
+    if (strides[i] < 0 || strides[i] % 8 != 0 || strides[i] >= (1LL << 39) || (sizes[i] > 1 && strides[i] == 0)) return B200Q_ERR_ALIGN;
   for (int i = 0; i < 3; ++i)
     if (out_strides[i] < 0 || out_strides[i] % 8 != 0) return B200Q_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
@@ -93,12 +512,31 @@ int b200q_window_attention(const void* q, const void* k, const void* v, int dtyp
   p.q = static_cast<const char*>(q), p.k = static_cast<const char*>(k), p.v = static_cast<const char*>(v), p.out = static_cast<char*>(out);
   for (int i = 0; i < 3; ++i) p.q_s[i] = strides[i], p.k_s[i] = strides[3 + i], p.v_s[i] = strides[6 + i], p.o_s[i] = out_strides[i];
   p.q_lens = q_lens, p.k_lens = k_lens;
-  p.Hq = static_cast<int>(Hq), p.group = static_cast<int>(Hq / Hkv), p.Sq = static_cast<int>(Sq), p.Sk = static_cast<int>(Sk), p.D = static_cast<int>(D);
-  p.scale = scale, p.window = window, p.sinks = sinks;
-  const dim3 grid(static_cast<unsigned>((Sq + 3) / 4), static_cast<unsigned>(B * Hq));
+  p.Hq = static_cast<int>(Hq), p.Hkv = static_cast<int>(Hkv), p.group = static_cast<int>(Hq / Hkv);
+  p.Sq = static_cast<int>(Sq), p.Sk = static_cast<int>(Sk), p.D = static_cast<int>(D), p.B = static_cast<int>(B);
+  p.scale = scale;
+  p.window = window <= 0 || window >= Sk ? 0 : static_cast<int>(window);     // as wide as the keys: none
+  p.sinks = static_cast<int>(sinks < Sk ? sinks : Sk);
+  p.status = gemm::device_status_word();
+  if (p.status == nullptr) return B200Q_ERR_CUDA;
+  // few queries: the rows of several heads of a group in one tile
+  p.rp = kTileRows, p.nh = 1;
+  while (p.rp > 8 && Sq <= p.rp / 2 && p.group % (2 * p.nh) == 0) p.rp /= 2, p.nh *= 2;
+  p.pair_heads = p.group % (2 * p.nh) == 0 ? 1 : 0;
+  p.units = p.group / (p.pair_heads ? 2 * p.nh : p.nh);
+  const int rows = p.pair_heads ? p.rp : 2 * p.rp;
+  p.q_blocks = static_cast<int>((Sq + rows - 1) / rows);
+  const int64_t ctas = static_cast<int64_t>(p.q_blocks) * B * Hkv * p.units;
+  if (ctas > 0x7fffffffLL) return B200Q_ERR_INVALID;
+  CUtensorMap tq, tk, tv;
+  if (int rc = make_map(&tq, q, dtype, D, Sq, Hq, B, strides, p.rp, p.nh)) return rc;
+  // no keys: nothing is loaded, but the maps have to be valid
+  if (int rc = make_map(&tk, Sk > 0 ? k : q, dtype, D, Sk > 0 ? Sk : Sq, Sk > 0 ? Hkv : Hq, B, Sk > 0 ? strides + 3 : strides, kTileKeys, 1)) return rc;
+  if (int rc = make_map(&tv, Sk > 0 ? v : q, dtype, D, Sk > 0 ? Sk : Sq, Sk > 0 ? Hkv : Hq, B, Sk > 0 ? strides + 6 : strides, kTileKeys, 1)) return rc;
   const auto st = static_cast<cudaStream_t>(stream);
-  if (dtype == B200Q_BF16) window_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(p); else window_kernel<__half><<<grid, 128, 0, st>>>(p);
-  return check_launch();
+  const auto n = static_cast<unsigned>(ctas);
+  if (dtype == B200Q_BF16) return D <= 64 ? launch_window<__nv_bfloat16, 64>(tq, tk, tv, p, n, st) : launch_window<__nv_bfloat16, 128>(tq, tk, tv, p, n, st);
+  return D <= 64 ? launch_window<__half, 64>(tq, tk, tv, p, n, st) : launch_window<__half, 128>(tq, tk, tv, p, n, st);
 }
 
 }  // extern "C"
