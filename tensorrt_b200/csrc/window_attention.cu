@@ -25,14 +25,16 @@
 #include <cuda.h>
 
 #include "common.cuh"
+#include "ex2.cuh"
 #include "gemm_host.cuh"
 #include "tcgen05.cuh"
 
 namespace b200q {
 namespace {
 
-constexpr int kTileRows = 128, kTileKeys = 128, kThreads = 320, kTmemCols = 512;
+constexpr int kTileRows = 128, kTileKeys = 128, kThreads = 384, kTmemCols = 512;
 constexpr float kLazy = 8.0f;   // log2 of how far the reference may lie below the maximum
+constexpr int kPolyPairs = 4;   // of 16 pairs of exponentials: on the FMA pipe
 
 struct WindowParams {
   const char* q;
@@ -93,6 +95,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// true in one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// the n lowest bits, n of any size
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   uint32_t r;
@@ -119,11 +129,12 @@ struct Work {
   int head[2], q0[2], lowest[2], highest[2];  // per query tile: first head, first query, positions of its rows (highest < 0: none)
   int sink_tiles, first, tiles;             // key tiles 0 .. sink_tiles - 1, then first, first + 1, ..
   __device__ __forceinline__ int tile(int j) const { return j < sink_tiles ? j : first + j - sink_tiles; }
-  __device__ __forceinline__ bool needs(const WindowParams& p, int s, int t) const {
-    const int k0 = t * kTileKeys;
-    return k0 <= highest[s] && (p.window == 0 || k0 + kTileKeys - 1 > lowest[s] - p.window || k0 < p.sinks);
-  }
 };
+// Whether rows at positions lowest .. highest see a key of tile t.
+__device__ __forceinline__ bool needs(const WindowParams& p, int lowest, int highest, int t) {
+  const int k0 = t * kTileKeys;
+  return k0 <= highest && (p.window == 0 || k0 + kTileKeys - 1 > lowest - p.window || k0 < p.sinks);
+}
 
 __device__ __forceinline__ Work work_of(const WindowParams& p) {
   Work w;
@@ -160,7 +171,7 @@ template <int DPAD>
 struct Layout {
   static constexpr int kBoxes = DPAD / 64, kBoxBytes = 128 * 128, kTileBytes = kBoxes * kBoxBytes;
   static constexpr int kStages = DPAD == 128 ? 5 : 8;
-  static constexpr int kBars = 2 * kStages + 1 + 6 + 1;
+  static constexpr int kBars = 2 * kStages + 1 + 8 + 1;
   static constexpr int kSmem = 1024 + (2 + kStages) * kTileBytes + kBars * 8 + 16;
 };
 
@@ -208,7 +219,8 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   uint64_t* const q_full = empty + L::kStages;
   uint64_t* const s_full = q_full + 1;
   uint64_t* const p_full = s_full + 2;
-  uint64_t* const o_full = p_full + 2;
+  uint64_t* const p_half = p_full + 2;
+  uint64_t* const o_full = p_half + 2;
   uint64_t* const done = o_full + 2;
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -218,7 +230,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     ptx::tmem_relinquish<1>();
   } else if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * L::kStages + 1; ++i) ptx::mbar_init(bars + i, 1);
-    for (int s = 0; s < 2; ++s) ptx::mbar_init(s_full + s, 1), ptx::mbar_init(p_full + s, 4), ptx::mbar_init(o_full + s, 1);
+    for (int s = 0; s < 2; ++s) ptx::mbar_init(s_full + s, 1), ptx::mbar_init(p_full + s, 4), ptx::mbar_init(p_half + s, 4), ptx::mbar_init(o_full + s, 1);
     ptx::mbar_init(done, 1);
     ptx::fence_barrier_init();
   }
@@ -230,7 +242,9 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   pdl_wait();
   const Work w = work_of(p);
 
-  if (warp == 9) {
+  if (warp >= 8) {
+    ptx::setmaxnreg_dec<88>();                     // 128 x 88 + 256 x 208 = 384 x 168, what the CTA was launched with
+    if (warp == 9) {
     // ------------------------------------------------------------- loads
     if (lane == 0 && w.tiles > 0) {
       ptx::mbar_arrive_expect_tx(q_full, 2 * L::kTileBytes);
@@ -261,84 +275,99 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     }
   } else if (warp == 8) {
     // ------------------------------------------------------------- products
-    if (lane == 0 && w.tiles > 0) {
+    // The warp walks the loop together, so that barriers, phases and descriptors stay in uniform registers; one lane issues.
+    if (w.tiles > 0) {
       constexpr int kFormat = std::is_same<T, __half>::value ? 0 : 1;
       const uint32_t id_s = idesc_16(kFormat, 128, kTileKeys, 0), id_o = idesc_16(kFormat, 128, p.D, 1);
       const int steps = p.D / 16;
       // V as the second operand: rows of 64 elements of D, 8 keys to 1024 bytes, the next 64 elements a box further on
       constexpr uint32_t kHiV = (1024u >> 4) | (1u << 14) | (2u << 29);
       constexpr uint32_t kLeadV = (L::kBoxBytes >> 4) << 16;
+      const uint32_t ring_lo = (ptx::smem_u32(ring) >> 4) & 0x3fffu, q_lo = ptx::desc_lo_sw128(ptx::smem_u32(sq));
+      const bool leader = elect_one();
       bool ok = ptx::mbar_wait(q_full, 0);
       if (!ok) timed_out(p.status, 82);
       uint32_t p_phase[2] = {0, 0};
       bool waiting[2] = {false, false}, begun[2] = {false, false};   // a P that is to be multiplied; O holds something
-      int v_stage = 0;                                               // of the key tile before
+      int stage = 0, v_stage = 0;                                    // of this tile's K; of the V of the tile before
+      uint32_t phase = 0, v_phase = 0;
       for (int j = 0; j <= w.tiles && ok; ++j) {
-        const int k_load = 2 * j, k_stage = k_load % L::kStages;
         const bool more = j < w.tiles;
         const int t = more ? w.tile(j) : 0;
-        bool k_here = false, v_here = false;
-        for (int s = 0; s < 2 && ok; ++s) {
-          if (waiting[s]) {
-            if (!v_here) {
-              const int v_load = 2 * j - 1;
-              v_stage = v_load % L::kStages;
-              ok = ptx::mbar_wait(full + v_stage, (v_load / L::kStages) & 1);
-              v_here = true;
-            }
-            ok = ok && ptx::mbar_wait(p_full + s, p_phase[s]);
-            if (!ok) {
-              timed_out(p.status, 83);
-              break;
-            }
-            p_phase[s] ^= 1u;
-            ptx::tc_fence_after();
-            const uint32_t lo = ((ptx::smem_u32(ring + v_stage * L::kTileBytes) >> 4) & 0x3fffu) | kLeadV;
-#pragma unroll
-            for (int k = 0; k < kTileKeys / 16; ++k)
-              mma_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, ptx::desc_join(lo + k * (2048 >> 4), kHiV), id_o, begun[s] || k > 0);
-            begun[s] = true;
-            waiting[s] = false;
-          }
-          if (more && w.needs(p, s, t)) {
-            if (!k_here) {
-              ok = ptx::mbar_wait(full + k_stage, (k_load / L::kStages) & 1);
-              k_here = true;
-              if (!ok) {
-                timed_out(p.status, 84);
-                break;
-              }
-              ptx::tc_fence_after();
-            }
-            const uint32_t a = ptx::desc_lo_sw128(ptx::smem_u32(sq + s * L::kTileBytes)), b = ptx::desc_lo_sw128(ptx::smem_u32(ring + k_stage * L::kTileBytes));
-            for (int k = 0; k < steps; ++k) {
-              const uint32_t at = ((k >> 2) * L::kBoxBytes + (k & 3) * 32) >> 4;
-              mma_ss(tmem + s * 128, ptx::desc_join(a + at, ptx::kDescHiSw128), ptx::desc_join(b + at, ptx::kDescHiSw128), id_s, k > 0);
-            }
-            ptx::tc_commit<1>(s_full + s);
-            waiting[s] = true;
-          }
-        }
         // a stage is given back only once its copy has arrived, read or not
-        if (ok && more && !k_here) ok = ptx::mbar_wait(full + k_stage, (k_load / L::kStages) & 1);
-        if (ok && j > 0 && !v_here) ok = ptx::mbar_wait(full + (k_load - 1) % L::kStages, ((k_load - 1) / L::kStages) & 1);
+        if (more) ok = ptx::mbar_wait(full + stage, phase);
+        if (j > 0) ok = ok && ptx::mbar_wait(full + v_stage, v_phase);
         if (!ok) {
           timed_out(p.status, 84);
           break;
         }
-        if (j > 0) ptx::tc_commit<1>(empty + (2 * j - 1) % L::kStages);     // V of the tile before
-        if (more) ptx::tc_commit<1>(empty + k_stage);
+        ptx::tc_fence_after();
+        const uint32_t v_lo = (ring_lo + v_stage * (L::kTileBytes >> 4)) | kLeadV, k_lo = (ring_lo + stage * (L::kTileBytes >> 4)) | (1u << 16);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (waiting[s]) {
+            // the first half of the keys as soon as it is there
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              ok = ok && ptx::mbar_wait((half == 0 ? p_half : p_full) + s, p_phase[s]);
+              ptx::tc_fence_after();
+              if (leader) {
+#pragma unroll
+                for (int k = 0; k < kTileKeys / 32; ++k)
+                  mma_ts(tmem + 256 + s * 128, tmem + s * 128 + half * 32 + k * 8, ptx::desc_join(v_lo + (half * 4 + k) * (2048 >> 4), kHiV), id_o,
+                         half > 0 || k > 0 ? 1u : (begun[s] ? 1u : 0u));
+              }
+              __syncwarp();
+            }
+            p_phase[s] ^= 1u;
+            begun[s] = true;
+            waiting[s] = false;
+          }
+          if (more && needs(p, w.lowest[s], w.highest[s], t)) {
+            if (leader) {
+#pragma unroll
+              for (int k = 0; k < DPAD / 16; ++k) {
+                const uint32_t at = ((k >> 2) * L::kBoxBytes + (k & 3) * 32) >> 4;
+                if (k < steps)
+                  mma_ss(tmem + s * 128, ptx::desc_join(q_lo + s * (L::kTileBytes >> 4) + at, ptx::kDescHiSw128), ptx::desc_join(k_lo + at, ptx::kDescHiSw128), id_s,
+                         k > 0);
+              }
+              ptx::tc_commit<1>(s_full + s);
+            }
+            __syncwarp();
+            waiting[s] = true;
+          }
+        }
+        if (!ok) {
+          timed_out(p.status, 83);
+          break;
+        }
+        if (leader) {
+          if (j > 0) ptx::tc_commit<1>(empty + v_stage);
+          if (more) ptx::tc_commit<1>(empty + stage);
+        }
+        __syncwarp();
+        v_stage = stage + 1, v_phase = phase;
+        if (v_stage == L::kStages) v_stage = 0, v_phase ^= 1u;
+        stage = v_stage + 1, phase = v_phase;
+        if (stage == L::kStages) stage = 0, phase ^= 1u;
       }
-      for (int s = 0; s < 2; ++s) ptx::tc_commit<1>(o_full + s);
-      ptx::tc_commit<1>(done);
+      if (leader) {
+        for (int s = 0; s < 2; ++s) ptx::tc_commit<1>(o_full + s);
+        ptx::tc_commit<1>(done);
+      }
+      __syncwarp();
       if (!ptx::mbar_wait(done, 0)) timed_out(p.status, 85);
+    }
     }
   } else {
     // ------------------------------------------------------------- softmax of query tile s, one thread to a row
+    ptx::setmaxnreg_inc<208>();
     const int s = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;     // this warp's 32 lanes of tensor memory
     const uint32_t ts = tmem + s * 128 + lanes, to = tmem + 256 + s * 128 + lanes;
-    const int h = w.head[s] + r / p.rp, i = w.q0[s] + r % p.rp;
+    const int q0 = s ? w.q0[1] : w.q0[0], lowest = s ? w.lowest[1] : w.lowest[0], highest = s ? w.highest[1] : w.highest[0];
+    const int h = (s ? w.head[1] : w.head[0]) + r / p.rp, i = q0 + r % p.rp;
     const int at = i < w.nq ? i + w.off : -1;                         // position; < 0: sees nothing
     const float sl = fmaxf(p.scale * 1.4426950408889634f, 1e-30f);    // 0 times a masked -inf would be NaN
     const uint64_t sl2 = pack2(sl, sl);
@@ -347,7 +376,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     uint32_t phase = 0;
     for (int j = 0; j < w.tiles && ok; ++j) {
       const int t = w.tile(j), k0 = t * kTileKeys;
-      if (!w.needs(p, s, t)) continue;
+      if (!needs(p, lowest, highest, t)) continue;
       ok = ptx::mbar_wait(s_full + s, phase);
       if (!ok) {
         timed_out(p.status, 86);
@@ -359,13 +388,16 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
 #pragma unroll
       for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32(ts + c * 32, x + c * 32);
       ptx::tmem_ld_wait();
-      const bool inside = k0 + kTileKeys - 1 <= w.lowest[s] && w.q0[s] + p.rp <= w.nq && w.q0[s] + w.off >= 0 &&
-                          (p.window == 0 || k0 > w.highest[s] - p.window || k0 + kTileKeys <= p.sinks);
+      // no row of this tile that sees anything is at an edge; the others are not written
+      const bool inside = k0 + kTileKeys - 1 <= lowest && (p.window == 0 || k0 > highest - p.window || k0 + kTileKeys <= p.sinks);
       if (!inside) {
-        const int last = at - k0, first = p.window > 0 ? last - p.window : -1, sinks = p.sinks - k0;
+        const int last = at - k0, first = p.window > 0 ? last - p.window : -1, sinks = p.sinks - k0;   // seen: c <= last with c > first or c < sinks
 #pragma unroll
-        for (int c = 0; c < kTileKeys; ++c)
-          if (c > last || (c <= first && c >= sinks)) x[c] = 0xff800000u;
+        for (int c = 0; c < kTileKeys; c += 32) {
+          const uint32_t seen = low_bits(last + 1 - c) & (~low_bits(first + 1 - c) | low_bits(sinks - c));
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[c + e] = seen & (1u << e) ? x[c + e] : 0xff800000u;
+        }
       }
       float top[4];
 #pragma unroll
@@ -401,16 +433,26 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       for (int c = 0; c < kTileKeys; c += 32) {
         uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float2 a = unpack2(fma2(pack2(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 1])), sl2, back2));
-          const float2 b = unpack2(fma2(pack2(__uint_as_float(x[c + e + 2]), __uint_as_float(x[c + e + 3])), sl2, back2));
-          const float e0 = exp2_fast(a.x), e1 = exp2_fast(a.y), e2 = exp2_fast(b.x), e3 = exp2_fast(b.y);
-          sum0 = add2(sum0, pack2(e0, e1));
-          sum1 = add2(sum1, pack2(e2, e3));
-          pk[e / 2] = pack16<T>(e0, e1);
-          pk[e / 2 + 1] = pack16<T>(e2, e3);
+        for (int e = 0; e < 16; ++e) {
+          const uint64_t y = fma2(pack2(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])), sl2, back2);
+          uint64_t v;
+          if ((e + 1) * kPolyPairs / 16 != e * kPolyPairs / 16) {
+            v = ex2_poly2(y);
+          } else {
+            const float2 a = unpack2(y);
+            v = pack2(exp2_fast(a.x), exp2_fast(a.y));
+          }
+          if (e & 1) sum1 = add2(sum1, v); else sum0 = add2(sum0, v);
+          const float2 a = unpack2(v);
+          pk[e] = pack16<T>(a.x, a.y);
         }
         ptx::tmem_st_32x32_x16(ts + c / 2, pk);
+        if (c == 32) {
+          ptx::tmem_st_wait();
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(p_half + s);
+        }
       }
       const float2 s0 = unpack2(sum0), s1 = unpack2(sum1);
       l += (s0.x + s0.y) + (s1.x + s1.y);
