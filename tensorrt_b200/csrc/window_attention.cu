@@ -34,7 +34,7 @@ namespace {
 
 constexpr int kTileRows = 128, kTileKeys = 128, kThreads = 384, kTmemCols = 512;
 constexpr float kLazy = 8.0f;   // log2 of how far the reference may lie below the maximum
-constexpr int kPolyPairs = 4;   // of 16 pairs of exponentials: on the FMA pipe
+constexpr int kPolyPairs = 2;   // of 16 pairs of exponentials: on the FMA pipe
 
 struct WindowParams {
   const char* q;
@@ -233,6 +233,9 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     for (int s = 0; s < 2; ++s) ptx::mbar_init(s_full + s, 1), ptx::mbar_init(p_full + s, 4), ptx::mbar_init(p_half + s, 4), ptx::mbar_init(o_full + s, 1);
     ptx::mbar_init(done, 1);
     ptx::fence_barrier_init();
+    ptx::prefetch_tmap(&tq);
+    ptx::prefetch_tmap(&tk);
+    ptx::prefetch_tmap(&tv);
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -243,7 +246,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   const Work w = work_of(p);
 
   if (warp >= 8) {
-    ptx::setmaxnreg_dec<88>();                     // 128 x 88 + 256 x 208 = 384 x 168, what the CTA was launched with
+    ptx::setmaxnreg_dec<120>();                    // 128 x 120 + 256 x 192 = 384 x 168, what the CTA was launched with
     if (warp == 9) {
     // ------------------------------------------------------------- loads
     if (lane == 0 && w.tiles > 0) {
@@ -362,7 +365,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     }
   } else {
     // ------------------------------------------------------------- softmax of query tile s, one thread to a row
-    ptx::setmaxnreg_inc<208>();
+    ptx::setmaxnreg_inc<192>();
     const int s = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;     // this warp's 32 lanes of tensor memory
     const uint32_t ts = tmem + s * 128 + lanes, to = tmem + 256 + s * 128 + lanes;
