@@ -1,5 +1,6 @@
 // Rows in and out of the paged key-value cache: append and evict.
 #include "paged.cuh"
+#include "tcgen05.cuh"
 
 namespace b200q {
 namespace {
@@ -85,72 +86,187 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One CTA per sequence and kv head.  The smallest kept key is found bit by bit; then one pass in the order of the tokens.
-__global__ void __launch_bounds__(256) evict_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ int counts[8];
-  const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// Which tokens stay.  A cluster of CTAs per sequence and kv head, each with a part of the tokens.  The `want`-th largest key is found
+// eight bits at a time, from the top: every CTA counts the digits of its keys that agree with the bits found so far, the
+// counts of the cluster are added through shared memory, and all CTAs step to the same digit.  The counts also say how many tokens each
+// CTA keeps in front of the next, so that one more walk in the order of the tokens writes the list.  Bound by latency: five walks
+// over the part (from L2 after the first) and one cluster barrier a digit.
+constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kMaxCluster = 8;
+
+__device__ __forceinline__ int ld_cluster_i32(const int* p, unsigned cta) {
+  int v;
+  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(ptx::mapa_u32(ptx::smem_u32(p), cta)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ld_f32(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+
+__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
+  __shared__ int counts[4][256];
+  __shared__ int found[2];                      // digit, how many of its keys are wanted
+  __shared__ int published[2];                  // of this CTA's part: tokens kept for sure, candidates equal to the smallest kept key
+  __shared__ int warp_sum[2][kSelectWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = static_cast<int>(ptx::cluster_ctarank()), ctas = static_cast<int>(cluster_size());
+  const int b = blockIdx.y, h = blockIdx.x / ctas;
+  for (int i = tid; i < 4 * 256; i += kSelectThreads) counts[0][i] = 0;
+  pdl_launch_dependents();
+  pdl_wait();
   const int n = paged::cached_tokens(p.c, b, p.L), m = min(n, p.keep);
-  const int64_t line = (static_cast<int64_t>(b) * p.c.heads + h);
+  const int64_t line = static_cast<int64_t>(b) * p.c.heads + h;
   const float* w = p.weights + line * p.L;
   float* nw = p.new_weights + line * p.L;
   int32_t* kept = p.kept + line * p.keep;
-  if (h == 0 && tid == 0) p.new_lens[b] = m;
+  if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = m;
+  for (int64_t j = m + rank * kSelectThreads + tid; j < p.keep; j += ctas * kSelectThreads) kept[j] = -1;
+  for (int64_t j = m + rank * kSelectThreads + tid; j < p.L; j += ctas * kSelectThreads) nw[j] = 0.0f;
+  if (m == n) {                                 // the same for the whole cluster
+    for (int t = rank * kSelectThreads + tid; t < n; t += ctas * kSelectThreads) kept[t] = t, nw[t] = ld_f32(w + t);
+    return;
+  }
   const int lo = min(p.sinks, n), hi = max(lo, n - p.recent);       // candidates: [lo, hi)
   const int want = m - lo - (n - hi);                               // of them stay
-  auto total = [&](int v) {
-    v = __reduce_add_sync(0xffffffffu, v);
-    if (lane == 0) counts[warp] = v;
-    __syncthreads();
-    int s = 0;
-    for (int i = 0; i < 8; ++i) s += counts[i];
-    __syncthreads();
-    return s;
-  };
-  uint32_t least = 0;                                               // the largest key that `want` candidates reach
-  for (int bit = 31; bit >= 0 && want > 0; --bit) {
-    const uint32_t probe = least | (1u << bit);
-    int v = 0;
-    for (int t = lo + tid; t < hi; t += 256) v += weight_key(w[t]) >= probe;
-    if (total(v) >= want) least = probe;
-  }
-  int above = 0;
-  for (int t = lo + tid; t < hi; t += 256) above += weight_key(w[t]) > least;
-  const int equal = want - total(above);                            // of the candidates equal to it: the first ones
-  __shared__ int warp_kept[8], warp_equal[8];
-  int done = 0, done_equal = 0;
-  for (int t0 = 0; t0 < n; t0 += 256) {
-    const int t = t0 + tid;
-    const bool fixed = t < n && (t < lo || t >= hi), inside = t < n && !fixed;
-    const uint32_t key = inside ? weight_key(w[t]) : 0;
-    const unsigned eq = __ballot_sync(0xffffffffu, inside && want > 0 && key == least);
-    if (lane == 0) warp_equal[warp] = __popc(eq);
-    __syncthreads();
-    int rank = done_equal + __popc(eq & ((1u << lane) - 1));
-    for (int i = 0; i < warp; ++i) rank += warp_equal[i];
-    const bool stay = fixed || (inside && want > 0 && (key > least || (key == least && rank < equal)));
-    const unsigned st = __ballot_sync(0xffffffffu, stay);
-    if (lane == 0) warp_kept[warp] = __popc(st);
-    __syncthreads();
-    int at = done + __popc(st & ((1u << lane) - 1));
-    for (int i = 0; i < warp; ++i) at += warp_kept[i];
-    if (stay) kept[at] = t, nw[at] = w[t];
-    for (int i = 0; i < 8; ++i) done += warp_kept[i], done_equal += warp_equal[i];
-    __syncthreads();
-  }
-  for (int j = m + tid; j < p.keep; j += 256) kept[j] = -1;
-  for (int64_t j = m + tid; j < p.L; j += 256) nw[j] = 0.0f;
+  const int part = (n + ctas - 1) / ctas, t0 = min(rank * part, n), t1 = min(t0 + part, n);
+  const int c0 = max(t0, lo), c1 = min(t1, hi);                     // candidates of this part
   __syncthreads();
-  const int pieces = p.row_bytes / 16;
+  uint32_t least = 0;
+  int left = want, above = 0;                   // wanted among the keys that agree so far; this part's keys above them
+  if (want > 0) {
+#pragma unroll 1
+    for (int d = 0; d < 4; ++d) {
+      const int shift = 24 - 8 * d;
+      for (int t = c0 + tid; t < c1; t += 4 * kSelectThreads) {
+        float v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = t + u * kSelectThreads < c1 ? ld_f32(w + t + u * kSelectThreads) : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t key = weight_key(v[u]);
+          if (t + u * kSelectThreads < c1 && (d == 0 || (key ^ least) >> (shift + 8) == 0)) atomicAdd(&counts[d][(key >> shift) & 255], 1);
+        }
+      }
+      ptx::cluster_sync();
+      if (warp == 0) {                          // eight digits a lane, the largest in lane 0
+        int sum[8], all = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          sum[e] = 0;
+          for (int r = 0; r < ctas; ++r) sum[e] += ld_cluster_i32(&counts[d][255 - lane * 8 - e], r);
+          all += sum[e];
+        }
+        int before = all;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += v;
+        }
+        before -= all;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (before < left && left <= before + sum[e]) found[0] = 255 - lane * 8 - e, found[1] = left - before;
+          before += sum[e];
+        }
+      }
+      __syncthreads();
+      const int digit = found[0];
+      left = found[1];
+      least |= static_cast<uint32_t>(digit) << shift;
+      for (int e = digit + 1 + lane; e < 256; e += 32) above += warp == 0 ? counts[d][e] : 0;
+      __syncthreads();
+    }
+  }
+  if (warp == 0) {
+    above = __reduce_add_sync(0xffffffffu, above);
+    if (lane == 0) published[0] = above + max(0, min(t1, lo) - t0) + max(0, t1 - max(t0, hi)), published[1] = want > 0 ? counts[3][least & 255] : 0;
+  }
+  ptx::cluster_sync();
+  int sure = 0, equal = 0;                      // in the parts in front
+  for (int r = 0; r < rank; ++r) sure += ld_cluster_i32(&published[0], r), equal += ld_cluster_i32(&published[1], r);
+  // each warp a run of this part; 32 tokens at a time
+  const int run = ((t1 - t0 + kSelectWarps - 1) / kSelectWarps + 31) & ~31, r0 = min(t0 + warp * run, t1), r1 = min(r0 + run, t1);
+  auto look = [&](int t, bool* is_sure, bool* is_equal, float* v) {
+    *is_sure = *is_equal = false, *v = 0.0f;
+    if (t >= r1) return;
+    *v = ld_f32(w + t);
+    const bool candidate = t >= lo && t < hi;
+    const uint32_t key = weight_key(*v);
+    *is_sure = !candidate || (want > 0 && key > least);
+    *is_equal = candidate && want > 0 && key == least;
+  };
+  int my_sure = 0, my_equal = 0;
+  for (int t = r0 + lane; t - lane < r1; t += 32) {
+    bool a, e;
+    float v;
+    look(t, &a, &e, &v);
+    my_sure += __popc(__ballot_sync(0xffffffffu, a)), my_equal += __popc(__ballot_sync(0xffffffffu, e));
+  }
+  if (lane == 0) warp_sum[0][warp] = my_sure, warp_sum[1][warp] = my_equal;
+  __syncthreads();
+  for (int i = 0; i < warp; ++i) sure += warp_sum[0][i], equal += warp_sum[1][i];
+  for (int t = r0 + lane; t - lane < r1; t += 32) {
+    bool a, e;
+    float v;
+    look(t, &a, &e, &v);
+    const unsigned as = __ballot_sync(0xffffffffu, a), es = __ballot_sync(0xffffffffu, e), below = (1u << lane) - 1;
+    const int eq = equal + __popc(es & below);  // equal keys in front; the first `left` stay
+    if (a || (e && eq < left)) {
+      const int at = sure + __popc(as & below) + min(eq, left);
+      kept[at] = t, nw[at] = v;
+    }
+    sure += __popc(as), equal += __popc(es);
+  }
+  ptx::cluster_sync();                          // nobody leaves while its counts may still be read
+}
+
+// The kept rows to their new pages: 16 bytes of K and of V a thread and row, several rows at once.  Bound by the memory.
+constexpr int kMoveThreads = 256, kMoveRows = 4;
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int m = min(paged::cached_tokens(p.c, b, p.L), p.keep);
+  const int pieces = p.row_bytes / 16, per = kMoveThreads / pieces;       // rows that the CTA takes at once
+  const int r = static_cast<int>(threadIdx.x) / pieces, piece = (static_cast<int>(threadIdx.x) % pieces) * 16;
+  const int32_t* kept = p.kept + (static_cast<int64_t>(b) * p.c.heads + h) * p.keep;
   const int32_t* from = p.c.table + b * p.c.table_stride;
   const int32_t* to = p.out_table + b * p.out_stride;
-  for (int64_t i = tid; i < static_cast<int64_t>(m) * pieces; i += 256) {
-    const int j = static_cast<int>(i / pieces), piece = static_cast<int>(i % pieces) * 16, t = kept[j];
-    const int sp = paged::page_of(from, t, p.c), dp = paged::page_of(to, j, p.c);
-    if (sp < 0 || dp < 0) continue;
-    const int sr = t % p.c.page_size, dr = j % p.c.page_size;
-    *reinterpret_cast<uint4*>(paged::row_at(p.c.k, dp, h, dr) + piece) = *reinterpret_cast<const uint4*>(paged::row_at(p.c.k, sp, h, sr) + piece);
-    *reinterpret_cast<uint4*>(paged::row_at(p.c.v, dp, h, dr) + piece) = *reinterpret_cast<const uint4*>(paged::row_at(p.c.v, sp, h, sr) + piece);
+  if (r >= per) return;
+  const int first = static_cast<int>(blockIdx.x) * per * kMoveRows + r;
+  uint4 kv[kMoveRows], vv[kMoveRows];
+  int token[kMoveRows], sp[kMoveRows], dp[kMoveRows];
+#pragma unroll
+  for (int u = 0; u < kMoveRows; ++u) {
+    const int j = first + u * per;
+    token[u] = j < m ? ld_i32(kept + j) : -1;
   }
+#pragma unroll
+  for (int u = 0; u < kMoveRows; ++u) {
+    sp[u] = token[u] >= 0 ? paged::page_of(from, token[u], p.c) : -1;
+    dp[u] = token[u] >= 0 ? paged::page_of(to, first + u * per, p.c) : -1;
+    if (dp[u] < 0) sp[u] = -1;
+  }
+#pragma unroll
+  for (int u = 0; u < kMoveRows; ++u)
+    if (sp[u] >= 0) {
+      const int row = token[u] % p.c.page_size;
+      kv[u] = ld_128(paged::row_at(p.c.k, sp[u], h, row) + piece);
+      vv[u] = ld_128(paged::row_at(p.c.v, sp[u], h, row) + piece);
+    }
+#pragma unroll
+  for (int u = 0; u < kMoveRows; ++u)
+    if (sp[u] >= 0) {
+      const int row = (first + u * per) % p.c.page_size;
+      *reinterpret_cast<uint4*>(paged::row_at(p.c.k, dp[u], h, row) + piece) = kv[u];
+      *reinterpret_cast<uint4*>(paged::row_at(p.c.v, dp[u], h, row) + piece) = vv[u];
+    }
 }
 
 }  // namespace
@@ -211,7 +327,29 @@ int b200q_paged_evict(const b200q_paged_cache* cache, const int32_t* block_table
   p.new_lens = new_lens;
   p.new_weights = new_weights;
   p.row_bytes = p.c.D * (p.c.codes ? 1 : 2);
-  evict_kernel<<<dim3(p.c.heads, static_cast<unsigned>(B)), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  const auto st = static_cast<cudaStream_t>(stream);
+  // a row of tokens over as many CTAs as the GPU has room for, but not less than 2048 tokens to each
+  const int64_t rows = B * p.c.heads;
+  int ctas = 1;
+  while (ctas < kMaxCluster && rows * ctas * 2 <= 2 * sm_count() && weights_len >= 2048 * ctas * 2) ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.c.heads * ctas), static_cast<unsigned>(B));
+  cfg.blockDim = dim3(kSelectThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(ctas), attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, evict_select_kernel, p) != cudaSuccess) return B200Q_ERR_CUDA;
+  if (int rc = check_launch()) return rc;
+  if (keep == 0 || table_width == 0) return B200Q_OK;
+  const int64_t per = kMoveThreads / (p.row_bytes / 16) * kMoveRows, blocks = (keep + per - 1) / per;
+  if (blocks > 0x7fffffffLL) return B200Q_ERR_INVALID;
+  if (launch_pdl(evict_move_kernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(p.c.heads), static_cast<unsigned>(B)), dim3(kMoveThreads), 0, st, p) != cudaSuccess)
+    return B200Q_ERR_CUDA;
   return check_launch();
 }
 
