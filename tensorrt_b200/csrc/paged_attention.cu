@@ -152,9 +152,11 @@ struct Stage {
 __device__ __forceinline__ int64_t piece(int64_t tiles, int c, int ctas) { return tiles * c / ctas; }
 
 // Adds up the tiles of all sequences and finds the one that holds tile `piece(total, cta)`; all threads take part.
-__device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, int ctas, int* b_out, int64_t* before_out) {
+__device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, int ctas, int* b_out, int64_t* before_out, Seen* seen_out) {
   __shared__ int64_t sums[kWarps];
   __shared__ int64_t found[2];
+  __shared__ Seen found_keys;
+  Seen keys{0, 0, 0};
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t per = static_cast<int64_t>(p.c.heads) * p.blocks;
   int64_t total = 0, inclusive = 0, mine = 0;
@@ -178,19 +180,22 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
     return all;
   };
   for (int base = 0; base < p.B; base += kThreads) {
-    mine = base + tid < p.B ? keys_seen(p, base + tid).tiles() * per : 0;
+    if (base + tid < p.B) keys = keys_seen(p, base + tid);
+    mine = base + tid < p.B ? keys.tiles() * per : 0;
     total += scan(mine);
   }
   const int64_t want = piece(total, cta, ctas);
   if (p.B <= kThreads) {
-    if (want >= inclusive - mine && want < inclusive) found[0] = tid, found[1] = inclusive - mine;
+    if (want >= inclusive - mine && want < inclusive) found[0] = tid, found[1] = inclusive - mine, found_keys = keys;
     __syncthreads();
   } else {
     int64_t before = 0;
     for (int base = 0; base < p.B; base += kThreads) {
-      mine = base + tid < p.B ? keys_seen(p, base + tid).tiles() * per : 0;
+      if (base + tid < p.B) keys = keys_seen(p, base + tid);
+      mine = base + tid < p.B ? keys.tiles() * per : 0;
       const int64_t all = scan(mine);
-      if (want >= before + inclusive - mine && want < before + inclusive) found[0] = base + tid, found[1] = before + inclusive - mine;
+      if (want >= before + inclusive - mine && want < before + inclusive)
+        found[0] = base + tid, found[1] = before + inclusive - mine, found_keys = keys;
       before += all;
       if (before > want) break;
     }
@@ -198,6 +203,7 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
   }
   *b_out = static_cast<int>(found[0]);
   *before_out = found[1];
+  *seen_out = found_keys;
   return total;
 }
 
@@ -219,17 +225,17 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
 
   int b;
   int64_t before;
-  const int64_t total = find_start(p, cta, ctas, &b, &before);
+  Seen see;
+  const int64_t total = find_start(p, cta, ctas, &b, &before, &see);
   int64_t at = piece(total, cta, ctas);
   const int64_t first_tile = at, end = piece(total, cta + 1, ctas);
   while (at < end) {
     // ------------------------------------------------------------- the item
-    Seen see = keys_seen(p, b);
     const int tiles = see.tiles();
     const int64_t item = (at - before) / tiles;       // kv head and block of query heads, within the sequence
     if (item >= static_cast<int64_t>(p.c.heads) * p.blocks) {
       before += static_cast<int64_t>(tiles) * p.c.heads * p.blocks;
-      ++b;
+      see = keys_seen(p, ++b);
       continue;
     }
     const int h = static_cast<int>(item / p.blocks), block = static_cast<int>(item % p.blocks);
@@ -274,18 +280,10 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
       copy_commit();
       return __ballot_sync(0xffffffffu, page >= 0 && lane < 16);
     };
-    uint32_t there[S::kDepth];                         // which of the 16 keys of a stage exist
-    int2 ahead = find_page(tile0);
-#pragma unroll
-    for (int s = 0; s < S::kDepth - 1; ++s) {
-      const int2 now = ahead;
-      ahead = find_page(tile0 + s + 1);
-      there[s] = issue(s, now);
-    }
-
     // ------------------------------------------------------------- queries: head g of each block, the elements that this lane's K chunks meet
     uint32_t q[BLOCKS8][kSteps][2];
     float unit[BLOCKS8];
+    int2 ahead = find_page(tile0);
     {
       const char* base = p.q + b * p.q_batch + head0 * p.q_head;
 #pragma unroll
@@ -300,6 +298,20 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
           if (row < rows && e < p.c.D) u = ld_128(src + e * 2);
           w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
         }
+      }
+    }
+    uint32_t there[S::kDepth];                         // which of the 16 keys of a stage exist
+#pragma unroll
+    for (int s = 0; s < S::kDepth - 1; ++s) {
+      const int2 now = ahead;
+      ahead = find_page(tile0 + s + 1);
+      there[s] = issue(s, now);
+    }
+
+    {
+#pragma unroll
+      for (int r = 0; r < BLOCKS8; ++r) {
+        uint32_t* w = &q[r][0][0];
         unit[r] = 1.0f;
         if constexpr (CODES && !std::is_same<T, __half>::value) {
           float top = 0.0f;

@@ -86,11 +86,13 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Which tokens stay.  A cluster of CTAs per sequence and kv head, each with a part of the tokens.  The `want`-th largest key is found
-// eight bits at a time, from the top: every CTA counts the digits of its keys that agree with the bits found so far, the
-// counts of the cluster are added through shared memory, and all CTAs step to the same digit.  The counts also say how many tokens each
-// CTA keeps in front of the next, so that one more walk in the order of the tokens writes the list.  Bound by latency: five walks
-// over the part (from L2 after the first) and one cluster barrier a digit.
+// Which tokens stay.  A cluster of CTAs per sequence and kv head, each with a part of the tokens, their keys in shared memory (up to
+// kHeldKeys, else read again on each walk).  The `want`-th largest key is found eight bits at a time, from the top: every CTA counts
+// the digits of its keys that agree with the bits found so far, the counts of the cluster are added through shared memory, and all
+// CTAs step to the same digit.  A lane counts in a column of its own: attention weights share a few exponents, and 32 lanes adding
+// to the same few words wait for one another.  The counts also say how many tokens a CTA keeps in front of the next, so that two
+// more walks in the order of the tokens, a run of them to each warp, write the list.  Bound by latency, and since all of it runs a few
+// times only, by the size of the code as well: loops are unrolled no further than their loads need.
 constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kMaxCluster = 8;
 
 __device__ __forceinline__ int ld_cluster_i32(const int* p, unsigned cta) {
@@ -109,15 +111,20 @@ __device__ __forceinline__ unsigned cluster_size() {
   return r;
 }
 
+constexpr int kHeldKeys = 12288;
+template <bool HELD>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ int counts[4][256];
-  __shared__ int found[2];                      // digit, how many of its keys are wanted
-  __shared__ int published[2];                  // of this CTA's part: tokens kept for sure, candidates equal to the smallest kept key
+  extern __shared__ uint32_t keys[];                // HELD: those of the part
+  __shared__ __align__(16) int columns[256 * 32];   // [digit][lane]
+  __shared__ int counts[4][256];                    // of this CTA
+  __shared__ int scan_sums[8][2];
+  __shared__ int found[3];                          // digit; how many of its keys are wanted; this CTA's keys above it
+  __shared__ int published[2];                      // of this CTA's part: tokens kept for sure, candidates equal to the smallest kept key
   __shared__ int warp_sum[2][kSelectWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(ptx::cluster_ctarank()), ctas = static_cast<int>(cluster_size());
   const int b = blockIdx.y, h = blockIdx.x / ctas;
-  for (int i = tid; i < 4 * 256; i += kSelectThreads) counts[0][i] = 0;
+  for (int i = tid; i < 256 * 32 / 4; i += kSelectThreads) reinterpret_cast<int4*>(columns)[i] = make_int4(0, 0, 0, 0);
   pdl_launch_dependents();
   pdl_wait();
   const int n = paged::cached_tokens(p.c, b, p.L), m = min(n, p.keep);
@@ -126,16 +133,21 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   float* nw = p.new_weights + line * p.L;
   int32_t* kept = p.kept + line * p.keep;
   if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = m;
+  const int part = (n + ctas - 1) / ctas, t0 = min(rank * part, n), size = min(t0 + part, n) - t0;
+  if (m == n) {                                     // the same for the whole cluster
+#pragma unroll 4
+    for (int i = tid; i < size; i += kSelectThreads) kept[t0 + i] = t0 + i, nw[t0 + i] = ld_f32(w + t0 + i);
+  } else if (HELD) {
+#pragma unroll 4
+    for (int i = tid; i < size; i += kSelectThreads) keys[i] = weight_key(ld_f32(w + t0 + i));
+  }
+  auto key_of = [&](int i) { return HELD ? keys[i] : weight_key(ld_f32(w + t0 + i)); };
   for (int64_t j = m + rank * kSelectThreads + tid; j < p.keep; j += ctas * kSelectThreads) kept[j] = -1;
   for (int64_t j = m + rank * kSelectThreads + tid; j < p.L; j += ctas * kSelectThreads) nw[j] = 0.0f;
-  if (m == n) {                                 // the same for the whole cluster
-    for (int t = rank * kSelectThreads + tid; t < n; t += ctas * kSelectThreads) kept[t] = t, nw[t] = ld_f32(w + t);
-    return;
-  }
+  if (m == n) return;
   const int lo = min(p.sinks, n), hi = max(lo, n - p.recent);       // candidates: [lo, hi)
   const int want = m - lo - (n - hi);                               // of them stay
-  const int part = (n + ctas - 1) / ctas, t0 = min(rank * part, n), t1 = min(t0 + part, n);
-  const int c0 = max(t0, lo), c1 = min(t1, hi);                     // candidates of this part
+  const int c0 = max(lo - t0, 0), c1 = min(hi - t0, size);          // candidates of this part
   __syncthreads();
   uint32_t least = 0;
   int left = want, above = 0;                   // wanted among the keys that agree so far; this part's keys above them
@@ -143,87 +155,94 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
 #pragma unroll 1
     for (int d = 0; d < 4; ++d) {
       const int shift = 24 - 8 * d;
-      for (int t = c0 + tid; t < c1; t += 4 * kSelectThreads) {
-        float v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = t + u * kSelectThreads < c1 ? ld_f32(w + t + u * kSelectThreads) : 0.0f;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const uint32_t key = weight_key(v[u]);
-          if (t + u * kSelectThreads < c1 && (d == 0 || (key ^ least) >> (shift + 8) == 0)) atomicAdd(&counts[d][(key >> shift) & 255], 1);
-        }
+#pragma unroll 4
+      for (int i = c0 + tid; i < c1; i += kSelectThreads) {
+        const uint32_t key = key_of(i);
+        if (static_cast<uint64_t>(key ^ least) >> (shift + 8) == 0) atomicAdd(&columns[((key >> shift) & 255) * 32 + lane], 1);
       }
-      ptx::cluster_sync();
-      if (warp == 0) {                          // eight digits a lane, the largest in lane 0
-        int sum[8], all = 0;
+      __syncthreads();
+      {                                         // two threads to a digit, 16 columns each, turned so that no two meet a bank; cleared for the next
+        int4* mine = reinterpret_cast<int4*>(columns) + (tid >> 1) * 8 + (tid & 1) * 4;
+        int sum = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sum[e] = 0;
-          for (int r = 0; r < ctas; ++r) sum[e] += ld_cluster_i32(&counts[d][255 - lane * 8 - e], r);
-          all += sum[e];
+        for (int i = 0; i < 4; ++i) {
+          int4* at = mine + ((i + (tid >> 1)) & 3);
+          const int4 v = *at;
+          *at = make_int4(0, 0, 0, 0);
+          sum += v.x + v.y + v.z + v.w;
         }
-        int before = all;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        if ((tid & 1) == 0) counts[d][tid >> 1] = sum;
+      }
+      if (ctas > 1) ptx::cluster_sync(); else __syncthreads();
+      int own = 0, all = 0, own_up = 0, all_up = 0;   // digit 255 - tid: its keys, here and in the cluster; with those above it
+      if (tid < 256) {
+        own = all = counts[d][255 - tid];
+        if (ctas > 1) {
+          int v[kMaxCluster];
+#pragma unroll
+          for (int r = 0; r < kMaxCluster; ++r) v[r] = r < ctas ? ld_cluster_i32(&counts[d][255 - tid], r) : 0;
+          all = 0;
+#pragma unroll
+          for (int r = 0; r < kMaxCluster; ++r) all += v[r];
+        }
+        own_up = own, all_up = all;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, before, o);
-          if (lane >= o) before += v;
+          const int x = __shfl_up_sync(0xffffffffu, own_up, o), y = __shfl_up_sync(0xffffffffu, all_up, o);
+          if (lane >= o) own_up += x, all_up += y;
         }
-        before -= all;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (before < left && left <= before + sum[e]) found[0] = 255 - lane * 8 - e, found[1] = left - before;
-          before += sum[e];
-        }
+        if (lane == 31) scan_sums[warp][0] = own_up, scan_sums[warp][1] = all_up;
       }
       __syncthreads();
-      const int digit = found[0];
-      left = found[1];
-      least |= static_cast<uint32_t>(digit) << shift;
-      for (int e = digit + 1 + lane; e < 256; e += 32) above += warp == 0 ? counts[d][e] : 0;
+      if (tid < 256) {
+        for (int i = 0; i < warp; ++i) own_up += scan_sums[i][0], all_up += scan_sums[i][1];
+        if (all_up - all < left && left <= all_up) found[0] = 255 - tid, found[1] = left - (all_up - all), found[2] = own_up - own;
+      }
       __syncthreads();
+      left = found[1];
+      above += found[2];
+      least |= static_cast<uint32_t>(found[0]) << shift;
     }
   }
-  if (warp == 0) {
-    above = __reduce_add_sync(0xffffffffu, above);
-    if (lane == 0) published[0] = above + max(0, min(t1, lo) - t0) + max(0, t1 - max(t0, hi)), published[1] = want > 0 ? counts[3][least & 255] : 0;
-  }
-  ptx::cluster_sync();
-  int sure = 0, equal = 0;                      // in the parts in front
-  for (int r = 0; r < rank; ++r) sure += ld_cluster_i32(&published[0], r), equal += ld_cluster_i32(&published[1], r);
-  // each warp a run of this part; 32 tokens at a time
-  const int run = ((t1 - t0 + kSelectWarps - 1) / kSelectWarps + 31) & ~31, r0 = min(t0 + warp * run, t1), r1 = min(r0 + run, t1);
-  auto look = [&](int t, bool* is_sure, bool* is_equal, float* v) {
-    *is_sure = *is_equal = false, *v = 0.0f;
-    if (t >= r1) return;
-    *v = ld_f32(w + t);
-    const bool candidate = t >= lo && t < hi;
-    const uint32_t key = weight_key(*v);
-    *is_sure = !candidate || (want > 0 && key > least);
-    *is_equal = candidate && want > 0 && key == least;
+  if (tid == 0) published[0] = above + min(max(lo - t0, 0), size) + size - max(min(hi - t0, size), min(max(lo - t0, 0), size)), published[1] = want > 0 ? counts[3][least & 255] : 0;
+  // each warp a run of the part, 32 tokens at a time
+  const bool some = want > 0;
+  const uint64_t at_least = some ? static_cast<uint64_t>(least) + 1 : 1ull << 32;     // keys that stay for sure
+  const int run = ((size + kSelectWarps - 1) / kSelectWarps + 31) & ~31, r0 = min(warp * run, size), r1 = min(r0 + run, size);
+  auto judge = [&](int i, unsigned* sure_lanes, unsigned* equal_lanes) {
+    const bool inside = i < r1, candidate = (i >= c0) & (i < c1);
+    const uint32_t key = key_of(min(i, size - 1));
+    *sure_lanes = __ballot_sync(0xffffffffu, inside & (!candidate | (key >= at_least)));
+    *equal_lanes = __ballot_sync(0xffffffffu, inside & candidate & (key == least) & some);
   };
   int my_sure = 0, my_equal = 0;
-  for (int t = r0 + lane; t - lane < r1; t += 32) {
-    bool a, e;
-    float v;
-    look(t, &a, &e, &v);
-    my_sure += __popc(__ballot_sync(0xffffffffu, a)), my_equal += __popc(__ballot_sync(0xffffffffu, e));
+#pragma unroll 4
+  for (int base = r0; base < r1; base += 32) {
+    unsigned as, es;
+    judge(base + lane, &as, &es);
+    my_sure += __popc(as), my_equal += __popc(es);
   }
   if (lane == 0) warp_sum[0][warp] = my_sure, warp_sum[1][warp] = my_equal;
-  __syncthreads();
+  if (ctas > 1) ptx::cluster_sync(); else __syncthreads();
+  int sure = 0, equal = 0;                      // in the parts and runs in front
+#pragma unroll
+  for (int r = 0; r < kMaxCluster - 1; ++r)
+    if (r < rank) sure += ld_cluster_i32(&published[0], r), equal += ld_cluster_i32(&published[1], r);
   for (int i = 0; i < warp; ++i) sure += warp_sum[0][i], equal += warp_sum[1][i];
-  for (int t = r0 + lane; t - lane < r1; t += 32) {
-    bool a, e;
-    float v;
-    look(t, &a, &e, &v);
-    const unsigned as = __ballot_sync(0xffffffffu, a), es = __ballot_sync(0xffffffffu, e), below = (1u << lane) - 1;
+#pragma unroll 4
+  for (int base = r0; base < r1; base += 32) {
+    unsigned as, es;
+    judge(base + lane, &as, &es);
+    const unsigned me = 1u << lane, below = me - 1;
     const int eq = equal + __popc(es & below);  // equal keys in front; the first `left` stay
-    if (a || (e && eq < left)) {
+    if (((as & me) != 0) | (((es & me) != 0) & (eq < left))) {
       const int at = sure + __popc(as & below) + min(eq, left);
-      kept[at] = t, nw[at] = v;
+      kept[at] = t0 + base + lane, nw[at] = ld_f32(w + t0 + base + lane);
     }
     sure += __popc(as), equal += __popc(es);
   }
-  ptx::cluster_sync();                          // nobody leaves while its counts may still be read
+  if (ctas > 1) ptx::cluster_sync();            // nobody leaves while its counts may still be read
 }
 
 // The kept rows to their new pages: 16 bytes of K and of V a thread and row, several rows at once.  Bound by the memory.
@@ -343,7 +362,12 @@ int b200q_paged_evict(const b200q_paged_cache* cache, const int32_t* block_table
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, evict_select_kernel, p) != cudaSuccess) return B200Q_ERR_CUDA;
+  const int64_t part = (weights_len + ctas - 1) / ctas;
+  const int held = part <= kHeldKeys ? static_cast<int>(part) : 0;          // a longer part is not held at all
+  cfg.dynamicSmemBytes = held * sizeof(uint32_t);
+  if (held > 0 && cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldKeys * sizeof(uint32_t)) != cudaSuccess)
+    return B200Q_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, held > 0 ? evict_select_kernel<true> : evict_select_kernel<false>, p) != cudaSuccess) return B200Q_ERR_CUDA;
   if (int rc = check_launch()) return rc;
   if (keep == 0 || table_width == 0) return B200Q_OK;
   const int64_t per = kMoveThreads / (p.row_bytes / 16) * kMoveRows, blocks = (keep + per - 1) / per;
