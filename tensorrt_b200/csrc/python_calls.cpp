@@ -31,6 +31,7 @@
 
 #include "b200q.h"
 #include "internal.h"
+#include "paged_calls.h"
 
 namespace {
 
@@ -556,6 +557,83 @@ PyObject* py_decoder_stack(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- paged key-value cache
+// The same bodies as the torch.library ops, without the dispatcher in front: 4 to 8 us of a call's host time, which is longer than the
+// kernels of a small batch run.  `tensors`: arguments that are tensors, or None where the function takes that.
+bool all_plain(PyObject* const* a, int tensors, std::optional<Tensor>* t) {
+  for (int i = 0; i < tensors; ++i) {
+    if (a[i] == Py_None) continue;
+    if (!plain(a[i])) return false;
+    t[i] = THPVariable_Unpack(a[i]);
+  }
+  return !modes_active();
+}
+bool ints(PyObject* const* a, int n, int64_t* out) {
+  for (int i = 0; i < n; ++i) {
+    if (!PyLong_Check(a[i])) return false;
+    out[i] = PyLong_AsLongLong(a[i]);
+    if (out[i] == -1 && PyErr_Occurred()) {
+      PyErr_Clear();
+      return false;
+    }
+  }
+  return true;
+}
+
+PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_VALUE(n == 9, "paged_append: 9 arguments expected");
+  std::optional<Tensor> t[9];
+  if (!all_plain(a, 9, t)) Py_RETURN_FALSE;
+  for (int i = 0; i < 6; ++i)
+    if (!t[i]) Py_RETURN_FALSE;
+  b200q_calls::paged_append(*t[0], *t[1], *t[2], *t[3], *t[4], *t[5], t[6], t[7], t[8]);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_VALUE(n == 11, "paged_attention: 11 arguments expected");
+  std::optional<Tensor> t[8];
+  int64_t v[2];
+  if (!all_plain(a, 8, t) || !PyFloat_Check(a[8]) || !ints(a + 9, 2, v)) Py_RETURN_NONE;
+  for (int i = 0; i < 5; ++i)
+    if (!t[i]) Py_RETURN_NONE;
+  return THPVariable_Wrap(b200q_calls::paged_attention(*t[0], *t[1], *t[2], *t[3], *t[4], t[5], t[6], t[7], PyFloat_AS_DOUBLE(a[8]), v[0], v[1]));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_paged_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_VALUE(n == 9, "paged_evict: 9 arguments expected");
+  std::optional<Tensor> t[6];
+  int64_t v[3];
+  if (!all_plain(a, 6, t) || !ints(a + 6, 3, v)) Py_RETURN_NONE;
+  for (const auto& x : t)
+    if (!x) Py_RETURN_NONE;
+  auto r = b200q_calls::paged_evict(*t[0], *t[1], *t[2], *t[3], *t[4], *t[5], v[0], v[1], v[2]);
+  PyObject* out = PyTuple_New(3);
+  if (out == nullptr) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::get<0>(r)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::get<1>(r)));
+  PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::get<2>(r)));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_VALUE(n == 8, "window_attention: 8 arguments expected");
+  std::optional<Tensor> t[5];
+  int64_t v[2];
+  if (!all_plain(a, 5, t) || !PyFloat_Check(a[5]) || !ints(a + 6, 2, v)) Py_RETURN_NONE;
+  for (int i = 0; i < 3; ++i)
+    if (!t[i]) Py_RETURN_NONE;
+  return THPVariable_Wrap(b200q_calls::window_attention(*t[0], *t[1], *t[2], t[3], t[4], PyFloat_AS_DOUBLE(a[5]), v[0], v[1]));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"fp8_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_fp8_linear)), METH_FASTCALL,
      "x, w_codes, w_scales, bias, x_amax, tile_n -> bf16 tensor, or None: take the general path"},
@@ -567,6 +645,14 @@ PyMethodDef methods[] = {
      "q, k, v, amax_q, amax_k, amax_v, is_causal, scale -> tensor like q or None"},
     {"decoder_stack", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_decoder_stack)), METH_FASTCALL,
      "h, layers, n_q, n_kv, head_dim, seq_len, eps, fp8, fuse_gate_up -> tensor like h or None"},
+    {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_append)), METH_FASTCALL,
+     "k, v, k_pages, v_pages, block_table, lens, cu_new, k_amax, v_amax -> whether it was taken"},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_attention)), METH_FASTCALL,
+     "q, k_pages, v_pages, block_table, lens, weights, k_amax, v_amax, scale, window, sinks -> tensor like q or None"},
+    {"paged_evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_evict)), METH_FASTCALL,
+     "k_pages, v_pages, block_table, lens, weights, out_table, keep, recent, sinks -> (kept, lens, weights) or None"},
+    {"window_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_window_attention)), METH_FASTCALL,
+     "q, k, v, q_lens, k_lens, scale, window, sinks -> tensor like q or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "b200q_native", "Whole calls of the b200q modules", -1, methods, nullptr, nullptr, nullptr, nullptr};

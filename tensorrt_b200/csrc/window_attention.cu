@@ -24,6 +24,8 @@
 // again, by one warp each, over the keys that they see.  That costs nothing where all is finite.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "ex2.cuh"
 #include "gemm_host.cuh"
@@ -525,7 +527,13 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int64_t D, int64_t r
 template <typename T, int DPAD>
 int launch_window(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const WindowParams& p, unsigned ctas, cudaStream_t st) {
   auto kernel = window_kernel<T, DPAD>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DPAD>::kSmem) != cudaSuccess) return B200Q_ERR_CUDA;
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return B200Q_ERR_CUDA;
+  if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DPAD>::kSmem) != cudaSuccess) return B200Q_ERR_CUDA;
+    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
+  }
   if (launch_pdl(kernel, dim3(ctas), dim3(kThreads), Layout<DPAD>::kSmem, st, tq, tk, tv, p) != cudaSuccess) return B200Q_ERR_CUDA;
   return check_launch();
 }

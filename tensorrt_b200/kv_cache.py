@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _native
 from .ops import load_ops
 
 load_ops()
@@ -27,7 +28,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     """Writes k, v [tokens, kv heads, D] into the pages.  The tokens of sequence b are rows cu_new[b] .. cu_new[b + 1] and the last of
     its lens[b] (cu_new None: one token of every sequence).  FP8 pages: codes of x / (amax / 448), `k_amax` and `v_amax` one value or
     one per kv head."""
-    _append(k, v, k_pages, v_pages, block_table, lens, cu_new, k_amax, v_amax)
+    if not _native.paged_append(k, v, k_pages, v_pages, block_table, lens, cu_new, k_amax, v_amax):
+        _append(k, v, k_pages, v_pages, block_table, lens, cu_new, k_amax, v_amax)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, *,
@@ -36,7 +38,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """softmax(q K^T * scale) V of one new token of every sequence: q [B, query heads, D] -> the same shape and type.  With
     window > 0 the token sees the last `window` keys and the first `sinks`.  `weights` (float32 [B, kv heads, keys]) gets each seen
     key's attention weight added, summed over the query heads of its kv head.  scale None: 1 / sqrt(D)."""
-    return _attention(q, k_pages, v_pages, block_table, lens, weights, k_amax, v_amax, 0.0 if scale is None else scale, window, sinks)
+    args = (q, k_pages, v_pages, block_table, lens, weights, k_amax, v_amax, 0.0 if scale is None else scale, window, sinks)
+    out = _native.paged_attention(*args)
+    return _attention(*args) if out is None else out
 
 
 def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, weights: torch.Tensor,
@@ -44,7 +48,9 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     """Cuts every sequence to `keep` tokens per kv head: the first `sinks`, the last `recent` and, of the others, those with the
     largest weights (equal ones: the lower token).  Their rows move, in order, to the pages of `out_table` [B, pages], which must not
     be among the pages read.  -> (kept tokens int32 [B, kv heads, keep], -1 beyond a shorter sequence; new lens; new weights)."""
-    return _evict(k_pages, v_pages, block_table, lens, weights, out_table, keep, recent, sinks)
+    args = (k_pages, v_pages, block_table, lens, weights, out_table, keep, recent, sinks)
+    out = _native.paged_evict(*args)
+    return _evict(*args) if out is None else out
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None, window: int = 0, sinks: int = 0,
@@ -52,4 +58,6 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale
     """Causal (lower-right aligned) attention: q [B, query heads, Sq, D], k and v [B, kv heads, Sk, D] -> q's shape and type.  With
     window > 0 a query sees the last `window` keys up to its own and the first `sinks`.  `q_lens`, `k_lens` int32 [B]: the queries and
     keys that each sequence has; rows beyond them, and rows that see no key, are zero.  scale None: 1 / sqrt(D)."""
-    return _window(q, k, v, q_lens, k_lens, 0.0 if scale is None else scale, window, sinks)
+    args = (q, k, v, q_lens, k_lens, 0.0 if scale is None else scale, window, sinks)
+    out = _native.window_attention(*args)
+    return _window(*args) if out is None else out

@@ -183,3 +183,18 @@ def test_one_token_agrees_with_the_paged_form(b200):
         ref, mass = reference(q[:, :, -1:], k, v, window, sinks, [1], [n])
         check(one[:, :, None], ref, mass)
         check(all_[:, :, -1:], ref, mass)
+
+
+def test_inputs_that_cannot_be_read_in_place(b200):
+    """K and V expanded over batches and heads, rows that start between 16-byte boundaries, a head dimension with a stride."""
+    g = torch.Generator(device="cuda").manual_seed(16)
+    q, k, v = inputs(g, 3, 4, 4, 130, 130, 64, torch.bfloat16, False)
+    one = k[:1, :1].expand(3, 4, 130, 64)
+    ref, mass = reference(q, one, v, 0, 0, [130] * 3, [130] * 3)
+    check(b200.window_attention(q, one, v), ref, mass)
+    odd = torch.randn(3 * 4 * 130 * 64 + 1, device="cuda", generator=g).bfloat16()[1:].view(3, 4, 130, 64)
+    ref, mass = reference(odd, k, odd, 0, 0, [130] * 3, [130] * 3)
+    check(b200.window_attention(odd, k, odd), ref, mass)
+    across = torch.randn(3, 4, 64, 130, device="cuda", generator=g).bfloat16().transpose(2, 3)
+    ref, mass = reference(across, k, across, 0, 0, [130] * 3, [130] * 3)
+    check(b200.window_attention(across, k, across), ref, mass)
