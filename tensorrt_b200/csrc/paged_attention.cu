@@ -148,11 +148,18 @@ struct Stage {
   }
 };
 
-// The piece of the line of tiles that CTA c of `ctas` takes.
-__device__ __forceinline__ int64_t piece(int64_t tiles, int c, int ctas) { return tiles * c / ctas; }
+// a / b of numbers that are not negative; a division of 64 bits takes some hundred clocks, one of 32 bits a third of that
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  return (a | b) >> 32 == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+// Where the piece of CTA c of `ctas` begins in the line of tiles, ctas <= tiles; no piece is empty.
+__device__ __forceinline__ int64_t piece(int64_t tiles, int c, int ctas) { return divide(tiles * c, ctas); }
+// The CTA whose piece holds tile x.
+__device__ __forceinline__ int holder(int64_t tiles, int64_t x, int ctas) { return static_cast<int>(divide((x + 1) * ctas - 1, tiles)); }
 
-// Adds up the tiles of all sequences and finds the one that holds tile `piece(total, cta)`; all threads take part.
-__device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, int ctas, int* b_out, int64_t* before_out, Seen* seen_out) {
+// Adds up the tiles of all sequences and finds the one that holds the first tile of this CTA's piece; all threads take part.
+// `ctas`: of those launched, as many as there are tiles.
+__device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, int* ctas, int* b_out, int64_t* before_out, Seen* seen_out) {
   __shared__ int64_t sums[kWarps];
   __shared__ int64_t found[2];
   __shared__ Seen found_keys;
@@ -184,7 +191,9 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
     mine = base + tid < p.B ? keys.tiles() * per : 0;
     total += scan(mine);
   }
-  const int64_t want = piece(total, cta, ctas);
+  if (total < *ctas) *ctas = static_cast<int>(total);
+  if (cta >= *ctas) return total;
+  const int64_t want = piece(total, cta, *ctas);
   if (p.B <= kThreads) {
     if (want >= inclusive - mine && want < inclusive) found[0] = tid, found[1] = inclusive - mine, found_keys = keys;
     __syncthreads();
@@ -217,7 +226,8 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
   __shared__ float row_max[kWarps][kRows], row_sum[kWarps][kRows];
   __shared__ int last_one;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int cta = blockIdx.x, ctas = gridDim.x;
+  const int cta = blockIdx.x;
+  int ctas = gridDim.x;
   char* const ring = smem + warp * S::kDepth * S::kBytes;
   const uint32_t ring_u32 = smem_u32(ring);
   pdl_launch_dependents();
@@ -226,20 +236,17 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
   int b;
   int64_t before;
   Seen see;
-  const int64_t total = find_start(p, cta, ctas, &b, &before, &see);
+  const int64_t total = find_start(p, cta, &ctas, &b, &before, &see);
+  if (cta >= ctas) return;
   int64_t at = piece(total, cta, ctas);
   const int64_t first_tile = at, end = piece(total, cta + 1, ctas);
+  // the item: kv head and block of query heads, within sequence b
+  int64_t item = divide(at - before, see.tiles());
+  int h = static_cast<int>(divide(item, p.blocks)), block = static_cast<int>(item) - h * p.blocks;
+  int64_t item_start = before + item * see.tiles();
   while (at < end) {
-    // ------------------------------------------------------------- the item
     const int tiles = see.tiles();
-    const int64_t item = (at - before) / tiles;       // kv head and block of query heads, within the sequence
-    if (item >= static_cast<int64_t>(p.c.heads) * p.blocks) {
-      before += static_cast<int64_t>(tiles) * p.c.heads * p.blocks;
-      see = keys_seen(p, ++b);
-      continue;
-    }
-    const int h = static_cast<int>(item / p.blocks), block = static_cast<int>(item % p.blocks);
-    const int64_t item_start = before + item * tiles, item_end = item_start + tiles;
+    const int64_t item_end = item_start + tiles;
     const int tile0 = static_cast<int>(at - item_start), tile1 = static_cast<int>((end < item_end ? end : item_end) - item_start);
     const int head0 = h * p.group + block * p.rows, rows = min(p.rows, p.group - block * p.rows);
     const int32_t* line = p.c.table + b * p.c.table_stride;
@@ -283,7 +290,9 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
     // ------------------------------------------------------------- queries: head g of each block, the elements that this lane's K chunks meet
     uint32_t q[BLOCKS8][kSteps][2];
     float unit[BLOCKS8];
-    int2 ahead = find_page(tile0);
+    int2 pages[S::kDepth];                             // of the stages to be filled: their loads do not wait for one another
+#pragma unroll
+    for (int s = 0; s < S::kDepth; ++s) pages[s] = find_page(tile0 + s);
     {
       const char* base = p.q + b * p.q_batch + head0 * p.q_head;
 #pragma unroll
@@ -302,12 +311,8 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
     }
     uint32_t there[S::kDepth];                         // which of the 16 keys of a stage exist
 #pragma unroll
-    for (int s = 0; s < S::kDepth - 1; ++s) {
-      const int2 now = ahead;
-      ahead = find_page(tile0 + s + 1);
-      there[s] = issue(s, now);
-    }
-
+    for (int s = 0; s < S::kDepth - 1; ++s) there[s] = issue(s, pages[s]);
+    int2 ahead = pages[S::kDepth - 1];
     {
 #pragma unroll
       for (int r = 0; r < BLOCKS8; ++r) {
@@ -478,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
     __syncthreads();
     const bool whole = tile0 == 0 && tile1 == tiles;
     // CTAs that share the item: c0 .. c1, those with a piece of it; the counter of the one that begins it
-    const int c0 = static_cast<int>(((item_start + 1) * ctas - 1) / total), c1 = static_cast<int>((item_end * ctas - 1) / total);
+    const int c0 = whole ? cta : holder(total, item_start, ctas), c1 = whole ? cta : holder(total, item_end - 1, ctas);
     float* part = p.parts + (static_cast<int64_t>(cta) * 2 + (at == first_tile ? 0 : 1)) * kPart;
     constexpr int kQuads = DPAD / 4;
     for (int i = tid; i < rows * kQuads; i += kThreads) {
@@ -517,12 +522,10 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
     }
     // ------------------------------------------------------------- the CTAs' parts together, by the one that comes last
     if (!whole) {
-      __threadfence();
       __syncthreads();
       if (tid == 0) {
-        const unsigned n = static_cast<unsigned>(total >= ctas ? c1 - c0 + 1 : tiles);
-        const unsigned order = atomicAdd(p.tickets + c0, 1u);
-        last_one = order == n - 1;
+        __threadfence();                               // what the CTA has written, seen through the barrier, in front of the ticket
+        last_one = atomicAdd(p.tickets + c0, 1u) == static_cast<unsigned>(c1 - c0);
         if (last_one) p.tickets[c0] = 0;
       }
       __syncthreads();
@@ -533,21 +536,17 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
           const int row = i / kQuads, d = (i % kQuads) * 4;
           float top = -INFINITY, sum = 0.0f, acc[4] = {};
           bool has = false;
-          constexpr int kAtOnce = 4;
-          int c = c0;
-          while (c <= c1) {
+          constexpr int kAtOnce = 8;
+          for (int c = c0; c <= c1; c += kAtOnce) {
             float pm[kAtOnce], ps[kAtOnce];
             float4 v[kAtOnce];
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k) {        // the loads first: they do not wait for one another
-              if (total < ctas)
-                while (c <= c1 && piece(total, c, ctas) == piece(total, c + 1, ctas)) ++c;
               ps[k] = -1.0f;
-              if (c > c1) continue;
-              const float* src = p.parts + (static_cast<int64_t>(c) * 2 + (c == c0 && second ? 1 : 0)) * kPart;
+              if (c + k > c1) continue;
+              const float* src = p.parts + (static_cast<int64_t>(c + k) * 2 + (c + k == c0 && second ? 1 : 0)) * kPart;
               pm[k] = __ldcg(src + kRows * DPAD + row), ps[k] = __ldcg(src + kRows * DPAD + kRows + row);
               v[k] = __ldcg(reinterpret_cast<const float4*>(src + row * DPAD + d));
-              ++c;
             }
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k) {
@@ -577,6 +576,12 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
     }
     __syncthreads();
     at += tile1 - tile0;
+    if (at >= end) break;
+    item_start = item_end;
+    if (++block == p.blocks) {
+      block = 0;
+      if (++h == p.c.heads) h = 0, see = keys_seen(p, ++b);
+    }
   }
 }
 
