@@ -36,6 +36,7 @@ constexpr int kMaxCtas = 1024;                                                 /
 struct DecodeParams {
   Cache c;
   int page_shift;            // log2 of the page size, or -1
+  bool one_layout;           // K and V pages have the same strides
   const char* q;
   int64_t q_batch, q_head;   // bytes
   void* out;
@@ -49,12 +50,13 @@ struct DecodeParams {
   float* parts;              // [kMaxCtas][2][kPart]
 };
 
+constexpr float kLazy = 8.0f;   // log2 of how far the reference of a sum may lie below its largest term
 constexpr int kPart = kRows * paged::kMaxD + 2 * kRows;   // result rows, maxima, sums
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-// 16 bytes to shared memory, zeros where `there` is false.
-__device__ __forceinline__ void copy16(uint32_t dst, const char* src, bool there) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+// 16 bytes to shared memory: `bytes` of them from `src`, zeros behind.
+__device__ __forceinline__ void copy16(uint32_t dst, const char* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -89,10 +91,9 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint32_t codes_f16x2(uint32_t v) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(v)));
-  return h;
+// four codes -> four fp16 values, two and two
+__device__ __forceinline__ void widen(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -224,6 +225,7 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
   constexpr int kSteps = DPAD / 16;
   extern __shared__ __align__(128) char smem[];
   __shared__ float row_max[kWarps][kRows], row_sum[kWarps][kRows];
+  __shared__ uint32_t there[kWarps][S::kDepth];        // which of the 16 keys of a stage exist
   __shared__ int last_one;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x;
@@ -250,11 +252,12 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
     const int tile0 = static_cast<int>(at - item_start), tile1 = static_cast<int>((end < item_end ? end : item_end) - item_start);
     const int head0 = h * p.group + block * p.rows, rows = min(p.rows, p.group - block * p.rows);
     const int32_t* line = p.c.table + b * p.c.table_stride;
-    const char* kbase = p.c.k.base + h * p.c.k.head;
-    const char* vbase = p.c.v.base + h * p.c.v.head;
+    const char* const k_lane = p.c.k.base + h * p.c.k.head + lane % (S::kChunks < 8 ? S::kChunks : 8) * 16;
+    const char* const v_lane = p.c.v.base + h * p.c.v.head + lane % (S::kChunks < 8 ? S::kChunks : 8) * 16;
 
     // ------------------------------------------------------------- copies of a warp's 16 keys of a tile
-    auto find_page = [&](int tile) {                  // lane: page of key lane % 16, -1 where there is none; row within it
+    // lane: of key lane % 16, its page (-1: none) and its row within it
+    auto find_page = [&](int tile) {
       const int i = tile * kTile + warp * kKeys + (lane & 15);
       int page = -1, row = 0;
       if (tile < tile1 && i < see.seen) {
@@ -265,34 +268,32 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
       return make_int2(page, row);
     };
     auto issue = [&](int slot, int2 where) {
-      const int page = static_cast<unsigned>(where.x) < static_cast<unsigned>(p.c.num_pages) ? where.x : -1;
+      const bool exists = static_cast<unsigned>(where.x) < static_cast<unsigned>(p.c.num_pages);
       constexpr int kLanes = S::kChunks < 8 ? S::kChunks : 8, kPer = 32 / kLanes;     // lanes to a row, rows to an instruction
+      const int64_t k_row = exists ? where.x * p.c.k.page + where.y * p.c.k.row : -1;
+      const int64_t v_row = p.one_layout ? k_row : (exists ? where.x * p.c.v.page + where.y * p.c.v.row : -1);
       const uint32_t kdst = ring_u32 + slot * S::kBytes, vdst = kdst + kKeys * S::kRowBytes;
 #pragma unroll
       for (int j = 0; j < kKeys / kPer; ++j) {
         const int key = j * kPer + lane / kLanes;
-        const int pg = __shfl_sync(0xffffffffu, page, key), row = __shfl_sync(0xffffffffu, where.y, key);
-        const int64_t safe = pg < 0 ? 0 : pg;
-        const char* ks = kbase + safe * p.c.k.page + row * p.c.k.row;
-        const char* vs = vbase + safe * p.c.v.page + row * p.c.v.row;
+        int64_t k_off = __shfl_sync(0xffffffffu, k_row, key), v_off = k_off;
+        if (!p.one_layout) v_off = __shfl_sync(0xffffffffu, v_row, key);
+        const int there_bytes = k_off < 0 ? 0 : 16;
 #pragma unroll
         for (int c0 = 0; c0 < S::kChunks; c0 += kLanes) {
           const int c = c0 + lane % kLanes;
-          const bool inside = c * 16 < p.c.D * (CODES ? 1 : 2);
-          const int src = inside ? c * 16 : 0;
-          copy16(kdst + key * S::kRowBytes + S::k_chunk(key, c) * 16, ks + src, pg >= 0 && inside);
-          copy16(vdst + key * S::kRowBytes + S::v_chunk(key, c) * 16, vs + src, pg >= 0 && inside);
+          const int bytes = c * 16 < p.c.D * (CODES ? 1 : 2) ? there_bytes : 0;      // 0: nothing is read, zeros are written
+          copy16(kdst + key * S::kRowBytes + S::k_chunk(key, c) * 16, k_lane + k_off + c0 * 16, bytes);
+          copy16(vdst + key * S::kRowBytes + S::v_chunk(key, c) * 16, v_lane + v_off + c0 * 16, bytes);
         }
       }
-      copy_commit();
-      return __ballot_sync(0xffffffffu, page >= 0 && lane < 16);
+      const uint32_t keys = __ballot_sync(0xffffffffu, exists && lane < 16);
+      if (lane == 0) there[warp][slot] = keys;
     };
     // ------------------------------------------------------------- queries: head g of each block, the elements that this lane's K chunks meet
     uint32_t q[BLOCKS8][kSteps][2];
     float unit[BLOCKS8];
-    int2 pages[S::kDepth];                             // of the stages to be filled: their loads do not wait for one another
-#pragma unroll
-    for (int s = 0; s < S::kDepth; ++s) pages[s] = find_page(tile0 + s);
+    int2 page0 = find_page(tile0), page1 = find_page(tile0 + 1), page2 = find_page(tile0 + 2);   // three ahead: a load from the table takes as long as a tile
     {
       const char* base = p.q + b * p.q_batch + head0 * p.q_head;
 #pragma unroll
@@ -309,10 +310,6 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
         }
       }
     }
-    uint32_t there[S::kDepth];                         // which of the 16 keys of a stage exist
-#pragma unroll
-    for (int s = 0; s < S::kDepth - 1; ++s) there[s] = issue(s, pages[s]);
-    int2 ahead = pages[S::kDepth - 1];
     {
 #pragma unroll
       for (int r = 0; r < BLOCKS8; ++r) {
@@ -357,113 +354,114 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
       m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.0f;
     }
     bool any = false;
-    for (int tile = tile0; tile < tile1;) {
+    int slot = 0;                                       // of the tile that is requested; the next one holds the oldest
+#pragma unroll 1
+    for (int ahead = tile0; ahead < tile1 + S::kDepth - 1; ++ahead) {
+      if (ahead < tile1) issue(slot, page0);
+      copy_commit();                                // an empty group behind the last tile
+      page0 = page1, page1 = page2, page2 = find_page(ahead + 3);
+      slot = slot + 1 == S::kDepth ? 0 : slot + 1;
+      const int tile = ahead - (S::kDepth - 1);
+      if (tile < tile0) continue;
+      copy_wait<S::kDepth - 1>();
+      __syncwarp();
+      const uint32_t ks = ring_u32 + slot * S::kBytes, vs = ks + kKeys * S::kRowBytes, keys = there[warp][slot];
+      any = any || keys != 0;
+      // S^T: keys g and g + 8, heads 2 t and 2 t + 1; two chains of sums, the products of one wait for each other
+      float x[BLOCKS8][4], y[BLOCKS8][4];
 #pragma unroll
-      for (int s = 0; s < S::kDepth; ++s) {
-        if (tile < tile1) {
-          copy_wait<S::kDepth - 2>();
-          __syncwarp();
-          const uint32_t ks = ring_u32 + s * S::kBytes, vs = ks + kKeys * S::kRowBytes, keys = there[s];
-          any = any || keys != 0;
-          // S^T: keys g and g + 8, heads 2 t and 2 t + 1; two chains of sums, the products of one wait for each other
-          float x[BLOCKS8][4], y[BLOCKS8][4];
+      for (int r = 0; r < BLOCKS8; ++r) x[r][0] = x[r][1] = x[r][2] = x[r][3] = y[r][0] = y[r][1] = y[r][2] = y[r][3] = 0.0f;
 #pragma unroll
-          for (int r = 0; r < BLOCKS8; ++r) x[r][0] = x[r][1] = x[r][2] = x[r][3] = y[r][0] = y[r][1] = y[r][2] = y[r][3] = 0.0f;
+      for (int i = 0; i < kSteps / (CODES ? 4 : 2); ++i) {
+        const uint4 u = lds128(ks + g * S::kRowBytes + S::k_chunk(g, i * 4 + t) * 16);
+        const uint4 v = lds128(ks + (g + 8) * S::kRowBytes + S::k_chunk(g + 8, i * 4 + t) * 16);
+        if constexpr (CODES) {
+          const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-          for (int i = 0; i < kSteps / (CODES ? 4 : 2); ++i) {
-            const uint4 u = lds128(ks + g * S::kRowBytes + S::k_chunk(g, i * 4 + t) * 16);
-            const uint4 v = lds128(ks + (g + 8) * S::kRowBytes + S::k_chunk(g + 8, i * 4 + t) * 16);
-            if constexpr (CODES) {
-              const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+          for (int e = 0; e < 4; ++e) {
+            uint32_t a[4];
+            widen(uw[e], a[0], a[2]);
+            widen(vw[e], a[1], a[3]);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t a[4] = {codes_f16x2(uw[e]), codes_f16x2(vw[e]), codes_f16x2(uw[e] >> 16), codes_f16x2(vw[e] >> 16)};
-#pragma unroll
-                for (int r = 0; r < BLOCKS8; ++r) mma<kHalf>(e & 1 ? y[r] : x[r], a, q[r][i * 4 + e][0], q[r][i * 4 + e][1]);
-              }
-            } else {
-              const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
-#pragma unroll
-              for (int r = 0; r < BLOCKS8; ++r) {
-                mma<kHalf>(x[r], a0, q[r][i * 2][0], q[r][i * 2][1]);
-                mma<kHalf>(y[r], a1, q[r][i * 2 + 1][0], q[r][i * 2 + 1][1]);
-              }
-            }
+            for (int r = 0; r < BLOCKS8; ++r) mma<kHalf>(e & 1 ? y[r] : x[r], a, q[r][i * 4 + e][0], q[r][i * 4 + e][1]);
           }
-          const bool there0 = (keys >> g) & 1, there1 = (keys >> (g + 8)) & 1;
-          uint32_t pt[BLOCKS8][2];
+        } else {
+          const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
 #pragma unroll
           for (int r = 0; r < BLOCKS8; ++r) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[r][e] = (e < 2 ? there0 : there1) ? (x[r][e] + y[r][e]) * sl[r][e & 1] : -INFINITY;
-            if (p.logits != nullptr) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int i = tile * kTile + warp * kKeys + g + 8 * (e >> 1), row = 8 * r + 2 * t + (e & 1);
-                if (row < rows && i < see.seen && see.token(i) < p.weights_len)
-                  p.logits[(static_cast<int64_t>(b) * p.Hq + head0 + row) * p.logits_stride + i] = x[r][e];
-              }
-            }
-            const float m0 = fmaxf(m[r][0], column_max(fmaxf(x[r][0], x[r][2]))), m1 = fmaxf(m[r][1], column_max(fmaxf(x[r][1], x[r][3])));
-            if (__any_sync(0xffffffffu, m0 > m[r][0] || m1 > m[r][1])) {
-              const float f0 = m0 == -INFINITY ? 1.0f : exp2_fast(m[r][0] - m0), f1 = m1 == -INFINITY ? 1.0f : exp2_fast(m[r][1] - m1);
-              l[r][0] *= f0, l[r][1] *= f1, m[r][0] = m0, m[r][1] = m1;
-#pragma unroll
-              for (int i = 0; i < kSteps; ++i) o[r][i][0] *= f0, o[r][i][1] *= f1, o[r][i][2] *= f0, o[r][i][3] *= f1;
-            }
-            const float base0 = m0 == -INFINITY ? 0.0f : m0, base1 = m1 == -INFINITY ? 0.0f : m1;
-            x[r][0] = exp2_fast(x[r][0] - base0), x[r][1] = exp2_fast(x[r][1] - base1);
-            x[r][2] = exp2_fast(x[r][2] - base0), x[r][3] = exp2_fast(x[r][3] - base1);
-            l[r][0] += x[r][0] + x[r][2], l[r][1] += x[r][1] + x[r][3];
-            pt[r][0] = transpose8x8(pack16<kHalf>(x[r][0], x[r][1]));
-            pt[r][1] = transpose8x8(pack16<kHalf>(x[r][2], x[r][3]));
+            mma<kHalf>(x[r], a0, q[r][i * 2][0], q[r][i * 2][1]);
+            mma<kHalf>(y[r], a1, q[r][i * 2 + 1][0], q[r][i * 2 + 1][1]);
           }
-          if constexpr (CODES) {
-            constexpr int kWords = DPAD / 32;           // of the row pieces that this lane widens
-            uint32_t w[4][kWords];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int key = t * 2 + (k & 1) + (k >> 1) * 8;
-              if constexpr (DPAD == 128) {
-                const uint4 u = lds128(vs + key * S::kRowBytes + S::v_chunk(key, g) * 16);
-                w[k][0] = u.x, w[k][1] = u.y, w[k][2] = u.z, w[k][3] = u.w;
-              } else {
-                const uint2 u = lds64(vs + key * S::kRowBytes + S::v_chunk(key, g >> 1) * 16 + (g & 1) * 8);
-                w[k][0] = u.x, w[k][1] = u.y;
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-              const uint32_t lo0 = __byte_perm(w[0][i], w[1][i], 0x5140), hi0 = __byte_perm(w[0][i], w[1][i], 0x7362);
-              const uint32_t lo1 = __byte_perm(w[2][i], w[3][i], 0x5140), hi1 = __byte_perm(w[2][i], w[3][i], 0x7362);
-              const uint32_t a0[4] = {codes_f16x2(lo0), codes_f16x2(lo0 >> 16), codes_f16x2(lo1), codes_f16x2(lo1 >> 16)};
-              const uint32_t a1[4] = {codes_f16x2(hi0), codes_f16x2(hi0 >> 16), codes_f16x2(hi1), codes_f16x2(hi1 >> 16)};
-#pragma unroll
-              for (int r = 0; r < BLOCKS8; ++r) {
-                mma<kHalf>(o[r][2 * i], a0, pt[r][0], pt[r][1]);
-                mma<kHalf>(o[r][2 * i + 1], a1, pt[r][0], pt[r][1]);
-              }
-            }
-          } else {
-            const int key = (lane & 7) + ((lane >> 4) & 1) * 8;
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-              uint32_t a[4];
-              ldmatrix_trans(vs + key * S::kRowBytes + S::v_chunk(key, 2 * i + ((lane >> 3) & 1)) * 16, a);
-#pragma unroll
-              for (int r = 0; r < BLOCKS8; ++r) mma<kHalf>(o[r][i], a, pt[r][0], pt[r][1]);
-            }
-          }
-          __syncwarp();
-          const int2 now = ahead;
-          ahead = find_page(tile + S::kDepth);
-          there[(s + S::kDepth - 1) % S::kDepth] = issue((s + S::kDepth - 1) % S::kDepth, now);
-          ++tile;
         }
       }
+      const bool there0 = (keys >> g) & 1, there1 = (keys >> (g + 8)) & 1;
+      uint32_t pt[BLOCKS8][2];
+#pragma unroll
+      for (int r = 0; r < BLOCKS8; ++r) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[r][e] = (e < 2 ? there0 : there1) ? (x[r][e] + y[r][e]) * sl[r][e & 1] : -INFINITY;
+        if (p.logits != nullptr) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = tile * kTile + warp * kKeys + g + 8 * (e >> 1), row = 8 * r + 2 * t + (e & 1);
+            if (row < rows && i < see.seen && see.token(i) < p.weights_len)
+              p.logits[(static_cast<int64_t>(b) * p.Hq + head0 + row) * p.logits_stride + i] = x[r][e];
+          }
+        }
+        // the reference stays while no logit is more than 2^8 times above it: sums and P hold that, and the exchange among lanes is rare
+        if (__any_sync(0xffffffffu, fmaxf(x[r][0], x[r][2]) > m[r][0] + kLazy || fmaxf(x[r][1], x[r][3]) > m[r][1] + kLazy)) {
+          const float m0 = fmaxf(m[r][0], column_max(fmaxf(x[r][0], x[r][2]))), m1 = fmaxf(m[r][1], column_max(fmaxf(x[r][1], x[r][3])));
+          const float f0 = m0 == -INFINITY ? 1.0f : exp2_fast(m[r][0] - m0), f1 = m1 == -INFINITY ? 1.0f : exp2_fast(m[r][1] - m1);
+          l[r][0] *= f0, l[r][1] *= f1, m[r][0] = m0, m[r][1] = m1;
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) o[r][i][0] *= f0, o[r][i][1] *= f1, o[r][i][2] *= f0, o[r][i][3] *= f1;
+        }
+        const float base0 = m[r][0] == -INFINITY ? 0.0f : m[r][0], base1 = m[r][1] == -INFINITY ? 0.0f : m[r][1];
+        x[r][0] = exp2_fast(x[r][0] - base0), x[r][1] = exp2_fast(x[r][1] - base1);
+        x[r][2] = exp2_fast(x[r][2] - base0), x[r][3] = exp2_fast(x[r][3] - base1);
+        l[r][0] += x[r][0] + x[r][2], l[r][1] += x[r][1] + x[r][3];
+        pt[r][0] = transpose8x8(pack16<kHalf>(x[r][0], x[r][1]));
+        pt[r][1] = transpose8x8(pack16<kHalf>(x[r][2], x[r][3]));
+      }
+      if constexpr (CODES) {
+        constexpr int kWords = DPAD / 32;           // of the row pieces that this lane widens
+        uint32_t w[4][kWords];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int key = t * 2 + (k & 1) + (k >> 1) * 8;
+          if constexpr (DPAD == 128) {
+            const uint4 u = lds128(vs + key * S::kRowBytes + S::v_chunk(key, g) * 16);
+            w[k][0] = u.x, w[k][1] = u.y, w[k][2] = u.z, w[k][3] = u.w;
+          } else {
+            const uint2 u = lds64(vs + key * S::kRowBytes + S::v_chunk(key, g >> 1) * 16 + (g & 1) * 8);
+            w[k][0] = u.x, w[k][1] = u.y;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          const uint32_t lo0 = __byte_perm(w[0][i], w[1][i], 0x5140), hi0 = __byte_perm(w[0][i], w[1][i], 0x7362);
+          const uint32_t lo1 = __byte_perm(w[2][i], w[3][i], 0x5140), hi1 = __byte_perm(w[2][i], w[3][i], 0x7362);
+          uint32_t a0[4], a1[4];
+          widen(lo0, a0[0], a0[1]), widen(lo1, a0[2], a0[3]);
+          widen(hi0, a1[0], a1[1]), widen(hi1, a1[2], a1[3]);
+#pragma unroll
+          for (int r = 0; r < BLOCKS8; ++r) {
+            mma<kHalf>(o[r][2 * i], a0, pt[r][0], pt[r][1]);
+            mma<kHalf>(o[r][2 * i + 1], a1, pt[r][0], pt[r][1]);
+          }
+        }
+      } else {
+        const int key = (lane & 7) + ((lane >> 4) & 1) * 8;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          uint32_t a[4];
+          ldmatrix_trans(vs + key * S::kRowBytes + S::v_chunk(key, 2 * i + ((lane >> 3) & 1)) * 16, a);
+#pragma unroll
+          for (int r = 0; r < BLOCKS8; ++r) mma<kHalf>(o[r][i], a, pt[r][0], pt[r][1]);
+        }
+      }
+      __syncwarp();
     }
-    copy_wait<0>();
-    __syncwarp();
 
     // ------------------------------------------------------------- the four warps' parts together
     float* mine = reinterpret_cast<float*>(ring);     // rows of DPAD: the ring is empty
@@ -536,7 +534,8 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
           const int row = i / kQuads, d = (i % kQuads) * 4;
           float top = -INFINITY, sum = 0.0f, acc[4] = {};
           bool has = false;
-          constexpr int kAtOnce = 8;
+          constexpr int kAtOnce = 4;
+#pragma unroll 1
           for (int c = c0; c <= c1; c += kAtOnce) {
             float pm[kAtOnce], ps[kAtOnce];
             float4 v[kAtOnce];
@@ -664,6 +663,7 @@ int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, co
   p.page_shift = -1;
   if ((p.c.page_size & (p.c.page_size - 1)) == 0)
     for (p.page_shift = 0; (1 << p.page_shift) < p.c.page_size;) ++p.page_shift;
+  p.one_layout = p.c.k.page == p.c.v.page && p.c.k.row == p.c.v.row;
   p.q = static_cast<const char*>(q);
   p.q_batch = q_strides[0] * 2, p.q_head = q_strides[1] * 2;
   p.out = out;
