@@ -173,7 +173,7 @@ template <int DPAD>
 struct Layout {
   static constexpr int kBoxes = DPAD / 64, kBoxBytes = 128 * 128, kTileBytes = kBoxes * kBoxBytes;
   static constexpr int kStages = DPAD == 128 ? 5 : 8;
-  static constexpr int kBars = 2 * kStages + 1 + 8 + 1;
+  static constexpr int kBars = 2 * kStages + 2 + 8 + 1;
   static constexpr int kSmem = 1024 + (2 + kStages) * kTileBytes + kBars * 8 + 16;
 };
 
@@ -219,7 +219,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   uint64_t* const full = bars;
   uint64_t* const empty = bars + L::kStages;
   uint64_t* const q_full = empty + L::kStages;
-  uint64_t* const s_full = q_full + 1;
+  uint64_t* const s_full = q_full + 2;
   uint64_t* const p_full = s_full + 2;
   uint64_t* const p_half = p_full + 2;
   uint64_t* const o_full = p_half + 2;
@@ -231,7 +231,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     ptx::tmem_alloc<1>(tmem_slot, kTmemCols);
     ptx::tmem_relinquish<1>();
   } else if (threadIdx.x == 0) {
-    for (int i = 0; i < 2 * L::kStages + 1; ++i) ptx::mbar_init(bars + i, 1);
+    for (int i = 0; i < 2 * L::kStages + 2; ++i) ptx::mbar_init(bars + i, 1);
     for (int s = 0; s < 2; ++s) ptx::mbar_init(s_full + s, 1), ptx::mbar_init(p_full + s, 4), ptx::mbar_init(p_half + s, 4), ptx::mbar_init(o_full + s, 1);
     ptx::mbar_init(done, 1);
     ptx::fence_barrier_init();
@@ -252,9 +252,11 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     if (warp == 9) {
     // ------------------------------------------------------------- loads
     if (lane == 0 && w.tiles > 0) {
-      ptx::mbar_arrive_expect_tx(q_full, 2 * L::kTileBytes);
-      for (int s = 0; s < 2; ++s)
-        for (int x = 0; x < L::kBoxes; ++x) tma_load_4d(sq + s * L::kTileBytes + x * L::kBoxBytes, &tq, q_full, x * 64, w.q0[s], w.head[s], w.b);
+      auto load_q = [&](int s, int q0, int head) {
+        ptx::mbar_arrive_expect_tx(q_full + s, L::kTileBytes);
+        for (int x = 0; x < L::kBoxes; ++x) tma_load_4d(sq + s * L::kTileBytes + x * L::kBoxBytes, &tq, q_full + s, x * 64, q0, head, w.b);
+      };
+      load_q(0, w.q0[0], w.head[0]);
       int st = 0, issued = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -269,12 +271,12 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           ptx::mbar_arrive_expect_tx(full + st, L::kTileBytes);
           for (int x = 0; x < L::kBoxes; ++x)
             tma_load_4d(ring + st * L::kTileBytes + x * L::kBoxBytes, kv == 0 ? &tk : &tv, full + st, x * 64, row, w.kv_head, w.b);
-          ++issued;
+          if (++issued == 1) load_q(1, w.q0[1], w.head[1]);      // the first product waits for the first query tile and the first keys
           if (++st == L::kStages) st = 0, ph ^= 1u;
         }
       }
       // no copy may be under way when the CTA ends, whatever became of its readers
-      if (!ptx::mbar_wait(q_full, 0)) timed_out(p.status, 81);
+      if (!ptx::mbar_wait(q_full, 0) || (issued > 0 && !ptx::mbar_wait(q_full + 1, 0))) timed_out(p.status, 81);
       for (int i = max(0, issued - L::kStages); i < issued; ++i)
         if (!ptx::mbar_wait(full + i % L::kStages, (i / L::kStages) & 1)) timed_out(p.status, 81);
     }
@@ -290,8 +292,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       constexpr uint32_t kLeadV = (L::kBoxBytes >> 4) << 16;
       const uint32_t ring_lo = (ptx::smem_u32(ring) >> 4) & 0x3fffu, q_lo = ptx::desc_lo_sw128(ptx::smem_u32(sq));
       const bool leader = elect_one();
-      bool ok = ptx::mbar_wait(q_full, 0);
-      if (!ok) timed_out(p.status, 82);
+      bool ok = true;
       uint32_t p_phase[2] = {0, 0};
       bool waiting[2] = {false, false}, begun[2] = {false, false};   // a P that is to be multiplied; O holds something
       int stage = 0, v_stage = 0;                                    // of this tile's K; of the V of the tile before
@@ -328,7 +329,11 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
             begun[s] = true;
             waiting[s] = false;
           }
-          if (more && needs(p, w.lowest[s], w.highest[s], t)) {
+          if (!more && leader) ptx::tc_commit<1>(o_full + s);
+          __syncwarp();
+          if (j == 0 && ok && !ptx::mbar_wait(q_full + s, 0)) ok = false;
+          if (ok && more && needs(p, w.lowest[s], w.highest[s], t)) {
+            if (j == 0) ptx::tc_fence_after();
             if (leader) {
 #pragma unroll
               for (int k = 0; k < DPAD / 16; ++k) {
@@ -357,10 +362,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         stage = v_stage + 1, phase = v_phase;
         if (stage == L::kStages) stage = 0, phase ^= 1u;
       }
-      if (leader) {
-        for (int s = 0; s < 2; ++s) ptx::tc_commit<1>(o_full + s);
-        ptx::tc_commit<1>(done);
-      }
+      if (leader) ptx::tc_commit<1>(done);
       __syncwarp();
       if (!ptx::mbar_wait(done, 0)) timed_out(p.status, 85);
     }
@@ -474,7 +476,10 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       ptx::tc_fence_after();
       const float f = 1.0f / l;
       float probe = 0.0f;
-      T* dst = reinterpret_cast<T*>(p.out) + w.b * p.o_s[0] + h * p.o_s[1] + static_cast<int64_t>(i) * p.o_s[2];
+      // Through the place of this tile's queries, which no product reads any more: a thread has a whole row, and 32 rows' pieces of 16 bytes
+      // in one store instruction are 32 lines (5700 clocks for a tile; so 1000).
+      constexpr int kRowBytes = DPAD * 2, kPieces = kRowBytes / 16;
+      char* const rows = sq + s * L::kTileBytes;
 #pragma unroll
       for (int c = 0; c < DPAD / 32; ++c) {
         uint32_t o[32];
@@ -484,17 +489,32 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         }
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
-          if (c * 32 + e >= p.D || i >= p.Sq) continue;
           uint4 u = make_uint4(0, 0, 0, 0);
           if (at >= 0) {
             float y[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(o[e + k]) * f, probe = fmaf(y[k], 0.0f, probe);
+            for (int k = 0; k < 8; ++k) {
+              y[k] = __uint_as_float(o[e + k]) * f;
+              if (c * 32 + e < p.D) probe = fmaf(y[k], 0.0f, probe);
+            }
             u = make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
           }
-          *reinterpret_cast<uint4*>(dst + c * 32 + e) = u;
+          *reinterpret_cast<uint4*>(rows + r * kRowBytes + (((c * 4 + e / 8) ^ (r & 7)) * 16)) = u;
         }
       }
+      __syncwarp();
+      const int64_t row_at = w.b * p.o_s[0] + h * p.o_s[1] + static_cast<int64_t>(i) * p.o_s[2];
+#pragma unroll 4
+      for (int k = 0; k < 32; k += 32 / kPieces) {
+        const int from = k + lane / kPieces, piece = lane % kPieces;        // row of this warp
+        const int64_t dst = __shfl_sync(0xffffffffu, row_at, from);
+        const bool there = __shfl_sync(0xffffffffu, i, from) < p.Sq && piece * 8 < p.D;
+        const int row = (r & ~31) + from;
+        if (there)
+          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + dst + piece * 8) =
+              *reinterpret_cast<const uint4*>(rows + row * kRowBytes + ((piece ^ (row & 7)) * 16));
+      }
+      __syncwarp();
       for (unsigned bad = __ballot_sync(0xffffffffu, probe != probe); bad; bad &= bad - 1) {
         const int who = __ffs(bad) - 1;
         row_again<T>(p, w.b, __shfl_sync(0xffffffffu, h, who), __shfl_sync(0xffffffffu, i, who), __shfl_sync(0xffffffffu, at, who));
