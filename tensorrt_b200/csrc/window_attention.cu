@@ -34,7 +34,7 @@
 namespace b200q {
 namespace {
 
-constexpr int kTileRows = 128, kTileKeys = 128, kThreads = 384, kTmemCols = 512;
+constexpr int kTileRows = 128, kTileKeys = 128;
 constexpr float kLazy = 8.0f;   // log2 of how far the reference may lie below the maximum
 constexpr int kPolyPairs = 2;   // of 16 pairs of exponentials: on the FMA pipe
 
@@ -53,6 +53,7 @@ struct WindowParams {
   int pair_heads;            // the second query tile: the next heads (1) or the next rows (0)
   int units;                 // CTAs that share a kv head and rows
   int q_blocks;
+  int splits;                // CTAs of a cluster that share an item's key tiles (one query tile a CTA)
   int B;
   int* status;
 };
@@ -97,6 +98,16 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float2 ld_cluster_f2(const float2* p, unsigned cta) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(ptx::mapa_u32(ptx::smem_u32(p), cta)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(const float* p, unsigned cta) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(ptx::mapa_u32(ptx::smem_u32(p), cta)) : "memory");
+  return v;
+}
 // true in one lane of a converged warp
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -125,12 +136,13 @@ __device__ __forceinline__ void load4(const T* p, float* f) {
   }
 }
 
-// What a CTA works on.
+// What a CTA works on: NQ query tiles.
+template <int NQ>
 struct Work {
   int b, kv_head, nq, off;                  // off: position of query 0
-  int head[2], q0[2], lowest[2], highest[2];  // per query tile: first head, first query, positions of its rows (highest < 0: none)
-  int sink_tiles, first, tiles;             // key tiles 0 .. sink_tiles - 1, then first, first + 1, ..
-  __device__ __forceinline__ int tile(int j) const { return j < sink_tiles ? j : first + j - sink_tiles; }
+  int head[NQ], q0[NQ], lowest[NQ], highest[NQ];  // per query tile: first head, first query, positions of its rows (highest < 0: none)
+  int sink_tiles, first, begin, tiles;      // key tiles 0 .. sink_tiles - 1, then first, first + 1, ..; of them `tiles` from the `begin`-th on
+  __device__ __forceinline__ int tile(int j) const { return begin + j < sink_tiles ? begin + j : first + begin + j - sink_tiles; }
 };
 // Whether rows at positions lowest .. highest see a key of tile t.
 __device__ __forceinline__ bool needs(const WindowParams& p, int lowest, int highest, int t) {
@@ -138,11 +150,12 @@ __device__ __forceinline__ bool needs(const WindowParams& p, int lowest, int hig
   return k0 <= highest && (p.window == 0 || k0 + kTileKeys - 1 > lowest - p.window || k0 < p.sinks);
 }
 
-__device__ __forceinline__ Work work_of(const WindowParams& p) {
-  Work w;
-  const int per_row_block = p.B * p.Hkv * p.units;
+template <int NQ>
+__device__ __forceinline__ Work<NQ> work_of(const WindowParams& p) {
+  Work<NQ> w;
+  const int per_row_block = p.B * p.Hkv * p.units, item = static_cast<int>(blockIdx.x) / p.splits, part = static_cast<int>(blockIdx.x) % p.splits;
   // the last queries first: they see most
-  const int block = p.q_blocks - 1 - static_cast<int>(blockIdx.x) / per_row_block, at = static_cast<int>(blockIdx.x) % per_row_block;
+  const int block = p.q_blocks - 1 - item / per_row_block, at = item % per_row_block;
   const int unit = at % p.units;
   w.kv_head = at / p.units % p.Hkv;
   w.b = at / p.units / p.Hkv;
@@ -151,14 +164,14 @@ __device__ __forceinline__ Work work_of(const WindowParams& p) {
   w.off = nk - w.nq;
   int low = 0x7fffffff, high = -1;
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    w.head[s] = w.kv_head * p.group + (p.pair_heads ? 2 * unit + s : unit) * p.nh;
-    w.q0[s] = p.pair_heads ? block * p.rp : (2 * block + s) * p.rp;
+  for (int s = 0; s < NQ; ++s) {
+    w.head[s] = w.kv_head * p.group + (p.pair_heads ? NQ * unit + s : unit) * p.nh;
+    w.q0[s] = p.pair_heads ? block * p.rp : (NQ * block + s) * p.rp;
     w.lowest[s] = max(w.q0[s] + w.off, 0);
     w.highest[s] = w.q0[s] < w.nq ? min(w.q0[s] + p.rp, w.nq) - 1 + w.off : -1;
     if (w.highest[s] >= 0) low = min(low, w.lowest[s]), high = max(high, w.highest[s]);
   }
-  w.sink_tiles = w.first = w.tiles = 0;
+  w.sink_tiles = w.first = w.begin = w.tiles = 0;
   if (high >= 0) {
     if (p.window > 0) {
       w.first = max(0, low - p.window + 1) / kTileKeys;
@@ -166,15 +179,24 @@ __device__ __forceinline__ Work work_of(const WindowParams& p) {
     }
     w.tiles = w.sink_tiles + high / kTileKeys - w.first + 1;
   }
+  const int all = w.tiles;
+  w.begin = all * part / p.splits;
+  w.tiles = all * (part + 1) / p.splits - w.begin;
   return w;
 }
 
-template <int DPAD>
+template <int DPAD, int NQ>
 struct Layout {
   static constexpr int kBoxes = DPAD / 64, kBoxBytes = 128 * 128, kTileBytes = kBoxes * kBoxBytes;
-  static constexpr int kStages = DPAD == 128 ? 5 : 8;
-  static constexpr int kBars = 2 * kStages + 2 + 8 + 1;
-  static constexpr int kSmem = 1024 + (2 + kStages) * kTileBytes + kBars * 8 + 16;
+  static constexpr int kPerSm = NQ == 1 ? 2 : 1;
+  static constexpr int kStages = NQ == 2 ? (DPAD == 128 ? 5 : 8) : (DPAD == 128 ? 2 : 4);
+  static constexpr int kBars = 2 * kStages + NQ + 4 * NQ + 1;
+  static constexpr int kSmem = 1024 + (NQ + kStages) * kTileBytes + kBars * 8 + 16;
+  static constexpr int kAlone = NQ == 1 ? 120 * 1024 : kSmem;
+  static constexpr int kMmaWarp = 4 * NQ, kLoadWarp = kMmaWarp + 1, kThreads = 128 * (NQ + 1);
+  static constexpr int kTmemCols = 256 * NQ;       // S of each query tile, then O of each
+  // registers of a thread: 65536 / kPerSm for all; a softmax thread holds 128 scores
+  static constexpr int kSoftmaxRegs = NQ == 2 ? 192 : 184, kOtherRegs = NQ == 2 ? 120 : 72;
 };
 
 // One row over the keys that it sees, by one warp, four elements a lane: for rows that a masked key spoiled.
@@ -206,33 +228,85 @@ __device__ __noinline__ void row_again(const WindowParams& p, int b, int h, int 
   }
 }
 
-template <typename T, int DPAD>
-__global__ void __launch_bounds__(kThreads, 1)
+// The rows of this CTA from the parts of its cluster, by its first four warps: a warp takes 8 / SPLITS rows at once, so that eight loads are
+// on their way together.
+template <typename T, int DPAD, int SPLITS>
+__device__ __noinline__ void join_rows(const WindowParams& p, const float* part, const float2* part_ml, int b, int head, int q0, int nq, int off) {
+  constexpr int kRows = 8 / SPLITS, kPerWarp = kTileRows / SPLITS / 4;
+  const int lane = threadIdx.x & 31, first = static_cast<int>(ptx::cluster_ctarank()) * (kTileRows / SPLITS) + (threadIdx.x >> 5) * kPerWarp;
+  const int d = min(lane * 4, DPAD - 4);
+  const float sl = fmaxf(p.scale * 1.4426950408889634f, 1e-30f);
+  unsigned bad = 0;
+#pragma unroll 1
+  for (int r0 = 0; r0 < kPerWarp; r0 += kRows) {
+    float2 ml[kRows][SPLITS];
+    float4 o[kRows][SPLITS];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int k = 0; k < SPLITS; ++k) {
+        const int row = first + r0 + r;
+        ml[r][k] = ld_cluster_f2(part_ml + row, k);
+        o[r][k] = ld_cluster_f4(part + row * DPAD + (d ^ ((row & 7) * 4)), k);
+      }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const int row = first + r0 + r, h = head + row / p.rp, i = q0 + row % p.rp, at = i < nq ? i + off : -1;
+      float top = ml[r][0].x, l = 0.0f, y[4] = {};
+#pragma unroll
+      for (int k = 1; k < SPLITS; ++k) top = fmaxf(top, ml[r][k].x);
+      const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int k = 0; k < SPLITS; ++k) {
+        const float f = exp2_fast((ml[r][k].x - base) * sl);
+        l += ml[r][k].y * f;
+        y[0] += o[r][k].x * f, y[1] += o[r][k].y * f, y[2] += o[r][k].z * f, y[3] += o[r][k].w * f;
+      }
+      const float f = 1.0f / l;
+      float probe = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] *= f, probe = fmaf(y[e], 0.0f, probe);
+      if (__any_sync(0xffffffffu, lane * 4 < p.D && probe != probe) && at >= 0 && i < p.Sq) bad |= 1u << (r0 + r);
+      if (lane * 4 < p.D && i < p.Sq) {
+        uint2 u = make_uint2(0, 0);
+        if (at >= 0) u = make_uint2(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]));
+        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + b * p.o_s[0] + h * p.o_s[1] + static_cast<int64_t>(i) * p.o_s[2] + lane * 4) = u;
+      }
+    }
+  }
+  for (; bad; bad &= bad - 1) {
+    const int row = first + __ffs(bad) - 1, i = q0 + row % p.rp;
+    row_again<T>(p, b, head + row / p.rp, i, i + off);
+  }
+}
+
+template <typename T, int DPAD, int NQ>
+__global__ void __launch_bounds__(Layout<DPAD, NQ>::kThreads, Layout<DPAD, NQ>::kPerSm)
 window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
               const __grid_constant__ WindowParams p) {
-  using L = Layout<DPAD>;
+  using L = Layout<DPAD, NQ>;
   extern __shared__ char smem_raw[];
   char* const base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
   char* const sq = base;
-  char* const ring = base + 2 * L::kTileBytes;
+  char* const ring = base + NQ * L::kTileBytes;
   uint64_t* const bars = reinterpret_cast<uint64_t*>(ring + L::kStages * L::kTileBytes);
   uint64_t* const full = bars;
   uint64_t* const empty = bars + L::kStages;
   uint64_t* const q_full = empty + L::kStages;
-  uint64_t* const s_full = q_full + 2;
-  uint64_t* const p_full = s_full + 2;
-  uint64_t* const p_half = p_full + 2;
-  uint64_t* const o_full = p_half + 2;
-  uint64_t* const done = o_full + 2;
+  uint64_t* const s_full = q_full + NQ;
+  uint64_t* const p_full = s_full + NQ;
+  uint64_t* const p_half = p_full + NQ;
+  uint64_t* const o_full = p_half + NQ;
+  uint64_t* const done = o_full + NQ;
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (warp == 8) {
-    ptx::tmem_alloc<1>(tmem_slot, kTmemCols);
+  if (warp == L::kMmaWarp) {
+    ptx::tmem_alloc<1>(tmem_slot, L::kTmemCols);
     ptx::tmem_relinquish<1>();
   } else if (threadIdx.x == 0) {
-    for (int i = 0; i < 2 * L::kStages + 2; ++i) ptx::mbar_init(bars + i, 1);
-    for (int s = 0; s < 2; ++s) ptx::mbar_init(s_full + s, 1), ptx::mbar_init(p_full + s, 4), ptx::mbar_init(p_half + s, 4), ptx::mbar_init(o_full + s, 1);
+    for (int i = 0; i < 2 * L::kStages + NQ; ++i) ptx::mbar_init(bars + i, 1);
+    for (int s = 0; s < NQ; ++s) ptx::mbar_init(s_full + s, 1), ptx::mbar_init(p_full + s, 4), ptx::mbar_init(p_half + s, 4), ptx::mbar_init(o_full + s, 1);
     ptx::mbar_init(done, 1);
     ptx::fence_barrier_init();
     ptx::prefetch_tmap(&tq);
@@ -245,11 +319,11 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents();
   pdl_wait();
-  const Work w = work_of(p);
+  const Work<NQ> w = work_of<NQ>(p);
 
-  if (warp >= 8) {
-    ptx::setmaxnreg_dec<120>();                    // 128 x 120 + 256 x 192 = 384 x 168, what the CTA was launched with
-    if (warp == 9) {
+  if (warp >= L::kMmaWarp) {
+    ptx::setmaxnreg_dec<L::kOtherRegs>();          // two query tiles: 128 x 120 + 256 x 192 = 384 x 168, one: 128 x (72 + 184) = 256 x 128, as launched
+    if (warp == L::kLoadWarp) {
     // ------------------------------------------------------------- loads
     if (lane == 0 && w.tiles > 0) {
       auto load_q = [&](int s, int q0, int head) {
@@ -271,16 +345,16 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           ptx::mbar_arrive_expect_tx(full + st, L::kTileBytes);
           for (int x = 0; x < L::kBoxes; ++x)
             tma_load_4d(ring + st * L::kTileBytes + x * L::kBoxBytes, kv == 0 ? &tk : &tv, full + st, x * 64, row, w.kv_head, w.b);
-          if (++issued == 1) load_q(1, w.q0[1], w.head[1]);      // the first product waits for the first query tile and the first keys
+          if (++issued == 1 && NQ == 2) load_q(1, w.q0[NQ - 1], w.head[NQ - 1]);      // the first product waits for the first query tile and the first keys
           if (++st == L::kStages) st = 0, ph ^= 1u;
         }
       }
       // no copy may be under way when the CTA ends, whatever became of its readers
-      if (!ptx::mbar_wait(q_full, 0) || (issued > 0 && !ptx::mbar_wait(q_full + 1, 0))) timed_out(p.status, 81);
+      if (!ptx::mbar_wait(q_full, 0) || (NQ == 2 && issued > 0 && !ptx::mbar_wait(q_full + 1, 0))) timed_out(p.status, 81);
       for (int i = max(0, issued - L::kStages); i < issued; ++i)
         if (!ptx::mbar_wait(full + i % L::kStages, (i / L::kStages) & 1)) timed_out(p.status, 81);
     }
-  } else if (warp == 8) {
+  } else if (warp == L::kMmaWarp) {
     // ------------------------------------------------------------- products
     // The warp walks the loop together, so that barriers, phases and descriptors stay in uniform registers; one lane issues.
     if (w.tiles > 0) {
@@ -293,8 +367,8 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       const uint32_t ring_lo = (ptx::smem_u32(ring) >> 4) & 0x3fffu, q_lo = ptx::desc_lo_sw128(ptx::smem_u32(sq));
       const bool leader = elect_one();
       bool ok = true;
-      uint32_t p_phase[2] = {0, 0};
-      bool waiting[2] = {false, false}, begun[2] = {false, false};   // a P that is to be multiplied; O holds something
+      uint32_t p_phase[NQ] = {};
+      bool waiting[NQ] = {}, begun[NQ] = {};   // a P that is to be multiplied; O holds something
       int stage = 0, v_stage = 0;                                    // of this tile's K; of the V of the tile before
       uint32_t phase = 0, v_phase = 0;
       for (int j = 0; j <= w.tiles && ok; ++j) {
@@ -310,7 +384,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         ptx::tc_fence_after();
         const uint32_t v_lo = (ring_lo + v_stage * (L::kTileBytes >> 4)) | kLeadV, k_lo = (ring_lo + stage * (L::kTileBytes >> 4)) | (1u << 16);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < NQ; ++s) {
           if (waiting[s]) {
             // the first half of the keys as soon as it is there
 #pragma unroll
@@ -320,7 +394,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
               if (leader) {
 #pragma unroll
                 for (int k = 0; k < kTileKeys / 32; ++k)
-                  mma_ts(tmem + 256 + s * 128, tmem + s * 128 + half * 32 + k * 8, ptx::desc_join(v_lo + (half * 4 + k) * (2048 >> 4), kHiV), id_o,
+                  mma_ts(tmem + (NQ + s) * 128, tmem + s * 128 + half * 32 + k * 8, ptx::desc_join(v_lo + (half * 4 + k) * (2048 >> 4), kHiV), id_o,
                          half > 0 || k > 0 ? 1u : (begun[s] ? 1u : 0u));
               }
               __syncwarp();
@@ -369,12 +443,12 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     }
   } else {
     // ------------------------------------------------------------- softmax of query tile s, one thread to a row
-    ptx::setmaxnreg_inc<192>();
-    const int s = warp >> 2, r = threadIdx.x & 127;
+    ptx::setmaxnreg_inc<L::kSoftmaxRegs>();
+    const int s = NQ == 1 ? 0 : warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;     // this warp's 32 lanes of tensor memory
-    const uint32_t ts = tmem + s * 128 + lanes, to = tmem + 256 + s * 128 + lanes;
-    const int q0 = s ? w.q0[1] : w.q0[0], lowest = s ? w.lowest[1] : w.lowest[0], highest = s ? w.highest[1] : w.highest[0];
-    const int h = (s ? w.head[1] : w.head[0]) + r / p.rp, i = q0 + r % p.rp;
+    const uint32_t ts = tmem + s * 128 + lanes, to = tmem + (NQ + s) * 128 + lanes;
+    const int q0 = s ? w.q0[NQ - 1] : w.q0[0], lowest = s ? w.lowest[NQ - 1] : w.lowest[0], highest = s ? w.highest[NQ - 1] : w.highest[0];
+    const int h = (s ? w.head[NQ - 1] : w.head[0]) + r / p.rp, i = q0 + r % p.rp;
     const int at = i < w.nq ? i + w.off : -1;                         // position; < 0: sees nothing
     const float sl = fmaxf(p.scale * 1.4426950408889634f, 1e-30f);    // 0 times a masked -inf would be NaN
     const uint64_t sl2 = pack2(sl, sl);
@@ -474,6 +548,22 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     }
     if (ok) {
       ptx::tc_fence_after();
+      if (NQ == 1 && p.splits > 1) {
+        // this CTA's part of the row: O, referred to m, over the ring (its last tile has been read); m and l over the queries
+        float* const rows = reinterpret_cast<float*>(ring) + r * DPAD;
+        reinterpret_cast<float2*>(sq)[r] = make_float2(m, l);
+#pragma unroll
+        for (int c = 0; c < DPAD / 32; ++c) {
+          uint32_t o[32] = {};
+          if (begun) {
+            ptx::tmem_ld_32x32(to + c * 32, o);
+            ptx::tmem_ld_wait();
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)            // pieces of 16 bytes turned by the row: 32 rows in one instruction
+            *reinterpret_cast<uint4*>(rows + ((c * 32 + e) ^ ((r & 7) * 4))) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      } else {
       const float f = 1.0f / l;
       float probe = 0.0f;
       // Through the place of this tile's queries, which no product reads any more: a thread has a whole row, and 32 rows' pieces of 16 bytes
@@ -519,13 +609,28 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         const int who = __ffs(bad) - 1;
         row_again<T>(p, w.b, __shfl_sync(0xffffffffu, h, who), __shfl_sync(0xffffffffu, i, who), __shfl_sync(0xffffffffu, at, who));
       }
+      }
     }
+  }
+  if (NQ == 1 && p.splits > 1) {
+    // ------------------------------------------------------------- the parts of a cluster together: each CTA some of the rows, a warp a row
+    __syncwarp();
+    ptx::cluster_sync();
+    if (warp < 4) {
+      const float* const o = reinterpret_cast<const float*>(ring);
+      const float2* const ml = reinterpret_cast<const float2*>(sq);
+      if (p.splits == 2) join_rows<T, DPAD, 2>(p, o, ml, w.b, w.head[0], w.q0[0], w.nq, w.off);
+      else if (p.splits == 4) join_rows<T, DPAD, 4>(p, o, ml, w.b, w.head[0], w.q0[0], w.nq, w.off);
+      else join_rows<T, DPAD, 8>(p, o, ml, w.b, w.head[0], w.q0[0], w.nq, w.off);
+    }
+    __syncwarp();
+    ptx::cluster_sync();                          // nobody leaves while its part may still be read
   }
   ptx::tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == L::kMmaWarp) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc<1>(tmem, kTmemCols);
+    ptx::tmem_dealloc<1>(tmem, L::kTmemCols);
   }
 }
 
@@ -544,18 +649,84 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int64_t D, int64_t r
   return r == CUDA_SUCCESS ? B200Q_OK : B200Q_ERR_CUDA;
 }
 
-template <typename T, int DPAD>
+// Query tiles of a CTA and CTAs that share an item's keys.
+//
+// Two query tiles keep the tensor cores busy on their own and read K and V once for 256 rows; one query tile, two CTAs to an SM,
+// hides start and end of a CTA behind its neighbour and wastes fewer rows and keys; splitting an item's keys over a cluster shortens the chain
+// of its tiles where there are few items.  The costs in us are fitted to 190 shapes (1 to 8 sequences, groups of 1, 4 and 8, D 64 and
+// 128, 61 to 4096 queries, 61 to 16000 keys, windows of 256, 1024 and none), one / two query tiles measured: 4096 queries without a window,
+// 32 / 8 heads of 128 135 / 124, window 256 52 / 51, 12 / 12 heads of 64 x 8 sequences window 256 111 / 126; 300 queries of 4000 keys, 12 / 12
+// heads x 8 84 / 116 (288 and 192 items on 296 and 148 places); 61 queries of 16000 keys, 32 / 8 heads 204 / 210, split over 8 CTAs 43;
+// of 1999 keys behind a window of 1024 20.3 / 21.9, split 14.5.
+struct Shape {
+  int nq, splits;
+};
+int64_t blocks_of(const WindowParams& p, int nq) {
+  const int rows = nq == 2 && p.group % (2 * p.nh) != 0 ? 2 * p.rp : p.rp;
+  return (p.Sq + rows - 1) / rows;
+}
+Shape choose_shape(const WindowParams& p) {
+  const int sms = sm_count();
+  const bool narrow = p.D <= 64, pairs = p.group % (2 * p.nh) == 0;
+  const double items1 = static_cast<double>(blocks_of(p, 1)) * p.B * p.Hkv * (p.group / p.nh);
+  const double items2 = static_cast<double>(blocks_of(p, 2)) * p.B * p.Hkv * (p.group / (pairs ? 2 * p.nh : p.nh));
+  // key tiles of a query tile, on average
+  double keys = p.Sk - 0.5 * p.Sq;
+  if (keys < 1.0) keys = 1.0;
+  if (p.window > 0 && static_cast<double>(p.window) + p.rp + p.sinks < keys) keys = static_cast<double>(p.window) + p.rp + p.sinks;
+  const double tiles1 = keys / kTileKeys + 0.5, tiles2 = tiles1 + (pairs ? 0.0 : static_cast<double>(p.rp) / kTileKeys);
+  auto rounds = [](double x) { return x <= 1.0 ? 1.0 : (x <= 2.0 ? 2.0 : (x <= 3.0 ? 3.0 : x + 0.5)); };
+  Shape best{2, 1};
+  double least = rounds(items2 / sms) * ((narrow ? 7.7 : 8.0) + (narrow ? 1.4 : 1.75) * tiles2);
+  for (int k = 1; k <= 8; k *= 2) {
+    const double ctas = items1 * k;
+    if (k > 1 && ctas > 1.75 * sms) break;       // a cluster that has to wait for its places gains nothing
+    const double tile = ctas <= sms ? (narrow ? 1.4 : 1.6) : (narrow ? 1.55 : 2.1), join = k == 1 ? 0.0 : (k == 2 ? 5.5 : (k == 4 ? 3.6 : 2.8));
+    const double mine = tiles1 / k < 1.0 ? 1.0 : tiles1 / k;
+    const double cost = rounds(ctas / (2 * sms)) * ((narrow ? 6.3 : 7.5) + tile * mine) + join;
+    if (cost < least) least = cost, best = Shape{1, k};
+  }
+  return best;
+}
+
+template <typename T, int DPAD, int NQ>
 int launch_window(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const WindowParams& p, unsigned ctas, cudaStream_t st) {
-  auto kernel = window_kernel<T, DPAD>;
+  using L = Layout<DPAD, NQ>;
+  auto kernel = window_kernel<T, DPAD, NQ>;
   static std::atomic<bool> ready[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return B200Q_ERR_CUDA;
   if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DPAD>::kSmem) != cudaSuccess) return B200Q_ERR_CUDA;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlone) != cudaSuccess) return B200Q_ERR_CUDA;
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
   }
-  if (launch_pdl(kernel, dim3(ctas), dim3(kThreads), Layout<DPAD>::kSmem, st, tq, tk, tv, p) != cudaSuccess) return B200Q_ERR_CUDA;
+  // CTAs of a programmatic launch pile up on the SMs that the kernel in front left first: where one to an SM is enough, more shared
+  // memory than two of them can have
+  const int smem = NQ == 1 && p.splits == 1 && ctas <= static_cast<unsigned>(sm_count()) ? L::kAlone : L::kSmem;
+  if (NQ == 2 || p.splits == 1) {
+    if (launch_pdl(kernel, dim3(ctas), dim3(L::kThreads), smem, st, tq, tk, tv, p) != cudaSuccess) return B200Q_ERR_CUDA;
+    return check_launch();
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(L::kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(p.splits), attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, tq, tk, tv, p) != cudaSuccess) return B200Q_ERR_CUDA;
   return check_launch();
+}
+
+template <typename T>
+int launch_window_n(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const WindowParams& p, int nq, unsigned ctas, cudaStream_t st) {
+  if (p.D <= 64) return nq == 2 ? launch_window<T, 64, 2>(tq, tk, tv, p, ctas, st) : launch_window<T, 64, 1>(tq, tk, tv, p, ctas, st);
+  return nq == 2 ? launch_window<T, 128, 2>(tq, tk, tv, p, ctas, st) : launch_window<T, 128, 1>(tq, tk, tv, p, ctas, st);
 }
 
 }  // namespace
@@ -595,11 +766,12 @@ int b200q_window_attention(const void* q, const void* k, const void* v, int dtyp
   // few queries: the rows of several heads of a group in one tile
   p.rp = kTileRows, p.nh = 1;
   while (p.rp > 8 && Sq <= p.rp / 2 && p.group % (2 * p.nh) == 0) p.rp /= 2, p.nh *= 2;
-  p.pair_heads = p.group % (2 * p.nh) == 0 ? 1 : 0;
+  const Shape shape = choose_shape(p);
+  p.pair_heads = shape.nq == 2 && p.group % (2 * p.nh) == 0 ? 1 : 0;
   p.units = p.group / (p.pair_heads ? 2 * p.nh : p.nh);
-  const int rows = p.pair_heads ? p.rp : 2 * p.rp;
-  p.q_blocks = static_cast<int>((Sq + rows - 1) / rows);
-  const int64_t ctas = static_cast<int64_t>(p.q_blocks) * B * Hkv * p.units;
+  p.q_blocks = static_cast<int>(blocks_of(p, shape.nq));
+  p.splits = shape.splits;
+  const int64_t ctas = static_cast<int64_t>(p.q_blocks) * B * Hkv * p.units * p.splits;
   if (ctas > 0x7fffffffLL) return B200Q_ERR_INVALID;
   CUtensorMap tq, tk, tv;
   if (int rc = make_map(&tq, q, dtype, D, Sq, Hq, B, strides, p.rp, p.nh)) return rc;
@@ -608,8 +780,7 @@ int b200q_window_attention(const void* q, const void* k, const void* v, int dtyp
   if (int rc = make_map(&tv, Sk > 0 ? v : q, dtype, D, Sk > 0 ? Sk : Sq, Sk > 0 ? Hkv : Hq, B, Sk > 0 ? strides + 6 : strides, kTileKeys, 1)) return rc;
   const auto st = static_cast<cudaStream_t>(stream);
   const auto n = static_cast<unsigned>(ctas);
-  if (dtype == B200Q_BF16) return D <= 64 ? launch_window<__nv_bfloat16, 64>(tq, tk, tv, p, n, st) : launch_window<__nv_bfloat16, 128>(tq, tk, tv, p, n, st);
-  return D <= 64 ? launch_window<__half, 64>(tq, tk, tv, p, n, st) : launch_window<__half, 128>(tq, tk, tv, p, n, st);
+  return dtype == B200Q_BF16 ? launch_window_n<__nv_bfloat16>(tq, tk, tv, p, shape.nq, n, st) : launch_window_n<__half>(tq, tk, tv, p, shape.nq, n, st);
 }
 
 }  // extern "C"
