@@ -23,45 +23,74 @@ __device__ __forceinline__ int ld_i32(const int32_t* p) {
   return v;
 }
 
-// One thread per 16 elements of a row of K or V.
+// The pages of a CTA's tokens are found first, a warp to a token; then its threads move 16 elements of K and of V at a time, several at once.
+// Bound by the memory for prompts, by three loads that wait for one another (lengths, table, rows) for a decode step.
+constexpr int kAppendThreads = 256, kAppendTokens = 64, kAppendAtOnce = 4;
+
 template <typename T, bool CODES>
-__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
-  const int parts = p.c.D / 16, per_token = p.c.heads * parts;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= p.T * per_token * 2) return;
-  const int part = static_cast<int>(at % parts);
-  const int head = static_cast<int>(at / parts % p.c.heads);
-  const bool is_v = (at / per_token) & 1;
-  const int64_t t = at / per_token / 2;
-  int b, i, fresh;
-  if (p.cu_new == nullptr) {
-    b = static_cast<int>(t), i = 0, fresh = 1;
-  } else {
-    int lo = 0, hi = p.B;                       // cu_new[lo] <= t < cu_new[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (ld_i32(p.cu_new + mid) <= t) lo = mid; else hi = mid;
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p, int tokens) {
+  __shared__ int2 place[kAppendTokens];       // page (-1: none) and row
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * tokens;
+  const int here = static_cast<int>(p.T - first < tokens ? p.T - first : tokens);
+  pdl_launch_dependents();
+  pdl_wait();
+  for (int i = tid >> 5; i < here; i += kAppendThreads / 32) {
+    const int64_t t = first + i;
+    int b = static_cast<int>(t), at = 0, fresh = 1;
+    if (p.cu_new != nullptr) {                // the last sequence that begins at or before the token, 32 candidates a step
+      int lo = 0, span = p.B;                 // cu_new[lo] <= t, and the sequence is one of lo .. lo + span - 1
+      while (span > 1) {
+        const int step = (span + 31) / 32, probe = lo + lane * step;
+        const unsigned below = __ballot_sync(0xffffffffu, lane * step < span && ld_i32(p.cu_new + min(probe, p.B)) <= t);
+        const int last = 31 - __clz(below | 1u);
+        span = min(step, span - last * step);
+        lo += last * step;
+      }
+      b = lo;
+      const int begin = ld_i32(p.cu_new + lo);
+      at = static_cast<int>(t - begin), fresh = ld_i32(p.cu_new + lo + 1) - begin;
     }
-    b = lo;
-    const int first = ld_i32(p.cu_new + lo);
-    i = static_cast<int>(t - first), fresh = ld_i32(p.cu_new + lo + 1) - first;
+    const int64_t token = static_cast<int64_t>(ld_i32(p.c.lens + b)) - fresh + at;
+    if (lane == 0) {
+      int2 found = make_int2(-1, 0);
+      if (token >= 0 && token < p.c.capacity)
+        found = make_int2(paged::page_of(p.c.table + b * p.c.table_stride, static_cast<int>(token), p.c), static_cast<int>(token % p.c.page_size));
+      place[i] = found;
+    }
   }
-  const int64_t token = static_cast<int64_t>(ld_i32(p.c.lens + b)) - fresh + i;
-  if (token < 0 || token >= p.c.capacity) return;
-  const int page = paged::page_of(p.c.table + b * p.c.table_stride, static_cast<int>(token), p.c);
-  if (page < 0) return;
-  const char* src = is_v ? p.v + t * p.v_token + head * p.v_head : p.k + t * p.k_token + head * p.k_head;
-  char* dst = paged::row_at(is_v ? p.c.v : p.c.k, page, head, static_cast<int>(token % p.c.page_size));
-  Raw16<T, false> raw;
-  raw.load(reinterpret_cast<const T*>(src) + part * 16);
-  if constexpr (CODES) {
-    const float scale = paged::head_scale(is_v ? p.c.v_amax : p.c.k_amax, p.c.amax_stride, head);
-    *reinterpret_cast<uint4*>(dst + part * 16) =
-        e4m3_of_16(raw, scale, __frcp_rn(scale), scale * 512.0f, b200q_div_fast_ok(scale));
-  } else {
-    uint4* d = reinterpret_cast<uint4*>(dst + part * 32);
-    d[0] = make_uint4(raw.w[0].v[0], raw.w[0].v[1], raw.w[0].v[2], raw.w[0].v[3]);
-    d[1] = make_uint4(raw.w[0].v[4], raw.w[0].v[5], raw.w[0].v[6], raw.w[0].v[7]);
+  __syncthreads();
+  const int parts = p.c.D / 16, per_token = p.c.heads * parts, all = here * per_token;
+  for (int base = tid; base < all; base += kAppendThreads * kAppendAtOnce) {
+    Raw16<T, false> kr[kAppendAtOnce], vr[kAppendAtOnce];
+    int head[kAppendAtOnce], part[kAppendAtOnce];
+    int2 to[kAppendAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAppendAtOnce; ++u) {
+      const int i = base + u * kAppendThreads, token = i / per_token, rest = i - token * per_token;
+      head[u] = rest / parts, part[u] = rest - head[u] * parts;
+      to[u] = i < all ? place[token] : make_int2(-1, 0);
+      if (to[u].x < 0) continue;
+      kr[u].load(reinterpret_cast<const T*>(p.k + (first + token) * p.k_token + head[u] * p.k_head) + part[u] * 16);
+      vr[u].load(reinterpret_cast<const T*>(p.v + (first + token) * p.v_token + head[u] * p.v_head) + part[u] * 16);
+    }
+#pragma unroll
+    for (int u = 0; u < kAppendAtOnce; ++u) {
+      if (to[u].x < 0) continue;
+      char* const kd = paged::row_at(p.c.k, to[u].x, head[u], to[u].y);
+      char* const vd = paged::row_at(p.c.v, to[u].x, head[u], to[u].y);
+      if constexpr (CODES) {
+        const float ks = paged::head_scale(p.c.k_amax, p.c.amax_stride, head[u]), vs = paged::head_scale(p.c.v_amax, p.c.amax_stride, head[u]);
+        *reinterpret_cast<uint4*>(kd + part[u] * 16) = e4m3_of_16(kr[u], ks, __frcp_rn(ks), ks * 512.0f, b200q_div_fast_ok(ks));
+        *reinterpret_cast<uint4*>(vd + part[u] * 16) = e4m3_of_16(vr[u], vs, __frcp_rn(vs), vs * 512.0f, b200q_div_fast_ok(vs));
+      } else {
+        uint4* const k4 = reinterpret_cast<uint4*>(kd + part[u] * 32);
+        uint4* const v4 = reinterpret_cast<uint4*>(vd + part[u] * 32);
+        const U32x8 &kw = kr[u].w[0], &vw = vr[u].w[0];
+        k4[0] = make_uint4(kw.v[0], kw.v[1], kw.v[2], kw.v[3]), k4[1] = make_uint4(kw.v[4], kw.v[5], kw.v[6], kw.v[7]);
+        v4[0] = make_uint4(vw.v[0], vw.v[1], vw.v[2], vw.v[3]), v4[1] = make_uint4(vw.v[4], vw.v[5], vw.v[6], vw.v[7]);
+      }
+    }
   }
 }
 
@@ -304,8 +333,6 @@ int b200q_paged_append(const void* k, const void* v, int dtype, const int64_t* s
   if (T == 0 || table_width == 0) return B200Q_OK;
   if (k == nullptr || v == nullptr || strides == nullptr) return B200Q_ERR_INVALID;
   if (!aligned(k, 16) || !aligned(v, 16) || !paged::strides_ok(strides, 4, 8)) return B200Q_ERR_ALIGN;
-  const int64_t threads = T * p.c.heads * (p.c.D / 16) * 2, blocks = (threads + 255) / 256;
-  if (blocks > 0x7fffffffLL) return B200Q_ERR_INVALID;
   if (int rc = check_arch()) return rc;
   p.k = static_cast<const char*>(k);
   p.v = static_cast<const char*>(v);
@@ -314,14 +341,17 @@ int b200q_paged_append(const void* k, const void* v, int dtype, const int64_t* s
   p.T = T;
   p.B = static_cast<int>(B);
   const auto st = static_cast<cudaStream_t>(stream);
-  const auto n = static_cast<unsigned>(blocks);
+  // tokens of a CTA: what keeps its threads busy once, fewer where that leaves SMs without a CTA
+  const int64_t pieces = static_cast<int64_t>(p.c.heads) * (p.c.D / 16), fill = kAppendThreads * kAppendAtOnce / pieces, spread = T / (2 * sm_count());
+  int64_t tokens = fill < spread ? fill : spread;
+  tokens = tokens < 1 ? 1 : (tokens > kAppendTokens ? kAppendTokens : tokens);
+  const dim3 grid(static_cast<unsigned>((T + tokens - 1) / tokens)), block(kAppendThreads);
+  const int n = static_cast<int>(tokens);
   const bool half = dtype == B200Q_F16;
-  if (p.c.codes) {
-    if (half) append_kernel<__half, true><<<n, 256, 0, st>>>(p); else append_kernel<__nv_bfloat16, true><<<n, 256, 0, st>>>(p);
-  } else {
-    if (half) append_kernel<__half, false><<<n, 256, 0, st>>>(p); else append_kernel<__nv_bfloat16, false><<<n, 256, 0, st>>>(p);
-  }
-  return check_launch();
+  cudaError_t e;
+  if (p.c.codes) e = half ? launch_pdl(append_kernel<__half, true>, grid, block, 0, st, p, n) : launch_pdl(append_kernel<__nv_bfloat16, true>, grid, block, 0, st, p, n);
+  else e = half ? launch_pdl(append_kernel<__half, false>, grid, block, 0, st, p, n) : launch_pdl(append_kernel<__nv_bfloat16, false>, grid, block, 0, st, p, n);
+  return e == cudaSuccess ? check_launch() : B200Q_ERR_CUDA;
 }
 
 int b200q_paged_evict(const b200q_paged_cache* cache, const int32_t* block_table, int64_t table_stride, int64_t table_width,
