@@ -7,6 +7,7 @@
     tensorrt_b200.Nvfp4Linear.from_float(linear)(x)                         # real-quant NVFP4 GEMM path
     tensorrt_b200.fuse_quantized_linear(graph_module)                       # Q/DQ-wrapped linears -> GEMM nodes
     tensorrt_b200.fuse_gated_mlp(graph_module)                              # silu(gate(x)) * up(x) -> one GEMM
+    tensorrt_b200.CachedDecoder(stack, tensorrt_b200.PagedKvCache(..))      # prompts and single tokens over a paged key-value cache
 
 Only CUDA (compute capability 10.x) is implemented; there is no CPU or other-GPU fallback.
 """
@@ -16,9 +17,9 @@ from .ops import load_ops, ops_loaded  # noqa: F401
 from .linear import Fp8GatedMlp, Fp8Linear, Nvfp4Linear, QuantizedLinear, fp8_linear, nvfp4_linear  # noqa: F401
 from .plugin import register_with_torch_tensorrt  # noqa: F401
 from .fx_passes import fuse_all_reduce_wait, fuse_fp8_sdpa, fuse_gated_mlp, fuse_quantized_linear  # noqa: F401
-from .kv_cache import paged_append, paged_attention, paged_evict, window_attention  # noqa: F401
+from .kv_cache import CachedDecoder, PagedKvCache, paged_append, paged_attention, paged_evict, window_attention  # noqa: F401
 
-__all__ = ["paged_append", "paged_attention", "paged_evict", "window_attention", "capi", "B200QError", "load_library", "load_ops", "ops_loaded", "Fp8GatedMlp", "Fp8Linear", "Nvfp4Linear",
+__all__ = ["CachedDecoder", "PagedKvCache", "paged_append", "paged_attention", "paged_evict", "window_attention", "capi", "B200QError", "load_library", "load_ops", "ops_loaded", "Fp8GatedMlp", "Fp8Linear", "Nvfp4Linear",
            "QuantizedLinear", "fp8_linear", "nvfp4_linear", "register_with_torch_tensorrt", "fuse_quantized_linear", "fuse_all_reduce_wait", "fuse_fp8_sdpa", "fuse_gated_mlp"]
 
 load_ops()

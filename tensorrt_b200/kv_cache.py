@@ -61,3 +61,183 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale
     args = (q, k, v, q_lens, k_lens, 0.0 if scale is None else scale, window, sinks)
     out = _native.window_attention(*args)
     return _window(*args) if out is None else out
+
+
+class PagedKvCache:
+    """The pages of a batch of sequences for every layer of a decoder, and the calls above on them.
+
+    Page p of a sequence is the same page number in every layer; the pools, [pages, kv heads, page_size, head_dim] each, are allocated
+    once.  Pages are handed out on the host: `grow` before the layers of a step, with the number of new tokens of each sequence, then
+    `append` and `attend` (or `attend_prompt`) once a layer.  Inside a captured CUDA graph only these two belong; `grow` outside it,
+    and a graph that is replayed on a fixed table needs the pages of its whole run reserved in front (`reserve`).
+
+    dtype bfloat16 or float16 as the tokens are, or float8_e4m3fn with `k_amax`, `v_amax`: per layer one value or one per kv head.
+    `weights` True keeps the sums of attention weights by which `evict` chooses."""
+
+    def __init__(self, layers: int, batch: int, n_kv: int, head_dim: int, pages: int, max_tokens: int, page_size: int = 16, dtype=torch.bfloat16,
+                 k_amax=None, v_amax=None, weights: bool = False, device="cuda"):
+        if page_size < 1 or pages < 1 or max_tokens < 1:
+            raise ValueError("pages, their rows and the tokens of a sequence must be at least one")
+        if dtype not in (torch.bfloat16, torch.float16, torch.float8_e4m3fn):
+            raise ValueError(f"received pages of {dtype} type. Supported types: float16 | bfloat16 | float8_e4m3fn")
+        if (dtype == torch.float8_e4m3fn) != (k_amax is not None) or (k_amax is None) != (v_amax is None):
+            raise ValueError("FP8 pages need k_amax and v_amax of every layer, other pages take none")
+        self.layers, self.batch, self.page_size, self.max_tokens = layers, batch, page_size, max_tokens
+        self.n_kv, self.head_dim = n_kv, head_dim
+        self.k_amax, self.v_amax = k_amax or [None] * layers, v_amax or [None] * layers
+        shape = (pages, n_kv, page_size, head_dim)
+        self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
+        self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
+        width = -(-max_tokens // page_size)
+        self.table = torch.full((batch, width), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.weights = [torch.zeros(batch, n_kv, max_tokens, device=device) for _ in range(layers)] if weights else [None] * layers
+        self._free = list(range(pages - 1, -1, -1))
+        self._pages: list = [[] for _ in range(batch)]     # of each sequence, in order
+        self._tokens = [0] * batch
+        self._new, self._cu = [0] * batch, None
+
+    def tokens(self) -> list:
+        """Tokens of each sequence."""
+        return list(self._tokens)
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def reserve(self, tokens: list) -> None:
+        """Pages for sequences of up to `tokens[b]` tokens."""
+        if len(tokens) != self.batch or any(n > self.max_tokens for n in tokens):
+            raise ValueError(f"expected {self.batch} counts of up to {self.max_tokens} tokens, got {tokens}")
+        need = [max(0, -(-n // self.page_size) - len(p)) for n, p in zip(tokens, self._pages)]
+        if sum(need) > len(self._free):
+            raise RuntimeError(f"{sum(need)} pages are needed and {len(self._free)} are free")
+        rows, cols, vals = [], [], []
+        for b, n in enumerate(need):
+            for _ in range(n):
+                rows.append(b), cols.append(len(self._pages[b])), vals.append(self._free.pop())
+                self._pages[b].append(vals[-1])
+        if vals:
+            at = torch.tensor([rows, cols, vals], device=self.table.device)
+            self.table[at[0], at[1]] = at[2].int()
+
+    def grow(self, new: list) -> None:
+        """Makes room for new[b] tokens of sequence b; the next `append` of every layer brings them."""
+        if len(new) != self.batch or any(n < 0 for n in new):
+            raise ValueError(f"expected {self.batch} counts of new tokens, got {new}")
+        self.reserve([t + n for t, n in zip(self._tokens, new)])
+        self._tokens = [t + n for t, n in zip(self._tokens, new)]
+        self._new = list(new)
+        if all(n == 1 for n in new):
+            self._cu = None
+            self.lens += 1
+        else:
+            at = torch.tensor([0] + list(new), dtype=torch.int32)
+            self._cu = at.cumsum(0).to(torch.int32).to(self.lens.device)
+            self.lens += at[1:].to(self.lens.device)
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """K and V rows [tokens, kv heads, head_dim] of the tokens that `grow` made room for, sequence after sequence."""
+        paged_append(k, v, self.k[layer], self.v[layer], self.table, self.lens, self._cu, k_amax=self.k_amax[layer], v_amax=self.v_amax[layer])
+
+    def attend(self, layer: int, q: torch.Tensor, *, scale: float | None = None, window: int = 0, sinks: int = 0) -> torch.Tensor:
+        """Attention of the newest token of every sequence: q [batch, query heads, head_dim]."""
+        return paged_attention(q, self.k[layer], self.v[layer], self.table, self.lens, k_amax=self.k_amax[layer], v_amax=self.v_amax[layer],
+                               weights=self.weights[layer], scale=scale, window=window, sinks=sinks)
+
+    def attend_prompt(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None, window: int = 0,
+                      sinks: int = 0) -> torch.Tensor:
+        """Attention of the tokens of whole prompts over themselves: q, k, v [tokens, heads, head_dim], sequence after sequence ->
+        [tokens, query heads, head_dim].  Every sequence's tokens must be new ones."""
+        if self._new != self._tokens:
+            raise ValueError("prompts are attended to as a whole: sequences must hold no tokens but the new ones")
+        most = max(self._new)
+        if all(n == most for n in self._new):
+            rows = lambda t: t.unflatten(0, (self.batch, most)).transpose(1, 2)  # noqa: E731
+            return window_attention(rows(q), rows(k), rows(v), scale=scale, window=window, sinks=sinks).transpose(1, 2).flatten(0, 1)
+        lens = torch.tensor(self._new, dtype=torch.int32, device=q.device)
+        there = torch.arange(most, device=q.device) < lens[:, None]
+
+        def rows(t):
+            out = t.new_zeros(self.batch, most, *t.shape[1:])
+            out[there] = t
+            return out.transpose(1, 2)
+
+        return window_attention(rows(q), rows(k), rows(v), scale=scale, window=window, sinks=sinks, q_lens=lens, k_lens=lens).transpose(1, 2)[there]
+
+    def evict(self, keep: int, recent: int = 0, sinks: int = 0) -> list:
+        """Cuts every sequence to `keep` tokens per kv head, by the sums of attention weights of each layer, and frees the pages they
+        were in.  -> the kept tokens of every layer, int32 [batch, kv heads, keep]."""
+        if self.weights[0] is None:
+            raise ValueError("eviction goes by attention weights: the cache was made with weights=False")
+        width = -(-keep // self.page_size)
+        if width * self.batch > len(self._free):
+            raise RuntimeError(f"{width * self.batch} pages are needed and {len(self._free)} are free")
+        fresh = [[self._free.pop() for _ in range(-(-min(keep, t) // self.page_size))] for t in self._tokens]
+        out = torch.tensor([p + [-1] * (max(width, 1) - len(p)) for p in fresh], dtype=torch.int32, device=self.table.device)
+        kept = []
+        for layer in range(self.layers):
+            which, lens, left = paged_evict(self.k[layer], self.v[layer], self.table, self.lens, self.weights[layer], out, keep=keep,
+                                            recent=recent, sinks=sinks)
+            self.weights[layer].copy_(left)      # in place, as the table and the lengths: a captured step reads them where they are
+            kept.append(which)
+        self.lens.copy_(lens)
+        self.table.fill_(-1)
+        self.table[:, :width] = out[:, :width]
+        for old in self._pages:
+            self._free.extend(old)
+        self._pages, self._tokens = fresh, [min(keep, t) for t in self._tokens]
+        self._new = [0] * self.batch
+        return kept
+
+    def release(self, b: int) -> None:
+        """Sequence b is done: its pages are free, and it is empty."""
+        self._free.extend(self._pages[b])
+        self._pages[b], self._tokens[b], self._new[b] = [], 0, 0
+        self.lens[b] = 0
+        self.table[b] = -1
+        for w in self.weights:
+            if w is not None:
+                w[b] = 0
+
+
+class CachedDecoder:
+    """A `DecoderStack` on one rank that generates: prompts and single tokens through its layers, with the attention of a
+    `PagedKvCache` in the place of the stack's own (no position encoding, as in the stack).
+
+        decoder = CachedDecoder(stack, cache, window=4096, sinks=4)
+        decoder.prompt(h, [n0, n1, ..])      # h [n0 + n1 + .., hidden]: the prompts, one behind the other -> the same shape
+        decoder.step(h)                      # h [batch, hidden]: one token of every sequence -> the same shape
+    """
+
+    def __init__(self, stack, cache: PagedKvCache, window: int = 0, sinks: int = 0):
+        cfg = stack.cfg
+        if stack.world != 1:
+            raise ValueError("the cached decoder runs on one rank")
+        if (cache.layers, cache.n_kv, cache.head_dim) != (len(stack.layers), cfg.n_kv, cfg.head_dim):
+            raise ValueError(f"cache of {cache.layers} layers, {cache.n_kv} kv heads of {cache.head_dim} for a stack of {len(stack.layers)}, "
+                             f"{cfg.n_kv} of {cfg.head_dim}")
+        self.stack, self.cache, self.window, self.sinks = stack, cache, window, sinks
+
+    def _walk(self, h: torch.Tensor, attend) -> torch.Tensor:
+        cfg, delta = self.stack.cfg, None
+        for i, layer in enumerate(self.stack.layers):
+            def core(qkv, i=i):
+                heads = qkv.unflatten(1, (cfg.n_q + 2 * cfg.n_kv, cfg.head_dim))
+                q, k, v = heads.split((cfg.n_q, cfg.n_kv, cfg.n_kv), dim=1)
+                self.cache.append(i, k, v)
+                return attend(i, q, k, v).flatten(1)
+
+            h, delta = layer.forward(h, delta, core)
+        return self.stack.backend.add(h, delta)
+
+    def prompt(self, h: torch.Tensor, lens: list) -> torch.Tensor:
+        if h.dim() != 2 or h.shape[0] != sum(lens):
+            raise ValueError(f"expected [{sum(lens)}, hidden], got {tuple(h.shape)}")
+        self.cache.grow(lens)
+        return self._walk(h, lambda i, q, k, v: self.cache.attend_prompt(i, q, k, v, window=self.window, sinks=self.sinks))
+
+    def step(self, h: torch.Tensor) -> torch.Tensor:
+        if h.dim() != 2 or h.shape[0] != self.cache.batch:
+            raise ValueError(f"expected [{self.cache.batch}, hidden], got {tuple(h.shape)}")
+        self.cache.grow([1] * self.cache.batch)
+        return self._walk(h, lambda i, q, k, v: self.cache.attend(i, q, window=self.window, sinks=self.sinks))

@@ -384,14 +384,15 @@ class DecoderLayer:
             act = None if amax is None else be.silu_mul_quantize_static(gu, amax)
         return be.silu_mul(gu) if act is None else act
 
-    def forward(self, h: torch.Tensor, delta=None):
+    def forward(self, h: torch.Tensor, delta=None, attention=None):
         """h: [tokens, hidden] bf16 residual stream; `delta`: output of the previous row-parallel
-        linear that has not been added to h yet (the add is fused into the next norm).
+        linear that has not been added to h yet (the add is fused into the next norm).  `attention`: takes the place of the
+        layer's own attention core, from the QKV projection [tokens, ..] to [tokens, query width].
         Returns (h, delta) in the same form."""
         cfg, be, w = self.cfg, self.backend, self.world
         h, xq = be.add_norm_quantize(h, delta, self.norm1, cfg.eps, self._norm_amax("qkv", h, delta, self.norm1))
         qkv = be.matmul(xq, self.wqkv)                                   # [T, (q + 2 kv) / W]
-        attn = self._attention(qkv)
+        attn = self._attention(qkv) if attention is None else attention(qkv)
         delta = self.row_parallel(attn, self.wo, self._amax("o", attn))
         h, xq = be.add_norm_quantize(h, delta, self.norm2, cfg.eps, self._norm_amax("gate_up", h, delta, self.norm2))
         act = self._ffn_act(xq)
