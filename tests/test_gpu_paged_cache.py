@@ -435,3 +435,49 @@ def test_what_is_refused(b200):
     refused(f, q, k, k, q_lens=torch.zeros(2, dtype=torch.int32, device="cuda"), match="q_lens")
     refused(f, q, k, k, k_lens=torch.zeros(1, device="cuda"), match="k_lens")
     refused(f, q[0], k[0], k[0], match="expected q")
+
+
+# ----------------------------------------------------------------------------- sizes of the other forms
+@pytest.mark.parametrize("lens,heads,keep", [([120000, 30], 1, 50000), ([13000, 12000], 160, 700), ([5000] * 3, 4, 4999), ([100000], 8, 257)])
+def test_evict_long_rows_against_a_sort(b200, lens, heads, keep):
+    """Rows over clusters, whose keys are held in shared memory or read again on each walk."""
+    g = torch.Generator(device="cuda").manual_seed(keep)
+    rows, d, L = 64, 16, max(lens)
+    table, pages = table_of(g, lens, rows)
+    spare = -(-keep // rows)
+    kp, vp, _, _ = pool(g, pages + spare * len(lens), heads, rows, d, E4M3)
+    fresh = torch.arange(pages, pages + spare * len(lens), dtype=torch.int32, device="cuda").view(len(lens), spare)
+    w = (torch.randn(len(lens), heads, L, device="cuda", generator=g) * 2).exp()
+    w = torch.where(torch.rand(w.shape, device="cuda", generator=g) < 0.5, (w * 2).round() / 2, w)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    kept, m, nw = b200.paged_evict(kp, vp, table, n, w, fresh, keep=keep, recent=keep // 8, sinks=3)
+    for b, x in enumerate(lens):
+        held = w[b, :, :x].clone()
+        held[:, :3] = math.inf
+        held[:, max(0, x - keep // 8):] = math.inf
+        at = held.sort(dim=1, descending=True, stable=True).indices[:, :min(x, keep)].sort(dim=1).values
+        assert torch.equal(kept[b, :, :at.shape[1]].long(), at) and (kept[b, :, at.shape[1]:] == -1).all()
+        assert torch.equal(nw[b, :, :at.shape[1]], w[b].gather(1, at)) and not nw[b, :, at.shape[1]:].any()
+        j = torch.arange(at.shape[1], device="cuda")
+        for h in (0, heads - 1):
+            assert torch.equal(raw(vp)[fresh[b].long()[j // rows], h, j % rows], raw(vp)[table[b].long()[at[h] // rows], h, at[h] % rows])
+
+
+def test_the_ops_and_the_functions_are_one(b200):
+    """The torch.library ops, which a graph holds, and the functions give the same bits; inference tensors and other dtypes of scale pass."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    lens = [70, 300]
+    table, pages = table_of(g, lens, 16)
+    kp, vp, ka, va = pool(g, pages, 2, 16, 64, E4M3)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 6, 64, device="cuda", generator=g).bfloat16()
+    w1, w2 = (torch.zeros(2, 2, 320, device="cuda") for _ in range(2))
+    a = b200.paged_attention(q, kp, vp, table, n, k_amax=ka, v_amax=va, weights=w1, scale=0.25, window=100, sinks=2)
+    b = torch.ops.tensorrt.b200_paged_attention(q, kp, vp, table, n, w2, ka, va, 0.25, 100, 2)
+    assert torch.equal(a, b) and torch.equal(w1, w2)
+    assert torch.equal(a, b200.paged_attention(q, kp, vp, table, n, k_amax=ka.double(), v_amax=va.half().float().fill_(va.item()), scale=0.25, window=100, sinks=2))
+    with torch.inference_mode():
+        assert torch.equal(b200.paged_attention(q.clone(), kp, vp, table, n, k_amax=ka, v_amax=va, scale=1), torch.ops.tensorrt.b200_paged_attention(
+            q, kp, vp, table, n, None, ka, va, 1.0, 0, 0))
+    x = torch.randn(1, 4, 40, 64, device="cuda", generator=g).half()
+    assert torch.equal(b200.window_attention(x, x, x, window=9), torch.ops.tensorrt.b200_window_attention(x, x, x, None, None, 0.0, 9, 0))

@@ -198,3 +198,55 @@ def test_inputs_that_cannot_be_read_in_place(b200):
     across = torch.randn(3, 4, 64, 130, device="cuda", generator=g).bfloat16().transpose(2, 3)
     ref, mass = reference(across, k, across, 0, 0, [130] * 3, [130] * 3)
     check(b200.window_attention(across, k, across), ref, mass)
+
+
+# Sizes at which a call takes each form: two query tiles a CTA (two heads of a group, two blocks of rows), one, and one with its keys
+# split over clusters of 2, 4 and 8.
+FORMS = [
+    (2, 8, 2, 1500, 1500, 128, 0, 0),
+    (1, 16, 16, 2000, 2000, 112, 700, 3),
+    (1, 6, 2, 900, 1100, 64, 0, 0),
+    (1, 32, 8, 300, 4000, 128, 0, 0),
+    (1, 8, 1, 1000, 8000, 128, 0, 0),
+    (1, 8, 1, 61, 4000, 80, 0, 0),
+    (2, 4, 1, 33, 9000, 64, 5000, 200),
+]
+
+
+@pytest.mark.parametrize("bad", [None, float("nan"), float("inf")])
+@pytest.mark.parametrize("shape", FORMS, ids=str)
+def test_every_form_of_the_kernel(b200, shape, bad):
+    """The form depends on the sizes alone; in each, a key or value that is not finite shows in the rows that see it, and in no other."""
+    b, hq, hkv, sq, sk, d, window, sinks = shape
+    g = torch.Generator(device="cuda").manual_seed(sq + sk)
+    q, k, v = inputs(g, b, hq, hkv, sq, sk, d, torch.bfloat16, True)
+    ref, mass = reference(q, k, v, window, sinks, [sq] * b, [sk] * b)
+    if bad is None:
+        out = b200.window_attention(q, k, v, window=window, sinks=sinks)
+        check(out, ref, mass)
+        assert torch.equal(out, b200.window_attention(q, k, v, window=window, sinks=sinks))
+        return
+    at = sk - sq + (2 * sq) // 3                          # seen by the later rows only
+    pos = torch.arange(sq, device="cuda") + sk - sq
+    seen = pos >= at
+    if window > 0:
+        seen &= pos < at + window
+    k, v = k.clone(), v.clone()
+    v[0, 0, at] = bad
+    k[0, 0, at, 0] = bad
+    out = b200.window_attention(q, k, v, window=window, sinks=sinks)
+    check(out[0, :, ~seen], ref[0, :, ~seen], mass[0, :, ~seen])
+    check(out[1:], ref[1:], mass[1:])
+    check(out[:, hq // hkv:], ref[:, hq // hkv:], mass[:, hq // hkv:])
+    assert not torch.isfinite(out[0, :hq // hkv][:, seen].float()).all(-1).any() if bad != bad else True
+
+
+def test_ragged_lengths_in_a_large_call(b200):
+    g = torch.Generator(device="cuda").manual_seed(17)
+    nq, nk = [1000, 3, 700, 0, 129], [1000, 300, 900, 10, 129]
+    q, k, v = inputs(g, 5, 16, 4, 1000, 1000, 128, torch.float16, True)
+    lens = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (nq, nk)]
+    for window, sinks in ((0, 0), (300, 130)):
+        out = b200.window_attention(q, k, v, window=window, sinks=sinks, q_lens=lens[0], k_lens=lens[1])
+        ref, mass = reference(q, k, v, window, sinks, nq, nk)
+        check(out, ref, mass)
