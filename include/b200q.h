@@ -452,9 +452,10 @@ int b200q_paged_append(const void* k, const void* v, int dtype, const int64_t* s
  *   P = softmax(q K^T * scale) in fp32, out = P V; a sequence without keys gets zeros.
  * weights (may be NULL): fp32 [B, heads, weights_len], contiguous; weights[b, h, j] += the sum of P over the query heads of
  * kv head h, for keys j < weights_len that are seen.
- * workspace: b200q_paged_attention_workspace_bytes() bytes, 16-byte aligned, zero the first time it is used and left zero
- * where it has to be; calls sharing one must not overlap.  scratch (with weights only):
+ * workspace: b200q_paged_attention_workspace_bytes() bytes, 16-byte aligned; its first B200Q_PAGED_ATTENTION_ZERO_BYTES are
+ * zero the first time it is used and are left zero again; calls sharing one must not overlap.  scratch (with weights only):
  * b200q_paged_attention_scratch_bytes(B, Hq, weights_len) bytes, any content. */
+#define B200Q_PAGED_ATTENTION_ZERO_BYTES 4096
 size_t b200q_paged_attention_workspace_bytes(void);
 size_t b200q_paged_attention_scratch_bytes(int64_t B, int64_t Hq, int64_t weights_len);
 int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, const b200q_paged_cache* cache,

@@ -32,6 +32,7 @@ using paged::Cache;
 
 constexpr int kThreads = 128, kWarps = 4, kRows = 16, kTile = 64, kKeys = 16;   // kRows: most query heads of an item; kKeys: of one warp
 constexpr int kMaxCtas = 1024;                                                 // resident at once, on any part
+static_assert(kMaxCtas * sizeof(unsigned) == B200Q_PAGED_ATTENTION_ZERO_BYTES, "the header says how much has to be zero");
 
 struct DecodeParams {
   Cache c;
@@ -46,7 +47,7 @@ struct DecodeParams {
   int B, Hq, group, blocks, rows;   // `blocks` of up to `rows` query heads per kv head
   float scale;
   int64_t window, sinks;
-  unsigned* tickets;         // [kMaxCtas], zero between calls
+  unsigned* tickets;         // [kMaxCtas], zero between calls: B200Q_PAGED_ATTENTION_ZERO_BYTES
   float* parts;              // [kMaxCtas][2][kPart]
 };
 
@@ -276,9 +277,11 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
 #pragma unroll
       for (int j = 0; j < kKeys / kPer; ++j) {
         const int key = j * kPer + lane / kLanes;
-        int64_t k_off = __shfl_sync(0xffffffffu, k_row, key), v_off = k_off;
-        if (!p.one_layout) v_off = __shfl_sync(0xffffffffu, v_row, key);
+        int64_t k_off = __shfl_sync(0xffffffffu, k_row, key);
         const int there_bytes = k_off < 0 ? 0 : 16;
+        k_off = k_off < 0 ? 0 : k_off;                  // an aligned address even where nothing is read
+        int64_t v_off = k_off;
+        if (!p.one_layout) v_off = max(__shfl_sync(0xffffffffu, v_row, key), int64_t{0});
 #pragma unroll
         for (int c0 = 0; c0 < S::kChunks; c0 += kLanes) {
           const int c = c0 + lane % kLanes;

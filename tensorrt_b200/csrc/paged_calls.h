@@ -4,8 +4,8 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
+#include <cuda_runtime_api.h>
 
 #include <cmath>
 #include <map>
@@ -146,19 +146,31 @@ void paged_append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages,
                "b200q_paged_append");
 }
 
-// One zeroed workspace per device and stream, kept for the life of the process: the kernels leave it as they found it.  A
-// stream that is being captured and has none yet gets one that the graph itself clears.
+// A workspace whose head is zero, which the kernels leave as they found it: one per device and stream, kept for the life of the
+// process.  A graph may be replayed on any stream beside that one, so a stream that is being captured gets one of the graph's own, which
+// the graph clears where it first uses it; held here until the stream's next capture, then the graph's memory pool alone has it.
 Tensor attention_workspace(const Tensor& like) {
+  struct Kept {
+    unsigned long long capture = 0;
+    Tensor workspace;
+  };
   static std::mutex mu;
-  static auto* kept = new std::map<std::pair<int, cudaStream_t>, Tensor>;      // not destroyed: the context may be gone by then
-  const auto stream = at::cuda::getCurrentCUDAStream();
-  const std::pair<int, cudaStream_t> key{like.get_device(), stream.stream()};
+  static auto* kept = new std::map<std::tuple<int, cudaStream_t, bool>, Kept>;      // not destroyed: the context may be gone by then
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  TORCH_CHECK(cudaStreamGetCaptureInfo(stream, &status, &capture) == cudaSuccess, "b200_paged_attention: cudaStreamGetCaptureInfo failed");
+  const bool captured = status == cudaStreamCaptureStatusActive;
+  if (!captured) capture = 0;
   std::lock_guard<std::mutex> lk(mu);
-  auto it = kept->find(key);
-  if (it != kept->end()) return it->second;
-  Tensor w = at::zeros({static_cast<int64_t>(b200q_paged_attention_workspace_bytes())}, like.options().dtype(at::kByte));
-  if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) kept->emplace(key, w);
-  return w;
+  Kept& k = (*kept)[{like.get_device(), stream, captured}];
+  if (!k.workspace.defined() || k.capture != capture) {
+    k.workspace = Tensor();
+    k.workspace = at::empty({static_cast<int64_t>(b200q_paged_attention_workspace_bytes())}, like.options().dtype(at::kByte));
+    k.workspace.narrow(0, 0, B200Q_PAGED_ATTENTION_ZERO_BYTES).zero_();
+    k.capture = capture;
+  }
+  return k.workspace;
 }
 
 Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens,

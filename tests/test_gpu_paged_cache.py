@@ -481,3 +481,31 @@ def test_the_ops_and_the_functions_are_one(b200):
             q, kp, vp, table, n, None, ka, va, 1.0, 0, 0))
     x = torch.randn(1, 4, 40, 64, device="cuda", generator=g).half()
     assert torch.equal(b200.window_attention(x, x, x, window=9), torch.ops.tensorrt.b200_window_attention(x, x, x, None, None, 0.0, 9, 0))
+
+
+def test_graphs_share_no_workspace_with_their_stream(b200):
+    """Two graphs captured on one stream, replayed side by side on others while that stream goes on: each has a workspace of its own."""
+    g = torch.Generator(device="cuda").manual_seed(10)
+    lens = [5000, 3000]
+    table, pages = table_of(g, lens, 16)
+    kp, vp, _, _ = pool(g, pages, 2, 16, 128, torch.bfloat16)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    qs = [torch.randn(2, 8, 128, device="cuda", generator=g).bfloat16() for _ in range(3)]
+    want = [b200.paged_attention(q, kp, vp, table, n) for q in qs]
+    home, others = torch.cuda.Stream(), [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs, outs = [], []
+    for q in qs[:2]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=home):
+            outs.append([b200.paged_attention(q, kp, vp, table, n) for _ in range(4)])
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for st, graph in zip(others, graphs):
+            with torch.cuda.stream(st):
+                graph.replay()
+        with torch.cuda.stream(home):
+            eager = [b200.paged_attention(qs[2], kp, vp, table, n) for _ in range(4)]
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(o, want[i]) for o in outs[i])
+        assert all(torch.equal(o, want[2]) for o in eager)
