@@ -38,6 +38,22 @@ constexpr int kTileRows = 128, kTileKeys = 128;
 constexpr float kLazy = 8.0f;   // log2 of how far the reference may lie below the maximum
 constexpr int kPolyPairs = 2;   // of 16 pairs of exponentials: on the FMA pipe
 
+// Division of numbers below 2^31 by one that the host knows: n / d = (mulhi(n, mul) + n) >> shift.
+struct Divisor {
+  uint32_t d, mul;
+  int shift;
+};
+Divisor divisor(uint32_t d) {
+  int shift = 0;
+  while ((1ull << shift) < d) ++shift;
+  return Divisor{d, static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1), shift};
+}
+__device__ __forceinline__ int divide(int n, const Divisor& v, int* rest) {
+  const uint32_t q = (__umulhi(static_cast<uint32_t>(n), v.mul) + static_cast<uint32_t>(n)) >> v.shift;
+  *rest = n - static_cast<int>(q * v.d);
+  return static_cast<int>(q);
+}
+
 struct WindowParams {
   const char* q;
   const char* k;
@@ -49,7 +65,8 @@ struct WindowParams {
   int Hq, Hkv, group, Sq, Sk, D;
   float scale;
   int window, sinks;         // window 0: none
-  int rp, nh;                // rows of one head and heads in a query tile, rp * nh = 128
+  int rp, rp_log2, nh;       // rows of one head and heads in a query tile, rp * nh = 128
+  Divisor by_block, by_split, by_unit, by_head;   // query blocks, splits, units, kv heads in the number of a CTA
   int pair_heads;            // the second query tile: the next heads (1) or the next rows (0)
   int units;                 // CTAs that share a kv head and rows
   int q_blocks;
@@ -153,12 +170,10 @@ __device__ __forceinline__ bool needs(const WindowParams& p, int lowest, int hig
 template <int NQ>
 __device__ __forceinline__ Work<NQ> work_of(const WindowParams& p) {
   Work<NQ> w;
-  const int per_row_block = p.B * p.Hkv * p.units, item = static_cast<int>(blockIdx.x) / p.splits, part = static_cast<int>(blockIdx.x) % p.splits;
-  // the last queries first: they see most
-  const int block = p.q_blocks - 1 - item / per_row_block, at = item % per_row_block;
-  const int unit = at % p.units;
-  w.kv_head = at / p.units % p.Hkv;
-  w.b = at / p.units / p.Hkv;
+  int part, at, unit;
+  const int item = divide(static_cast<int>(blockIdx.x), p.by_split, &part);
+  const int block = p.q_blocks - 1 - divide(item, p.by_block, &at);        // the last queries first: they see most
+  w.b = divide(divide(at, p.by_unit, &unit), p.by_head, &w.kv_head);
   w.nq = length_of(p.q_lens, w.b, p.Sq);
   const int nk = length_of(p.k_lens, w.b, p.Sk);
   w.off = nk - w.nq;
@@ -251,7 +266,7 @@ __device__ __noinline__ void join_rows(const WindowParams& p, const float* part,
       }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int row = first + r0 + r, h = head + row / p.rp, i = q0 + row % p.rp, at = i < nq ? i + off : -1;
+      const int row = first + r0 + r, h = head + (row >> p.rp_log2), i = q0 + (row & (p.rp - 1)), at = i < nq ? i + off : -1;
       float top = ml[r][0].x, l = 0.0f, y[4] = {};
 #pragma unroll
       for (int k = 1; k < SPLITS; ++k) top = fmaxf(top, ml[r][k].x);
@@ -275,8 +290,8 @@ __device__ __noinline__ void join_rows(const WindowParams& p, const float* part,
     }
   }
   for (; bad; bad &= bad - 1) {
-    const int row = first + __ffs(bad) - 1, i = q0 + row % p.rp;
-    row_again<T>(p, b, head + row / p.rp, i, i + off);
+    const int row = first + __ffs(bad) - 1, i = q0 + (row & (p.rp - 1));
+    row_again<T>(p, b, head + (row >> p.rp_log2), i, i + off);
   }
 }
 
@@ -448,7 +463,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;     // this warp's 32 lanes of tensor memory
     const uint32_t ts = tmem + s * 128 + lanes, to = tmem + (NQ + s) * 128 + lanes;
     const int q0 = s ? w.q0[NQ - 1] : w.q0[0], lowest = s ? w.lowest[NQ - 1] : w.lowest[0], highest = s ? w.highest[NQ - 1] : w.highest[0];
-    const int h = (s ? w.head[NQ - 1] : w.head[0]) + r / p.rp, i = q0 + r % p.rp;
+    const int h = (s ? w.head[NQ - 1] : w.head[0]) + (r >> p.rp_log2), i = q0 + (r & (p.rp - 1));
     const int at = i < w.nq ? i + w.off : -1;                         // position; < 0: sees nothing
     const float sl = fmaxf(p.scale * 1.4426950408889634f, 1e-30f);    // 0 times a masked -inf would be NaN
     const uint64_t sl2 = pack2(sl, sl);
@@ -771,6 +786,11 @@ int b200q_window_attention(const void* q, const void* k, const void* v, int dtyp
   p.units = p.group / (p.pair_heads ? 2 * p.nh : p.nh);
   p.q_blocks = static_cast<int>(blocks_of(p, shape.nq));
   p.splits = shape.splits;
+  while ((1 << p.rp_log2) < p.rp) ++p.rp_log2;
+  p.by_split = divisor(static_cast<uint32_t>(p.splits));
+  p.by_block = divisor(static_cast<uint32_t>(B * Hkv * p.units));
+  p.by_unit = divisor(static_cast<uint32_t>(p.units));
+  p.by_head = divisor(static_cast<uint32_t>(Hkv));
   const int64_t ctas = static_cast<int64_t>(p.q_blocks) * B * Hkv * p.units * p.splits;
   if (ctas > 0x7fffffffLL) return B200Q_ERR_INVALID;
   CUtensorMap tq, tk, tv;
