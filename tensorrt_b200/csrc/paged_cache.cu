@@ -24,7 +24,8 @@ __device__ __forceinline__ int ld_i32(const int32_t* p) {
 }
 
 // The pages of a CTA's tokens are found first, a warp to a token; then its threads move 16 elements of K and of V at a time, several at once.
-// Bound by the memory for prompts, by three loads that wait for one another (lengths, table, rows) for a decode step.
+// Bound by the memory for prompts (16650 tokens of 8 heads of 128, bf16, 79 MB: 18.9 us, 4.2 TB/s; the copy rate gives 12.0), by three loads that
+// wait for one another (lengths, table, rows) for a decode step (64 tokens 2.6 us, of which an empty launch is most).
 constexpr int kAppendThreads = 256, kAppendTokens = 64, kAppendAtOnce = 4;
 
 template <typename T, bool CODES>
@@ -121,7 +122,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // CTAs step to the same digit.  A lane counts in a column of its own: attention weights share a few exponents, and 32 lanes adding
 // to the same few words wait for one another.  The counts also say how many tokens a CTA keeps in front of the next, so that two
 // more walks in the order of the tokens, a run of them to each warp, write the list.  Bound by latency, and since all of it runs a few
-// times only, by the size of the code as well: loops are unrolled no further than their loads need.
+// times only, by the size of the code as well: loops are unrolled no further than their loads need.  32000 tokens to 8192, 8 heads: about 19 us of
+// the call's 38; 24 sequences of 1500 to 6000 to 2048, 8 heads: 25 of 62.  The counting is most of it (2500 clocks a digit for 4000 keys).
 constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kMaxCluster = 8;
 
 __device__ __forceinline__ int ld_cluster_i32(const int* p, unsigned cta) {
@@ -274,7 +276,8 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   if (ctas > 1) ptx::cluster_sync();            // nobody leaves while its counts may still be read
 }
 
-// The kept rows to their new pages: 16 bytes of K and of V a thread and row, several rows at once.  Bound by the memory.
+// The kept rows to their new pages: 16 bytes of K and of V a thread and row, several rows at once.  Bound by the memory
+// (24 x 8 heads, 2048 rows of 128 bytes, 200 MB: 37 us, 5.5 TB/s).
 constexpr int kMoveThreads = 256, kMoveRows = 4;
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p) {
   pdl_launch_dependents();

@@ -7,13 +7,22 @@
 // units of an SM need the same time (a tile of 128 rows and 128 keys is 1024 clocks of both), so the two have to run under each
 // other all the time.
 //
-// A CTA, one to an SM, holds two tiles of 128 query rows: of two heads that share their K and V where the group is even, of one head
+// A CTA holds two tiles of 128 query rows: of two heads that share their K and V where the group is even, of one head
 // otherwise; with few queries a tile holds the rows of several heads.  One warp loads (TMA; Q once, then K and V tiles of 128
 // keys through a ring), one issues tcgen05.mma (S = Q K^T into tensor memory, O += P V with P read from tensor memory), and four
 // warps for each query tile run its softmax, one thread to a row, so that maximum and sum need no exchange: while one tile is in its softmax
-// the tensor cores work on the other.  P takes the place of the S it came from.  Only key tiles that some row of the CTA
-// sees are visited, and a query tile passes over those that none of its own rows sees; the comparisons of the mask
-// run on tiles at an edge of it.
+// the tensor cores work on the other.  The one issuing warp takes the two tiles in turn, and that keeps them in opposite phase; with a warp
+// each, or with P beside S so that the next scores could be made early (D 64), both softmaxes ran at once on the same
+// special-function units and the tensor cores idled (2 x 32 x 8192 rows of 128, window 4096: 722 -> 816 us; of 64: 606 -> 757).  P takes the place
+// of the S it came from.  Only key tiles that some row of the CTA sees are visited, and a query tile passes over those that none of
+// its own rows sees; the mask, a word for 32 keys, is applied to tiles at an edge of it.  Where that is shorter a CTA holds one query tile, two to an
+// SM, or the CTAs of a cluster share the keys of one (choose_shape).
+//
+// Measured (us a call, bf16): 2 x 32 / 8 heads, 8192 rows of 128, window 4096 with 4 sinks 722 at full clock, 820 call after call under the power
+// cap (1143 and 1006 TFLOP/s; the library's dense product 1633 and 1382); 32 / 8 heads, 4096 rows, no window 126 (1090).  A key tile of both query tiles
+// takes about 3300 clocks: 2100 of softmax, the rest the second half of P V, Q K^T (79 clocks a product of 64 ideal) and barriers.  Counters at the
+// latter: tensor pipe 54 % active, special-function pipe 48 %, issue slots 43 %.  Two threads to a row 1085 us, scores read twice
+// instead of held in registers 802, persistent CTAs in a fixed order 800; exponentials on the FMA pipe, of 16 pairs: none 715, 2 714, 4 733, 8 823.
 //
 // The running maximum is followed lazily: O and the sum stay referred to an older maximum while the new one is at most 2^8 times
 // larger, which 32-bit sums and the exponent range of both 16-bit types hold without loss; so the rescaling of O in tensor memory is
