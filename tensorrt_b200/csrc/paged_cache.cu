@@ -117,19 +117,26 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 // Which tokens stay.  A cluster of CTAs per sequence and kv head, each with a part of the tokens, their keys in shared memory (up to
-// kHeldKeys, else read again on each walk).  The `want`-th largest key is found eight bits at a time, from the top: every CTA counts
-// the digits of its keys that agree with the bits found so far, the counts of the cluster are added through shared memory, and all
-// CTAs step to the same digit.  A lane counts in a column of its own: attention weights share a few exponents, and 32 lanes adding
-// to the same few words wait for one another.  The counts also say how many tokens a CTA keeps in front of the next, so that two
-// more walks in the order of the tokens, a run of them to each warp, write the list.  Bound by latency, and since all of it runs a few
-// times only, by the size of the code as well: loops are unrolled no further than their loads need.  32000 tokens to 8192, 8 heads: about 19 us of
-// the call's 38; 24 sequences of 1500 to 6000 to 2048, 8 heads: 25 of 62.  The counting is most of it (2500 clocks a digit for 4000 keys).
-constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kMaxCluster = 8;
+// kHeldKeys, else read again on each walk).  Sinks and recent tokens have a key above all others, so the m largest keys stay.  The m-th
+// largest key is found eight bits at a time, from the top: every CTA counts the digits of its keys that agree with the bits found so
+// far and writes the counts into every CTA of the cluster (reading the others' from there instead takes 1850 clocks a digit, not 400);
+// one warp adds them, and all CTAs step to the same digit, up to the digit whose keys all stay.  Lanes count in 16 columns: attention
+// weights share a few exponents, and 32 lanes adding to the same few words wait for one another; 8 and 32 columns are 1 us slower.
+// The counts also say how many tokens a CTA keeps in front of the next, so that two more walks in the order of the tokens, a run of them
+// to each warp, write the list; a weight is its key read backwards, since a load from memory in that loop takes 5000 clocks in all.
+// Bound by latency and, since all of it runs a few times only, by the size of the code: what unrolling more loops saves is lost to
+// instruction fetches (34.6 us become 40.3).  32000 tokens to 8192, 8 heads: about 16 us of the call's 34.6 (clusters of 4: 39.5 in
+// all); 24 sequences of 1500 to 6000 to 2048, 8 heads: 19 of 56.2.  Of 30000 clocks there 17000 are the four digits, 7000 the keys.
+constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kMaxCluster = 8, kColumns = 16;
+constexpr uint32_t kStays = 0xffffffffu, kLowest = 0x007fffffu, kZero = 0x80000000u;      // no weight's key; that of -inf and NaN; that of 0 and -0
 
 __device__ __forceinline__ int ld_cluster_i32(const int* p, unsigned cta) {
   int v;
   asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(ptx::mapa_u32(ptx::smem_u32(p), cta)) : "memory");
   return v;
+}
+__device__ __forceinline__ void st_cluster_i32(int* p, unsigned cta, int v) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(ptx::mapa_u32(ptx::smem_u32(p), cta)), "r"(v) : "memory");
 }
 __device__ __forceinline__ float ld_f32(const float* p) {
   float v;
@@ -145,17 +152,16 @@ __device__ __forceinline__ unsigned cluster_size() {
 constexpr int kHeldKeys = 12288;
 template <bool HELD>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
-  extern __shared__ uint32_t keys[];                // HELD: those of the part
-  __shared__ __align__(16) int columns[256 * 32];   // [digit][lane]
-  __shared__ int counts[4][256];                    // of this CTA
-  __shared__ int scan_sums[8][2];
-  __shared__ int found[3];                          // digit; how many of its keys are wanted; this CTA's keys above it
-  __shared__ int published[2];                      // of this CTA's part: tokens kept for sure, candidates equal to the smallest kept key
+  extern __shared__ __align__(16) uint32_t keys[];  // HELD: those of the part, zeros up to a multiple of 4
+  __shared__ __align__(16) int columns[256 * kColumns];       // [digit][lane & 15]
+  __shared__ __align__(16) int counts[2][kMaxCluster][256];   // [round & 1][CTA][255 - digit], written by the CTA that they are of
+  __shared__ int found[4];                          // digit; how many of its keys are wanted; this CTA's keys above it; its own of them if all stay, else -1
+  __shared__ int published[2];                      // of this CTA's part: tokens kept for sure, keys equal to the smallest kept key
   __shared__ int warp_sum[2][kSelectWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(ptx::cluster_ctarank()), ctas = static_cast<int>(cluster_size());
   const int b = blockIdx.y, h = blockIdx.x / ctas;
-  for (int i = tid; i < 256 * 32 / 4; i += kSelectThreads) reinterpret_cast<int4*>(columns)[i] = make_int4(0, 0, 0, 0);
+  for (int i = tid; i < 256 * kColumns / 4; i += kSelectThreads) reinterpret_cast<int4*>(columns)[i] = make_int4(0, 0, 0, 0);
   pdl_launch_dependents();
   pdl_wait();
   const int n = paged::cached_tokens(p.c, b, p.L), m = min(n, p.keep);
@@ -165,90 +171,119 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   int32_t* kept = p.kept + line * p.keep;
   if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = m;
   const int part = (n + ctas - 1) / ctas, t0 = min(rank * part, n), size = min(t0 + part, n) - t0;
+  const int c0 = min(p.sinks, n) - t0, c1 = max(p.sinks, n - p.recent) - t0;      // the others of the part stay
+  auto key_at = [&](int i) { return (i >= c0) & (i < c1) ? weight_key(ld_f32(w + t0 + i)) : kStays; };
+  auto key_of = [&](int i) { return HELD ? keys[i] : key_at(i); };
   if (m == n) {                                     // the same for the whole cluster
 #pragma unroll 4
     for (int i = tid; i < size; i += kSelectThreads) kept[t0 + i] = t0 + i, nw[t0 + i] = ld_f32(w + t0 + i);
   } else if (HELD) {
 #pragma unroll 4
-    for (int i = tid; i < size; i += kSelectThreads) keys[i] = weight_key(ld_f32(w + t0 + i));
+    for (int i = tid; i < size; i += kSelectThreads) keys[i] = key_at(i);
+    if (tid < (-size & 3)) keys[size + tid] = 0;
   }
-  auto key_of = [&](int i) { return HELD ? keys[i] : weight_key(ld_f32(w + t0 + i)); };
   for (int64_t j = m + rank * kSelectThreads + tid; j < p.keep; j += ctas * kSelectThreads) kept[j] = -1;
   for (int64_t j = m + rank * kSelectThreads + tid; j < p.L; j += ctas * kSelectThreads) nw[j] = 0.0f;
-  if (m == n) return;
-  const int lo = min(p.sinks, n), hi = max(lo, n - p.recent);       // candidates: [lo, hi)
-  const int want = m - lo - (n - hi);                               // of them stay
-  const int c0 = max(lo - t0, 0), c1 = min(hi - t0, size);          // candidates of this part
-  __syncthreads();
-  uint32_t least = 0;
-  int left = want, above = 0;                   // wanted among the keys that agree so far; this part's keys above them
-  if (want > 0) {
+  if (m == n || m == 0) return;
+  if (ctas > 1) ptx::cluster_sync(); else __syncthreads();           // the others run, and may be written to
+  uint32_t least = 0, agree = 0;                // the bits found, and which they are
+  int left = m, above = 0, equals = 0;          // wanted among the keys that agree so far; this part's keys above them, and of those that agree
 #pragma unroll 1
-    for (int d = 0; d < 4; ++d) {
-      const int shift = 24 - 8 * d;
+  for (int d = 0; d < 4; ++d) {
+    const int shift = 24 - 8 * d;
+    auto count = [&](uint32_t key) {
+      if ((key & agree) == least) atomicAdd(&columns[((key >> shift) & 255) * kColumns + (lane & (kColumns - 1))], 1);
+    };
+    if (HELD) {
+#pragma unroll 1
+      for (int i = tid; i < (size + 3) / 4; i += kSelectThreads) {
+        const uint4 four = reinterpret_cast<const uint4*>(keys)[i];
+        count(four.x), count(four.y), count(four.z), count(four.w);
+      }
+    } else {
 #pragma unroll 4
-      for (int i = c0 + tid; i < c1; i += kSelectThreads) {
-        const uint32_t key = key_of(i);
-        if (static_cast<uint64_t>(key ^ least) >> (shift + 8) == 0) atomicAdd(&columns[((key >> shift) & 255) * 32 + lane], 1);
-      }
-      __syncthreads();
-      {                                         // two threads to a digit, 16 columns each, turned so that no two meet a bank; cleared for the next
-        int4* mine = reinterpret_cast<int4*>(columns) + (tid >> 1) * 8 + (tid & 1) * 4;
-        int sum = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          int4* at = mine + ((i + (tid >> 1)) & 3);
-          const int4 v = *at;
-          *at = make_int4(0, 0, 0, 0);
-          sum += v.x + v.y + v.z + v.w;
-        }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        if ((tid & 1) == 0) counts[d][tid >> 1] = sum;
-      }
-      if (ctas > 1) ptx::cluster_sync(); else __syncthreads();
-      int own = 0, all = 0, own_up = 0, all_up = 0;   // digit 255 - tid: its keys, here and in the cluster; with those above it
-      if (tid < 256) {
-        own = all = counts[d][255 - tid];
-        if (ctas > 1) {
-          int v[kMaxCluster];
-#pragma unroll
-          for (int r = 0; r < kMaxCluster; ++r) v[r] = r < ctas ? ld_cluster_i32(&counts[d][255 - tid], r) : 0;
-          all = 0;
-#pragma unroll
-          for (int r = 0; r < kMaxCluster; ++r) all += v[r];
-        }
-        own_up = own, all_up = all;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int x = __shfl_up_sync(0xffffffffu, own_up, o), y = __shfl_up_sync(0xffffffffu, all_up, o);
-          if (lane >= o) own_up += x, all_up += y;
-        }
-        if (lane == 31) scan_sums[warp][0] = own_up, scan_sums[warp][1] = all_up;
-      }
-      __syncthreads();
-      if (tid < 256) {
-        for (int i = 0; i < warp; ++i) own_up += scan_sums[i][0], all_up += scan_sums[i][1];
-        if (all_up - all < left && left <= all_up) found[0] = 255 - tid, found[1] = left - (all_up - all), found[2] = own_up - own;
-      }
-      __syncthreads();
-      left = found[1];
-      above += found[2];
-      least |= static_cast<uint32_t>(found[0]) << shift;
+      for (int i = tid; i < size; i += kSelectThreads) count(key_at(i));
     }
+    __syncthreads();
+    {                                           // two threads to a digit, half of its columns each, turned so that no two meet a bank; cleared for the next
+      int4* mine = reinterpret_cast<int4*>(columns) + tid * 2;
+      int sum = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        int4* at = mine + (i ^ ((tid >> 2) & 1));
+        const int4 v = *at;
+        *at = make_int4(0, 0, 0, 0);
+        sum += v.x + v.y + v.z + v.w;
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      int* const slot = &counts[d & 1][rank][255 - (tid >> 1)];       // the largest digit first
+      if (ctas == 1) {
+        if ((tid & 1) == 0) *slot = sum;
+      } else {
+#pragma unroll 1
+        for (int r = tid & 1; r < ctas; r += 2) st_cluster_i32(slot, r, sum);
+      }
+    }
+    if (ctas > 1) ptx::cluster_sync(); else __syncthreads();
+    if (warp == 0) {                            // a lane has eight digits: their keys, here and in the cluster, and those of the lanes in front
+      int own[8], all[8] = {};
+#pragma unroll 1
+      for (int r = 0; r < ctas; ++r) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int4 v = *reinterpret_cast<const int4*>(&counts[d & 1][r][lane * 8 + i * 4]);
+          const int of[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            all[4 * i + j] += of[j];
+            if (r == rank) own[4 * i + j] = of[j];
+          }
+        }
+      }
+      int own_up = 0, all_up = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) own_up += own[i], all_up += all[i];
+      const int own_sum = own_up, all_sum = all_up;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, own_up, o), y = __shfl_up_sync(0xffffffffu, all_up, o);
+        if (lane >= o) own_up += x, all_up += y;
+      }
+      own_up -= own_sum, all_up -= all_sum;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (all_up < left && left <= all_up + all[i]) {
+          const int rest = left - all_up;
+          found[0] = 255 - lane * 8 - i, found[1] = rest, found[2] = own_up, found[3] = rest == all[i] ? own[i] : -1;
+        }
+        own_up += own[i], all_up += all[i];
+      }
+    }
+    __syncthreads();
+    left = found[1];
+    above += found[2];
+    least |= static_cast<uint32_t>(found[0]) << shift;
+    if (found[3] >= 0) {                        // every key with these bits stays: nothing is left to tell apart
+      above += found[3], left = 0;
+      break;
+    }
+    agree |= 255u << shift;
+    equals = counts[d & 1][rank][255 - found[0]];
   }
-  if (tid == 0) published[0] = above + min(max(lo - t0, 0), size) + size - max(min(hi - t0, size), min(max(lo - t0, 0), size)), published[1] = want > 0 ? counts[3][least & 255] : 0;
+  if (tid == 0) published[0] = above, published[1] = left > 0 ? equals : 0;
   // each warp a run of the part, 32 tokens at a time
-  const bool some = want > 0;
-  const uint64_t at_least = some ? static_cast<uint64_t>(least) + 1 : 1ull << 32;     // keys that stay for sure
+  const bool some = left > 0;                   // of the keys that equal the least, the first `left` stay
   const int run = ((size + kSelectWarps - 1) / kSelectWarps + 31) & ~31, r0 = min(warp * run, size), r1 = min(r0 + run, size);
   auto judge = [&](int i, unsigned* sure_lanes, unsigned* equal_lanes) {
-    const bool inside = i < r1, candidate = (i >= c0) & (i < c1);
+    const bool inside = i < r1;
     const uint32_t key = key_of(min(i, size - 1));
-    *sure_lanes = __ballot_sync(0xffffffffu, inside & (!candidate | (key >= at_least)));
-    *equal_lanes = __ballot_sync(0xffffffffu, inside & candidate & (key == least) & some);
+    const bool equal = key == least && some;
+    *sure_lanes = __ballot_sync(0xffffffffu, inside && key >= least && !equal);
+    *equal_lanes = __ballot_sync(0xffffffffu, inside && equal);
+    return key;
   };
   int my_sure = 0, my_equal = 0;
-#pragma unroll 4
+#pragma unroll 1
   for (int base = r0; base < r1; base += 32) {
     unsigned as, es;
     judge(base + lane, &as, &es);
@@ -261,15 +296,17 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   for (int r = 0; r < kMaxCluster - 1; ++r)
     if (r < rank) sure += ld_cluster_i32(&published[0], r), equal += ld_cluster_i32(&published[1], r);
   for (int i = 0; i < warp; ++i) sure += warp_sum[0][i], equal += warp_sum[1][i];
-#pragma unroll 4
+#pragma unroll 1
   for (int base = r0; base < r1; base += 32) {
     unsigned as, es;
-    judge(base + lane, &as, &es);
+    const uint32_t key = judge(base + lane, &as, &es);
     const unsigned me = 1u << lane, below = me - 1;
     const int eq = equal + __popc(es & below);  // equal keys in front; the first `left` stay
     if (((as & me) != 0) | (((es & me) != 0) & (eq < left))) {
       const int at = sure + __popc(as & below) + min(eq, left);
-      kept[at] = t0 + base + lane, nw[at] = ld_f32(w + t0 + base + lane);
+      float weight = __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+      if (key == kStays || key == kLowest || key == kZero) weight = ld_f32(w + t0 + base + lane);
+      kept[at] = t0 + base + lane, nw[at] = weight;
     }
     sure += __popc(as), equal += __popc(es);
   }
@@ -396,7 +433,7 @@ int b200q_paged_evict(const b200q_paged_cache* cache, const int32_t* block_table
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   const int64_t part = (weights_len + ctas - 1) / ctas;
-  const int held = part <= kHeldKeys ? static_cast<int>(part) : 0;          // a longer part is not held at all
+  const int held = part <= kHeldKeys ? static_cast<int>((part + 3) & ~int64_t{3}) : 0;      // a longer part is not held at all
   cfg.dynamicSmemBytes = held * sizeof(uint32_t);
   if (held > 0 && cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldKeys * sizeof(uint32_t)) != cudaSuccess)
     return B200Q_ERR_CUDA;
