@@ -23,10 +23,14 @@ __device__ __forceinline__ int ld_i32(const int32_t* p) {
   return v;
 }
 
-// The pages of a CTA's tokens are found first, a warp to a token; then its threads move 16 elements of K and of V at a time, several at once.
-// Bound by the memory for prompts (16650 tokens of 8 heads of 128, bf16, 79 MB: 18.9 us, 4.2 TB/s; the copy rate gives 12.0), by three loads that
-// wait for one another (lengths, table, rows) for a decode step (64 tokens 2.6 us, of which an empty launch is most).
-constexpr int kAppendThreads = 256, kAppendTokens = 64, kAppendAtOnce = 4;
+// A thread moves 16 elements of K and of V, read first; the pages of the CTA's tokens are found while they come: a warp
+// looks for the sequence of its first token, whose other tokens it holds as well, and so on; then a lane finds the page of a token.
+// Bound by the memory for prompts (16650 tokens of 8 heads of 128, bf16, 79 MB: 16.9 us, 4.7 TB/s; the copy rate gives 12.0), by three loads that
+// wait for one another (lengths, table, rows) for a decode step (64 tokens 2.4 us, of which an empty launch is most).  Many small CTAs: two or
+// four pieces a thread take the registers of others (18.4 and 21.8 us; pages first and four pieces 19.0), 256 threads 17.3, 64 threads 16.6 but
+// more rounds for wide rows.  32000 tokens of one head of 64 to 8-bit pages 4.9 us; with a search to each token 12.2.
+constexpr int kAppendThreads = 128, kAppendTokens = 64;
+static_assert(kAppendTokens <= kAppendThreads, "a lane finds one token");
 
 template <typename T, bool CODES>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p, int tokens) {
@@ -36,61 +40,61 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   const int here = static_cast<int>(p.T - first < tokens ? p.T - first : tokens);
   pdl_launch_dependents();
   pdl_wait();
-  for (int i = tid >> 5; i < here; i += kAppendThreads / 32) {
-    const int64_t t = first + i;
-    int b = static_cast<int>(t), at = 0, fresh = 1;
-    if (p.cu_new != nullptr) {                // the last sequence that begins at or before the token, 32 candidates a step
-      int lo = 0, span = p.B;                 // cu_new[lo] <= t, and the sequence is one of lo .. lo + span - 1
-      while (span > 1) {
-        const int step = (span + 31) / 32, probe = lo + lane * step;
-        const unsigned below = __ballot_sync(0xffffffffu, lane * step < span && ld_i32(p.cu_new + min(probe, p.B)) <= t);
-        const int last = 31 - __clz(below | 1u);
-        span = min(step, span - last * step);
-        lo += last * step;
+  auto find_places = [&] {
+    const int share = (here + kAppendThreads / 32 - 1) / (kAppendThreads / 32), i = (tid >> 5) * share + lane;    // at most 32 tokens to a warp
+    const bool mine = lane < share && i < here;
+    const int t = static_cast<int>(first) + i;
+    int b = t, at = 0, fresh = 1;
+    if (p.cu_new != nullptr) {
+      unsigned left = __ballot_sync(0xffffffffu, mine);
+      while (left != 0) {                     // the sequence of the first token left, and all the tokens that it holds
+        const int leader = __ffs(left) - 1, of = __shfl_sync(0xffffffffu, t, leader);
+        int lo = 0, span = p.B;               // the last that begins at or before it, 32 candidates a step: one of lo .. lo + span - 1
+        while (span > 1) {
+          const int step = (span + 31) / 32, probe = lo + lane * step;
+          const unsigned below = __ballot_sync(0xffffffffu, lane * step < span && ld_i32(p.cu_new + min(probe, p.B)) <= of);
+          const int last = 31 - __clz(below | 1u);
+          span = min(step, span - last * step);
+          lo += last * step;
+        }
+        const int begin = ld_i32(p.cu_new + lo), end = ld_i32(p.cu_new + lo + 1);
+        const bool here_too = lane == leader || ((left >> lane) & 1 && t < end);
+        if (here_too) b = lo, at = t - begin, fresh = end - begin;
+        left &= ~__ballot_sync(0xffffffffu, here_too);
       }
-      b = lo;
-      const int begin = ld_i32(p.cu_new + lo);
-      at = static_cast<int>(t - begin), fresh = ld_i32(p.cu_new + lo + 1) - begin;
     }
-    const int64_t token = static_cast<int64_t>(ld_i32(p.c.lens + b)) - fresh + at;
-    if (lane == 0) {
+    if (mine) {
+      const int64_t token = static_cast<int64_t>(ld_i32(p.c.lens + b)) - fresh + at;
       int2 found = make_int2(-1, 0);
       if (token >= 0 && token < p.c.capacity)
         found = make_int2(paged::page_of(p.c.table + b * p.c.table_stride, static_cast<int>(token), p.c), static_cast<int>(token % p.c.page_size));
       place[i] = found;
     }
-  }
-  __syncthreads();
+    __syncthreads();
+  };
   const int parts = p.c.D / 16, per_token = p.c.heads * parts, all = here * per_token;
-  for (int base = tid; base < all; base += kAppendThreads * kAppendAtOnce) {
-    Raw16<T, false> kr[kAppendAtOnce], vr[kAppendAtOnce];
-    int head[kAppendAtOnce], part[kAppendAtOnce];
-    int2 to[kAppendAtOnce];
-#pragma unroll
-    for (int u = 0; u < kAppendAtOnce; ++u) {
-      const int i = base + u * kAppendThreads, token = i / per_token, rest = i - token * per_token;
-      head[u] = rest / parts, part[u] = rest - head[u] * parts;
-      to[u] = i < all ? place[token] : make_int2(-1, 0);
-      if (to[u].x < 0) continue;
-      kr[u].load(reinterpret_cast<const T*>(p.k + (first + token) * p.k_token + head[u] * p.k_head) + part[u] * 16);
-      vr[u].load(reinterpret_cast<const T*>(p.v + (first + token) * p.v_token + head[u] * p.v_head) + part[u] * 16);
+  for (int base = 0; base < all; base += kAppendThreads) {
+    const int i = base + tid, token = i / per_token, rest = i - token * per_token, head = rest / parts, part = rest - head * parts;
+    Raw16<T, false> kr, vr;
+    if (i < all) {
+      kr.load(reinterpret_cast<const T*>(p.k + (first + token) * p.k_token + head * p.k_head) + part * 16);
+      vr.load(reinterpret_cast<const T*>(p.v + (first + token) * p.v_token + head * p.v_head) + part * 16);
     }
-#pragma unroll
-    for (int u = 0; u < kAppendAtOnce; ++u) {
-      if (to[u].x < 0) continue;
-      char* const kd = paged::row_at(p.c.k, to[u].x, head[u], to[u].y);
-      char* const vd = paged::row_at(p.c.v, to[u].x, head[u], to[u].y);
-      if constexpr (CODES) {
-        const float ks = paged::head_scale(p.c.k_amax, p.c.amax_stride, head[u]), vs = paged::head_scale(p.c.v_amax, p.c.amax_stride, head[u]);
-        *reinterpret_cast<uint4*>(kd + part[u] * 16) = e4m3_of_16(kr[u], ks, __frcp_rn(ks), ks * 512.0f, b200q_div_fast_ok(ks));
-        *reinterpret_cast<uint4*>(vd + part[u] * 16) = e4m3_of_16(vr[u], vs, __frcp_rn(vs), vs * 512.0f, b200q_div_fast_ok(vs));
-      } else {
-        uint4* const k4 = reinterpret_cast<uint4*>(kd + part[u] * 32);
-        uint4* const v4 = reinterpret_cast<uint4*>(vd + part[u] * 32);
-        const U32x8 &kw = kr[u].w[0], &vw = vr[u].w[0];
-        k4[0] = make_uint4(kw.v[0], kw.v[1], kw.v[2], kw.v[3]), k4[1] = make_uint4(kw.v[4], kw.v[5], kw.v[6], kw.v[7]);
-        v4[0] = make_uint4(vw.v[0], vw.v[1], vw.v[2], vw.v[3]), v4[1] = make_uint4(vw.v[4], vw.v[5], vw.v[6], vw.v[7]);
-      }
+    if (base == 0) find_places();
+    const int2 to = i < all ? place[token] : make_int2(-1, 0);
+    if (to.x < 0) continue;
+    char* const kd = paged::row_at(p.c.k, to.x, head, to.y);
+    char* const vd = paged::row_at(p.c.v, to.x, head, to.y);
+    if constexpr (CODES) {
+      const float ks = paged::head_scale(p.c.k_amax, p.c.amax_stride, head), vs = paged::head_scale(p.c.v_amax, p.c.amax_stride, head);
+      *reinterpret_cast<uint4*>(kd + part * 16) = e4m3_of_16(kr, ks, __frcp_rn(ks), ks * 512.0f, b200q_div_fast_ok(ks));
+      *reinterpret_cast<uint4*>(vd + part * 16) = e4m3_of_16(vr, vs, __frcp_rn(vs), vs * 512.0f, b200q_div_fast_ok(vs));
+    } else {
+      uint4* const k4 = reinterpret_cast<uint4*>(kd + part * 32);
+      uint4* const v4 = reinterpret_cast<uint4*>(vd + part * 32);
+      const U32x8 &kw = kr.w[0], &vw = vr.w[0];
+      k4[0] = make_uint4(kw.v[0], kw.v[1], kw.v[2], kw.v[3]), k4[1] = make_uint4(kw.v[4], kw.v[5], kw.v[6], kw.v[7]);
+      v4[0] = make_uint4(vw.v[0], vw.v[1], vw.v[2], vw.v[3]), v4[1] = make_uint4(vw.v[4], vw.v[5], vw.v[6], vw.v[7]);
     }
   }
 }
@@ -382,7 +386,7 @@ int b200q_paged_append(const void* k, const void* v, int dtype, const int64_t* s
   p.B = static_cast<int>(B);
   const auto st = static_cast<cudaStream_t>(stream);
   // tokens of a CTA: what keeps its threads busy once, fewer where that leaves SMs without a CTA
-  const int64_t pieces = static_cast<int64_t>(p.c.heads) * (p.c.D / 16), fill = kAppendThreads * kAppendAtOnce / pieces, spread = T / (2 * sm_count());
+  const int64_t pieces = static_cast<int64_t>(p.c.heads) * (p.c.D / 16), fill = kAppendThreads / pieces, spread = T / (2 * sm_count());
   int64_t tokens = fill < spread ? fill : spread;
   tokens = tokens < 1 ? 1 : (tokens > kAppendTokens ? kAppendTokens : tokens);
   const dim3 grid(static_cast<unsigned>((T + tokens - 1) / tokens)), block(kAppendThreads);

@@ -313,6 +313,26 @@ def test_append(b200, dt, codes, heads, d, rows, new, layout):
         assert torch.equal(r.view(torch.uint8) if codes else r.view(torch.int16), full.view(torch.uint8) if codes else full.view(torch.int16))
 
 
+@pytest.mark.parametrize("heads,most", [(1, 40), (2, 1), (1, 3000)])
+def test_append_of_many_sequences(b200, heads, most):
+    """A CTA's tokens are of many sequences, some of which bring nothing, or all of one."""
+    g = torch.Generator(device="cuda").manual_seed(most)
+    fresh = torch.randint(0, most + 1, (60000 // (most + 1) + 2,), device="cuda", generator=g)
+    old = torch.randint(0, 20, fresh.shape, device="cuda", generator=g)
+    lens, rows, d = fresh + old, 8, 16
+    table, pages = table_of(g, lens.tolist(), rows)
+    kp, vp, _, _ = pool(g, pages, heads, rows, d, torch.bfloat16)
+    want_k, want_v = kp.clone(), vp.clone()
+    cu = torch.nn.functional.pad(fresh.cumsum(0), (1, 0)).to(torch.int32)
+    k, v = (torch.randn(int(cu[-1]), heads, d, device="cuda", dtype=torch.bfloat16, generator=g) for _ in range(2))
+    b = torch.repeat_interleave(torch.arange(fresh.numel(), device="cuda"), fresh)
+    at = old[b] + torch.arange(b.numel(), device="cuda") - cu[b]
+    page = table[b, at // rows].long()
+    want_k[page, :, at % rows], want_v[page, :, at % rows] = k, v
+    b200.paged_append(k, v, kp, vp, table, lens.to(torch.int32), cu)
+    assert torch.equal(kp.view(torch.int16), want_k.view(torch.int16)) and torch.equal(vp.view(torch.int16), want_v.view(torch.int16))
+
+
 def test_append_leaves_what_it_is_not_given_alone(b200):
     """Tokens without a page, before the first token or beyond the table are left out; unaligned rows are copied first."""
     heads, d, rows = 2, 64, 8
