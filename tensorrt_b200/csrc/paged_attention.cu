@@ -604,9 +604,10 @@ __global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ De
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < see.seen; i += static_cast<int64_t>(gridDim.x) * 256) {
     const int token = see.token(static_cast<int>(i));
     if (token >= p.weights_len) return;
+    const float old = w[token];            // read beside the logits, not behind them (1 us of 41)
     float sum = 0.0f;
     for (int g = 0; g < p.group; ++g) sum += exp2_fast(p.logits[(first + g) * p.logits_stride + i] - p.lse[first + g]);
-    w[token] += sum;
+    w[token] = old + sum;
   }
 }
 
