@@ -125,12 +125,12 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // largest key is found eight bits at a time, from the top: every CTA counts the digits of its keys that agree with the bits found so
 // far and writes the counts into every CTA of the cluster (reading the others' from there instead takes 1850 clocks a digit, not 400);
 // one warp adds them, and all CTAs step to the same digit, up to the digit whose keys all stay.  Lanes count in 16 columns: attention
-// weights share a few exponents, and 32 lanes adding to the same few words wait for one another; 8 and 32 columns are 1 us slower.
+// weights share a few exponents, and 32 lanes adding to the same few words wait for one another; 8 columns are no faster.
 // The counts also say how many tokens a CTA keeps in front of the next, so that two more walks in the order of the tokens, a run of them
 // to each warp, write the list; a weight is its key read backwards, since a load from memory in that loop takes 5000 clocks in all.
 // Bound by latency and, since all of it runs a few times only, by the size of the code: what unrolling more loops saves is lost to
-// instruction fetches (34.6 us become 40.3).  32000 tokens to 8192, 8 heads: about 16 us of the call's 34.6 (clusters of 4: 39.5 in
-// all); 24 sequences of 1500 to 6000 to 2048, 8 heads: 19 of 56.2.  Of 30000 clocks there 17000 are the four digits, 7000 the keys.
+// instruction fetches (34.6 us for the first of these calls became 40.3).  32000 tokens to 8192, 8 heads: about 18 us of the call's 31.4 (clusters of 4: 5 us
+// more); 24 sequences of 1500 to 6000 to 2048, 8 heads: 19 of 52.9.  Of 30000 clocks there 17000 are the four digits, 7000 the keys.
 constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kMaxCluster = 8, kColumns = 16;
 constexpr uint32_t kStays = 0xffffffffu, kLowest = 0x007fffffu, kZero = 0x80000000u;      // no weight's key; that of -inf and NaN; that of 0 and -0
 
@@ -317,9 +317,10 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   if (ctas > 1) ptx::cluster_sync();            // nobody leaves while its counts may still be read
 }
 
-// The kept rows to their new pages: 16 bytes of K and of V a thread and row, several rows at once.  Bound by the memory
-// (24 x 8 heads, 2048 rows of 128 bytes, 200 MB: 37 us, 5.5 TB/s).
-constexpr int kMoveThreads = 256, kMoveRows = 4;
+// The kept rows to their new pages: 16 bytes of K and of V a thread and row, two rows at once.  Bound by the memory
+// (24 x 8 heads, 2048 rows of 128 bytes, 200 MB: 34 us, 5.9 TB/s).  Four rows at once take registers from other CTAs (the two calls 34.8 and
+// 56.5 us, not 31.4 and 52.9), one leaves too little on its way (31.1 and 56.6).
+constexpr int kMoveThreads = 128, kMoveRows = 2;
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p) {
   pdl_launch_dependents();
   pdl_wait();
