@@ -23,6 +23,9 @@
 // takes about 3300 clocks: 2100 of softmax, the rest the second half of P V, Q K^T (79 clocks a product of 64 ideal) and barriers.  Counters at the
 // latter: tensor pipe 54 % active, special-function pipe 48 %, issue slots 43 %.  Two threads to a row 1085 us, scores read twice
 // instead of held in registers 802, persistent CTAs in a fixed order 800; exponentials on the FMA pipe, of 16 pairs: none 715, 2 714, 4 733, 8 823.
+// 8 sequences of up to 1500, 12 / 12 heads of 80, window 512 41.8.  What runs once or rarely in a CTA (rescaling, the way out) stays in loops: short
+// calls pay for fetching the code, and registers spill less (43.9 with those unrolled).  A branch that took a tile of sinks alone as 32 keys cost
+// more than it saved there (42.7; 8192 rows the same).
 //
 // The running maximum is followed lazily: O and the sum stay referred to an older maximum while the new one is at most 2^8 times
 // larger, which 32-bit sums and the exponent range of both 16-bit types hold without loss; so the rescaling of O in tensor memory is
@@ -520,7 +523,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         const float now = fmaxf(m, mx), f = now == -INFINITY ? 1.0f : exp2_fast((m - now) * sl);
         m = now;
         l *= f;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < DPAD / 32; ++c) {
           uint32_t o[32];
           ptx::tmem_ld_32x32(to + c * 32, o);
@@ -576,7 +579,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
         // this CTA's part of the row: O, referred to m, over the ring (its last tile has been read); m and l over the queries
         float* const rows = reinterpret_cast<float*>(ring) + r * DPAD;
         reinterpret_cast<float2*>(sq)[r] = make_float2(m, l);
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < DPAD / 32; ++c) {
           uint32_t o[32] = {};
           if (begun) {
@@ -594,7 +597,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       // in one store instruction are 32 lines (5700 clocks for a tile; so 1000).
       constexpr int kRowBytes = DPAD * 2, kPieces = kRowBytes / 16;
       char* const rows = sq + s * L::kTileBytes;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < DPAD / 32; ++c) {
         uint32_t o[32];
         if (begun) {
