@@ -20,7 +20,7 @@
 //
 // Measured (us a call): 64 sequences of 1 to 8190 tokens, 64 / 8 heads of 128, bf16 174 (6.2 TB/s, 0.94 of the copy rate; DRAM 6.1 TB/s, issue
 // slots 28 %); 3 of 60000 to 131071, 8-bit pages 106 (5.5 TB/s: widening codes takes issue slots, 58 %); 32 of 900 to 16000, 16 / 16 heads of 64, window
-// 2048 48 (5.5 TB/s); one of 411 tokens 7.3, the chain from the lengths to the joined parts.  With the query heads as the 16-row
+// 2048 48 (5.5 TB/s); one of 411 tokens 7.0, the chain from the lengths to the joined parts (7.3 with four parts read at once, 7.7 with two).  With the query heads as the 16-row
 // operand 187 / 144 / 69 / 8.3.  The loop in three or six copies, one for each stage of the ring, made short calls longer (instructions are
 // fetched once) and long ones no shorter; four CTAs to an SM for 8-bit pages 111.
 //
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
           const int row = i / kQuads, d = (i % kQuads) * 4;
           float top = -INFINITY, sum = 0.0f, acc[4] = {};
           bool has = false;
-          constexpr int kAtOnce = 4;
+          constexpr int kAtOnce = 8;
 #pragma unroll 1
           for (int c = c0; c <= c1; c += kAtOnce) {
             float pm[kAtOnce], ps[kAtOnce];
