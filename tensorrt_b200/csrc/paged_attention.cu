@@ -9,7 +9,9 @@
 // Work.  An item is a sequence, a kv head and up to 16 of its query heads; its keys are tiles of 64.  The tiles of all items
 // stand in one line, which the resident CTAs cut into equal pieces (the lengths are on the device, so every CTA adds them up
 // for itself).  A CTA that ends inside an item leaves its part (maximum, sum, unnormalised result, 32 bits) in the workspace; the
-// CTA that arrives last joins the parts in the order of the keys, so that results do not depend on who is last.
+// CTA that arrives last joins the parts in the order of the keys, so that results do not depend on who is last.  More than 16 parts are
+// joined in two steps (one sequence of 100000, 8 / 1 heads of 128, 444 parts 25 us instead of 78; of 30000, 64 / 4 heads, 8-bit pages 28.6 instead of 51;
+// of 4000, 32 / 8 heads 11.0 instead of 12.3).
 //
 // A warp takes 16 of a tile's 64 keys through a ring of its own in shared memory, filled by asynchronous copies of 16 bytes, and
 // has its own maximum, sum and result; nothing but the end of an item makes warps wait for one another.  The products run on
@@ -20,7 +22,7 @@
 //
 // Measured (us a call): 64 sequences of 1 to 8190 tokens, 64 / 8 heads of 128, bf16 174 (6.2 TB/s, 0.94 of the copy rate; DRAM 6.1 TB/s, issue
 // slots 28 %); 3 of 60000 to 131071, 8-bit pages 106 (5.5 TB/s: widening codes takes issue slots, 58 %); 32 of 900 to 16000, 16 / 16 heads of 64, window
-// 2048 48 (5.5 TB/s); one of 411 tokens 7.0, the chain from the lengths to the joined parts (7.3 with four parts read at once, 7.7 with two).  With the query heads as the 16-row
+// 2048 48 (5.5 TB/s); one of 411 tokens 7.3, the chain from the lengths to the joined parts.  With the query heads as the 16-row
 // operand 187 / 144 / 69 / 8.3.  The loop in three or six copies, one for each stage of the ring, made short calls longer (instructions are
 // fetched once) and long ones no shorter; four CTAs to an SM for 8-bit pages 111.
 //
@@ -37,8 +39,9 @@ namespace {
 using paged::Cache;
 
 constexpr int kThreads = 128, kWarps = 4, kRows = 16, kTile = 64, kKeys = 16;   // kRows: most query heads of an item; kKeys: of one warp
-constexpr int kMaxCtas = 1024;                                                 // resident at once, on any part
-static_assert(kMaxCtas * sizeof(unsigned) == B200Q_PAGED_ATTENTION_ZERO_BYTES, "the header says how much has to be zero");
+constexpr int kMaxCtas = 512;                                                  // of a launch
+constexpr int kGroupsFrom = 16;                                                 // parts are joined in two steps from one more on
+static_assert(2 * kMaxCtas * sizeof(unsigned) == B200Q_PAGED_ATTENTION_ZERO_BYTES, "the header says how much has to be zero");
 
 struct DecodeParams {
   Cache c;
@@ -53,12 +56,12 @@ struct DecodeParams {
   int B, Hq, group, blocks, rows;   // `blocks` of up to `rows` query heads per kv head
   float scale;
   int64_t window, sinks;
-  unsigned* tickets;         // [kMaxCtas], zero between calls: B200Q_PAGED_ATTENTION_ZERO_BYTES
+  unsigned* tickets;         // [2][kMaxCtas], of items and of groups, zero between calls: B200Q_PAGED_ATTENTION_ZERO_BYTES
   float* parts;              // [kMaxCtas][2][kPart]
 };
 
 constexpr float kLazy = 8.0f;   // log2 of how far the reference of a sum may lie below its largest term
-constexpr int kPart = kRows * paged::kMaxD + 2 * kRows;   // result rows, maxima, sums
+constexpr int kPart = kRows * paged::kMaxD + 4 * kRows;   // result rows, maxima, sums; maxima and sums of a group
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 // 16 bytes to shared memory: `bytes` of them from `src`, zeros behind.
@@ -528,32 +531,40 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
       }
     }
     // ------------------------------------------------------------- the CTAs' parts together, by the one that comes last
+    // Many parts in two steps: 8 or 16 neighbours by the last of them, into the place of the first, then the groups.
     if (!whole) {
-      __syncthreads();
-      if (tid == 0) {
-        __threadfence();                               // what the CTA has written, seen through the barrier, in front of the ticket
-        last_one = atomicAdd(p.tickets + c0, 1u) == static_cast<unsigned>(c1 - c0);
-        if (last_one) p.tickets[c0] = 0;
-      }
-      __syncthreads();
-      if (last_one) {
+      const int more = c1 - c0, group = more < kGroupsFrom ? 0 : (more < 128 ? 3 : 4);     // log2 of the parts of a group, 0: no groups
+      int lo = group > 0 ? c0 + ((cta - c0) >> group << group) : c0, hi = group > 0 ? min(lo + (1 << group) - 1, c1) : c1, step = 1;
+#pragma unroll 1
+      for (bool grouping = group > 0;; grouping = false) {
+        __syncthreads();
+        if (tid == 0) {
+          __threadfence();                             // what the CTA has written, seen through the barrier, in front of the ticket
+          unsigned* const ticket = p.tickets + (grouping ? kMaxCtas : 0) + lo;
+          last_one = lo == hi || atomicAdd(ticket, 1u) == static_cast<unsigned>((hi - lo) >> (step > 1 ? group : 0));
+          if (last_one && lo != hi) *ticket = 0;
+        }
+        __syncthreads();
+        if (!last_one) break;
         __threadfence();
         const bool second = piece(total, c0, ctas) < item_start;     // the item is not the first that CTA c0 worked on
         for (int i = tid; i < rows * kQuads; i += kThreads) {
           const int row = i / kQuads, d = (i % kQuads) * 4;
+          const int from = kRows * DPAD + (step > 1 ? 2 * kRows : 0) + row;        // of the maxima
           float top = -INFINITY, sum = 0.0f, acc[4] = {};
           bool has = false;
           constexpr int kAtOnce = 8;
 #pragma unroll 1
-          for (int c = c0; c <= c1; c += kAtOnce) {
+          for (int c = lo; c <= hi; c += kAtOnce * step) {
             float pm[kAtOnce], ps[kAtOnce];
             float4 v[kAtOnce];
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k) {        // the loads first: they do not wait for one another
               ps[k] = -1.0f;
-              if (c + k > c1) continue;
-              const float* src = p.parts + (static_cast<int64_t>(c + k) * 2 + (c + k == c0 && second ? 1 : 0)) * kPart;
-              pm[k] = __ldcg(src + kRows * DPAD + row), ps[k] = __ldcg(src + kRows * DPAD + kRows + row);
+              const int of = c + k * step;
+              if (of > hi) continue;
+              const float* src = p.parts + (static_cast<int64_t>(of) * 2 + (of == c0 && second ? 1 : 0)) * kPart;
+              pm[k] = __ldcg(src + from), ps[k] = __ldcg(src + from + kRows);
               v[k] = __ldcg(reinterpret_cast<const float4*>(src + row * DPAD + d));
             }
 #pragma unroll
@@ -566,6 +577,12 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
               acc[2] = acc[2] * f0 + v[k].z * f1, acc[3] = acc[3] * f0 + v[k].w * f1;
               top = now;
             }
+          }
+          if (grouping) {
+            float* dst = p.parts + (static_cast<int64_t>(lo) * 2 + (lo == c0 && second ? 1 : 0)) * kPart;
+            *reinterpret_cast<float4*>(dst + row * DPAD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            if (d == 0) dst[kRows * DPAD + 2 * kRows + row] = top, dst[kRows * DPAD + 3 * kRows + row] = has ? sum : -1.0f;
+            continue;
           }
           if (d < p.c.D) {
             const float f = v_scale / sum;
@@ -580,6 +597,8 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
           if (d == 0 && p.lse != nullptr)
             p.lse[static_cast<int64_t>(b) * p.Hq + head0 + row] = has ? (top == -INFINITY ? 0.0f : top) + log2f(sum) : 0.0f;
         }
+        if (!grouping) break;
+        lo = c0, hi = c0 + (more >> group << group), step = 1 << group;
       }
     }
     __syncthreads();
@@ -648,7 +667,7 @@ using namespace b200q;
 
 extern "C" {
 
-size_t b200q_paged_attention_workspace_bytes(void) { return kMaxCtas * sizeof(unsigned) + static_cast<size_t>(kMaxCtas) * 2 * kPart * sizeof(float); }
+size_t b200q_paged_attention_workspace_bytes(void) { return 2 * kMaxCtas * sizeof(unsigned) + static_cast<size_t>(kMaxCtas) * 2 * kPart * sizeof(float); }
 
 size_t b200q_paged_attention_scratch_bytes(int64_t B, int64_t Hq, int64_t weights_len) {
   if (B <= 0 || Hq <= 0 || weights_len < 0) return 16;
@@ -684,7 +703,7 @@ int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, co
   p.scale = scale;
   p.window = window, p.sinks = sinks;
   p.tickets = static_cast<unsigned*>(workspace);
-  p.parts = reinterpret_cast<float*>(p.tickets + kMaxCtas);
+  p.parts = reinterpret_cast<float*>(p.tickets + 2 * kMaxCtas);
   if (weights != nullptr && weights_len > 0) {
     p.logits_stride = round4(weights_len);
     p.weights_len = weights_len;

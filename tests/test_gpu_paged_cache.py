@@ -272,6 +272,29 @@ def test_other_streams_and_graphs(b200):
         assert torch.equal(kp[table[torch.arange(3), last // rows].long(), :, last % rows], k)
 
 
+@pytest.mark.parametrize("tiles,heads,group,d,pt", [([16], 1, 8, 128, torch.bfloat16), ([17], 1, 1, 64, torch.bfloat16), ([25, 18], 1, 16, 80, E4M3),
+                                                    ([128], 1, 4, 128, E4M3), ([129], 1, 3, 128, torch.bfloat16), ([130, 1, 140], 1, 9, 64, torch.bfloat16),
+                                                    ([1600], 1, 2, 128, torch.bfloat16), ([700, 3, 500], 2, 5, 64, E4M3)])
+def test_attention_joined_from_many_parts(b200, tiles, heads, group, d, pt):
+    """Sequences whose keys many CTAs share: the parts are joined at once or in two steps, some of them of no key, and twice the same bits."""
+    g = torch.Generator(device="cuda").manual_seed(sum(tiles))
+    rows, lens = 32, [64 * t - 5 for t in tiles]
+    table, pages = table_of(g, lens, rows)
+    kp, vp, ka, va = pool(g, pages, heads, rows, d, pt)
+    table[:, 6:10] = -1                                   # two tiles and two halves without a page
+    table[0, 20:32] = -1
+    q = torch.randn(len(lens), heads * group, d, device="cuda", generator=g).bfloat16()
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    w = torch.zeros(len(lens), heads, table.shape[1] * rows, device="cuda")
+    out = b200.paged_attention(q, kp, vp, table, n, k_amax=ka, v_amax=va, weights=w)
+    ref, mass, gained = attention_ref(q, kp, vp, table, lens, ka, va, 0, 0)
+    check_out(out, ref, mass)
+    assert (w.double() - gained).abs().max() <= 2.0 ** -11
+    for _ in range(5):
+        again = b200.paged_attention(q, kp, vp, table, n, k_amax=ka, v_amax=va)
+        assert torch.equal(out.view(torch.int16), again.view(torch.int16))
+
+
 # ----------------------------------------------------------------------------- append
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("codes", [False, True])
