@@ -153,7 +153,8 @@ __device__ __forceinline__ unsigned cluster_size() {
   return r;
 }
 
-constexpr int kHeldKeys = 12288;
+// What fits beside the counts: 320 rows of 45000 keys, one CTA to an SM, 187 us a call, 242 from memory; of 30 x 16 rows of 15000 93 and 138.
+constexpr int kHeldKeys = 49152;
 template <bool HELD>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
   extern __shared__ __align__(16) uint32_t keys[];  // HELD: those of the part, zeros up to a multiple of 4

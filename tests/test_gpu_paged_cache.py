@@ -481,7 +481,7 @@ def test_what_is_refused(b200):
 
 
 # ----------------------------------------------------------------------------- sizes of the other forms
-@pytest.mark.parametrize("lens,heads,keep", [([120000, 30], 1, 50000), ([13000, 12000], 160, 700), ([5000] * 3, 4, 4999), ([100000], 8, 257)])
+@pytest.mark.parametrize("lens,heads,keep", [([120000, 30], 1, 50000), ([13000, 12000], 160, 700), ([5000] * 3, 4, 4999), ([100000], 8, 257), ([400001, 7], 1, 30000), ([49000, 48999], 160, 300)])
 def test_evict_long_rows_against_a_sort(b200, lens, heads, keep):
     """Rows over clusters, whose keys are held in shared memory or read again on each walk."""
     g = torch.Generator(device="cuda").manual_seed(keep)
