@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   // each warp a run of the part, 32 tokens at a time
   const bool some = left > 0;                   // of the keys that equal the least, the first `left` stay
   const int run = ((size + kSelectWarps - 1) / kSelectWarps + 31) & ~31, r0 = min(warp * run, size), r1 = min(r0 + run, size);
-  auto judge = [&](int i, unsigned* sure_lanes, unsigned* equal_lanes) {
+  auto classify = [&](int i, unsigned* sure_lanes, unsigned* equal_lanes) {
     const bool inside = i < r1;
     const uint32_t key = key_of(min(i, size - 1));
     const bool equal = key == least && some;
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
 #pragma unroll 1
   for (int base = r0; base < r1; base += 32) {
     unsigned as, es;
-    judge(base + lane, &as, &es);
+    classify(base + lane, &as, &es);
     my_sure += __popc(as), my_equal += __popc(es);
   }
   if (lane == 0) warp_sum[0][warp] = my_sure, warp_sum[1][warp] = my_equal;
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
 #pragma unroll 1
   for (int base = r0; base < r1; base += 32) {
     unsigned as, es;
-    const uint32_t key = judge(base + lane, &as, &es);
+    const uint32_t key = classify(base + lane, &as, &es);
     const unsigned me = 1u << lane, below = me - 1;
     const int eq = equal + __popc(es & below);  // equal keys in front; the first `left` stay
     if (((as & me) != 0) | (((es & me) != 0) & (eq < left))) {
