@@ -464,9 +464,10 @@ int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, co
                           int64_t weights_len, void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes,
                           b200q_stream_t stream);
 
-/* Which keys stay, and their rows moved to fresh pages.  Of a sequence's n = lens[b] tokens each kv head keeps
- * min(n, keep): the first `sinks`, the last `recent`, and of the others those of the largest weights[b, h, :] (fp32
- * [B, heads, weights_len], contiguous; equal ones: the lower token; NaN counts as -inf).  sinks + recent <= keep.
+/* Which keys stay, and their rows moved to fresh pages.  Of a sequence's n tokens (lens[b], but for those in pages that the
+ * table does not name) each kv head keeps min(n, keep): those among the first `sinks` and the last `recent` of the lens[b], and of
+ * the others those of the largest weights[b, h, :] (fp32 [B, heads, weights_len], contiguous; equal ones: the lower token;
+ * NaN counts as -inf).  sinks + recent <= keep.
  * Their rows go, in the order of the tokens, to rows 0, 1, .. of the pages out_table[b * out_stride + ..]; these pages
  * must not hold rows that the call reads.  Pages may be shared between sequences on the reading side.
  *   kept         int32 [B, heads, keep]: the tokens kept, ascending, -1 beyond the last

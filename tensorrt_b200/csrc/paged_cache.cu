@@ -105,6 +105,7 @@ struct EvictParams {
   int64_t L;
   const int32_t* out_table;
   int64_t out_stride;
+  int64_t table_width;
   int keep, recent, sinks;
   int32_t* kept;
   int32_t* new_lens;
@@ -169,22 +170,51 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
   for (int i = tid; i < 256 * kColumns / 4; i += kSelectThreads) reinterpret_cast<int4*>(columns)[i] = make_int4(0, 0, 0, 0);
   pdl_launch_dependents();
   pdl_wait();
-  const int n = paged::cached_tokens(p.c, b, p.L), m = min(n, p.keep);
+  // Tokens whose page the table does not name are not there, so they are not among those that stay: their key is zero, below every weight's.
+  // The first entries are read beside the length, not behind it.
+  constexpr int kAhead = 4;
+  const int32_t* const table = p.c.table + b * p.c.table_stride;
+  int entry[kAhead], gone = 0;
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) entry[u] = tid + u * kSelectThreads < p.table_width ? ld_i32(table + tid + u * kSelectThreads) : 0;
+  const int n = paged::cached_tokens(p.c, b, p.L);
   const int64_t line = static_cast<int64_t>(b) * p.c.heads + h;
+  auto gone_of = [&](int64_t i, int page) {
+    const int64_t left = n - i * p.c.page_size;
+    return left > 0 && static_cast<unsigned>(page) >= static_cast<unsigned>(p.c.num_pages) ? static_cast<int>(left < p.c.page_size ? left : p.c.page_size) : 0;
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) gone += gone_of(tid + u * kSelectThreads, entry[u]);
+#pragma unroll 1
+  for (int64_t i = tid + kAhead * kSelectThreads; i * p.c.page_size < n; i += kSelectThreads) gone += gone_of(i, ld_i32(table + i));
+  const bool holes = __syncthreads_or(gone);
+  if (holes) {
+    gone = __reduce_add_sync(0xffffffffu, gone);
+    if (lane == 0) warp_sum[0][warp] = gone;
+    __syncthreads();
+    gone = 0;
+    for (int i = 0; i < kSelectWarps; ++i) gone += warp_sum[0][i];
+  }
+  const int m = min(n - gone, p.keep);
   const float* w = p.weights + line * p.L;
   float* nw = p.new_weights + line * p.L;
   int32_t* kept = p.kept + line * p.keep;
   if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = m;
   const int part = (n + ctas - 1) / ctas, t0 = min(rank * part, n), size = min(t0 + part, n) - t0;
   const int c0 = min(p.sinks, n) - t0, c1 = max(p.sinks, n - p.recent) - t0;      // the others of the part stay
-  auto key_at = [&](int i) { return (i >= c0) & (i < c1) ? weight_key(ld_f32(w + t0 + i)) : kStays; };
+  auto weight_at = [&](int i) { return (i >= c0) & (i < c1) ? weight_key(ld_f32(w + t0 + i)) : kStays; };
+  auto key_at = [&](int i) { return holes && paged::page_of(table, t0 + i, p.c) < 0 ? 0u : weight_at(i); };
   auto key_of = [&](int i) { return HELD ? keys[i] : key_at(i); };
   if (m == n) {                                     // the same for the whole cluster
 #pragma unroll 4
     for (int i = tid; i < size; i += kSelectThreads) kept[t0 + i] = t0 + i, nw[t0 + i] = ld_f32(w + t0 + i);
   } else if (HELD) {
 #pragma unroll 4
-    for (int i = tid; i < size; i += kSelectThreads) keys[i] = key_at(i);
+    for (int i = tid; i < size; i += kSelectThreads) keys[i] = weight_at(i);
+    if (holes)
+#pragma unroll 1
+      for (int i = tid; i < size; i += kSelectThreads)
+        if (paged::page_of(table, t0 + i, p.c) < 0) keys[i] = 0;
     if (tid < (-size & 3)) keys[size + tid] = 0;
   }
   for (int64_t j = m + rank * kSelectThreads + tid; j < p.keep; j += ctas * kSelectThreads) kept[j] = -1;
@@ -417,6 +447,7 @@ int b200q_paged_evict(const b200q_paged_cache* cache, const int32_t* block_table
   p.L = weights_len;
   p.out_table = out_table;
   p.out_stride = out_stride;
+  p.table_width = table_width;
   p.keep = static_cast<int>(keep), p.recent = static_cast<int>(recent), p.sinks = static_cast<int>(sinks);
   p.kept = kept;
   p.new_lens = new_lens;

@@ -46,8 +46,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, weights: torch.Tensor,
                 out_table: torch.Tensor, *, keep: int, recent: int = 0, sinks: int = 0):
     """Cuts every sequence to `keep` tokens per kv head: the first `sinks`, the last `recent` and, of the others, those with the
-    largest weights (equal ones: the lower token).  Their rows move, in order, to the pages of `out_table` [B, pages], which must not
-    be among the pages read.  -> (kept tokens int32 [B, kv heads, keep], -1 beyond a shorter sequence; new lens; new weights)."""
+    largest weights (equal ones: the lower token).  Tokens in pages that the table does not name are not among those that stay.  The rows
+    move, in order, to the pages of `out_table` [B, pages], which must not be among the pages read.  -> (kept tokens int32 [B, kv heads,
+    keep], -1 beyond a shorter sequence; new lens; new weights)."""
     args = (k_pages, v_pages, block_table, lens, weights, out_table, keep, recent, sinks)
     out = _native.paged_evict(*args)
     return _evict(*args) if out is None else out

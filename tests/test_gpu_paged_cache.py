@@ -552,3 +552,54 @@ def test_graphs_share_no_workspace_with_their_stream(b200):
         for i in range(2):
             assert all(torch.equal(o, want[i]) for o in outs[i])
         assert all(torch.equal(o, want[2]) for o in eager)
+
+
+# ----------------------------------------------------------------------------- tokens that are not there
+@pytest.mark.parametrize("lens,heads,rows,keep,recent,sinks,gone", [
+    ([40, 40, 17], 2, 8, 16, 4, 2, 0.4),                 # some more, some fewer than `keep` are there
+    ([40, 0, 7], 2, 8, 40, 30, 10, 0.5),                 # all that are there stay
+    ([300, 64, 1000], 3, 5, 64, 0, 0, 0.3),
+    ([700, 650], 1, 1, 650, 64, 8, 0.05),
+    ([33, 64], 1, 64, 20, 3, 3, 1.0),                    # none is there
+    ([20000, 9], 2, 32, 5000, 100, 4, 0.3),              # over a cluster
+    ([400001, 70], 1, 64, 30000, 300, 10, 0.2),          # whose keys are read again on each walk
+    ([400001, 70], 1, 64, 30000, 0, 0, 0.95),
+])
+@pytest.mark.parametrize("values", ["quarters", "lowest"])
+def test_evict_of_tokens_without_a_page(b200, lens, heads, rows, keep, recent, sinks, gone, values):
+    """A page that the table does not name (given back behind a window) holds no tokens that could stay: what stays is attended to as
+    the same tokens were before."""
+    g = torch.Generator(device="cuda").manual_seed(keep + rows)
+    d, L = 16, max(max(lens), keep)
+    table, pages = table_of(g, lens, rows)
+    spare = -(-keep // rows)
+    kp, vp, _, _ = pool(g, pages + spare * len(lens), heads, rows, d, torch.bfloat16)
+    kp[pages:], vp[pages:] = float("nan"), float("nan")   # what the fresh pages hold beyond the rows that move is nobody's
+    fresh = (pages + torch.randperm(spare * len(lens), device="cuda", generator=g)).to(torch.int32).view(len(lens), spare)
+    holes = torch.rand(table.shape, device="cuda", generator=g) < gone
+    table[holes] = torch.where(torch.rand(table.shape, device="cuda", generator=g) < 0.5, -1, kp.shape[0])[holes].to(torch.int32)
+    w = (torch.randn(len(lens), heads, L, device="cuda", generator=g) * 2).exp().mul(4).round().div(4)
+    if values == "lowest":
+        w = torch.where(w < 1.0, w, -float("inf"))
+        w[torch.rand(w.shape, device="cuda", generator=g) < 0.3] = float("nan")
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    kept, m, nw = b200.paged_evict(kp, vp, table, n, w, fresh, keep=keep, recent=recent, sinks=sinks)
+    for b, x in enumerate(lens):
+        at = torch.arange(x, device="cuda")
+        there = ((table[b] >= 0) & (table[b] < kp.shape[0]))[at // rows]
+        stays = min(int(there.sum()), keep)
+        assert int(m[b]) == stays
+        for h in range(heads):
+            rank = torch.where(w[b, h, :x].isnan(), -math.inf, w[b, h, :x])
+            order = rank.sort(descending=True, stable=True).indices
+            group = torch.where(there, torch.where((at < sinks) | (at >= x - recent), 2, 1), 0)
+            order = order[group[order].sort(descending=True, stable=True).indices]
+            ref = order[:stays].sort().values
+            assert torch.equal(kept[b, h, :stays].long(), ref) and (kept[b, h, stays:] == -1).all()
+            assert torch.equal(nw[b, h, :stays].view(torch.int32), w[b, h, ref].view(torch.int32)) and not nw[b, h, stays:].any()
+            j = torch.arange(stays, device="cuda")
+            for p in (kp, vp):
+                assert torch.equal(p[fresh[b].long()[j // rows], h, j % rows], p[table[b].long()[ref // rows], h, ref % rows])
+    q = torch.randn(len(lens), heads, d, device="cuda", generator=g).bfloat16()
+    ref, mass, _ = attention_ref(q, kp, vp, fresh, m.tolist(), None, None, 0, 0)
+    check_out(b200.paged_attention(q, kp, vp, fresh, m), ref, mass)
