@@ -439,8 +439,9 @@ typedef struct b200q_paged_cache {
 
 /* The rows of T new tokens into their pages: k, v [T, heads, D] (dtype B200Q_F16 or B200Q_BF16; the pages' own unless
  * those hold codes), strides: token and head of k, then of v (elements, multiples of 16 bytes, D contiguous).  The tokens
- * of sequence b are rows cu_new[b] .. cu_new[b + 1] of k and v (cu_new[0] = 0, cu_new[B] = T, ascending) and the LAST of
- * its lens[b]; cu_new NULL: one token of every sequence, T = B. */
+ * of sequence b are rows cu_new[b] .. cu_new[b + 1] of k and v (ascending; rows before cu_new[0] and from cu_new[B] on
+ * are written nowhere, so that tokens may be padded to a fixed T) and the LAST of its lens[b]; cu_new NULL: one token of every
+ * sequence, T = B. */
 int b200q_paged_append(const void* k, const void* v, int dtype, const int64_t* strides, int64_t T, const int32_t* cu_new,
                        const b200q_paged_cache* cache, const int32_t* block_table, int64_t table_stride,
                        int64_t table_width, const int32_t* lens, int64_t B, b200q_stream_t stream);

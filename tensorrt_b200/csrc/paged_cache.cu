@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     if (mine) {
       const int64_t token = static_cast<int64_t>(ld_i32(p.c.lens + b)) - fresh + at;
       int2 found = make_int2(-1, 0);
-      if (token >= 0 && token < p.c.capacity)
+      if (at >= 0 && at < fresh && token >= 0 && token < p.c.capacity)      // else: a row that no sequence brings
         found = make_int2(paged::page_of(p.c.table + b * p.c.table_stride, static_cast<int>(token), p.c), static_cast<int>(token % p.c.page_size));
       place[i] = found;
     }

@@ -26,8 +26,8 @@ _evict, _window = _ops.b200_paged_evict.default, _ops.b200_window_attention.defa
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
                  cu_new: torch.Tensor | None = None, *, k_amax: torch.Tensor | None = None, v_amax: torch.Tensor | None = None) -> None:
     """Writes k, v [tokens, kv heads, D] into the pages.  The tokens of sequence b are rows cu_new[b] .. cu_new[b + 1] and the last of
-    its lens[b] (cu_new None: one token of every sequence).  FP8 pages: codes of x / (amax / 448), `k_amax` and `v_amax` one value or
-    one per kv head."""
+    its lens[b] (cu_new None: one token of every sequence); rows behind cu_new[B] are written nowhere.  FP8 pages: codes of
+    x / (amax / 448), `k_amax` and `v_amax` one value or one per kv head."""
     if not _native.paged_append(k, v, k_pages, v_pages, block_table, lens, cu_new, k_amax, v_amax):
         _append(k, v, k_pages, v_pages, block_table, lens, cu_new, k_amax, v_amax)
 

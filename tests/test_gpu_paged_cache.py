@@ -603,3 +603,28 @@ def test_evict_of_tokens_without_a_page(b200, lens, heads, rows, keep, recent, s
     q = torch.randn(len(lens), heads, d, device="cuda", generator=g).bfloat16()
     ref, mass, _ = attention_ref(q, kp, vp, fresh, m.tolist(), None, None, 0, 0)
     check_out(b200.paged_attention(q, kp, vp, fresh, m), ref, mass)
+
+
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("counts,rows_given", [([1, 1, 1], 5), ([3, 0, 6], 40), ([0, 0, 0], 4), ([70, 1, 300], 1000)])
+def test_append_of_rows_that_no_sequence_brings(b200, counts, rows_given, codes):
+    """Rows behind the last sequence's (tokens padded to a fixed number) are written nowhere, whatever the table names there."""
+    g = torch.Generator(device="cuda").manual_seed(rows_given)
+    heads, d, rows = 2, 64, 16
+    lens = [c + 5 * i for i, c in enumerate(counts)]
+    table, pages = table_of(g, lens, rows, width=200)
+    table[table < 0] = 0                                  # entries not in use: page 0, which belongs to somebody
+    kp, vp, ka, va = pool(g, pages, heads, rows, d, E4M3 if codes else torch.bfloat16)
+    k, v = (torch.randn(rows_given, heads, d, device="cuda", generator=g).bfloat16() for _ in range(2))
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0] + counts, device="cuda").cumsum(0).to(torch.int32)
+    want_k, want_v = kp.clone(), vp.clone()
+    b200.paged_append(k[:sum(counts)], v[:sum(counts)], want_k, want_v, table, n, cu, k_amax=ka, v_amax=va)
+    b200.paged_append(k, v, kp, vp, table, n, cu, k_amax=ka, v_amax=va)
+    for got, want in ((kp, want_k), (vp, want_v)):
+        assert torch.equal(raw(got).view(torch.uint8), raw(want).view(torch.uint8))
+    later = cu + 2                                        # rows in front of the first sequence's are nobody's either
+    kp2, vp2 = want_k.clone(), want_v.clone()
+    pad = lambda t: torch.cat([torch.full_like(t[:2], 7.0), t[:sum(counts)]])  # noqa: E731
+    b200.paged_append(pad(k), pad(v), kp2, vp2, table, n, later, k_amax=ka, v_amax=va)
+    assert torch.equal(raw(kp2).view(torch.uint8), raw(want_k).view(torch.uint8)) and torch.equal(raw(vp2).view(torch.uint8), raw(want_v).view(torch.uint8))
