@@ -27,7 +27,8 @@
 // fetched once) and long ones no shorter; four CTAs to an SM for 8-bit pages 111.
 //
 // Rounding.  Products are summed in 32 bits, the softmax is 32-bit.  P is rounded to the 16-bit type of V's operand for the second
-// product: an error of one rounding of each term, of the size of the result's own.  8-bit K and V are exact in fp16; bf16
+// product: an error of one rounding of each term, of the size of the result's own; in fp16 that holds for terms down to 2^-25 of the largest
+// one of their warp's keys, and those below are off by up to 2^-36 of it (Reference).  8-bit K and V are exact in fp16; bf16
 // queries in front of them are scaled by a power of two into fp16's range, which loses nothing above 2^-38 of the largest.
 #include <atomic>
 
@@ -60,7 +61,22 @@ struct DecodeParams {
   float* parts;              // [kMaxCtas][2][kPart]
 };
 
-constexpr float kLazy = 8.0f;   // log2 of how far the reference of a sum may lie below its largest term
+// What P is referred to.  fp16 (fp16 pages, and codes, which are widened to fp16): set 2^11 below the largest term, so that P is rounded like
+// any normal number down to 2^-25 of it (2^-14 if it were set at it), and kept until a term is 2^15 above, within fp16's range.  bf16 has the range.
+template <bool HALF>
+struct Reference {
+  static constexpr float kBelow = HALF ? 11.0f : 0.0f;
+  static constexpr float kMost = HALF ? 15.0f : 8.0f;
+  // Logits from 2^24 on stand so far apart that a sum of two numbers is rounded to more than it should be.
+  __device__ static __forceinline__ float of(float top) {
+    const float r = top - kBelow;
+    return top - r > kMost ? top : r;
+  }
+  __device__ static __forceinline__ float most(float r) {
+    const float limit = r + kMost;
+    return limit - r > kMost ? r : limit;
+  }
+};
 constexpr int kPart = kRows * paged::kMaxD + 4 * kRows;   // result rows, maxima, sums; maxima and sums of a group
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -233,6 +249,7 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
   using S = Stage<CODES, DPAD, BLOCKS8>;
   constexpr bool kHalf = CODES || std::is_same<T, __half>::value;
   constexpr int kSteps = DPAD / 16;
+  using R = Reference<kHalf>;
   extern __shared__ __align__(128) char smem[];
   __shared__ float row_max[kWarps][kRows], row_sum[kWarps][kRows];
   __shared__ uint32_t there[kWarps][S::kDepth];        // which of the 16 keys of a stage exist
@@ -358,12 +375,12 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
 
     // ------------------------------------------------------------- the keys
     float o[BLOCKS8][kSteps][4];                        // O^T: rows of 16 elements, heads 2 t and 2 t + 1
-    float m[BLOCKS8][2], l[BLOCKS8][2];
+    float m[BLOCKS8][2], most[BLOCKS8][2], l[BLOCKS8][2];     // reference, up to which logit it stays, sum
 #pragma unroll
     for (int r = 0; r < BLOCKS8; ++r) {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.0f;
-      m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.0f;
+      m[r][0] = m[r][1] = most[r][0] = most[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.0f;
     }
     bool any = false;
     int slot = 0;                                       // of the tile that is requested; the next one holds the oldest
@@ -420,11 +437,11 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
               p.logits[(static_cast<int64_t>(b) * p.Hq + head0 + row) * p.logits_stride + i] = x[r][e];
           }
         }
-        // the reference stays while no logit is more than 2^8 times above it: sums and P hold that, and the exchange among lanes is rare
-        if (__any_sync(0xffffffffu, fmaxf(x[r][0], x[r][2]) > m[r][0] + kLazy || fmaxf(x[r][1], x[r][3]) > m[r][1] + kLazy)) {
-          const float m0 = fmaxf(m[r][0], column_max(fmaxf(x[r][0], x[r][2]))), m1 = fmaxf(m[r][1], column_max(fmaxf(x[r][1], x[r][3])));
+        // the reference stays while no logit is too far above it: sums and P hold that, and the exchange among lanes is rare
+        if (__any_sync(0xffffffffu, fmaxf(x[r][0], x[r][2]) > most[r][0] || fmaxf(x[r][1], x[r][3]) > most[r][1])) {
+          const float m0 = fmaxf(m[r][0], R::of(column_max(fmaxf(x[r][0], x[r][2])))), m1 = fmaxf(m[r][1], R::of(column_max(fmaxf(x[r][1], x[r][3]))));
           const float f0 = m0 == -INFINITY ? 1.0f : exp2_fast(m[r][0] - m0), f1 = m1 == -INFINITY ? 1.0f : exp2_fast(m[r][1] - m1);
-          l[r][0] *= f0, l[r][1] *= f1, m[r][0] = m0, m[r][1] = m1;
+          l[r][0] *= f0, l[r][1] *= f1, m[r][0] = m0, m[r][1] = m1, most[r][0] = R::most(m0), most[r][1] = R::most(m1);
 #pragma unroll
           for (int i = 0; i < kSteps; ++i) o[r][i][0] *= f0, o[r][i][1] *= f1, o[r][i][2] *= f0, o[r][i][3] *= f1;
         }

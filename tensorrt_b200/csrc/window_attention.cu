@@ -27,10 +27,11 @@
 // calls pay for fetching the code, and registers spill less (43.9 with those unrolled).  A branch that took a tile of sinks alone as 32 keys cost
 // more than it saved there (42.7; 8192 rows the same).
 //
-// The running maximum is followed lazily: O and the sum stay referred to an older maximum while the new one is at most 2^8 times
-// larger, which 32-bit sums and the exponent range of both 16-bit types hold without loss; so the rescaling of O in tensor memory is
+// The running maximum is followed lazily: O and the sum stay referred to an older maximum while the new one is at most 2^8 (fp16: 2^4)
+// times larger, which 32-bit sums and the types' exponents hold; so the rescaling of O in tensor memory is
 // rare.  Rounding: S, the softmax, O and the sums are 32-bit; P is rounded to 16 bits for the second product, an error of one rounding
-// of each term, of the size of the result's own.
+// of each term, of the size of the result's own; in fp16 that holds for terms down to 2^-25 of the largest, and those below are off by up to
+// 2^-36 of it (kRaise; with P of at most one, 2^-14 and 2^-25).
 //
 // A masked key has P = 0, and 0 times an infinity or a NaN of its V row would be a NaN: rows whose result is not finite are computed
 // again, by one warp each, over the keys that they see.  That costs nothing where all is finite.
@@ -47,7 +48,12 @@ namespace b200q {
 namespace {
 
 constexpr int kTileRows = 128, kTileKeys = 128;
-constexpr float kLazy = 8.0f;   // log2 of how far the reference may lie below the maximum
+// log2 of how far the reference of the sums may lie below the maximum, and of the factor that P, the sums and O carry beside it: fp16 is a
+// normal number from 2^-14 on only, so P is raised by 2^11 there and stays below 2^15.  bf16 has the range.
+template <typename T>
+constexpr float kLazy = std::is_same<T, __half>::value ? 4.0f : 8.0f;
+template <typename T>
+constexpr float kRaise = std::is_same<T, __half>::value ? 11.0f : 0.0f;
 constexpr int kPolyPairs = 2;   // of 16 pairs of exponentials: on the FMA pipe
 
 // Division of numbers below 2^31 by one that the host knows: n / d = (mulhi(n, mul) + n) >> shift.
@@ -518,7 +524,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
       if (!begun) {
         m = mx;
         begun = true;
-      } else if (__any_sync(0xffffffffu, (mx - m) * sl > kLazy)) {
+      } else if (__any_sync(0xffffffffu, (mx - m) * sl > kLazy<T>)) {
         // O is complete up to the tile before: its product was issued in front of the S that has just arrived
         const float now = fmaxf(m, mx), f = now == -INFINITY ? 1.0f : exp2_fast((m - now) * sl);
         m = now;
@@ -534,7 +540,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           ptx::tmem_st_32x32_x16(to + c * 32 + 16, o + 16);
         }
       }
-      const float back = m == -INFINITY ? 0.0f : -m * sl;
+      const float back = m == -INFINITY ? 0.0f : kRaise<T> - m * sl;
       const uint64_t back2 = pack2(back, back);
       uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll

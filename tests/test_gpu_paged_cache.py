@@ -628,3 +628,57 @@ def test_append_of_rows_that_no_sequence_brings(b200, counts, rows_given, codes)
     pad = lambda t: torch.cat([torch.full_like(t[:2], 7.0), t[:sum(counts)]])  # noqa: E731
     b200.paged_append(pad(k), pad(v), kp2, vp2, table, n, later, k_amax=ka, v_amax=va)
     assert torch.equal(raw(kp2).view(torch.uint8), raw(want_k).view(torch.uint8)) and torch.equal(raw(vp2).view(torch.uint8), raw(want_v).view(torch.uint8))
+
+
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("nats", [8.0, 12.0, 16.0])
+@pytest.mark.parametrize("dt,pt,heads,group,d,n", [
+    (torch.float16, torch.float16, 2, 4, 64, 700), (torch.float16, torch.float16, 1, 16, 128, 40), (torch.float16, E4M3, 2, 1, 128, 700),
+    (torch.bfloat16, E4M3, 1, 8, 64, 5000), (torch.bfloat16, torch.bfloat16, 1, 2, 80, 700), (torch.bfloat16, E4M3, 1, 12, 96, 20)])
+def test_keys_far_below_the_heaviest(b200, dt, pt, heads, group, d, n, nats, weighted):
+    """A first key with nearly all of the weight and no value: the result is made of the others, whose weights are far below one.  P is
+    held in 16 bits with the heaviest of its keys at 2^11 or above, so that a weight of e^-17 is still a normal number of fp16; the values
+    are large, so that the result is one too."""
+    g = torch.Generator(device="cuda").manual_seed(n + d)
+    rows = 16
+    table, pages = table_of(g, [n], rows)
+    k, v = torch.randn(n, heads, d, device="cuda", generator=g) * 0.02, (torch.rand(n, heads, d, device="cuda", generator=g) + 0.5) * 4096
+    q = torch.randn(1, heads * group, d, device="cuda", generator=g)
+    q[..., 0], k[..., 0] = 4.0, 0.0
+    k[0], v[0] = 0.0, 0.0
+    k[0, :, 0] = nats / 4
+    q, k, v = q.to(dt), k.to(dt), v.to(dt)
+    kp, vp = (torch.zeros(pages, heads, rows, d, device="cuda", dtype=pt) for _ in range(2))
+    ka, va = (torch.tensor([a], device="cuda") if pt == E4M3 else None for a in (4.0, 8192.0))
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    b200.paged_append(k, v, kp, vp, table, lens, torch.tensor([0, n], dtype=torch.int32, device="cuda"), k_amax=ka, v_amax=va)
+    w = torch.zeros(1, heads, n, device="cuda") if weighted else None
+    out = b200.paged_attention(q, kp, vp, table, lens, k_amax=ka, v_amax=va, weights=w, scale=1.0)
+    ref, mass, gained = attention_ref(q, kp, vp, table, [n], ka, va, 0, 0, scale=1.0)
+    assert (ref[..., 1:].abs() > 0).all() and gained[0, :, 0].min() > 0.5
+    check_out(out, ref, mass)
+    if weighted:
+        assert ((w.double() - gained[:, :, :n]).abs() <= 2.0 ** -12 * gained[:, :, :n]).all()
+
+
+@pytest.mark.parametrize("dt,pt", [(torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, E4M3)])
+@pytest.mark.parametrize("size", [2.0 ** e for e in (4, 12, 20, 23, 24, 25, 26, 27, 28, 30, 60)], ids=str)
+def test_logits_that_32_bits_hold_coarsely(b200, dt, pt, size):
+    """Logits whose neighbours in 32 bits are up to many nats apart, rising along the keys: P stays in the range of its type, the result a mean
+    of the values."""
+    g = torch.Generator(device="cuda").manual_seed(31)
+    n, d, rows = 1500, 64, 16
+    table, pages = table_of(g, [n], rows)
+    kp, vp, ka, va = pool(g, pages, 1, rows, d, pt)
+    rising = torch.linspace(3.0, 4.0, n, device="cuda")
+    where = (table[0].long()[torch.arange(n, device="cuda") // rows], 0, torch.arange(n, device="cuda") % rows)
+    if pt == E4M3:
+        ka = torch.tensor([448.0], device="cuda")
+        raw(kp)[where] = (rising[:, None] * torch.ones(d, device="cuda")).to(E4M3).view(torch.uint8)
+    else:
+        kp[where] = (rising[:, None] * torch.ones(d, device="cuda")).to(dt)
+    q = (torch.rand(1, 4, d, device="cuda", generator=g) + 0.5).to(dt)
+    out = b200.paged_attention(q, kp, vp, table, torch.tensor([n], dtype=torch.int32, device="cuda"), k_amax=ka, v_amax=va, scale=size / (4 * d)).float()
+    values = raw(vp)[where].view(vp.dtype).float() * (1.0 if va is None else va / 448)
+    room = 2.0 ** -6 * values.abs().amax()               # roundings of P, of its sum and of the result
+    assert torch.isfinite(out).all() and (out >= values.amin(0) - room).all() and (out <= values.amax(0) + room).all()

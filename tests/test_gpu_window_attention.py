@@ -250,3 +250,23 @@ def test_ragged_lengths_in_a_large_call(b200):
         out = b200.window_attention(q, k, v, window=window, sinks=sinks, q_lens=lens[0], k_lens=lens[1])
         ref, mass = reference(q, k, v, window, sinks, nq, nk)
         check(out, ref, mass)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("nats", [8.0, 12.0, 16.0])
+@pytest.mark.parametrize("shape", [(1, 2, 1, 300, 300, 128, 0, 0), (2, 4, 4, 129, 129, 64, 0, 0), (1, 32, 8, 61, 1999, 128, 1024, 4), (1, 4, 1, 40, 3000, 80, 0, 0),
+                                   (4, 8, 2, 2000, 2000, 128, 600, 1), (1, 32, 8, 2500, 2500, 64, 0, 0)], ids=str)
+def test_keys_far_below_the_heaviest(b200, shape, nats, dt):
+    """A first key with nearly all of the weight and no value, seen by every row: the results are made of keys whose weights, down to e^-17
+    of the heaviest, P holds as normal numbers of fp16; the values are large, so that the results are normal numbers too."""
+    b, hq, hkv, sq, sk, d, window, sinks = shape
+    g = torch.Generator(device="cuda").manual_seed(sq + d)
+    q, k, v = inputs(g, b, hq, hkv, sq, sk, d, torch.float32, False)
+    k, v = k * 0.02, (v.abs() + 0.5) * 4096
+    q[..., 0], k[..., 0] = 4.0, 0.0
+    k[:, :, 0], v[:, :, 0] = 0.0, 0.0
+    k[:, :, 0, 0] = nats / 4
+    q, k, v = q.to(dt), k.to(dt), v.to(dt)
+    out = b200.window_attention(q, k, v, window=window, sinks=sinks, scale=1.0)
+    ref, mass = reference(q, k, v, window, sinks, [sq] * b, [sk] * b, scale=1.0)
+    check(out, ref, mass)
