@@ -34,7 +34,8 @@
 // 2^-36 of it (kRaise; with P of at most one, 2^-14 and 2^-25).
 //
 // A masked key has P = 0, and 0 times an infinity or a NaN of its V row would be a NaN: rows whose result is not finite are computed
-// again, by one warp each, over the keys that they see.  That costs nothing where all is finite.
+// again, by one warp each, over the keys that they see.  That costs nothing where all is finite; where nothing is, a call takes hundreds of times
+// as long, so padding behind ragged K and V is better cleared than left as it was allocated.
 #include <cuda.h>
 
 #include <atomic>
@@ -54,6 +55,10 @@ template <typename T>
 constexpr float kLazy = std::is_same<T, __half>::value ? 4.0f : 8.0f;
 template <typename T>
 constexpr float kRaise = std::is_same<T, __half>::value ? 11.0f : 0.0f;
+// The term of the reference is 2^kRaise, and the sum is no less, but for logits from 2^24 on: there the reference is rounded by a power of two or more,
+// which cancels where the exponents of P hold it.  fp16's do not, so rows with a smaller sum (and those where P is infinite) are computed again.
+template <typename T>
+constexpr float kLeast = std::is_same<T, __half>::value ? 1024.0f : 0.0f;
 constexpr int kPolyPairs = 2;   // of 16 pairs of exponentials: on the FMA pipe
 
 // Division of numbers below 2^31 by one that the host knows: n / d = (mulhi(n, mul) + n) >> shift.
@@ -286,6 +291,7 @@ __device__ __noinline__ void join_rows(const WindowParams& p, const float* part,
     for (int r = 0; r < kRows; ++r) {
       const int row = first + r0 + r, h = head + (row >> p.rp_log2), i = q0 + (row & (p.rp - 1)), at = i < nq ? i + off : -1;
       float top = ml[r][0].x, l = 0.0f, y[4] = {};
+      bool small = false;
 #pragma unroll
       for (int k = 1; k < SPLITS; ++k) top = fmaxf(top, ml[r][k].x);
       const float base = top == -INFINITY ? 0.0f : top;
@@ -293,13 +299,14 @@ __device__ __noinline__ void join_rows(const WindowParams& p, const float* part,
       for (int k = 0; k < SPLITS; ++k) {
         const float f = exp2_fast((ml[r][k].x - base) * sl);
         l += ml[r][k].y * f;
+        small |= ml[r][k].x != -INFINITY && ml[r][k].y < kLeast<T>;
         y[0] += o[r][k].x * f, y[1] += o[r][k].y * f, y[2] += o[r][k].z * f, y[3] += o[r][k].w * f;
       }
       const float f = 1.0f / l;
       float probe = 0.0f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] *= f, probe = fmaf(y[e], 0.0f, probe);
-      if (__any_sync(0xffffffffu, lane * 4 < p.D && probe != probe) && at >= 0 && i < p.Sq) bad |= 1u << (r0 + r);
+      if (__any_sync(0xffffffffu, small || (lane * 4 < p.D && probe != probe)) && at >= 0 && i < p.Sq) bad |= 1u << (r0 + r);
       if (lane * 4 < p.D && i < p.Sq) {
         uint2 u = make_uint2(0, 0);
         if (at >= 0) u = make_uint2(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]));
@@ -638,7 +645,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
               *reinterpret_cast<const uint4*>(rows + row * kRowBytes + ((piece ^ (row & 7)) * 16));
       }
       __syncwarp();
-      for (unsigned bad = __ballot_sync(0xffffffffu, probe != probe); bad; bad &= bad - 1) {
+      for (unsigned bad = __ballot_sync(0xffffffffu, at >= 0 && (probe != probe || l < kLeast<T>)); bad; bad &= bad - 1) {
         const int who = __ffs(bad) - 1;
         row_again<T>(p, w.b, __shfl_sync(0xffffffffu, h, who), __shfl_sync(0xffffffffu, i, who), __shfl_sync(0xffffffffu, at, who));
       }

@@ -270,3 +270,18 @@ def test_keys_far_below_the_heaviest(b200, shape, nats, dt):
     out = b200.window_attention(q, k, v, window=window, sinks=sinks, scale=1.0)
     ref, mass = reference(q, k, v, window, sinks, [sq] * b, [sk] * b, scale=1.0)
     check(out, ref, mass)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sq,sk", [(700, 700), (40, 3000), (4000, 4000)])
+@pytest.mark.parametrize("size", [2.0 ** e for e in (4, 12, 20, 23, 24, 25, 26, 27, 28, 30, 60)], ids=str)
+def test_logits_that_32_bits_hold_coarsely(b200, sq, sk, dt, size):
+    """Logits whose neighbours in 32 bits are up to many nats apart, rising along the keys: every result is a mean of the values."""
+    g = torch.Generator(device="cuda").manual_seed(32)
+    q, _, v = inputs(g, 1, 4, 2, sq, sk, 64, dt, False)
+    q = (q.float().abs() + 0.5).to(dt)
+    k = (torch.linspace(3.0, 4.0, sk, device="cuda")[:, None] * torch.ones(64, device="cuda")).to(dt).expand(1, 2, sk, 64)
+    out = b200.window_attention(q, k, v, scale=size / (4 * 64)).float().view(1, 2, 2, sq, 64)
+    room = 2.0 ** -6 * v.float().abs().amax()            # roundings of P, of its sum and of the result
+    top, low = (t[:, :, None, sk - sq:] for t in (v.float().cummax(2).values, v.float().cummin(2).values))
+    assert torch.isfinite(out).all() and (out >= low - room).all() and (out <= top + room).all()
