@@ -170,17 +170,22 @@ class PagedKvCache:
         were in.  -> the kept tokens of every layer, int32 [batch, kv heads, keep]."""
         if self.weights[0] is None:
             raise ValueError("eviction goes by attention weights: the cache was made with weights=False")
+        if min(keep, recent, sinks) < 0 or recent + sinks > keep or keep > self.max_tokens:
+            raise ValueError(f"need recent + sinks <= keep <= {self.max_tokens} tokens, none negative, got {recent}, {sinks}, {keep}")
         width = -(-keep // self.page_size)
         if width * self.batch > len(self._free):
             raise RuntimeError(f"{width * self.batch} pages are needed and {len(self._free)} are free")
         fresh = [[self._free.pop() for _ in range(-(-min(keep, t) // self.page_size))] for t in self._tokens]
-        out = torch.tensor([p + [-1] * (max(width, 1) - len(p)) for p in fresh], dtype=torch.int32, device=self.table.device)
-        kept = []
-        for layer in range(self.layers):
-            which, lens, left = paged_evict(self.k[layer], self.v[layer], self.table, self.lens, self.weights[layer], out, keep=keep,
-                                            recent=recent, sinks=sinks)
-            self.weights[layer].copy_(left)      # in place, as the table and the lengths: a captured step reads them where they are
-            kept.append(which)
+        try:
+            out = torch.tensor([p + [-1] * (max(width, 1) - len(p)) for p in fresh], dtype=torch.int32, device=self.table.device)
+            cut = [paged_evict(self.k[layer], self.v[layer], self.table, self.lens, self.weights[layer], out, keep=keep, recent=recent, sinks=sinks)
+                   for layer in range(self.layers)]
+        except BaseException:                    # nothing but rows of the fresh pages has been written yet
+            self._free.extend(p for pages in reversed(fresh) for p in reversed(pages))
+            raise
+        kept = [which for which, _, _ in cut]
+        for w, (_, lens, left) in zip(self.weights, cut):
+            w.copy_(left)                        # in place, as the table and the lengths: a captured step reads them where they are
         self.lens.copy_(lens)
         self.table.fill_(-1)
         self.table[:, :width] = out[:, :width]

@@ -108,3 +108,25 @@ def test_cpu_tensors_are_refused(b200):
                  lambda: b200.window_attention(x[None], x[None], x[None])):
         with pytest.raises((RuntimeError, NotImplementedError)):
             call()
+
+
+# ----------------------------------------------------------------------------- PagedKvCache on the host
+def host_cache(b200, **kw):
+    return b200.PagedKvCache(**{**dict(layers=2, batch=3, n_kv=2, head_dim=16, pages=14, max_tokens=64, page_size=8, weights=True, device="cpu"), **kw})
+
+
+def state(cache):
+    return cache.tokens(), cache.lens.tolist(), cache.table.tolist(), sorted(cache._free), [list(p) for p in cache._pages]
+
+
+@pytest.mark.parametrize("bad", [dict(keep=16, recent=10, sinks=7), dict(keep=65), dict(keep=-1), dict(keep=8, recent=-1), dict(keep=8, sinks=-1)], ids=str)
+def test_a_refused_eviction_loses_no_pages(b200, bad):
+    cache = host_cache(b200)
+    cache.grow([20, 9, 0])
+    before = state(cache)
+    with pytest.raises(ValueError):
+        cache.evict(**bad)
+    assert state(cache) == before
+    with pytest.raises((RuntimeError, NotImplementedError)):      # no device: refused by the call behind
+        cache.evict(8, 2, 1)
+    assert state(cache) == before
