@@ -172,10 +172,10 @@ class PagedKvCache:
             raise ValueError("eviction goes by attention weights: the cache was made with weights=False")
         if min(keep, recent, sinks) < 0 or recent + sinks > keep or keep > self.max_tokens:
             raise ValueError(f"need recent + sinks <= keep <= {self.max_tokens} tokens, none negative, got {recent}, {sinks}, {keep}")
-        width = -(-keep // self.page_size)
-        if width * self.batch > len(self._free):
-            raise RuntimeError(f"{width * self.batch} pages are needed and {len(self._free)} are free")
-        fresh = [[self._free.pop() for _ in range(-(-min(keep, t) // self.page_size))] for t in self._tokens]
+        width, need = -(-keep // self.page_size), [-(-min(keep, t) // self.page_size) for t in self._tokens]
+        if sum(need) > len(self._free):
+            raise RuntimeError(f"{sum(need)} pages are needed and {len(self._free)} are free")
+        fresh = [[self._free.pop() for _ in range(n)] for n in need]
         try:
             out = torch.tensor([p + [-1] * (max(width, 1) - len(p)) for p in fresh], dtype=torch.int32, device=self.table.device)
             cut = [paged_evict(self.k[layer], self.v[layer], self.table, self.lens, self.weights[layer], out, keep=keep, recent=recent, sinks=sinks)

@@ -130,3 +130,20 @@ def test_a_refused_eviction_loses_no_pages(b200, bad):
     with pytest.raises((RuntimeError, NotImplementedError)):      # no device: refused by the call behind
         cache.evict(8, 2, 1)
     assert state(cache) == before
+
+
+def test_eviction_asks_for_the_pages_that_it_takes(b200, monkeypatch):
+    """Short sequences need room for what they have, not for `keep` tokens; one page less is too few."""
+    import tensorrt_b200.kv_cache as kv
+
+    def evict(k, v, table, lens, weights, out, *, keep, recent, sinks):
+        return torch.zeros(3, 2, keep, dtype=torch.int32), lens.clamp(max=keep), torch.zeros_like(weights)
+
+    monkeypatch.setattr(kv, "paged_evict", evict)
+    cache = host_cache(b200)
+    cache.grow([40, 9, 3])                               # 5 + 2 + 1 of 14 pages; of 32 tokens 4 + 2 + 1 would be fresh
+    with pytest.raises(RuntimeError, match="7 pages are needed and 6 are free"):
+        cache.evict(32)
+    cache.evict(24)                                      # 3 + 2 + 1
+    assert cache.tokens() == [24, 9, 3] == cache.lens.tolist() and cache.free_pages() == 8
+    assert [(r >= 0).sum().item() for r in cache.table] == [3, 2, 1]
