@@ -96,7 +96,7 @@ class PagedKvCache:
         self._free = list(range(pages - 1, -1, -1))
         self._pages: list = [[] for _ in range(batch)]     # of each sequence, in order
         self._tokens = [0] * batch
-        self._new, self._cu = [0] * batch, None
+        self._new, self._cu, self._rows = [0] * batch, None, batch      # of the last `grow`: counts, their sums on the device, rows of an append
 
     def tokens(self) -> list:
         """Tokens of each sequence."""
@@ -127,7 +127,7 @@ class PagedKvCache:
             raise ValueError(f"expected {self.batch} counts of new tokens, got {new}")
         self.reserve([t + n for t, n in zip(self._tokens, new)])
         self._tokens = [t + n for t, n in zip(self._tokens, new)]
-        self._new = list(new)
+        self._new, self._rows = list(new), sum(new)
         if all(n == 1 for n in new):
             self._cu = None
             self.lens += 1
@@ -138,6 +138,8 @@ class PagedKvCache:
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """K and V rows [tokens, kv heads, head_dim] of the tokens that `grow` made room for, sequence after sequence."""
+        if k.shape[0] != self._rows or v.shape[0] != self._rows:
+            raise ValueError(f"expected the rows of {self._rows} new tokens, got {k.shape[0]} and {v.shape[0]}")
         paged_append(k, v, self.k[layer], self.v[layer], self.table, self.lens, self._cu, k_amax=self.k_amax[layer], v_amax=self.v_amax[layer])
 
     def attend(self, layer: int, q: torch.Tensor, *, scale: float | None = None, window: int = 0, sinks: int = 0) -> torch.Tensor:

@@ -147,3 +147,15 @@ def test_eviction_asks_for_the_pages_that_it_takes(b200, monkeypatch):
     cache.evict(24)                                      # 3 + 2 + 1
     assert cache.tokens() == [24, 9, 3] == cache.lens.tolist() and cache.free_pages() == 8
     assert [(r >= 0).sum().item() for r in cache.table] == [3, 2, 1]
+
+
+def test_the_cache_takes_the_rows_that_were_announced(b200):
+    cache = host_cache(b200)
+    rows = lambda n: (torch.zeros(n, 2, 16, dtype=torch.bfloat16),) * 2  # noqa: E731
+    cache.grow([4, 0, 2])
+    for n in (3, 5, 7):
+        with pytest.raises(ValueError, match="6 new tokens"):
+            cache.append(0, *rows(n))
+    cache.grow([1, 1, 1])
+    with pytest.raises(ValueError, match="3 new tokens"):
+        cache.append(0, *rows(6))
