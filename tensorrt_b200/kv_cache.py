@@ -64,6 +64,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale
     return _window(*args) if out is None else out
 
 
+_WHOLE = "prompts are attended to as a whole: sequences must hold no tokens but the new ones"
+
+
 class PagedKvCache:
     """The pages of a batch of sequences for every layer of a decoder, and the calls above on them.
 
@@ -121,10 +124,13 @@ class PagedKvCache:
             at = torch.tensor([rows, cols, vals], device=self.table.device)
             self.table[at[0], at[1]] = at[2].int()
 
-    def grow(self, new: list) -> None:
-        """Makes room for new[b] tokens of sequence b; the next `append` of every layer brings them."""
+    def _check_counts(self, new: list) -> None:
         if len(new) != self.batch or any(n < 0 for n in new):
             raise ValueError(f"expected {self.batch} counts of new tokens, got {new}")
+
+    def grow(self, new: list) -> None:
+        """Makes room for new[b] tokens of sequence b; the next `append` of every layer brings them."""
+        self._check_counts(new)
         self.reserve([t + n for t, n in zip(self._tokens, new)])
         self._tokens = [t + n for t, n in zip(self._tokens, new)]
         self._new, self._rows = list(new), sum(new)
@@ -135,6 +141,12 @@ class PagedKvCache:
             at = torch.tensor([0] + list(new), dtype=torch.int32)
             self._cu = at.cumsum(0).to(torch.int32).to(self.lens.device)
             self.lens += at[1:].to(self.lens.device)
+
+    def check_prompt(self, new: list) -> None:
+        """Raises where `attend_prompt` would after `grow(new)`."""
+        self._check_counts(new)
+        if any(self._tokens):
+            raise ValueError(_WHOLE)
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """K and V rows [tokens, kv heads, head_dim] of the tokens that `grow` made room for, sequence after sequence."""
@@ -152,7 +164,7 @@ class PagedKvCache:
         """Attention of the tokens of whole prompts over themselves: q, k, v [tokens, heads, head_dim], sequence after sequence ->
         [tokens, query heads, head_dim].  Every sequence's tokens must be new ones."""
         if self._new != self._tokens:
-            raise ValueError("prompts are attended to as a whole: sequences must hold no tokens but the new ones")
+            raise ValueError(_WHOLE)
         most = max(self._new)
         if all(n == most for n in self._new):
             rows = lambda t: t.unflatten(0, (self.batch, most)).transpose(1, 2)  # noqa: E731
@@ -224,6 +236,8 @@ class CachedDecoder:
         if (cache.layers, cache.n_kv, cache.head_dim) != (len(stack.layers), cfg.n_kv, cfg.head_dim):
             raise ValueError(f"cache of {cache.layers} layers, {cache.n_kv} kv heads of {cache.head_dim} for a stack of {len(stack.layers)}, "
                              f"{cfg.n_kv} of {cfg.head_dim}")
+        if cache.k[0].dtype == torch.float16:
+            raise ValueError("the stack's tokens are bfloat16: pages of that type or of float8_e4m3fn, not float16")
         self.stack, self.cache, self.window, self.sinks = stack, cache, window, sinks
 
     def _walk(self, h: torch.Tensor, attend) -> torch.Tensor:
@@ -238,14 +252,19 @@ class CachedDecoder:
             h, delta = layer.forward(h, delta, core)
         return self.stack.backend.add(h, delta)
 
+    # What is refused is refused before `grow`: later the cache counts tokens that no layer holds.
+    def _check(self, h: torch.Tensor, rows: int) -> None:
+        hidden = self.stack.cfg.hidden
+        if h.dim() != 2 or tuple(h.shape) != (rows, hidden) or h.dtype != torch.bfloat16:
+            raise ValueError(f"expected [{rows}, {hidden}] of bfloat16, got {tuple(h.shape)} of {h.dtype}")
+
     def prompt(self, h: torch.Tensor, lens: list) -> torch.Tensor:
-        if h.dim() != 2 or h.shape[0] != sum(lens):
-            raise ValueError(f"expected [{sum(lens)}, hidden], got {tuple(h.shape)}")
+        self._check(h, sum(lens))
+        self.cache.check_prompt(lens)
         self.cache.grow(lens)
         return self._walk(h, lambda i, q, k, v: self.cache.attend_prompt(i, q, k, v, window=self.window, sinks=self.sinks))
 
     def step(self, h: torch.Tensor) -> torch.Tensor:
-        if h.dim() != 2 or h.shape[0] != self.cache.batch:
-            raise ValueError(f"expected [{self.cache.batch}, hidden], got {tuple(h.shape)}")
+        self._check(h, self.cache.batch)
         self.cache.grow([1] * self.cache.batch)
         return self._walk(h, lambda i, q, k, v: self.cache.attend(i, q, window=self.window, sinks=self.sinks))

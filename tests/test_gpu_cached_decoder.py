@@ -139,3 +139,20 @@ def test_what_the_classes_refuse(b200):
     cache.grow([1, 1, 1])
     with pytest.raises(ValueError, match="as a whole"):
         cache.attend_prompt(0, *(torch.zeros(3, n, 64, dtype=torch.bfloat16, device="cuda") for n in (8, 2, 2)))
+
+
+# ----------------------------------------------------------------------------- slots that are freed and filled again
+def test_a_refused_prompt_changes_nothing(b200):
+    stack, cache = make(b200)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    decoder = b200.CachedDecoder(stack, cache)
+    h = torch.randn(60, 512, device="cuda", generator=g).bfloat16()
+    decoder.prompt(h[:30], [10, 12, 8])
+    before = cache.tokens(), cache.lens.tolist(), cache.free_pages(), cache.table.clone(), [t.clone() for t in cache.k + cache.v]
+    for lens in ([20, 20, 20], [0, 60, 0]):
+        with pytest.raises(ValueError, match="as a whole"):
+            decoder.prompt(h, lens)
+        with pytest.raises(ValueError, match="expected"):
+            decoder.prompt(h[:, :256], lens)
+    assert (cache.tokens(), cache.lens.tolist(), cache.free_pages()) == before[:3] and torch.equal(cache.table, before[3])
+    assert all(torch.equal(a, b) for a, b in zip(cache.k + cache.v, before[4]))

@@ -159,3 +159,33 @@ def test_the_cache_takes_the_rows_that_were_announced(b200):
     cache.grow([1, 1, 1])
     with pytest.raises(ValueError, match="3 new tokens"):
         cache.append(0, *rows(6))
+
+
+class NoLayers:
+    """What CachedDecoder asks of a stack, without its kernels."""
+    world = 1
+
+    def __init__(self, **kw):
+        from types import SimpleNamespace
+
+        self.cfg = SimpleNamespace(**{**dict(hidden=64, n_q=4, n_kv=2, head_dim=16), **kw})
+        self.layers = [None, None]
+
+
+def test_what_the_decoder_refuses_changes_nothing(b200):
+    cache = host_cache(b200)
+    decoder = b200.CachedDecoder(NoLayers(), cache)
+    cache.grow([4, 0, 2])
+    before = state(cache)
+    h = lambda n, hidden=64: torch.zeros(n, hidden, dtype=torch.bfloat16)  # noqa: E731
+    with pytest.raises(ValueError, match="as a whole"):
+        decoder.prompt(h(5), [0, 3, 2])
+    with pytest.raises(ValueError, match="expected"):
+        decoder.prompt(h(5, 32), [0, 5, 0])
+    with pytest.raises(ValueError, match="expected"):
+        decoder.step(h(3, 32))
+    with pytest.raises(ValueError, match="counts"):
+        decoder.prompt(h(5), [0, 5])
+    assert state(cache) == before
+    with pytest.raises(ValueError, match="type"):
+        b200.CachedDecoder(NoLayers(), host_cache(b200, dtype=torch.float16))
