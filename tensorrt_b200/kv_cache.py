@@ -64,7 +64,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale
     return _window(*args) if out is None else out
 
 
-_WHOLE = "prompts are attended to as a whole: sequences must hold no tokens but the new ones"
+_WHOLE = "prompts are attended to as a whole: a sequence that brings tokens must hold no older ones"
 
 
 class PagedKvCache:
@@ -145,7 +145,7 @@ class PagedKvCache:
     def check_prompt(self, new: list) -> None:
         """Raises where `attend_prompt` would after `grow(new)`."""
         self._check_counts(new)
-        if any(self._tokens):
+        if any(n and t for n, t in zip(new, self._tokens)):
             raise ValueError(_WHOLE)
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -162,18 +162,24 @@ class PagedKvCache:
     def attend_prompt(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None, window: int = 0,
                       sinks: int = 0) -> torch.Tensor:
         """Attention of the tokens of whole prompts over themselves: q, k, v [tokens, heads, head_dim], sequence after sequence ->
-        [tokens, query heads, head_dim].  Every sequence's tokens must be new ones."""
-        if self._new != self._tokens:
+        [tokens, query heads, head_dim].  A sequence that brings tokens holds no older ones; one that brings none (a sequence that is
+        generating beside it) takes no part."""
+        if any(n and n != t for n, t in zip(self._new, self._tokens)):
             raise ValueError(_WHOLE)
-        most = max(self._new)
-        if all(n == most for n in self._new):
-            rows = lambda t: t.unflatten(0, (self.batch, most)).transpose(1, 2)  # noqa: E731
+        if q.shape[0] != sum(self._new):
+            raise ValueError(f"expected the rows of {sum(self._new)} new tokens, got {q.shape[0]}")
+        new = [n for n in self._new if n]
+        if not new:
+            return torch.empty_like(q)
+        most = max(new)
+        if min(new) == most:
+            rows = lambda t: t.unflatten(0, (len(new), most)).transpose(1, 2)  # noqa: E731
             return window_attention(rows(q), rows(k), rows(v), scale=scale, window=window, sinks=sinks).transpose(1, 2).flatten(0, 1)
-        lens = torch.tensor(self._new, dtype=torch.int32, device=q.device)
+        lens = torch.tensor(new, dtype=torch.int32, device=q.device)
         there = torch.arange(most, device=q.device) < lens[:, None]
 
         def rows(t):
-            out = t.new_zeros(self.batch, most, *t.shape[1:])
+            out = t.new_zeros(len(new), most, *t.shape[1:])
             out[there] = t
             return out.transpose(1, 2)
 
@@ -226,6 +232,7 @@ class CachedDecoder:
 
         decoder = CachedDecoder(stack, cache, window=4096, sinks=4)
         decoder.prompt(h, [n0, n1, ..])      # h [n0 + n1 + .., hidden]: the prompts, one behind the other -> the same shape
+        decoder.prompt(h, [0, n1, ..])       # sequences that go on bring none: a released one takes a new prompt
         decoder.step(h)                      # h [batch, hidden]: one token of every sequence -> the same shape
     """
 

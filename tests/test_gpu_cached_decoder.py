@@ -156,3 +156,25 @@ def test_a_refused_prompt_changes_nothing(b200):
             decoder.prompt(h[:, :256], lens)
     assert (cache.tokens(), cache.lens.tolist(), cache.free_pages()) == before[:3] and torch.equal(cache.table, before[3])
     assert all(torch.equal(a, b) for a, b in zip(cache.k + cache.v, before[4]))
+
+
+@pytest.mark.parametrize("lens", [[0, 25, 0], [13, 0, 0]])
+def test_a_freed_slot_takes_a_new_prompt(b200, lens):
+    """Beside sequences that go on: the same as in a cache of its own, and the others do not notice."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    stack, cache = make(b200)
+    decoder = b200.CachedDecoder(stack, cache, 16, 2)
+    decoder.prompt(torch.randn(90, 512, device="cuda", generator=g).bfloat16(), [40, 20, 30])
+    b = [i for i, n in enumerate(lens) if n][0]
+    cache.release(b)
+    h = torch.randn(sum(lens), 512, device="cuda", generator=g).bfloat16()
+    kept = [i for i in range(3) if i != b]
+    rows = {i: cache.k[1][cache.table[i, :2].long()].clone() for i in kept}
+    got = decoder.prompt(h, lens)
+    own_stack, own = make(b200, batch=1)
+    alone = b200.CachedDecoder(own_stack, own, 16, 2)
+    assert rel(got, alone.prompt(h, [sum(lens)])) <= 2e-2
+    assert all(torch.equal(cache.k[1][cache.table[i, :2].long()], rows[i]) for i in kept)
+    step = torch.randn(3, 512, device="cuda", generator=g).bfloat16()
+    assert rel(decoder.step(step)[b], alone.step(step[b:b + 1])[0]) <= 2e-2
+    assert cache.tokens() == [n + 1 if n else (40, 20, 30)[i] + 1 for i, n in enumerate(lens)] == cache.lens.tolist()

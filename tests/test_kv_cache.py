@@ -189,3 +189,13 @@ def test_what_the_decoder_refuses_changes_nothing(b200):
     assert state(cache) == before
     with pytest.raises(ValueError, match="type"):
         b200.CachedDecoder(NoLayers(), host_cache(b200, dtype=torch.float16))
+
+
+def test_prompts_of_some_sequences(b200):
+    cache = host_cache(b200)
+    cache.grow([4, 0, 2])
+    cache.release(2)
+    cache.check_prompt([0, 3, 5])
+    for new in ([1, 0, 0], [1, 3, 0]):
+        with pytest.raises(ValueError, match="as a whole"):
+            cache.check_prompt(new)
