@@ -71,9 +71,10 @@ class PagedKvCache:
     """The pages of a batch of sequences for every layer of a decoder, and the calls above on them.
 
     Page p of a sequence is the same page number in every layer; the pools, [pages, kv heads, page_size, head_dim] each, are allocated
-    once.  Pages are handed out on the host: `grow` before the layers of a step, with the number of new tokens of each sequence, then
-    `append` and `attend` (or `attend_prompt`) once a layer.  Inside a captured CUDA graph only these two belong; `grow` outside it,
-    and a graph that is replayed on a fixed table needs the pages of its whole run reserved in front (`reserve`).
+    once.  Pages are handed out on the host: `grow` before the layers of a step, with the number of new tokens of each sequence
+    (`grow_all`: one of each that goes on), then `append` and `attend` (or `attend_prompt`) once a layer.  Inside a captured CUDA graph
+    only these two belong; `grow` outside it, and a graph that is replayed on a fixed table needs the pages of its whole run reserved
+    in front (`reserve`).
 
     dtype bfloat16 or float16 as the tokens are, or float8_e4m3fn with `k_amax`, `v_amax`: per layer one value or one per kv head.
     `weights` True keeps the sums of attention weights by which `evict` chooses."""
@@ -99,6 +100,7 @@ class PagedKvCache:
         self._free = list(range(pages - 1, -1, -1))
         self._pages: list = [[] for _ in range(batch)]     # of each sequence, in order
         self._tokens = [0] * batch
+        self._released: set = set()
         self._new, self._cu, self._rows = [0] * batch, None, batch      # of the last `grow`: counts, their sums on the device, rows of an append
 
     def tokens(self) -> list:
@@ -133,6 +135,7 @@ class PagedKvCache:
         self._check_counts(new)
         self.reserve([t + n for t, n in zip(self._tokens, new)])
         self._tokens = [t + n for t, n in zip(self._tokens, new)]
+        self._released -= {b for b, n in enumerate(new) if n}
         self._new, self._rows = list(new), sum(new)
         if all(n == 1 for n in new):
             self._cu = None
@@ -141,6 +144,13 @@ class PagedKvCache:
             at = torch.tensor([0] + list(new), dtype=torch.int32)
             self._cu = at.cumsum(0).to(torch.int32).to(self.lens.device)
             self.lens += at[1:].to(self.lens.device)
+
+    def grow_all(self) -> None:
+        """Makes room for one new token of every sequence that has not been released.  `append` and `attend` take a row of each all the
+        same: a released one's goes nowhere, and its result is zero."""
+        new = [0 if b in self._released else 1 for b in range(self.batch)]
+        self.grow(new)
+        self._cu, self._rows = None, self.batch      # a sequence of no tokens has no place for a new one
 
     def check_prompt(self, new: list) -> None:
         """Raises where `attend_prompt` would after `grow(new)`."""
@@ -216,9 +226,10 @@ class PagedKvCache:
         return kept
 
     def release(self, b: int) -> None:
-        """Sequence b is done: its pages are free, and it is empty."""
+        """Sequence b is done: its pages are free, and it is empty until `grow` brings it tokens again."""
         self._free.extend(self._pages[b])
         self._pages[b], self._tokens[b], self._new[b] = [], 0, 0
+        self._released.add(b % self.batch)
         self.lens[b] = 0
         self.table[b] = -1
         for w in self.weights:
@@ -233,7 +244,7 @@ class CachedDecoder:
         decoder = CachedDecoder(stack, cache, window=4096, sinks=4)
         decoder.prompt(h, [n0, n1, ..])      # h [n0 + n1 + .., hidden]: the prompts, one behind the other -> the same shape
         decoder.prompt(h, [0, n1, ..])       # sequences that go on bring none: a released one takes a new prompt
-        decoder.step(h)                      # h [batch, hidden]: one token of every sequence -> the same shape
+        decoder.step(h)                      # h [batch, hidden]: one token of every sequence that is not released -> the same shape
     """
 
     def __init__(self, stack, cache: PagedKvCache, window: int = 0, sinks: int = 0):
@@ -273,5 +284,5 @@ class CachedDecoder:
 
     def step(self, h: torch.Tensor) -> torch.Tensor:
         self._check(h, self.cache.batch)
-        self.cache.grow([1] * self.cache.batch)
+        self.cache.grow_all()
         return self._walk(h, lambda i, q, k, v: self.cache.attend(i, q, window=self.window, sinks=self.sinks))

@@ -178,3 +178,24 @@ def test_a_freed_slot_takes_a_new_prompt(b200, lens):
     step = torch.randn(3, 512, device="cuda", generator=g).bfloat16()
     assert rel(decoder.step(step)[b], alone.step(step[b:b + 1])[0]) <= 2e-2
     assert cache.tokens() == [n + 1 if n else (40, 20, 30)[i] + 1 for i, n in enumerate(lens)] == cache.lens.tolist()
+
+
+def test_steps_leave_freed_slots_alone(b200):
+    """A freed slot takes no token and no page; its row of a step is nobody's."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    h = torch.randn(60, 512, device="cuda", generator=g).bfloat16()
+    steps = torch.randn(20, 3, 512, device="cuda", generator=g).bfloat16()
+    outs = []
+    for freed in (False, True):
+        stack, cache = make(b200, weights=True)
+        decoder = b200.CachedDecoder(stack, cache)
+        decoder.prompt(h, [10, 30, 20])
+        if freed:
+            cache.release(1)
+        free = cache.free_pages()
+        outs.append([decoder.step(s) for s in steps])
+        if freed:
+            assert cache.tokens() == [30, 0, 40] == cache.lens.tolist() and (cache.table[1] == -1).all()
+            assert free - cache.free_pages() == (4 - 2) + (5 - 3) and not cache.weights[0][1].any()
+    for a, b in zip(*outs):
+        assert torch.isfinite(b.float()).all() and torch.equal(a[0::2], b[0::2])

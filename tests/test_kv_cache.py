@@ -199,3 +199,15 @@ def test_prompts_of_some_sequences(b200):
     for new in ([1, 0, 0], [1, 3, 0]):
         with pytest.raises(ValueError, match="as a whole"):
             cache.check_prompt(new)
+
+
+def test_a_released_sequence_takes_no_token_of_a_step(b200):
+    cache = host_cache(b200)
+    cache.grow([4, 9, 2])
+    cache.release(1)
+    for _ in range(40):
+        cache.grow_all()
+    assert cache.tokens() == [44, 0, 42] == cache.lens.tolist() and cache.free_pages() == 14 - 12
+    cache.grow([0, 3, 0])                                # until it is asked for by name
+    cache.grow_all()
+    assert cache.tokens() == [45, 4, 43] == cache.lens.tolist() and cache.free_pages() == 14 - 13
