@@ -64,6 +64,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale
     return _window(*args) if out is None else out
 
 
+def _on_device(values, device, dtype=torch.int32) -> torch.Tensor:
+    """Values of the host as a tensor on `device`, without a wait for its stream (a copy from pageable memory is one)."""
+    t = torch.as_tensor(values, dtype=dtype)
+    return t.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else t
+
+
 _WHOLE = "prompts are attended to as a whole: a sequence that brings tokens must hold no older ones"
 
 
@@ -101,6 +107,7 @@ class PagedKvCache:
         self._pages: list = [[] for _ in range(batch)]     # of each sequence, in order
         self._tokens = [0] * batch
         self._released: set = set()
+        self._padded = None
         self._new, self._cu, self._rows = [0] * batch, None, batch      # of the last `grow`: counts, their sums on the device, rows of an append
 
     def tokens(self) -> list:
@@ -123,8 +130,8 @@ class PagedKvCache:
                 rows.append(b), cols.append(len(self._pages[b])), vals.append(self._free.pop())
                 self._pages[b].append(vals[-1])
         if vals:
-            at = torch.tensor([rows, cols, vals], device=self.table.device)
-            self.table[at[0], at[1]] = at[2].int()
+            at = _on_device([rows, cols, vals], self.table.device)
+            self.table[at[0], at[1]] = at[2]
 
     def _check_counts(self, new: list) -> None:
         if len(new) != self.batch or any(n < 0 for n in new):
@@ -141,9 +148,22 @@ class PagedKvCache:
             self._cu = None
             self.lens += 1
         else:
-            at = torch.tensor([0] + list(new), dtype=torch.int32)
-            self._cu = at.cumsum(0).to(torch.int32).to(self.lens.device)
-            self.lens += at[1:].to(self.lens.device)
+            counts = torch.tensor([0] + self._new, dtype=torch.int32)
+            both = _on_device(torch.stack([counts.cumsum(0), counts]), self.lens.device)
+            self._cu = both[0]
+            self.lens += both[1, 1:]
+        self._padded = self._padding()
+
+    def _padding(self):
+        """Of prompts of different lengths: (longest, lengths, place of each token among rows of that length); else None.  Made once for
+        all layers, from what the host knows."""
+        new = [n for n in self._new if n]
+        if not new or min(new) == max(new) or self._new != [t if n else 0 for n, t in zip(self._new, self._tokens)]:
+            return None
+        counts = torch.tensor(new)
+        first = counts.cumsum(0) - counts
+        place = torch.arange(sum(new)) + torch.repeat_interleave(torch.arange(len(new)) * max(new) - first, counts)
+        return max(new), _on_device(counts, self.lens.device), _on_device(place, self.lens.device, torch.int64)
 
     def grow_all(self) -> None:
         """Makes room for one new token of every sequence that has not been released.  `append` and `attend` take a row of each all the
@@ -181,19 +201,17 @@ class PagedKvCache:
         new = [n for n in self._new if n]
         if not new:
             return torch.empty_like(q)
-        most = max(new)
-        if min(new) == most:
-            rows = lambda t: t.unflatten(0, (len(new), most)).transpose(1, 2)  # noqa: E731
+        if self._padded is None:
+            rows = lambda t: t.unflatten(0, (len(new), new[0])).transpose(1, 2)  # noqa: E731
             return window_attention(rows(q), rows(k), rows(v), scale=scale, window=window, sinks=sinks).transpose(1, 2).flatten(0, 1)
-        lens = torch.tensor(new, dtype=torch.int32, device=q.device)
-        there = torch.arange(most, device=q.device) < lens[:, None]
+        most, lens, place = self._padded
 
         def rows(t):
-            out = t.new_zeros(len(new), most, *t.shape[1:])
-            out[there] = t
-            return out.transpose(1, 2)
+            out = t.new_zeros(len(new) * most, *t.shape[1:])
+            return out.index_copy_(0, place, t).unflatten(0, (len(new), most)).transpose(1, 2)
 
-        return window_attention(rows(q), rows(k), rows(v), scale=scale, window=window, sinks=sinks, q_lens=lens, k_lens=lens).transpose(1, 2)[there]
+        out = window_attention(rows(q), rows(k), rows(v), scale=scale, window=window, sinks=sinks, q_lens=lens, k_lens=lens)
+        return out.transpose(1, 2).flatten(0, 1).index_select(0, place)
 
     def evict(self, keep: int, recent: int = 0, sinks: int = 0) -> list:
         """Cuts every sequence to `keep` tokens per kv head, by the sums of attention weights of each layer, and frees the pages they
@@ -207,7 +225,7 @@ class PagedKvCache:
             raise RuntimeError(f"{sum(need)} pages are needed and {len(self._free)} are free")
         fresh = [[self._free.pop() for _ in range(n)] for n in need]
         try:
-            out = torch.tensor([p + [-1] * (max(width, 1) - len(p)) for p in fresh], dtype=torch.int32, device=self.table.device)
+            out = _on_device([p + [-1] * (max(width, 1) - len(p)) for p in fresh], self.table.device)
             cut = [paged_evict(self.k[layer], self.v[layer], self.table, self.lens, self.weights[layer], out, keep=keep, recent=recent, sinks=sinks)
                    for layer in range(self.layers)]
         except BaseException:                    # nothing but rows of the fresh pages has been written yet
@@ -230,11 +248,11 @@ class PagedKvCache:
         self._free.extend(self._pages[b])
         self._pages[b], self._tokens[b], self._new[b] = [], 0, 0
         self._released.add(b % self.batch)
-        self.lens[b] = 0
-        self.table[b] = -1
+        self.lens[b].zero_()
+        self.table[b].fill_(-1)
         for w in self.weights:
             if w is not None:
-                w[b] = 0
+                w[b].zero_()
 
 
 class CachedDecoder:

@@ -199,3 +199,22 @@ def test_steps_leave_freed_slots_alone(b200):
             assert free - cache.free_pages() == (4 - 2) + (5 - 3) and not cache.weights[0][1].any()
     for a, b in zip(*outs):
         assert torch.isfinite(b.float()).all() and torch.equal(a[0::2], b[0::2])
+
+
+@pytest.mark.parametrize("lens", [[21, 21, 21], [40, 7, 90], [0, 9, 300]])
+def test_prompts_and_steps_do_not_wait_for_the_device(b200, lens):
+    g = torch.Generator(device="cuda").manual_seed(8)
+    h = torch.randn(sum(lens), 512, device="cuda", generator=g).bfloat16()
+    step = torch.randn(3, 512, device="cuda", generator=g).bfloat16()
+    for _ in range(2):                                    # once for what is set up on first use
+        stack, cache = make(b200)
+        decoder = b200.CachedDecoder(stack, cache, 30, 1)
+        torch.cuda.synchronize()
+        torch.cuda.set_sync_debug_mode("error" if _ else "default")
+        try:
+            decoder.prompt(h, lens)
+            cache.release(1)
+            decoder.step(step)
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+    assert cache.tokens() == [lens[0] + 1, 0, lens[2] + 1] == cache.lens.tolist()
