@@ -17,11 +17,13 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/TensorSubclassLikeUtils.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime_api.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
@@ -560,13 +562,17 @@ PyObject* py_decoder_stack(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // ---------------------------------------------------------------- paged key-value cache
 // The same bodies as the torch.library ops, without the dispatcher in front: 4 to 8 us of a call's host time, which is longer than the
 // kernels of a small batch run.  `tensors`: arguments that are tensors, or None where the function takes that.
+// Not taken, since torch has its part in them: inputs that require gradients (the op's result says that it has none) or carry tangents, and
+// calls that are traced.
 bool all_plain(PyObject* const* a, int tensors, std::optional<Tensor>* t) {
+  const bool grad = c10::GradMode::is_enabled();
   for (int i = 0; i < tensors; ++i) {
     if (a[i] == Py_None) continue;
     if (!plain(a[i])) return false;
     t[i] = THPVariable_Unpack(a[i]);
+    if ((grad && t[i]->requires_grad()) || t[i]->_fw_grad(0).defined()) return false;
   }
-  return !modes_active();
+  return !modes_active() && !torch::jit::tracer::isTracing();
 }
 bool ints(PyObject* const* a, int n, int64_t* out) {
   for (int i = 0; i < n; ++i) {

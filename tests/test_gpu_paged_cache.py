@@ -682,3 +682,36 @@ def test_logits_that_32_bits_hold_coarsely(b200, dt, pt, size):
     values = raw(vp)[where].view(vp.dtype).float() * (1.0 if va is None else va / 448)
     room = 2.0 ** -6 * values.abs().amax()               # roundings of P, of its sum and of the result
     assert torch.isfinite(out).all() and (out >= values.amin(0) - room).all() and (out <= values.amax(0) + room).all()
+
+
+def test_inputs_that_require_gradients(b200):
+    """No gradient is defined: a result of such inputs says so as that of the op does, and is not a constant without a word."""
+    from torch.autograd import forward_ad
+
+    g = torch.Generator(device="cuda").manual_seed(21)
+    table, pages = table_of(g, [40, 9], 16)
+    kp, vp, _, _ = pool(g, pages, 2, 16, 64, torch.bfloat16)
+    n = torch.tensor([40, 9], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 4, 64, device="cuda", generator=g).bfloat16()
+    x = torch.randn(1, 2, 40, 64, device="cuda", generator=g).bfloat16()
+    ops = torch.ops.tensorrt
+    calls = [(lambda t: b200.paged_attention(t, kp, vp, table, n), lambda t: ops.b200_paged_attention(t, kp, vp, table, n, None, None, None, 0.0, 0, 0), q),
+             (lambda t: b200.window_attention(t, x, x), lambda t: ops.b200_window_attention(t, x, x, None, None, 0.0, 0, 0), x),
+             (lambda t: b200.window_attention(x, x, t), lambda t: ops.b200_window_attention(x, x, t, None, None, 0.0, 0, 0), x)]
+    for f, op, t in calls:
+        plain = f(t)
+        assert not plain.requires_grad
+        leaf = t.clone().requires_grad_()
+        assert f(leaf).requires_grad and op(leaf).requires_grad and torch.equal(f(leaf), plain)
+        with torch.no_grad():
+            assert not f(leaf).requires_grad and torch.equal(f(leaf), plain)
+
+        def dual(call):
+            with forward_ad.dual_level():
+                try:
+                    return forward_ad.unpack_dual(call(forward_ad.make_dual(t, torch.ones_like(t)))).tangent is None
+                except (RuntimeError, NotImplementedError) as e:
+                    return str(e)
+
+        assert dual(f) == dual(op)
+        assert "b200_" in str(torch.jit.trace(f, (t,), check_trace=False).graph)
