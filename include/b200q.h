@@ -455,10 +455,11 @@ int b200q_paged_append(const void* k, const void* v, int dtype, const int64_t* s
  * kv head h, for keys j < weights_len that are seen.
  * workspace: b200q_paged_attention_workspace_bytes() bytes, 16-byte aligned; its first B200Q_PAGED_ATTENTION_ZERO_BYTES are
  * zero the first time it is used and are left zero again; calls sharing one must not overlap.  scratch (with weights only):
- * b200q_paged_attention_scratch_bytes(B, Hq, weights_len) bytes, any content. */
+ * b200q_paged_attention_scratch_bytes(B, Hq, keys) bytes, any content; keys: the least of weights_len, table_width * page_size and
+ * (window > 0) window + sinks. */
 #define B200Q_PAGED_ATTENTION_ZERO_BYTES 4096
 size_t b200q_paged_attention_workspace_bytes(void);
-size_t b200q_paged_attention_scratch_bytes(int64_t B, int64_t Hq, int64_t weights_len);
+size_t b200q_paged_attention_scratch_bytes(int64_t B, int64_t Hq, int64_t keys);
 int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, const b200q_paged_cache* cache,
                           const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* lens,
                           int64_t B, int64_t Hq, float scale, int64_t window, int64_t sinks, void* out, float* weights,

@@ -686,9 +686,9 @@ extern "C" {
 
 size_t b200q_paged_attention_workspace_bytes(void) { return 2 * kMaxCtas * sizeof(unsigned) + static_cast<size_t>(kMaxCtas) * 2 * kPart * sizeof(float); }
 
-size_t b200q_paged_attention_scratch_bytes(int64_t B, int64_t Hq, int64_t weights_len) {
-  if (B <= 0 || Hq <= 0 || weights_len < 0) return 16;
-  return static_cast<size_t>(B * Hq) * (round4(weights_len) + 1) * sizeof(float) + 16;
+size_t b200q_paged_attention_scratch_bytes(int64_t B, int64_t Hq, int64_t keys) {
+  if (B <= 0 || Hq <= 0 || keys < 0) return 16;
+  return static_cast<size_t>(B * Hq) * (round4(keys) + 1) * sizeof(float) + 16;
 }
 
 int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, const b200q_paged_cache* cache, const int32_t* block_table,
@@ -703,7 +703,10 @@ int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, co
     return B200Q_ERR_INVALID;
   if (!aligned(q, 16) || !aligned(out, 16) || !paged::strides_ok(q_strides, 2, 8)) return B200Q_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < b200q_paged_attention_workspace_bytes()) return B200Q_ERR_WORKSPACE;
-  if (weights != nullptr && (scratch == nullptr || scratch_bytes < b200q_paged_attention_scratch_bytes(B, Hq, weights_len))) return B200Q_ERR_WORKSPACE;
+  // keys that a token of the longest sequence in the table sees
+  const int64_t most = window > 0 && sinks < (1LL << 40) && window < (1LL << 40) && window + sinks < p.c.capacity ? window + sinks : p.c.capacity;
+  const int64_t keys = most < weights_len ? most : weights_len;
+  if (weights != nullptr && (scratch == nullptr || scratch_bytes < b200q_paged_attention_scratch_bytes(B, Hq, keys))) return B200Q_ERR_WORKSPACE;
   if (!aligned(workspace, 16) || !aligned(scratch, 16)) return B200Q_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
   p.page_shift = -1;
@@ -722,19 +725,18 @@ int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, co
   p.tickets = static_cast<unsigned*>(workspace);
   p.parts = reinterpret_cast<float*>(p.tickets + 2 * kMaxCtas);
   if (weights != nullptr && weights_len > 0) {
-    p.logits_stride = round4(weights_len);
+    p.logits_stride = round4(keys);
     p.weights_len = weights_len;
     p.logits = static_cast<float*>(scratch);
     p.lse = p.logits + B * Hq * p.logits_stride;
   }
-  // the longest sequence that the table can hold: no more CTAs than tiles
-  const int64_t most = window > 0 && sinks < (1LL << 40) && window < (1LL << 40) && window + sinks < p.c.capacity ? window + sinks : p.c.capacity;
+  // no more CTAs than tiles
   const int64_t tiles = (most > 0 ? (most + kTile - 1) / kTile : 1) * B * p.c.heads * p.blocks;
   const auto st = static_cast<cudaStream_t>(stream);
   const int rc = dtype == B200Q_BF16 ? (p.c.codes ? launch_decode_d<__nv_bfloat16, true>(p, tiles, st) : launch_decode_d<__nv_bfloat16, false>(p, tiles, st))
                                      : (p.c.codes ? launch_decode_d<__half, true>(p, tiles, st) : launch_decode_d<__half, false>(p, tiles, st));
   if (rc != B200Q_OK || p.logits == nullptr) return rc;
-  const int64_t keys = most < weights_len ? most : weights_len, chunks = (keys + 255) / 256;
+  const int64_t chunks = (keys + 255) / 256;
   const dim3 grid(static_cast<unsigned>(chunks < 1 ? 1 : (chunks < 65535 ? chunks : 65535)), static_cast<unsigned>(p.c.heads), static_cast<unsigned>(B));
   if (launch_pdl(weights_kernel, grid, dim3(256), 0, st, p, weights) != cudaSuccess) return B200Q_ERR_CUDA;
   return check_launch();

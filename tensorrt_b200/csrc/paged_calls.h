@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime_api.h>
 
+#include <algorithm>
 #include <cmath>
 #include <map>
 #include <mutex>
@@ -193,7 +194,9 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& 
                 op, ": weights must be contiguous float32 [", a.B, ", ", a.c.heads, ", keys], got ", weights->sizes(), " of ", weights->scalar_type());
     w = weights->data_ptr<float>();
     wl = weights->size(2);
-    scratch = at::empty({static_cast<int64_t>(b200q_paged_attention_scratch_bytes(a.B, Hq, wl))}, q_in.options().dtype(at::kByte));
+    int64_t keys = std::min<int64_t>(wl, a.table_width * a.c.page_size);       // logits of what a token can see
+    if (window > 0 && window < keys && sinks < keys) keys = std::min(keys, window + sinks);
+    scratch = at::empty({static_cast<int64_t>(b200q_paged_attention_scratch_bytes(a.B, Hq, keys))}, q_in.options().dtype(at::kByte));
   }
   Tensor out = at::empty(q_in.sizes(), q_in.options());
   if (a.B == 0) return out;

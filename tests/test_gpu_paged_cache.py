@@ -715,3 +715,24 @@ def test_inputs_that_require_gradients(b200):
 
         assert dual(f) == dual(op)
         assert "b200_" in str(torch.jit.trace(f, (t,), check_trace=False).graph)
+
+
+@pytest.mark.parametrize("window,sinks", [(100, 4), (0, 0)])
+def test_wide_tables_and_weights_take_no_more_room_than_what_is_seen(b200, window, sinks):
+    g = torch.Generator(device="cuda").manual_seed(22)
+    lens, heads, group, rows, d = [3000, 40, 0, 101], 4, 8, 16, 64
+    width = 8192 if window else 200                       # 131072 tokens, of which a window sees 104
+    table, pages = table_of(g, lens, rows, width=width)
+    kp, vp, _, _ = pool(g, pages, heads, rows, d, torch.bfloat16)
+    q = torch.randn(4, heads * group, d, device="cuda", generator=g).bfloat16()
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    w = torch.zeros(4, heads, 131072, device="cuda")
+    b200.paged_attention(q, kp, vp, table, n, weights=w, window=window, sinks=sinks)      # the workspace is there
+    w.zero_()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = b200.paged_attention(q, kp, vp, table, n, weights=w, window=window, sinks=sinks)
+    assert torch.cuda.max_memory_allocated() - before <= 4 * 32 * 4 * ((104 if window else 3200) + 4) + (1 << 20)
+    ref, mass, gained = attention_ref(q, kp, vp, table[:, :200], lens, None, None, window, sinks)
+    check_out(out, ref, mass)
+    assert (w[..., :3200].double() - gained).abs().max() <= 2.0 ** -10 and not w[..., 3200:].any()

@@ -211,3 +211,18 @@ def test_a_released_sequence_takes_no_token_of_a_step(b200):
     cache.grow([0, 3, 0])                                # until it is asked for by name
     cache.grow_all()
     assert cache.tokens() == [45, 4, 43] == cache.lens.tolist() and cache.free_pages() == 14 - 13
+
+
+def test_scratch_is_for_the_keys_that_can_be_seen(b200, p):
+    from tensorrt_b200 import _lib
+
+    lib, i64 = _lib.load(), ctypes.c_int64
+    c, s2 = ctypes.byref(cache_of(p)), (i64 * 2)(128, 64)     # pages of 16 rows
+    attend = lambda sn, width, window, sinks, wl: lib.b200q_paged_attention(  # noqa: E731
+        p, 2, s2, c, p, width, width, p, 3, 4, 1.0, window, sinks, p, p, wl, p, 1 << 40, p, sn, None)
+    for width, window, sinks, wl, keys in ((4, 0, 0, 64, 64), (4, 0, 0, 1 << 17, 64), (1 << 13, 0, 0, 500, 500), (1 << 13, 100, 20, 1 << 17, 120),
+                                           (1 << 13, 100, 1 << 62, 1 << 17, 1 << 17), (4, 1 << 62, 3, 1 << 17, 64), (0, 0, 0, 64, 0)):
+        n = lib.b200q_paged_attention_scratch_bytes(3, 4, keys)
+        assert attend(n - 1, width, window, sinks, wl) == -5
+        if not torch.cuda.is_available():
+            assert attend(n, width, window, sinks, wl) not in (0, -1, -2, -5)     # as far as the device
