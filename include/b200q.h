@@ -493,6 +493,12 @@ int b200q_window_attention(const void* q, const void* k, const void* v, int dtyp
                            int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, float scale, int64_t window, int64_t sinks,
                            b200q_stream_t stream);
 
+/* The form that the call above takes at these sizes on the current device: form[0] query tiles of 128 rows a CTA (1 or 2), form[1] CTAs
+ * of a cluster that share an item's keys (1, 2, 4, 8), form[2] whether two query tiles are of two heads (1) or of two blocks of rows (0).
+ * It goes by the sizes of the tensors alone. */
+int b200q_window_attention_form(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, int64_t window,
+                                int64_t sinks, int32_t form[3]);
+
 /* ------------------------------------------------------------------ glue of the decoder linear stack
  * The benchmark workloads wrap the quantized linears in a Llama-shaped decoder layer
  * (RMSNorm -> QKV -> attention replaced by identity on V -> O -> residual -> RMSNorm ->

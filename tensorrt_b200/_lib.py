@@ -64,6 +64,7 @@ SIGNATURES = {
     "b200q_paged_attention": (_c.c_int, [_p, _c.c_int, _p, _p, _p, _i64, _i64, _p, _i64, _i64, _c.c_float, _i64, _i64, _p, _p, _i64, _p, _c.c_size_t, _p, _c.c_size_t, _p]),
     "b200q_paged_evict": (_c.c_int, [_p, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p]),
     "b200q_window_attention": (_c.c_int, [_p, _p, _p, _c.c_int, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _c.c_float, _i64, _i64, _p]),
+    "b200q_window_attention_form": (_c.c_int, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
     "b200q_rms_norm": (_c.c_int, [_p, _p, _p, _i64, _i64, _c.c_float, _p]),
     "b200q_add_rms_norm_fp8_quantize": (_c.c_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _c.c_float, _p]),
     "b200q_silu_mul": (_c.c_int, [_p, _p, _i64, _i64, _p]),

@@ -729,6 +729,28 @@ Shape choose_shape(const WindowParams& p) {
   return best;
 }
 
+bool sizes_ok(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, int64_t sinks) {
+  return !(B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Sq < 0 || Sk < 0 || Sq > 0x3fffff00LL || Sk > 0x3fffff00LL || D <= 0 || D > 128 ||
+           D % 16 != 0 || sinks < 0 || B > 65535 || Hq > 0x7fffffffLL || B * Hq > 65535);
+}
+
+// The sizes of a call, what a query tile holds, and its form.
+Shape plan(WindowParams* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, int64_t window, int64_t sinks) {
+  p->Hq = static_cast<int>(Hq), p->Hkv = static_cast<int>(Hkv), p->group = static_cast<int>(Hq / Hkv);
+  p->Sq = static_cast<int>(Sq), p->Sk = static_cast<int>(Sk), p->D = static_cast<int>(D), p->B = static_cast<int>(B);
+  p->window = window <= 0 || window >= Sk ? 0 : static_cast<int>(window);     // as wide as the keys: none
+  p->sinks = static_cast<int>(sinks < Sk ? sinks : Sk);
+  // few queries: the rows of several heads of a group in one tile
+  p->rp = kTileRows, p->nh = 1;
+  while (p->rp > 8 && Sq <= p->rp / 2 && p->group % (2 * p->nh) == 0) p->rp /= 2, p->nh *= 2;
+  const Shape shape = choose_shape(*p);
+  p->pair_heads = shape.nq == 2 && p->group % (2 * p->nh) == 0 ? 1 : 0;
+  p->units = p->group / (p->pair_heads ? 2 * p->nh : p->nh);
+  p->q_blocks = static_cast<int>(blocks_of(*p, shape.nq));
+  p->splits = shape.splits;
+  return shape;
+}
+
 template <typename T, int DPAD, int NQ>
 int launch_window(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const WindowParams& p, unsigned ctas, cudaStream_t st) {
   using L = Layout<DPAD, NQ>;
@@ -776,13 +798,20 @@ using namespace b200q;
 
 extern "C" {
 
+int b200q_window_attention_form(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, int64_t window, int64_t sinks, int32_t form[3]) {
+  if (!sizes_ok(B, Hq, Hkv, Sq, Sk, D, sinks) || B == 0 || Sq == 0 || form == nullptr) return B200Q_ERR_INVALID;
+  if (int rc = check_arch()) return rc;
+  WindowParams p{};
+  const Shape shape = plan(&p, B, Hq, Hkv, Sq, Sk, D, window, sinks);
+  form[0] = shape.nq, form[1] = shape.splits, form[2] = p.pair_heads;
+  return B200Q_OK;
+}
+
 int b200q_window_attention(const void* q, const void* k, const void* v, int dtype, const int64_t* strides, void* out, const int64_t* out_strides,
                            const int32_t* q_lens, const int32_t* k_lens, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D,
                            float scale, int64_t window, int64_t sinks, b200q_stream_t stream) {
   if (dtype != B200Q_F16 && dtype != B200Q_BF16) return B200Q_ERR_INVALID;
-  if (B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Sq < 0 || Sk < 0 || Sq > 0x3fffff00LL || Sk > 0x3fffff00LL || D <= 0 || D > 128 ||
-      D % 16 != 0 || sinks < 0 || !(scale >= 0.0f) || B > 65535 || B * Hq > 65535)
-    return B200Q_ERR_INVALID;
+  if (!sizes_ok(B, Hq, Hkv, Sq, Sk, D, sinks) || !(scale >= 0.0f)) return B200Q_ERR_INVALID;
   if (B == 0 || Sq == 0) return B200Q_OK;
   if (q == nullptr || out == nullptr || strides == nullptr || out_strides == nullptr || (Sk > 0 && (k == nullptr || v == nullptr))) return B200Q_ERR_INVALID;
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16)) return B200Q_ERR_ALIGN;
@@ -796,21 +825,10 @@ int b200q_window_attention(const void* q, const void* k, const void* v, int dtyp
   p.q = static_cast<const char*>(q), p.k = static_cast<const char*>(k), p.v = static_cast<const char*>(v), p.out = static_cast<char*>(out);
   for (int i = 0; i < 3; ++i) p.q_s[i] = strides[i], p.k_s[i] = strides[3 + i], p.v_s[i] = strides[6 + i], p.o_s[i] = out_strides[i];
   p.q_lens = q_lens, p.k_lens = k_lens;
-  p.Hq = static_cast<int>(Hq), p.Hkv = static_cast<int>(Hkv), p.group = static_cast<int>(Hq / Hkv);
-  p.Sq = static_cast<int>(Sq), p.Sk = static_cast<int>(Sk), p.D = static_cast<int>(D), p.B = static_cast<int>(B);
   p.scale = scale;
-  p.window = window <= 0 || window >= Sk ? 0 : static_cast<int>(window);     // as wide as the keys: none
-  p.sinks = static_cast<int>(sinks < Sk ? sinks : Sk);
   p.status = gemm::device_status_word();
   if (p.status == nullptr) return B200Q_ERR_CUDA;
-  // few queries: the rows of several heads of a group in one tile
-  p.rp = kTileRows, p.nh = 1;
-  while (p.rp > 8 && Sq <= p.rp / 2 && p.group % (2 * p.nh) == 0) p.rp /= 2, p.nh *= 2;
-  const Shape shape = choose_shape(p);
-  p.pair_heads = shape.nq == 2 && p.group % (2 * p.nh) == 0 ? 1 : 0;
-  p.units = p.group / (p.pair_heads ? 2 * p.nh : p.nh);
-  p.q_blocks = static_cast<int>(blocks_of(p, shape.nq));
-  p.splits = shape.splits;
+  const Shape shape = plan(&p, B, Hq, Hkv, Sq, Sk, D, window, sinks);
   while ((1 << p.rp_log2) < p.rp) ++p.rp_log2;
   p.by_split = divisor(static_cast<uint32_t>(p.splits));
   p.by_block = divisor(static_cast<uint32_t>(B * Hkv * p.units));

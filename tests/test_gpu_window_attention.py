@@ -285,3 +285,100 @@ def test_logits_that_32_bits_hold_coarsely(b200, sq, sk, dt, size):
     room = 2.0 ** -6 * v.float().abs().amax()            # roundings of P, of its sum and of the result
     top, low = (t[:, :, None, sk - sq:] for t in (v.float().cummax(2).values, v.float().cummin(2).values))
     assert torch.isfinite(out).all() and (out >= low - room).all() and (out <= top + room).all()
+
+
+# ----------------------------------------------------------------------------- the forms by name
+# sizes -> (query tiles a CTA, CTAs that share an item's keys, the two tiles are of two heads) on 148 SMs
+NAMED = [
+    ((4, 8, 2, 900, 900, 128, 200, 2), (2, 1, 1)), ((5, 16, 4, 1000, 1000, 112, 0, 0), (2, 1, 1)),
+    ((4, 20, 4, 193, 977, 80, 0, 4), (2, 1, 0)), ((4, 10, 2, 404, 1013, 128, 1000, 1), (2, 1, 0)),
+    ((4, 16, 4, 280, 1345, 64, 0, 130), (2, 1, 1)), ((2, 16, 8, 591, 1478, 48, 1000, 4), (2, 1, 1)), ((4, 20, 4, 149, 2454, 48, 0, 4), (2, 1, 0)),
+    ((7, 4, 2, 400, 450, 80, 0, 0), (1, 1, 0)), ((1, 16, 4, 2000, 2000, 64, 0, 0), (1, 1, 0)), ((8, 12, 12, 500, 500, 128, 130, 1), (1, 1, 0)),
+    ((8, 12, 4, 28, 2252, 128, 0, 130), (1, 2, 0)), ((3, 8, 8, 278, 1100, 80, 1000, 1), (1, 2, 0)), ((2, 40, 8, 53, 1155, 64, 0, 4), (1, 2, 0)),
+    ((1, 20, 4, 131, 555, 80, 0, 0), (1, 4, 0)), ((3, 12, 4, 27, 577, 128, 1000, 4), (1, 4, 0)), ((2, 24, 8, 21, 793, 64, 300, 130), (1, 4, 0)),
+    ((4, 1, 1, 20, 514, 80, 300, 130), (1, 8, 0)), ((3, 8, 2, 60, 3000, 128, 0, 0), (1, 8, 0)), ((3, 8, 2, 60, 3000, 64, 0, 0), (1, 8, 0)),
+]
+
+
+def form_of(b, hq, hkv, sq, sk, d, window, sinks):
+    import ctypes
+
+    from tensorrt_b200 import _lib
+
+    form = (ctypes.c_int32 * 3)()
+    assert _lib.load().b200q_window_attention_form(b, hq, hkv, sq, sk, d, window, sinks, ctypes.byref(form)) == 0
+    return tuple(form)
+
+
+needs_148 = pytest.mark.skipif("torch.cuda.is_available() and torch.cuda.get_device_properties(0).multi_processor_count != 148",
+                               reason="the choice of a form goes by the SMs")
+
+
+@needs_148
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape,form", NAMED, ids=str)
+def test_each_form_on_its_own(b200, shape, form, dt):
+    """Whole and ragged sequences, some with fewer key tiles than a cluster has CTAs, some without queries or keys."""
+    assert form_of(*shape) == form
+    b, hq, hkv, sq, sk, d, window, sinks = shape
+    g = torch.Generator(device="cuda").manual_seed(sq + sk)
+    q, k, v = inputs(g, b, hq, hkv, sq, sk, d, dt, True)
+    out = b200.window_attention(q, k, v, window=window, sinks=sinks)
+    check(out, *reference(q, k, v, window, sinks, [sq] * b, [sk] * b))
+    for turn in range(3):
+        nq = [(sq, sq // 2 + 1, 1, 0, sq - 1)[(i + turn) % 5] for i in range(b)]
+        nk = [(100, sk, sk // 3, 7, sk - 3, 0, 129)[(i + 2 * turn) % 7] for i in range(b)]
+        lens = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (nq, nk)]
+        qq, kk, vv = q.clone(), k.clone(), v.clone()
+        for i in range(b):
+            qq[i, :, nq[i]:], kk[i, :, nk[i]:], vv[i, :, nk[i]:] = float("nan"), float("nan"), float("inf")
+        out = b200.window_attention(qq, kk, vv, window=window, sinks=sinks, q_lens=lens[0], k_lens=lens[1])
+        check(out, *reference(q, k, v, window, sinks, nq, nk))
+
+
+@needs_148
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape,form", NAMED, ids=str)
+def test_each_form_with_values_that_are_not_finite(b200, shape, form, dt):
+    """A value that is not finite is the whole result of the rows that see it; a key that makes their logit infinite makes them NaN or, at
+    -inf, is a key less.  Other rows and heads are as they were."""
+    b, hq, hkv, sq, sk, d, window, sinks = shape
+    g = torch.Generator(device="cuda").manual_seed(sq - sk)
+    q, k, v = inputs(g, b, hq, hkv, sq, sk, d, dt, False)
+    group = hq // hkv
+    ref, mass = reference(q, k, v, window, sinks, [sq] * b, [sk] * b)
+    at = sk - sq + (2 * sq) // 3                          # seen by the later rows only
+    pos, j = torch.arange(sq, device="cuda") + sk - sq, torch.arange(sk, device="cuda")
+    seen = j <= pos[:, None]
+    if window > 0:
+        seen = seen & ((j > pos[:, None] - window) | (j < sinks))
+    hit = seen[:, at]
+    assert hit.any() and not hit.all()
+
+    def others(out):
+        check(out[:, group:], ref[:, group:], mass[:, group:])
+        check(out[1:], ref[1:], mass[1:])
+        check(out[0, :group, ~hit], ref[0, :group, ~hit], mass[0, :group, ~hit])
+        return out[0, :group, hit]
+
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        vv = v.clone()
+        vv[0, 0, at] = bad
+        mine = others(b200.window_attention(q, k, vv, window=window, sinks=sinks))
+        assert (mine.isnan() if bad != bad else mine == bad).all()
+        vv = v.clone()
+        vv[0, 0, at, 5] = bad                             # one element of it: the others are as they were
+        mine = others(b200.window_attention(q, k, vv, window=window, sinks=sinks))
+        assert (mine[..., 5].isnan() if bad != bad else mine[..., 5] == bad).all()
+        rest = [x for x in range(d) if x != 5]
+        check(mine[..., rest], ref[0, :group, hit][..., rest], mass[0, :group, hit][..., rest])
+        kk = k.clone()
+        kk[0, 0, at, 0] = bad
+        mine = others(b200.window_attention(q, kk, v, window=window, sinks=sinks))
+        sign = q[0, :group, hit, 0].float() * bad
+        gone = sign == -math.inf
+        assert mine[~gone].isnan().all()
+        for h in range(group):
+            s = (q[0, h].double() @ k[0, 0].double().T / math.sqrt(d)).masked_fill(~seen | (j == at), -math.inf)[hit]
+            p = torch.softmax(s, -1)[gone[h]]
+            check(mine[h][gone[h]], p @ v[0, 0].double(), p @ v[0, 0].double().abs())
