@@ -486,7 +486,8 @@ int b200q_paged_evict(const b200q_paged_cache* cache, const int32_t* block_table
  * those of out (elements, multiples of 16 bytes, D contiguous).  Sequence b has q_lens[b] queries and k_lens[b] keys (NULL:
  * Sq and Sk); its query i stands at position p = i + k_lens[b] - q_lens[b] and sees the keys 0 <= j <= p with j > p - window
  * or j < sinks (window <= 0: all of them).  P = softmax(q k^T * scale) in fp32, out = P V; rows that see no key and rows
- * beyond q_lens[b] get zeros.  What lies in masked rows of k and v, infinities and NaN included, does not matter.
+ * beyond q_lens[b] get zeros.  What lies in masked rows of k and v, infinities and NaN included, does not matter to the
+ * results; to the time it does, since rows beside such keys are computed twice, the second time slowly: clear padding.
  * Hq % Hkv == 0, D a multiple of 16 up to 128, B * Hq <= 65535. */
 int b200q_window_attention(const void* q, const void* k, const void* v, int dtype, const int64_t* strides, void* out,
                            const int64_t* out_strides, const int32_t* q_lens, const int32_t* k_lens, int64_t B, int64_t Hq,

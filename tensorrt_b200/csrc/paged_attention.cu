@@ -2,9 +2,9 @@
 //
 //   x_j = (q . k_j) * scale,  out = sum_j exp(x_j - m) v_j / sum_j exp(x_j - m),  m = max_j x_j
 //
-// over the keys j that the token sees, in one pass with a running maximum and sum.  Every K and V row is read once and takes
-// part in 4 * D operations per query head, so the memory binds the kernel, whatever the group: what has to be found is enough
-// bytes in flight on every SM, and work of the same size for each of them.
+// over the keys j that the token sees, in one pass with a running maximum and sum.  Every K and V row is read once for up to 16
+// query heads (a larger group is several items, each of which reads it) and takes part in 4 * D operations per query head, so the
+// memory binds the kernel: what has to be found is enough bytes in flight on every SM, and work of the same size for each of them.
 //
 // Work.  An item is a sequence, a kv head and up to 16 of its query heads; its keys are tiles of 64.  The tiles of all items
 // stand in one line, which the resident CTAs cut into equal pieces (the lengths are on the device, so every CTA adds them up
@@ -20,7 +20,7 @@
 // let 8-bit codes be widened between shared memory and the product.  P^T turns from the result of one product into the operand
 // of the next by an 8 x 8 transpose among the lanes.
 //
-// Measured (us a call): 64 sequences of 1 to 8190 tokens, 64 / 8 heads of 128, bf16 174 (6.2 TB/s, 0.94 of the copy rate; DRAM 6.1 TB/s, issue
+// Measured (us a call): 64 sequences of 1 to 8190 tokens, 64 / 8 heads of 128, bf16 174 (6.18 TB/s, 0.94 of the copy rate; DRAM 6.1 TB/s, issue
 // slots 28 %); 3 of 60000 to 131071, 8-bit pages 106 (5.5 TB/s: widening codes takes issue slots, 58 %); 32 of 900 to 16000, 16 / 16 heads of 64, window
 // 2048 48 (5.5 TB/s); one of 411 tokens 7.3, the chain from the lengths to the joined parts.  With the query heads as the 16-row
 // operand 187 / 144 / 69 / 8.3.  The loop in three or six copies, one for each stage of the ring, made short calls longer (instructions are
@@ -30,6 +30,7 @@
 // product: an error of one rounding of each term, of the size of the result's own; in fp16 that holds for terms down to 2^-25 of the largest
 // one of their warp's keys, and those below are off by up to 2^-36 of it (Reference).  8-bit K and V are exact in fp16; bf16
 // queries in front of them are scaled by a power of two into fp16's range, which loses nothing above 2^-38 of the largest.
+// Sums of P V are unnormalised: bf16 values up to 2^100 leave them room (P up to 2^8, 2^17 keys).
 #include <atomic>
 
 #include "paged.cuh"

@@ -25,7 +25,7 @@ __device__ __forceinline__ int ld_i32(const int32_t* p) {
 
 // A thread moves 16 elements of K and of V, read first; the pages of the CTA's tokens are found while they come: a warp
 // looks for the sequence of its first token, whose other tokens it holds as well, and so on; then a lane finds the page of a token.
-// Bound by the memory for prompts (16650 tokens of 8 heads of 128, bf16, 79 MB: 16.9 us, 4.7 TB/s; the copy rate gives 12.0), by three loads that
+// Bound by the memory for prompts (9620 tokens of 8 heads of 128, bf16, 79 MB: 16.9 us, 4.7 TB/s; the copy rate gives 12.0), by three loads that
 // wait for one another (lengths, table, rows) for a decode step (64 tokens 2.4 us, of which an empty launch is most).  Many small CTAs: two or
 // four pieces a thread take the registers of others (18.4 and 21.8 us; pages first and four pieces 19.0), 256 threads 17.3, 64 threads 16.6 but
 // more rounds for wide rows.  32000 tokens of one head of 64 to 8-bit pages 4.9 us; with a search to each token 12.2.
@@ -130,8 +130,9 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // The counts also say how many tokens a CTA keeps in front of the next, so that two more walks in the order of the tokens, a run of them
 // to each warp, write the list; a weight is its key read backwards, since a load from memory in that loop takes 5000 clocks in all.
 // Bound by latency and, since all of it runs a few times only, by the size of the code: what unrolling more loops saves is lost to
-// instruction fetches (34.6 us for the first of these calls became 40.3).  32000 tokens to 8192, 8 heads: about 18 us of the call's 31.4 (clusters of 4: 5 us
-// more); 24 sequences of 1500 to 6000 to 2048, 8 heads: 19 of 52.9.  Of 30000 clocks there 17000 are the four digits, 7000 the keys.
+// instruction fetches (34.6 us for the first of these calls became 40.3).  32000 tokens to 8192, 8 heads: about 19 us of the call's 32.3 (clusters of 4: 5 us
+// more); 24 sequences of 1500 to 6000 to 2048, 8 heads: 19 of 53.7.  Of 30000 clocks there 17000 are the four digits, 7000 the keys.  The table
+// is looked through for pages that are not there: 0.3 us of either call, 2 us more where its entries are read behind the length.
 constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kMaxCluster = 8, kColumns = 16;
 constexpr uint32_t kStays = 0xffffffffu, kLowest = 0x007fffffu, kZero = 0x80000000u;      // no weight's key; that of -inf and NaN; that of 0 and -0
 

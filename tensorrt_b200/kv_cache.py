@@ -58,7 +58,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale
                      q_lens: torch.Tensor | None = None, k_lens: torch.Tensor | None = None) -> torch.Tensor:
     """Causal (lower-right aligned) attention: q [B, query heads, Sq, D], k and v [B, kv heads, Sk, D] -> q's shape and type.  With
     window > 0 a query sees the last `window` keys up to its own and the first `sinks`.  `q_lens`, `k_lens` int32 [B]: the queries and
-    keys that each sequence has; rows beyond them, and rows that see no key, are zero.  scale None: 1 / sqrt(D)."""
+    keys that each sequence has; rows beyond them, and rows that see no key, are zero.  What lies in keys beyond them does not matter, but
+    infinities and NaN there make the call many times slower: clear padding that was never written.  scale None: 1 / sqrt(D)."""
     args = (q, k, v, q_lens, k_lens, 0.0 if scale is None else scale, window, sinks)
     out = _native.window_attention(*args)
     return _window(*args) if out is None else out
@@ -215,7 +216,8 @@ class PagedKvCache:
 
     def evict(self, keep: int, recent: int = 0, sinks: int = 0) -> list:
         """Cuts every sequence to `keep` tokens per kv head, by the sums of attention weights of each layer, and frees the pages they
-        were in.  -> the kept tokens of every layer, int32 [batch, kv heads, keep]."""
+        were in, reserved ones among them.  Only `attend` adds to the sums: right behind a prompt all are equal, and beside the first
+        `sinks` and the last `recent` the lowest tokens stay.  -> the kept tokens of every layer, int32 [batch, kv heads, keep]."""
         if self.weights[0] is None:
             raise ValueError("eviction goes by attention weights: the cache was made with weights=False")
         if min(keep, recent, sinks) < 0 or recent + sinks > keep or keep > self.max_tokens:
