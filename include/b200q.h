@@ -500,6 +500,52 @@ int b200q_window_attention(const void* q, const void* k, const void* v, int dtyp
 int b200q_window_attention_form(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D, int64_t window,
                                 int64_t sinks, int32_t form[3]);
 
+/* ------------------------------------------------------------------ several continuations of one prompt
+ * Pages src[i] -> dst[i] in every one of `n_pools` pools (K and V of all layers, say): element (page, head, row) of each lies at
+ * pools[k] + page * strides[0] + head * strides[1] + row * strides[2] (BYTES) and is row_bytes long.  rows[i] (NULL: page_size): the
+ * first rows of the page that are copied.  src, dst, rows are HOST arrays, read before the call returns: they travel with the launch, and a
+ * captured call keeps them.  No page may be written twice, nor be both read and written: B200Q_ERR_INVALID.
+ * Pools 16-byte aligned, strides and row_bytes (at most 256) multiples of 16. */
+int b200q_paged_copy(void* const* pools, int64_t n_pools, int64_t num_pages, int64_t heads, int32_t page_size,
+                     int64_t row_bytes, const int64_t* strides, const int32_t* src, const int32_t* dst, const int32_t* rows,
+                     int64_t pairs, b200q_stream_t stream);
+
+/* b200q_paged_attention (no window, no weights) where groups of sequences share the pages of a prefix: the keys of the prefix are
+ * attended to by all of a group at once, and read once for up to 128 of its rows.
+ * The plan says who shares what: group g holds the sequences members[cu[g]] .. members[cu[g + 1] - 1] (cu[0] = 0; a group may be empty),
+ * whose first tokens[g] tokens are the same.  These are found through the line of block_table of the group's FIRST sequence; the keys
+ * behind them, and all keys of a sequence that is in no group, through its own.  A sequence that holds fewer tokens than
+ * its group's prefix is attended to through its own line alone.
+ * b200q_shared_prefix_plan writes b200q_shared_prefix_plan_values(B, groups) int32 to `plan`, all of it HOST memory (the caller takes it to
+ * the device), and refuses a sequence outside the batch or in two groups.  It goes by sequences, not by pages: it stays valid as
+ * sequences grow.  The call never reads or writes out of bounds, whatever the plan holds.
+ *   plan      on the device, 4-byte aligned; `groups` as it was made with; largest: sequences of the largest group (more are left out)
+ *   attention_workspace  as of b200q_paged_attention
+ *   workspace b200q_shared_prefix_workspace_bytes(..) bytes, 16-byte aligned, any content; not shared by calls that overlap
+ * B * Hq < 2^30. */
+int64_t b200q_shared_prefix_plan_values(int64_t B, int64_t groups);
+int b200q_shared_prefix_plan(const int32_t* members, const int32_t* cu, const int32_t* tokens, int64_t groups, int64_t B,
+                             int32_t* plan);
+size_t b200q_shared_prefix_workspace_bytes(int64_t B, int64_t Hq, int64_t heads, int64_t D, int64_t groups, int64_t largest);
+int b200q_shared_prefix_attention(const void* q, int dtype, const int64_t* q_strides, const b200q_paged_cache* cache,
+                                  const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* lens,
+                                  int64_t B, int64_t Hq, const int32_t* plan, int64_t groups, int64_t largest, float scale,
+                                  void* out, void* attention_workspace, size_t attention_workspace_bytes, void* workspace,
+                                  size_t workspace_bytes, b200q_stream_t stream);
+
+/* Of each row of logits x [rows, vocabulary] (dtype B200Q_F32, B200Q_F16 or B200Q_BF16; rows row_stride elements apart, at any
+ * address their type has), with p = softmax(x * scale), in 32 bits:
+ *   log_probs      fp32 [rows]: log p of tokens[row] (int32 or int64: token_bytes 4 or 8); 0 for a token outside the vocabulary
+ *                  (a row of padding).  tokens and log_probs may both be NULL.
+ *   entropy        fp32 [rows], in nats, a token of p = 0 counting 0; may be NULL
+ *   top_log_probs  fp32 [rows, top], top_tokens int32 [rows, top]: the `top` largest logits, descending (equal ones: the lower token
+ *                  first; NaN above all), 0 <= top <= 64 and <= vocabulary; may be NULL with top = 0
+ * A row whose largest logit is not finite (nothing but -inf, an infinity, a NaN) has no distribution: its log probabilities and its
+ * entropy are NaN, its top_tokens in the same order.  scale > 0, finite. */
+int b200q_token_log_probs(const void* logits, int dtype, int64_t rows, int64_t vocabulary, int64_t row_stride,
+                          const void* tokens, int token_bytes, float scale, float* log_probs, float* entropy, int64_t top,
+                          float* top_log_probs, int32_t* top_tokens, b200q_stream_t stream);
+
 /* ------------------------------------------------------------------ glue of the decoder linear stack
  * The benchmark workloads wrap the quantized linears in a Llama-shaped decoder layer
  * (RMSNorm -> QKV -> attention replaced by identity on V -> O -> residual -> RMSNorm ->

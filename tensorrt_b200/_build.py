@@ -26,7 +26,8 @@ PYTHON_LIB = PKG / "libb200q_python.so"
 
 CUDA_SOURCES = ["runtime.cu", "quantize_fp8.cu", "quantize_nvfp4.cu", "gemm_fp8.cu", "gemm_nvfp4.cu",
                 "fused_ops.cu", "p2p_allreduce.cu", "attention_fp8.cu", "comm_context.cu",
-                "paged_cache.cu", "paged_attention.cu", "window_attention.cu"]
+                "paged_cache.cu", "paged_attention.cu", "window_attention.cu",
+                "page_copy.cu", "shared_prefix.cu", "token_scores.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-Xptxas", "-v"]
 
@@ -134,7 +135,7 @@ def _build_torch_extension(src: Path, lib: Path, name: str, includes: list, libs
     import torch
     from torch.utils import cpp_extension
 
-    stamp = _stamp([src, CSRC / "internal.h", CSRC / "paged_calls.h", ROOT / "include" / "b200q.h"], torch.__version__ + abi)
+    stamp = _stamp([src, CSRC / "internal.h", CSRC / "paged_calls.h", CSRC / "score_calls.h", ROOT / "include" / "b200q.h"], torch.__version__ + abi)
     stamp_file = PKG / "build" / f"{name}.stamp"
     if not force and lib.exists() and stamp_file.exists() and stamp_file.read_text() == stamp:
         return lib

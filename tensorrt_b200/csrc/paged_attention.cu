@@ -34,6 +34,7 @@
 #include <atomic>
 
 #include "paged.cuh"
+#include "shared_prefix.cuh"
 
 namespace b200q {
 namespace {
@@ -60,6 +61,7 @@ struct DecodeParams {
   int64_t window, sinks;
   unsigned* tickets;         // [2][kMaxCtas], of items and of groups, zero between calls: B200Q_PAGED_ATTENTION_ZERO_BYTES
   float* parts;              // [kMaxCtas][2][kPart]
+  paged::Prefix x;           // behind a shared prefix only
 };
 
 // What P is referred to.  fp16 (fp16 pages, and codes, which are widened to fp16): set 2^11 below the largest term, so that P is rounded like
@@ -154,8 +156,13 @@ struct Seen {
   __device__ __forceinline__ int token(int i) const { return i < sinks ? i : i + gap; }
   __device__ __forceinline__ int tiles() const { return seen > 0 ? (seen + kTile - 1) / kTile : 1; }   // 1: somebody writes the zeros
 };
+template <bool JOIN>
 __device__ __forceinline__ Seen keys_seen(const DecodeParams& p, int b) {
   const int n = paged::cached_tokens(p.c, b, 0x7fffffff);
+  if constexpr (JOIN) {
+    const int shared = paged::prefix_tokens(p.x, b, n);
+    return Seen{n - shared, 0, shared};
+  }
   const int first = p.window > 0 && n > p.window ? static_cast<int>(n - p.window) : 0;
   const int sinks = p.sinks < first ? static_cast<int>(p.sinks) : first;
   return Seen{n - (first - sinks), sinks, first - sinks};
@@ -176,17 +183,9 @@ struct Stage {
   }
 };
 
-// a / b of numbers that are not negative; a division of 64 bits takes some hundred clocks, one of 32 bits a third of that
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
-  return (a | b) >> 32 == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
-}
-// Where the piece of CTA c of `ctas` begins in the line of tiles, ctas <= tiles; no piece is empty.
-__device__ __forceinline__ int64_t piece(int64_t tiles, int c, int ctas) { return divide(tiles * c, ctas); }
-// The CTA whose piece holds tile x.
-__device__ __forceinline__ int holder(int64_t tiles, int64_t x, int ctas) { return static_cast<int>(divide((x + 1) * ctas - 1, tiles)); }
-
 // Adds up the tiles of all sequences and finds the one that holds the first tile of this CTA's piece; all threads take part.
 // `ctas`: of those launched, as many as there are tiles.
+template <bool JOIN>
 __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, int* ctas, int* b_out, int64_t* before_out, Seen* seen_out) {
   __shared__ int64_t sums[kWarps];
   __shared__ int64_t found[2];
@@ -215,7 +214,7 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
     return all;
   };
   for (int base = 0; base < p.B; base += kThreads) {
-    if (base + tid < p.B) keys = keys_seen(p, base + tid);
+    if (base + tid < p.B) keys = keys_seen<JOIN>(p, base + tid);
     mine = base + tid < p.B ? keys.tiles() * per : 0;
     total += scan(mine);
   }
@@ -228,7 +227,7 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
   } else {
     int64_t before = 0;
     for (int base = 0; base < p.B; base += kThreads) {
-      if (base + tid < p.B) keys = keys_seen(p, base + tid);
+      if (base + tid < p.B) keys = keys_seen<JOIN>(p, base + tid);
       mine = base + tid < p.B ? keys.tiles() * per : 0;
       const int64_t all = scan(mine);
       if (want >= before + inclusive - mine && want < before + inclusive)
@@ -244,8 +243,68 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
   return total;
 }
 
-// BLOCKS8: query heads of an item in blocks of 8.
-template <typename T, bool CODES, int DPAD, int BLOCKS8>
+// Where the parts of a sequence's prefix lie, for one kv head.
+struct PrefixPlace {
+  int64_t total, start;      // tiles of all, tiles in front of the kv head's items
+  int ctas, tiles, item, row;  // CTAs, tiles of an item, first item, first row
+  bool on;
+};
+__device__ __noinline__ PrefixPlace prefix_place(const DecodeParams& p, int b, int h) {
+  PrefixPlace w{};
+  const int g = paged::ld_index(p.x.group_of + b);
+  w.on = paged::prefix_tokens(p.x, b, paged::cached_tokens(p.c, b, 0x7fffffff)) > 0 && g >= 0 && g < p.x.groups;
+  if (!w.on) return w;
+  const paged::GroupWork group = paged::group_work(p.x, p.c, g);
+  const int place = paged::ld_index(p.x.place_of + b);
+  const int64_t* const line = p.x.lines;
+  w.on = group.tiles > 0 && place >= 0 && place < group.n;
+  w.total = __ldcg(line + 2 * p.x.groups), w.ctas = static_cast<int>(__ldcg(line + 2 * p.x.groups + 1));
+  w.tiles = group.tiles, w.row = place * p.group;
+  w.item = static_cast<int>(__ldcg(line + 2 * g + 1)) + h * group.row_tiles;
+  w.start = __ldcg(line + 2 * g) + static_cast<int64_t>(h) * group.row_tiles * group.tiles;
+  return w;
+}
+// Adds the parts of the prefix, in the order of the keys, to four elements of a row.
+struct Joined {
+  float top, sum, acc[4];
+  bool has;
+};
+template <int DPAD>
+__device__ __noinline__ Joined join_prefix(const DecodeParams& p, const PrefixPlace w, int head, int d, Joined a) {
+  const int row = w.row + head, tile = row / paged::kPrefixRows, r = row % paged::kPrefixRows;
+  const int64_t start = w.start + static_cast<int64_t>(tile) * w.tiles;
+  const int c0 = holder(w.total, start, w.ctas), c1 = holder(w.total, start + w.tiles - 1, w.ctas);
+  constexpr int kAtOnce = 8;
+#pragma unroll 1
+  for (int c = c0; c <= c1; c += kAtOnce) {
+    float2 s[kAtOnce];
+    float4 v[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      s[k].y = -1.0f;
+      const int64_t slot = static_cast<int64_t>(w.item) + tile + c + k;
+      if (c + k > c1 || r >= p.x.rows || slot >= p.x.slots) continue;
+      s[k] = __ldcg(p.x.stats + slot * p.x.rows + r);
+      v[k] = __ldcg(reinterpret_cast<const float4*>(p.x.parts + (slot * p.x.rows + r) * DPAD + d));
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (s[k].y < 0.0f) continue;
+      a.has = true;
+      const float now = fmaxf(a.top, s[k].x), base = now == -INFINITY ? 0.0f : now, f0 = exp2_fast(a.top - base), f1 = exp2_fast(s[k].x - base);
+      a.sum = a.sum * f0 + s[k].y * f1;
+      a.acc[0] = a.acc[0] * f0 + v[k].x * f1, a.acc[1] = a.acc[1] * f0 + v[k].y * f1;
+      a.acc[2] = a.acc[2] * f0 + v[k].z * f1, a.acc[3] = a.acc[3] * f0 + v[k].w * f1;
+      a.top = now;
+    }
+  }
+  return a;
+}
+
+// BLOCKS8: query heads of an item in blocks of 8.  JOIN: behind the kernel of shared prefixes, whose parts of a row are joined with those found here.
+// Nothing else of that kernel is read, and it lets this one start only once everything in front of it has completed: what is waited for stands
+// where the parts are read.
+template <typename T, bool CODES, int DPAD, int BLOCKS8, bool JOIN>
 __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm) decode_kernel(const __grid_constant__ DecodeParams p) {
   using S = Stage<CODES, DPAD, BLOCKS8>;
   constexpr bool kHalf = CODES || std::is_same<T, __half>::value;
@@ -261,13 +320,16 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
   char* const ring = smem + warp * S::kDepth * S::kBytes;
   const uint32_t ring_u32 = smem_u32(ring);
   pdl_launch_dependents();
-  pdl_wait();
+  if constexpr (!JOIN) pdl_wait();
 
   int b;
   int64_t before;
   Seen see;
-  const int64_t total = find_start(p, cta, &ctas, &b, &before, &see);
-  if (cta >= ctas) return;
+  const int64_t total = find_start<JOIN>(p, cta, &ctas, &b, &before, &see);
+  if (cta >= ctas) {
+    if constexpr (JOIN) pdl_wait();             // this kernel has ended only when the one in front has
+    return;
+  }
   int64_t at = piece(total, cta, ctas);
   const int64_t first_tile = at, end = piece(total, cta + 1, ctas);
   // the item: kv head and block of query heads, within sequence b
@@ -509,6 +571,11 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
             mine[row * DPAD + (CODES ? g * (DPAD / 8) + 2 * i + half : 16 * i + 8 * half + g)] = o[r][i][2 * half + e];
       }
     __syncthreads();
+    PrefixPlace place{};
+    if constexpr (JOIN) {
+      pdl_wait();
+      place = prefix_place(p, b, h);
+    }
     const bool whole = tile0 == 0 && tile1 == tiles;
     // CTAs that share the item: c0 .. c1, those with a piece of it; the counter of the one that begins it
     const int c0 = whole ? cta : holder(total, item_start, ctas), c1 = whole ? cta : holder(total, item_end - 1, ctas);
@@ -532,6 +599,13 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
         acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
       }
       if (whole) {
+        if constexpr (JOIN) {
+          if (place.on) {
+            const Joined a = join_prefix<DPAD>(p, place, block * p.rows + row, d, Joined{top, sum, {acc[0], acc[1], acc[2], acc[3]}, has});
+            top = a.top, sum = a.sum, has = a.has;
+            acc[0] = a.acc[0], acc[1] = a.acc[1], acc[2] = a.acc[2], acc[3] = a.acc[3];
+          }
+        }
         if (d < p.c.D) {
           const float f = v_scale / sum;
           T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.Hq + head0 + row) * p.c.D + d;
@@ -602,6 +676,13 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
             if (d == 0) dst[kRows * DPAD + 2 * kRows + row] = top, dst[kRows * DPAD + 3 * kRows + row] = has ? sum : -1.0f;
             continue;
           }
+          if constexpr (JOIN) {
+            if (place.on) {
+            const Joined a = join_prefix<DPAD>(p, place, block * p.rows + row, d, Joined{top, sum, {acc[0], acc[1], acc[2], acc[3]}, has});
+            top = a.top, sum = a.sum, has = a.has;
+            acc[0] = a.acc[0], acc[1] = a.acc[1], acc[2] = a.acc[2], acc[3] = a.acc[3];
+          }
+          }
           if (d < p.c.D) {
             const float f = v_scale / sum;
             T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.Hq + head0 + row) * p.c.D + d;
@@ -625,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
     item_start = item_end;
     if (++block == p.blocks) {
       block = 0;
-      if (++h == p.c.heads) h = 0, see = keys_seen(p, ++b);
+      if (++h == p.c.heads) h = 0, see = keys_seen<JOIN>(p, ++b);
     }
   }
 }
@@ -635,7 +716,7 @@ __global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ De
   pdl_launch_dependents();
   pdl_wait();
   const int b = blockIdx.z, h = blockIdx.y;
-  const Seen see = keys_seen(p, b);
+  const Seen see = keys_seen<false>(p, b);
   const int64_t first = static_cast<int64_t>(b) * p.Hq + h * p.group;
   float* w = weights + (static_cast<int64_t>(b) * p.c.heads + h) * p.weights_len;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < see.seen; i += static_cast<int64_t>(gridDim.x) * 256) {
@@ -648,12 +729,12 @@ __global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ De
   }
 }
 
-template <typename T, bool CODES, int DPAD, int BLOCKS8>
+template <typename T, bool CODES, int DPAD, int BLOCKS8, bool JOIN>
 int launch_decode(const DecodeParams& p, int64_t most_tiles, cudaStream_t st) {
   using S = Stage<CODES, DPAD, BLOCKS8>;
   constexpr int kSmem = kWarps * S::kDepth * S::kBytes;
   static_assert(S::kDepth * S::kBytes >= 8 * BLOCKS8 * DPAD * 4, "a warp's result takes its ring");
-  auto kernel = decode_kernel<T, CODES, DPAD, BLOCKS8>;
+  auto kernel = decode_kernel<T, CODES, DPAD, BLOCKS8, JOIN>;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return B200Q_ERR_CUDA;
   static std::atomic<int> resident[64];                // CTAs that one SM holds; 0: not asked yet
@@ -670,15 +751,49 @@ int launch_decode(const DecodeParams& p, int64_t most_tiles, cudaStream_t st) {
   return check_launch();
 }
 
-template <typename T, bool CODES>
+template <typename T, bool CODES, bool JOIN>
 int launch_decode_d(const DecodeParams& p, int64_t most_tiles, cudaStream_t st) {
-  if (p.rows <= 8) return p.c.D <= 64 ? launch_decode<T, CODES, 64, 1>(p, most_tiles, st) : launch_decode<T, CODES, 128, 1>(p, most_tiles, st);
-  return p.c.D <= 64 ? launch_decode<T, CODES, 64, 2>(p, most_tiles, st) : launch_decode<T, CODES, 128, 2>(p, most_tiles, st);
+  if (p.rows <= 8) return p.c.D <= 64 ? launch_decode<T, CODES, 64, 1, JOIN>(p, most_tiles, st) : launch_decode<T, CODES, 128, 1, JOIN>(p, most_tiles, st);
+  return p.c.D <= 64 ? launch_decode<T, CODES, 64, 2, JOIN>(p, most_tiles, st) : launch_decode<T, CODES, 128, 2, JOIN>(p, most_tiles, st);
+}
+template <bool JOIN>
+int launch_decode_t(const DecodeParams& p, int dtype, int64_t most_tiles, cudaStream_t st) {
+  if (dtype == B200Q_BF16)
+    return p.c.codes ? launch_decode_d<__nv_bfloat16, true, JOIN>(p, most_tiles, st) : launch_decode_d<__nv_bfloat16, false, JOIN>(p, most_tiles, st);
+  return p.c.codes ? launch_decode_d<__half, true, JOIN>(p, most_tiles, st) : launch_decode_d<__half, false, JOIN>(p, most_tiles, st);
+}
+
+// What the query heads of a kv head, the pages and the workspace make of the parameters.
+void set_shape(DecodeParams* p, const void* q, const int64_t* q_strides, void* out, int64_t B, int64_t Hq, float scale, void* workspace) {
+  p->page_shift = -1;
+  if ((p->c.page_size & (p->c.page_size - 1)) == 0)
+    for (p->page_shift = 0; (1 << p->page_shift) < p->c.page_size;) ++p->page_shift;
+  p->one_layout = p->c.k.page == p->c.v.page && p->c.k.row == p->c.v.row;
+  p->q = static_cast<const char*>(q);
+  p->q_batch = q_strides[0] * 2, p->q_head = q_strides[1] * 2;
+  p->out = out;
+  p->B = static_cast<int>(B), p->Hq = static_cast<int>(Hq), p->group = static_cast<int>(Hq / p->c.heads);
+  p->blocks = (p->group + kRows - 1) / kRows;
+  p->rows = (p->group + p->blocks - 1) / p->blocks;
+  p->blocks = (p->group + p->rows - 1) / p->rows;
+  p->scale = scale;
+  p->tickets = static_cast<unsigned*>(workspace);
+  p->parts = reinterpret_cast<float*>(p->tickets + 2 * kMaxCtas);
 }
 
 int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
 
 }  // namespace
+
+int paged::attend_behind_prefix(const Cache& c, const Prefix& x, const void* q, int dtype, const int64_t* q_strides, int64_t B, int64_t Hq, float scale,
+                                void* out, void* workspace, cudaStream_t st) {
+  DecodeParams p{};
+  p.c = c, p.x = x;
+  set_shape(&p, q, q_strides, out, B, Hq, scale, workspace);
+  const int64_t tiles = (c.capacity > 0 ? (c.capacity + kTile - 1) / kTile : 1) * B * c.heads * p.blocks;
+  return launch_decode_t<true>(p, dtype, tiles, st);
+}
+
 }  // namespace b200q
 
 using namespace b200q;
@@ -710,21 +825,8 @@ int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, co
   if (weights != nullptr && (scratch == nullptr || scratch_bytes < b200q_paged_attention_scratch_bytes(B, Hq, keys))) return B200Q_ERR_WORKSPACE;
   if (!aligned(workspace, 16) || !aligned(scratch, 16)) return B200Q_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
-  p.page_shift = -1;
-  if ((p.c.page_size & (p.c.page_size - 1)) == 0)
-    for (p.page_shift = 0; (1 << p.page_shift) < p.c.page_size;) ++p.page_shift;
-  p.one_layout = p.c.k.page == p.c.v.page && p.c.k.row == p.c.v.row;
-  p.q = static_cast<const char*>(q);
-  p.q_batch = q_strides[0] * 2, p.q_head = q_strides[1] * 2;
-  p.out = out;
-  p.B = static_cast<int>(B), p.Hq = static_cast<int>(Hq), p.group = static_cast<int>(Hq / p.c.heads);
-  p.blocks = (p.group + kRows - 1) / kRows;
-  p.rows = (p.group + p.blocks - 1) / p.blocks;
-  p.blocks = (p.group + p.rows - 1) / p.rows;
-  p.scale = scale;
+  set_shape(&p, q, q_strides, out, B, Hq, scale, workspace);
   p.window = window, p.sinks = sinks;
-  p.tickets = static_cast<unsigned*>(workspace);
-  p.parts = reinterpret_cast<float*>(p.tickets + 2 * kMaxCtas);
   if (weights != nullptr && weights_len > 0) {
     p.logits_stride = round4(keys);
     p.weights_len = weights_len;
@@ -734,8 +836,7 @@ int b200q_paged_attention(const void* q, int dtype, const int64_t* q_strides, co
   // no more CTAs than tiles
   const int64_t tiles = (most > 0 ? (most + kTile - 1) / kTile : 1) * B * p.c.heads * p.blocks;
   const auto st = static_cast<cudaStream_t>(stream);
-  const int rc = dtype == B200Q_BF16 ? (p.c.codes ? launch_decode_d<__nv_bfloat16, true>(p, tiles, st) : launch_decode_d<__nv_bfloat16, false>(p, tiles, st))
-                                     : (p.c.codes ? launch_decode_d<__half, true>(p, tiles, st) : launch_decode_d<__half, false>(p, tiles, st));
+  const int rc = launch_decode_t<false>(p, dtype, tiles, st);
   if (rc != B200Q_OK || p.logits == nullptr) return rc;
   const int64_t chunks = (keys + 255) / 256;
   const dim3 grid(static_cast<unsigned>(chunks < 1 ? 1 : (chunks < 65535 ? chunks : 65535)), static_cast<unsigned>(p.c.heads), static_cast<unsigned>(B));

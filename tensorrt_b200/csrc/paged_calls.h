@@ -14,6 +14,7 @@
 #include <optional>
 #include <tuple>
 #include <utility>
+#include <vector>
 
 #include "b200q.h"
 
@@ -209,6 +210,84 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& 
                                      w ? static_cast<size_t>(scratch.numel()) : 0, stream_of_call()),
                "b200q_paged_attention");
   return out;
+}
+
+// As b200_paged_attention where groups of sequences share a prefix (`plan`, made for `groups` groups of up to `largest` sequences).
+Tensor shared_prefix_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens, const Tensor& plan,
+                               int64_t groups, int64_t largest, const std::optional<Tensor>& k_amax, const std::optional<Tensor>& v_amax, double scale) {
+  const char* op = "b200_shared_prefix_attention";
+  c10::cuda::CUDAGuard guard(k_pages.device());
+  CacheArgs a = cache_args(k_pages, v_pages, table, lens, k_amax, v_amax, false, op);
+  const int dt = token_dtype(q_in, a, k_pages, op);
+  TORCH_CHECK(q_in.dim() == 3 && q_in.size(0) == a.B && q_in.size(2) == a.c.D, op, ": expected q [", a.B, ", query heads, ", a.c.D, "], got ", q_in.sizes());
+  const int64_t Hq = q_in.size(1);
+  TORCH_CHECK_VALUE(Hq > 0 && Hq % a.c.heads == 0, op, ": query heads (", Hq, ") must be a multiple of the kv heads (", a.c.heads, ")");
+  TORCH_CHECK_VALUE(groups >= 0 && groups <= a.B && largest >= 0 && largest <= a.B && (groups == 0 || largest > 0), op, ": no plan of a batch of ", a.B,
+                    " has ", groups, " groups of up to ", largest);
+  TORCH_CHECK(plan.device() == k_pages.device() && plan.scalar_type() == at::kInt && plan.dim() == 1 && plan.is_contiguous() &&
+                  plan.size(0) == b200q_shared_prefix_plan_values(a.B, groups),
+              op, ": the plan must be ", b200q_shared_prefix_plan_values(a.B, groups), " contiguous int32 values on the device of the pages (a batch of ", a.B,
+              ", ", groups, " groups), got ", plan.sizes(), " of ", plan.scalar_type());
+  Tensor out = at::empty(q_in.sizes(), q_in.options());
+  if (a.B == 0) return out;
+  Tensor q = rows_of_16(q_in);
+  const int64_t strides[2] = {outer_stride(q, 0), outer_stride(q, 1)};
+  const float sm = softmax_scale(scale, a.c.D, op);
+  Tensor ws = attention_workspace(q);
+  Tensor scratch = at::empty({static_cast<int64_t>(b200q_shared_prefix_workspace_bytes(a.B, Hq, a.c.heads, a.c.D, groups, largest))}, q_in.options().dtype(at::kByte));
+  must_be_ok(b200q_shared_prefix_attention(q.data_ptr(), dt, strides, &a.c, a.table, a.table_stride, a.table_width, a.lens, a.B, Hq, plan.data_ptr<int32_t>(),
+                                           groups, largest, sm, out.data_ptr(), ws.data_ptr(), static_cast<size_t>(ws.numel()), scratch.data_ptr(),
+                                           static_cast<size_t>(scratch.numel()), stream_of_call()),
+             "b200q_shared_prefix_attention");
+  return out;
+}
+
+// Pages src[i] -> dst[i] (their first rows[i] rows) in every pool.
+void paged_copy(at::TensorList k_pages, at::TensorList v_pages, at::IntArrayRef src, at::IntArrayRef dst, at::OptionalIntArrayRef rows) {
+  const char* op = "b200_paged_copy";
+  TORCH_CHECK_VALUE(src.size() == dst.size() && (!rows.has_value() || rows->size() == src.size()), op, ": expected as many pages to write (", dst.size(),
+                    ") and numbers of rows as pages to read (", src.size(), ")");
+  TORCH_CHECK_VALUE(k_pages.size() == v_pages.size(), op, ": expected as many pools of K (", k_pages.size(), ") as of V (", v_pages.size(), ")");
+  if (k_pages.empty()) return;
+  const Tensor& first = k_pages[0];
+  std::vector<const Tensor*> pools;
+  for (const auto& list : {k_pages, v_pages})
+    for (const Tensor& t : list) {
+      TORCH_CHECK(t.is_cuda(), op, ": b200q operates on CUDA tensors only; there is no CPU implementation");
+      TORCH_CHECK(t.dim() == 4 && t.sizes() == first.sizes() && t.scalar_type() == first.scalar_type() && t.device() == first.device(), op,
+                  ": expected pools [pages, kv heads, rows, D] of one size, type and device, got ", first.sizes(), " and ", t.sizes());
+      TORCH_CHECK(rows_16(t), op, ": rows of pages must be contiguous, 16-byte aligned and multiples of 16 bytes apart, got strides ", t.strides());
+      pools.push_back(&t);
+    }
+  const auto type = first.scalar_type();
+  TORCH_CHECK_VALUE(type == at::kHalf || type == at::kBFloat16 || type == at::kFloat8_e4m3fn || type == at::kByte, op, " received pages of ", type,
+                    " type. Supported types: float16 | bfloat16 | float8_e4m3fn | uint8 (its codes)");
+  const int64_t pages = first.size(0), size = first.size(2);
+  TORCH_CHECK_VALUE(first.size(3) % 16 == 0 && first.size(3) > 0 && first.size(3) <= 128 && size > 0 && size <= (1 << 20) && first.size(1) > 0, op,
+                    ": need a head dimension that is a multiple of 16 up to 128 and pages of at least one row, got pages ", first.sizes());
+  std::vector<int32_t> numbers(src.size() * 3);
+  for (size_t i = 0; i < src.size(); ++i) {
+    const int64_t n = rows.has_value() ? (*rows)[i] : size;
+    TORCH_CHECK_VALUE(src[i] >= 0 && src[i] < pages && dst[i] >= 0 && dst[i] < pages && n >= 0 && n <= size, op, ": ", n, " rows of page ", src[i], " to page ", dst[i],
+                      " are not within pools ", first.sizes());
+    numbers[i] = static_cast<int32_t>(src[i]), numbers[src.size() + i] = static_cast<int32_t>(dst[i]), numbers[2 * src.size() + i] = static_cast<int32_t>(n);
+  }
+  TORCH_CHECK_VALUE(static_cast<int64_t>(src.size()) <= pages, op, ": a page is written twice");
+  c10::cuda::CUDAGuard guard(first.device());
+  std::vector<void*> data;
+  for (size_t i = 0; i < pools.size();) {             // pools of equal strides together: one launch, or one for K and one for V
+    data.clear();
+    size_t end = i;
+    for (; end < pools.size() && pools[end]->strides() == pools[i]->strides(); ++end) data.push_back(pools[end]->data_ptr());
+    int64_t strides[3];
+    for (int k = 0; k < 3; ++k) strides[k] = outer_stride(*pools[i], k) * first.element_size();
+    const int rc = b200q_paged_copy(data.data(), static_cast<int64_t>(data.size()), pages, first.size(1), static_cast<int32_t>(size),
+                                    first.size(3) * first.element_size(), strides, numbers.data(), numbers.data() + src.size(), numbers.data() + 2 * src.size(),
+                                    static_cast<int64_t>(src.size()), stream_of_call());
+    TORCH_CHECK_VALUE(rc != B200Q_ERR_INVALID, op, ": a page is written twice, or both read and written, or too large");
+    must_be_ok(rc, "b200q_paged_copy");
+    i = end;
+  }
 }
 
 std::tuple<Tensor, Tensor, Tensor> paged_evict(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens,

@@ -34,6 +34,7 @@
 #include "b200q.h"
 #include "internal.h"
 #include "paged_calls.h"
+#include "score_calls.h"
 
 namespace {
 
@@ -640,6 +641,72 @@ PyObject* py_window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* py_shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_VALUE(n == 11, "shared_prefix_attention: 11 arguments expected");
+  std::optional<Tensor> t[8];
+  int64_t v[2];
+  if (!all_plain(a, 8, t) || !PyFloat_Check(a[8]) || !ints(a + 9, 2, v)) Py_RETURN_NONE;
+  for (int i = 0; i < 6; ++i)
+    if (!t[i]) Py_RETURN_NONE;
+  return THPVariable_Wrap(b200q_calls::shared_prefix_attention(*t[0], *t[1], *t[2], *t[3], *t[4], *t[5], v[0], v[1], t[6], t[7], PyFloat_AS_DOUBLE(a[8])));
+  END_HANDLE_TH_ERRORS
+}
+
+// A list of plain tensors, of integers.
+bool tensor_list(PyObject* o, std::vector<Tensor>* out) {
+  if (!PyList_CheckExact(o)) return false;
+  const Py_ssize_t n = PyList_GET_SIZE(o);
+  out->reserve(static_cast<size_t>(n));
+  std::optional<Tensor> t;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* item = PyList_GET_ITEM(o, i);
+    t.reset();
+    if (!all_plain(&item, 1, &t) || !t) return false;
+    out->push_back(*t);
+  }
+  return true;
+}
+bool int_list(PyObject* o, std::vector<int64_t>* out) {
+  if (!PyList_CheckExact(o)) return false;
+  const Py_ssize_t n = PyList_GET_SIZE(o);
+  out->resize(static_cast<size_t>(n));
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* item = PyList_GET_ITEM(o, i);
+    if (!ints(&item, 1, &(*out)[i])) return false;
+  }
+  return true;
+}
+
+PyObject* py_paged_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_VALUE(n == 5, "paged_copy: 5 arguments expected");
+  std::vector<Tensor> k, v;
+  std::vector<int64_t> src, dst, rows;
+  if (modes_active() || !tensor_list(a[0], &k) || !tensor_list(a[1], &v) || !int_list(a[2], &src) || !int_list(a[3], &dst)) Py_RETURN_FALSE;
+  if (a[4] != Py_None && !int_list(a[4], &rows)) Py_RETURN_FALSE;
+  b200q_calls::paged_copy(k, v, src, dst, a[4] == Py_None ? at::OptionalIntArrayRef() : at::OptionalIntArrayRef(rows));
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_VALUE(n == 4, "token_log_probs: 4 arguments expected");
+  std::optional<Tensor> t[2];
+  int64_t top;
+  if (!all_plain(a, 2, t) || !t[0] || !ints(a + 2, 1, &top) || !PyFloat_Check(a[3])) Py_RETURN_NONE;
+  auto r = b200q_calls::token_log_probs(*t[0], t[1], top, PyFloat_AS_DOUBLE(a[3]));
+  PyObject* out = PyTuple_New(4);
+  if (out == nullptr) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::get<0>(r)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::get<1>(r)));
+  PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::get<2>(r)));
+  PyTuple_SET_ITEM(out, 3, THPVariable_Wrap(std::get<3>(r)));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"fp8_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_fp8_linear)), METH_FASTCALL,
      "x, w_codes, w_scales, bias, x_amax, tile_n -> bf16 tensor, or None: take the general path"},
@@ -659,6 +726,12 @@ PyMethodDef methods[] = {
      "k_pages, v_pages, block_table, lens, weights, out_table, keep, recent, sinks -> (kept, lens, weights) or None"},
     {"window_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_window_attention)), METH_FASTCALL,
      "q, k, v, q_lens, k_lens, scale, window, sinks -> tensor like q or None"},
+    {"shared_prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_shared_prefix_attention)), METH_FASTCALL,
+     "q, k_pages, v_pages, block_table, lens, plan, k_amax, v_amax, scale, groups, largest -> tensor like q or None"},
+    {"paged_copy", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_copy)), METH_FASTCALL,
+     "k_pages, v_pages, src, dst, rows -> whether it was taken"},
+    {"token_log_probs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_token_log_probs)), METH_FASTCALL,
+     "logits, tokens, top, scale -> (log_probs, entropy, top_log_probs, top_tokens) or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "b200q_native", "Whole calls of the b200q modules", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -23,6 +23,7 @@
 
 #include "b200q.h"
 #include "paged_calls.h"
+#include "score_calls.h"
 
 namespace {
 
@@ -479,6 +480,13 @@ Tensor window_attention_meta(const Tensor& q, const Tensor&, const Tensor&, cons
   return like_queries(q);
 }
 
+Tensor shared_prefix_attention_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t, int64_t,
+                                    const std::optional<Tensor>&, const std::optional<Tensor>&, double) {
+  return at::empty(q.sizes(), q.options());
+}
+void paged_copy_meta(at::TensorList, at::TensorList, at::IntArrayRef, at::IntArrayRef, at::OptionalIntArrayRef) {}
+Scores token_log_probs_meta(const Tensor& logits, const std::optional<Tensor>&, int64_t top, double) { return score_outputs(logits, top); }
+
 bool schema_exists(const char* name) {
   return c10::Dispatcher::singleton().findSchema({name, ""}).has_value();
 }
@@ -568,6 +576,19 @@ TORCH_LIBRARY_FRAGMENT(tensorrt, m) {
       "b200_window_attention(Tensor q, Tensor k, Tensor v, Tensor? q_lens, Tensor? k_lens, float scale, int window, int sinks) -> Tensor");
   m.impl("b200_window_attention", c10::DispatchKey::CUDA, TORCH_FN(window_attention));
   m.impl("b200_window_attention", c10::DispatchKey::Meta, TORCH_FN(window_attention_meta));
+
+  // Several continuations of one prompt; scale 0 = 1 / sqrt(head_dim)
+  m.def(
+      "b200_shared_prefix_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor lens, Tensor plan, int groups, int largest, "
+      "Tensor? k_amax, Tensor? v_amax, float scale) -> Tensor");
+  m.impl("b200_shared_prefix_attention", c10::DispatchKey::CUDA, TORCH_FN(shared_prefix_attention));
+  m.impl("b200_shared_prefix_attention", c10::DispatchKey::Meta, TORCH_FN(shared_prefix_attention_meta));
+  m.def("b200_paged_copy(Tensor(a!)[] k_pages, Tensor(b!)[] v_pages, int[] src, int[] dst, int[]? rows) -> ()");
+  m.impl("b200_paged_copy", c10::DispatchKey::CUDA, TORCH_FN(paged_copy));
+  m.impl("b200_paged_copy", c10::DispatchKey::Meta, TORCH_FN(paged_copy_meta));
+  m.def("b200_token_log_probs(Tensor logits, Tensor? tokens, int top, float scale) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.impl("b200_token_log_probs", c10::DispatchKey::CUDA, TORCH_FN(token_log_probs));
+  m.impl("b200_token_log_probs", c10::DispatchKey::Meta, TORCH_FN(token_log_probs_meta));
 
   // One-node quantized linears (activation first, result in the activation's dtype): the ops handed
   // to torch_tensorrt.dynamo.conversion.plugins.custom_op.

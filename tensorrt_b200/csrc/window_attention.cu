@@ -43,7 +43,7 @@
 #include "common.cuh"
 #include "ex2.cuh"
 #include "gemm_host.cuh"
-#include "tcgen05.cuh"
+#include "softmax_tc.cuh"
 
 namespace b200q {
 namespace {
@@ -98,8 +98,6 @@ struct WindowParams {
   int* status;
 };
 
-__device__ __forceinline__ void timed_out(int* status, int where) { atomicCAS(status, 0, where); }
-
 __device__ __forceinline__ int length_of(const int32_t* lens, int b, int most) {
   if (lens == nullptr) return most;
   int n;
@@ -114,30 +112,6 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uin
       "l"(reinterpret_cast<uint64_t>(m)), "r"(ptx::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
 }
-// kind::f16, fp32 accumulator; format 0 = fp16, 1 = bf16 for both operands; B K-major or N-major
-__device__ __forceinline__ uint32_t idesc_16(int format, int m, int n, int b_n_major) {
-  return (1u << 4) | (static_cast<uint32_t>(format) << 7) | (static_cast<uint32_t>(format) << 10) | (static_cast<uint32_t>(b_n_major) << 16) |
-         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float2 ld_cluster_f2(const float2* p, unsigned cta) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(ptx::mapa_u32(ptx::smem_u32(p), cta)) : "memory");
@@ -147,21 +121,6 @@ __device__ __forceinline__ float4 ld_cluster_f4(const float* p, unsigned cta) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(ptx::mapa_u32(ptx::smem_u32(p), cta)) : "memory");
   return v;
-}
-// true in one lane of a converged warp
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r != 0;
-}
-// the n lowest bits, n of any size
-__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
-template <typename T>
-__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
-  uint32_t r;
-  if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
 }
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, float* f) {

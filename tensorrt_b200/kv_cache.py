@@ -4,6 +4,8 @@
     paged_attention   one new token of every sequence over its pages
     paged_evict       the keys of the largest attention weights stay, their rows move to fresh pages
     window_attention  causal attention with a sliding window and sinks over contiguous K and V (prompts and their chunks)
+    paged_copy        pages to other pages, in the pools of all layers at once
+    shared_prefix_attention  paged_attention of a batch in which groups of sequences share the pages of a prefix (`SharedPrefix`)
 
 Pages are tensors [pages, kv heads, rows, D] (any strides with D contiguous) of float16, bfloat16, float8_e4m3fn or uint8 (FP8
 codes); token t of sequence b is row t % rows of page block_table[b, t // rows].  `lens` [B] counts the tokens of each sequence that
@@ -12,15 +14,19 @@ synchronises, and the calls can be captured in a CUDA graph.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
-from . import _native
+from . import _lib, _native
 from .ops import load_ops
+from .scores import TokenScores, token_log_probs
 
 load_ops()
 _ops = torch.ops.tensorrt
 _append, _attention = _ops.b200_paged_append.default, _ops.b200_paged_attention.default
 _evict, _window = _ops.b200_paged_evict.default, _ops.b200_window_attention.default
+_copy, _shared = _ops.b200_paged_copy.default, _ops.b200_shared_prefix_attention.default
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
@@ -65,10 +71,89 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale
     return _window(*args) if out is None else out
 
 
+def paged_copy(k_pages, v_pages, src: list, dst: list, rows: list | None = None) -> None:
+    """Copies page src[i] to page dst[i] in every pool: `k_pages` and `v_pages` a tensor each, or lists of as many (a layer's pools, or all
+    layers').  rows[i]: the first rows of the page that are copied (None: all).  The numbers are the host's and travel with the launch.  No
+    page may be written twice, nor be both read and written."""
+    k, v = ([p] if isinstance(p, torch.Tensor) else list(p) for p in (k_pages, v_pages))
+    args = (k, v, list(src), list(dst), None if rows is None else list(rows))
+    if not _native.paged_copy(*args):
+        _copy(*args)
+
+
+class SharedPrefix:
+    """Which sequences of a batch share a prefix: the sequences members[g] have their first tokens[g] tokens in the same pages, which are found
+    through the line of the block table of the first of them.  It goes by sequences and stays valid as they grow.
+
+    Groups of one sequence and prefixes of no token are left out: nothing is shared.  `update` says anew who shares what, in place, so that a
+    captured call goes by it; it takes up to `groups` groups of up to `largest` sequences (None: those given here)."""
+
+    def __init__(self, members: list, tokens: list, batch: int, device="cuda", groups: int | None = None, largest: int | None = None):
+        if batch < 0 or batch > 65535:
+            raise ValueError(f"need a batch of up to 65535 sequences, got {batch}")
+        kept = self._kept(members, tokens)
+        self.batch = batch
+        self.groups = len(kept) if groups is None else groups
+        self.largest = max([len(m) for m, _ in kept], default=0) if largest is None else largest
+        if not 0 <= self.groups <= batch or not 0 <= self.largest <= batch:
+            raise ValueError(f"{self.groups} groups of up to {self.largest} sequences are not in a batch of {batch}")
+        self.plan = torch.zeros(_lib.load().b200q_shared_prefix_plan_values(batch, self.groups), dtype=torch.int32, device=device)
+        self.update(members, tokens)
+
+    @staticmethod
+    def _kept(members: list, tokens: list) -> list:
+        if len(members) != len(tokens):
+            raise ValueError(f"expected as many prefixes ({len(tokens)}) as groups ({len(members)})")
+        if any(t < 0 or t > 0x7FFFFFFF for t in tokens):
+            raise ValueError(f"a prefix has from 0 to {0x7FFFFFFF} tokens, got {tokens}")
+        return [(list(m), t) for m, t in zip(members, tokens) if len(m) > 1 and t > 0]
+
+    def update(self, members: list, tokens: list) -> None:
+        kept = self._kept(members, tokens)
+        if len(kept) > self.groups or any(len(m) > self.largest for m, _ in kept):
+            raise ValueError(f"made for {self.groups} groups of up to {self.largest} sequences, got groups of {[len(m) for m, _ in kept]}")
+        flat = [b for m, _ in kept for b in m]
+        seen = set(flat)
+        if len(seen) != len(flat) or any(b < 0 or b >= self.batch for b in seen):
+            raise ValueError(f"a sequence of a batch of {self.batch} is in one group at most, got {members}")
+        ends = [0]
+        for m, _ in kept:
+            ends.append(ends[-1] + len(m))
+        ends += ends[-1:] * (self.groups - len(kept))                       # empty groups
+        shared = [t for _, t in kept] + [0] * (self.groups - len(kept))
+        ints = lambda v: (ctypes.c_int32 * max(len(v), 1))(*v)  # noqa: E731
+        plan = torch.empty(self.plan.shape, dtype=torch.int32)
+        _lib.check(_lib.load().b200q_shared_prefix_plan(ints(flat), ints(ends), ints(shared), self.groups, self.batch, plan.data_ptr()),
+                   "b200q_shared_prefix_plan")
+        self.plan.copy_(plan.pin_memory() if self.plan.is_cuda else plan, non_blocking=True)
+
+
+def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
+                            prefix: SharedPrefix, *, k_amax: torch.Tensor | None = None, v_amax: torch.Tensor | None = None,
+                            scale: float | None = None) -> torch.Tensor:
+    """`paged_attention` of a batch in which groups of sequences share a prefix: its keys are attended to by all rows of a group at once, and read
+    once for up to 128 of them; the keys behind it through each sequence's own line of the table.  A sequence with fewer tokens than
+    its group's prefix is attended to through its own line alone."""
+    if prefix.batch != q.shape[0]:
+        raise ValueError(f"the prefixes are those of a batch of {prefix.batch}, q is {tuple(q.shape)}")
+    scale = 0.0 if scale is None else scale
+    out = _native.shared_prefix_attention(q, k_pages, v_pages, block_table, lens, prefix.plan, k_amax, v_amax, scale, prefix.groups, prefix.largest)
+    return _shared(q, k_pages, v_pages, block_table, lens, prefix.plan, prefix.groups, prefix.largest, k_amax, v_amax, scale) if out is None else out
+
+
 def _on_device(values, device, dtype=torch.int32) -> torch.Tensor:
     """Values of the host as a tensor on `device`, without a wait for its stream (a copy from pageable memory is one)."""
     t = torch.as_tensor(values, dtype=dtype)
     return t.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else t
+
+
+def _common(a: list, b: list) -> int:
+    """Length of the longest common beginning, by comparisons of whole slices."""
+    low, high = 0, min(len(a), len(b))
+    while low < high:
+        mid = (low + high + 1) // 2
+        low, high = (mid, high) if a[low:mid] == b[low:mid] else (low, mid - 1)
+    return low
 
 
 _WHOLE = "prompts are attended to as a whole: a sequence that brings tokens must hold no older ones"
@@ -84,7 +169,11 @@ class PagedKvCache:
     in front (`reserve`).
 
     dtype bfloat16 or float16 as the tokens are, or float8_e4m3fn with `k_amax`, `v_amax`: per layer one value or one per kv head.
-    `weights` True keeps the sums of attention weights by which `evict` chooses."""
+    `weights` True keeps the sums of attention weights by which `evict` chooses.
+
+    `fork` continues a sequence several times: the continuations share its pages, `attend` attends to what a group of them shares at once, and
+    a page that is not full is copied when the first of those that share it grows.  `truncate` takes tokens back, `compact` moves the pages in
+    use to the front of the pools, `resize` changes how many there are."""
 
     def __init__(self, layers: int, batch: int, n_kv: int, head_dim: int, pages: int, max_tokens: int, page_size: int = 16, dtype=torch.bfloat16,
                  k_amax=None, v_amax=None, weights: bool = False, device="cuda"):
@@ -106,6 +195,8 @@ class PagedKvCache:
         self.weights = [torch.zeros(batch, n_kv, max_tokens, device=device) for _ in range(layers)] if weights else [None] * layers
         self._free = list(range(pages - 1, -1, -1))
         self._pages: list = [[] for _ in range(batch)]     # of each sequence, in order
+        self._uses = [0] * pages                           # sequences that a page is part of
+        self._prefix, self._shares, self._regroup = None, False, False
         self._tokens = [0] * batch
         self._released: set = set()
         self._padded = None
@@ -119,17 +210,36 @@ class PagedKvCache:
         return len(self._free)
 
     def reserve(self, tokens: list) -> None:
-        """Pages for sequences of up to `tokens[b]` tokens."""
+        """Pages for sequences of up to `tokens[b]` tokens.  A sequence that is to grow and whose last page is not full gets that page for
+        itself: a copy, where others share it."""
         if len(tokens) != self.batch or any(n > self.max_tokens for n in tokens):
             raise ValueError(f"expected {self.batch} counts of up to {self.max_tokens} tokens, got {tokens}")
         need = [max(0, -(-n // self.page_size) - len(p)) for n, p in zip(tokens, self._pages)]
-        if sum(need) > len(self._free):
-            raise RuntimeError(f"{sum(need)} pages are needed and {len(self._free)} are free")
+        own, left = [], {}                                 # sequences that need a copy; of a page, those that still share it
+        for b, (n, t) in enumerate(zip(tokens, self._tokens)):
+            if n > t and t % self.page_size:
+                last = self._pages[b][t // self.page_size]
+                left.setdefault(last, self._uses[last])
+                if left[last] > 1:                         # the last one of them keeps the page
+                    left[last] -= 1
+                    own.append(b)
+        if sum(need) + len(own) > len(self._free):
+            raise RuntimeError(f"{sum(need) + len(own)} pages are needed and {len(self._free)} are free")
         rows, cols, vals = [], [], []
+        if own:
+            at = [self._tokens[b] // self.page_size for b in own]
+            fresh = self._free[-len(own):][::-1]
+            paged_copy(self.k, self.v, [self._pages[b][i] for b, i in zip(own, at)], fresh, [self._tokens[b] % self.page_size for b in own])
+            del self._free[-len(own):]
+            for b, i, page in zip(own, at, fresh):
+                self._uses[self._pages[b][i]] -= 1
+                self._uses[page], self._pages[b][i] = 1, page
+            rows, cols, vals = list(own), at, list(fresh)
         for b, n in enumerate(need):
             for _ in range(n):
                 rows.append(b), cols.append(len(self._pages[b])), vals.append(self._free.pop())
                 self._pages[b].append(vals[-1])
+                self._uses[vals[-1]] = 1
         if vals:
             at = _on_device([rows, cols, vals], self.table.device)
             self.table[at[0], at[1]] = at[2]
@@ -186,7 +296,11 @@ class PagedKvCache:
         paged_append(k, v, self.k[layer], self.v[layer], self.table, self.lens, self._cu, k_amax=self.k_amax[layer], v_amax=self.v_amax[layer])
 
     def attend(self, layer: int, q: torch.Tensor, *, scale: float | None = None, window: int = 0, sinks: int = 0) -> torch.Tensor:
-        """Attention of the newest token of every sequence: q [batch, query heads, head_dim]."""
+        """Attention of the newest token of every sequence: q [batch, query heads, head_dim].  Without a window and without weights, what groups
+        of forked sequences share is attended to once for all of a group."""
+        if self.weights[layer] is None and window <= 0 and self._sharing():
+            return shared_prefix_attention(q, self.k[layer], self.v[layer], self.table, self.lens, self._prefix, k_amax=self.k_amax[layer],
+                                           v_amax=self.v_amax[layer], scale=scale)
         return paged_attention(q, self.k[layer], self.v[layer], self.table, self.lens, k_amax=self.k_amax[layer], v_amax=self.v_amax[layer],
                                weights=self.weights[layer], scale=scale, window=window, sinks=sinks)
 
@@ -239,22 +353,135 @@ class PagedKvCache:
         self.lens.copy_(lens)
         self.table.fill_(-1)
         self.table[:, :width] = out[:, :width]
+        for p in (p for pages in fresh for p in pages):
+            self._uses[p] = 1
         for old in self._pages:
-            self._free.extend(old)
+            self._give_back(old)
         self._pages, self._tokens = fresh, [min(keep, t) for t in self._tokens]
         self._new = [0] * self.batch
+        self._regroup = True
         return kept
 
+    def _give_back(self, pages: list) -> None:
+        for p in pages:
+            self._uses[p] -= 1
+            if self._uses[p] == 0:
+                self._free.append(p)
+
     def release(self, b: int) -> None:
-        """Sequence b is done: its pages are free, and it is empty until `grow` brings it tokens again."""
-        self._free.extend(self._pages[b])
+        """Sequence b is done: its pages are free (those that others share once these are done too), and it is empty until `grow` brings it
+        tokens again."""
+        self._give_back(self._pages[b])
         self._pages[b], self._tokens[b], self._new[b] = [], 0, 0
+        self._regroup = True
         self._released.add(b % self.batch)
         self.lens[b].zero_()
         self.table[b].fill_(-1)
         for w in self.weights:
             if w is not None:
                 w[b].zero_()
+
+    def fork(self, parents: list) -> None:
+        """Sequence b goes on from where sequence parents[b] is (b itself: from where it was), for all at once: [0] * batch continues the first one
+        `batch` times, and a step of a beam search is `fork` of the beams that were chosen.  Nothing is copied but what `evict` goes by: the
+        tokens stay in the pages that they are in.  What sequence b held before is gone, as after `release`; pages reserved for the parent
+        stay the parent's."""
+        if len(parents) != self.batch or any(p < 0 or p >= self.batch for p in parents):
+            raise ValueError(f"expected {self.batch} sequences to go on from, got {parents}")
+        moved = [b for b, p in enumerate(parents) if p != b]
+        if not moved:
+            return
+        held = {b: self._pages[parents[b]][:-(-self._tokens[parents[b]] // self.page_size)] for b in moved}
+        same = {b: _common(pages, self._pages[b]) for b, pages in held.items()}      # what a beam has in common with the one that it follows
+        for b, pages in held.items():
+            for p in pages[same[b]:]:
+                self._uses[p] += 1
+        for b in moved:
+            self._give_back(self._pages[b][same[b]:])
+        self._released = {b for b, p in enumerate(parents) if p in self._released}
+        self._tokens, self._new = [self._tokens[p] for p in parents], [0] * self.batch
+        for b, pages in held.items():
+            self._pages[b] = pages
+        width = self.table.shape[1]
+        both = _on_device([parents, [len(held[b]) if b in held else width for b in range(self.batch)]], self.table.device, torch.int64)
+        line = self.table.index_select(0, both[0])
+        self.table.copy_(line.masked_fill_(torch.arange(width, device=line.device) >= both[1][:, None], -1))
+        self.lens.copy_(self.lens.index_select(0, both[0]))
+        for w in self.weights:
+            if w is not None:
+                w.copy_(w.index_select(0, both[0]))
+        self._regroup = True
+
+    def truncate(self, tokens: list) -> None:
+        """Cuts every sequence to its first tokens[b] tokens (those that a verification turned down go, say); the pages behind them are free, reserved
+        ones among them."""
+        if len(tokens) != self.batch or any(n < 0 or n > t for n, t in zip(tokens, self._tokens)):
+            raise ValueError(f"expected {self.batch} counts of up to {self._tokens} tokens, got {tokens}")
+        keep = [-(-n // self.page_size) for n in tokens]
+        both = _on_device([list(tokens), keep], self.table.device)
+        for b, n in enumerate(keep):
+            self._give_back(self._pages[b][n:])
+            del self._pages[b][n:]
+        self._tokens, self._new = list(tokens), [0] * self.batch
+        self.table.masked_fill_(torch.arange(self.table.shape[1], device=self.table.device) >= both[1][:, None], -1)
+        self.lens.copy_(both[0])
+        for w in self.weights:
+            if w is not None:
+                w.masked_fill_(torch.arange(w.shape[2], device=w.device) >= both[0][:, None, None], 0.0)
+        self._regroup = True
+
+    def compact(self) -> int:
+        """Moves the pages in use to the front of the pools, shared ones once, and returns how many they are."""
+        used = sum(1 for n in self._uses if n)
+        src = [p for p in range(used, len(self._uses)) if self._uses[p]]
+        dst = [p for p in range(used) if not self._uses[p]]
+        if src:
+            paged_copy(self.k, self.v, src, dst)
+            to = dict(zip(src, dst))
+            self._pages = [[to.get(p, p) for p in pages] for pages in self._pages]
+            for a, b in to.items():
+                self._uses[b], self._uses[a] = self._uses[a], 0
+            place = list(range(len(self._uses)))
+            for a, b in to.items():
+                place[a] = b
+            place = _on_device(place, self.table.device)
+            self.table.copy_(torch.where(self.table < 0, self.table, place[self.table.clamp_min(0).long()]))
+        self._free = list(range(len(self._uses) - 1, used - 1, -1))
+        return used
+
+    def resize(self, pages: int) -> None:
+        """Pools of `pages` pages, at least those in use, in the place of the old ones: `k` and `v` are other tensors then, and captured steps are to be
+        captured again."""
+        used = sum(1 for n in self._uses if n)
+        if pages < max(used, 1):
+            raise ValueError(f"{used} pages are in use, {pages} are too few")
+        self.compact()
+        for pools in (self.k, self.v):
+            for i, old in enumerate(pools):
+                new = torch.zeros((pages, *old.shape[1:]), dtype=old.dtype, device=old.device)
+                new.view(torch.uint8)[:used] = old.view(torch.uint8)[:used]
+                pools[i] = new
+                del old, new
+        self._uses = self._uses[:used] + [0] * (pages - used)
+        self._free = list(range(pages - 1, used - 1, -1))
+
+    def _sharing(self) -> bool:
+        """Whether any sequences share a prefix; who shares what is found anew behind what changed it, and kept where a captured step reads it."""
+        if self._regroup:
+            self._regroup = False
+            first: dict = {}
+            for b, pages in enumerate(self._pages):
+                if self._tokens[b] >= self.page_size and self._uses[pages[0]] > 1:
+                    first.setdefault(pages[0], []).append(b)
+            members = [m for m in first.values() if len(m) > 1]
+            # pages that all of a group have in common and that are full
+            shared = [self.page_size * min(min(_common(self._pages[m[0]], self._pages[b]), self._tokens[b] // self.page_size) for b in m) for m in members]
+            self._shares = bool(members)
+            if self._prefix is None and members:
+                self._prefix = SharedPrefix([], [], self.batch, self.table.device, groups=self.batch // 2, largest=self.batch)
+            if self._prefix is not None:
+                self._prefix.update(members, shared)
+        return self._shares
 
 
 class CachedDecoder:
@@ -265,6 +492,8 @@ class CachedDecoder:
         decoder.prompt(h, [n0, n1, ..])      # h [n0 + n1 + .., hidden]: the prompts, one behind the other -> the same shape
         decoder.prompt(h, [0, n1, ..])       # sequences that go on bring none: a released one takes a new prompt
         decoder.step(h)                      # h [batch, hidden]: one token of every sequence that is not released -> the same shape
+        decoder.score(h, head, top=4)        # what ranks the continuations: log probabilities, entropy, the most likely tokens
+        cache.fork([0, 0, 1, 1])             # and those that are chosen go on
     """
 
     def __init__(self, stack, cache: PagedKvCache, window: int = 0, sinks: int = 0):
@@ -306,3 +535,7 @@ class CachedDecoder:
         self._check(h, self.cache.batch)
         self.cache.grow_all()
         return self._walk(h, lambda i, q, k, v: self.cache.attend(i, q, window=self.window, sinks=self.sinks))
+
+    def score(self, h: torch.Tensor, head, tokens: torch.Tensor | None = None, *, top: int = 0, scale: float = 1.0) -> TokenScores:
+        """`token_log_probs` of the logits that `head` (an `Fp8Linear`, `Nvfp4Linear` or any other module) makes of h [rows, hidden]."""
+        return token_log_probs(head(h), tokens, top=top, scale=scale)
