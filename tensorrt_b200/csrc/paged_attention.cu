@@ -243,67 +243,9 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
   return total;
 }
 
-// Where the parts of a sequence's prefix lie, for one kv head.
-struct PrefixPlace {
-  int64_t total, start;      // tiles of all, tiles in front of the kv head's items
-  int ctas, tiles, item, row;  // CTAs, tiles of an item, first item, first row
-  bool on;
-};
-__device__ __noinline__ PrefixPlace prefix_place(const DecodeParams& p, int b, int h) {
-  PrefixPlace w{};
-  const int g = paged::ld_index(p.x.group_of + b);
-  w.on = paged::prefix_tokens(p.x, b, paged::cached_tokens(p.c, b, 0x7fffffff)) > 0 && g >= 0 && g < p.x.groups;
-  if (!w.on) return w;
-  const paged::GroupWork group = paged::group_work(p.x, p.c, g);
-  const int place = paged::ld_index(p.x.place_of + b);
-  const int64_t* const line = p.x.lines;
-  w.on = group.tiles > 0 && place >= 0 && place < group.n;
-  w.total = __ldcg(line + 2 * p.x.groups), w.ctas = static_cast<int>(__ldcg(line + 2 * p.x.groups + 1));
-  w.tiles = group.tiles, w.row = place * p.group;
-  w.item = static_cast<int>(__ldcg(line + 2 * g + 1)) + h * group.row_tiles;
-  w.start = __ldcg(line + 2 * g) + static_cast<int64_t>(h) * group.row_tiles * group.tiles;
-  return w;
-}
-// Adds the parts of the prefix, in the order of the keys, to four elements of a row.
-struct Joined {
-  float top, sum, acc[4];
-  bool has;
-};
-template <int DPAD>
-__device__ __noinline__ Joined join_prefix(const DecodeParams& p, const PrefixPlace w, int head, int d, Joined a) {
-  const int row = w.row + head, tile = row / paged::kPrefixRows, r = row % paged::kPrefixRows;
-  const int64_t start = w.start + static_cast<int64_t>(tile) * w.tiles;
-  const int c0 = holder(w.total, start, w.ctas), c1 = holder(w.total, start + w.tiles - 1, w.ctas);
-  constexpr int kAtOnce = 8;
-#pragma unroll 1
-  for (int c = c0; c <= c1; c += kAtOnce) {
-    float2 s[kAtOnce];
-    float4 v[kAtOnce];
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      s[k].y = -1.0f;
-      const int64_t slot = static_cast<int64_t>(w.item) + tile + c + k;
-      if (c + k > c1 || r >= p.x.rows || slot >= p.x.slots) continue;
-      s[k] = __ldcg(p.x.stats + slot * p.x.rows + r);
-      v[k] = __ldcg(reinterpret_cast<const float4*>(p.x.parts + (slot * p.x.rows + r) * DPAD + d));
-    }
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      if (s[k].y < 0.0f) continue;
-      a.has = true;
-      const float now = fmaxf(a.top, s[k].x), base = now == -INFINITY ? 0.0f : now, f0 = exp2_fast(a.top - base), f1 = exp2_fast(s[k].x - base);
-      a.sum = a.sum * f0 + s[k].y * f1;
-      a.acc[0] = a.acc[0] * f0 + v[k].x * f1, a.acc[1] = a.acc[1] * f0 + v[k].y * f1;
-      a.acc[2] = a.acc[2] * f0 + v[k].z * f1, a.acc[3] = a.acc[3] * f0 + v[k].w * f1;
-      a.top = now;
-    }
-  }
-  return a;
-}
-
-// BLOCKS8: query heads of an item in blocks of 8.  JOIN: behind the kernel of shared prefixes, whose parts of a row are joined with those found here.
-// Nothing else of that kernel is read, and it lets this one start only once everything in front of it has completed: what is waited for stands
-// where the parts are read.
+// BLOCKS8: query heads of an item in blocks of 8.  JOIN: behind the kernel of shared prefixes, over the keys that a sequence has to itself; the result
+// is a part of each row, as that kernel's are.  It reads nothing of that kernel, which lets it start only once everything in front has
+// completed: it waits at its end, so that it has ended only when the one in front has.
 template <typename T, bool CODES, int DPAD, int BLOCKS8, bool JOIN>
 __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm) decode_kernel(const __grid_constant__ DecodeParams p) {
   using S = Stage<CODES, DPAD, BLOCKS8>;
@@ -327,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
   Seen see;
   const int64_t total = find_start<JOIN>(p, cta, &ctas, &b, &before, &see);
   if (cta >= ctas) {
-    if constexpr (JOIN) pdl_wait();             // this kernel has ended only when the one in front has
+    if constexpr (JOIN) pdl_wait();
     return;
   }
   int64_t at = piece(total, cta, ctas);
@@ -571,11 +513,6 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
             mine[row * DPAD + (CODES ? g * (DPAD / 8) + 2 * i + half : 16 * i + 8 * half + g)] = o[r][i][2 * half + e];
       }
     __syncthreads();
-    PrefixPlace place{};
-    if constexpr (JOIN) {
-      pdl_wait();
-      place = prefix_place(p, b, h);
-    }
     const bool whole = tile0 == 0 && tile1 == tiles;
     // CTAs that share the item: c0 .. c1, those with a piece of it; the counter of the one that begins it
     const int c0 = whole ? cta : holder(total, item_start, ctas), c1 = whole ? cta : holder(total, item_end - 1, ctas);
@@ -600,13 +537,10 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
       }
       if (whole) {
         if constexpr (JOIN) {
-          if (place.on) {
-            const Joined a = join_prefix<DPAD>(p, place, block * p.rows + row, d, Joined{top, sum, {acc[0], acc[1], acc[2], acc[3]}, has});
-            top = a.top, sum = a.sum, has = a.has;
-            acc[0] = a.acc[0], acc[1] = a.acc[1], acc[2] = a.acc[2], acc[3] = a.acc[3];
-          }
-        }
-        if (d < p.c.D) {
+          const int64_t at = static_cast<int64_t>(b) * p.Hq + head0 + row;
+          *reinterpret_cast<float4*>(p.x.own + at * DPAD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          if (d == 0) p.x.own_stats[at] = make_float2(top, has ? sum : -1.0f);
+        } else if (d < p.c.D) {
           const float f = v_scale / sum;
           T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.Hq + head0 + row) * p.c.D + d;
           uint2 r = make_uint2(0, 0);
@@ -677,13 +611,10 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
             continue;
           }
           if constexpr (JOIN) {
-            if (place.on) {
-            const Joined a = join_prefix<DPAD>(p, place, block * p.rows + row, d, Joined{top, sum, {acc[0], acc[1], acc[2], acc[3]}, has});
-            top = a.top, sum = a.sum, has = a.has;
-            acc[0] = a.acc[0], acc[1] = a.acc[1], acc[2] = a.acc[2], acc[3] = a.acc[3];
-          }
-          }
-          if (d < p.c.D) {
+            const int64_t to = static_cast<int64_t>(b) * p.Hq + head0 + row;
+            *reinterpret_cast<float4*>(p.x.own + to * DPAD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            if (d == 0) p.x.own_stats[to] = make_float2(top, has ? sum : -1.0f);
+          } else if (d < p.c.D) {
             const float f = v_scale / sum;
             T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.Hq + head0 + row) * p.c.D + d;
             uint2 r = make_uint2(0, 0);
@@ -709,6 +640,7 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
       if (++h == p.c.heads) h = 0, see = keys_seen<JOIN>(p, ++b);
     }
   }
+  if constexpr (JOIN) pdl_wait();
 }
 
 // weights[b, h, token] += sum over the query heads of P, from the logits that the kernel above left and their normalisers.
@@ -786,10 +718,10 @@ int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
 }  // namespace
 
 int paged::attend_behind_prefix(const Cache& c, const Prefix& x, const void* q, int dtype, const int64_t* q_strides, int64_t B, int64_t Hq, float scale,
-                                void* out, void* workspace, cudaStream_t st) {
+                                void* workspace, cudaStream_t st) {
   DecodeParams p{};
   p.c = c, p.x = x;
-  set_shape(&p, q, q_strides, out, B, Hq, scale, workspace);
+  set_shape(&p, q, q_strides, nullptr, B, Hq, scale, workspace);
   const int64_t tiles = (c.capacity > 0 ? (c.capacity + kTile - 1) / kTile : 1) * B * c.heads * p.blocks;
   return launch_decode_t<true>(p, dtype, tiles, st);
 }

@@ -37,6 +37,7 @@ struct PrefixParams {
   Cache c;
   Prefix x;
   int page_shift;            // log2 of the page size, or -1
+  int box_rows, box_shift;   // rows of a page that a copy by tensor map takes, a power of two, and its logarithm
   const char* q;
   int64_t q_batch, q_head;   // bytes
   float scale;
@@ -54,7 +55,7 @@ template <int DPAD>
 struct Layout {
   static constexpr int kBoxes = DPAD / 64, kBoxBytes = 128 * 128, kTileBytes = kBoxes * kBoxBytes;
   static constexpr int kStages = DPAD == 128 ? 2 : 4;
-  static constexpr int kBars = 2 * kStages + 6;
+  static constexpr int kBars = 3 * kStages + 6;
   static constexpr int kSlots = 8;                      // of tiles whose masks are kept
   static constexpr int kSmem = 1024 + (1 + kStages) * kTileBytes + kBars * 8 + kSlots * 16 + 16;
   static constexpr int kMmaWarp = 4, kThreads = 128 + 32 * (1 + kLoadWarps);
@@ -179,13 +180,56 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
 __device__ __forceinline__ void widen(uint32_t v, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
 }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
+// 4-D tiled load into this CTA's shared memory, completion on this CTA's own barrier.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int32_t x, int32_t y, int32_t z, int32_t w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(ptx::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
 // Place of 16 bytes (piece c of a row) in a tile of 128 rows: boxes of 64 elements, 128-byte swizzle.
 __device__ __forceinline__ uint32_t tile_at(int row, int c) {
   return static_cast<uint32_t>((c >> 3) * (128 * 128) + row * 128 + (((c & 7) ^ (row & 7)) * 16));
 }
 
-template <typename T, bool CODES, int DPAD>
-__global__ void __launch_bounds__(Layout<DPAD>::kThreads, kPerSm) prefix_kernel(const __grid_constant__ PrefixParams p) {
+// Rows of codes, each in the first bytes of 128, to rows of fp16 in their tile: a row's place takes its own codes' place, so nothing but the warp that
+// widens it need have read it.  Rows without a key become zeros.  `first`: of the warp's rows; `there`: 32 bits for 32 keys.
+template <int DPAD, int ROWS>
+__device__ __forceinline__ void widen_rows(uint32_t tile, int first, int D, const uint4& there) {
+  constexpr int kLanes = DPAD / 16, kAtOnce = 32 / kLanes, kBatch = 4;
+  const int lane = threadIdx.x & 31, c = lane % kLanes;
+  const uint32_t codes = tile + (DPAD == 128 ? 128 * 128 : 0);
+  const uint32_t words[4] = {there.x, there.y, there.z, there.w};
+#pragma unroll 1
+  for (int r0 = first; r0 < first + ROWS; r0 += kAtOnce * kBatch) {
+    uint4 v[kBatch];
+    const uint32_t word = words[r0 >> 5] >> (r0 & 31);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = k * kAtOnce + lane / kLanes;
+      v[k] = (word >> i) & 1 ? lds128(codes + (r0 + i) * 128 + c * 16) : make_uint4(0, 0, 0, 0);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int r = r0 + k * kAtOnce + lane / kLanes;
+      uint4 a, b;
+      widen(v[k].x, a.x, a.y), widen(v[k].y, a.z, a.w), widen(v[k].z, b.x, b.y), widen(v[k].w, b.z, b.w);
+      if (c * 16 < D) sts128(tile + tile_at(r, 2 * c), a), sts128(tile + tile_at(r, 2 * c + 1), b);
+    }
+    __syncwarp();
+  }
+}
+
+// MAPS: K and V rows come by tensor maps, box_rows of a page at once (pages of a multiple of eight rows); otherwise by threads, 16 bytes each.
+template <typename T, bool CODES, int DPAD, bool MAPS>
+__global__ void __launch_bounds__(Layout<DPAD>::kThreads, kPerSm)
+prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ PrefixParams p) {
   using L = Layout<DPAD>;
   constexpr bool kHalf = CODES || std::is_same<T, __half>::value;
   using E = std::conditional_t<kHalf, __half, __nv_bfloat16>;       // of the products
@@ -196,7 +240,8 @@ __global__ void __launch_bounds__(Layout<DPAD>::kThreads, kPerSm) prefix_kernel(
   uint64_t* const bars = reinterpret_cast<uint64_t*>(ring + L::kStages * L::kTileBytes);
   uint64_t* const full = bars;
   uint64_t* const empty = bars + L::kStages;
-  uint64_t* const q_full = empty + L::kStages;
+  uint64_t* const raw = empty + L::kStages;            // codes are there
+  uint64_t* const q_full = raw + L::kStages;
   uint64_t* const s_full = q_full + 1;
   uint64_t* const p_half = s_full + 1;
   uint64_t* const p_full = p_half + 1;
@@ -210,8 +255,9 @@ __global__ void __launch_bounds__(Layout<DPAD>::kThreads, kPerSm) prefix_kernel(
     ptx::tmem_alloc<1>(tmem_slot, L::kTmemCols);
     ptx::tmem_relinquish<1>();
   } else if (threadIdx.x == 0) {
-    // a stage is full when each loading thread's copies are there and the mask is written
-    for (int i = 0; i < L::kStages; ++i) ptx::mbar_init(full + i, 32 * kLoadWarps + 1), ptx::mbar_init(empty + i, 1);
+    // a stage is full when its boxes are there (codes: when two warps have widened them); or each loading thread's copies, and the mask is written
+    for (int i = 0; i < L::kStages; ++i)
+      ptx::mbar_init(full + i, MAPS ? (CODES ? 2 : 1) : 32 * kLoadWarps + 1), ptx::mbar_init(empty + i, 1), ptx::mbar_init(raw + i, 1);
     ptx::mbar_init(q_full, 4);
     ptx::mbar_init(s_full, 2);
     ptx::mbar_init(p_half, 4);
@@ -219,6 +265,10 @@ __global__ void __launch_bounds__(Layout<DPAD>::kThreads, kPerSm) prefix_kernel(
     ptx::mbar_init(o_full, 1);
     ptx::mbar_init(done, 1);
     ptx::fence_barrier_init();
+    if constexpr (MAPS) {
+      ptx::prefetch_tmap(&tk);
+      ptx::prefetch_tmap(&tv);
+    }
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -230,8 +280,116 @@ __global__ void __launch_bounds__(Layout<DPAD>::kThreads, kPerSm) prefix_kernel(
 
   if (warp >= L::kMmaWarp) {
     ptx::setmaxnreg_dec<L::kOtherRegs>();
-    if (warp > L::kMmaWarp) {
-      // ------------------------------------------------------------- loads
+    if (MAPS && warp == L::kMmaWarp + 1) {
+      // ------------------------------------------------------------- loads: a lane asks for a box of each tile
+      const int boxes = kPrefixKeys >> p.box_shift, rows = p.box_rows;
+      uint64_t* const arrival = CODES ? raw : full;
+      bool ok = true;
+      int st = 0, n = 0, issued = 0;
+      uint32_t ph = 0;
+      for (; walk.left > 0 && ok; walk.next(p)) {
+        const int count = walk.count(), tokens = walk.w.tokens;
+        const int leader = paged::ld_index(p.x.order + walk.w.first);
+        const bool named = leader >= 0 && leader < p.x.B;
+        const int32_t* line = p.c.table + (named ? leader : 0) * p.c.table_stride;
+        int page, row;                                // of this lane's box
+        auto find = [&](int tile) {
+          const int t = tile * kPrefixKeys + lane * rows;
+          page = -1, row = 0;
+          if (named && lane < boxes && t < tokens) {
+            const int at = p.page_shift >= 0 ? t >> p.page_shift : t / p.c.page_size;
+            page = paged::ld_index(line + at);
+            row = t - at * p.c.page_size;
+          }
+        };
+        find(walk.tile);
+        for (int j = 0; j < count && ok; ++j) {
+          const int t = (walk.tile + j) * kPrefixKeys + lane * rows;
+          const bool exists = static_cast<unsigned>(page) < static_cast<unsigned>(p.c.num_pages);
+          const int there_rows = exists ? min(rows, tokens - t) : 0;
+          const int z = exists ? page : p.c.num_pages, y = row;      // behind the last page: zeros
+          if (j + 1 < count) find(walk.tile + j + 1);
+          // a box that the prefix ends in: what lies behind may be anything, and 0 times a NaN of V would be one
+          const unsigned cut = __ballot_sync(0xffffffffu, there_rows > 0 && there_rows < rows);
+          uint4 words = make_uint4(~0u, ~0u, ~0u, ~0u);
+          if (!__all_sync(0xffffffffu, lane >= boxes || there_rows == rows)) {
+            uint32_t w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int key = u * 32 + lane;
+              w[u] = __ballot_sync(0xffffffffu, (key & (rows - 1)) < __shfl_sync(0xffffffffu, there_rows, key >> p.box_shift));
+            }
+            words = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          if (lane == 0) there[n % L::kSlots] = words;
+          ++n;
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv) {
+            if (!ptx::mbar_wait(empty + st, ph ^ 1u)) {
+              timed_out(p.status, 90);
+              ok = false;
+              break;
+            }
+            const uint32_t dst = ptx::smem_u32(ring + st * L::kTileBytes);
+            const bool by_rows = !CODES && kv == 1 && cut != 0;      // one box at most: the last
+            if (by_rows) {
+              const int who = __ffs(cut) - 1, left = __shfl_sync(0xffffffffu, there_rows, who);
+              const int64_t off = __shfl_sync(0xffffffffu, z, who) * p.c.v.page + __shfl_sync(0xffffffffu, y, who) * p.c.v.row + walk.h * p.c.v.head;
+              for (int i = lane; i < rows * (DPAD / 8); i += 32) {
+                const int r = i / (DPAD / 8), c = i % (DPAD / 8);
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (r < left && c * 8 < p.c.D) v = ld_128(p.c.v.base + off + r * p.c.v.row + c * 16);
+                sts128(dst + tile_at(who * rows + r, c), v);
+              }
+              ptx::fence_proxy_async();
+              __syncwarp();
+            }
+            if (lane == 0) ptx::mbar_arrive_expect_tx(arrival + st, (CODES ? 128 * 128 : L::kTileBytes) - (by_rows ? rows * L::kBoxes * 128 : 0));
+            __syncwarp();
+            if (lane < boxes && !(by_rows && cut >> lane & 1)) {
+              const uint32_t to = dst + lane * rows * 128;
+              if constexpr (CODES) {
+                tma_load_4d(to + (DPAD == 128 ? 128 * 128 : 0), kv == 0 ? &tk : &tv, raw + st, 0, y, walk.h, z);
+              } else {
+#pragma unroll
+                for (int x = 0; x < L::kBoxes; ++x) tma_load_4d(to + x * L::kBoxBytes, kv == 0 ? &tk : &tv, full + st, x * 64, y, walk.h, z);
+              }
+            }
+            ++issued;
+            if (++st == L::kStages) st = 0, ph ^= 1u;
+          }
+        }
+      }
+      // no copy may be under way when the CTA ends, whatever became of its readers
+      for (int i = max(0, issued - L::kStages); i < issued; ++i)
+        if (!ptx::mbar_wait(arrival + i % L::kStages, (i / L::kStages) & 1)) timed_out(p.status, 91);
+    } else if (MAPS && warp > L::kMmaWarp) {
+      // ------------------------------------------------------------- codes to fp16, half of a tile's rows a warp
+      if constexpr (CODES) {
+        bool ok = true;
+        int st = 0, n = 0;
+        uint32_t ph = 0;
+        for (; walk.left > 0 && ok; walk.next(p)) {
+          const int count = walk.count();
+          for (int j = 0; j < count && ok; ++j, ++n) {
+#pragma unroll 1
+            for (int kv = 0; kv < 2; ++kv) {
+              if (!ptx::mbar_wait(raw + st, ph)) {
+                timed_out(p.status, 92);
+                ok = false;
+                break;
+              }
+              widen_rows<DPAD, 64>(ptx::smem_u32(ring + st * L::kTileBytes), (warp - L::kMmaWarp - 2) * 64, p.c.D, there[n % L::kSlots]);
+              ptx::fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) ptx::mbar_arrive(full + st);
+              if (++st == L::kStages) st = 0, ph ^= 1u;
+            }
+          }
+        }
+      }
+    } else if (warp > L::kMmaWarp) {
+      // ------------------------------------------------------------- loads by threads
       const int loader = warp - L::kMmaWarp - 1;
       bool ok = true;
       int st = 0, n = 0;                              // stage; tiles so far
@@ -284,9 +442,8 @@ __global__ void __launch_bounds__(Layout<DPAD>::kThreads, kPerSm) prefix_kernel(
               for (int u = 0; u < 4; ++u) {
                 for (int r0 = loader * kRowsAtOnce; r0 < 32; r0 += kLoadWarps * kRowsAtOnce) {
                   const int r = r0 + lane / kLanes;
-                  const bool in = r < 32;
-                  const int64_t off = __shfl_sync(0xffffffffu, kv == 0 ? k_row[u] : v_row[u], in ? r : 0);
-                  if (in && c * 8 < p.c.D) copy16(dst + tile_at(u * 32 + r, c), src + (off < 0 ? 0 : off) + c * 16, off < 0 ? 0 : 16);
+                  const int64_t off = __shfl_sync(0xffffffffu, kv == 0 ? k_row[u] : v_row[u], r);
+                  if (c * 8 < p.c.D) copy16(dst + tile_at(u * 32 + r, c), src + (off < 0 ? 0 : off) + c * 16, off < 0 ? 0 : 16);
                 }
               }
               arrive_with_copies(full + st);
@@ -297,9 +454,8 @@ __global__ void __launch_bounds__(Layout<DPAD>::kThreads, kPerSm) prefix_kernel(
               for (int u = 0; u < 4; ++u) {
                 for (int r0 = loader * kRowsAtOnce; r0 < 32; r0 += kLoadWarps * kRowsAtOnce) {
                   const int r = r0 + lane / kLanes;
-                  const bool in = r < 32;
-                  const int64_t off = __shfl_sync(0xffffffffu, kv == 0 ? k_row[u] : v_row[u], in ? r : 0);
-                  if (in && c * 16 < p.c.D) {
+                  const int64_t off = __shfl_sync(0xffffffffu, kv == 0 ? k_row[u] : v_row[u], r);
+                  if (c * 16 < p.c.D) {
                     uint4 v = make_uint4(0, 0, 0, 0);
                     if (off >= 0) v = ld_128(src + off + c * 16);
                     uint4 a, b;
@@ -566,10 +722,116 @@ __global__ void __launch_bounds__(Layout<DPAD>::kThreads, kPerSm) prefix_kernel(
   }
 }
 
-template <typename T, bool CODES, int DPAD>
-int launch_prefix(const PrefixParams& p, cudaStream_t st) {
+// The parts of every row together: those of its prefix, in the order of the keys, and that of its own keys.  A row has 1, 2, 4 or 8 of a CTA's warps, a
+// share of the parts each.
+struct JoinParams {
+  Cache c;
+  Prefix x;
+  void* out;
+  int B, Hq, rows_log2;      // rows of a CTA
+};
+constexpr int kJoinWarps = 8;
+
+struct PartSum {
+  float top, sum, acc[4];
+  bool has;
+  __device__ __forceinline__ void add(const float2& s, const float4& v) {
+    if (s.y < 0.0f) return;
+    has = true;
+    const float now = fmaxf(top, s.x), base = now == -INFINITY ? 0.0f : now, f0 = exp2_fast(top - base), f1 = exp2_fast(s.x - base);
+    sum = sum * f0 + s.y * f1;
+    acc[0] = acc[0] * f0 + v.x * f1, acc[1] = acc[1] * f0 + v.y * f1;
+    acc[2] = acc[2] * f0 + v.z * f1, acc[3] = acc[3] * f0 + v.w * f1;
+    top = now;
+  }
+};
+
+template <typename T, int DPAD>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ JoinParams p) {
+  __shared__ float4 acc_of[kJoinWarps][32];
+  __shared__ float2 stats_of[kJoinWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share_log2 = 3 - p.rows_log2, share = warp & ((1 << share_log2) - 1);
+  const int64_t id = (static_cast<int64_t>(blockIdx.x) << p.rows_log2) + (warp >> share_log2);
+  const bool there = id < static_cast<int64_t>(p.B) * p.Hq;
+  const int b = there ? static_cast<int>(id / p.Hq) : 0, hq = there ? static_cast<int>(id - static_cast<int64_t>(b) * p.Hq) : 0;
+  const int h = hq / p.x.group, d = lane * 4;
+  pdl_launch_dependents();
+  pdl_wait();
+  PartSum a{-INFINITY, 0.0f, {}, false};
+  if (there) {
+    const int g = paged::ld_index(p.x.group_of + b), place = paged::ld_index(p.x.place_of + b);
+    const bool grouped = paged::prefix_tokens(p.x, b, paged::cached_tokens(p.c, b, 0x7fffffff)) > 0 && g >= 0 && g < p.x.groups;
+    const GroupWork w = grouped ? paged::group_work(p.x, p.c, g) : GroupWork{};
+    if (grouped && w.tiles > 0 && place >= 0 && place < w.n) {
+      const int64_t total = __ldcg(p.x.lines + 2 * p.x.groups);
+      const int ctas = static_cast<int>(__ldcg(p.x.lines + 2 * p.x.groups + 1));
+      const int row = place * p.x.group + hq - h * p.x.group, tile = row / kPrefixRows, r = row % kPrefixRows;
+      const int64_t items = static_cast<int64_t>(h) * w.row_tiles + tile, start = __ldcg(p.x.lines + 2 * g) + items * w.tiles;
+      const int64_t slot0 = __ldcg(p.x.lines + 2 * g + 1) + items;
+      const int c0 = holder(total, start, ctas), c1 = holder(total, start + w.tiles - 1, ctas);
+      const int parts = c1 - c0 + 1, from = c0 + (parts * share >> share_log2), to = c0 + (parts * (share + 1) >> share_log2);
+      constexpr int kAtOnce = 8;
+#pragma unroll 1
+      for (int c = from; c < to; c += kAtOnce) {
+        float2 s[kAtOnce];
+        float4 v[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {            // the loads first: they do not wait for one another
+          s[k].y = -1.0f;
+          const int64_t slot = slot0 + c + k;
+          if (c + k >= to || r >= p.x.rows || slot >= p.x.slots) continue;
+          s[k] = __ldcg(p.x.stats + slot * p.x.rows + r);
+          if (d < DPAD) v[k] = __ldcg(reinterpret_cast<const float4*>(p.x.parts + (slot * p.x.rows + r) * DPAD + d));
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) a.add(s[k], v[k]);
+      }
+    }
+    if (share == (1 << share_log2) - 1) {              // behind the prefix
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (d < DPAD) v = __ldcg(reinterpret_cast<const float4*>(p.x.own + id * DPAD + d));
+      a.add(__ldcg(p.x.own_stats + id), v);
+    }
+  }
+  if (share_log2 > 0) {
+    acc_of[warp][lane] = make_float4(a.acc[0], a.acc[1], a.acc[2], a.acc[3]);
+    if (lane == 0) stats_of[warp] = make_float2(a.top, a.has ? a.sum : -1.0f);
+    __syncthreads();
+    if (share > 0) return;
+    for (int k = 1; k < 1 << share_log2; ++k) a.add(stats_of[warp + k], acc_of[warp + k][lane]);
+  }
+  if (!there || d >= p.c.D) return;
+  uint2 u = make_uint2(0, 0);
+  if (a.has) {
+    const float f = (p.c.codes ? paged::head_scale(p.c.v_amax, p.c.amax_stride, h) : 1.0f) / a.sum;
+    u = make_uint2(pack16<T>(a.acc[0] * f, a.acc[1] * f), pack16<T>(a.acc[2] * f, a.acc[3] * f));
+  }
+  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + id * p.c.D + d) = u;
+}
+
+// [D, rows, heads, pages] -> boxes of 128 bytes x box_rows of one head and page, zeros out of bounds; false where a tensor map cannot hold the strides
+bool make_map(CUtensorMap* map, const paged::Pool& pool, const Cache& c, int dtype, int box_rows) {
+  gemm::EncodeTiledFn fn = gemm::encode_tiled();
+  if (fn == nullptr) return false;
+  const int size = c.codes ? 1 : 2;
+  const int64_t strides_in[3] = {pool.row, pool.head, pool.page}, counts[3] = {c.page_size, c.heads, c.num_pages};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) {
+    if (counts[i] > 1 && (strides_in[i] <= 0 || strides_in[i] >= (1LL << 40))) return false;
+    strides[i] = static_cast<cuuint64_t>(counts[i] > 1 ? strides_in[i] : 256);       // where there is one only, any stride will do
+  }
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.D), static_cast<cuuint64_t>(c.page_size), static_cast<cuuint64_t>(c.heads),
+                              static_cast<cuuint64_t>(c.num_pages)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / size), static_cast<cuuint32_t>(box_rows), 1, 1}, unit[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = c.codes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : (dtype == B200Q_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+  return fn(map, type, 4, pool.base, dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, c.codes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, bool CODES, int DPAD, bool MAPS>
+int launch_prefix(const CUtensorMap& tk, const CUtensorMap& tv, const PrefixParams& p, cudaStream_t st) {
   using L = Layout<DPAD>;
-  auto kernel = prefix_kernel<T, CODES, DPAD>;
+  auto kernel = prefix_kernel<T, CODES, DPAD, MAPS>;
   static std::atomic<bool> ready[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return B200Q_ERR_CUDA;
@@ -578,13 +840,26 @@ int launch_prefix(const PrefixParams& p, cudaStream_t st) {
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
   }
   const int ctas = kPerSm * sm_count() < kMostCtas ? kPerSm * sm_count() : kMostCtas;
-  if (launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(L::kThreads), L::kSmem, st, p) != cudaSuccess) return B200Q_ERR_CUDA;
+  if (launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(L::kThreads), L::kSmem, st, tk, tv, p) != cudaSuccess) return B200Q_ERR_CUDA;
+  return check_launch();
+}
+template <typename T, bool CODES>
+int launch_prefix_d(bool maps, const CUtensorMap& tk, const CUtensorMap& tv, const PrefixParams& p, cudaStream_t st) {
+  if (p.c.D <= 64) return maps ? launch_prefix<T, CODES, 64, true>(tk, tv, p, st) : launch_prefix<T, CODES, 64, false>(tk, tv, p, st);
+  return maps ? launch_prefix<T, CODES, 128, true>(tk, tv, p, st) : launch_prefix<T, CODES, 128, false>(tk, tv, p, st);
+}
+
+template <typename T>
+int launch_join(const JoinParams& p, cudaStream_t st) {
+  const int64_t rows = static_cast<int64_t>(p.B) * p.Hq, ctas = (rows + (1 << p.rows_log2) - 1) >> p.rows_log2;
+  auto kernel = p.c.D <= 64 ? join_kernel<T, 64> : join_kernel<T, 128>;
+  if (launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kJoinWarps * 32), 0, st, p) != cudaSuccess) return B200Q_ERR_CUDA;
   return check_launch();
 }
 
 // Parts of a call, at most, and the rows of each: all of its CTAs' and all items.
 struct Sizes {
-  int64_t rows, slots, parts, stats, lines, bytes;
+  int64_t rows, slots, parts, stats, lines, own, own_stats, bytes;
 };
 bool sizes_of(int64_t B, int64_t Hq, int64_t heads, int64_t D, int64_t groups, int64_t largest, Sizes* s) {
   if (B <= 0 || Hq <= 0 || heads <= 0 || Hq % heads != 0 || D <= 0 || D > paged::kMaxD || groups < 0 || groups > B || largest < 0 || largest > B ||
@@ -595,12 +870,13 @@ bool sizes_of(int64_t B, int64_t Hq, int64_t heads, int64_t D, int64_t groups, i
   // sum over the groups of ceil(sequences * group / 128), each at most its own number of row tiles, all together one more than full ones each
   const int64_t most = groups * ((largest * group + kPrefixRows - 1) / kPrefixRows), all = B * group / kPrefixRows + groups;
   s->slots = heads * (most < all ? most : all) + kMostCtas;
-  s->lines = (2 * groups + 2) * 8;
-  s->stats = s->slots * s->rows * 8;
-  s->parts = s->slots * s->rows * up * 4;
   const auto round = [](int64_t n) { return (n + 255) / 256 * 256; };
-  s->lines = round(s->lines), s->stats = round(s->stats);
-  s->bytes = s->lines + s->stats + round(s->parts);
+  s->lines = round((2 * groups + 2) * 8);
+  s->stats = round(s->slots * s->rows * 8);
+  s->own_stats = round(B * Hq * 8);
+  s->own = round(B * Hq * up * 4);
+  s->parts = round(s->slots * s->rows * up * 4);
+  s->bytes = s->lines + s->stats + s->own_stats + s->own + s->parts;
   return true;
 }
 
@@ -665,22 +941,28 @@ int b200q_shared_prefix_attention(const void* q, int dtype, const int64_t* q_str
   p.scale = scale;
   p.status = gemm::device_status_word();
   if (p.status == nullptr) return B200Q_ERR_CUDA;
-  char* const ws = static_cast<char*>(workspace);
+  char* at = static_cast<char*>(workspace);
+  const auto take = [&at](int64_t n) { char* const here = at; at += n; return here; };
   p.x = Prefix{plan, plan + B, plan + 2 * B, plan + 3 * B, plan + 4 * B, plan + 4 * B + groups + 1, static_cast<int>(B), static_cast<int>(groups),
-               static_cast<int>(largest), p.c.heads, static_cast<int>(Hq / p.c.heads), static_cast<int>(s.rows), s.slots,
-               reinterpret_cast<float*>(ws + s.lines + s.stats), reinterpret_cast<float2*>(ws + s.lines), reinterpret_cast<int64_t*>(ws)};
+               static_cast<int>(largest), p.c.heads, static_cast<int>(Hq / p.c.heads), static_cast<int>(s.rows), s.slots};
+  p.x.lines = reinterpret_cast<int64_t*>(take(s.lines));
+  p.x.stats = reinterpret_cast<float2*>(take(s.stats));
+  p.x.own_stats = reinterpret_cast<float2*>(take(s.own_stats));
+  p.x.own = reinterpret_cast<float*>(take(s.own));
+  p.x.parts = reinterpret_cast<float*>(take(s.parts));
   const auto st = static_cast<cudaStream_t>(stream);
-  const bool narrow = p.c.D <= 64;
+  CUtensorMap tk{}, tv{};
+  for (p.box_rows = 1; p.box_rows < kPrefixKeys && p.c.page_size % (2 * p.box_rows) == 0;) p.box_rows *= 2, ++p.box_shift;
+  const bool maps = p.box_rows >= 8 && p.c.num_pages > 0 && make_map(&tk, p.c.k, p.c, dtype, p.box_rows) && make_map(&tv, p.c.v, p.c, dtype, p.box_rows);
   int rc;
-  if (dtype == B200Q_BF16) {
-    if (p.c.codes) rc = narrow ? launch_prefix<__nv_bfloat16, true, 64>(p, st) : launch_prefix<__nv_bfloat16, true, 128>(p, st);
-    else rc = narrow ? launch_prefix<__nv_bfloat16, false, 64>(p, st) : launch_prefix<__nv_bfloat16, false, 128>(p, st);
-  } else {
-    if (p.c.codes) rc = narrow ? launch_prefix<__half, true, 64>(p, st) : launch_prefix<__half, true, 128>(p, st);
-    else rc = narrow ? launch_prefix<__half, false, 64>(p, st) : launch_prefix<__half, false, 128>(p, st);
-  }
+  if (dtype == B200Q_BF16) rc = p.c.codes ? launch_prefix_d<__nv_bfloat16, true>(maps, tk, tv, p, st) : launch_prefix_d<__nv_bfloat16, false>(maps, tk, tv, p, st);
+  else rc = p.c.codes ? launch_prefix_d<__half, true>(maps, tk, tv, p, st) : launch_prefix_d<__half, false>(maps, tk, tv, p, st);
+  if (rc == B200Q_OK) rc = paged::attend_behind_prefix(p.c, p.x, q, dtype, q_strides, B, Hq, scale, attention_workspace, st);
   if (rc != B200Q_OK) return rc;
-  return paged::attend_behind_prefix(p.c, p.x, q, dtype, q_strides, B, Hq, scale, out, attention_workspace, st);
+  // a warp to a row where there are rows for all SMs, up to eight otherwise
+  JoinParams join{p.c, p.x, out, static_cast<int>(B), static_cast<int>(Hq), 3};
+  while (join.rows_log2 > 0 && (B * Hq) >> join.rows_log2 < 2 * sm_count()) --join.rows_log2;
+  return dtype == B200Q_BF16 ? launch_join<__nv_bfloat16>(join, st) : launch_join<__half>(join, st);
 }
 
 }  // extern "C"

@@ -42,6 +42,8 @@ struct Prefix {
   float* parts;                 // [slots][rows][D up to 64 or 128], unnormalised
   float2* stats;                // [slots][rows] base-2 logarithm of what they are referred to, sum (-1: no key)
   int64_t* lines;               // [groups][2] tiles and items in front of each group; behind them: tiles of all, CTAs
+  float* own;                   // [B][Hq][D up to 64 or 128] the part of each row's own keys
+  float2* own_stats;            // [B][Hq]
 };
 
 struct GroupWork {
@@ -64,8 +66,8 @@ __device__ __forceinline__ int prefix_tokens(const Prefix& x, int b, int n) {
   return t > 0 && t <= n ? t : 0;
 }
 
-// The kernel behind that of the prefixes: single-token attention over the keys that a sequence has to itself, joined with the parts of its prefix.
-int attend_behind_prefix(const Cache& c, const Prefix& x, const void* q, int dtype, const int64_t* q_strides, int64_t B, int64_t Hq, float scale, void* out,
+// Behind the kernel of the prefixes: single-token attention over the keys that a sequence has to itself, into `own` and `own_stats`.
+int attend_behind_prefix(const Cache& c, const Prefix& x, const void* q, int dtype, const int64_t* q_strides, int64_t B, int64_t Hq, float scale,
                          void* workspace, cudaStream_t st);
 
 }  // namespace paged
