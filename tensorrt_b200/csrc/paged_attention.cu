@@ -216,9 +216,16 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
   for (int base = 0; base < p.B; base += kThreads) {
     if (base + tid < p.B) keys = keys_seen<JOIN>(p, base + tid);
     mine = base + tid < p.B ? keys.tiles() * per : 0;
+    const int64_t before = total;
     total += scan(mine);
+    if constexpr (JOIN) {
+      if (cta == 0 && base + tid < p.B) p.x.own_lines[base + tid] = before + inclusive - mine;
+    }
   }
   if (total < *ctas) *ctas = static_cast<int>(total);
+  if constexpr (JOIN) {
+    if (cta == 0 && tid == 0) p.x.own_lines[p.B] = total, p.x.own_lines[p.B + 1] = *ctas;
+  }
   if (cta >= *ctas) return total;
   const int64_t want = piece(total, cta, *ctas);
   if (p.B <= kThreads) {
@@ -245,7 +252,8 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
 
 // BLOCKS8: query heads of an item in blocks of 8.  JOIN: behind the kernel of shared prefixes, over the keys that a sequence has to itself; the result
 // is a part of each row, as that kernel's are.  It reads nothing of that kernel, which lets it start only once everything in front has
-// completed: it waits at its end, so that it has ended only when the one in front has.
+// completed: it waits at its end, so that it has ended only when the one in front has.  Parts are joined by the kernel behind, not here: with many short
+// sequences the exchange among CTAs was most of the time.
 template <typename T, bool CODES, int DPAD, int BLOCKS8, bool JOIN>
 __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm) decode_kernel(const __grid_constant__ DecodeParams p) {
   using S = Stage<CODES, DPAD, BLOCKS8>;
@@ -513,7 +521,8 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
             mine[row * DPAD + (CODES ? g * (DPAD / 8) + 2 * i + half : 16 * i + 8 * half + g)] = o[r][i][2 * half + e];
       }
     __syncthreads();
-    const bool whole = tile0 == 0 && tile1 == tiles;
+    const bool whole = JOIN || (tile0 == 0 && tile1 == tiles);
+    const int64_t own_slot = (static_cast<int64_t>(b) * p.c.heads + h) * p.blocks + block;
     // CTAs that share the item: c0 .. c1, those with a piece of it; the counter of the one that begins it
     const int c0 = whole ? cta : holder(total, item_start, ctas), c1 = whole ? cta : holder(total, item_end - 1, ctas);
     float* part = p.parts + (static_cast<int64_t>(cta) * 2 + (at == first_tile ? 0 : 1)) * kPart;
@@ -535,12 +544,12 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
         const float4 v = *reinterpret_cast<const float4*>(smem + w * S::kDepth * S::kBytes + (row * DPAD + d) * 4);
         acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
       }
-      if (whole) {
-        if constexpr (JOIN) {
-          const int64_t at = static_cast<int64_t>(b) * p.Hq + head0 + row;
-          *reinterpret_cast<float4*>(p.x.own + at * DPAD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-          if (d == 0) p.x.own_stats[at] = make_float2(top, has ? sum : -1.0f);
-        } else if (d < p.c.D) {
+      if constexpr (JOIN) {
+        const int64_t to = (own_slot + cta) * p.rows + row;
+        *reinterpret_cast<float4*>(p.x.own + to * DPAD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        if (d == 0) p.x.own_stats[to] = make_float2(top, has ? sum : -1.0f);
+      } else if (whole) {
+        if (d < p.c.D) {
           const float f = v_scale / sum;
           T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.Hq + head0 + row) * p.c.D + d;
           uint2 r = make_uint2(0, 0);
@@ -610,11 +619,7 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
             if (d == 0) dst[kRows * DPAD + 2 * kRows + row] = top, dst[kRows * DPAD + 3 * kRows + row] = has ? sum : -1.0f;
             continue;
           }
-          if constexpr (JOIN) {
-            const int64_t to = static_cast<int64_t>(b) * p.Hq + head0 + row;
-            *reinterpret_cast<float4*>(p.x.own + to * DPAD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-            if (d == 0) p.x.own_stats[to] = make_float2(top, has ? sum : -1.0f);
-          } else if (d < p.c.D) {
+          if (d < p.c.D) {
             const float f = v_scale / sum;
             T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.Hq + head0 + row) * p.c.D + d;
             uint2 r = make_uint2(0, 0);
@@ -696,6 +701,11 @@ int launch_decode_t(const DecodeParams& p, int dtype, int64_t most_tiles, cudaSt
 }
 
 // What the query heads of a kv head, the pages and the workspace make of the parameters.
+void heads_of_items(int group, int* rows, int* blocks) {
+  *blocks = (group + kRows - 1) / kRows;
+  *rows = (group + *blocks - 1) / *blocks;
+  *blocks = (group + *rows - 1) / *rows;
+}
 void set_shape(DecodeParams* p, const void* q, const int64_t* q_strides, void* out, int64_t B, int64_t Hq, float scale, void* workspace) {
   p->page_shift = -1;
   if ((p->c.page_size & (p->c.page_size - 1)) == 0)
@@ -705,9 +715,7 @@ void set_shape(DecodeParams* p, const void* q, const int64_t* q_strides, void* o
   p->q_batch = q_strides[0] * 2, p->q_head = q_strides[1] * 2;
   p->out = out;
   p->B = static_cast<int>(B), p->Hq = static_cast<int>(Hq), p->group = static_cast<int>(Hq / p->c.heads);
-  p->blocks = (p->group + kRows - 1) / kRows;
-  p->rows = (p->group + p->blocks - 1) / p->blocks;
-  p->blocks = (p->group + p->rows - 1) / p->rows;
+  heads_of_items(p->group, &p->rows, &p->blocks);
   p->scale = scale;
   p->tickets = static_cast<unsigned*>(workspace);
   p->parts = reinterpret_cast<float*>(p->tickets + 2 * kMaxCtas);
@@ -716,6 +724,11 @@ void set_shape(DecodeParams* p, const void* q, const int64_t* q_strides, void* o
 int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
 
 }  // namespace
+
+void paged::own_shape(int64_t B, int64_t Hq, int64_t heads, int* rows, int* blocks, int64_t* slots) {
+  heads_of_items(static_cast<int>(Hq / heads), rows, blocks);
+  *slots = B * heads * *blocks + kMaxCtas;
+}
 
 int paged::attend_behind_prefix(const Cache& c, const Prefix& x, const void* q, int dtype, const int64_t* q_strides, int64_t B, int64_t Hq, float scale,
                                 void* workspace, cudaStream_t st) {

@@ -7,15 +7,17 @@
 // the prefix belong to one sequence each: the kernel of paged_attention.cu attends to them, and joins its result with the parts left here:
 // with m = max_i m_i, sum = sum_i l_i 2^(m_i - m), out = sum_i o_i 2^(m_i - m) / sum.
 //
-// Work: items (shared_prefix.cuh) cut into tiles of 128 keys, and the line of all tiles into equal pieces, one for each resident CTA, two to an SM.  A
-// CTA: four warps run the softmax, one thread to a row; one warp issues the products; three load K and V rows, which pages scatter, into
-// swizzled tiles (8-bit codes are widened to fp16 on the way, exactly).  P takes the place of the scores it came from in tensor memory.
+// Work: shared_prefix.cuh, a CTA to an SM.  Two times four warps run the softmax of a tile of 128 x 128 scores each, one thread to a row; one warp
+// issues the products of both in turn, so that the tensor cores work on one while the other is in its softmax; one asks for K and V rows, which
+// pages scatter, box by box (tensor maps); codes are widened to fp16, exactly, by four more warps in the place that they came to.  P takes the
+// place of the scores that it came from in tensor memory.
 //
 // Rounding: S, the softmax, O and the sums are 32-bit; P is rounded to 16 bits for the second product, an error of one rounding of each term,
 // of the size of the result's own.  fp16 (fp16 pages and codes): P is raised by 2^11, so that holds for terms down to 2^-25 of the largest.  bf16
 // queries in front of codes are scaled by a power of two into fp16's range, which loses nothing above 2^-38 of a row's largest.
 #include <atomic>
 
+#include "ex2.cuh"
 #include "gemm_host.cuh"
 #include "shared_prefix.cuh"
 #include "softmax_tc.cuh"
@@ -29,9 +31,7 @@ using paged::Prefix;
 using paged::kPrefixKeys;
 using paged::kPrefixRows;
 
-constexpr int kLoadWarps = 3;
-constexpr int kPerSm = 2;
-constexpr int kMostCtas = 320;                   // of a launch
+constexpr int kMostCtas = 192;                   // of a launch
 
 struct PrefixParams {
   Cache c;
@@ -50,121 +50,156 @@ template <bool HALF>
 constexpr float kLazy = HALF ? 4.0f : 8.0f;
 template <bool HALF>
 constexpr float kRaise = HALF ? 11.0f : 0.0f;
+constexpr int kPolyPairs = 2;   // of 16 pairs of exponentials: on the FMA pipe
 
-template <int DPAD>
+template <int DPAD, bool CODES>
 struct Layout {
   static constexpr int kBoxes = DPAD / 64, kBoxBytes = 128 * 128, kTileBytes = kBoxes * kBoxBytes;
-  static constexpr int kStages = DPAD == 128 ? 2 : 4;
-  static constexpr int kBars = 3 * kStages + 6;
-  static constexpr int kSlots = 8;                      // of tiles whose masks are kept
-  static constexpr int kSmem = 1024 + (1 + kStages) * kTileBytes + kBars * 8 + kSlots * 16 + 16;
-  static constexpr int kMmaWarp = 4, kThreads = 128 + 32 * (1 + kLoadWarps);
-  static constexpr int kTmemCols = 256;                 // S, then O
-  // 256 x 128 registers at launch = 128 x (184 + 72)
-  static constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
+  static constexpr int kTiles = DPAD == 128 ? 7 : 10;   // queries, then the ring; a second tile of queries takes a stage of it
+  static constexpr int kMostStages = kTiles - 1;
+  static constexpr int kBars = 3 * kMostStages + 11;
+  static constexpr int kSlots = 16;                     // of tiles whose masks are kept
+  static constexpr int kSmem = 1024 + kTiles * kTileBytes + kBars * 8 + 16 + kSlots * 16 + 16 + 128;
+  static constexpr int kThreads = CODES ? 512 : 384, kMmaWarp = 8, kLoadWarp = 9, kWidenWarp = 12, kWidenWarps = 4;
+  static constexpr int kLoadWarps = kThreads / 32 - kLoadWarp;        // where threads load
+  static constexpr int kTmemCols = 512;                 // the scores of both tiles, then O of both
+  // registers at launch: 384 x 168 = 256 x 192 + 128 x 120, 512 x 128 = 256 x 192 + 256 x 64
+  static constexpr int kSoftmaxRegs = 192, kOtherRegs = CODES ? 64 : 120;
 };
+
+// A wait whose long way stands in the code once: what a short call runs it also fetches, 40 KB of it in 5 us.
+__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, int* status, int where) {
+  if (ptx::mbar_wait(bar, parity)) return true;
+  timed_out(status, where);
+  return false;
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* status, int where) {
+  return ptx::mbar_try_wait(bar, parity) || wait_on(bar, parity, status, where);
+}
 
 // A CTA's way along its piece of the line, item after item.
 struct Walk {
-  int64_t left;              // tiles from here to the end of the piece
-  int g, h, row_tile, tile;  // the item, and the first tile of this CTA's part of it
-  int64_t item;              // its number
+  int64_t left;              // steps from here to the end of the piece
+  int64_t item;              // number of the item
+  int g, h, block, step;     // the item, and the first step of this CTA's part of it
+  int steps, blocks;         // of an item, of a kv head
+  bool paired;
   GroupWork w;
-  __device__ __forceinline__ int count() const { return static_cast<int>(left < w.tiles - tile ? left : w.tiles - tile); }
+  __device__ __forceinline__ int count() const { return static_cast<int>(left < steps - step ? left : steps - step); }
+  // first row of tile s, first key tile of step j of it; whether there are any
+  __device__ __forceinline__ int row0(int s) const { return paired ? block * 256 + s * 128 : block * 128; }
+  __device__ __forceinline__ int tile(int j, int s) const { return paired ? step + j : 2 * (step + j) + s; }
+  __device__ __forceinline__ bool has(int j, int s) const { return s == 0 || (paired ? row0(1) < w.rows : tile(j, 1) < w.tiles); }
+  // key tiles of the first `count` steps that are loaded
+  __device__ __forceinline__ int loaded(int count) const { return paired ? count : 2 * count - (has(count - 1, 1) ? 0 : 1); }
+  __device__ __noinline__ void set_group(const PrefixParams& p, int group) {
+    g = group;
+    w = paged::group_work(p.x, p.c, g);
+    steps = w.steps(paired), blocks = w.blocks(paired);
+  }
   __device__ __forceinline__ void next(const PrefixParams& p) {
-    left -= count();
-    tile = 0;
+    left -= count() + paged::kItemSteps;
+    step = 0;
     if (left <= 0) return;
     ++item;
-    if (++row_tile < w.row_tiles) return;
-    row_tile = 0;
+    if (++block < blocks) return;
+    block = 0;
     if (++h < p.x.heads) return;
     h = 0;
     do {
-      if (++g >= p.x.groups) {
+      if (g + 1 >= p.x.groups) {
         left = 0;
         return;
       }
-      w = paged::group_work(p.x, p.c, g);
-    } while (w.tiles == 0);
+      set_group(p, g + 1);
+    } while (steps == 0);
   }
 };
 
-// Adds up the tiles of all groups and finds the one that holds the first tile of this CTA's piece; all threads take part.  CTA 0 leaves the sums
-// where the kernel behind finds them.
-template <int THREADS>
-__device__ __forceinline__ Walk find_start(const PrefixParams& p, int cta, int ctas) {
-  constexpr int kWarps = THREADS / 32;
-  __shared__ int64_t sums[2][kWarps];
-  __shared__ int64_t found[3];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t tiles = 0, items = 0, mine_tiles = 0, mine_items = 0;      // in front of and of this thread's group
-  auto group = [&](int g) {
-    mine_tiles = mine_items = 0;
-    if (g < p.x.groups) {
-      const GroupWork w = paged::group_work(p.x, p.c, g);
-      if (w.tiles > 0) mine_items = static_cast<int64_t>(p.x.heads) * w.row_tiles, mine_tiles = mine_items * w.tiles;
-    }
-  };
-  auto scan = [&](int64_t* all_tiles, int64_t* all_items) {
-    int64_t a = mine_tiles, b = mine_items;
+static_assert(sizeof(Walk) <= 128, "has a place in shared memory");
+
+// A place in the ring of stages.
+struct Ring {
+  int stage, stages;
+  uint32_t phase;
+  __device__ __forceinline__ void advance(int n) {
+    stage += n;
+    if (stage >= stages) stage -= stages, phase ^= 1u;
+  }
+};
+
+__device__ __noinline__ int64_t warp_scan(int64_t v) {               // inclusive
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t oa = __shfl_up_sync(0xffffffffu, a, d), ob = __shfl_up_sync(0xffffffffu, b, d);
-      if (lane >= d) a += oa, b += ob;
-    }
-    if (lane == 31) sums[0][warp] = a, sums[1][warp] = b;
-    __syncthreads();
-    int64_t ta = 0, tb = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) a += sums[0][w], b += sums[1][w];
-      ta += sums[0][w], tb += sums[1][w];
-    }
-    __syncthreads();
-    tiles = a - mine_tiles, items = b - mine_items;
-    *all_tiles = ta, *all_items = tb;
-  };
-  int64_t total = 0, ignored = 0, items_before = 0;
-  for (int base = 0; base < p.x.groups; base += THREADS) {
-    int64_t t, n;
-    group(base + tid);
-    scan(&t, &n);
-    if (cta == 0 && base + tid < p.x.groups) {
-      p.x.lines[2 * (base + tid)] = total + tiles;
-      p.x.lines[2 * (base + tid) + 1] = items_before + items;
-    }
-    total += t, items_before += n;
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t o = __shfl_up_sync(0xffffffffu, v, d);
+    if ((threadIdx.x & 31) >= d) v += o;
   }
-  if (total < ctas) ctas = static_cast<int>(total);
-  if (cta == 0 && tid == 0) p.x.lines[2 * p.x.groups] = total, p.x.lines[2 * p.x.groups + 1] = ctas;
-  Walk walk{};
-  if (cta >= ctas) return walk;
-  const int64_t want = piece(total, cta, ctas);
-  int64_t before = 0;
-  items_before = 0;
-  for (int base = 0; base < p.x.groups; base += THREADS) {
-    int64_t t, n;
-    if (p.x.groups > THREADS) {
-      group(base + tid);
-      scan(&t, &n);
-    } else {
-      t = total, n = ignored;
-    }
-    if (want >= before + tiles && want < before + tiles + mine_tiles) found[0] = base + tid, found[1] = before + tiles, found[2] = items_before + items;
-    before += t, items_before += n;
-    if (before > want) break;
-  }
-  __syncthreads();
-  walk.g = static_cast<int>(found[0]);
-  walk.w = paged::group_work(p.x, p.c, walk.g);
-  const int64_t rel = want - found[1], item = divide(rel, walk.w.tiles);
-  walk.tile = static_cast<int>(rel - item * walk.w.tiles);
-  walk.h = static_cast<int>(divide(item, walk.w.row_tiles));
-  walk.row_tile = static_cast<int>(item - static_cast<int64_t>(walk.h) * walk.w.row_tiles);
-  walk.item = found[2] + item;
-  walk.left = piece(total, cta + 1, ctas) - want;
-  return walk;
+  return v;
 }
+
+// Adds up the steps of all groups, paired and not, takes what is less, and finds the group that holds the first step of this CTA's piece, by one
+// warp: where all took part the others' barriers and the code cost more than the sums.  CTA 0 leaves the sums where the kernel behind finds them.
+__device__ __forceinline__ void find_start(const PrefixParams& p, int cta, int ctas, Walk* out) {
+  const int lane = threadIdx.x & 31;
+  int64_t all[2] = {}, steps[2], items[2];             // not paired, paired
+  auto group = [&](int g) {
+    GroupWork w{};
+    if (g < p.x.groups) w = paged::group_work(p.x, p.c, g);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      items[i] = w.tiles > 0 ? static_cast<int64_t>(p.x.heads) * w.blocks(i) : 0;
+      steps[i] = items[i] * (w.steps(i) + paged::kItemSteps);
+    }
+  };
+#pragma unroll 1
+  for (int base = 0; base < p.x.groups; base += 32) {
+    group(base + lane);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) all[i] += __shfl_sync(0xffffffffu, warp_scan(steps[i]), 31);
+  }
+  const bool paired = all[1] <= all[0];
+  const int64_t total = paired ? all[1] : all[0];
+  if (total < ctas) ctas = static_cast<int>(total);
+  if (cta == 0 && lane == 0) {
+    int64_t* const end = p.x.lines + 2 * p.x.groups;
+    end[0] = total, end[1] = ctas, end[2] = paired ? 1 : 0;
+  }
+  Walk walk{};
+  walk.paired = paired;
+  if (cta < ctas) {
+    const int64_t want = piece(total, cta, ctas);
+    int64_t before = 0, before_items = 0, at = 0, item0 = 0;
+    int found = 0;
+#pragma unroll 1
+    for (int base = 0; base < p.x.groups; base += 32) {
+      if (p.x.groups > 32) group(base + lane);
+      const int64_t own = steps[paired], own_items = items[paired], upto = warp_scan(own), upto_items = warp_scan(own_items);
+      const int64_t begin = before + upto - own, begin_items = before_items + upto_items - own_items;
+      if (cta == 0 && base + lane < p.x.groups) p.x.lines[2 * (base + lane)] = begin, p.x.lines[2 * (base + lane) + 1] = begin_items;
+      const unsigned here = __ballot_sync(0xffffffffu, want >= begin && want < begin + own);
+      if (here != 0) {
+        const int who = __ffs(here) - 1;
+        found = base + who, at = __shfl_sync(0xffffffffu, begin, who), item0 = __shfl_sync(0xffffffffu, begin_items, who);
+        if (cta != 0) break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31), before_items += __shfl_sync(0xffffffffu, upto_items, 31);
+    }
+    walk.set_group(p, found);
+    const int64_t rel = want - at, item = divide(rel, walk.steps + paged::kItemSteps);
+    const int step = static_cast<int>(rel - item * (walk.steps + paged::kItemSteps)) - paged::kItemSteps;
+    walk.h = static_cast<int>(divide(item, walk.blocks));
+    walk.block = static_cast<int>(item - static_cast<int64_t>(walk.h) * walk.blocks);
+    walk.item = item0 + item;
+    walk.left = piece(total, cta + 1, ctas) - want;
+    if (step < 0) walk.left += step;                   // begins in front of the item's first step
+    walk.step = step < 0 ? 0 : step;
+  }
+  if (lane == 0) *out = walk;
+}
+
+// All threads of the CTA, at different places of the code: the start of the CTA's piece is known.
+template <int THREADS>
+__device__ __forceinline__ void found_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const char* src, int bytes) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -180,11 +215,6 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
 __device__ __forceinline__ void widen(uint32_t v, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
 }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 r;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
-  return r;
-}
 // 4-D tiled load into this CTA's shared memory, completion on this CTA's own barrier.
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int32_t x, int32_t y, int32_t z, int32_t w) {
   asm volatile(
@@ -197,72 +227,105 @@ __device__ __forceinline__ uint32_t tile_at(int row, int c) {
   return static_cast<uint32_t>((c >> 3) * (128 * 128) + row * 128 + (((c & 7) ^ (row & 7)) * 16));
 }
 
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
+  return r;
+}
 // Rows of codes, each in the first bytes of 128, to rows of fp16 in their tile: a row's place takes its own codes' place, so nothing but the warp that
-// widens it need have read it.  Rows without a key become zeros.  `first`: of the warp's rows; `there`: 32 bits for 32 keys.
-template <int DPAD, int ROWS>
-__device__ __forceinline__ void widen_rows(uint32_t tile, int first, int D, const uint4& there) {
-  constexpr int kLanes = DPAD / 16, kAtOnce = 32 / kLanes, kBatch = 4;
-  const int lane = threadIdx.x & 31, c = lane % kLanes;
+// widens it need have read it.  Rows without a key become zeros.  `first`: of the warp's 32 rows; `there`: a bit for each of them.
+// Eight lanes to a row, 8 codes each of either half of it; odd rows take the halves in the other order, so that two rows meet no bank twice.
+template <int DPAD>
+__device__ __forceinline__ void widen_rows(uint32_t tile, int first, int D, uint32_t there) {
+  constexpr int kBatch = 4;
+  const int lane = threadIdx.x & 31, c = lane & 7, turn = DPAD == 128 ? (lane >> 3) & 1 : 0;
   const uint32_t codes = tile + (DPAD == 128 ? 128 * 128 : 0);
-  const uint32_t words[4] = {there.x, there.y, there.z, there.w};
-#pragma unroll 1
-  for (int r0 = first; r0 < first + ROWS; r0 += kAtOnce * kBatch) {
-    uint4 v[kBatch];
-    const uint32_t word = words[r0 >> 5] >> (r0 & 31);
+#pragma unroll
+  for (int r0 = 0; r0 < 32; r0 += 4 * kBatch) {
+    uint2 v[kBatch][2];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int i = k * kAtOnce + lane / kLanes;
-      v[k] = (word >> i) & 1 ? lds128(codes + (r0 + i) * 128 + c * 16) : make_uint4(0, 0, 0, 0);
+      const int i = r0 + k * 4 + (lane >> 3);
+#pragma unroll
+      for (int half = 0; half < DPAD / 64; ++half)
+        v[k][half] = (there >> i) & 1 ? lds64(codes + (first + i) * 128 + (half ^ turn) * 64 + c * 8) : make_uint2(0, 0);
     }
     __syncwarp();
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int r = r0 + k * kAtOnce + lane / kLanes;
-      uint4 a, b;
-      widen(v[k].x, a.x, a.y), widen(v[k].y, a.z, a.w), widen(v[k].z, b.x, b.y), widen(v[k].w, b.z, b.w);
-      if (c * 16 < D) sts128(tile + tile_at(r, 2 * c), a), sts128(tile + tile_at(r, 2 * c + 1), b);
+      const int r = first + r0 + k * 4 + (lane >> 3);
+#pragma unroll
+      for (int half = 0; half < DPAD / 64; ++half) {
+        uint4 a;
+        widen(v[k][half].x, a.x, a.y), widen(v[k][half].y, a.z, a.w);
+        sts128(tile + tile_at(r, (half ^ turn) * 8 + c), a);        // behind D: zeros, as they came
+      }
     }
-    __syncwarp();
   }
+}
+
+// -inf in the place of the scores of keys that are not there, a bit for each key; all of a warp.  Rare: once an item, at holes in a table.
+__device__ __forceinline__ void mask_scores(uint32_t scores, uint4 there) {
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t word = c == 0 ? there.x : (c == 1 ? there.y : (c == 2 ? there.z : there.w));
+    uint32_t x[32];
+    ptx::tmem_ld_32x32(scores + c * 32, x);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e] = word & (1u << e) ? x[e] : 0xff800000u;
+    ptx::tmem_st_32x32_x16(scores + c * 32, x);
+    ptx::tmem_st_32x32_x16(scores + c * 32 + 16, x + 16);
+  }
+  ptx::tmem_st_wait();
+}
+// The first `left` of `rows` rows of a page into a tile of V, zeros behind, by one warp.
+template <int DPAD>
+__device__ __noinline__ void rows_by_hand(const PrefixParams& p, uint32_t tile, const char* src, int first, int rows, int left) {
+  for (int k = threadIdx.x & 31; k < rows * (DPAD / 8); k += 32) {
+    const int r = k / (DPAD / 8), c = k % (DPAD / 8);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < left && c * 8 < p.c.D) v = ld_128(src + r * p.c.v.row + c * 16);
+    sts128(tile + tile_at(first + r, c), v);
+  }
+  ptx::fence_proxy_async();
+  __syncwarp();
 }
 
 // MAPS: K and V rows come by tensor maps, box_rows of a page at once (pages of a multiple of eight rows); otherwise by threads, 16 bytes each.
 template <typename T, bool CODES, int DPAD, bool MAPS>
-__global__ void __launch_bounds__(Layout<DPAD>::kThreads, kPerSm)
+__global__ void __launch_bounds__(Layout<DPAD, CODES>::kThreads, 1)
 prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ PrefixParams p) {
-  using L = Layout<DPAD>;
+  using L = Layout<DPAD, CODES>;
   constexpr bool kHalf = CODES || std::is_same<T, __half>::value;
   using E = std::conditional_t<kHalf, __half, __nv_bfloat16>;       // of the products
   extern __shared__ char smem_raw[];
   char* const base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
   char* const sq = base;
-  char* const ring = base + L::kTileBytes;
-  uint64_t* const bars = reinterpret_cast<uint64_t*>(ring + L::kStages * L::kTileBytes);
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(base + L::kTiles * L::kTileBytes);
   uint64_t* const full = bars;
-  uint64_t* const empty = bars + L::kStages;
-  uint64_t* const raw = empty + L::kStages;            // codes are there
-  uint64_t* const q_full = raw + L::kStages;
-  uint64_t* const s_full = q_full + 1;
-  uint64_t* const p_half = s_full + 1;
-  uint64_t* const p_full = p_half + 1;
-  uint64_t* const o_full = p_full + 1;
-  uint64_t* const done = o_full + 1;
+  uint64_t* const empty = full + L::kMostStages;
+  uint64_t* const raw = empty + L::kMostStages;          // codes are there
+  uint64_t* const q_full = raw + L::kMostStages;
+  uint64_t* const s_full = q_full + 2;
+  uint64_t* const p_half = s_full + 2;
+  uint64_t* const p_full = p_half + 2;
+  uint64_t* const o_full = p_full + 2;
+  uint64_t* const done = o_full + 2;
   uint4* const there = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(done + 1) + 15) & ~uintptr_t{15});   // which keys of a tile exist
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(there + L::kSlots);
+  Walk* const start = reinterpret_cast<Walk*>(tmem_slot + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == L::kMmaWarp) {
     ptx::tmem_alloc<1>(tmem_slot, L::kTmemCols);
     ptx::tmem_relinquish<1>();
   } else if (threadIdx.x == 0) {
-    // a stage is full when its boxes are there (codes: when two warps have widened them); or each loading thread's copies, and the mask is written
-    for (int i = 0; i < L::kStages; ++i)
-      ptx::mbar_init(full + i, MAPS ? (CODES ? 2 : 1) : 32 * kLoadWarps + 1), ptx::mbar_init(empty + i, 1), ptx::mbar_init(raw + i, 1);
-    ptx::mbar_init(q_full, 4);
-    ptx::mbar_init(s_full, 2);
-    ptx::mbar_init(p_half, 4);
-    ptx::mbar_init(p_full, 4);
-    ptx::mbar_init(o_full, 1);
+    // a stage is full when its boxes are there (codes: when four warps have widened them); or each loading thread's copies, and the mask is written
+    for (int i = 0; i < L::kMostStages; ++i)
+      ptx::mbar_init(full + i, MAPS ? (CODES ? L::kWidenWarps : 1) : 32 * L::kLoadWarps + 1), ptx::mbar_init(empty + i, 1), ptx::mbar_init(raw + i, 1);
+    for (int s = 0; s < 2; ++s)
+      ptx::mbar_init(q_full + s, 4), ptx::mbar_init(s_full + s, 2), ptx::mbar_init(p_half + s, 4), ptx::mbar_init(p_full + s, 4), ptx::mbar_init(o_full + s, 1);
     ptx::mbar_init(done, 1);
     ptx::fence_barrier_init();
     if constexpr (MAPS) {
@@ -274,132 +337,141 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_enter(true);           // the kernel behind starts once everything in front of this one has completed, and reads that without a wait
   const int cta = static_cast<int>(blockIdx.x);
-  Walk walk = find_start<L::kThreads>(p, cta, static_cast<int>(gridDim.x));
 
   if (warp >= L::kMmaWarp) {
     ptx::setmaxnreg_dec<L::kOtherRegs>();
-    if (MAPS && warp == L::kMmaWarp + 1) {
+    pdl_enter(true);         // the kernel behind starts once everything in front of this one has completed, and reads that without a wait
+    if (warp == L::kLoadWarp) find_start(p, cta, static_cast<int>(gridDim.x), start);
+    found_barrier<L::kThreads>();
+    Walk walk = *start;
+    // paired: two tiles of queries, a stage less
+    char* const ring_at = base + (walk.paired ? 2 : 1) * L::kTileBytes;
+    Ring ring{0, walk.paired ? L::kMostStages - 1 : L::kMostStages, 0};
+    if (MAPS && warp == L::kLoadWarp) {
       // ------------------------------------------------------------- loads: a lane asks for a box of each tile
       const int boxes = kPrefixKeys >> p.box_shift, rows = p.box_rows;
       uint64_t* const arrival = CODES ? raw : full;
       bool ok = true;
-      int st = 0, n = 0, issued = 0;
-      uint32_t ph = 0;
+      int n = 0, issued = 0;                          // tiles so far; stages filled
       for (; walk.left > 0 && ok; walk.next(p)) {
         const int count = walk.count(), tokens = walk.w.tokens;
         const int leader = paged::ld_index(p.x.order + walk.w.first);
         const bool named = leader >= 0 && leader < p.x.B;
         const int32_t* line = p.c.table + (named ? leader : 0) * p.c.table_stride;
-        int page, row;                                // of this lane's box
-        auto find = [&](int tile) {
-          const int t = tile * kPrefixKeys + lane * rows;
-          page = -1, row = 0;
-          if (named && lane < boxes && t < tokens) {
-            const int at = p.page_shift >= 0 ? t >> p.page_shift : t / p.c.page_size;
-            page = paged::ld_index(line + at);
-            row = t - at * p.c.page_size;
+        int page[2], row[2];                          // of this lane's box, of each tile of a step
+        auto find = [&](int j) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (s == 1 && walk.paired) break;
+            const int t = walk.tile(j, s) * kPrefixKeys + lane * rows;
+            page[s] = -1, row[s] = 0;
+            if (named && lane < boxes && t < tokens) {
+              const int at = p.page_shift >= 0 ? t >> p.page_shift : t / p.c.page_size;
+              page[s] = paged::ld_index(line + at);
+              row[s] = t - at * p.c.page_size;
+            }
           }
         };
-        find(walk.tile);
+        find(0);
         for (int j = 0; j < count && ok; ++j) {
-          const int t = (walk.tile + j) * kPrefixKeys + lane * rows;
-          const bool exists = static_cast<unsigned>(page) < static_cast<unsigned>(p.c.num_pages);
-          const int there_rows = exists ? min(rows, tokens - t) : 0;
-          const int z = exists ? page : p.c.num_pages, y = row;      // behind the last page: zeros
-          if (j + 1 < count) find(walk.tile + j + 1);
-          // a box that the prefix ends in: what lies behind may be anything, and 0 times a NaN of V would be one
-          const unsigned cut = __ballot_sync(0xffffffffu, there_rows > 0 && there_rows < rows);
-          uint4 words = make_uint4(~0u, ~0u, ~0u, ~0u);
-          if (!__all_sync(0xffffffffu, lane >= boxes || there_rows == rows)) {
-            uint32_t w[4];
+          const int tiles = walk.paired || !walk.has(j, 1) ? 1 : 2;
+          int z[2], y[2], held[2];
+          unsigned cut[2];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int key = u * 32 + lane;
-              w[u] = __ballot_sync(0xffffffffu, (key & (rows - 1)) < __shfl_sync(0xffffffffu, there_rows, key >> p.box_shift));
-            }
-            words = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-          if (lane == 0) there[n % L::kSlots] = words;
-          ++n;
-#pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv) {
-            if (!ptx::mbar_wait(empty + st, ph ^ 1u)) {
-              timed_out(p.status, 90);
-              ok = false;
-              break;
-            }
-            const uint32_t dst = ptx::smem_u32(ring + st * L::kTileBytes);
-            const bool by_rows = !CODES && kv == 1 && cut != 0;      // one box at most: the last
-            if (by_rows) {
-              const int who = __ffs(cut) - 1, left = __shfl_sync(0xffffffffu, there_rows, who);
-              const int64_t off = __shfl_sync(0xffffffffu, z, who) * p.c.v.page + __shfl_sync(0xffffffffu, y, who) * p.c.v.row + walk.h * p.c.v.head;
-              for (int i = lane; i < rows * (DPAD / 8); i += 32) {
-                const int r = i / (DPAD / 8), c = i % (DPAD / 8);
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < left && c * 8 < p.c.D) v = ld_128(p.c.v.base + off + r * p.c.v.row + c * 16);
-                sts128(dst + tile_at(who * rows + r, c), v);
+          for (int s = 0; s < 2; ++s) {
+            if (s >= tiles) break;
+            const int t = walk.tile(j, s) * kPrefixKeys + lane * rows;
+            const bool exists = static_cast<unsigned>(page[s]) < static_cast<unsigned>(p.c.num_pages);
+            held[s] = exists ? min(rows, tokens - t) : 0;
+            z[s] = exists ? page[s] : p.c.num_pages, y[s] = row[s];        // behind the last page: zeros
+            // a box that the prefix ends in: what lies behind may be anything, and 0 times a NaN of V would be one
+            cut[s] = __ballot_sync(0xffffffffu, held[s] > 0 && held[s] < rows);
+            uint4 words = make_uint4(~0u, ~0u, ~0u, ~0u);
+            if (!__all_sync(0xffffffffu, lane >= boxes || held[s] == rows)) {
+              uint32_t w[4];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                const int key = u * 32 + lane;
+                w[u] = __ballot_sync(0xffffffffu, (key & (rows - 1)) < __shfl_sync(0xffffffffu, held[s], key >> p.box_shift));
               }
-              ptx::fence_proxy_async();
-              __syncwarp();
+              words = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            if (lane == 0) ptx::mbar_arrive_expect_tx(arrival + st, (CODES ? 128 * 128 : L::kTileBytes) - (by_rows ? rows * L::kBoxes * 128 : 0));
+            if (lane == 0) there[(n + s) % L::kSlots] = words;
+          }
+          n += tiles;
+          if (j + 1 < count) find(j + 1);
+#pragma unroll 1
+          for (int i = 0; i < 2 * tiles; ++i) {       // K of the step's tiles, then V
+            const int kv = i >= tiles, s = kv ? i - tiles : i;
+            if (!ok) continue;
+            const int page_at = s ? z[1] : z[0], row_at = s ? y[1] : y[0];
+            if (!wait(empty + ring.stage, ring.phase ^ 1u, p.status, 90)) {
+              ok = false;
+              continue;
+            }
+            uint64_t* const bar = arrival + ring.stage;
+            const uint32_t dst = ptx::smem_u32(ring_at + ring.stage * L::kTileBytes);
+            const bool by_rows = !CODES && kv == 1 && (s ? cut[1] : cut[0]) != 0;      // one box at most: the last
+            if (by_rows) {
+              const int who = __ffs(s ? cut[1] : cut[0]) - 1, left = __shfl_sync(0xffffffffu, s ? held[1] : held[0], who);
+              const int64_t off = __shfl_sync(0xffffffffu, page_at, who) * p.c.v.page + __shfl_sync(0xffffffffu, row_at, who) * p.c.v.row + walk.h * p.c.v.head;
+              rows_by_hand<DPAD>(p, dst, p.c.v.base + off, who * rows, rows, left);
+            }
+            if (lane == 0) ptx::mbar_arrive_expect_tx(bar, (CODES ? 128 * 128 : L::kTileBytes) - (by_rows ? rows * L::kBoxes * 128 : 0));
             __syncwarp();
-            if (lane < boxes && !(by_rows && cut >> lane & 1)) {
+            if (lane < boxes && !(by_rows && (s ? cut[1] : cut[0]) >> lane & 1)) {
               const uint32_t to = dst + lane * rows * 128;
               if constexpr (CODES) {
-                tma_load_4d(to + (DPAD == 128 ? 128 * 128 : 0), kv == 0 ? &tk : &tv, raw + st, 0, y, walk.h, z);
+                tma_load_4d(to + (DPAD == 128 ? 128 * 128 : 0), kv == 0 ? &tk : &tv, bar, 0, row_at, walk.h, page_at);
               } else {
 #pragma unroll
-                for (int x = 0; x < L::kBoxes; ++x) tma_load_4d(to + x * L::kBoxBytes, kv == 0 ? &tk : &tv, full + st, x * 64, y, walk.h, z);
+                for (int x = 0; x < L::kBoxes; ++x) tma_load_4d(to + x * L::kBoxBytes, kv == 0 ? &tk : &tv, bar, x * 64, row_at, walk.h, page_at);
               }
             }
             ++issued;
-            if (++st == L::kStages) st = 0, ph ^= 1u;
+            ring.advance(1);
           }
         }
       }
       // no copy may be under way when the CTA ends, whatever became of its readers
-      for (int i = max(0, issued - L::kStages); i < issued; ++i)
-        if (!ptx::mbar_wait(arrival + i % L::kStages, (i / L::kStages) & 1)) timed_out(p.status, 91);
-    } else if (MAPS && warp > L::kMmaWarp) {
-      // ------------------------------------------------------------- codes to fp16, half of a tile's rows a warp
-      if constexpr (CODES) {
-        bool ok = true;
-        int st = 0, n = 0;
-        uint32_t ph = 0;
-        for (; walk.left > 0 && ok; walk.next(p)) {
-          const int count = walk.count();
-          for (int j = 0; j < count && ok; ++j, ++n) {
+      for (int i = max(0, issued - ring.stages); i < issued; ++i)
+        wait(arrival + i % ring.stages, (i / ring.stages) & 1, p.status, 91);
+    } else if (MAPS && CODES && warp >= L::kWidenWarp) {
+      // ------------------------------------------------------------- codes to fp16, a quarter of a tile's rows a warp
+      bool ok = true;
+      int n = 0;
+      for (; walk.left > 0 && ok; walk.next(p)) {
+        const int count = walk.count();
+        for (int j = 0; j < count && ok; ++j) {
+          const int tiles = walk.paired || !walk.has(j, 1) ? 1 : 2;
 #pragma unroll 1
-            for (int kv = 0; kv < 2; ++kv) {
-              if (!ptx::mbar_wait(raw + st, ph)) {
-                timed_out(p.status, 92);
-                ok = false;
-                break;
-              }
-              widen_rows<DPAD, 64>(ptx::smem_u32(ring + st * L::kTileBytes), (warp - L::kMmaWarp - 2) * 64, p.c.D, there[n % L::kSlots]);
-              ptx::fence_proxy_async();
-              __syncwarp();
-              if (lane == 0) ptx::mbar_arrive(full + st);
-              if (++st == L::kStages) st = 0, ph ^= 1u;
+          for (int i = 0; i < 2 * tiles; ++i) {
+            if (!wait(raw + ring.stage, ring.phase, p.status, 92)) {
+              ok = false;
+              break;
             }
+            const uint32_t* const words = reinterpret_cast<const uint32_t*>(there + (n + (tiles == 2 ? i & 1 : 0)) % L::kSlots);
+            widen_rows<DPAD>(ptx::smem_u32(ring_at + ring.stage * L::kTileBytes), (warp - L::kWidenWarp) * 32, p.c.D, words[warp - L::kWidenWarp]);
+            ptx::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(full + ring.stage);
+            ring.advance(1);
           }
+          n += tiles;
         }
       }
-    } else if (warp > L::kMmaWarp) {
+    } else if (!MAPS && warp >= L::kLoadWarp) {
       // ------------------------------------------------------------- loads by threads
-      const int loader = warp - L::kMmaWarp - 1;
+      const int loader = warp - L::kLoadWarp;
       bool ok = true;
-      int st = 0, n = 0;                              // stage; tiles so far
-      uint32_t ph = 0;
+      int n = 0;
       for (; walk.left > 0 && ok; walk.next(p)) {
         const int count = walk.count(), tokens = walk.w.tokens;
         const int leader = paged::ld_index(p.x.order + walk.w.first);
         const bool named = leader >= 0 && leader < p.x.B;
         const int32_t* line = p.c.table + (named ? leader : 0) * p.c.table_stride;
-        int page[4], row[4];                          // of keys lane, lane + 32, .. of the tile: page (-1: none), row
+        int page[4], row[4];                          // of keys lane, lane + 32, .. of a tile: page (-1: none), row
         auto find = [&](int tile) {
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
@@ -412,221 +484,256 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
             }
           }
         };
-        find(walk.tile);
+        find(walk.tile(0, 0));
         for (int j = 0; j < count && ok; ++j) {
-          uint32_t words[4];
-          int64_t k_row[4], v_row[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const bool exists = static_cast<unsigned>(page[u]) < static_cast<unsigned>(p.c.num_pages);
-            words[u] = __ballot_sync(0xffffffffu, exists);
-            k_row[u] = exists ? page[u] * p.c.k.page + row[u] * p.c.k.row : -1;
-            v_row[u] = exists ? page[u] * p.c.v.page + row[u] * p.c.v.row : -1;
-          }
-          if (j + 1 < count) find(walk.tile + j + 1);
-          if (loader == 0 && lane == 0) there[n % L::kSlots] = make_uint4(words[0], words[1], words[2], words[3]);
-          ++n;
+          const int tiles = walk.paired || !walk.has(j, 1) ? 1 : 2;
 #pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv) {
-            if (!ptx::mbar_wait(empty + st, ph ^ 1u)) {
-              timed_out(p.status, 90);
+          for (int i = 0; i < 2 * tiles; ++i) {       // K of the step's tiles, then V
+            const int kv = i >= tiles, s = kv ? i - tiles : i;
+            const int64_t page_step = kv ? p.c.v.page : p.c.k.page, row_step = kv ? p.c.v.row : p.c.k.row;
+            const char* const src = kv ? p.c.v.base + walk.h * p.c.v.head : p.c.k.base + walk.h * p.c.k.head;
+            uint32_t words[4];
+            int64_t at[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const bool exists = static_cast<unsigned>(page[u]) < static_cast<unsigned>(p.c.num_pages);
+              words[u] = __ballot_sync(0xffffffffu, exists);
+              at[u] = exists ? page[u] * page_step + row[u] * row_step : -1;
+            }
+            if (i + 1 < 2 * tiles) find(walk.tile(j, i + 1 >= tiles ? i + 1 - tiles : i + 1));
+            else if (j + 1 < count) find(walk.tile(j + 1, 0));
+            if (!kv && loader == 0 && lane == 0) there[(n + s) % L::kSlots] = make_uint4(words[0], words[1], words[2], words[3]);
+            if (!wait(empty + ring.stage, ring.phase ^ 1u, p.status, 90)) {
               ok = false;
               break;
             }
-            const uint32_t dst = ptx::smem_u32(ring + st * L::kTileBytes);
-            const char* const src = kv == 0 ? p.c.k.base + walk.h * p.c.k.head : p.c.v.base + walk.h * p.c.v.head;
-            if constexpr (!CODES) {
-              constexpr int kLanes = DPAD / 8, kRowsAtOnce = 32 / kLanes;      // lanes to a row
-              const int c = lane % kLanes;
+            const uint32_t dst = ptx::smem_u32(ring_at + ring.stage * L::kTileBytes);
+            constexpr int kLanes = DPAD / (CODES ? 16 : 8), kRowsAtOnce = 32 / kLanes;      // lanes to a row
+            const int c = lane % kLanes;
 #pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                for (int r0 = loader * kRowsAtOnce; r0 < 32; r0 += kLoadWarps * kRowsAtOnce) {
-                  const int r = r0 + lane / kLanes;
-                  const int64_t off = __shfl_sync(0xffffffffu, kv == 0 ? k_row[u] : v_row[u], r);
-                  if (c * 8 < p.c.D) copy16(dst + tile_at(u * 32 + r, c), src + (off < 0 ? 0 : off) + c * 16, off < 0 ? 0 : 16);
-                }
-              }
-              arrive_with_copies(full + st);
-            } else {
-              constexpr int kLanes = DPAD / 16, kRowsAtOnce = 32 / kLanes;
-              const int c = lane % kLanes;
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                for (int r0 = loader * kRowsAtOnce; r0 < 32; r0 += kLoadWarps * kRowsAtOnce) {
-                  const int r = r0 + lane / kLanes;
-                  const int64_t off = __shfl_sync(0xffffffffu, kv == 0 ? k_row[u] : v_row[u], r);
+            for (int u = 0; u < 4; ++u) {
+              for (int r0 = loader * kRowsAtOnce; r0 < 32; r0 += L::kLoadWarps * kRowsAtOnce) {
+                const int r = r0 + lane / kLanes;
+                const int64_t off = __shfl_sync(0xffffffffu, at[u], r);
+                if constexpr (CODES) {
                   if (c * 16 < p.c.D) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
+                    uint4 v = make_uint4(0, 0, 0, 0), a, b;
                     if (off >= 0) v = ld_128(src + off + c * 16);
-                    uint4 a, b;
                     widen(v.x, a.x, a.y), widen(v.y, a.z, a.w), widen(v.z, b.x, b.y), widen(v.w, b.z, b.w);
                     sts128(dst + tile_at(u * 32 + r, 2 * c), a);
                     sts128(dst + tile_at(u * 32 + r, 2 * c + 1), b);
                   }
+                } else {
+                  if (c * 8 < p.c.D) copy16(dst + tile_at(u * 32 + r, c), src + (off < 0 ? 0 : off) + c * 16, off < 0 ? 0 : 16);
                 }
               }
-              ptx::fence_proxy_async();
-              ptx::mbar_arrive(full + st);
             }
-            if (loader == 0 && lane == 0) ptx::mbar_arrive(full + st);       // behind the mask
-            if (++st == L::kStages) st = 0, ph ^= 1u;
+            if constexpr (CODES) {
+              ptx::fence_proxy_async();
+              ptx::mbar_arrive(full + ring.stage);
+            } else {
+              arrive_with_copies(full + ring.stage);
+            }
+            if (loader == 0 && lane == 0) ptx::mbar_arrive(full + ring.stage);       // behind the mask
+            ring.advance(1);
           }
+          n += tiles;
         }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");       // no copy may be under way when the CTA ends
-    } else {
+    } else if (warp == L::kMmaWarp) {
       // ------------------------------------------------------------- products
+      // The warp walks the loop together, so that barriers, phases and descriptors stay in uniform registers; one lane issues.
       constexpr int kFormat = kHalf ? 0 : 1;
       const uint32_t id_s = idesc_16(kFormat, 128, kPrefixKeys, 0), id_o = idesc_16(kFormat, 128, p.c.D, 1);
       const int steps = p.c.D / 16;
       // V as the second operand: rows of 64 elements of D, 8 keys to 1024 bytes, the next 64 elements a box further on
       constexpr uint32_t kHiV = (1024u >> 4) | (1u << 14) | (2u << 29);
       constexpr uint32_t kLeadV = (L::kBoxBytes >> 4) << 16;
-      const uint32_t ring_lo = (ptx::smem_u32(ring) >> 4) & 0x3fffu, q_lo = ptx::desc_lo_sw128(ptx::smem_u32(sq));
-      const bool leader = elect_one();
+      const uint32_t ring_lo = (ptx::smem_u32(ring_at) >> 4) & 0x3fffu, q_lo = ptx::desc_lo_sw128(ptx::smem_u32(sq));
+      const bool leader = elect_one(), paired = walk.paired;
       bool ok = true;
-      uint32_t p_phase = 0, q_phase = 0;
-      int stage = 0, v_stage = 0;                                    // of this tile's K; of the V of the tile before
-      uint32_t phase = 0, v_phase = 0;
+      uint32_t p_phase[2] = {}, q_phase[2] = {};
       const bool any = walk.left > 0;
       for (; walk.left > 0 && ok; walk.next(p)) {
         const int count = walk.count();
-        if (!ptx::mbar_wait(q_full, q_phase)) ok = false;
-        q_phase ^= 1u;
+        bool waiting[2] = {}, begun[2] = {};                         // a P that is to be multiplied; O holds something
+        Ring v_at[2] = {ring, ring};                                 // its V
         for (int j = 0; j <= count && ok; ++j) {
           const bool more = j < count;
-          if (more) ok = ptx::mbar_wait(full + stage, phase);
-          if (j > 0) ok = ok && ptx::mbar_wait(full + v_stage, v_phase);
-          if (!ok) break;
-          ptx::fence_proxy_async();                    // rows written by asynchronous copies of threads, read by the tensor cores
-          ptx::tc_fence_after();
-          const uint32_t v_lo = (ring_lo + v_stage * (L::kTileBytes >> 4)) | kLeadV, k_lo = (ring_lo + stage * (L::kTileBytes >> 4)) | (1u << 16);
-          if (j > 0) {
-            // the first half of the keys as soon as it is there
+          const bool two = more && walk.has(j, 1);
+          Ring k_at[2] = {ring, ring}, v_next[2] = {ring, ring};
+          if (paired) {
+            v_next[0].advance(1);
+            v_next[1] = v_next[0];
+          } else {
+            k_at[1].advance(1);
+            v_next[0].advance(two ? 2 : 1);
+            v_next[1] = v_next[0];
+            v_next[1].advance(1);
+          }
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              ok = ok && ptx::mbar_wait(half == 0 ? p_half : p_full, p_phase);
+          for (int s = 0; s < 2; ++s) {
+            if (waiting[s]) {
+              ok = ok && wait(full + v_at[s].stage, v_at[s].phase, p.status, 93);
+              ptx::fence_proxy_async();                // rows that threads have written, read by the tensor cores
+              const uint32_t v_lo = (ring_lo + v_at[s].stage * (L::kTileBytes >> 4)) | kLeadV;
+              // the first half of the keys as soon as it is there
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                ok = ok && wait((half == 0 ? p_half : p_full) + s, p_phase[s], p.status, 94);
+                ptx::tc_fence_after();
+                if (leader && ok) {
+#pragma unroll
+                  for (int k = 0; k < kPrefixKeys / 32; ++k)
+                    mma_ts(tmem + (2 + s) * 128, tmem + s * 128 + half * 32 + k * 8, ptx::desc_join(v_lo + (half * 4 + k) * (2048 >> 4), kHiV), id_o,
+                           half > 0 || k > 0 ? 1u : (begun[s] ? 1u : 0u));
+                }
+                __syncwarp();
+              }
+              p_phase[s] ^= 1u;
+              begun[s] = true;
+              waiting[s] = false;
+              if (leader && ok && (!paired || s == 1 || !walk.has(0, 1))) ptx::tc_commit<1>(empty + v_at[s].stage);
+            }
+            if (!more && begun[s] && leader && ok) ptx::tc_commit<1>(o_full + s);
+            __syncwarp();
+            if (more && (s == 0 || two) && ok) {
+              if (j == 0 && (s == 0 || paired)) {
+                ok = wait(q_full + s, q_phase[s], p.status, 95);
+                q_phase[s] ^= 1u;
+              }
+              ok = ok && wait(full + k_at[s].stage, k_at[s].phase, p.status, 93);
+              ptx::fence_proxy_async();
               ptx::tc_fence_after();
               if (leader && ok) {
+                const uint32_t k_lo = (ring_lo + k_at[s].stage * (L::kTileBytes >> 4)) | (1u << 16), mine = q_lo + (paired ? s * (L::kTileBytes >> 4) : 0);
 #pragma unroll
-                for (int k = 0; k < kPrefixKeys / 32; ++k)
-                  mma_ts(tmem + 128, tmem + half * 32 + k * 8, ptx::desc_join(v_lo + (half * 4 + k) * (2048 >> 4), kHiV), id_o, half > 0 || k > 0 || j > 1 ? 1u : 0u);
+                for (int k = 0; k < DPAD / 16; ++k) {
+                  const uint32_t at = ((k >> 2) * L::kBoxBytes + (k & 3) * 32) >> 4;
+                  if (k < steps) mma_ss(tmem + s * 128, ptx::desc_join(mine + at, ptx::kDescHiSw128), ptx::desc_join(k_lo + at, ptx::kDescHiSw128), id_s, k > 0);
+                }
+                ptx::tc_commit<1>(s_full + s);
+                ptx::mbar_arrive(s_full + s);          // the mask of the tile goes along
+                if (!paired || s == 1 || !two) ptx::tc_commit<1>(empty + k_at[s].stage);
               }
               __syncwarp();
+              waiting[s] = true;
+              v_at[s] = v_next[s];
             }
-            p_phase ^= 1u;
-            if (!more && leader) ptx::tc_commit<1>(o_full);
-            __syncwarp();
           }
-          if (more && ok) {
-            if (leader) {
-#pragma unroll
-              for (int k = 0; k < DPAD / 16; ++k) {
-                const uint32_t at = ((k >> 2) * L::kBoxBytes + (k & 3) * 32) >> 4;
-                if (k < steps) mma_ss(tmem, ptx::desc_join(q_lo + at, ptx::kDescHiSw128), ptx::desc_join(k_lo + at, ptx::kDescHiSw128), id_s, k > 0);
-              }
-              ptx::tc_commit<1>(s_full);
-              ptx::mbar_arrive(s_full);                // the mask of the tile goes along
-            }
-            __syncwarp();
-          }
-          if (!ok) break;
-          if (leader) {
-            if (j > 0) ptx::tc_commit<1>(empty + v_stage);
-            if (more) ptx::tc_commit<1>(empty + stage);
-          }
-          __syncwarp();
-          if (more) {
-            v_stage = stage + 1, v_phase = phase;
-            if (v_stage == L::kStages) v_stage = 0, v_phase ^= 1u;
-            stage = v_stage + 1, phase = v_phase;
-            if (stage == L::kStages) stage = 0, phase ^= 1u;
-          }
+          if (more) ring.advance(paired ? 2 : (two ? 4 : 2));
         }
-        if (!ok) timed_out(p.status, 94);
       }
       if (any) {
         if (leader) ptx::tc_commit<1>(done);
         __syncwarp();
-        if (!ptx::mbar_wait(done, 0)) timed_out(p.status, 95);
+        wait(done, 0, p.status, 98);
       }
     }
   } else {
-    // ------------------------------------------------------------- softmax, one thread to a row
+    // ------------------------------------------------------------- softmax of tile s, one thread to a row
     ptx::setmaxnreg_inc<L::kSoftmaxRegs>();
-    const int r = threadIdx.x;
-    const uint32_t lanes = static_cast<uint32_t>(warp) << 21;         // this warp's 32 lanes of tensor memory
-    const uint32_t ts = tmem + lanes, to = tmem + 128 + lanes;
+    const int s = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;     // this warp's 32 lanes of tensor memory
+    const uint32_t ts = tmem + s * 128 + lanes, to = tmem + (2 + s) * 128 + lanes;
     bool ok = true;
     uint32_t phase = 0, o_phase = 0;
-    int n = 0;
-    for (; walk.left > 0 && ok; walk.next(p)) {
+    int n = 0;                                         // tiles loaded so far
+    // The first pass is dry: it waits for nothing, writes nothing and fetches the code below from memory, which takes longer than a tile, under the sums
+    // of the line and the kernel in front.
+    bool dry = p.x.heads > 0;
+    Walk walk{};
+    walk.left = walk.steps = 1, walk.w.tiles = 128;
+    while (walk.left > 0 && ok) {
       const int count = walk.count();
-      // the row's query: products with those of the item before have ended (its last scores are here)
-      const int at = walk.row_tile * kPrefixRows + r, place = at / p.x.group;
+      const int64_t half = 2 * (walk.item + cta) + s;
+      const bool keeps = r < p.x.rows && (half >> 1) < p.x.slots;
+      bool mine = false;
+      float sl = p.scale * 1.4426950408889634f;
+      if (!dry) {
+      if (!walk.has(0, s)) {                           // no row (which nobody asks for), or no second tile of keys in this part
+        if (keeps && !walk.paired) p.x.stats[half * p.x.rows + r] = make_float2(-INFINITY, -1.0f);
+        n += walk.loaded(count);
+        walk.next(p);
+        continue;
+      }
+      // the row's query: products with those of the item before have ended (this tile's O was complete)
+      const int at = walk.row0(s) + r, place = at / p.x.group;
       int b = -1;
       if (place < walk.w.n) b = paged::ld_index(p.x.order + walk.w.first + place);
-      const bool mine = b >= 0 && b < p.x.B && paged::cached_tokens(p.c, b, 0x7fffffff) >= walk.w.tokens;
-      float sl = p.scale * 1.4426950408889634f;
+      mine = b >= 0 && b < p.x.B && paged::cached_tokens(p.c, b, 0x7fffffff) >= walk.w.tokens;
       {
-        const char* src = p.q + (mine ? b : 0) * p.q_batch + (walk.h * p.x.group + at - place * p.x.group) * p.q_head;
-        uint4 u[DPAD / 8];
+        // a row's pieces of 16 bytes by neighbouring lanes
+        constexpr int kLanes = DPAD / 8, kRowsAtOnce = 32 / kLanes, kRounds = 32 / kRowsAtOnce, kBatch = 8;
+        const int64_t off = mine ? b * p.q_batch + (walk.h * p.x.group + at - place * p.x.group) * p.q_head : -1;
+        const int c = lane % kLanes;
+        constexpr bool kScaled = CODES && !std::is_same<T, __half>::value;
+        float back = 1.0f;
+        if constexpr (CODES) sl *= paged::head_scale(p.c.k_amax, p.c.amax_stride, walk.h);
+        const uint32_t dst = ptx::smem_u32(sq) + (walk.paired ? s * L::kTileBytes : 0);
+#pragma unroll 1
+        for (int i0 = 0; i0 < kRounds; i0 += kBatch) {
+          uint4 u[kBatch];
 #pragma unroll
-        for (int c = 0; c < DPAD / 8; ++c) {
-          u[c] = make_uint4(0, 0, 0, 0);
-          if (mine && c * 8 < p.c.D) u[c] = ld_128(src + c * 16);
-        }
-        if constexpr (CODES) {
-          sl *= paged::head_scale(p.c.k_amax, p.c.amax_stride, walk.h);
-          if constexpr (!std::is_same<T, __half>::value) {
-            uint32_t* w = &u[0].x;
-            float top = 0.0f;
+          for (int i = 0; i < kBatch; ++i) {
+            const int64_t row = __shfl_sync(0xffffffffu, off, (i0 + i) * kRowsAtOnce + lane / kLanes);
+            u[i] = make_uint4(0, 0, 0, 0);
+            if (row >= 0 && c * 8 < p.c.D) u[i] = ld_128(p.q + row + c * 16);
+          }
 #pragma unroll
-            for (int i = 0; i < DPAD / 2; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
-            // 2^(13 - exponent): the largest lands in [2^13, 2^14); zero, infinity and NaN stay as they are
-            const int e = static_cast<int>(__float_as_uint(top) >> 23);
-            float f = 1.0f;
-            if (top != 0.0f && e < 255) {
-              const int s = min(140 - max(e, 1), 124);
-              f = __uint_as_float(static_cast<uint32_t>(max(s, -125) + 127) << 23);
+          for (int i = 0; i < kBatch; ++i) {
+            if constexpr (kScaled) {
+              uint32_t* w = &u[i].x;
+              float top = 0.0f;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u))));
+#pragma unroll
+              for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+              // 2^(13 - exponent): the largest lands in [2^13, 2^14); zero, infinity and NaN stay as they are
+              const int e = static_cast<int>(__float_as_uint(top) >> 23), up = min(max(140 - max(e, 1), -125), 124);
+              const float f = top != 0.0f && e < 255 ? __uint_as_float(static_cast<uint32_t>(up + 127) << 23) : 1.0f;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[k] = pack16<__half>(__uint_as_float(w[k] << 16) * f, __uint_as_float(w[k] & 0xffff0000u) * f);
+              const float of = __shfl_sync(0xffffffffu, f, lane % kRowsAtOnce * kLanes);     // this lane's row is one of round lane / kRowsAtOnce
+              if (lane / kRowsAtOnce == i0 + i) back = of;
             }
-            sl *= 1.0f / f;
-#pragma unroll
-            for (int i = 0; i < DPAD / 2; ++i) w[i] = pack16<__half>(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
+            // not paired: the second tile has the same rows as the first
+            if (s == 0 || walk.paired) sts128(dst + tile_at((warp & 3) * 32 + (i0 + i) * kRowsAtOnce + lane / kLanes, c), u[i]);
           }
         }
-        const uint32_t dst = ptx::smem_u32(sq);
-#pragma unroll
-        for (int c = 0; c < DPAD / 8; ++c) sts128(dst + tile_at(r, c), u[c]);
+        if constexpr (kScaled) sl *= 1.0f / back;
+        if (s == 0 || walk.paired) {
+          ptx::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(q_full + s);
+        }
       }
-      ptx::fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(q_full);
-      sl = fmaxf(sl, 1e-30f);                                         // 0 times a masked -inf would be NaN
-      const bool works = __any_sync(0xffffffffu, mine);
+      }
+      sl = fmaxf(sl, 1e-30f);                          // 0 times a masked -inf would be NaN
+      const bool works = dry || __any_sync(0xffffffffu, mine);
       const uint64_t sl2 = pack2(sl, sl);
       float m = -INFINITY, l = 0.0f;
       bool begun = false, any = false;
       for (int j = 0; j < count && ok; ++j) {
-        ok = ptx::mbar_wait(s_full, phase);
-        if (!ok) {
-          timed_out(p.status, 96);
-          break;
+        if (!walk.has(j, s)) break;                    // the last step of an item may have one tile of keys
+        if (!dry) {
+          ok = ptx::mbar_wait(s_full + s, phase);
+          if (!ok) {
+            timed_out(p.status, 96);
+            break;
+          }
+          phase ^= 1u;
         }
-        phase ^= 1u;
         ptx::tc_fence_after();
-        const uint4 words = there[n++ % L::kSlots];
+        const uint4 words = there[(n + (walk.paired ? j : 2 * j + s)) % L::kSlots];
         any = any || (words.x | words.y | words.z | words.w) != 0;
         if (works) {
+          if (!dry && (words.x & words.y & words.z & words.w) != 0xffffffffu) mask_scores(ts, words);
           uint32_t x[kPrefixKeys];
 #pragma unroll
           for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32(ts + c * 32, x + c * 32);
           ptx::tmem_ld_wait();
-          if ((words.x & words.y & words.z & words.w) != 0xffffffffu) {
-            const uint32_t seen[4] = {words.x, words.y, words.z, words.w};
-#pragma unroll
-            for (int c = 0; c < kPrefixKeys; ++c) x[c] = seen[c / 32] & (1u << (c % 32)) ? x[c] : 0xff800000u;
-          }
           float top[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) top[c] = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[4 + c]));
@@ -650,8 +757,10 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
               ptx::tmem_ld_wait();
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              ptx::tmem_st_32x32_x16(to + c * 32, o);
-              ptx::tmem_st_32x32_x16(to + c * 32 + 16, o + 16);
+              if (!dry) {
+                ptx::tmem_st_32x32_x16(to + c * 32, o);
+                ptx::tmem_st_32x32_x16(to + c * 32 + 16, o + 16);
+              }
             }
           }
           // the difference first: logits of 2^24 and more would lose the factor
@@ -663,18 +772,24 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float2 y = unpack2(fma2(add2(pack2(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])), back2), sl2, raise2));
-              const uint64_t v = pack2(exp2_fast(y.x), exp2_fast(y.y));
+              const uint64_t y = fma2(add2(pack2(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])), back2), sl2, raise2);
+              uint64_t v;
+              if ((e + 1) * kPolyPairs / 16 != e * kPolyPairs / 16) {
+                v = ex2_poly2(y);
+              } else {
+                const float2 a = unpack2(y);
+                v = pack2(exp2_fast(a.x), exp2_fast(a.y));
+              }
               if (e & 1) sum1 = add2(sum1, v); else sum0 = add2(sum0, v);
               const float2 a = unpack2(v);
               pk[e] = pack16<E>(a.x, a.y);
             }
-            ptx::tmem_st_32x32_x16(ts + c / 2, pk);
+            if (!dry) ptx::tmem_st_32x32_x16(ts + c / 2, pk);
             if (c == 32) {
               ptx::tmem_st_wait();
               ptx::tc_fence_before();
               __syncwarp();
-              if (lane == 0) ptx::mbar_arrive(p_half);
+              if (lane == 0 && !dry) ptx::mbar_arrive(p_half + s);
             }
           }
           const float2 s0 = unpack2(sum0), s1 = unpack2(sum1);
@@ -682,36 +797,43 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
           ptx::tmem_st_wait();
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(p_full);
+          if (lane == 0 && !dry) ptx::mbar_arrive(p_full + s);
         } else if (lane == 0) {                        // rows of nobody: what their P holds reaches their own O only
-          ptx::mbar_arrive(p_half);
-          ptx::mbar_arrive(p_full);
+          ptx::mbar_arrive(p_half + s);
+          ptx::mbar_arrive(p_full + s);
         }
       }
-      if (ok && !ptx::mbar_wait(o_full, o_phase)) {
+      if (dry) {
+        found_barrier<L::kThreads>();
+        pdl_wait();
+        walk = *start;
+        dry = false;
+        continue;
+      }
+      n += walk.loaded(count);
+      if (ok && !ptx::mbar_wait(o_full + s, o_phase)) {
         timed_out(p.status, 97);
         ok = false;
       }
       o_phase ^= 1u;
       if (!ok) break;
       ptx::tc_fence_after();
-      const int64_t slot = walk.item + cta;
-      const bool keeps = r < p.x.rows && slot < p.x.slots;
-      if (keeps) p.x.stats[slot * p.x.rows + r] = make_float2(m == -INFINITY ? m : m * sl - kRaise<kHalf>, mine && any ? l : -1.0f);
+      if (keeps) p.x.stats[half * p.x.rows + r] = make_float2(m == -INFINITY ? m : m * sl - kRaise<kHalf>, mine && any ? l : -1.0f);
       if (works) {
-        float* const dst = p.x.parts + (slot * p.x.rows + r) * DPAD;
+        float* const dst = p.x.parts + (half * p.x.rows + r) * DPAD;
 #pragma unroll 1
         for (int c = 0; c < DPAD / 32; ++c) {
-          uint32_t o[32];
-          ptx::tmem_ld_32x32(to + c * 32, o);
+          U32x8 o[4];
+          ptx::tmem_ld_32x32(to + c * 32, &o[0].v[0]);
           ptx::tmem_ld_wait();
           if (keeps && mine) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(dst + c * 32 + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int e = 0; e < 4; ++e) st_256(dst + c * 32 + e * 8, o[e]);
           }
         }
       }
       ptx::tc_fence_before();                          // these reads of O in front of the next item's products
+      walk.next(p);
     }
   }
   ptx::tc_fence_before();
@@ -722,7 +844,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
   }
 }
 
-// The parts of every row together: those of its prefix, in the order of the keys, and that of its own keys.  A row has 1, 2, 4 or 8 of a CTA's warps, a
+// The parts of every row together, in the order of the keys: those of its prefix, then those of its own keys.  A row has 1, 2, 4 or 8 of a CTA's warps, a
 // share of the parts each.
 struct JoinParams {
   Cache c;
@@ -735,14 +857,21 @@ constexpr int kJoinWarps = 8;
 struct PartSum {
   float top, sum, acc[4];
   bool has;
-  __device__ __forceinline__ void add(const float2& s, const float4& v) {
-    if (s.y < 0.0f) return;
-    has = true;
-    const float now = fmaxf(top, s.x), base = now == -INFINITY ? 0.0f : now, f0 = exp2_fast(top - base), f1 = exp2_fast(s.x - base);
-    sum = sum * f0 + s.y * f1;
-    acc[0] = acc[0] * f0 + v.x * f1, acc[1] = acc[1] * f0 + v.y * f1;
-    acc[2] = acc[2] * f0 + v.z * f1, acc[3] = acc[3] * f0 + v.w * f1;
-    top = now;
+  template <int N>
+  __device__ __forceinline__ void add(const float2 (&s)[N], const float4 (&v)[N]) {
+    float now = top;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (!(s[k].y < 0.0f)) now = fmaxf(now, s[k].x), has = true;
+    const float base = now == -INFINITY ? 0.0f : now, f0 = exp2_fast(top - base);
+    sum *= f0, acc[0] *= f0, acc[1] *= f0, acc[2] *= f0, acc[3] *= f0, top = now;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if (s[k].y < 0.0f) continue;
+      const float f = exp2_fast(s[k].x - base);
+      sum += s[k].y * f;
+      acc[0] += v[k].x * f, acc[1] += v[k].y * f, acc[2] += v[k].z * f, acc[3] += v[k].w * f;
+    }
   }
 };
 
@@ -759,38 +888,50 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
   pdl_wait();
   PartSum a{-INFINITY, 0.0f, {}, false};
   if (there) {
-    const int g = paged::ld_index(p.x.group_of + b), place = paged::ld_index(p.x.place_of + b);
-    const bool grouped = paged::prefix_tokens(p.x, b, paged::cached_tokens(p.c, b, 0x7fffffff)) > 0 && g >= 0 && g < p.x.groups;
-    const GroupWork w = grouped ? paged::group_work(p.x, p.c, g) : GroupWork{};
-    if (grouped && w.tiles > 0 && place >= 0 && place < w.n) {
-      const int64_t total = __ldcg(p.x.lines + 2 * p.x.groups);
-      const int ctas = static_cast<int>(__ldcg(p.x.lines + 2 * p.x.groups + 1));
-      const int row = place * p.x.group + hq - h * p.x.group, tile = row / kPrefixRows, r = row % kPrefixRows;
-      const int64_t items = static_cast<int64_t>(h) * w.row_tiles + tile, start = __ldcg(p.x.lines + 2 * g) + items * w.tiles;
-      const int64_t slot0 = __ldcg(p.x.lines + 2 * g + 1) + items;
-      const int c0 = holder(total, start, ctas), c1 = holder(total, start + w.tiles - 1, ctas);
-      const int parts = c1 - c0 + 1, from = c0 + (parts * share >> share_log2), to = c0 + (parts * (share + 1) >> share_log2);
-      constexpr int kAtOnce = 8;
-#pragma unroll 1
-      for (int c = from; c < to; c += kAtOnce) {
-        float2 s[kAtOnce];
-        float4 v[kAtOnce];
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {            // the loads first: they do not wait for one another
-          s[k].y = -1.0f;
-          const int64_t slot = slot0 + c + k;
-          if (c + k >= to || r >= p.x.rows || slot >= p.x.slots) continue;
-          s[k] = __ldcg(p.x.stats + slot * p.x.rows + r);
-          if (d < DPAD) v[k] = __ldcg(reinterpret_cast<const float4*>(p.x.parts + (slot * p.x.rows + r) * DPAD + d));
-        }
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) a.add(s[k], v[k]);
+    const int head = hq - h * p.x.group, g = paged::ld_index(p.x.group_of + b), place = paged::ld_index(p.x.place_of + b);
+    const int held = paged::cached_tokens(p.c, b, 0x7fffffff), shared = paged::prefix_tokens(p.x, b, held);
+    // its own keys: tiles of 64
+    const int64_t own_total = __ldcg(p.x.own_lines + p.B), own_ctas = __ldcg(p.x.own_lines + p.B + 1);
+    const int own_tiles = held > shared ? (held - shared + 63) / 64 : 1, own_block = head / p.x.own_rows;
+    const int64_t own_start = __ldcg(p.x.own_lines + b) + (static_cast<int64_t>(h) * p.x.own_blocks + own_block) * own_tiles;
+    const int o0 = holder(own_total, own_start, static_cast<int>(own_ctas)), o1 = holder(own_total, own_start + own_tiles - 1, static_cast<int>(own_ctas));
+    const int64_t own_at = ((static_cast<int64_t>(b) * p.c.heads + h) * p.x.own_blocks + own_block + o0) * p.x.own_rows + head - own_block * p.x.own_rows;
+    // its prefix: of each part the half that holds the row, or (not paired) both
+    int parts = 0, log2 = 0;
+    int64_t at = 0, slots = 0;                         // the first, in rows; slots that there are from there on
+    if (shared > 0 && g >= 0 && g < p.x.groups) {
+      const GroupWork w = paged::group_work(p.x, p.c, g);
+      const int64_t* const end = p.x.lines + 2 * p.x.groups;
+      const int64_t total = __ldcg(end), ctas = __ldcg(end + 1);
+      const bool paired = __ldcg(end + 2) != 0;
+      const int row = place * p.x.group + head, block = row >> (paired ? 8 : 7), r = row & 127, steps = w.steps(paired);
+      if (w.tiles > 0 && place >= 0 && place < w.n && r < p.x.rows && total > 0) {
+        const int64_t item = static_cast<int64_t>(h) * w.blocks(paired) + block;
+        const int64_t start = __ldcg(p.x.lines + 2 * g) + item * (steps + paged::kItemSteps) + paged::kItemSteps;
+        const int c0 = holder(total, start, static_cast<int>(ctas)), c1 = holder(total, start + steps - 1, static_cast<int>(ctas));
+        const int64_t slot = __ldcg(p.x.lines + 2 * g + 1) + item + c0;
+        log2 = paired ? 0 : 1;
+        parts = (c1 - c0 + 1) << log2;
+        at = (2 * slot + (paired ? (row >> 7) & 1 : 0)) * p.x.rows + r;
+        slots = p.x.slots - slot;
       }
     }
-    if (share == (1 << share_log2) - 1) {              // behind the prefix
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (d < DPAD) v = __ldcg(reinterpret_cast<const float4*>(p.x.own + id * DPAD + d));
-      a.add(__ldcg(p.x.own_stats + id), v);
+    const int all = parts + o1 - o0 + 1, from = all * share >> share_log2, to = all * (share + 1) >> share_log2;
+    constexpr int kAtOnce = 8;
+#pragma unroll 1
+    for (int i = from; i < to; i += kAtOnce) {
+      float2 s[kAtOnce];
+      float4 v[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {              // the loads first: they do not wait for one another
+        s[k].y = -1.0f;
+        const int n = i + k;
+        if (n >= to || (n < parts && n >> log2 >= slots)) continue;
+        const int64_t of = n < parts ? at + static_cast<int64_t>(log2 ? n : 2 * n) * p.x.rows : own_at + static_cast<int64_t>(n - parts) * p.x.own_rows;
+        s[k] = __ldcg((n < parts ? p.x.stats : p.x.own_stats) + of);
+        if (d < DPAD) v[k] = __ldcg(reinterpret_cast<const float4*>((n < parts ? p.x.parts : p.x.own) + of * DPAD + d));
+      }
+      a.add(s, v);
     }
   }
   if (share_log2 > 0) {
@@ -798,7 +939,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
     if (lane == 0) stats_of[warp] = make_float2(a.top, a.has ? a.sum : -1.0f);
     __syncthreads();
     if (share > 0) return;
-    for (int k = 1; k < 1 << share_log2; ++k) a.add(stats_of[warp + k], acc_of[warp + k][lane]);
+#pragma unroll 1
+    for (int k = 1; k < 1 << share_log2; ++k) {
+      const float2 s[1] = {stats_of[warp + k]};
+      const float4 v[1] = {acc_of[warp + k][lane]};
+      a.add(s, v);
+    }
   }
   if (!there || d >= p.c.D) return;
   uint2 u = make_uint2(0, 0);
@@ -830,7 +976,7 @@ bool make_map(CUtensorMap* map, const paged::Pool& pool, const Cache& c, int dty
 
 template <typename T, bool CODES, int DPAD, bool MAPS>
 int launch_prefix(const CUtensorMap& tk, const CUtensorMap& tv, const PrefixParams& p, cudaStream_t st) {
-  using L = Layout<DPAD>;
+  using L = Layout<DPAD, CODES>;
   auto kernel = prefix_kernel<T, CODES, DPAD, MAPS>;
   static std::atomic<bool> ready[64];
   int dev = 0;
@@ -839,7 +985,7 @@ int launch_prefix(const CUtensorMap& tk, const CUtensorMap& tv, const PrefixPara
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess) return B200Q_ERR_CUDA;
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
   }
-  const int ctas = kPerSm * sm_count() < kMostCtas ? kPerSm * sm_count() : kMostCtas;
+  const int ctas = sm_count() < kMostCtas ? sm_count() : kMostCtas;
   if (launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(L::kThreads), L::kSmem, st, tk, tv, p) != cudaSuccess) return B200Q_ERR_CUDA;
   return check_launch();
 }
@@ -859,7 +1005,8 @@ int launch_join(const JoinParams& p, cudaStream_t st) {
 
 // Parts of a call, at most, and the rows of each: all of its CTAs' and all items.
 struct Sizes {
-  int64_t rows, slots, parts, stats, lines, own, own_stats, bytes;
+  int64_t rows, slots, parts, stats, lines, own, own_stats, own_lines, bytes;
+  int own_rows, own_blocks;
 };
 bool sizes_of(int64_t B, int64_t Hq, int64_t heads, int64_t D, int64_t groups, int64_t largest, Sizes* s) {
   if (B <= 0 || Hq <= 0 || heads <= 0 || Hq % heads != 0 || D <= 0 || D > paged::kMaxD || groups < 0 || groups > B || largest < 0 || largest > B ||
@@ -871,12 +1018,15 @@ bool sizes_of(int64_t B, int64_t Hq, int64_t heads, int64_t D, int64_t groups, i
   const int64_t most = groups * ((largest * group + kPrefixRows - 1) / kPrefixRows), all = B * group / kPrefixRows + groups;
   s->slots = heads * (most < all ? most : all) + kMostCtas;
   const auto round = [](int64_t n) { return (n + 255) / 256 * 256; };
-  s->lines = round((2 * groups + 2) * 8);
-  s->stats = round(s->slots * s->rows * 8);
-  s->own_stats = round(B * Hq * 8);
-  s->own = round(B * Hq * up * 4);
-  s->parts = round(s->slots * s->rows * up * 4);
-  s->bytes = s->lines + s->stats + s->own_stats + s->own + s->parts;
+  s->lines = round((2 * groups + 3) * 8);
+  s->stats = round(2 * s->slots * s->rows * 8);
+  int64_t own_slots;
+  paged::own_shape(B, Hq, heads, &s->own_rows, &s->own_blocks, &own_slots);
+  s->own_lines = round((B + 2) * 8);
+  s->own_stats = round(own_slots * s->own_rows * 8);
+  s->own = round(own_slots * s->own_rows * up * 4);
+  s->parts = round(2 * s->slots * s->rows * up * 4);
+  s->bytes = s->lines + s->stats + s->own_lines + s->own_stats + s->own + s->parts;
   return true;
 }
 
@@ -947,6 +1097,8 @@ int b200q_shared_prefix_attention(const void* q, int dtype, const int64_t* q_str
                static_cast<int>(largest), p.c.heads, static_cast<int>(Hq / p.c.heads), static_cast<int>(s.rows), s.slots};
   p.x.lines = reinterpret_cast<int64_t*>(take(s.lines));
   p.x.stats = reinterpret_cast<float2*>(take(s.stats));
+  p.x.own_rows = s.own_rows, p.x.own_blocks = s.own_blocks;
+  p.x.own_lines = reinterpret_cast<int64_t*>(take(s.own_lines));
   p.x.own_stats = reinterpret_cast<float2*>(take(s.own_stats));
   p.x.own = reinterpret_cast<float*>(take(s.own));
   p.x.parts = reinterpret_cast<float*>(take(s.parts));
