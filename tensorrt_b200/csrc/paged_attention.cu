@@ -154,7 +154,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 struct Seen {
   int seen, sinks, gap;
   __device__ __forceinline__ int token(int i) const { return i < sinks ? i : i + gap; }
-  __device__ __forceinline__ int tiles() const { return seen > 0 ? (seen + kTile - 1) / kTile : 1; }   // 1: somebody writes the zeros
+  // JOIN: tiles of one warp
+  template <bool JOIN>
+  __device__ __forceinline__ int tiles() const {
+    constexpr int kOf = JOIN ? kKeys : kTile;
+    return seen > 0 ? (seen + kOf - 1) / kOf : 1;                        // 1: somebody writes the zeros
+  }
 };
 template <bool JOIN>
 __device__ __forceinline__ Seen keys_seen(const DecodeParams& p, int b) {
@@ -188,8 +193,9 @@ struct Stage {
 template <bool JOIN>
 __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, int* ctas, int* b_out, int64_t* before_out, Seen* seen_out) {
   __shared__ int64_t sums[kWarps];
-  __shared__ int64_t found[2];
-  __shared__ Seen found_keys;
+  constexpr int kWants = JOIN ? kWarps : 1;          // pieces of a CTA
+  __shared__ int64_t found[kWants][2];
+  __shared__ Seen found_keys[kWants];
   Seen keys{0, 0, 0};
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t per = static_cast<int64_t>(p.c.heads) * p.blocks;
@@ -215,7 +221,7 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
   };
   for (int base = 0; base < p.B; base += kThreads) {
     if (base + tid < p.B) keys = keys_seen<JOIN>(p, base + tid);
-    mine = base + tid < p.B ? keys.tiles() * per : 0;
+    mine = base + tid < p.B ? (keys.tiles<JOIN>() + (JOIN ? paged::kOwnItemTiles : 0)) * per : 0;
     const int64_t before = total;
     total += scan(mine);
     if constexpr (JOIN) {
@@ -226,34 +232,43 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
   if constexpr (JOIN) {
     if (cta == 0 && tid == 0) p.x.own_lines[p.B] = total, p.x.own_lines[p.B + 1] = *ctas;
   }
-  if (cta >= *ctas) return total;
-  const int64_t want = piece(total, cta, *ctas);
+  if (cta * kWants >= *ctas) return total;
+  auto look = [&](int at, int64_t begin) {           // whether a piece begins in sequence `at`, whose tiles begin there
+#pragma unroll
+    for (int w = 0; w < kWants; ++w) {
+      if (cta * kWants + w >= *ctas) break;
+      const int64_t want = piece(total, cta * kWants + w, *ctas);
+      if (want >= begin && want < begin + mine) found[w][0] = at, found[w][1] = begin, found_keys[w] = keys;
+    }
+  };
+  const int64_t last = piece(total, min(cta * kWants + kWants, *ctas) - 1, *ctas);
   if (p.B <= kThreads) {
-    if (want >= inclusive - mine && want < inclusive) found[0] = tid, found[1] = inclusive - mine, found_keys = keys;
+    look(tid, inclusive - mine);
     __syncthreads();
   } else {
     int64_t before = 0;
     for (int base = 0; base < p.B; base += kThreads) {
       if (base + tid < p.B) keys = keys_seen<JOIN>(p, base + tid);
-      mine = base + tid < p.B ? keys.tiles() * per : 0;
+      mine = base + tid < p.B ? (keys.tiles<JOIN>() + (JOIN ? paged::kOwnItemTiles : 0)) * per : 0;
       const int64_t all = scan(mine);
-      if (want >= before + inclusive - mine && want < before + inclusive)
-        found[0] = base + tid, found[1] = before + inclusive - mine, found_keys = keys;
+      look(base + tid, before + inclusive - mine);
       before += all;
-      if (before > want) break;
+      if (before > last) break;
     }
     __syncthreads();
   }
-  *b_out = static_cast<int>(found[0]);
-  *before_out = found[1];
-  *seen_out = found_keys;
+  const int w = JOIN ? warp : 0;
+  *b_out = static_cast<int>(found[w][0]);
+  *before_out = found[w][1];
+  *seen_out = found_keys[w];
   return total;
 }
 
 // BLOCKS8: query heads of an item in blocks of 8.  JOIN: behind the kernel of shared prefixes, over the keys that a sequence has to itself; the result
 // is a part of each row, as that kernel's are.  It reads nothing of that kernel, which lets it start only once everything in front has
-// completed: it waits at its end, so that it has ended only when the one in front has.  Parts are joined by the kernel behind, not here: with many short
-// sequences the exchange among CTAs was most of the time.
+// completed: it waits at its end, so that it has ended only when the one in front has.  Here a warp takes a piece of the line by itself, in tiles of 16 keys,
+// and the kernel behind joins: these keys are few for every sequence, and what ends an item would be most of the time (100 sequences of 14 to 310 keys,
+// 12 / 12 heads of 80: @@).
 template <typename T, bool CODES, int DPAD, int BLOCKS8, bool JOIN>
 __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm) decode_kernel(const __grid_constant__ DecodeParams p) {
   using S = Stage<CODES, DPAD, BLOCKS8>;
@@ -265,8 +280,8 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
   __shared__ uint32_t there[kWarps][S::kDepth];        // which of the 16 keys of a stage exist
   __shared__ int last_one;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int cta = blockIdx.x;
-  int ctas = gridDim.x;
+  const int cta = JOIN ? blockIdx.x * kWarps + warp : blockIdx.x;       // JOIN: every warp by itself
+  int ctas = JOIN ? gridDim.x * kWarps : gridDim.x;
   char* const ring = smem + warp * S::kDepth * S::kBytes;
   const uint32_t ring_u32 = smem_u32(ring);
   pdl_launch_dependents();
@@ -275,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
   int b;
   int64_t before;
   Seen see;
-  const int64_t total = find_start<JOIN>(p, cta, &ctas, &b, &before, &see);
+  const int64_t total = find_start<JOIN>(p, static_cast<int>(blockIdx.x), &ctas, &b, &before, &see);
   if (cta >= ctas) {
     if constexpr (JOIN) pdl_wait();
     return;
@@ -283,11 +298,16 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
   int64_t at = piece(total, cta, ctas);
   const int64_t first_tile = at, end = piece(total, cta + 1, ctas);
   // the item: kv head and block of query heads, within sequence b
-  int64_t item = divide(at - before, see.tiles());
+  constexpr int kFront = JOIN ? paged::kOwnItemTiles : 0;               // room in front of an item's tiles
+  int64_t item = divide(at - before, see.tiles<JOIN>() + kFront);
   int h = static_cast<int>(divide(item, p.blocks)), block = static_cast<int>(item) - h * p.blocks;
-  int64_t item_start = before + item * see.tiles();
+  int64_t item_start = before + item * (see.tiles<JOIN>() + kFront) + kFront;
   while (at < end) {
-    const int tiles = see.tiles();
+    if constexpr (JOIN) {
+      if (at < item_start) at = item_start;
+      if (at >= end) break;
+    }
+    const int tiles = see.tiles<JOIN>();
     const int64_t item_end = item_start + tiles;
     const int tile0 = static_cast<int>(at - item_start), tile1 = static_cast<int>((end < item_end ? end : item_end) - item_start);
     const int head0 = h * p.group + block * p.rows, rows = min(p.rows, p.group - block * p.rows);
@@ -298,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
     // ------------------------------------------------------------- copies of a warp's 16 keys of a tile
     // lane: of key lane % 16, its page (-1: none) and its row within it
     auto find_page = [&](int tile) {
-      const int i = tile * kTile + warp * kKeys + (lane & 15);
+      const int i = (JOIN ? tile * kKeys : tile * kTile + warp * kKeys) + (lane & 15);
       int page = -1, row = 0;
       if (tile < tile1 && i < see.seen) {
         const int token = see.token(i), n = p.page_shift >= 0 ? token >> p.page_shift : token / p.c.page_size;
@@ -505,6 +525,24 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
       __syncwarp();
     }
 
+    if constexpr (JOIN) {
+      // ----------------------------------------------------------- the warp's part: 8 elements of a head by neighbouring lanes
+      const int64_t slot = (static_cast<int64_t>(b) * p.c.heads + h) * p.blocks + block + cta;
+#pragma unroll
+      for (int r = 0; r < BLOCKS8; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = 8 * r + 2 * t + e;
+          const float sum = column_sum(l[r][e]);
+          if (row >= rows) continue;
+          const int64_t to = slot * p.rows + row;
+          if (g == 0) p.x.own_stats[to] = make_float2(m[r][e], any ? sum : -1.0f);
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) p.x.own[to * DPAD + (CODES ? g * (DPAD / 8) + 2 * i + half : 16 * i + 8 * half + g)] = o[r][i][2 * half + e];
+        }
+    } else {
     // ------------------------------------------------------------- the four warps' parts together
     float* mine = reinterpret_cast<float*>(ring);     // rows of DPAD: the ring is empty
 #pragma unroll
@@ -521,8 +559,7 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
             mine[row * DPAD + (CODES ? g * (DPAD / 8) + 2 * i + half : 16 * i + 8 * half + g)] = o[r][i][2 * half + e];
       }
     __syncthreads();
-    const bool whole = JOIN || (tile0 == 0 && tile1 == tiles);
-    const int64_t own_slot = (static_cast<int64_t>(b) * p.c.heads + h) * p.blocks + block;
+    const bool whole = tile0 == 0 && tile1 == tiles;
     // CTAs that share the item: c0 .. c1, those with a piece of it; the counter of the one that begins it
     const int c0 = whole ? cta : holder(total, item_start, ctas), c1 = whole ? cta : holder(total, item_end - 1, ctas);
     float* part = p.parts + (static_cast<int64_t>(cta) * 2 + (at == first_tile ? 0 : 1)) * kPart;
@@ -544,11 +581,7 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
         const float4 v = *reinterpret_cast<const float4*>(smem + w * S::kDepth * S::kBytes + (row * DPAD + d) * 4);
         acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
       }
-      if constexpr (JOIN) {
-        const int64_t to = (own_slot + cta) * p.rows + row;
-        *reinterpret_cast<float4*>(p.x.own + to * DPAD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        if (d == 0) p.x.own_stats[to] = make_float2(top, has ? sum : -1.0f);
-      } else if (whole) {
+      if (whole) {
         if (d < p.c.D) {
           const float f = v_scale / sum;
           T* dst = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.Hq + head0 + row) * p.c.D + d;
@@ -637,9 +670,10 @@ __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm)
       }
     }
     __syncthreads();
+    }
     at += tile1 - tile0;
     if (at >= end) break;
-    item_start = item_end;
+    item_start = item_end + kFront;
     if (++block == p.blocks) {
       block = 0;
       if (++h == p.c.heads) h = 0, see = keys_seen<JOIN>(p, ++b);
@@ -727,7 +761,7 @@ int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
 
 void paged::own_shape(int64_t B, int64_t Hq, int64_t heads, int* rows, int* blocks, int64_t* slots) {
   heads_of_items(static_cast<int>(Hq / heads), rows, blocks);
-  *slots = B * heads * *blocks + kMaxCtas;
+  *slots = B * heads * *blocks + kMaxCtas * kWarps;
 }
 
 int paged::attend_behind_prefix(const Cache& c, const Prefix& x, const void* q, int dtype, const int64_t* q_strides, int64_t B, int64_t Hq, float scale,
@@ -735,7 +769,7 @@ int paged::attend_behind_prefix(const Cache& c, const Prefix& x, const void* q, 
   DecodeParams p{};
   p.c = c, p.x = x;
   set_shape(&p, q, q_strides, nullptr, B, Hq, scale, workspace);
-  const int64_t tiles = (c.capacity > 0 ? (c.capacity + kTile - 1) / kTile : 1) * B * c.heads * p.blocks;
+  const int64_t tiles = ((c.capacity > 0 ? (c.capacity + kTile - 1) / kTile : 1) + 1) * B * c.heads * p.blocks;
   return launch_decode_t<true>(p, dtype, tiles, st);
 }
 

@@ -890,10 +890,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
   if (there) {
     const int head = hq - h * p.x.group, g = paged::ld_index(p.x.group_of + b), place = paged::ld_index(p.x.place_of + b);
     const int held = paged::cached_tokens(p.c, b, 0x7fffffff), shared = paged::prefix_tokens(p.x, b, held);
-    // its own keys: tiles of 64
+    // its own keys
     const int64_t own_total = __ldcg(p.x.own_lines + p.B), own_ctas = __ldcg(p.x.own_lines + p.B + 1);
-    const int own_tiles = held > shared ? (held - shared + 63) / 64 : 1, own_block = head / p.x.own_rows;
-    const int64_t own_start = __ldcg(p.x.own_lines + b) + (static_cast<int64_t>(h) * p.x.own_blocks + own_block) * own_tiles;
+    const int own_tiles = held > shared ? (held - shared + 15) / 16 : 1, own_block = head / p.x.own_rows;
+    const int64_t own_start = __ldcg(p.x.own_lines + b) + (static_cast<int64_t>(h) * p.x.own_blocks + own_block) * (own_tiles + paged::kOwnItemTiles) + paged::kOwnItemTiles;
     const int o0 = holder(own_total, own_start, static_cast<int>(own_ctas)), o1 = holder(own_total, own_start + own_tiles - 1, static_cast<int>(own_ctas));
     const int64_t own_at = ((static_cast<int64_t>(b) * p.c.heads + h) * p.x.own_blocks + own_block + o0) * p.x.own_rows + head - own_block * p.x.own_rows;
     // its prefix: of each part the half that holds the row, or (not paired) both

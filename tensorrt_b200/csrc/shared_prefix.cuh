@@ -19,6 +19,7 @@ __device__ __forceinline__ int holder(int64_t tiles, int64_t x, int ctas) { retu
 namespace paged {
 
 constexpr int kPrefixRows = 128, kPrefixKeys = 128;      // of a tile
+constexpr int kOwnItemTiles = 2;                         // the same for a sequence's own keys, in their tiles
 constexpr int kItemSteps = 2;                            // what beginning another item costs a CTA, in steps: room in front of each item in the line
 
 __device__ __forceinline__ int ld_index(const int32_t* p) {
@@ -46,11 +47,12 @@ struct Prefix {
   float* parts;                 // [slots][2][rows][D up to 64 or 128], unnormalised
   float2* stats;                // [slots][2][rows] base-2 logarithm of what they are referred to, sum (-1: no key)
   int64_t* lines;               // [groups][2] steps and items in front of each group; behind them: steps of all, CTAs, whether paired
-  // The keys that a sequence has to itself, the same way: items are a sequence, a kv head and a block of its query heads, tiles are of 64 keys.
+  // The keys that a sequence has to itself, the same way: items are a sequence, a kv head and a block of its query heads, tiles are of 16 keys, and
+  // every warp has a piece of the line.
   int own_rows, own_blocks;     // query heads of an item, items of a kv head
   float* own;                   // [slots][own_rows][D up to 64 or 128]
   float2* own_stats;            // [slots][own_rows]
-  int64_t* own_lines;           // [B] tiles in front of each sequence; behind them: tiles of all, CTAs
+  int64_t* own_lines;           // [B] tiles in front of each sequence; behind them: tiles of all, warps
 };
 
 struct GroupWork {
