@@ -516,16 +516,16 @@ int b200q_paged_copy(void* const* pools, int64_t n_pools, int64_t num_pages, int
  * whose first tokens[g] tokens are the same.  These are found through the line of block_table of the group's FIRST sequence; the keys
  * behind them, and all keys of a sequence that is in no group, through its own.  A sequence that holds fewer tokens than
  * its group's prefix is attended to through its own line alone.
- * b200q_shared_prefix_plan writes b200q_shared_prefix_plan_values(B, groups) int32 to `plan`, all of it HOST memory (the caller takes it to
- * the device), and refuses a sequence outside the batch or in two groups.  It goes by sequences, not by pages: it stays valid as
- * sequences grow.  The call never reads or writes out of bounds, whatever the plan holds.
- *   plan      on the device, 4-byte aligned; `groups` as it was made with; largest: sequences of the largest group (more are left out)
+ * b200q_shared_prefix_plan writes b200q_shared_prefix_plan_values(..) int32 to `plan`, all of it HOST memory (the caller takes it to
+ * the device), and refuses a sequence outside the batch or in two groups and a group of more than `largest`.  It goes by sequences,
+ * not by pages: it stays valid as sequences grow.  The call never reads or writes out of bounds, whatever the plan holds.
+ *   plan      on the device, 16-byte aligned, made for the same B, Hq, heads, groups and largest
  *   attention_workspace  as of b200q_paged_attention
  *   workspace b200q_shared_prefix_workspace_bytes(..) bytes, 16-byte aligned, any content; not shared by calls that overlap
  * B * Hq < 2^30. */
-int64_t b200q_shared_prefix_plan_values(int64_t B, int64_t groups);
-int b200q_shared_prefix_plan(const int32_t* members, const int32_t* cu, const int32_t* tokens, int64_t groups, int64_t B,
-                             int32_t* plan);
+int64_t b200q_shared_prefix_plan_values(int64_t B, int64_t Hq, int64_t heads, int64_t groups, int64_t largest);
+int b200q_shared_prefix_plan(const int32_t* members, const int32_t* cu, const int32_t* tokens, int64_t B, int64_t Hq,
+                             int64_t heads, int64_t groups, int64_t largest, int32_t* plan);
 size_t b200q_shared_prefix_workspace_bytes(int64_t B, int64_t Hq, int64_t heads, int64_t D, int64_t groups, int64_t largest);
 int b200q_shared_prefix_attention(const void* q, int dtype, const int64_t* q_strides, const b200q_paged_cache* cache,
                                   const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* lens,

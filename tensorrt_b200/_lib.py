@@ -66,8 +66,8 @@ SIGNATURES = {
     "b200q_window_attention": (_c.c_int, [_p, _p, _p, _c.c_int, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _c.c_float, _i64, _i64, _p]),
     "b200q_window_attention_form": (_c.c_int, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
     "b200q_paged_copy": (_c.c_int, [_p, _i64, _i64, _i64, _c.c_int32, _i64, _p, _p, _p, _p, _i64, _p]),
-    "b200q_shared_prefix_plan_values": (_i64, [_i64, _i64]),
-    "b200q_shared_prefix_plan": (_c.c_int, [_p, _p, _p, _i64, _i64, _p]),
+    "b200q_shared_prefix_plan_values": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "b200q_shared_prefix_plan": (_c.c_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "b200q_shared_prefix_workspace_bytes": (_c.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "b200q_shared_prefix_attention": (_c.c_int, [_p, _c.c_int, _p, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _c.c_float, _p, _p, _c.c_size_t, _p, _c.c_size_t, _p]),
     "b200q_token_log_probs": (_c.c_int, [_p, _c.c_int, _i64, _i64, _i64, _p, _c.c_int, _c.c_float, _p, _p, _i64, _p, _p, _p]),

@@ -225,9 +225,10 @@ Tensor shared_prefix_attention(const Tensor& q_in, const Tensor& k_pages, const 
   TORCH_CHECK_VALUE(groups >= 0 && groups <= a.B && largest >= 0 && largest <= a.B && (groups == 0 || largest > 0), op, ": no plan of a batch of ", a.B,
                     " has ", groups, " groups of up to ", largest);
   TORCH_CHECK(plan.device() == k_pages.device() && plan.scalar_type() == at::kInt && plan.dim() == 1 && plan.is_contiguous() &&
-                  plan.size(0) == b200q_shared_prefix_plan_values(a.B, groups),
-              op, ": the plan must be ", b200q_shared_prefix_plan_values(a.B, groups), " contiguous int32 values on the device of the pages (a batch of ", a.B,
-              ", ", groups, " groups), got ", plan.sizes(), " of ", plan.scalar_type());
+                  (groups == 0 || (plan.size(0) == b200q_shared_prefix_plan_values(a.B, Hq, a.c.heads, groups, largest) &&
+                                  reinterpret_cast<uintptr_t>(plan.data_ptr()) % 16 == 0)),
+              op, ": the plan must be ", b200q_shared_prefix_plan_values(a.B, Hq, a.c.heads, groups, largest), " contiguous int32 values on the device of the pages (a batch of ",
+              a.B, ", ", Hq, " / ", a.c.heads, " heads, ", groups, " groups of up to ", largest, "), 16-byte aligned, got ", plan.sizes(), " of ", plan.scalar_type());
   Tensor out = at::empty(q_in.sizes(), q_in.options());
   if (a.B == 0) return out;
   Tensor q = rows_of_16(q_in);

@@ -7,7 +7,7 @@
 // the prefix belong to one sequence each: the kernel of paged_attention.cu attends to them, and joins its result with the parts left here:
 // with m = max_i m_i, sum = sum_i l_i 2^(m_i - m), out = sum_i o_i 2^(m_i - m) / sum.
 //
-// Work: shared_prefix.cuh, a CTA to an SM.  Two times four warps run the softmax of a tile of 128 x 128 scores each, one thread to a row; one warp
+// Work: shared_prefix.cuh, a CTA to an SM.  (Found by the CTAs themselves from the plan's groups, their pieces cost 3 us in front of every call.)  Two times four warps run the softmax of a tile of 128 x 128 scores each, one thread to a row; one warp
 // issues the products of both in turn, so that the tensor cores work on one while the other is in its softmax; one asks for K and V rows, which
 // pages scatter, box by box (tensor maps); codes are widened to fp16, exactly, by four more warps in the place that they came to.  P takes the
 // place of the scores that it came from in tensor memory.
@@ -26,12 +26,11 @@ namespace b200q {
 namespace {
 
 using paged::Cache;
-using paged::GroupWork;
+using paged::PlanLayout;
 using paged::Prefix;
 using paged::kPrefixKeys;
 using paged::kPrefixRows;
 
-constexpr int kMostCtas = 192;                   // of a launch
 
 struct PrefixParams {
   Cache c;
@@ -59,7 +58,7 @@ struct Layout {
   static constexpr int kMostStages = kTiles - 1;
   static constexpr int kBars = 3 * kMostStages + 11;
   static constexpr int kSlots = 16;                     // of tiles whose masks are kept
-  static constexpr int kSmem = 1024 + kTiles * kTileBytes + kBars * 8 + 16 + kSlots * 16 + 16 + 128;
+  static constexpr int kSmem = 1024 + kTiles * kTileBytes + kBars * 8 + 16 + kSlots * 16 + 16;
   static constexpr int kThreads = CODES ? 512 : 384, kMmaWarp = 8, kLoadWarp = 9, kWidenWarp = 12, kWidenWarps = 4;
   static constexpr int kLoadWarps = kThreads / 32 - kLoadWarp;        // where threads load
   static constexpr int kTmemCols = 512;                 // the scores of both tiles, then O of both
@@ -79,44 +78,57 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* status
 
 // A CTA's way along its piece of the line, item after item.
 struct Walk {
-  int64_t left;              // steps from here to the end of the piece
-  int64_t item;              // number of the item
+  int left;                  // steps from here to the end of the piece
+  int item;                  // number of the item
   int g, h, block, step;     // the item, and the first step of this CTA's part of it
-  int steps, blocks;         // of an item, of a kv head
+  int first, n, tokens, leader;   // of the group
+  int tiles, rows;           // key tiles and rows of the group
   bool paired;
-  GroupWork w;
-  __device__ __forceinline__ int count() const { return static_cast<int>(left < steps - step ? left : steps - step); }
+  __device__ __forceinline__ int steps() const { return paired ? tiles : (tiles + 1) >> 1; }
+  __device__ __forceinline__ int blocks() const { return paired ? (rows + 255) >> 8 : (rows + 127) >> 7; }
+  __device__ __forceinline__ int count() const { return min(left, steps() - step); }
   // first row of tile s, first key tile of step j of it; whether there are any
   __device__ __forceinline__ int row0(int s) const { return paired ? block * 256 + s * 128 : block * 128; }
   __device__ __forceinline__ int tile(int j, int s) const { return paired ? step + j : 2 * (step + j) + s; }
-  __device__ __forceinline__ bool has(int j, int s) const { return s == 0 || (paired ? row0(1) < w.rows : tile(j, 1) < w.tiles); }
+  __device__ __forceinline__ bool has(int j, int s) const { return s == 0 || (paired ? row0(1) < rows : tile(j, 1) < tiles); }
   // key tiles of the first `count` steps that are loaded
   __device__ __forceinline__ int loaded(int count) const { return paired ? count : 2 * count - (has(count - 1, 1) ? 0 : 1); }
-  __device__ __noinline__ void set_group(const PrefixParams& p, int group) {
-    g = group;
-    w = paged::group_work(p.x, p.c, g);
-    steps = w.steps(paired), blocks = w.blocks(paired);
+  // of the group: place of its first sequence, sequences, tokens, leader
+  __device__ __forceinline__ void set_group(const PrefixParams& p, const int4& of) {
+    first = min(max(of.x, 0), p.x.B), n = min(max(min(of.y, p.x.largest), 0), p.x.B - first);
+    tokens = min(max(of.z, 0), 0x7fffff00), leader = of.w;
+    tiles = (tokens + kPrefixKeys - 1) / kPrefixKeys, rows = n * p.x.group;
   }
   __device__ __forceinline__ void next(const PrefixParams& p) {
     left -= count() + paged::kItemSteps;
     step = 0;
     if (left <= 0) return;
     ++item;
-    if (++block < blocks) return;
+    if (++block < blocks()) return;
     block = 0;
     if (++h < p.x.heads) return;
     h = 0;
     do {
-      if (g + 1 >= p.x.groups) {
+      if (++g >= p.x.groups) {
         left = 0;
         return;
       }
-      set_group(p, g + 1);
-    } while (steps == 0);
+      set_group(p, paged::ld_index4(p.x.plan + p.x.at.groups + PlanLayout::kGroup * g));
+    } while (tiles == 0 || rows == 0);
   }
 };
 
-static_assert(sizeof(Walk) <= 128, "has a place in shared memory");
+// The piece of CTA `cta`, empty where there is none.
+__device__ __forceinline__ Walk find_start(const PrefixParams& p, int cta) {
+  const int32_t* const at = p.x.plan + p.x.at.ctas + PlanLayout::kCta * cta;
+  const int4 a = paged::ld_index4(at), b = paged::ld_index4(at + 4), of = paged::ld_index4(at + 8);
+  Walk w;
+  w.paired = paged::ld_index(p.x.plan + p.x.at.head) != 0;
+  w.left = a.x, w.item = a.y, w.g = a.z, w.h = a.w, w.block = b.x, w.step = b.y;
+  w.set_group(p, of);
+  if (w.g < 0 || w.g >= p.x.groups || w.h < 0 || w.h >= p.x.heads || w.block < 0 || w.block >= w.blocks() || w.step < 0 || w.step >= w.steps()) w.left = 0;
+  return w;
+}
 
 // A place in the ring of stages.
 struct Ring {
@@ -127,79 +139,6 @@ struct Ring {
     if (stage >= stages) stage -= stages, phase ^= 1u;
   }
 };
-
-__device__ __noinline__ int64_t warp_scan(int64_t v) {               // inclusive
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t o = __shfl_up_sync(0xffffffffu, v, d);
-    if ((threadIdx.x & 31) >= d) v += o;
-  }
-  return v;
-}
-
-// Adds up the steps of all groups, paired and not, takes what is less, and finds the group that holds the first step of this CTA's piece, by one
-// warp: where all took part the others' barriers and the code cost more than the sums.  CTA 0 leaves the sums where the kernel behind finds them.
-__device__ __forceinline__ void find_start(const PrefixParams& p, int cta, int ctas, Walk* out) {
-  const int lane = threadIdx.x & 31;
-  int64_t all[2] = {}, steps[2], items[2];             // not paired, paired
-  auto group = [&](int g) {
-    GroupWork w{};
-    if (g < p.x.groups) w = paged::group_work(p.x, p.c, g);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      items[i] = w.tiles > 0 ? static_cast<int64_t>(p.x.heads) * w.blocks(i) : 0;
-      steps[i] = items[i] * (w.steps(i) + paged::kItemSteps);
-    }
-  };
-#pragma unroll 1
-  for (int base = 0; base < p.x.groups; base += 32) {
-    group(base + lane);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) all[i] += __shfl_sync(0xffffffffu, warp_scan(steps[i]), 31);
-  }
-  const bool paired = all[1] <= all[0];
-  const int64_t total = paired ? all[1] : all[0];
-  if (total < ctas) ctas = static_cast<int>(total);
-  if (cta == 0 && lane == 0) {
-    int64_t* const end = p.x.lines + 2 * p.x.groups;
-    end[0] = total, end[1] = ctas, end[2] = paired ? 1 : 0;
-  }
-  Walk walk{};
-  walk.paired = paired;
-  if (cta < ctas) {
-    const int64_t want = piece(total, cta, ctas);
-    int64_t before = 0, before_items = 0, at = 0, item0 = 0;
-    int found = 0;
-#pragma unroll 1
-    for (int base = 0; base < p.x.groups; base += 32) {
-      if (p.x.groups > 32) group(base + lane);
-      const int64_t own = steps[paired], own_items = items[paired], upto = warp_scan(own), upto_items = warp_scan(own_items);
-      const int64_t begin = before + upto - own, begin_items = before_items + upto_items - own_items;
-      if (cta == 0 && base + lane < p.x.groups) p.x.lines[2 * (base + lane)] = begin, p.x.lines[2 * (base + lane) + 1] = begin_items;
-      const unsigned here = __ballot_sync(0xffffffffu, want >= begin && want < begin + own);
-      if (here != 0) {
-        const int who = __ffs(here) - 1;
-        found = base + who, at = __shfl_sync(0xffffffffu, begin, who), item0 = __shfl_sync(0xffffffffu, begin_items, who);
-        if (cta != 0) break;
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31), before_items += __shfl_sync(0xffffffffu, upto_items, 31);
-    }
-    walk.set_group(p, found);
-    const int64_t rel = want - at, item = divide(rel, walk.steps + paged::kItemSteps);
-    const int step = static_cast<int>(rel - item * (walk.steps + paged::kItemSteps)) - paged::kItemSteps;
-    walk.h = static_cast<int>(divide(item, walk.blocks));
-    walk.block = static_cast<int>(item - static_cast<int64_t>(walk.h) * walk.blocks);
-    walk.item = item0 + item;
-    walk.left = piece(total, cta + 1, ctas) - want;
-    if (step < 0) walk.left += step;                   // begins in front of the item's first step
-    walk.step = step < 0 ? 0 : step;
-  }
-  if (lane == 0) *out = walk;
-}
-
-// All threads of the CTA, at different places of the code: the start of the CTA's piece is known.
-template <int THREADS>
-__device__ __forceinline__ void found_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const char* src, int bytes) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -314,7 +253,6 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
   uint64_t* const done = o_full + 2;
   uint4* const there = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(done + 1) + 15) & ~uintptr_t{15});   // which keys of a tile exist
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(there + L::kSlots);
-  Walk* const start = reinterpret_cast<Walk*>(tmem_slot + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == L::kMmaWarp) {
@@ -342,9 +280,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
   if (warp >= L::kMmaWarp) {
     ptx::setmaxnreg_dec<L::kOtherRegs>();
     pdl_enter(true);         // the kernel behind starts once everything in front of this one has completed, and reads that without a wait
-    if (warp == L::kLoadWarp) find_start(p, cta, static_cast<int>(gridDim.x), start);
-    found_barrier<L::kThreads>();
-    Walk walk = *start;
+    Walk walk = find_start(p, cta);
     // paired: two tiles of queries, a stage less
     char* const ring_at = base + (walk.paired ? 2 : 1) * L::kTileBytes;
     Ring ring{0, walk.paired ? L::kMostStages - 1 : L::kMostStages, 0};
@@ -355,10 +291,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       bool ok = true;
       int n = 0, issued = 0;                          // tiles so far; stages filled
       for (; walk.left > 0 && ok; walk.next(p)) {
-        const int count = walk.count(), tokens = walk.w.tokens;
-        const int leader = paged::ld_index(p.x.order + walk.w.first);
-        const bool named = leader >= 0 && leader < p.x.B;
-        const int32_t* line = p.c.table + (named ? leader : 0) * p.c.table_stride;
+        const int count = walk.count(), tokens = walk.tokens;
+        const bool named = walk.leader >= 0 && walk.leader < p.x.B && tokens <= p.c.capacity;
+        const int32_t* line = p.c.table + (named ? walk.leader : 0) * p.c.table_stride;
         int page[2], row[2];                          // of this lane's box, of each tile of a step
         auto find = [&](int j) {
 #pragma unroll
@@ -467,10 +402,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       bool ok = true;
       int n = 0;
       for (; walk.left > 0 && ok; walk.next(p)) {
-        const int count = walk.count(), tokens = walk.w.tokens;
-        const int leader = paged::ld_index(p.x.order + walk.w.first);
-        const bool named = leader >= 0 && leader < p.x.B;
-        const int32_t* line = p.c.table + (named ? leader : 0) * p.c.table_stride;
+        const int count = walk.count(), tokens = walk.tokens;
+        const bool named = walk.leader >= 0 && walk.leader < p.x.B && tokens <= p.c.capacity;
+        const int32_t* line = p.c.table + (named ? walk.leader : 0) * p.c.table_stride;
         int page[4], row[4];                          // of keys lane, lane + 32, .. of a tile: page (-1: none), row
         auto find = [&](int tile) {
 #pragma unroll
@@ -644,11 +578,11 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
     // of the line and the kernel in front.
     bool dry = p.x.heads > 0;
     Walk walk{};
-    walk.left = walk.steps = 1, walk.w.tiles = 128;
+    walk.left = 1, walk.tiles = 2;
     while (walk.left > 0 && ok) {
       const int count = walk.count();
-      const int64_t half = 2 * (walk.item + cta) + s;
-      const bool keeps = r < p.x.rows && (half >> 1) < p.x.slots;
+      const int64_t half = 2 * (static_cast<int64_t>(walk.item) + cta) + s;
+      const bool keeps = r < p.x.rows && walk.item >= 0 && walk.item < p.x.items;
       bool mine = false;
       float sl = p.scale * 1.4426950408889634f;
       if (!dry) {
@@ -660,13 +594,14 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       }
       // the row's query: products with those of the item before have ended (this tile's O was complete)
       const int at = walk.row0(s) + r, place = at / p.x.group;
-      int b = -1;
-      if (place < walk.w.n) b = paged::ld_index(p.x.order + walk.w.first + place);
-      mine = b >= 0 && b < p.x.B && paged::cached_tokens(p.c, b, 0x7fffffff) >= walk.w.tokens;
+      int b = -1, held = 0;
+      if (place < walk.n) b = paged::ld_index(p.x.plan + p.x.at.order + walk.first + place);
+      const bool there_is = b >= 0 && b < p.x.B;
+      if (there_is) held = paged::cached_tokens(p.c, b, 0x7fffffff);     // waited for behind the query's loads
       {
         // a row's pieces of 16 bytes by neighbouring lanes
         constexpr int kLanes = DPAD / 8, kRowsAtOnce = 32 / kLanes, kRounds = 32 / kRowsAtOnce, kBatch = 8;
-        const int64_t off = mine ? b * p.q_batch + (walk.h * p.x.group + at - place * p.x.group) * p.q_head : -1;
+        const int64_t off = there_is ? b * p.q_batch + (walk.h * p.x.group + at - place * p.x.group) * p.q_head : -1;
         const int c = lane % kLanes;
         constexpr bool kScaled = CODES && !std::is_same<T, __half>::value;
         float back = 1.0f;
@@ -703,6 +638,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
           }
         }
         if constexpr (kScaled) sl *= 1.0f / back;
+        mine = there_is && held >= walk.tokens;
         if (s == 0 || walk.paired) {
           ptx::fence_proxy_async();
           __syncwarp();
@@ -804,9 +740,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
         }
       }
       if (dry) {
-        found_barrier<L::kThreads>();
         pdl_wait();
-        walk = *start;
+        walk = find_start(p, cta);
         dry = false;
         continue;
       }
@@ -876,46 +811,39 @@ struct PartSum {
 };
 
 template <typename T, int DPAD>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ JoinParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 3) join_kernel(const __grid_constant__ JoinParams p) {
   __shared__ float4 acc_of[kJoinWarps][32];
   __shared__ float2 stats_of[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share_log2 = 3 - p.rows_log2, share = warp & ((1 << share_log2) - 1);
-  const int64_t id = (static_cast<int64_t>(blockIdx.x) << p.rows_log2) + (warp >> share_log2);
-  const bool there = id < static_cast<int64_t>(p.B) * p.Hq;
-  const int b = there ? static_cast<int>(id / p.Hq) : 0, hq = there ? static_cast<int>(id - static_cast<int64_t>(b) * p.Hq) : 0;
-  const int h = hq / p.x.group, d = lane * 4;
+  const int id = static_cast<int>(blockIdx.x << p.rows_log2) + (warp >> share_log2);
+  const bool there = id < p.B * p.Hq;
+  const int b = there ? id / p.Hq : 0, hq = there ? id - b * p.Hq : 0, h = hq / p.x.group, head = hq - h * p.x.group, d = lane * 4;
   pdl_launch_dependents();
   pdl_wait();
   PartSum a{-INFINITY, 0.0f, {}, false};
   if (there) {
-    const int head = hq - h * p.x.group, g = paged::ld_index(p.x.group_of + b), place = paged::ld_index(p.x.place_of + b);
-    const int held = paged::cached_tokens(p.c, b, 0x7fffffff), shared = paged::prefix_tokens(p.x, b, held);
-    // its own keys
-    const int64_t own_total = __ldcg(p.x.own_lines + p.B), own_ctas = __ldcg(p.x.own_lines + p.B + 1);
-    const int own_tiles = held > shared ? (held - shared + 15) / 16 : 1, own_block = head / p.x.own_rows;
-    const int64_t own_start = __ldcg(p.x.own_lines + b) + (static_cast<int64_t>(h) * p.x.own_blocks + own_block) * (own_tiles + paged::kOwnItemTiles) + paged::kOwnItemTiles;
-    const int o0 = holder(own_total, own_start, static_cast<int>(own_ctas)), o1 = holder(own_total, own_start + own_tiles - 1, static_cast<int>(own_ctas));
-    const int64_t own_at = ((static_cast<int64_t>(b) * p.c.heads + h) * p.x.own_blocks + own_block + o0) * p.x.own_rows + head - own_block * p.x.own_rows;
     // its prefix: of each part the half that holds the row, or (not paired) both
+    const int4 of = paged::ld_index4(p.x.plan + p.x.at.sequences + PlanLayout::kSequence * b);
+    const bool paired = paged::ld_index(p.x.plan + p.x.at.head) != 0;
+    const int held = paged::cached_tokens(p.c, b, 0x7fffffff);
+    const int64_t own_total = __ldcg(p.x.own_lines + p.B);
+    const int own_ctas = static_cast<int>(__ldcg(p.x.own_lines + p.B + 1));
+    const int64_t own_begin = __ldcg(p.x.own_lines + b);
+    const int shared = paged::prefix_tokens(of.x, held), row = of.w + head, item = of.y + h * of.z + (row >> (paired ? 8 : 7)), r = row & 127;
     int parts = 0, log2 = 0;
-    int64_t at = 0, slots = 0;                         // the first, in rows; slots that there are from there on
-    if (shared > 0 && g >= 0 && g < p.x.groups) {
-      const GroupWork w = paged::group_work(p.x, p.c, g);
-      const int64_t* const end = p.x.lines + 2 * p.x.groups;
-      const int64_t total = __ldcg(end), ctas = __ldcg(end + 1);
-      const bool paired = __ldcg(end + 2) != 0;
-      const int row = place * p.x.group + head, block = row >> (paired ? 8 : 7), r = row & 127, steps = w.steps(paired);
-      if (w.tiles > 0 && place >= 0 && place < w.n && r < p.x.rows && total > 0) {
-        const int64_t item = static_cast<int64_t>(h) * w.blocks(paired) + block;
-        const int64_t start = __ldcg(p.x.lines + 2 * g) + item * (steps + paged::kItemSteps) + paged::kItemSteps;
-        const int c0 = holder(total, start, static_cast<int>(ctas)), c1 = holder(total, start + steps - 1, static_cast<int>(ctas));
-        const int64_t slot = __ldcg(p.x.lines + 2 * g + 1) + item + c0;
-        log2 = paired ? 0 : 1;
-        parts = (c1 - c0 + 1) << log2;
-        at = (2 * slot + (paired ? (row >> 7) & 1 : 0)) * p.x.rows + r;
-        slots = p.x.slots - slot;
-      }
+    int64_t at = 0;                                    // the first, in rows
+    if (shared > 0 && row >= 0 && item >= 0 && item < p.x.items && r < p.x.rows) {
+      const int32_t* const entry = p.x.plan + p.x.at.items + PlanLayout::kItem * item;
+      const int c0 = min(max(paged::ld_index(entry), 0), paged::kPrefixCtas), ctas = min(max(paged::ld_index(entry + 1), 0), paged::kPrefixCtas - c0);
+      log2 = paired ? 0 : 1;
+      parts = ctas << log2;
+      at = (2 * (static_cast<int64_t>(item) + c0) + (paired ? (row >> 7) & 1 : 0)) * p.x.rows + r;
     }
+    // its own keys
+    const int own_tiles = held > shared ? (held - shared + 15) / 16 : 1, own_block = head / p.x.own_rows;
+    const int64_t own_start = own_begin + static_cast<int64_t>(h * p.x.own_blocks + own_block) * (own_tiles + paged::kOwnItemTiles) + paged::kOwnItemTiles;
+    const int o0 = holder(own_total, own_start, own_ctas), o1 = holder(own_total, own_start + own_tiles - 1, own_ctas);
+    const int64_t own_at = ((static_cast<int64_t>(b) * p.c.heads + h) * p.x.own_blocks + own_block + o0) * p.x.own_rows + head - own_block * p.x.own_rows;
     const int all = parts + o1 - o0 + 1, from = all * share >> share_log2, to = all * (share + 1) >> share_log2;
     constexpr int kAtOnce = 8;
 #pragma unroll 1
@@ -926,7 +854,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
       for (int k = 0; k < kAtOnce; ++k) {              // the loads first: they do not wait for one another
         s[k].y = -1.0f;
         const int n = i + k;
-        if (n >= to || (n < parts && n >> log2 >= slots)) continue;
+        if (n >= to) continue;
         const int64_t of = n < parts ? at + static_cast<int64_t>(log2 ? n : 2 * n) * p.x.rows : own_at + static_cast<int64_t>(n - parts) * p.x.own_rows;
         s[k] = __ldcg((n < parts ? p.x.stats : p.x.own_stats) + of);
         if (d < DPAD) v[k] = __ldcg(reinterpret_cast<const float4*>((n < parts ? p.x.parts : p.x.own) + of * DPAD + d));
@@ -952,7 +880,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
     const float f = (p.c.codes ? paged::head_scale(p.c.v_amax, p.c.amax_stride, h) : 1.0f) / a.sum;
     u = make_uint2(pack16<T>(a.acc[0] * f, a.acc[1] * f), pack16<T>(a.acc[2] * f, a.acc[3] * f));
   }
-  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + id * p.c.D + d) = u;
+  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + static_cast<int64_t>(id) * p.c.D + d) = u;
 }
 
 // [D, rows, heads, pages] -> boxes of 128 bytes x box_rows of one head and page, zeros out of bounds; false where a tensor map cannot hold the strides
@@ -985,8 +913,7 @@ int launch_prefix(const CUtensorMap& tk, const CUtensorMap& tv, const PrefixPara
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem) != cudaSuccess) return B200Q_ERR_CUDA;
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
   }
-  const int ctas = sm_count() < kMostCtas ? sm_count() : kMostCtas;
-  if (launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(L::kThreads), L::kSmem, st, tk, tv, p) != cudaSuccess) return B200Q_ERR_CUDA;
+  if (launch_pdl(kernel, dim3(paged::kPrefixCtas), dim3(L::kThreads), L::kSmem, st, tk, tv, p) != cudaSuccess) return B200Q_ERR_CUDA;
   return check_launch();
 }
 template <typename T, bool CODES>
@@ -1003,9 +930,9 @@ int launch_join(const JoinParams& p, cudaStream_t st) {
   return check_launch();
 }
 
-// Parts of a call, at most, and the rows of each: all of its CTAs' and all items.
+// Items of a call, at most, the rows of their parts, and the bytes of the workspace.
 struct Sizes {
-  int64_t rows, slots, parts, stats, lines, own, own_stats, own_lines, bytes;
+  int64_t rows, items, parts, stats, own, own_stats, own_lines, bytes;
   int own_rows, own_blocks;
 };
 bool sizes_of(int64_t B, int64_t Hq, int64_t heads, int64_t D, int64_t groups, int64_t largest, Sizes* s) {
@@ -1016,17 +943,18 @@ bool sizes_of(int64_t B, int64_t Hq, int64_t heads, int64_t D, int64_t groups, i
   s->rows = largest * group < kPrefixRows ? largest * group : kPrefixRows;
   // sum over the groups of ceil(sequences * group / 128), each at most its own number of row tiles, all together one more than full ones each
   const int64_t most = groups * ((largest * group + kPrefixRows - 1) / kPrefixRows), all = B * group / kPrefixRows + groups;
-  s->slots = heads * (most < all ? most : all) + kMostCtas;
+  s->items = heads * (most < all ? most : all);
+  if (s->items > 0x3fffffffLL) return false;
+  const int64_t slots = s->items + paged::kPrefixCtas;
   const auto round = [](int64_t n) { return (n + 255) / 256 * 256; };
-  s->lines = round((2 * groups + 3) * 8);
-  s->stats = round(2 * s->slots * s->rows * 8);
+  s->stats = round(2 * slots * s->rows * 8);
   int64_t own_slots;
   paged::own_shape(B, Hq, heads, &s->own_rows, &s->own_blocks, &own_slots);
   s->own_lines = round((B + 2) * 8);
   s->own_stats = round(own_slots * s->own_rows * 8);
   s->own = round(own_slots * s->own_rows * up * 4);
-  s->parts = round(2 * s->slots * s->rows * up * 4);
-  s->bytes = s->lines + s->stats + s->own_lines + s->own_stats + s->own + s->parts;
+  s->parts = round(2 * slots * s->rows * up * 4);
+  s->bytes = s->stats + s->own_lines + s->own_stats + s->own + s->parts;
   return true;
 }
 
@@ -1037,24 +965,102 @@ using namespace b200q;
 
 extern "C" {
 
-int64_t b200q_shared_prefix_plan_values(int64_t B, int64_t groups) { return B < 0 || groups < 0 || groups > B ? 0 : 4 * B + 2 * groups + 1; }
+int64_t b200q_shared_prefix_plan_values(int64_t B, int64_t Hq, int64_t heads, int64_t groups, int64_t largest) {
+  Sizes s;
+  return sizes_of(B, Hq, heads, 128, groups, largest, &s) ? paged::plan_layout(B, groups, s.items).values : 0;
+}
 
-int b200q_shared_prefix_plan(const int32_t* members, const int32_t* cu, const int32_t* tokens, int64_t groups, int64_t B, int32_t* plan) {
-  if (groups < 0 || B < 0 || B > 65535 || groups > B || plan == nullptr) return B200Q_ERR_INVALID;
-  if (groups > 0 && (cu == nullptr || tokens == nullptr || members == nullptr)) return B200Q_ERR_INVALID;
-  if (groups > 0 && cu[0] != 0) return B200Q_ERR_INVALID;
+int b200q_shared_prefix_plan(const int32_t* members, const int32_t* cu, const int32_t* tokens, int64_t B, int64_t Hq, int64_t heads, int64_t groups,
+                             int64_t largest, int32_t* plan) {
+  Sizes s;
+  if (!sizes_of(B, Hq, heads, 128, groups, largest, &s) || plan == nullptr) return B200Q_ERR_INVALID;
+  if (groups > 0 && (cu == nullptr || tokens == nullptr || members == nullptr || cu[0] != 0)) return B200Q_ERR_INVALID;
   for (int64_t g = 0; g < groups; ++g)
-    if (cu[g + 1] < cu[g] || cu[g + 1] > B || tokens[g] < 0) return B200Q_ERR_INVALID;
-  int32_t *const tokens_of = plan, *const group_of = plan + B, *const place_of = plan + 2 * B, *const order = plan + 3 * B, *const begin = plan + 4 * B,
-          *const shared = begin + groups + 1;
-  for (int64_t b = 0; b < B; ++b) tokens_of[b] = 0, group_of[b] = place_of[b] = order[b] = -1;
-  begin[0] = 0;
+    if (cu[g + 1] < cu[g] || cu[g + 1] > B || cu[g + 1] - cu[g] > largest || tokens[g] < 0) return B200Q_ERR_INVALID;
+  const PlanLayout l = paged::plan_layout(B, groups, s.items);
+  const int64_t group = Hq / heads;
+  for (int64_t i = 0; i < l.values; ++i) plan[i] = 0;
+  for (int64_t b = 0; b < B; ++b) plan[l.order + b] = -1;
   for (int64_t g = 0; g < groups; ++g) {
-    begin[g + 1] = cu[g + 1], shared[g] = tokens[g];
+    int32_t* const of = plan + l.groups + PlanLayout::kGroup * g;
+    of[0] = cu[g], of[1] = cu[g + 1] - cu[g], of[2] = tokens[g], of[3] = of[1] > 0 ? members[cu[g]] : -1;
     for (int32_t i = cu[g]; i < cu[g + 1]; ++i) {
       const int32_t b = members[i];
-      if (b < 0 || b >= B || group_of[b] >= 0) return B200Q_ERR_INVALID;      // of the batch, and in one group
-      order[i] = b, tokens_of[b] = tokens[g], group_of[b] = static_cast<int32_t>(g), place_of[b] = i - cu[g];
+      if (b < 0 || b >= B || plan[l.sequences + PlanLayout::kSequence * b + 2] != 0) return B200Q_ERR_INVALID;      // of the batch, and in one group
+      int32_t* const seq = plan + l.sequences + PlanLayout::kSequence * b;
+      seq[0] = tokens[g], seq[2] = 1, seq[3] = static_cast<int32_t>((i - cu[g]) * group);
+      plan[l.order + i] = b;
+    }
+  }
+  // Steps and blocks of a group, one way and the other, and the least longest piece, each item that is begun taken for kItemSteps more.
+  const auto steps = [&](int64_t g, bool paired) { const int64_t t = (static_cast<int64_t>(tokens[g]) + 127) / 128; return paired ? t : (t + 1) / 2; };
+  const auto blocks = [&](int64_t g, bool paired) {
+    const int64_t rows = (cu[g + 1] - cu[g]) * group, of = paired ? 256 : 128;
+    return tokens[g] > 0 ? (rows + of - 1) / of : 0;
+  };
+  const auto needed = [&](bool paired, int64_t longest) {    // pieces of up to that length
+    int64_t pieces = 0, room = 0;
+    for (int64_t g = 0; g < groups; ++g) {
+      const int64_t n = heads * blocks(g, paired), all = steps(g, paired);
+      for (int64_t i = 0; i < n; ++i) {
+        int64_t left = all;
+        if (room > paged::kItemSteps) {
+          const int64_t take = room - paged::kItemSteps < left ? room - paged::kItemSteps : left;
+          left -= take, room -= take + paged::kItemSteps;
+        }
+        if (left > 0) {
+          const int64_t full = (left - 1) / (longest - paged::kItemSteps);
+          left -= full * (longest - paged::kItemSteps);
+          pieces += full + 1, room = longest - paged::kItemSteps - left;
+        }
+        if (pieces > paged::kPrefixCtas) return pieces;
+      }
+    }
+    return pieces;
+  };
+  int64_t best[2];
+  for (int paired = 0; paired < 2; ++paired) {
+    int64_t total = 0;
+    for (int64_t g = 0; g < groups; ++g) total += heads * blocks(g, paired) * (steps(g, paired) + paged::kItemSteps);
+    int64_t low = paged::kItemSteps, high = total + paged::kItemSteps + 1;      // too short, long enough
+    while (high - low > 1) {
+      const int64_t mid = low + (high - low) / 2;
+      if (needed(paired, mid) <= paged::kPrefixCtas) high = mid;
+      else low = mid;
+    }
+    best[paired] = high;
+  }
+  const bool paired = best[1] <= best[0];
+  const int64_t longest = best[paired];
+  if (longest > 0x3fffffffLL) return B200Q_ERR_INVALID;
+  plan[l.head] = paired;
+  int64_t item = 0, room = 0, cta = -1;
+  for (int64_t g = 0; g < groups; ++g) {
+    const int64_t n = blocks(g, paired), all = steps(g, paired);
+    const int32_t* const of = plan + l.groups + PlanLayout::kGroup * g;
+    for (int32_t i = cu[g]; i < cu[g + 1]; ++i) {
+      int32_t* const seq = plan + l.sequences + PlanLayout::kSequence * members[i];
+      seq[1] = static_cast<int32_t>(item), seq[2] = static_cast<int32_t>(n);
+    }
+    for (int64_t k = 0; k < heads * n; ++k, ++item) {
+      int32_t* const entry = plan + l.items + PlanLayout::kItem * item;
+      int64_t at = 0;
+      bool begun = false;
+      while (at < all) {
+        int32_t* mine = plan + l.ctas + PlanLayout::kCta * cta;
+        if (at == 0 && !begun && room > paged::kItemSteps) {                    // behind the item before
+          room -= paged::kItemSteps, mine[0] += paged::kItemSteps;
+        } else {
+          ++cta, room = longest - paged::kItemSteps, mine = plan + l.ctas + PlanLayout::kCta * cta;
+          mine[1] = static_cast<int32_t>(item), mine[2] = static_cast<int32_t>(g), mine[3] = static_cast<int32_t>(k / n), mine[4] = static_cast<int32_t>(k % n);
+          mine[5] = static_cast<int32_t>(at);
+          for (int e = 0; e < 4; ++e) mine[8 + e] = of[e];
+        }
+        const int64_t take = room < all - at ? room : all - at;
+        mine[0] += static_cast<int32_t>(take), room -= take, at += take;
+        if (!begun) entry[0] = static_cast<int32_t>(cta), begun = true;
+        entry[1] = static_cast<int32_t>(cta - entry[0] + 1);
+      }
     }
   }
   return B200Q_OK;
@@ -1093,9 +1099,9 @@ int b200q_shared_prefix_attention(const void* q, int dtype, const int64_t* q_str
   if (p.status == nullptr) return B200Q_ERR_CUDA;
   char* at = static_cast<char*>(workspace);
   const auto take = [&at](int64_t n) { char* const here = at; at += n; return here; };
-  p.x = Prefix{plan, plan + B, plan + 2 * B, plan + 3 * B, plan + 4 * B, plan + 4 * B + groups + 1, static_cast<int>(B), static_cast<int>(groups),
-               static_cast<int>(largest), p.c.heads, static_cast<int>(Hq / p.c.heads), static_cast<int>(s.rows), s.slots};
-  p.x.lines = reinterpret_cast<int64_t*>(take(s.lines));
+  p.x.plan = plan, p.x.at = paged::plan_layout(B, groups, s.items);
+  p.x.B = static_cast<int>(B), p.x.groups = static_cast<int>(groups), p.x.largest = static_cast<int>(largest);
+  p.x.heads = p.c.heads, p.x.group = static_cast<int>(Hq / p.c.heads), p.x.rows = static_cast<int>(s.rows), p.x.items = static_cast<int>(s.items);
   p.x.stats = reinterpret_cast<float2*>(take(s.stats));
   p.x.own_rows = s.own_rows, p.x.own_blocks = s.own_blocks;
   p.x.own_lines = reinterpret_cast<int64_t*>(take(s.own_lines));

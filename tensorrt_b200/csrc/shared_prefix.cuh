@@ -19,62 +19,72 @@ __device__ __forceinline__ int holder(int64_t tiles, int64_t x, int ctas) { retu
 namespace paged {
 
 constexpr int kPrefixRows = 128, kPrefixKeys = 128;      // of a tile
-constexpr int kOwnItemTiles = 2;                         // the same for a sequence's own keys, in their tiles
-constexpr int kItemSteps = 2;                            // what beginning another item costs a CTA, in steps: room in front of each item in the line
+constexpr int kOwnItemTiles = 2;                         // what beginning another item costs a warp, in tiles: room in front of each in the line
+constexpr int kItemSteps = 2;                            // the same for a prefix's items, in steps
+constexpr int kPrefixCtas = 148;                         // SMs of a B200; any other number of them works through the same CTAs
 
 __device__ __forceinline__ int ld_index(const int32_t* p) {
   int v;
   asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
+__device__ __forceinline__ int4 ld_index4(const int32_t* p) {
+  int4 v;
+  asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
 
 // The rows of a group at a kv head: its sequences, one behind the other, each with the query heads of the kv head.  A CTA works on two tiles of
 // scores at once: of 256 rows and the same 128 keys ("paired"), or, where that is more, of 128 rows and two times 128 keys.  An item is a group,
-// a kv head and a block of that many rows, its keys are steps of 128 or 256.  The steps of all items stand in one line, which the CTAs cut into
-// equal pieces (each item with some room in front, which stands for its queries and its results); what a CTA computes of an item is a part, of two halves: the rows of each of the two tiles, or the same rows with every other 128
-// keys.  Along the line either the item or the CTA is another one from part to part, so item + CTA numbers the parts: their slots.
+// a kv head and a block of that many rows, its keys are steps of 128 or 256.  The steps of all items stand in one line, which the plan, made on the
+// host, cuts into a piece for each CTA, all as long as can be (with what it costs to begin another item); what a CTA computes of an item is
+// a part, of two halves: the rows of each of the two tiles, or the same rows with every other 128 keys.  Along the line either the item or the CTA
+// is another one from part to part, so item + CTA numbers the parts: their slots.
+//
+// The plan: 32-bit integers, each table at a multiple of four of them.  What is read of it is checked against the sizes of the call where an address
+// hangs on it.
+struct PlanLayout {
+  int64_t head, sequences, order, groups, ctas, items, values;
+  static constexpr int kHead = 4;                        // whether paired
+  static constexpr int kSequence = 4;                    // tokens of its prefix (0: none), first item, items of a kv head, its first row there
+  static constexpr int kGroup = 4;                       // place of its first sequence in `order`, sequences, tokens, the sequence whose line names them
+  static constexpr int kCta = 12;                        // steps (0: none), item, group, kv head, block, first step; of the group as above
+  static constexpr int kItem = 2;                        // first CTA, CTAs
+};
+inline PlanLayout plan_layout(int64_t B, int64_t groups, int64_t items) {
+  const auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
+  PlanLayout l{};
+  l.head = 0;
+  l.sequences = PlanLayout::kHead;
+  l.order = l.sequences + PlanLayout::kSequence * B;
+  l.groups = l.order + up(B);
+  l.ctas = l.groups + PlanLayout::kGroup * groups;
+  l.items = l.ctas + PlanLayout::kCta * kPrefixCtas;
+  l.values = l.items + up(PlanLayout::kItem * items);
+  return l;
+}
+
 struct Prefix {
-  const int32_t* tokens_of;     // [B] the plan (b200q_shared_prefix_plan): of each sequence, the tokens of its prefix,
-  const int32_t* group_of;      // [B] its group
-  const int32_t* place_of;      // [B] and its place there
-  const int32_t* order;         // [B] the sequences of all groups
-  const int32_t* cu;            // [groups + 1] where each begins there
-  const int32_t* tokens;        // [groups]
+  const int32_t* plan;
+  PlanLayout at;
   int B, groups, largest;       // largest: sequences of a group, at most
   int heads, group;             // kv heads, query heads of each
   int rows;                     // of half a part
-  int64_t slots;
-  float* parts;                 // [slots][2][rows][D up to 64 or 128], unnormalised
-  float2* stats;                // [slots][2][rows] base-2 logarithm of what they are referred to, sum (-1: no key)
-  int64_t* lines;               // [groups][2] steps and items in front of each group; behind them: steps of all, CTAs, whether paired
-  // The keys that a sequence has to itself, the same way: items are a sequence, a kv head and a block of its query heads, tiles are of 16 keys, and
-  // every warp has a piece of the line.
+  int items;                    // at most
+  float* parts;                 // [items + CTAs][2][rows][D up to 64 or 128], unnormalised
+  float2* stats;                // [items + CTAs][2][rows] base-2 logarithm of what they are referred to, sum (-1: no key)
+  // The keys that a sequence has to itself: items are a sequence, a kv head and a block of its query heads, tiles are of 16 keys, and every warp has
+  // a piece of their line, which it finds itself: the lengths are on the device.
   int own_rows, own_blocks;     // query heads of an item, items of a kv head
   float* own;                   // [slots][own_rows][D up to 64 or 128]
   float2* own_stats;            // [slots][own_rows]
   int64_t* own_lines;           // [B] tiles in front of each sequence; behind them: tiles of all, warps
 };
 
-struct GroupWork {
-  int first, n, tokens, tiles, rows;         // place of its first sequence, sequences, keys and their tiles of 128, rows of a kv head
-  __device__ __forceinline__ int steps(bool paired) const { return paired ? tiles : (tiles + 1) >> 1; }
-  __device__ __forceinline__ int blocks(bool paired) const { return paired ? (rows + 255) >> 8 : (rows + 127) >> 7; }
-};
-__device__ __forceinline__ GroupWork group_work(const Prefix& x, const Cache& c, int g) {
-  GroupWork w;
-  w.first = min(max(ld_index(x.cu + g), 0), x.B);
-  w.n = min(min(max(ld_index(x.cu + g + 1), w.first), x.B) - w.first, x.largest);
-  const int t = ld_index(x.tokens + g);
-  w.tokens = t > 0 && t <= c.capacity && w.n > 0 ? t : 0;
-  w.tiles = (w.tokens + kPrefixKeys - 1) / kPrefixKeys;
-  w.rows = w.n * x.group;
-  return w;
-}
-
 // Tokens of sequence b that are attended to with its group: of n in the cache, all of the prefix or (a sequence that has been cut or released) none.
+__device__ __forceinline__ int prefix_tokens(int shared, int n) { return shared > 0 && shared <= n ? shared : 0; }
 __device__ __forceinline__ int prefix_tokens(const Prefix& x, int b, int n) {
-  const int t = ld_index(x.tokens_of + b);
-  return t > 0 && t <= n ? t : 0;
+  return prefix_tokens(ld_index(x.plan + x.at.sequences + PlanLayout::kSequence * b), n);
 }
 
 // Rows and blocks of the kernel below, and its slots.

@@ -85,7 +85,8 @@ class SharedPrefix:
     """Which sequences of a batch share a prefix: the sequences members[g] have their first tokens[g] tokens in the same pages, which are found
     through the line of the block table of the first of them.  It goes by sequences and stays valid as they grow.
 
-    Groups of one sequence and prefixes of no token are left out: nothing is shared.  `update` says anew who shares what, in place, so that a
+    Groups of one sequence and prefixes of no token are left out: nothing is shared.  The first call of every pair of head counts makes a plan of the work
+    on the host, outside a stream capture, which later ones find on the device.  `update` says anew who shares what, in place, so that a
     captured call goes by it; it takes up to `groups` groups of up to `largest` sequences (None: those given here)."""
 
     def __init__(self, members: list, tokens: list, batch: int, device="cuda", groups: int | None = None, largest: int | None = None):
@@ -97,7 +98,7 @@ class SharedPrefix:
         self.largest = max([len(m) for m, _ in kept], default=0) if largest is None else largest
         if not 0 <= self.groups <= batch or not 0 <= self.largest <= batch:
             raise ValueError(f"{self.groups} groups of up to {self.largest} sequences are not in a batch of {batch}")
-        self.plan = torch.zeros(_lib.load().b200q_shared_prefix_plan_values(batch, self.groups), dtype=torch.int32, device=device)
+        self.device, self._plans = torch.device(device), {}
         self.update(members, tokens)
 
     @staticmethod
@@ -121,11 +122,29 @@ class SharedPrefix:
             ends.append(ends[-1] + len(m))
         ends += ends[-1:] * (self.groups - len(kept))                       # empty groups
         shared = [t for _, t in kept] + [0] * (self.groups - len(kept))
-        ints = lambda v: (ctypes.c_int32 * max(len(v), 1))(*v)  # noqa: E731
-        plan = torch.empty(self.plan.shape, dtype=torch.int32)
-        _lib.check(_lib.load().b200q_shared_prefix_plan(ints(flat), ints(ends), ints(shared), self.groups, self.batch, plan.data_ptr()),
-                   "b200q_shared_prefix_plan")
-        self.plan.copy_(plan.pin_memory() if self.plan.is_cuda else plan, non_blocking=True)
+        self._lists = [(ctypes.c_int32 * max(len(v), 1))(*v) for v in (flat, ends, shared)]
+        for heads, plan in self._plans.items():
+            host = self._made(*heads)
+            plan.copy_(host.pin_memory() if plan.is_cuda else host, non_blocking=True)
+
+    def _made(self, n_q: int, n_kv: int) -> torch.Tensor:
+        lib, sizes = _lib.load(), (self.batch, n_q, n_kv, self.groups, self.largest)
+        plan = torch.empty(lib.b200q_shared_prefix_plan_values(*sizes), dtype=torch.int32)
+        _lib.check(lib.b200q_shared_prefix_plan(*self._lists, *sizes, plan.data_ptr()), "b200q_shared_prefix_plan")
+        return plan
+
+    def plan(self, n_q: int, n_kv: int) -> torch.Tensor:
+        """The plan for this many query and kv heads, on the device."""
+        plan = self._plans.get((n_q, n_kv))
+        if plan is None:
+            if self.groups == 0:
+                plan = torch.empty(0, dtype=torch.int32, device=self.device)
+            else:
+                if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the plan of a shared prefix is made on the host: call once with these heads before the capture")
+                plan = _on_device(self._made(n_q, n_kv), self.device)
+            self._plans[n_q, n_kv] = plan
+        return plan
 
 
 def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
@@ -136,9 +155,12 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     its group's prefix is attended to through its own line alone."""
     if prefix.batch != q.shape[0]:
         raise ValueError(f"the prefixes are those of a batch of {prefix.batch}, q is {tuple(q.shape)}")
-    scale = 0.0 if scale is None else scale
-    out = _native.shared_prefix_attention(q, k_pages, v_pages, block_table, lens, prefix.plan, k_amax, v_amax, scale, prefix.groups, prefix.largest)
-    return _shared(q, k_pages, v_pages, block_table, lens, prefix.plan, prefix.groups, prefix.largest, k_amax, v_amax, scale) if out is None else out
+    if q.dim() != 3 or k_pages.dim() != 4 or k_pages.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k_pages.shape[1]:
+        raise ValueError(f"expected q [batch, query heads, D] and pages [pages, kv heads, rows, D], the kv heads dividing the query heads, got {tuple(q.shape)} "
+                         f"and {tuple(k_pages.shape)}")
+    scale, plan = 0.0 if scale is None else scale, prefix.plan(q.shape[1], k_pages.shape[1])
+    out = _native.shared_prefix_attention(q, k_pages, v_pages, block_table, lens, plan, k_amax, v_amax, scale, prefix.groups, prefix.largest)
+    return _shared(q, k_pages, v_pages, block_table, lens, plan, prefix.groups, prefix.largest, k_amax, v_amax, scale) if out is None else out
 
 
 def _on_device(values, device, dtype=torch.int32) -> torch.Tensor:

@@ -117,7 +117,7 @@ def test_shared_prefix(b200, case):
     check_out(out, ref, mass)
     for _ in range(3):                                     # no order of CTAs decides anything
         assert torch.equal(out, b200.shared_prefix_attention(q, kp, vp, table, on_device(lens), prefix, k_amax=ka, v_amax=va))
-    op = torch.ops.tensorrt.b200_shared_prefix_attention(q, kp, vp, table, on_device(lens), prefix.plan, prefix.groups, prefix.largest, ka, va, 0.0)
+    op = torch.ops.tensorrt.b200_shared_prefix_attention(q, kp, vp, table, on_device(lens), prefix.plan(q.shape[1], kp.shape[1]), prefix.groups, prefix.largest, ka, va, 0.0)
     assert torch.equal(out, op)
     # the same from a plan that leaves room for others
     wide = b200.SharedPrefix(members, tokens, len(lens), groups=len(lens), largest=len(lens))
