@@ -1087,7 +1087,7 @@ int b200q_shared_prefix_attention(const void* q, int dtype, const int64_t* q_str
   if (attention_workspace == nullptr || attention_workspace_bytes < b200q_paged_attention_workspace_bytes() || workspace == nullptr ||
       workspace_bytes < static_cast<size_t>(s.bytes))
     return B200Q_ERR_WORKSPACE;
-  if (!aligned(attention_workspace, 16) || !aligned(workspace, 16)) return B200Q_ERR_ALIGN;
+  if (!aligned(attention_workspace, 16) || !aligned(workspace, 16) || !aligned(plan, 16)) return B200Q_ERR_ALIGN;
   if (int rc = check_arch()) return rc;
   p.page_shift = -1;
   if ((p.c.page_size & (p.c.page_size - 1)) == 0)

@@ -122,6 +122,7 @@ class SharedPrefix:
             ends.append(ends[-1] + len(m))
         ends += ends[-1:] * (self.groups - len(kept))                       # empty groups
         shared = [t for _, t in kept] + [0] * (self.groups - len(kept))
+        self.tokens = max(shared, default=0)                                # of the longest prefix
         self._lists = [(ctypes.c_int32 * max(len(v), 1))(*v) for v in (flat, ends, shared)]
         for heads, plan in self._plans.items():
             host = self._made(*heads)
@@ -158,6 +159,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     if q.dim() != 3 or k_pages.dim() != 4 or k_pages.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k_pages.shape[1]:
         raise ValueError(f"expected q [batch, query heads, D] and pages [pages, kv heads, rows, D], the kv heads dividing the query heads, got {tuple(q.shape)} "
                          f"and {tuple(k_pages.shape)}")
+    if prefix.tokens > block_table.shape[-1] * k_pages.shape[2]:
+        raise ValueError(f"prefixes of up to {prefix.tokens} tokens do not fit the table's lines of {block_table.shape[-1]} pages of {k_pages.shape[2]} rows")
     scale, plan = 0.0 if scale is None else scale, prefix.plan(q.shape[1], k_pages.shape[1])
     out = _native.shared_prefix_attention(q, k_pages, v_pages, block_table, lens, plan, k_amax, v_amax, scale, prefix.groups, prefix.largest)
     return _shared(q, k_pages, v_pages, block_table, lens, plan, prefix.groups, prefix.largest, k_amax, v_amax, scale) if out is None else out
@@ -177,6 +180,12 @@ def _common(a: list, b: list) -> int:
         low, high = (mid, high) if a[low:mid] == b[low:mid] else (low, mid - 1)
     return low
 
+
+# Keys, times kv heads, that a batch's single-token attention has to read once instead of once more for each who shares them, before a cache takes the
+# kernels for shared prefixes.  Three launches cost what reading so much costs paged_attention.  Measured, paged / shared, in us: 8 kv heads x 4 of 128, 16
+# sequences behind 1024 tokens (0.12 M) 20.5 / 23.4, behind 4096 (0.49 M) 36.9 / 31.6; with 8-bit pages 22.4 / 26.7 and 36.9 / 36.0; 64 behind 256 (0.13 M)
+# 24.5 / 30.9, behind 1024 (0.52 M) 40.9 / 31.6; 2 kv heads x 4 of 64, 64 behind 1024 (0.13 M) 18.4 / 22.6, behind 4096 (0.52 M) 30.7 / 23.5.
+_SHARED_KEYS = 1 << 18
 
 _WHOLE = "prompts are attended to as a whole: a sequence that brings tokens must hold no older ones"
 
@@ -218,7 +227,7 @@ class PagedKvCache:
         self._free = list(range(pages - 1, -1, -1))
         self._pages: list = [[] for _ in range(batch)]     # of each sequence, in order
         self._uses = [0] * pages                           # sequences that a page is part of
-        self._prefix, self._shares, self._regroup = None, False, False
+        self._prefix, self._shares, self._n_q = None, False, 0
         self._tokens = [0] * batch
         self._released: set = set()
         self._padded = None
@@ -319,8 +328,10 @@ class PagedKvCache:
 
     def attend(self, layer: int, q: torch.Tensor, *, scale: float | None = None, window: int = 0, sinks: int = 0) -> torch.Tensor:
         """Attention of the newest token of every sequence: q [batch, query heads, head_dim].  Without a window and without weights, what groups
-        of forked sequences share is attended to once for all of a group."""
-        if self.weights[layer] is None and window <= 0 and self._sharing():
+        of forked sequences share is attended to once for all of a group, where that is much.  A captured step stays with the kernels that were
+        taken when it was captured, and is right behind any later call."""
+        self._n_q = q.shape[1] if q.dim() == 3 else 0
+        if self.weights[layer] is None and window <= 0 and self._shares:
             return shared_prefix_attention(q, self.k[layer], self.v[layer], self.table, self.lens, self._prefix, k_amax=self.k_amax[layer],
                                            v_amax=self.v_amax[layer], scale=scale)
         return paged_attention(q, self.k[layer], self.v[layer], self.table, self.lens, k_amax=self.k_amax[layer], v_amax=self.v_amax[layer],
@@ -381,7 +392,7 @@ class PagedKvCache:
             self._give_back(old)
         self._pages, self._tokens = fresh, [min(keep, t) for t in self._tokens]
         self._new = [0] * self.batch
-        self._regroup = True
+        self._share()
         return kept
 
     def _give_back(self, pages: list) -> None:
@@ -393,15 +404,17 @@ class PagedKvCache:
     def release(self, b: int) -> None:
         """Sequence b is done: its pages are free (those that others share once these are done too), and it is empty until `grow` brings it
         tokens again."""
+        shared = any(self._uses[p] > 1 for p in self._pages[b][:1])
         self._give_back(self._pages[b])
         self._pages[b], self._tokens[b], self._new[b] = [], 0, 0
-        self._regroup = True
         self._released.add(b % self.batch)
         self.lens[b].zero_()
         self.table[b].fill_(-1)
         for w in self.weights:
             if w is not None:
                 w[b].zero_()
+        if shared:
+            self._share()
 
     def fork(self, parents: list) -> None:
         """Sequence b goes on from where sequence parents[b] is (b itself: from where it was), for all at once: [0] * batch continues the first one
@@ -432,7 +445,7 @@ class PagedKvCache:
         for w in self.weights:
             if w is not None:
                 w.copy_(w.index_select(0, both[0]))
-        self._regroup = True
+        self._share()
 
     def truncate(self, tokens: list) -> None:
         """Cuts every sequence to its first tokens[b] tokens (those that a verification turned down go, say); the pages behind them are free, reserved
@@ -450,7 +463,7 @@ class PagedKvCache:
         for w in self.weights:
             if w is not None:
                 w.masked_fill_(torch.arange(w.shape[2], device=w.device) >= both[0][:, None, None], 0.0)
-        self._regroup = True
+        self._share()
 
     def compact(self) -> int:
         """Moves the pages in use to the front of the pools, shared ones once, and returns how many they are."""
@@ -487,23 +500,22 @@ class PagedKvCache:
         self._uses = self._uses[:used] + [0] * (pages - used)
         self._free = list(range(pages - 1, used - 1, -1))
 
-    def _sharing(self) -> bool:
-        """Whether any sequences share a prefix; who shares what is found anew behind what changed it, and kept where a captured step reads it."""
-        if self._regroup:
-            self._regroup = False
-            first: dict = {}
-            for b, pages in enumerate(self._pages):
-                if self._tokens[b] >= self.page_size and self._uses[pages[0]] > 1:
-                    first.setdefault(pages[0], []).append(b)
-            members = [m for m in first.values() if len(m) > 1]
-            # pages that all of a group have in common and that are full
-            shared = [self.page_size * min(min(_common(self._pages[m[0]], self._pages[b]), self._tokens[b] // self.page_size) for b in m) for m in members]
-            self._shares = bool(members)
-            if self._prefix is None and members:
-                self._prefix = SharedPrefix([], [], self.batch, self.table.device, groups=self.batch // 2, largest=self.batch)
-            if self._prefix is not None:
-                self._prefix.update(members, shared)
-        return self._shares
+    def _share(self) -> None:
+        """Finds who shares what, behind each call that changes it: a captured step reads the plan where it is, as it does the table."""
+        first: dict = {}
+        for b, pages in enumerate(self._pages):
+            if self._tokens[b] >= self.page_size and self._uses[pages[0]] > 1:
+                first.setdefault(pages[0], []).append(b)
+        members = [m for m in first.values() if len(m) > 1]
+        # pages that all of a group have in common and that are full
+        shared = [self.page_size * min(min(_common(self._pages[m[0]], self._pages[b]), self._tokens[b] // self.page_size) for b in m) for m in members]
+        self._shares = self.n_kv * sum((len(m) - 1) * t for m, t in zip(members, shared)) >= _SHARED_KEYS
+        if self._prefix is None and members:
+            self._prefix = SharedPrefix([], [], self.batch, self.table.device, groups=self.batch // 2, largest=self.batch)
+        if self._prefix is not None:
+            self._prefix.update(members, shared)
+            if self._n_q:                        # the first step behind a fork may be captured
+                self._prefix.plan(self._n_q, self.n_kv)
 
 
 class CachedDecoder:
