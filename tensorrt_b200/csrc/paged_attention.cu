@@ -268,7 +268,7 @@ __device__ __forceinline__ int64_t find_start(const DecodeParams& p, int cta, in
 // is a part of each row, as that kernel's are.  It reads nothing of that kernel, which lets it start only once everything in front has
 // completed: it waits at its end, so that it has ended only when the one in front has.  Here a warp takes a piece of the line by itself, in tiles of 16 keys,
 // and the kernel behind joins: these keys are few for every sequence, and what ends an item would be most of the time (100 sequences of 14 to 310 keys,
-// 12 / 12 heads of 80: @@).
+// 12 / 12 heads of 80: 40 us by whole items, 19.5 in pieces).
 template <typename T, bool CODES, int DPAD, int BLOCKS8, bool JOIN>
 __global__ void __launch_bounds__(kThreads, Stage<CODES, DPAD, BLOCKS8>::kPerSm) decode_kernel(const __grid_constant__ DecodeParams p) {
   using S = Stage<CODES, DPAD, BLOCKS8>;

@@ -3,21 +3,28 @@
 //   x_j = (q . k_j) * scale,  out = sum_j exp(x_j - m) v_j / sum_j exp(x_j - m),  m = max_j x_j
 //
 // The keys j < tokens of a group's prefix are the same for all of its sequences, so the rows of a group (its sequences times the query heads of a
-// kv head) meet them as one matrix product, S = Q K^T and O = P V on tcgen05, and every K and V row is read once for up to 128 rows.  The keys behind
-// the prefix belong to one sequence each: the kernel of paged_attention.cu attends to them, and joins its result with the parts left here:
+// kv head) meet them as one matrix product, S = Q K^T and O = P V on tcgen05, and every K and V row is read once for up to 256 rows.  The keys behind
+// the prefix belong to one sequence each: the kernel of paged_attention.cu attends to them, in parts.  A last kernel joins all parts of a row:
 // with m = max_i m_i, sum = sum_i l_i 2^(m_i - m), out = sum_i o_i 2^(m_i - m) / sum.
 //
-// Work: shared_prefix.cuh, a CTA to an SM.  (Found by the CTAs themselves from the plan's groups, their pieces cost 3 us in front of every call.)  Two times four warps run the softmax of a tile of 128 x 128 scores each, one thread to a row; one warp
-// issues the products of both in turn, so that the tensor cores work on one while the other is in its softmax; one asks for K and V rows, which
-// pages scatter, box by box (tensor maps); codes are widened to fp16, exactly, by four more warps in the place that they came to.  P takes the
-// place of the scores that it came from in tensor memory.
+// Work: shared_prefix.cuh, a CTA to an SM, pieces from the plan (found by the CTAs themselves they cost 3 us in front of every call).  Two times four
+// warps run the softmax of a tile of 128 x 128 scores each, one thread to a row; one warp issues the products of both in turn, so that the tensor
+// cores work on one while the other is in its softmax; one asks for K and V rows, which pages scatter, box by box (tensor maps); two copy queries
+// (by the softmax's threads, through registers, that took 3 to 10 us in front of the first product: their code came from memory in front of it); codes
+// are widened to fp16, exactly, by four more warps in the place that they came to.  P takes the place of the scores that it came from in tensor memory.
+//
+// What bounds it.  Long prefixes: the softmax.  A step of 256 rows x 128 keys x 128 takes 2.4 us (1030 TFLOP/s): a warp needs 24 clocks for a pair of
+// scores, alone on its quarter of the SM, whatever the order of its instructions, and the two tiles take turns with 1800 clocks of it each.  Tried in
+// vain, at 64 sequences x 8 heads behind 32768 tokens (80 us): one exponential in eight, in four, in two on the FMA pipe (80, 87, 97 us), two
+// threads to a row (135 us: 104 registers spill).  Short ones: what stands in front of the first product, some 4 us (launch, code from memory, queries,
+// the first boxes), and the two kernels behind.  64 sequences behind 8192 tokens, 64 / 8 heads of 128: prefix 26 us, own keys 11, join 10, 43 in a row;
+// 16 behind 100000 tokens of codes: 79, 15 and 11, 102 in a row.
 //
 // Rounding: S, the softmax, O and the sums are 32-bit; P is rounded to 16 bits for the second product, an error of one rounding of each term,
 // of the size of the result's own.  fp16 (fp16 pages and codes): P is raised by 2^11, so that holds for terms down to 2^-25 of the largest.  bf16
 // queries in front of codes are scaled by a power of two into fp16's range, which loses nothing above 2^-38 of a row's largest.
 #include <atomic>
 
-#include "ex2.cuh"
 #include "gemm_host.cuh"
 #include "shared_prefix.cuh"
 #include "softmax_tc.cuh"
@@ -30,7 +37,6 @@ using paged::PlanLayout;
 using paged::Prefix;
 using paged::kPrefixKeys;
 using paged::kPrefixRows;
-
 
 struct PrefixParams {
   Cache c;
@@ -49,17 +55,16 @@ template <bool HALF>
 constexpr float kLazy = HALF ? 4.0f : 8.0f;
 template <bool HALF>
 constexpr float kRaise = HALF ? 11.0f : 0.0f;
-constexpr int kPolyPairs = 2;   // of 16 pairs of exponentials: on the FMA pipe
 
 template <int DPAD, bool CODES>
 struct Layout {
   static constexpr int kBoxes = DPAD / 64, kBoxBytes = 128 * 128, kTileBytes = kBoxes * kBoxBytes;
   static constexpr int kTiles = DPAD == 128 ? 7 : 10;   // queries, then the ring; a second tile of queries takes a stage of it
   static constexpr int kMostStages = kTiles - 1;
-  static constexpr int kBars = 3 * kMostStages + 11;
+  static constexpr int kBars = 3 * kMostStages + 12;
   static constexpr int kSlots = 16;                     // of tiles whose masks are kept
-  static constexpr int kSmem = 1024 + kTiles * kTileBytes + kBars * 8 + 16 + kSlots * 16 + 16;
-  static constexpr int kThreads = CODES ? 512 : 384, kMmaWarp = 8, kLoadWarp = 9, kWidenWarp = 12, kWidenWarps = 4;
+  static constexpr int kSmem = 1024 + kTiles * kTileBytes + kBars * 8 + 16 + kSlots * 16 + 16 + 512;
+  static constexpr int kThreads = CODES ? 512 : 384, kMmaWarp = 8, kLoadWarp = 9, kQueryWarp = 10, kWidenWarp = 12, kWidenWarps = 4;
   static constexpr int kLoadWarps = kThreads / 32 - kLoadWarp;        // where threads load
   static constexpr int kTmemCols = 512;                 // the scores of both tiles, then O of both
   // registers at launch: 384 x 168 = 256 x 192 + 128 x 120, 512 x 128 = 256 x 192 + 256 x 64
@@ -166,6 +171,11 @@ __device__ __forceinline__ uint32_t tile_at(int row, int c) {
   return static_cast<uint32_t>((c >> 3) * (128 * 128) + row * 128 + (((c & 7) ^ (row & 7)) * 16));
 }
 
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
   uint2 r;
   asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
@@ -250,9 +260,11 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
   uint64_t* const p_half = s_full + 2;
   uint64_t* const p_full = p_half + 2;
   uint64_t* const o_full = p_full + 2;
-  uint64_t* const done = o_full + 2;
+  uint64_t* const q_empty = o_full + 2;
+  uint64_t* const done = q_empty + 1;
   uint4* const there = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(done + 1) + 15) & ~uintptr_t{15});   // which keys of a tile exist
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(there + L::kSlots);
+  int8_t* const ups = reinterpret_cast<int8_t*>(tmem_slot + 4);      // [items by turns][tiles][rows] powers of two that queries in front of codes are scaled by
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == L::kMmaWarp) {
@@ -263,8 +275,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
     for (int i = 0; i < L::kMostStages; ++i)
       ptx::mbar_init(full + i, MAPS ? (CODES ? L::kWidenWarps : 1) : 32 * L::kLoadWarps + 1), ptx::mbar_init(empty + i, 1), ptx::mbar_init(raw + i, 1);
     for (int s = 0; s < 2; ++s)
-      ptx::mbar_init(q_full + s, 4), ptx::mbar_init(s_full + s, 2), ptx::mbar_init(p_half + s, 4), ptx::mbar_init(p_full + s, 4), ptx::mbar_init(o_full + s, 1);
-    ptx::mbar_init(done, 1);
+      ptx::mbar_init(q_full + s, 64), ptx::mbar_init(s_full + s, 2), ptx::mbar_init(p_half + s, 4), ptx::mbar_init(p_full + s, 4), ptx::mbar_init(o_full + s, 1);
+    ptx::mbar_init(q_empty, 1), ptx::mbar_init(done, 1);
     ptx::fence_barrier_init();
     if constexpr (MAPS) {
       ptx::prefetch_tmap(&tk);
@@ -284,7 +296,67 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
     // paired: two tiles of queries, a stage less
     char* const ring_at = base + (walk.paired ? 2 : 1) * L::kTileBytes;
     Ring ring{0, walk.paired ? L::kMostStages - 1 : L::kMostStages, 0};
-    if (MAPS && warp == L::kLoadWarp) {
+    // The item's queries, half of each tile's rows a warp: all copies under way at once, by a few instructions in a loop.
+    bool q_turn = false;
+    auto load_queries = [&](const Walk& walk) {
+      constexpr bool kScaled = CODES && !std::is_same<T, __half>::value;
+      constexpr int kLanes = DPAD / 8, kRowsAtOnce = 32 / kLanes;        // a row's pieces of 16 bytes by neighbouring lanes
+      const int mine = (warp - L::kQueryWarp) * 64, c = lane % kLanes;
+      if (!wait(q_empty, q_turn ? 0u : 1u, p.status, 89)) return false;
+#pragma unroll 1
+      for (int s = 0; s < 2; ++s) {
+        if (s == 1 && (!walk.paired || !walk.has(0, 1))) break;
+        int64_t off[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int at = walk.row0(s) + mine + u * 32 + lane, place = at / p.x.group;
+          off[u] = -1;
+          if (place < walk.n) {
+            const int b = paged::ld_index(p.x.plan + p.x.at.order + walk.first + place);
+            if (b >= 0 && b < p.x.B) off[u] = b * p.q_batch + (walk.h * p.x.group + at - place * p.x.group) * p.q_head;
+          }
+        }
+        const uint32_t dst = ptx::smem_u32(sq) + s * L::kTileBytes;
+#pragma unroll 4
+        for (int i = 0; i < 64; i += kRowsAtOnce) {
+          const int r = i + lane / kLanes;
+          const int64_t from = __shfl_sync(0xffffffffu, i < 32 ? off[0] : off[1], r & 31);
+          copy16(dst + tile_at(mine + r, c), p.q + (from < 0 ? 0 : from) + c * 16, from < 0 || c * 8 >= p.c.D ? 0 : 16);
+        }
+        if constexpr (kScaled) {
+          // 2^(13 - exponent): the largest lands in [2^13, 2^14); zero, infinity and NaN stay as they are
+          asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 2
+          for (int i = 0; i < 64; i += kRowsAtOnce) {
+            const int r = mine + i + lane / kLanes;
+            uint4 v = lds128(dst + tile_at(r, c));       // this lane's own copy
+            uint32_t* w = &v.x;
+            float top = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u))));
+#pragma unroll
+            for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const int e = static_cast<int>(__float_as_uint(top) >> 23), up = top != 0.0f && e < 255 ? min(max(140 - max(e, 1), -125), 124) : 0;
+            const float f = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = pack16<__half>(__uint_as_float(w[k] << 16) * f, __uint_as_float(w[k] & 0xffff0000u) * f);
+            sts128(dst + tile_at(r, c), v);
+            if (c == 0) ups[(q_turn * 2 + s) * 128 + r] = static_cast<int8_t>(up);
+          }
+          ptx::fence_proxy_async();
+          ptx::mbar_arrive(q_full + s);
+        } else {
+          arrive_with_copies(q_full + s);
+        }
+      }
+      q_turn = !q_turn;
+      return true;
+    };
+    if (MAPS && (warp == L::kQueryWarp || warp == L::kQueryWarp + 1)) {
+      // ------------------------------------------------------------- queries
+      for (bool ok = true; walk.left > 0 && ok; walk.next(p)) ok = load_queries(walk);
+      asm volatile("cp.async.wait_all;" ::: "memory");       // no copy may be under way when the CTA ends
+    } else if (MAPS && warp == L::kLoadWarp) {
       // ------------------------------------------------------------- loads: a lane asks for a box of each tile
       const int boxes = kPrefixKeys >> p.box_shift, rows = p.box_rows;
       uint64_t* const arrival = CODES ? raw : full;
@@ -402,6 +474,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       bool ok = true;
       int n = 0;
       for (; walk.left > 0 && ok; walk.next(p)) {
+        if (warp == L::kQueryWarp || warp == L::kQueryWarp + 1) ok = load_queries(walk);
         const int count = walk.count(), tokens = walk.tokens;
         const bool named = walk.leader >= 0 && walk.leader < p.x.B && tokens <= p.c.capacity;
         const int32_t* line = p.c.table + (named ? walk.leader : 0) * p.c.table_stride;
@@ -556,6 +629,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
               v_at[s] = v_next[s];
             }
           }
+          if (j == count - 1 && leader && ok) ptx::tc_commit<1>(q_empty);
+          __syncwarp();
           if (more) ring.advance(paired ? 2 : (two ? 4 : 2));
         }
       }
@@ -574,9 +649,10 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
     bool ok = true;
     uint32_t phase = 0, o_phase = 0;
     int n = 0;                                         // tiles loaded so far
-    // The first pass is dry: it waits for nothing, writes nothing and fetches the code below from memory, which takes longer than a tile, under the sums
-    // of the line and the kernel in front.
-    bool dry = p.x.heads > 0;
+    // The first pass is dry: it waits for nothing, writes nothing and fetches the code below from memory, which takes longer than a tile, while the kernel in
+    // front still runs.
+    bool dry = p.x.heads > 0, q_turn = false;
+    constexpr bool kScaled = CODES && !std::is_same<T, __half>::value;
     Walk walk{};
     walk.left = 1, walk.tiles = 2;
     while (walk.left > 0 && ok) {
@@ -586,69 +662,22 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       bool mine = false;
       float sl = p.scale * 1.4426950408889634f;
       if (!dry) {
-      if (!walk.has(0, s)) {                           // no row (which nobody asks for), or no second tile of keys in this part
-        if (keeps && !walk.paired) p.x.stats[half * p.x.rows + r] = make_float2(-INFINITY, -1.0f);
-        n += walk.loaded(count);
-        walk.next(p);
-        continue;
-      }
-      // the row's query: products with those of the item before have ended (this tile's O was complete)
-      const int at = walk.row0(s) + r, place = at / p.x.group;
-      int b = -1, held = 0;
-      if (place < walk.n) b = paged::ld_index(p.x.plan + p.x.at.order + walk.first + place);
-      const bool there_is = b >= 0 && b < p.x.B;
-      if (there_is) held = paged::cached_tokens(p.c, b, 0x7fffffff);     // waited for behind the query's loads
-      {
-        // a row's pieces of 16 bytes by neighbouring lanes
-        constexpr int kLanes = DPAD / 8, kRowsAtOnce = 32 / kLanes, kRounds = 32 / kRowsAtOnce, kBatch = 8;
-        const int64_t off = there_is ? b * p.q_batch + (walk.h * p.x.group + at - place * p.x.group) * p.q_head : -1;
-        const int c = lane % kLanes;
-        constexpr bool kScaled = CODES && !std::is_same<T, __half>::value;
-        float back = 1.0f;
+        if (!walk.has(0, s)) {                           // no row (which nobody asks for), or no second tile of keys in this part
+          if (keeps && !walk.paired) p.x.stats[half * p.x.rows + r] = make_float2(-INFINITY, -1.0f);
+          n += walk.loaded(count);
+          walk.next(p);
+          q_turn = !q_turn;
+          continue;
+        }
+        const int at = walk.row0(s) + r, place = at / p.x.group;
+        if (place < walk.n) {
+          const int b = paged::ld_index(p.x.plan + p.x.at.order + walk.first + place);
+          mine = b >= 0 && b < p.x.B && paged::cached_tokens(p.c, b, 0x7fffffff) >= walk.tokens;
+        }
         if constexpr (CODES) sl *= paged::head_scale(p.c.k_amax, p.c.amax_stride, walk.h);
-        const uint32_t dst = ptx::smem_u32(sq) + (walk.paired ? s * L::kTileBytes : 0);
-#pragma unroll 1
-        for (int i0 = 0; i0 < kRounds; i0 += kBatch) {
-          uint4 u[kBatch];
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const int64_t row = __shfl_sync(0xffffffffu, off, (i0 + i) * kRowsAtOnce + lane / kLanes);
-            u[i] = make_uint4(0, 0, 0, 0);
-            if (row >= 0 && c * 8 < p.c.D) u[i] = ld_128(p.q + row + c * 16);
-          }
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            if constexpr (kScaled) {
-              uint32_t* w = &u[i].x;
-              float top = 0.0f;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u))));
-#pragma unroll
-              for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-              // 2^(13 - exponent): the largest lands in [2^13, 2^14); zero, infinity and NaN stay as they are
-              const int e = static_cast<int>(__float_as_uint(top) >> 23), up = min(max(140 - max(e, 1), -125), 124);
-              const float f = top != 0.0f && e < 255 ? __uint_as_float(static_cast<uint32_t>(up + 127) << 23) : 1.0f;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) w[k] = pack16<__half>(__uint_as_float(w[k] << 16) * f, __uint_as_float(w[k] & 0xffff0000u) * f);
-              const float of = __shfl_sync(0xffffffffu, f, lane % kRowsAtOnce * kLanes);     // this lane's row is one of round lane / kRowsAtOnce
-              if (lane / kRowsAtOnce == i0 + i) back = of;
-            }
-            // not paired: the second tile has the same rows as the first
-            if (s == 0 || walk.paired) sts128(dst + tile_at((warp & 3) * 32 + (i0 + i) * kRowsAtOnce + lane / kLanes, c), u[i]);
-          }
-        }
-        if constexpr (kScaled) sl *= 1.0f / back;
-        mine = there_is && held >= walk.tokens;
-        if (s == 0 || walk.paired) {
-          ptx::fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(q_full + s);
-        }
       }
-      }
-      sl = fmaxf(sl, 1e-30f);                          // 0 times a masked -inf would be NaN
       const bool works = dry || __any_sync(0xffffffffu, mine);
-      const uint64_t sl2 = pack2(sl, sl);
+      if (!kScaled) sl = fmaxf(sl, 1e-30f);            // 0 times a masked -inf would be NaN
       float m = -INFINITY, l = 0.0f;
       bool begun = false, any = false;
       for (int j = 0; j < count && ok; ++j) {
@@ -660,6 +689,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
             break;
           }
           phase ^= 1u;
+        }
+        if (kScaled && j == 0) {                       // the queries, and how far they were raised, are there as S is
+          sl = fmaxf(sl * __uint_as_float(static_cast<uint32_t>(127 - ups[(q_turn * 2 + (walk.paired ? s : 0)) * 128 + r]) << 23), 1e-30f);
         }
         ptx::tc_fence_after();
         const uint4 words = there[(n + (walk.paired ? j : 2 * j + s)) % L::kSlots];
@@ -701,7 +733,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
           }
           // the difference first: logits of 2^24 and more would lose the factor
           const float back = m == -INFINITY ? 0.0f : -m;
-          const uint64_t back2 = pack2(back, back), raise2 = pack2(kRaise<kHalf>, kRaise<kHalf>);
+          const uint64_t back2 = pack2(back, back), sl2 = pack2(sl, sl), raise2 = pack2(kRaise<kHalf>, kRaise<kHalf>);
           uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
           for (int c = 0; c < kPrefixKeys; c += 32) {
@@ -709,16 +741,10 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const uint64_t y = fma2(add2(pack2(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])), back2), sl2, raise2);
-              uint64_t v;
-              if ((e + 1) * kPolyPairs / 16 != e * kPolyPairs / 16) {
-                v = ex2_poly2(y);
-              } else {
-                const float2 a = unpack2(y);
-                v = pack2(exp2_fast(a.x), exp2_fast(a.y));
-              }
-              if (e & 1) sum1 = add2(sum1, v); else sum0 = add2(sum0, v);
-              const float2 a = unpack2(v);
-              pk[e] = pack16<E>(a.x, a.y);
+              const float2 a = unpack2(y);
+              const float px = exp2_fast(a.x), py = exp2_fast(a.y);
+              if (e & 1) sum1 = add2(sum1, pack2(px, py)); else sum0 = add2(sum0, pack2(px, py));
+              pk[e] = pack16<E>(px, py);
             }
             if (!dry) ptx::tmem_st_32x32_x16(ts + c / 2, pk);
             if (c == 32) {
@@ -745,6 +771,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
         dry = false;
         continue;
       }
+      q_turn = !q_turn;
       n += walk.loaded(count);
       if (ok && !ptx::mbar_wait(o_full + s, o_phase)) {
         timed_out(p.status, 97);
