@@ -110,6 +110,9 @@ class SharedPrefix:
         return [(list(m), t) for m, t in zip(members, tokens) if len(m) > 1 and t > 0]
 
     def update(self, members: list, tokens: list) -> None:
+        """Who shares what from now on, as given to the constructor; outside a capture, whose replays go by the plan as it is then."""
+        if self._plans and self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the plan of a shared prefix is made on the host: update it outside the capture")
         kept = self._kept(members, tokens)
         if len(kept) > self.groups or any(len(m) > self.largest for m, _ in kept):
             raise ValueError(f"made for {self.groups} groups of up to {self.largest} sequences, got groups of {[len(m) for m, _ in kept]}")
@@ -434,7 +437,7 @@ class PagedKvCache:
         for b in moved:
             self._give_back(self._pages[b][same[b]:])
         self._released = {b for b, p in enumerate(parents) if p in self._released}
-        self._tokens, self._new = [self._tokens[p] for p in parents], [0] * self.batch
+        self._tokens, self._new, self._rows = [self._tokens[p] for p in parents], [0] * self.batch, 0      # `grow` comes before the next `append`
         for b, pages in held.items():
             self._pages[b] = pages
         width = self.table.shape[1]
@@ -457,7 +460,7 @@ class PagedKvCache:
         for b, n in enumerate(keep):
             self._give_back(self._pages[b][n:])
             del self._pages[b][n:]
-        self._tokens, self._new = list(tokens), [0] * self.batch
+        self._tokens, self._new, self._rows = list(tokens), [0] * self.batch, 0
         self.table.masked_fill_(torch.arange(self.table.shape[1], device=self.table.device) >= both[1][:, None], -1)
         self.lens.copy_(both[0])
         for w in self.weights:

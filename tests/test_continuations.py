@@ -394,3 +394,23 @@ def test_a_plan_is_at_hand_for_a_first_step_that_is_captured(b200, monkeypatch):
     before = cache._prefix.plan(6, 2).clone()
     cache.truncate([9, 1, 9, 9])
     assert cache._prefix.tokens == 8 and not torch.equal(before, cache._prefix._plans[6, 2])
+
+
+def test_nothing_is_appended_behind_a_fork_or_a_cut_without_room(b200, monkeypatch):
+    """The newest rows are shared then, or gone."""
+    rows = torch.zeros(3, 2, 16, dtype=torch.bfloat16)
+    for change in (lambda c: c.fork([0, 0, 1]), lambda c: c.truncate([3, 2, 1])):
+        cache = b200.PagedKvCache(1, 3, 2, 16, pages=60, max_tokens=64, page_size=8, device="cpu")
+        cache.grow([5, 4, 3])
+        change(cache)
+        with pytest.raises(ValueError, match="expected the rows of 0 new tokens"):
+            cache.append(0, rows, rows)
+
+
+def test_a_plan_is_not_updated_in_a_capture(b200, monkeypatch):
+    prefix = b200.SharedPrefix([[0, 1]], [16], 4, device="cpu")
+    prefix.plan(4, 2)
+    prefix.device = torch.device("cuda")
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="outside the capture"):
+        prefix.update([[0, 1]], [8])
