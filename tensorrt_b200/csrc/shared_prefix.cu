@@ -10,15 +10,15 @@
 // Work: shared_prefix.cuh, a CTA to an SM, pieces from the plan (found by the CTAs themselves they cost 3 us in front of every call).  Two times four
 // warps run the softmax of a tile of 128 x 128 scores each, one thread to a row; one warp issues the products of both in turn, so that the tensor
 // cores work on one while the other is in its softmax; one asks for K and V rows, which pages scatter, box by box (tensor maps); two copy queries
-// (by the softmax's threads, through registers, that took 3 to 10 us in front of the first product: their code came from memory in front of it); codes
+// (by the softmax's threads, through registers, that took 3 to 10 us in front of the first product: their code came from memory first); codes
 // are widened to fp16, exactly, by four more warps in the place that they came to.  P takes the place of the scores that it came from in tensor memory.
 //
 // What bounds it.  Long prefixes: the softmax.  A step of 256 rows x 128 keys x 128 takes 2.4 us (1030 TFLOP/s): a warp needs 24 clocks for a pair of
 // scores, alone on its quarter of the SM, whatever the order of its instructions, and the two tiles take turns with 1800 clocks of it each.  Tried in
 // vain, at 64 sequences x 8 heads behind 32768 tokens (80 us): one exponential in eight, in four, in two on the FMA pipe (80, 87, 97 us), two
 // threads to a row (135 us: 104 registers spill).  Short ones: what stands in front of the first product, some 4 us (launch, code from memory, queries,
-// the first boxes), and the two kernels behind.  64 sequences behind 8192 tokens, 64 / 8 heads of 128: prefix 26 us, own keys 11, join 10, 43 in a row;
-// 16 behind 100000 tokens of codes: 79, 15 and 11, 102 in a row.
+// the first boxes), and the two kernels behind.  64 sequences behind 8192 tokens, 64 / 8 heads of 128: prefix 27 us, own keys 11, join 10, 42 in a row;
+// 16 behind 100000 tokens of codes: 77, 15 and 11, 99 in a row.
 //
 // Rounding: S, the softmax, O and the sums are 32-bit; P is rounded to 16 bits for the second product, an error of one rounding of each term,
 // of the size of the result's own.  fp16 (fp16 pages and codes): P is raised by 2^11, so that holds for terms down to 2^-25 of the largest.  bf16
@@ -324,24 +324,32 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
           copy16(dst + tile_at(mine + r, c), p.q + (from < 0 ? 0 : from) + c * 16, from < 0 || c * 8 >= p.c.D ? 0 : 16);
         }
         if constexpr (kScaled) {
-          // 2^(13 - exponent): the largest lands in [2^13, 2^14); zero, infinity and NaN stay as they are
+          // 2^(13 - exponent): the largest lands in [2^13, 2^14); zero, infinity and NaN stay as they are.  A lane has a row, so that no lane waits for
+          // another (a row's pieces by neighbouring lanes took 6 us for two tiles).
           asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll 2
-          for (int i = 0; i < 64; i += kRowsAtOnce) {
-            const int r = mine + i + lane / kLanes;
-            uint4 v = lds128(dst + tile_at(r, c));       // this lane's own copy
-            uint32_t* w = &v.x;
-            float top = 0.0f;
+          __syncwarp();
+#pragma unroll 1
+          for (int r = mine + lane; r < mine + 64; r += 32) {
+            __nv_bfloat162 tops = __float2bfloat162_rn(0.0f);
+#pragma unroll 4
+            for (int k = 0; k < kLanes; ++k) {
+              const uint4 v = lds128(dst + tile_at(r, k));
+              const auto* h = reinterpret_cast<const __nv_bfloat162*>(&v);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u))));
-#pragma unroll
-            for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+              for (int u = 0; u < 4; ++u) tops = __hmax2(tops, __habs2(h[u]));
+            }
+            const float top = __bfloat162float(__hmax(tops.x, tops.y));
             const int e = static_cast<int>(__float_as_uint(top) >> 23), up = top != 0.0f && e < 255 ? min(max(140 - max(e, 1), -125), 124) : 0;
             const float f = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+#pragma unroll 4
+            for (int k = 0; k < kLanes; ++k) {
+              uint4 v = lds128(dst + tile_at(r, k));
+              uint32_t* w = &v.x;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = pack16<__half>(__uint_as_float(w[k] << 16) * f, __uint_as_float(w[k] & 0xffff0000u) * f);
-            sts128(dst + tile_at(r, c), v);
-            if (c == 0) ups[(q_turn * 2 + s) * 128 + r] = static_cast<int8_t>(up);
+              for (int u = 0; u < 4; ++u) w[u] = pack16<__half>(__uint_as_float(w[u] << 16) * f, __uint_as_float(w[u] & 0xffff0000u) * f);
+              sts128(dst + tile_at(r, k), v);
+            }
+            ups[(q_turn * 2 + s) * 128 + r] = static_cast<int8_t>(up);
           }
           ptx::fence_proxy_async();
           ptx::mbar_arrive(q_full + s);
