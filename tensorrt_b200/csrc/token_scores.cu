@@ -16,6 +16,10 @@
 // of 64 groups of four threads the k-th largest has at least k elements at or above it, and elements at or above it lie in k groups only, a few
 // more than k as a rule.  Where they are too many (the largest all in one group's hands), a threshold that leaves enough and not too many is
 // searched by halving.
+//
+// Measured (us; the bytes at the copy rate): 2000 rows of 50001 bf16 logits, no list 43 (31); 200 rows of 100003 fp32 logits, most of them -inf, 8 of
+// the list 29 (12).  64 rows of 128000 bf16, 20 of the list 17 (2.5), and 3 rows of 32000, 6 of the list 8.8 (0.03): the chain of a row's load,
+// threshold, list, cut and exchange, and the code from memory.  CTAs that stay for the next row were slower.
 #include "common.cuh"
 #include "ex2.cuh"
 #include "tcgen05.cuh"

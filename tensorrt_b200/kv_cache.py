@@ -186,9 +186,10 @@ def _common(a: list, b: list) -> int:
 
 # Keys, times kv heads, that a batch's single-token attention has to read once instead of once more for each who shares them, before a cache takes the
 # kernels for shared prefixes.  Three launches cost what reading so much costs paged_attention.  Measured, paged / shared, in us: 8 kv heads x 4 of 128, 16
-# sequences behind 1024 tokens (0.12 M) 20.5 / 23.4, behind 4096 (0.49 M) 36.9 / 31.6; with 8-bit pages 22.4 / 26.7 and 36.9 / 36.0; 64 behind 256 (0.13 M)
-# 24.5 / 30.9, behind 1024 (0.52 M) 40.9 / 31.6; 2 kv heads x 4 of 64, 64 behind 1024 (0.13 M) 18.4 / 22.6, behind 4096 (0.52 M) 30.7 / 23.5.
-_SHARED_KEYS = 1 << 18
+# sequences behind 256 tokens (0.03 M) 18.4 / 19.5, behind 1024 (0.12 M) 22.5 / 21.5, behind 4096 (0.49 M) 37.8 / 27.6; with 8-bit pages 20.5 / 23.6,
+# 22.6 / 23.6 and 37.0 / 31.8; 64 behind 256 (0.13 M) 24.6 / 27.7, behind 1024 (0.52 M) 41.0 / 27.9; 2 kv heads x 4 of 64, 64 behind 1024 (0.13 M)
+# 18.5 / 21.5, behind 4096 (0.52 M) 30.8 / 21.5.
+_SHARED_KEYS = 1 << 17
 
 _WHOLE = "prompts are attended to as a whole: a sequence that brings tokens must hold no older ones"
 

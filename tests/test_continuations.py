@@ -367,9 +367,9 @@ def test_released_parents(model):
     assert m.cache.tokens() == [0, 0, 6, 1, 1]
 
 
-@pytest.mark.parametrize("n,shares", [((1 << 18) // 6, False), ((1 << 18) // 6 + 8, True)])
+@pytest.mark.parametrize("n,shares", [((1 << 17) // 6, False), ((1 << 17) // 6 + 8, True)])
 def test_what_is_shared_must_be_worth_it(b200, monkeypatch, n, shares):
-    """(sequences - 1) x tokens in full pages x kv heads, against 2^18."""
+    """(sequences - 1) x tokens in full pages x kv heads, against 2^17."""
     cache = b200.PagedKvCache(1, 4, 2, 16, pages=6000, max_tokens=n + 8, page_size=8, device="cpu")
     cache.grow([n, 0, 0, 0])
     assert not cache._shares
