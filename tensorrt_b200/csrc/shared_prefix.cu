@@ -13,12 +13,13 @@
 // (by the softmax's threads, through registers, that took 3 to 10 us in front of the first product: their code came from memory first); codes
 // are widened to fp16, exactly, by four more warps in the place that they came to.  P takes the place of the scores that it came from in tensor memory.
 //
-// What bounds it.  Long prefixes: the softmax.  A step of 256 rows x 128 keys x 128 takes 2.4 us (1030 TFLOP/s): a warp needs 24 clocks for a pair of
-// scores, alone on its quarter of the SM, whatever the order of its instructions, and the two tiles take turns with 1800 clocks of it each.  Tried in
-// vain, at 64 sequences x 8 heads behind 32768 tokens (80 us then, 74 now): one exponential in eight, in four, in two on the FMA pipe (80, 87, 97 us),
-// the maximum in the addend of the scaling instead of a subtraction in front (81), two threads to a row (135: 104 registers spill).  Short ones: what stands in front of the first product, some 4 us (launch, code from memory, queries,
-// the first boxes), and the two kernels behind.  64 sequences behind 8192 tokens, 64 / 8 heads of 128: prefix 27 us, own keys 11, join 10, 42 in a row;
-// 16 behind 100000 tokens of codes: 77, 15 and 11, 99 in a row.
+// What bounds it.  Long prefixes: the softmax.  A step of 256 rows x 128 keys x 128 takes 2.4 us (1030 TFLOP/s): a warp needs 24 clocks for a pair
+// of scores, alone on its quarter of the SM, whatever the order of its instructions, and the two tiles take turns with 1800 clocks of it each.
+// Tried in vain, at 64 sequences x 8 heads behind 32768 tokens (80 us then, 74 now): one exponential in eight, in four, in two on the FMA pipe (80,
+// 87, 97 us), the maximum in the addend of the scaling instead of a subtraction in front (81), two threads to a row (135: 104 registers spill).
+// Short ones: what stands in front of the first product, some 4 us (launch, code from memory, queries, the first boxes), and the two kernels behind.
+// 64 sequences behind 8192 tokens, 64 / 8 heads of 128: prefix 27 us, own keys 11, join 10, 42 in a row; 16 behind 100000 tokens of codes: 77, 15
+// and 11, 99 in a row.
 //
 // Rounding: S, the softmax, O and the sums are 32-bit; P is rounded to 16 bits for the second product, an error of one rounding of each term,
 // of the size of the result's own.  fp16 (fp16 pages and codes): P is raised by 2^11, so that holds for terms down to 2^-25 of the largest.  bf16
