@@ -325,8 +325,9 @@ __global__ void __launch_bounds__(kThreads, per_sm(TOP)) token_scores_kernel(con
           s[e & 1] += w, t[e & 1] = fmaf(w, y, t[e & 1]);
         }
       }
-      const float s1 = s[0] + s[1], grown = s1 * left * kLn2;
-      mine.s += s1 + grown, mine.t += fmaf(s1, left, t[0] + t[1]);
+      // sum of 2^(y + left) = 2^left s, and of 2^(y + left) (y + left) = 2^left (t + left s)
+      const float s1 = s[0] + s[1], grown = fmaf(left, kLn2, 1.0f);
+      mine.s = fmaf(s1, grown, mine.s), mine.t = fmaf(fmaf(s1, left, t[0] + t[1]), grown, mine.t);
     } else {                                         // products beyond the type, and no distribution
 #pragma unroll 1
       for (int k = 0; k < kVectors; ++k)
