@@ -309,11 +309,12 @@ __global__ void __launch_bounds__(kThreads, per_sm(TOP)) token_scores_kernel(con
     const float m = max_nan(mine.m, top);
     if (!(m == mine.m)) refer(mine, m, c);
     const float base = m == -INFINITY ? 0.0f : m;
-    // y = x c - base c in one step: base c is rounded once for all, and what that left out goes onto the sums behind
+    // y = x c - base c in one step: base c is rounded once for all, and what that left out goes onto the sums behind.  It is up to half a unit in the last
+    // place of base c: from 2^26 on more than 2, where 2^left and y + left would take their digits from the sums.  The difference first, then.
     const float shift = -base * c, left = fmaf(-base, c, -shift);
     float s[2] = {}, t[2] = {};
     // 0 times the -inf of a masked logit would be NaN: a floor under the logits, far enough below the maximum that its term is nothing
-    if (base < 1e30f && (base - E::kFloor) * c > 150.0f) {
+    if (fabsf(shift) < 0x1p26f && base < 1e30f && (base - E::kFloor) * c > 150.0f) {
 #pragma unroll
       for (int k = 0; k < kVectors; ++k) {
         if (at + k * kThreads >= mine_to) break;
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, per_sm(TOP)) token_scores_kernel(con
         }
       }
       // sum of 2^(y + left) = 2^left s, and of 2^(y + left) (y + left) = 2^left (t + left s)
-      const float s1 = s[0] + s[1], grown = fmaf(left, kLn2, 1.0f);
+      const float s1 = s[0] + s[1], grown = exp2_of(left);
       mine.s = fmaf(s1, grown, mine.s), mine.t = fmaf(fmaf(s1, left, t[0] + t[1]), grown, mine.t);
     } else {                                         // products beyond the type, and no distribution
 #pragma unroll 1

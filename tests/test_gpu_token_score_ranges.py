@@ -1,9 +1,13 @@
-"""`token_log_probs` over the whole range of scales and logits, against torch in 64 bits, by the bounds of tests/test_gpu_token_scores.py.
+"""`token_log_probs` over the whole range of scales and logits, against torch in 64 bits, by the bounds of tests/test_gpu_token_scores.py.  These count two
+roundings of z; a difference that is taken before the product has two more (the difference, and the product of the scale and the base's logarithm): together 4 x 2^-24 of
+|z|, whose mean over a distribution is at most 18 here, 2^-18 of S beside the 2^-17.5 of the exponentials and sums.
 """
+import math
+
 import pytest
 import torch
 
-from test_gpu_token_scores import check
+from test_gpu_token_scores import DTYPES, check, logits
 
 pytestmark = pytest.mark.gpu
 
@@ -18,3 +22,29 @@ def test_a_constant_changes_nothing(b200, by, size):
     check(b200, x + by, None, 1, 0.75)
     x[:, 4:] -= 50
     check(b200, x + by, x.argmax(1), 4)
+
+
+@pytest.mark.parametrize("scale", [1e4, 1e5, 1e6, 1e7, 1e9])
+@pytest.mark.parametrize("dt", DTYPES, ids=str)
+def test_scales_that_leave_the_largest_alone(b200, dt, scale):
+    """A temperature next to zero: the product of a logit and the scale is far beyond what 32 bits hold to a unit, differences are not."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x = logits(g, 24, 32000, dt).clone()
+    x[1, 31999] = x[1].max()                                # two maxima
+    x[2, :200] = x[2].max()
+    x[3] = x[3] / 1024
+    check(b200, x, x.float().argmax(1), 8, scale)
+    check(b200, x[:, :9], x[:, :9].float().argmin(1), 3, scale)
+
+
+@pytest.mark.parametrize("rows,size", [(3, 4), (2, 33000), (700, 5000)])
+@pytest.mark.parametrize("dt,large", [(torch.float32, 1e6), (torch.float32, 3e8), (torch.float32, -1e9), (torch.float32, 1e25), (torch.bfloat16, 1e6), (torch.bfloat16, -3e8),
+                                      (torch.float16, 6e4), (torch.float16, -6e4)], ids=str)
+def test_large_logits_close_to_one_another(b200, dt, large, rows, size):
+    at = torch.tensor(large, dtype=dt).float().item()
+    step = 2.0 ** (math.frexp(at)[1] - {torch.float32: 24, torch.bfloat16: 8, torch.float16: 11}[dt])      # of neighbouring values
+    i = torch.arange(size, device="cuda")
+    for x in (torch.full((size,), at, device="cuda"), at - (i % 5) * step, at - (i % 7 != 3) * step):
+        x = x.to(dt).expand(rows, size).contiguous()
+        for scale in (1.0, 1 / step, 300.0):
+            check(b200, x, torch.full((rows,), size - 1, device="cuda"), 3, torch.tensor(scale).item())
