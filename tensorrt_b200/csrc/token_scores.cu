@@ -313,8 +313,10 @@ __global__ void __launch_bounds__(kThreads, per_sm(TOP)) token_scores_kernel(con
     // place of base c: from 2^26 on more than 2, where 2^left and y + left would take their digits from the sums.  The difference first, then.
     const float shift = -base * c, left = fmaf(-base, c, -shift);
     float s[2] = {}, t[2] = {};
-    // 0 times the -inf of a masked logit would be NaN: a floor under the logits, far enough below the maximum that its term is nothing
-    if (fabsf(shift) < 0x1p26f && base < 1e30f && (base - E::kFloor) * c > 150.0f) {
+    // 0 times the -inf of a masked logit would be NaN: a floor under the logits, far enough below the maximum that its term is nothing, and not so far
+    // that its product is beyond the type
+    const float depth = (base - E::kFloor) * c;
+    if (fabsf(shift) < 0x1p26f && base < 1e30f && depth > 150.0f && depth < 1e38f) {
 #pragma unroll
       for (int k = 0; k < kVectors; ++k) {
         if (at + k * kThreads >= mine_to) break;

@@ -48,3 +48,18 @@ def test_large_logits_close_to_one_another(b200, dt, large, rows, size):
         x = x.to(dt).expand(rows, size).contiguous()
         for scale in (1.0, 1 / step, 300.0):
             check(b200, x, torch.full((rows,), size - 1, device="cuda"), 3, torch.tensor(scale).item())
+
+
+@pytest.mark.parametrize("scale", [1e9, 1e30])
+@pytest.mark.parametrize("dt", DTYPES, ids=str)
+def test_masked_logits_at_scales_that_leave_the_type(b200, dt, scale):
+    """The product of the scale and what stands in for a masked logit is an infinity; its term is nothing all the same."""
+    size = 9001
+    x = torch.full((5, size), -math.inf, device="cuda")
+    x[0, ::3] = 0.0                                         # equal ones: log of their number
+    x[1, 5:8] = 0.0
+    x[2, ::2] = -1.0 / scale
+    x[2, ::40] = 0.0
+    x[3, 4] = 2.0 ** -100
+    x[4] = torch.where(torch.arange(size, device="cuda") % 2 == 0, 0.0, torch.finfo(dt).min)
+    check(b200, x.to(dt), torch.full((5,), 4, device="cuda"), 3, torch.tensor(scale).item())
