@@ -116,8 +116,9 @@ __device__ __forceinline__ float exp2_of(float x) {
 struct Stats {
   float m, s, t;
 };
-__device__ __forceinline__ void refer(Stats& a, float m, float c) {      // to a maximum that is not below its own
-  const float d = fmaxf((a.m - m) * c, kLeast), f = exp2_of(d);
+// By the scale first: its product with log2 e may lie beyond the type.
+__device__ __forceinline__ void refer(Stats& a, float m, float scale) {  // to a maximum that is not below its own
+  const float d = fmaxf((a.m - m) * scale * kLog2e, kLeast), f = exp2_of(d);
   if (a.s > 0.0f) a.t = f * fmaf(a.s, d, a.t), a.s *= f;
   a.m = m;
 }
@@ -139,11 +140,11 @@ __device__ __forceinline__ void st_cluster(float* p, unsigned cta, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(ptx::mapa_u32(ptx::smem_u32(p), cta)), "f"(v) : "memory");
 }
 // Over the first `lanes` lanes of a warp, a power of two, in each of them: the maximum first, then two plain sums.
-__device__ __forceinline__ Stats over_lanes(Stats a, float c, int lanes) {
+__device__ __forceinline__ Stats over_lanes(Stats a, float scale, int lanes) {
   float m = a.m;
 #pragma unroll 1
   for (int d = lanes >> 1; d > 0; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
-  refer(a, m, c);
+  refer(a, m, scale);
 #pragma unroll 1
   for (int d = lanes >> 1; d > 0; d >>= 1) a.s += __shfl_xor_sync(0xffffffffu, a.s, d), a.t += __shfl_xor_sync(0xffffffffu, a.t, d);
   return a;
@@ -225,15 +226,15 @@ __device__ __noinline__ void list_piece(Lists& l, uint4 v, uint32_t place, uint6
   }
 }
 
-// Sums of 2^y and of 2^y y over a piece, y = (x - base) c.
+// Sums of 2^y and of 2^y y over a piece, y = (x - base) scale log2 e.
 template <typename T>
-__device__ __noinline__ float2 sums_of(uint4 v, float base, float c) {
+__device__ __noinline__ float2 sums_of(uint4 v, float base, float scale) {
   float f[Logits<T>::kPer];
   float2 sum = make_float2(0.0f, 0.0f);
   Logits<T>::widen(v, f);
 #pragma unroll
   for (int e = 0; e < Logits<T>::kPer; ++e) {
-    const float y = fmaxf((f[e] - base) * c, kLeast), w = exp2_of(y);
+    const float y = fmaxf((f[e] - base) * scale * kLog2e, kLeast), w = exp2_of(y);
     sum.x += w, sum.y = fmaf(w, y, sum.y);
   }
   return sum;
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, per_sm(TOP)) token_scores_kernel(con
       top = max_nan(top, tops[k]);
     }
     const float m = max_nan(mine.m, top);
-    if (!(m == mine.m)) refer(mine, m, c);
+    if (!(m == mine.m)) refer(mine, m, p.scale);
     const float base = m == -INFINITY ? 0.0f : m;
     // y = x c - base c in one step: base c is rounded once for all, and what that left out goes onto the sums behind.  It is up to half a unit in the last
     // place of base c: from 2^26 on more than 2, where 2^left and y + left would take their digits from the sums.  The difference first, then.
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, per_sm(TOP)) token_scores_kernel(con
 #pragma unroll 1
       for (int k = 0; k < kVectors; ++k)
         if (at + k * kThreads < mine_to) {
-          const float2 of = sums_of<T>(pick(v, k), base, c);
+          const float2 of = sums_of<T>(pick(v, k), base, p.scale);
           mine.s += of.x, mine.t += of.y;
         }
     }
@@ -386,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, per_sm(TOP)) token_scores_kernel(con
   }
   // ------------------------------------------------------------- the CTA's threads, then the cluster's CTAs
   if (p.parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // the first CTA is there
-  mine = over_lanes(mine, c, 32);
+  mine = over_lanes(mine, p.scale, 32);
   if (lane == 0) warps[0][warp] = mine.m, warps[1][warp] = mine.s, warps[2][warp] = mine.t;
   int listed = 0;
   if constexpr (TOP) listed = rank_list(lists_, held, p.top, part, p.parts > 1 ? 0 : -1);
@@ -395,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, per_sm(TOP)) token_scores_kernel(con
   Stats all{-INFINITY, 0.0f, 0.0f};
   if (TOP || writes) {
     if (lane < kThreads / 32) all = Stats{warps[0][lane], warps[1][lane], warps[2][lane]};
-    all = over_lanes(all, c, kThreads / 32);
+    all = over_lanes(all, p.scale, kThreads / 32);
   }
   if (p.parts > 1) {
     if (writes && lane == 0) {
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, per_sm(TOP)) token_scores_kernel(con
     if (part > 0) return;                            // nothing of it is read from here on
     all = Stats{-INFINITY, 0.0f, 0.0f};
     if (lane < p.parts) all = Stats{sums[0][lane], sums[1][lane], sums[2][lane]};
-    all = over_lanes(all, c, kMostParts);
+    all = over_lanes(all, p.scale, kMostParts);
   }
   all.m = __shfl_sync(0xffffffffu, all.m, 0), all.s = __shfl_sync(0xffffffffu, all.s, 0), all.t = __shfl_sync(0xffffffffu, all.t, 0);
   // a row without a finite maximum has no distribution

@@ -63,3 +63,14 @@ def test_masked_logits_at_scales_that_leave_the_type(b200, dt, scale):
     x[3, 4] = 2.0 ** -100
     x[4] = torch.where(torch.arange(size, device="cuda") % 2 == 0, 0.0, torch.finfo(dt).min)
     check(b200, x.to(dt), torch.full((5,), 4, device="cuda"), 3, torch.tensor(scale).item())
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=str)
+def test_the_largest_scales(b200, dt):
+    """Up to the type's largest: the scale times log2 e is beyond it, the products are not."""
+    size, scale = 3001, 1.75 * 2.0 ** 127
+    x = torch.zeros(4, size, device="cuda")
+    x[1, 1::2] = -math.inf
+    x[2, 1::2] = -2.0 ** -127
+    x[3, 7] = 1.0
+    check(b200, x.to(dt), torch.full((4,), 7, device="cuda"), 3, scale)
