@@ -4,6 +4,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime_api.h>
 
@@ -231,6 +232,8 @@ Tensor shared_prefix_attention(const Tensor& q_in, const Tensor& k_pages, const 
               a.B, ", ", Hq, " / ", a.c.heads, " heads, ", groups, " groups of up to ", largest, "), 16-byte aligned, got ", plan.sizes(), " of ", plan.scalar_type());
   Tensor out = at::empty(q_in.sizes(), q_in.options());
   if (a.B == 0) return out;
+  // the caller holds the groups, not the plan: its memory must outlive this call where they do not
+  if (groups > 0) c10::cuda::CUDACachingAllocator::recordStream(plan.storage().data_ptr(), at::cuda::getCurrentCUDAStream());
   Tensor q = rows_of_16(q_in);
   const int64_t strides[2] = {outer_stride(q, 0), outer_stride(q, 1)};
   const float sm = softmax_scale(scale, a.c.D, op);

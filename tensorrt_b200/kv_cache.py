@@ -10,7 +10,7 @@
 Pages are tensors [pages, kv heads, rows, D] (any strides with D contiguous) of float16, bfloat16, float8_e4m3fn or uint8 (FP8
 codes); token t of sequence b is row t % rows of page block_table[b, t // rows].  `lens` [B] counts the tokens of each sequence that
 are in the cache, the newest included, in every call.  Everything is enqueued on the current stream of the tensors' device, nothing
-synchronises, and the calls can be captured in a CUDA graph.
+synchronises (but the first call with a `SharedPrefix`, which waits for the copy of its plan), and the calls can be captured in a CUDA graph.
 """
 from __future__ import annotations
 
@@ -86,8 +86,8 @@ class SharedPrefix:
     through the line of the block table of the first of them.  It goes by sequences and stays valid as they grow.
 
     Groups of one sequence and prefixes of no token are left out: nothing is shared.  The first call of every pair of head counts makes a plan of the work
-    on the host, outside a stream capture, which later ones find on the device.  `update` says anew who shares what, in place, so that a
-    captured call goes by it; it takes up to `groups` groups of up to `largest` sequences (None: those given here)."""
+    on the host, outside a stream capture, and has it on the device before it returns, so that calls on any stream find it there.  `update` says anew who shares what,
+    in place, so that a captured call goes by it; it takes up to `groups` groups of up to `largest` sequences (None: those given here)."""
 
     def __init__(self, members: list, tokens: list, batch: int, device="cuda", groups: int | None = None, largest: int | None = None):
         if batch < 0 or batch > 65535:
@@ -110,7 +110,8 @@ class SharedPrefix:
         return [(list(m), t) for m, t in zip(members, tokens) if len(m) > 1 and t > 0]
 
     def update(self, members: list, tokens: list) -> None:
-        """Who shares what from now on, as given to the constructor; outside a capture, whose replays go by the plan as it is then."""
+        """Who shares what from now on, as given to the constructor; outside a capture, whose replays go by the plan as it is then.  Plans that calls
+        have made are written on the current stream, as a block table would be: calls and replays on other streams are ordered with that by the caller."""
         if self._plans and self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the plan of a shared prefix is made on the host: update it outside the capture")
         kept = self._kept(members, tokens)
@@ -130,6 +131,8 @@ class SharedPrefix:
         for heads, plan in self._plans.items():
             host = self._made(*heads)
             plan.copy_(host.pin_memory() if plan.is_cuda else host, non_blocking=True)
+            if plan.is_cuda:
+                plan.record_stream(torch.cuda.current_stream(plan.device))
 
     def _made(self, n_q: int, n_kv: int) -> torch.Tensor:
         lib, sizes = _lib.load(), (self.batch, n_q, n_kv, self.groups, self.largest)
@@ -146,7 +149,7 @@ class SharedPrefix:
             else:
                 if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("the plan of a shared prefix is made on the host: call once with these heads before the capture")
-                plan = _on_device(self._made(n_q, n_kv), self.device)
+                plan = _uploaded(self._made(n_q, n_kv), self.device)
             self._plans[n_q, n_kv] = plan
         return plan
 
@@ -173,6 +176,24 @@ def _on_device(values, device, dtype=torch.int32) -> torch.Tensor:
     """Values of the host as a tensor on `device`, without a wait for its stream (a copy from pageable memory is one)."""
     t = torch.as_tensor(values, dtype=dtype)
     return t.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else t
+
+
+_uploads: dict = {}
+
+
+def _uploaded(values: torch.Tensor, device) -> torch.Tensor:
+    """Values of the host as a tensor on `device` that is there for every stream.  The copy has a stream of its own: waiting for it does not wait for
+    the work of the current one."""
+    if device.type != "cuda":
+        return values
+    device = torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
+    stream = _uploads.get(device)
+    if stream is None:
+        stream = _uploads[device] = torch.cuda.Stream(device)
+    with torch.cuda.stream(stream):
+        t = values.pin_memory().to(device, non_blocking=True)
+    stream.synchronize()
+    return t
 
 
 def _common(a: list, b: list) -> int:
