@@ -128,7 +128,7 @@ class SharedPrefix:
         shared = [t for _, t in kept] + [0] * (self.groups - len(kept))
         self.tokens = max(shared, default=0)                                # of the longest prefix
         self._lists = [(ctypes.c_int32 * max(len(v), 1))(*v) for v in (flat, ends, shared)]
-        for heads, plan in self._plans.items():
+        for heads, plan in self._plans.items() if self.groups else ():     # of no groups: empty, whatever they are
             host = self._made(*heads)
             plan.copy_(host.pin_memory() if plan.is_cuda else host, non_blocking=True)
             if plan.is_cuda:
