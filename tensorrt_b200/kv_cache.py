@@ -98,6 +98,8 @@ class SharedPrefix:
         self.largest = max([len(m) for m, _ in kept], default=0) if largest is None else largest
         if not 0 <= self.groups <= batch or not 0 <= self.largest <= batch:
             raise ValueError(f"{self.groups} groups of up to {self.largest} sequences are not in a batch of {batch}")
+        if self.largest < 2:                                                # nobody to share with
+            self.groups = 0
         self.device, self._plans = torch.device(device), {}
         self.update(members, tokens)
 
