@@ -512,20 +512,31 @@ class PagedKvCache:
         return used
 
     def resize(self, pages: int) -> None:
-        """Pools of `pages` pages, at least those in use, in the place of the old ones: `k` and `v` are other tensors then, and captured steps are to be
-        captured again."""
+        """Pools of `pages` pages, at least those in use, in the place of the old ones, one pool after the other: `k` and `v` are other tensors then, and captured
+        steps are to be captured again.  Where memory runs out on the way this raises, and the cache has the smaller of the two numbers of pages."""
         used = sum(1 for n in self._uses if n)
         if pages < max(used, 1):
             raise ValueError(f"{used} pages are in use, {pages} are too few")
         self.compact()
-        for pools in (self.k, self.v):
-            for i, old in enumerate(pools):
-                new = torch.zeros((pages, *old.shape[1:]), dtype=old.dtype, device=old.device)
-                new.view(torch.uint8)[:used] = old.view(torch.uint8)[:used]
-                pools[i] = new
-                del old, new
-        self._uses = self._uses[:used] + [0] * (pages - used)
-        self._free = list(range(pages - 1, used - 1, -1))
+
+        def have(n):
+            self._uses = self._uses[:used] + [0] * (n - used)
+            self._free = list(range(n - 1, used - 1, -1))
+
+        least = min(pages, len(self._uses))
+        have(least)
+        try:
+            for pools in (self.k, self.v):
+                for i, old in enumerate(pools):
+                    new = torch.zeros((pages, *old.shape[1:]), dtype=old.dtype, device=old.device)
+                    new.view(torch.uint8)[:used] = old.view(torch.uint8)[:used]
+                    pools[i] = new
+                    del old, new
+        except BaseException:
+            for pools in (self.k, self.v):
+                pools[:] = [p[:least] for p in pools]
+            raise
+        have(pages)
 
     def _share(self) -> None:
         """Finds who shares what, behind each call that changes it: a captured step reads the plan where it is, as it does the table."""

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from test_continuations import model  # noqa: F401
+
 
 @pytest.mark.parametrize("batch,members,tokens", [(4, [], []), (4, [[0]], [64]), (4, [[1, 2]], [0]), (1, [], []), (0, [], [])])
 def test_an_update_where_nothing_is_shared(b200, batch, members, tokens):
@@ -25,3 +27,35 @@ def test_room_for_groups_of_nobody(b200, largest):
     prefix.update([[1]], [50])
     with pytest.raises(ValueError):
         prefix.update([[0, 1]], [50])
+
+
+@pytest.mark.parametrize("pages", [60, 14])
+@pytest.mark.parametrize("nth", [0, 1, 2, 3])
+def test_no_memory_for_the_pools_of_another_size(model, monkeypatch, pages, nth):  # noqa: F811
+    """A cache that could not be given all of its new pools has the smaller of the two numbers of pages in every layer, and goes on."""
+    m = model(pages=40, layers=2)
+    c = m.cache
+    m.grow([10, 2, 0, 5, 0])
+    c.release(3)
+    m.texts = [m.texts[0], m.texts[1], list(m.texts[0]), [], list(m.texts[0])]
+    c.fork([0, 1, 0, 3, 0])
+    made, zeros = [0], torch.zeros
+
+    def no_room(*a, **kw):
+        made[0] += 1
+        if made[0] > nth:
+            raise torch.OutOfMemoryError("no room")
+        return zeros(*a, **kw)
+
+    monkeypatch.setattr(torch, "zeros", no_room)
+    with pytest.raises(torch.OutOfMemoryError):
+        c.resize(pages)
+    monkeypatch.setattr(torch, "zeros", zeros)
+    assert [p.shape[0] for p in c.k + c.v] == [min(40, pages)] * 4 and len(c._uses) == min(40, pages)
+    m.check()
+    m.grow([2, 3, 1, 0, 1])                                  # with copies of the page that is shared and not full
+    c.compact()
+    m.check()
+    c.resize(30)
+    assert [p.shape[0] for p in c.k + c.v] == [30] * 4
+    m.grow([1, 1, 1, 4, 1])
