@@ -25,6 +25,7 @@
 // of the size of the result's own.  fp16 (fp16 pages and codes): P is raised by 2^11, so that holds for terms down to 2^-25 of the largest.  bf16
 // queries in front of codes are scaled by a power of two into fp16's range, which loses nothing above 2^-38 of a row's largest.
 #include <atomic>
+#include <cfloat>
 
 #include "gemm_host.cuh"
 #include "shared_prefix.cuh"
@@ -686,7 +687,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
         if constexpr (CODES) sl *= paged::head_scale(p.c.k_amax, p.c.amax_stride, walk.h);
       }
       const bool works = dry || __any_sync(0xffffffffu, mine);
-      if (!kScaled) sl = fmaxf(sl, 1e-30f);            // 0 times a masked -inf would be NaN
+      if (!kScaled) sl = fmaxf(sl, FLT_MIN);            // 0 times a masked -inf would be NaN
       float m = -INFINITY, l = 0.0f;
       bool begun = false, any = false;
       for (int j = 0; j < count && ok; ++j) {
@@ -700,7 +701,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
           phase ^= 1u;
         }
         if (kScaled && j == 0) {                       // the queries, and how far they were raised, are there as S is
-          sl = fmaxf(sl * __uint_as_float(static_cast<uint32_t>(127 - ups[(q_turn * 2 + (walk.paired ? s : 0)) * 128 + r]) << 23), 1e-30f);
+          sl = fmaxf(sl * __uint_as_float(static_cast<uint32_t>(127 - ups[(q_turn * 2 + (walk.paired ? s : 0)) * 128 + r]) << 23), FLT_MIN);
         }
         ptx::tc_fence_after();
         const uint4 words = there[(n + (walk.paired ? j : 2 * j + s)) % L::kSlots];
