@@ -208,10 +208,16 @@ def _common(a: list, b: list) -> int:
 
 
 # Keys, times kv heads, that a batch's single-token attention has to read once instead of once more for each who shares them, before a cache takes the
-# kernels for shared prefixes.  Three launches cost what reading so much costs paged_attention.  Measured, paged / shared, in us: 8 kv heads x 4 of 128, 16
-# sequences behind 256 tokens (0.03 M) 18.4 / 19.5, behind 1024 (0.12 M) 22.5 / 21.5, behind 4096 (0.49 M) 37.8 / 27.6; with 8-bit pages 20.5 / 23.6,
-# 22.6 / 23.6 and 37.0 / 31.8; 64 behind 256 (0.13 M) 24.6 / 27.7, behind 1024 (0.52 M) 41.0 / 27.9; 2 kv heads x 4 of 64, 64 behind 1024 (0.13 M)
-# 18.5 / 21.5, behind 4096 (0.52 M) 30.8 / 21.5.
+# kernels for shared prefixes.  Three launches, and the parts that they pass on, cost what reading so much costs paged_attention: for up to eight sequences; half
+# as much again for more of them, until paged_attention has 1024 sequences x kv heads to begin and end, which costs it as much; twice that with 8-bit
+# pages, whose rows and queries have to be converted first (three times from eight query heads of a kv head on) and where two sequences never gain.  Measured, paged / shared, in us at multiples of 2^17 keys x kv heads:
+#   8 kv heads x 4 of 128, 16 bits     4 sequences: 1 24.6 / 23.0, 2 32.9 / 27.7      16: 1 22.5 / 23.5, 1.5 24.6 / 24.2, 2 26.6 / 25.6
+#                                      64: 1 24.6 / 27.7, 1.5 26.7 / 27.6, 2 30.1 / 27.6, 4 41.0 / 28.3      256: 0.5 41.0 / 37.9, 1 41.0 / 37.9
+#   2 x 4 of 64, 16 bits               4: 1 22.6 / 21.5      16: 1 20.5 / 17.4      64: 1 18.5 / 21.3, 1.5 20.5 / 21.5, 3 26.6 / 21.5
+#   8 x 4 of 128, 8 bits               2: 1 30.3 / 29.7, 6 80.0 / 79.8      4: 1 24.6 / 25.6, 2 32.6 / 27.7      16: 1 22.6 / 23.7, 2 28.7 / 30.6, 3 33.1 / 31.5
+#                                      64: 1 23.0 / 35.8, 2 31.0 / 36.1, 3 36.4 / 36.1, 4 41.0 / 35.9      256: 1 41.2 / 46.0, 2 46.8 / 45.2
+#   8 x 8 of 128, 8 bits               64: 2 32.9 / 40.0, 4 43.0 / 43.9      256: 2 49.9 / 59.0, 3 55.3 / 60.2, 4 59.4 / 60.6
+#   1 x 4 of 64, 8 bits                2: 3 38.9 / 46.1, 6 59.0 / 69.8
 _SHARED_KEYS = 1 << 17
 
 _WHOLE = "prompts are attended to as a whole: a sequence that brings tokens must hold no older ones"
@@ -254,7 +260,7 @@ class PagedKvCache:
         self._free = list(range(pages - 1, -1, -1))
         self._pages: list = [[] for _ in range(batch)]     # of each sequence, in order
         self._uses = [0] * pages                           # sequences that a page is part of
-        self._prefix, self._shares, self._n_q = None, False, 0
+        self._prefix, self._shares, self._saved, self._n_q = None, False, (0, 0), 0      # `_saved`: keys that are read once, sequences that share them
         self._tokens = [0] * batch
         self._released: set = set()
         self._padded = None
@@ -357,7 +363,10 @@ class PagedKvCache:
         """Attention of the newest token of every sequence: q [batch, query heads, head_dim].  Without a window and without weights, what groups
         of forked sequences share is attended to once for all of a group, where that is much.  A captured step stays with the kernels that were
         taken when it was captured, and is right behind any later call."""
-        self._n_q = q.shape[1] if q.dim() == 3 else 0
+        n_q = q.shape[1] if q.dim() == 3 else 0
+        if n_q != self._n_q:
+            self._n_q = n_q
+            self._shares = self._worth()
         if self.weights[layer] is None and window <= 0 and self._shares:
             return shared_prefix_attention(q, self.k[layer], self.v[layer], self.table, self.lens, self._prefix, k_amax=self.k_amax[layer],
                                            v_amax=self.v_amax[layer], scale=scale)
@@ -538,6 +547,11 @@ class PagedKvCache:
             raise
         have(pages)
 
+    def _worth(self) -> bool:
+        keys, n = self._saved
+        many, codes = n > 8 and n * self.n_kv < 1024, self.k[0].element_size() == 1
+        return keys >= _SHARED_KEYS * (1.5 if many else 1) * ((3 if self._n_q >= 8 * self.n_kv else 2) if codes else 1)
+
     def _share(self) -> None:
         """Finds who shares what, behind each call that changes it: a captured step reads the plan where it is, as it does the table."""
         first: dict = {}
@@ -547,7 +561,9 @@ class PagedKvCache:
         members = [m for m in first.values() if len(m) > 1]
         # pages that all of a group have in common and that are full
         shared = [self.page_size * min(min(_common(self._pages[m[0]], self._pages[b]), self._tokens[b] // self.page_size) for b in m) for m in members]
-        self._shares = self.n_kv * sum((len(m) - 1) * t for m, t in zip(members, shared)) >= _SHARED_KEYS
+        codes = self.k[0].element_size() == 1
+        self._saved = self.n_kv * sum((len(m) - 1) * t for m, t in zip(members, shared) if len(m) > 2 or not codes), sum(len(m) for m in members)
+        self._shares = self._worth()
         if self._prefix is None and members:
             self._prefix = SharedPrefix([], [], self.batch, self.table.device, groups=self.batch // 2, largest=self.batch)
         if self._prefix is not None:

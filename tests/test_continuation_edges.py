@@ -59,3 +59,34 @@ def test_no_memory_for_the_pools_of_another_size(model, monkeypatch, pages, nth)
     c.resize(30)
     assert [p.shape[0] for p in c.k + c.v] == [30] * 4
     m.grow([1, 1, 1, 4, 1])
+
+
+@pytest.mark.parametrize("n,n_kv,tokens,codes,shares", [
+    (64, 8, 256, False, False), (64, 8, 272, False, False), (64, 8, 400, False, True), (16, 8, 1104, False, False), (16, 8, 1648, False, True), (64, 2, 1056, False, False),
+    (128, 8, 144, False, True), (8, 8, 2352, False, True), (2, 8, 16400, False, True), (8, 8, 2352, True, False), (8, 8, 4688, True, True), (64, 8, 528, True, False),
+    (64, 8, 800, True, True), (256, 8, 144, True, True), (256, 8, 112, True, False), (2, 1, 800000, True, False), (3, 1, 140000, True, True)])
+def test_the_choice_goes_by_what_was_measured(b200, n, n_kv, tokens, codes, shares):
+    amax = dict(dtype=torch.float8_e4m3fn, k_amax=[torch.ones(1)], v_amax=[torch.ones(1)]) if codes else {}
+    cache = b200.PagedKvCache(1, n, n_kv, 16, pages=1, max_tokens=tokens + 16, page_size=16, device="cpu", **amax)
+    cache._uses, cache._free = [0] * (tokens // 16 + 1), list(range(tokens // 16 + 1))      # numbers of pages only
+    cache.grow([tokens] + [0] * (n - 1))
+    cache.fork([0] * n)
+    assert cache._shares == shares
+
+
+def test_the_choice_goes_by_the_query_heads_too(b200, monkeypatch):
+    import tensorrt_b200.kv_cache as kv
+
+    calls = []
+    for name in ("shared_prefix_attention", "paged_attention"):
+        monkeypatch.setattr(kv, name, lambda q, *a, name=name, **kw: calls.append(name))
+    one = [torch.ones(1)]
+    cache = b200.PagedKvCache(1, 64, 8, 16, pages=1, max_tokens=1000, page_size=16, device="cpu", dtype=torch.float8_e4m3fn, k_amax=one, v_amax=one)
+    cache._uses, cache._free = [0] * 70, list(range(70))
+    cache.grow([800] + [0] * 63)
+    cache.fork([0] * 64)
+    for n_q in (32, 64, 8, 64):
+        cache.attend(0, torch.zeros(64, n_q, 16))
+        cache.fork([1] + [0] * 63)
+        cache.attend(0, torch.zeros(64, n_q, 16))
+    assert calls == ["shared_prefix_attention"] * 2 + ["paged_attention"] * 2 + ["shared_prefix_attention"] * 2 + ["paged_attention"] * 2
