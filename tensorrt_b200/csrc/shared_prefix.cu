@@ -98,6 +98,13 @@ struct Walk {
   __device__ __forceinline__ int row0(int s) const { return paired ? block * 256 + s * 128 : block * 128; }
   __device__ __forceinline__ int tile(int j, int s) const { return paired ? step + j : 2 * (step + j) + s; }
   __device__ __forceinline__ bool has(int j, int s) const { return s == 0 || (paired ? row0(1) < rows : tile(j, 1) < tiles); }
+  // rows of half s of a part; where row r of it lies, or a place behind all parts
+  __device__ __forceinline__ int half_rows(int s) const { return min(rows - row0(s), 128); }
+  __device__ __forceinline__ unsigned place_of(const PrefixParams& p, int cta, int s, int r) const {
+    if (item < 0 || item >= p.x.items || r >= half_rows(s)) return ~0u;
+    const int whole = paired ? min(rows - row0(0), 256) : 2 * half_rows(0);
+    return static_cast<unsigned>(paged::ld_index(p.x.plan + p.x.at.places + PlanLayout::kPlace * item) + cta * whole + s * half_rows(0) + r);
+  }
   // key tiles of the first `count` steps that are loaded
   __device__ __forceinline__ int loaded(int count) const { return paired ? count : 2 * count - (has(count - 1, 1) ? 0 : 1); }
   // of the group: place of its first sequence, sequences, tokens, leader
@@ -667,13 +674,12 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
     walk.left = 1, walk.tiles = 2;
     while (walk.left > 0 && ok) {
       const int count = walk.count();
-      const int64_t half = 2 * (static_cast<int64_t>(walk.item) + cta) + s;
-      const bool keeps = r < p.x.rows && walk.item >= 0 && walk.item < p.x.items;
       bool mine = false;
       float sl = p.scale * 1.4426950408889634f;
       if (!dry) {
         if (!walk.has(0, s)) {                           // no row (which nobody asks for), or no second tile of keys in this part
-          if (keeps && !walk.paired) p.x.stats[half * p.x.rows + r] = make_float2(-INFINITY, -1.0f);
+          const unsigned row = walk.place_of(p, cta, s, r);
+          if (!walk.paired && row < p.x.rows) p.x.stats[row] = make_float2(-INFINITY, -1.0f);
           n += walk.loaded(count);
           walk.next(p);
           q_turn = !q_turn;
@@ -783,6 +789,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       }
       q_turn = !q_turn;
       n += walk.loaded(count);
+      const unsigned row = walk.place_of(p, cta, s, r);
       if (ok && !ptx::mbar_wait(o_full + s, o_phase)) {
         timed_out(p.status, 97);
         ok = false;
@@ -790,9 +797,10 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
       o_phase ^= 1u;
       if (!ok) break;
       ptx::tc_fence_after();
-      if (keeps) p.x.stats[half * p.x.rows + r] = make_float2(m == -INFINITY ? m : m * sl - kRaise<kHalf>, mine && any ? l : -1.0f);
+      const bool keeps = row < p.x.rows;
+      if (keeps) p.x.stats[row] = make_float2(m == -INFINITY ? m : m * sl - kRaise<kHalf>, mine && any ? l : -1.0f);
       if (works) {
-        float* const dst = p.x.parts + (half * p.x.rows + r) * DPAD;
+        float* const dst = p.x.parts + static_cast<int64_t>(row) * DPAD;
 #pragma unroll 1
         for (int c = 0; c < DPAD / 32; ++c) {
           U32x8 o[4];
@@ -867,14 +875,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) join_kernel(const __grid_c
     const int own_ctas = static_cast<int>(__ldcg(p.x.own_lines + p.B + 1));
     const int64_t own_begin = __ldcg(p.x.own_lines + b);
     const int shared = paged::prefix_tokens(of.x, held), row = of.w + head, item = of.y + h * of.z + (row >> (paired ? 8 : 7)), r = row & 127;
-    int parts = 0, log2 = 0;
+    int parts = 0, apart = 0;
     int64_t at = 0;                                    // the first, in rows
-    if (shared > 0 && row >= 0 && item >= 0 && item < p.x.items && r < p.x.rows) {
+    if (shared > 0 && row >= 0 && item >= 0 && item < p.x.items) {
       const int32_t* const entry = p.x.plan + p.x.at.items + PlanLayout::kItem * item;
       const int c0 = min(max(paged::ld_index(entry), 0), paged::kPrefixCtas), ctas = min(max(paged::ld_index(entry + 1), 0), paged::kPrefixCtas - c0);
-      log2 = paired ? 0 : 1;
-      parts = ctas << log2;
-      at = (2 * (static_cast<int64_t>(item) + c0) + (paired ? (row >> 7) & 1 : 0)) * p.x.rows + r;
+      const int2 place = make_int2(paged::ld_index(p.x.plan + p.x.at.places + PlanLayout::kPlace * item), min(max(paged::ld_index(p.x.plan + p.x.at.places + PlanLayout::kPlace * item + 1), 0), 256));
+      parts = paired ? ctas : 2 * ctas, apart = paired ? place.y : place.y / 2;
+      at = static_cast<int64_t>(place.x) + c0 * place.y + (paired ? row & 128 : 0) + r;
+      if (at < 0 || at + static_cast<int64_t>(parts) * apart - apart >= p.x.rows) parts = 0;
     }
     // its own keys
     const int own_tiles = held > shared ? (held - shared + 15) / 16 : 1, own_block = head / p.x.own_rows;
@@ -892,7 +901,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) join_kernel(const __grid_c
         s[k].y = -1.0f;
         const int n = i + k;
         if (n >= to) continue;
-        const int64_t of = n < parts ? at + static_cast<int64_t>(log2 ? n : 2 * n) * p.x.rows : own_at + static_cast<int64_t>(n - parts) * p.x.own_rows;
+        const int64_t of = n < parts ? at + static_cast<int64_t>(n) * apart : own_at + static_cast<int64_t>(n - parts) * p.x.own_rows;
         s[k] = __ldcg((n < parts ? p.x.stats : p.x.own_stats) + of);
         if (d < DPAD) v[k] = __ldcg(reinterpret_cast<const float4*>((n < parts ? p.x.parts : p.x.own) + of * DPAD + d));
       }
@@ -977,20 +986,22 @@ bool sizes_of(int64_t B, int64_t Hq, int64_t heads, int64_t D, int64_t groups, i
       B > 65535 || Hq > 65535 || B * Hq > 0x3fffffffLL)
     return false;
   const int64_t group = Hq / heads, up = D <= 64 ? 64 : 128;
-  s->rows = largest * group < kPrefixRows ? largest * group : kPrefixRows;
   // sum over the groups of ceil(sequences * group / 128), each at most its own number of row tiles, all together one more than full ones each
   const int64_t most = groups * ((largest * group + kPrefixRows - 1) / kPrefixRows), all = B * group / kPrefixRows + groups;
   s->items = heads * (most < all ? most : all);
   if (s->items > 0x3fffffffLL) return false;
-  const int64_t slots = s->items + paged::kPrefixCtas;
+  // not paired: two halves of every row; and of one more part to each CTA, which begins within an item
+  const int64_t sharing = groups * largest < B ? groups * largest : B, part = 2 * largest * group < 256 ? 2 * largest * group : 256;
+  s->rows = 2 * sharing * Hq + paged::kPrefixCtas * part;
+  if (s->rows > 0x7fffffffLL) return false;
   const auto round = [](int64_t n) { return (n + 255) / 256 * 256; };
-  s->stats = round(2 * slots * s->rows * 8);
+  s->stats = round(s->rows * 8);
   int64_t own_slots;
   paged::own_shape(B, Hq, heads, &s->own_rows, &s->own_blocks, &own_slots);
   s->own_lines = round((B + 2) * 8);
   s->own_stats = round(own_slots * s->own_rows * 8);
   s->own = round(own_slots * s->own_rows * up * 4);
-  s->parts = round(2 * slots * s->rows * up * 4);
+  s->parts = round(s->rows * up * 4);
   s->bytes = s->stats + s->own_lines + s->own_stats + s->own + s->parts;
   return true;
 }
@@ -1071,7 +1082,7 @@ int b200q_shared_prefix_plan(const int32_t* members, const int32_t* cu, const in
   const int64_t longest = best[paired];
   if (longest > 0x3fffffffLL) return B200Q_ERR_INVALID;
   plan[l.head] = paired;
-  int64_t item = 0, room = 0, cta = -1;
+  int64_t item = 0, room = 0, cta = -1, place = 0;
   for (int64_t g = 0; g < groups; ++g) {
     const int64_t n = blocks(g, paired), all = steps(g, paired);
     const int32_t* const of = plan + l.groups + PlanLayout::kGroup * g;
@@ -1081,6 +1092,7 @@ int b200q_shared_prefix_plan(const int32_t* members, const int32_t* cu, const in
     }
     for (int64_t k = 0; k < heads * n; ++k, ++item) {
       int32_t* const entry = plan + l.items + PlanLayout::kItem * item;
+      const int64_t full = paired ? 256 : 128, left = (cu[g + 1] - cu[g]) * group - k % n * full, rows = (left < full ? left : full) * (paired ? 1 : 2);
       int64_t at = 0;
       bool begun = false;
       while (at < all) {
@@ -1095,8 +1107,12 @@ int b200q_shared_prefix_plan(const int32_t* members, const int32_t* cu, const in
         }
         const int64_t take = room < all - at ? room : all - at;
         mine[0] += static_cast<int32_t>(take), room -= take, at += take;
-        if (!begun) entry[0] = static_cast<int32_t>(cta), begun = true;
+        if (!begun) {
+          entry[0] = static_cast<int32_t>(cta), begun = true;
+          plan[l.places + PlanLayout::kPlace * item] = static_cast<int32_t>(place - cta * rows), plan[l.places + PlanLayout::kPlace * item + 1] = static_cast<int32_t>(rows);
+        }
         entry[1] = static_cast<int32_t>(cta - entry[0] + 1);
+        place += rows;
       }
     }
   }
@@ -1138,7 +1154,7 @@ int b200q_shared_prefix_attention(const void* q, int dtype, const int64_t* q_str
   const auto take = [&at](int64_t n) { char* const here = at; at += n; return here; };
   p.x.plan = plan, p.x.at = paged::plan_layout(B, groups, s.items);
   p.x.B = static_cast<int>(B), p.x.groups = static_cast<int>(groups), p.x.largest = static_cast<int>(largest);
-  p.x.heads = p.c.heads, p.x.group = static_cast<int>(Hq / p.c.heads), p.x.rows = static_cast<int>(s.rows), p.x.items = static_cast<int>(s.items);
+  p.x.heads = p.c.heads, p.x.group = static_cast<int>(Hq / p.c.heads), p.x.rows = static_cast<unsigned>(s.rows), p.x.items = static_cast<int>(s.items);
   p.x.stats = reinterpret_cast<float2*>(take(s.stats));
   p.x.own_rows = s.own_rows, p.x.own_blocks = s.own_blocks;
   p.x.own_lines = reinterpret_cast<int64_t*>(take(s.own_lines));

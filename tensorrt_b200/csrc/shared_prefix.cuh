@@ -38,18 +38,20 @@ __device__ __forceinline__ int4 ld_index4(const int32_t* p) {
 // scores at once: of 256 rows and the same 128 keys ("paired"), or, where that is more, of 128 rows and two times 128 keys.  An item is a group,
 // a kv head and a block of that many rows, its keys are steps of 128 or 256.  The steps of all items stand in one line, which the plan, made on the
 // host, cuts into a piece for each CTA, all as long as can be (with what it costs to begin another item); what a CTA computes of an item is
-// a part, of two halves: the rows of each of the two tiles, or the same rows with every other 128 keys.  Along the line either the item or the CTA
-// is another one from part to part, so item + CTA numbers the parts: their slots.
+// a part, of two halves: the rows of each of the two tiles, or the same rows with every other 128 keys.  Parts lie one behind the other in the order of the
+// line, each with as many rows as its item has (twice as many where it is not paired), so those of an item are equally far apart: what a call has to
+// have room for are the rows of its batch, and of one more item to each CTA, however many groups there may be.
 //
 // The plan: 32-bit integers, each table at a multiple of four of them.  What is read of it is checked against the sizes of the call where an address
 // hangs on it.
 struct PlanLayout {
-  int64_t head, sequences, order, groups, ctas, items, values;
+  int64_t head, sequences, order, groups, ctas, items, places, values;
   static constexpr int kHead = 4;                        // whether paired
   static constexpr int kSequence = 4;                    // tokens of its prefix (0: none), first item, items of a kv head, its first row there
   static constexpr int kGroup = 4;                       // place of its first sequence in `order`, sequences, tokens, the sequence whose line names them
   static constexpr int kCta = 12;                        // steps (0: none), item, group, kv head, block, first step; of the group as above
   static constexpr int kItem = 2;                        // first CTA, CTAs
+  static constexpr int kPlace = 2;                       // of an item: first row of the part that CTA 0 would have of it, rows of a part
 };
 inline PlanLayout plan_layout(int64_t B, int64_t groups, int64_t items) {
   const auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
@@ -60,7 +62,8 @@ inline PlanLayout plan_layout(int64_t B, int64_t groups, int64_t items) {
   l.groups = l.order + up(B);
   l.ctas = l.groups + PlanLayout::kGroup * groups;
   l.items = l.ctas + PlanLayout::kCta * kPrefixCtas;
-  l.values = l.items + up(PlanLayout::kItem * items);
+  l.places = l.items + up(PlanLayout::kItem * items);
+  l.values = l.places + up(PlanLayout::kPlace * items);
   return l;
 }
 
@@ -69,10 +72,10 @@ struct Prefix {
   PlanLayout at;
   int B, groups, largest;       // largest: sequences of a group, at most
   int heads, group;             // kv heads, query heads of each
-  int rows;                     // of half a part
+  unsigned rows;                // of all parts, at most
   int items;                    // at most
-  float* parts;                 // [items + CTAs][2][rows][D up to 64 or 128], unnormalised
-  float2* stats;                // [items + CTAs][2][rows] base-2 logarithm of what they are referred to, sum (-1: no key)
+  float* parts;                 // [rows][D up to 64 or 128], unnormalised
+  float2* stats;                // [rows] base-2 logarithm of what they are referred to, sum (-1: no key)
   // The keys that a sequence has to itself: items are a sequence, a kv head and a block of its query heads, tiles are of 16 keys, and every warp has
   // a piece of their line, which it finds itself: the lengths are on the device.
   int own_rows, own_blocks;     // query heads of an item, items of a kv head

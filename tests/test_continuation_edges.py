@@ -1,8 +1,10 @@
 """CPU checks of continuations at their edges: groups that hold nothing, calls that fail on the way."""
+import random
+
 import pytest
 import torch
 
-from test_continuations import model  # noqa: F401
+from test_continuations import CTAS, ITEM_STEPS, make_plan, model  # noqa: F401
 
 
 @pytest.mark.parametrize("batch,members,tokens", [(4, [], []), (4, [[0]], [64]), (4, [[1, 2]], [0]), (1, [], []), (0, [], [])])
@@ -90,3 +92,69 @@ def test_the_choice_goes_by_the_query_heads_too(b200, monkeypatch):
         cache.fork([1] + [0] * 63)
         cache.attend(0, torch.zeros(64, n_q, 16))
     assert calls == ["shared_prefix_attention"] * 2 + ["paged_attention"] * 2 + ["shared_prefix_attention"] * 2 + ["paged_attention"] * 2
+
+
+def places_of_parts(plan, members, tokens, batch, n_q, n_kv, groups, items_most):
+    """Rows of the scratch that each CTA writes, as the kernel finds them, and those that the join reads for each row of an item, as it finds them."""
+    up, group, paired = (lambda n: (n + 3) // 4 * 4), n_q // n_kv, plan[0]
+    ctas = 4 + 4 * batch + up(batch) + 4 * groups
+    items = ctas + 12 * CTAS
+    places = items + up(2 * items_most)
+    size = 256 if paired else 128
+    line = [(g, h, b) for g in range(len(members)) if tokens[g] for h in range(n_kv) for b in range(-(-len(members[g]) * group // size))]
+    tiles = lambda g: -(-tokens[g] // 128)  # noqa: E731
+    steps = lambda g: tiles(g) if paired else -(-tiles(g) // 2)  # noqa: E731
+    written, read = {}, {}
+    for c in range(CTAS):
+        left, item, _, _, _, step = plan[ctas + 12 * c:ctas + 12 * c + 6]
+        while left > 0:
+            g, h, b = line[item]
+            rows = len(members[g]) * group
+            half_rows = [min(rows - b * size - (s * 128 if paired else 0), 128) for s in range(2)]
+            whole = min(rows - b * size, 256) if paired else 2 * half_rows[0]
+            for s in range(2):
+                for r in range(half_rows[s]):
+                    at = plan[places + 2 * item] + c * whole + s * half_rows[0] + r
+                    assert at >= 0 and at not in written
+                    written[at] = item, b * size + (s * 128 if paired else 0) + r
+            left, step, item = left - min(left, steps(g) - step) - ITEM_STEPS, 0, item + 1
+    for i, (g, h, b) in enumerate(line):
+        base, rows = plan[places + 2 * i:places + 2 * i + 2]
+        c0, n = plan[items + 2 * i:items + 2 * i + 2]
+        for row in range(b * size, min((b + 1) * size, len(members[g]) * group)):
+            apart = rows if paired else rows // 2
+            for k in range(n if paired else 2 * n):
+                read[base + c0 * rows + (row & 128 if paired else 0) + (row & 127) + k * apart] = i, row
+    assert written == read
+    return max(written, default=-1) + 1
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_parts_have_places_of_their_own(b200, seed):
+    r = random.Random(seed)
+    n_kv = r.choice([1, 2, 8])
+    n_q, sizes = n_kv * r.choice([1, 2, 5, 8, 16]), [r.choice([1, 2, 3, 8, 40]) for _ in range(r.randint(1, 20))]
+    batch = sum(sizes) + r.randint(0, 3)
+    names = r.sample(range(batch), sum(sizes))
+    members = [[names.pop() for _ in range(n)] for n in sizes]
+    tokens = [r.choice([0, 1, 127, 128, 129, r.randint(1, 5000), r.randint(1, 100000)]) for _ in sizes]
+    groups, largest = (batch, batch) if r.random() < 0.5 else (len(members), max(sizes))
+    rc, plan = make_plan(members, tokens, batch, n_q, n_kv, groups, largest)
+    assert rc == 0
+    group = n_q // n_kv
+    items = n_kv * min(groups * -(-largest * group // 128), batch * group // 128 + groups)
+    rows = places_of_parts(plan, members, tokens, batch, n_q, n_kv, groups, items)
+    from tensorrt_b200 import _lib
+
+    room = 2 * min(groups * largest, batch) * n_q + CTAS * min(2 * largest * group, 256)
+    assert rows <= room
+    own = _lib.load().b200q_shared_prefix_workspace_bytes(batch, n_q, n_kv, 128, 0, 0)      # what there is beside parts and their sums
+    assert room * (512 + 8) <= _lib.load().b200q_shared_prefix_workspace_bytes(batch, n_q, n_kv, 128, groups, largest) - own <= room * (512 + 8) + 1024
+
+
+@pytest.mark.parametrize("batch,n_q,n_kv,most", [(64, 64, 8, 45), (256, 64, 8, 90), (1024, 64, 8, 260), (1024, 32, 32, 260)])
+def test_the_scratch_of_a_cache_goes_by_its_batch(b200, batch, n_q, n_kv, most):
+    """A cache has room for any groups: megabytes, and no more of them than its sequences' rows and a tile of each CTA need."""
+    from tensorrt_b200 import _lib
+
+    assert _lib.load().b200q_shared_prefix_workspace_bytes(batch, n_q, n_kv, 128, batch // 2, batch) <= most << 20
