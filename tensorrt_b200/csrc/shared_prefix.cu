@@ -1002,7 +1002,7 @@ bool sizes_of(int64_t B, int64_t Hq, int64_t heads, int64_t D, int64_t groups, i
   s->own_stats = round(own_slots * s->own_rows * 8);
   s->own = round(own_slots * s->own_rows * up * 4);
   s->parts = round(s->rows * up * 4);
-  s->bytes = s->stats + s->own_lines + s->own_stats + s->own + s->parts;
+  s->bytes = s->stats + s->own_lines + s->own_stats + s->own + s->parts + 256;      // the tables begin at a multiple of 256, parts are written 32 bytes at once
   return true;
 }
 
@@ -1150,7 +1150,7 @@ int b200q_shared_prefix_attention(const void* q, int dtype, const int64_t* q_str
   p.scale = scale;
   p.status = gemm::device_status_word();
   if (p.status == nullptr) return B200Q_ERR_CUDA;
-  char* at = static_cast<char*>(workspace);
+  char* at = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t{255});
   const auto take = [&at](int64_t n) { char* const here = at; at += n; return here; };
   p.x.plan = plan, p.x.at = paged::plan_layout(B, groups, s.items);
   p.x.B = static_cast<int>(B), p.x.groups = static_cast<int>(groups), p.x.largest = static_cast<int>(largest);

@@ -1,5 +1,7 @@
 """Attention over shared prefixes where its arithmetic or its loads are at an edge, against the 64-bit restatement of tests/test_gpu_shared_prefix.py and by its
 bounds."""
+import ctypes
+
 import pytest
 import torch
 
@@ -59,3 +61,28 @@ def test_the_largest_logit_takes_all(b200, dt, pt, size):
     assert clear.float().mean() > 0.9
     out = attend(b200, case, q, kp, vp, ka, va, table, lens, members, tokens, scale=size)
     check_out(out[clear], ref[clear], mass[clear])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("at", [0, 16, 32, 240])
+def test_a_workspace_at_any_multiple_of_16_bytes(b200, d, at):
+    """As callers of the C entry may have it; every buffer has exactly the bytes that are asked for, and what stands around them stays."""
+    from tensorrt_b200 import _lib
+
+    lib, i64 = _lib.load(), ctypes.c_int64
+    case = ([(300, [5, 9, 30])], [50], 2, 4, d, 16, torch.bfloat16, torch.bfloat16, "hnd", False)
+    q, kp, vp, _, _, table, lens, members, tokens = made(case)
+    q, n, prefix = q.contiguous(), on_device(lens), b200.SharedPrefix(members, tokens, 4)
+    want = b200.shared_prefix_attention(q, kp, vp, table, n, prefix)
+    strides = (i64 * 3)(*kp.stride()[:3])
+    cache = _lib.PagedCache(kp.data_ptr(), vp.data_ptr(), 2, 16, kp.shape[0], 2, d, strides, (i64 * 3)(*vp.stride()[:3]), None, None, 0)
+    size = lib.b200q_shared_prefix_workspace_bytes(4, 8, 2, d, 1, 3)
+    held = torch.full((1024 + size,), 0xA5, dtype=torch.uint8, device="cuda")
+    start = -held.data_ptr() % 256 + 256 + at
+    head = torch.zeros(lib.b200q_paged_attention_workspace_bytes(), dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(q)
+    rc = lib.b200q_shared_prefix_attention(q.data_ptr(), 2, (i64 * 2)(*q.stride()[:2]), ctypes.byref(cache), table.data_ptr(), table.stride(0), table.shape[1], n.data_ptr(), 4, 8,
+                                           prefix.plan(8, 2).data_ptr(), 1, 3, d ** -0.5, out.data_ptr(), head.data_ptr(), head.numel(), held.data_ptr() + start, size,
+                                           torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(out, want)
+    assert (held[:start] == 0xA5).all() and (held[start + size:] == 0xA5).all()
