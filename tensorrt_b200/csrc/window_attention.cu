@@ -39,6 +39,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <cfloat>
 
 #include "common.cuh"
 #include "ex2.cuh"
@@ -232,7 +233,7 @@ __device__ __noinline__ void join_rows(const WindowParams& p, const float* part,
   constexpr int kRows = 8 / SPLITS, kPerWarp = kTileRows / SPLITS / 4;
   const int lane = threadIdx.x & 31, first = static_cast<int>(ptx::cluster_ctarank()) * (kTileRows / SPLITS) + (threadIdx.x >> 5) * kPerWarp;
   const int d = min(lane * 4, DPAD - 4);
-  const float sl = fmaxf(p.scale * 1.4426950408889634f, 1e-30f);
+  const float sl = fmaxf(p.scale * 1.4426950408889634f, FLT_MIN);
   unsigned bad = 0;
 #pragma unroll 1
   for (int r0 = 0; r0 < kPerWarp; r0 += kRows) {
@@ -449,7 +450,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     const int q0 = s ? w.q0[NQ - 1] : w.q0[0], lowest = s ? w.lowest[NQ - 1] : w.lowest[0], highest = s ? w.highest[NQ - 1] : w.highest[0];
     const int h = (s ? w.head[NQ - 1] : w.head[0]) + (r >> p.rp_log2), i = q0 + (r & (p.rp - 1));
     const int at = i < w.nq ? i + w.off : -1;                         // position; < 0: sees nothing
-    const float sl = fmaxf(p.scale * 1.4426950408889634f, 1e-30f);    // 0 times a masked -inf would be NaN
+    const float sl = fmaxf(p.scale * 1.4426950408889634f, FLT_MIN);    // 0 times a masked -inf would be NaN
     const uint64_t sl2 = pack2(sl, sl);
     float m = -INFINITY, l = 0.0f;
     bool ok = true, begun = false;
