@@ -28,6 +28,8 @@
 
 #include <array>
 #include <cmath>
+#include <map>
+#include <mutex>
 #include <optional>
 #include <vector>
 
@@ -653,6 +655,33 @@ PyObject* py_shared_prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n
   END_HANDLE_TH_ERRORS
 }
 
+// Values of the host as a tensor of device `index` that every stream finds written: the copy has a stream of its own, and waiting for it does not wait for
+// the work of the current one.
+PyObject* py_uploaded(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t index;
+  TORCH_CHECK_VALUE(n == 2 && THPVariable_CheckExact(a[0]) && ints(a + 1, 1, &index), "uploaded: values and the index of a device expected");
+  const Tensor values = THPVariable_Unpack(a[0]);
+  TORCH_CHECK_VALUE(values.is_cpu() && values.is_contiguous(), "uploaded: contiguous values of the host expected");
+  Tensor t;
+  {
+    pybind11::gil_scoped_release no_gil;
+    static std::mutex mu;
+    static auto* streams = new std::map<int64_t, c10::cuda::CUDAStream>;      // not destroyed: the context may be gone by then
+    const auto device = static_cast<c10::DeviceIndex>(index);
+    std::lock_guard<std::mutex> lk(mu);
+    auto at = streams->find(index);
+    if (at == streams->end()) at = streams->emplace(index, c10::cuda::getStreamFromPool(false, device)).first;
+    c10::cuda::CUDAStreamGuard guard(at->second);
+    t = at::empty(values.sizes(), values.options().device(at::Device(at::kCUDA, device)));
+    TORCH_CHECK(cudaMemcpyAsync(t.data_ptr(), values.data_ptr(), values.nbytes(), cudaMemcpyHostToDevice, at->second.stream()) == cudaSuccess &&
+                    cudaStreamSynchronize(at->second.stream()) == cudaSuccess,
+                "uploaded: the copy failed: ", cudaGetErrorString(cudaGetLastError()));
+  }
+  return THPVariable_Wrap(t);
+  END_HANDLE_TH_ERRORS
+}
+
 // A list of plain tensors, of integers.
 bool tensor_list(PyObject* o, std::vector<Tensor>* out) {
   if (!PyList_CheckExact(o)) return false;
@@ -728,6 +757,7 @@ PyMethodDef methods[] = {
      "q, k, v, q_lens, k_lens, scale, window, sinks -> tensor like q or None"},
     {"shared_prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_shared_prefix_attention)), METH_FASTCALL,
      "q, k_pages, v_pages, block_table, lens, plan, k_amax, v_amax, scale, groups, largest -> tensor like q or None"},
+    {"uploaded", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_uploaded)), METH_FASTCALL, "values, device index -> tensor, written for every stream"},
     {"paged_copy", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_copy)), METH_FASTCALL,
      "k_pages, v_pages, src, dst, rows -> whether it was taken"},
     {"token_log_probs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_token_log_probs)), METH_FASTCALL,

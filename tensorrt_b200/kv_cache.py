@@ -151,7 +151,9 @@ class SharedPrefix:
             else:
                 if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("the plan of a shared prefix is made on the host: call once with these heads before the capture")
-                plan = _uploaded(self._made(n_q, n_kv), self.device)
+                plan = self._made(n_q, n_kv)
+                if self.device.type == "cuda":              # on a stream of its own, waited for: the next call may be on any
+                    plan = _native.uploaded(plan, torch.cuda.current_device() if self.device.index is None else self.device.index)
             self._plans[n_q, n_kv] = plan
         return plan
 
@@ -178,24 +180,6 @@ def _on_device(values, device, dtype=torch.int32) -> torch.Tensor:
     """Values of the host as a tensor on `device`, without a wait for its stream (a copy from pageable memory is one)."""
     t = torch.as_tensor(values, dtype=dtype)
     return t.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else t
-
-
-_uploads: dict = {}
-
-
-def _uploaded(values: torch.Tensor, device) -> torch.Tensor:
-    """Values of the host as a tensor on `device` that is there for every stream.  The copy has a stream of its own: waiting for it does not wait for
-    the work of the current one."""
-    if device.type != "cuda":
-        return values
-    device = torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
-    stream = _uploads.get(device)
-    if stream is None:
-        stream = _uploads[device] = torch.cuda.Stream(device)
-    with torch.cuda.stream(stream):
-        t = values.pin_memory().to(device, non_blocking=True)
-    stream.synchronize()
-    return t
 
 
 def _common(a: list, b: list) -> int:
