@@ -511,7 +511,7 @@ int b200q_paged_copy(void* const* pools, int64_t n_pools, int64_t num_pages, int
                      int64_t pairs, b200q_stream_t stream);
 
 /* b200q_paged_attention (no window, no weights) where groups of sequences share the pages of a prefix: the keys of the prefix are
- * attended to by all of a group at once, and read once for up to 128 of its rows.
+ * attended to by all of a group at once, and read once for each block of 256 of its rows (of 128, where the plan finds that shorter).
  * The plan says who shares what: group g holds the sequences members[cu[g]] .. members[cu[g + 1] - 1] (cu[0] = 0; a group may be empty),
  * whose first tokens[g] tokens are the same.  These are found through the line of block_table of the group's FIRST sequence; the keys
  * behind them, and all keys of a sequence that is in no group, through its own.  A sequence that holds fewer tokens than

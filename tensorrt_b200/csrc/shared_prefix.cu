@@ -168,13 +168,6 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
 __device__ __forceinline__ void widen(uint32_t v, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(v));
 }
-// 4-D tiled load into this CTA's shared memory, completion on this CTA's own barrier.
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int32_t x, int32_t y, int32_t z, int32_t w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(ptx::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
 // Place of 16 bytes (piece c of a row) in a tile of 128 rows: boxes of 64 elements, 128-byte swizzle.
 __device__ __forceinline__ uint32_t tile_at(int row, int c) {
   return static_cast<uint32_t>((c >> 3) * (128 * 128) + row * 128 + (((c & 7) ^ (row & 7)) * 16));
@@ -194,7 +187,7 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
 // widens it need have read it.  Rows without a key become zeros.  `first`: of the warp's 32 rows; `there`: a bit for each of them.
 // Eight lanes to a row, 8 codes each of either half of it; odd rows take the halves in the other order, so that two rows meet no bank twice.
 template <int DPAD>
-__device__ __forceinline__ void widen_rows(uint32_t tile, int first, int D, uint32_t there) {
+__device__ __forceinline__ void widen_rows(uint32_t tile, int first, uint32_t there) {
   constexpr int kBatch = 4;
   const int lane = threadIdx.x & 31, c = lane & 7, turn = DPAD == 128 ? (lane >> 3) & 1 : 0;
   const uint32_t codes = tile + (DPAD == 128 ? 128 * 128 : 0);
@@ -476,7 +469,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CU
               break;
             }
             const uint32_t* const words = reinterpret_cast<const uint32_t*>(there + (n + (tiles == 2 ? i & 1 : 0)) % L::kSlots);
-            widen_rows<DPAD>(ptx::smem_u32(ring_at + ring.stage * L::kTileBytes), (warp - L::kWidenWarp) * 32, p.c.D, words[warp - L::kWidenWarp]);
+            widen_rows<DPAD>(ptx::smem_u32(ring_at + ring.stage * L::kTileBytes), (warp - L::kWidenWarp) * 32, words[warp - L::kWidenWarp]);
             ptx::fence_proxy_async();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(full + ring.stage);

@@ -5,9 +5,9 @@
 // Every logit is read once and takes part in one exponential and some ten other operations, so the memory binds the kernel, with the
 // special-function unit not far behind for 16-bit logits (16 exponentials a clock, 12 logits a clock at the copy rate).
 //
-// A row is one CTA's, or, where there are few rows, a cluster's of up to eight.  A CTA takes 256 x 4 pieces of 16 bytes at once, the next ones on
-// their way meanwhile, and keeps them in registers.  A thread follows its own maximum, sum S and
-// sum of exp(z) z, so that for these nothing but the end of the row makes threads wait for one another.  The CTAs of a cluster write what they have found
+// A row is one CTA's, or, where there are few rows, a cluster's of up to eight.  A CTA takes 256 x 8 pieces of 16 bytes at once, into registers, and asks
+// for the next ones when it is done with them: its loads and its work take turns, which the two or three other CTAs of its SM hide in part.  A thread follows its own
+// maximum, sum S and sum of exp(z) z, so that for these nothing but the end of the row makes threads wait for one another.  The CTAs of a cluster write what they have found
 // into the first one's shared memory.  What runs once a row stands in loops and functions: a short call waits for its code (50 KB of it: 10 us).
 //
 // The most likely tokens.  An element is a number of 64 bits, unlike any other of its row: the logit in the order of numbers (NaN above all), then
@@ -17,12 +17,14 @@
 // more than k as a rule.  Where they are too many (the largest all in one group's hands), a threshold that leaves enough and not too many is
 // searched by halving.
 //
-// Measured (us; the bytes at the copy rate): 2000 rows of 50001 bf16 logits, no list 43 (31); 200 rows of 100003 fp32 logits, most of them -inf, 8 of
-// the list 29 (12).  64 rows of 128000 bf16, 20 of the list 17 (2.5), and 3 rows of 32000, 6 of the list 8.8 (0.03): the chain of a row's load,
-// threshold, list, cut and exchange, and the code from memory.  CTAs that stay for the next row were slower.
+// Measured (us; the bytes at the copy rate): 2000 rows of 50001 bf16 logits, no list 44 (31); 200 rows of 100003 fp32 logits, most of them -inf, 8 of
+// the list 29 (12): four and seven tiles to a CTA, with nothing on its way while one is worked on.  64 rows of 128000 bf16, 20 of the list 17 (2.5), two
+// tiles to a CTA of a cluster of four, and 3 rows of 32000, 6 of the list 8.9 (0.03): the chain of a row's load, threshold, list, cut and exchange, and the code
+// from memory.  CTAs that stay for the next row were slower.
+// The difference taken first (scale x largest logit from 2^26 / log2 e on): 1.7, 1.4 and 1.2 times the time of the first three.
 #include "common.cuh"
 #include "ex2.cuh"
-#include "tcgen05.cuh"
+#include "softmax_tc.cuh"
 
 namespace b200q {
 namespace {
@@ -106,19 +108,13 @@ struct Logits<float> {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLeast = -200.0f;                   // 2^-200 is zero here, and its product with what it belongs to too
 
-__device__ __forceinline__ float exp2_of(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Maximum, sum of 2^y and sum of 2^y y with y = (x - maximum) * scale * log2 e.
 struct Stats {
   float m, s, t;
 };
 // By the scale first: its product with log2 e may lie beyond the type.
 __device__ __forceinline__ void refer(Stats& a, float m, float scale) {  // to a maximum that is not below its own
-  const float d = fmaxf((a.m - m) * scale * kLog2e, kLeast), f = exp2_of(d);
+  const float d = fmaxf((a.m - m) * scale * kLog2e, kLeast), f = exp2_fast(d);
   if (a.s > 0.0f) a.t = f * fmaf(a.s, d, a.t), a.s *= f;
   a.m = m;
 }
@@ -234,7 +230,7 @@ __device__ __noinline__ float2 sums_of(uint4 v, float base, float scale) {
   Logits<T>::widen(v, f);
 #pragma unroll
   for (int e = 0; e < Logits<T>::kPer; ++e) {
-    const float y = fmaxf((f[e] - base) * scale * kLog2e, kLeast), w = exp2_of(y);
+    const float y = fmaxf((f[e] - base) * scale * kLog2e, kLeast), w = exp2_fast(y);
     sum.x += w, sum.y = fmaf(w, y, sum.y);
   }
   return sum;
@@ -325,12 +321,12 @@ __global__ void __launch_bounds__(kThreads, per_sm(TOP)) token_scores_kernel(con
         E::widen(E::floored(v[k]), f);
 #pragma unroll
         for (int e = 0; e < E::kPer; ++e) {
-          const float y = fmaf(f[e], c, shift), w = exp2_of(y);
+          const float y = fmaf(f[e], c, shift), w = exp2_fast(y);
           s[e & 1] += w, t[e & 1] = fmaf(w, y, t[e & 1]);
         }
       }
       // sum of 2^(y + left) = 2^left s, and of 2^(y + left) (y + left) = 2^left (t + left s)
-      const float s1 = s[0] + s[1], grown = exp2_of(left);
+      const float s1 = s[0] + s[1], grown = exp2_fast(left);
       mine.s = fmaf(s1, grown, mine.s), mine.t = fmaf(fmaf(s1, left, t[0] + t[1]), grown, mine.t);
     } else {                                         // products beyond the type, and no distribution
 #pragma unroll 1

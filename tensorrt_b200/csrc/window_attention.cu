@@ -106,13 +106,6 @@ __device__ __forceinline__ int length_of(const int32_t* lens, int b, int most) {
   return min(max(n, 0), most);
 }
 
-// 4-D tiled load into this CTA's shared memory, completion on this CTA's own barrier.
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int32_t x, int32_t y, int32_t z, int32_t w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(ptx::smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(ptx::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
 __device__ __forceinline__ float2 ld_cluster_f2(const float2* p, unsigned cta) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(ptx::mapa_u32(ptx::smem_u32(p), cta)) : "memory");
@@ -328,7 +321,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
     if (lane == 0 && w.tiles > 0) {
       auto load_q = [&](int s, int q0, int head) {
         ptx::mbar_arrive_expect_tx(q_full + s, L::kTileBytes);
-        for (int x = 0; x < L::kBoxes; ++x) tma_load_4d(sq + s * L::kTileBytes + x * L::kBoxBytes, &tq, q_full + s, x * 64, q0, head, w.b);
+        for (int x = 0; x < L::kBoxes; ++x) tma_load_4d(ptx::smem_u32(sq + s * L::kTileBytes + x * L::kBoxBytes), &tq, q_full + s, x * 64, q0, head, w.b);
       };
       load_q(0, w.q0[0], w.head[0]);
       int st = 0, issued = 0;
@@ -344,7 +337,7 @@ window_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CU
           }
           ptx::mbar_arrive_expect_tx(full + st, L::kTileBytes);
           for (int x = 0; x < L::kBoxes; ++x)
-            tma_load_4d(ring + st * L::kTileBytes + x * L::kBoxBytes, kv == 0 ? &tk : &tv, full + st, x * 64, row, w.kv_head, w.b);
+            tma_load_4d(ptx::smem_u32(ring + st * L::kTileBytes + x * L::kBoxBytes), kv == 0 ? &tk : &tv, full + st, x * 64, row, w.kv_head, w.b);
           if (++issued == 1 && NQ == 2) load_q(1, w.q0[NQ - 1], w.head[NQ - 1]);      // the first product waits for the first query tile and the first keys
           if (++st == L::kStages) st = 0, ph ^= 1u;
         }

@@ -162,7 +162,7 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
                             prefix: SharedPrefix, *, k_amax: torch.Tensor | None = None, v_amax: torch.Tensor | None = None,
                             scale: float | None = None) -> torch.Tensor:
     """`paged_attention` of a batch in which groups of sequences share a prefix: its keys are attended to by all rows of a group at once, and read
-    once for up to 128 of them; the keys behind it through each sequence's own line of the table.  A sequence with fewer tokens than
+    once for each 128 or 256 of them, as the plan finds shorter; the keys behind it through each sequence's own line of the table.  A sequence with fewer tokens than
     its group's prefix is attended to through its own line alone."""
     if prefix.batch != q.shape[0]:
         raise ValueError(f"the prefixes are those of a batch of {prefix.batch}, q is {tuple(q.shape)}")
