@@ -202,6 +202,10 @@ def _common(a: list, b: list) -> int:
 #                                      64: 1 23.0 / 35.8, 2 31.0 / 36.1, 3 36.4 / 36.1, 4 41.0 / 35.9      256: 1 41.2 / 46.0, 2 46.8 / 45.2
 #   8 x 8 of 128, 8 bits               64: 2 32.9 / 40.0, 4 43.0 / 43.9      256: 2 49.9 / 59.0, 3 55.3 / 60.2, 4 59.4 / 60.6
 #   1 x 4 of 64, 8 bits                2: 3 38.9 / 46.1, 6 59.0 / 69.8
+# Pages that are no multiple of eight rows are copied by threads, which takes what five (8-bit pages: some seventeen) readings by paged_attention take: there, groups
+# of fewer than 16 (64) sequences count next to nothing, and larger ones of 8-bit pages half.  Pages of 7 rows, 8 kv heads x 4 of 128:
+#   16 bits                            4: 4 51.0 / 64.3, 12 112 / 142      16: 2 28.7 / 29.2, 4 41.0 / 33.8      64: 4 43.0 / 33.8      256: 2 47.1 / 44.8
+#   8 bits                             4: 4 47.5 / 140, 12 105 / 364       16: 4 41.0 / 48.2, 40 246 / 271       64: 4 43.2 / 44.1, 12 86.1 / 54.5      256: 4 57.6 / 54.2
 _SHARED_KEYS = 1 << 17
 
 _WHOLE = "prompts are attended to as a whole: a sequence that brings tokens must hold no older ones"
@@ -531,6 +535,13 @@ class PagedKvCache:
             raise
         have(pages)
 
+    def _counts(self, n: int) -> float:
+        """How much of what a group of n sequences reads once counts."""
+        codes = self.k[0].element_size() == 1
+        if self.page_size % 8:
+            return (1 / 2 if n >= 64 else 1 / 64) if codes else (1 if n >= 16 else 1 / 32)
+        return 0 if codes and n == 2 else 1
+
     def _worth(self) -> bool:
         keys, n = self._saved
         many, codes = n > 8 and n * self.n_kv < 1024, self.k[0].element_size() == 1
@@ -545,8 +556,7 @@ class PagedKvCache:
         members = [m for m in first.values() if len(m) > 1]
         # pages that all of a group have in common and that are full
         shared = [self.page_size * min(min(_common(self._pages[m[0]], self._pages[b]), self._tokens[b] // self.page_size) for b in m) for m in members]
-        codes = self.k[0].element_size() == 1
-        self._saved = self.n_kv * sum((len(m) - 1) * t for m, t in zip(members, shared) if len(m) > 2 or not codes), sum(len(m) for m in members)
+        self._saved = self.n_kv * sum((len(m) - 1) * t * self._counts(len(m)) for m, t in zip(members, shared)), sum(len(m) for m in members)
         self._shares = self._worth()
         if self._prefix is None and members:
             self._prefix = SharedPrefix([], [], self.batch, self.table.device, groups=self.batch // 2, largest=self.batch)

@@ -158,3 +158,15 @@ def test_the_scratch_of_a_cache_goes_by_its_batch(b200, batch, n_q, n_kv, most):
     from tensorrt_b200 import _lib
 
     assert _lib.load().b200q_shared_prefix_workspace_bytes(batch, n_q, n_kv, 128, batch // 2, batch) <= most << 20
+
+
+@pytest.mark.parametrize("n,tokens,codes,shares", [(4, 22000, False, False), (4, 65000, False, False), (16, 2191, False, True), (64, 518, False, True), (4, 65000, True, False),
+                                                   (16, 43680, True, False), (64, 1036, True, False), (64, 3115, True, True), (256, 259, True, True)])
+def test_the_choice_goes_by_the_rows_of_a_page_too(b200, n, tokens, codes, shares):
+    """Pages of seven rows, which no tensor map takes."""
+    amax = dict(dtype=torch.float8_e4m3fn, k_amax=[torch.ones(1)], v_amax=[torch.ones(1)]) if codes else {}
+    cache = b200.PagedKvCache(1, n, 8, 16, pages=1, max_tokens=tokens + 16, page_size=7, device="cpu", **amax)
+    cache._uses, cache._free = [0] * (tokens // 7 + 1), list(range(tokens // 7 + 1))
+    cache.grow([tokens] + [0] * (n - 1))
+    cache.fork([0] * n)
+    assert cache._shares == shares
