@@ -193,8 +193,9 @@ def _common(a: list, b: list) -> int:
 
 # Keys, times kv heads, that a batch's single-token attention has to read once instead of once more for each who shares them, before a cache takes the
 # kernels for shared prefixes.  Three launches, and the parts that they pass on, cost what reading so much costs paged_attention: for up to eight sequences; half
-# as much again for more of them, until paged_attention has 1024 sequences x kv heads to begin and end, which costs it as much; twice that with 8-bit
-# pages, whose rows and queries have to be converted first (three times from eight query heads of a kv head on) and where two sequences never gain.  Measured, paged / shared, in us at multiples of 2^17 keys x kv heads:
+# as much again for more of them, but for one group where paged_attention has 1024 sequences x kv heads to begin and end, which costs it as much; twice that
+# with 8-bit pages, whose rows and queries have to be converted first (three times from eight query heads of a kv head on).  What two sequences share counts half,
+# and with 8-bit pages, where they do not gain, nothing.  Measured, paged / shared, in us at multiples of 2^17 keys x kv heads:
 #   8 kv heads x 4 of 128, 16 bits     4 sequences: 1 24.6 / 23.0, 2 32.9 / 27.7      16: 1 22.5 / 23.5, 1.5 24.6 / 24.2, 2 26.6 / 25.6
 #                                      64: 1 24.6 / 27.7, 1.5 26.7 / 27.6, 2 30.1 / 27.6, 4 41.0 / 28.3      256: 0.5 41.0 / 37.9, 1 41.0 / 37.9
 #   2 x 4 of 64, 16 bits               4: 1 22.6 / 21.5      16: 1 20.5 / 17.4      64: 1 18.5 / 21.3, 1.5 20.5 / 21.5, 3 26.6 / 21.5
@@ -202,6 +203,9 @@ def _common(a: list, b: list) -> int:
 #                                      64: 1 23.0 / 35.8, 2 31.0 / 36.1, 3 36.4 / 36.1, 4 41.0 / 35.9      256: 1 41.2 / 46.0, 2 46.8 / 45.2
 #   8 x 8 of 128, 8 bits               64: 2 32.9 / 40.0, 4 43.0 / 43.9      256: 2 49.9 / 59.0, 3 55.3 / 60.2, 4 59.4 / 60.6
 #   1 x 4 of 64, 8 bits                2: 3 38.9 / 46.1, 6 59.0 / 69.8
+#   8 x 4 of 128, groups, 16 bits      16 of 4: 1 28.7 / 29.7, 2 37.0 / 34.3      64 of 4: 1 43.0 / 46.3, 2 53.7 / 52.2      32 of 8: 1 41.0 / 39.9
+#                                      2 of 2: 2 45.4 / 44.7      16 of 2: 1 32.9 / 37.4, 2 52.8 / 50.2, 5 121 / 89.1      256 of 2: 1 74.0 / 94.3, 5 144 / 132
+#   8 x 4 of 128, groups, 8 bits       16 of 4: 2 35.5 / 35.9, 3 41.9 / 37.9      64 of 4: 3 57.6 / 57.6      64 of 2: 2 49.2 / 72.8, 5 82.9 / 101
 # Pages that are no multiple of eight rows are copied by threads, which takes what five (8-bit pages: some seventeen) readings by paged_attention take: there, groups
 # of fewer than 16 (64) sequences count next to nothing, and larger ones of 8-bit pages half.  Pages of 7 rows, 8 kv heads x 4 of 128:
 #   16 bits                            4: 4 51.0 / 64.3, 12 112 / 142      16: 2 28.7 / 29.2, 4 41.0 / 33.8      64: 4 43.0 / 33.8      256: 2 47.1 / 44.8
@@ -248,7 +252,7 @@ class PagedKvCache:
         self._free = list(range(pages - 1, -1, -1))
         self._pages: list = [[] for _ in range(batch)]     # of each sequence, in order
         self._uses = [0] * pages                           # sequences that a page is part of
-        self._prefix, self._shares, self._saved, self._n_q = None, False, (0, 0), 0      # `_saved`: keys that are read once, sequences that share them
+        self._prefix, self._shares, self._saved, self._n_q = None, False, (0, 0, 0), 0      # `_saved`: keys that are read once, sequences and groups that share them
         self._tokens = [0] * batch
         self._released: set = set()
         self._padded = None
@@ -540,11 +544,11 @@ class PagedKvCache:
         codes = self.k[0].element_size() == 1
         if self.page_size % 8:
             return (1 / 2 if n >= 64 else 1 / 64) if codes else (1 if n >= 16 else 1 / 32)
-        return 0 if codes and n == 2 else 1
+        return 1 if n > 2 else (0 if codes else 1 / 2)
 
     def _worth(self) -> bool:
-        keys, n = self._saved
-        many, codes = n > 8 and n * self.n_kv < 1024, self.k[0].element_size() == 1
+        keys, n, groups = self._saved
+        many, codes = n > 8 and (groups > 1 or n * self.n_kv < 1024), self.k[0].element_size() == 1
         return keys >= _SHARED_KEYS * (1.5 if many else 1) * ((3 if self._n_q >= 8 * self.n_kv else 2) if codes else 1)
 
     def _share(self) -> None:
@@ -556,7 +560,7 @@ class PagedKvCache:
         members = [m for m in first.values() if len(m) > 1]
         # pages that all of a group have in common and that are full
         shared = [self.page_size * min(min(_common(self._pages[m[0]], self._pages[b]), self._tokens[b] // self.page_size) for b in m) for m in members]
-        self._saved = self.n_kv * sum((len(m) - 1) * t * self._counts(len(m)) for m, t in zip(members, shared)), sum(len(m) for m in members)
+        self._saved = self.n_kv * sum((len(m) - 1) * t * self._counts(len(m)) for m, t in zip(members, shared)), sum(len(m) for m in members), len(members)
         self._shares = self._worth()
         if self._prefix is None and members:
             self._prefix = SharedPrefix([], [], self.batch, self.table.device, groups=self.batch // 2, largest=self.batch)

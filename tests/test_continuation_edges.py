@@ -65,7 +65,7 @@ def test_no_memory_for_the_pools_of_another_size(model, monkeypatch, pages, nth)
 
 @pytest.mark.parametrize("n,n_kv,tokens,codes,shares", [
     (64, 8, 256, False, False), (64, 8, 272, False, False), (64, 8, 400, False, True), (16, 8, 1104, False, False), (16, 8, 1648, False, True), (64, 2, 1056, False, False),
-    (128, 8, 144, False, True), (8, 8, 2352, False, True), (2, 8, 16400, False, True), (8, 8, 2352, True, False), (8, 8, 4688, True, True), (64, 8, 528, True, False),
+    (128, 8, 144, False, True), (8, 8, 2352, False, True), (2, 8, 32752, False, False), (2, 8, 32784, False, True), (8, 8, 2352, True, False), (8, 8, 4688, True, True), (64, 8, 528, True, False),
     (64, 8, 800, True, True), (256, 8, 144, True, True), (256, 8, 112, True, False), (2, 1, 800000, True, False), (3, 1, 140000, True, True)])
 def test_the_choice_goes_by_what_was_measured(b200, n, n_kv, tokens, codes, shares):
     amax = dict(dtype=torch.float8_e4m3fn, k_amax=[torch.ones(1)], v_amax=[torch.ones(1)]) if codes else {}
@@ -169,4 +169,16 @@ def test_the_choice_goes_by_the_rows_of_a_page_too(b200, n, tokens, codes, share
     cache._uses, cache._free = [0] * (tokens // 7 + 1), list(range(tokens // 7 + 1))
     cache.grow([tokens] + [0] * (n - 1))
     cache.fork([0] * n)
+    assert cache._shares == shares
+
+
+@pytest.mark.parametrize("groups,per,tokens,codes,shares", [(16, 4, 336, False, False), (16, 4, 528, False, True), (64, 4, 80, False, False), (64, 4, 160, False, True), (16, 2, 2048, False, False),
+                                                           (16, 2, 3200, False, True), (16, 4, 672, True, False), (16, 4, 1040, True, True), (64, 2, 1280, True, False)])
+def test_the_choice_goes_by_the_groups_too(b200, groups, per, tokens, codes, shares):
+    amax = dict(dtype=torch.float8_e4m3fn, k_amax=[torch.ones(1)], v_amax=[torch.ones(1)]) if codes else {}
+    n, pages = groups * per, groups * (tokens // 16)
+    cache = b200.PagedKvCache(1, n, 8, 16, pages=1, max_tokens=tokens + 16, page_size=16, device="cpu", **amax)
+    cache._uses, cache._free = [0] * pages, list(range(pages))
+    cache.grow([0 if b % per else tokens for b in range(n)])
+    cache.fork([b - b % per for b in range(n)])
     assert cache._shares == shares
