@@ -87,7 +87,8 @@ class SharedPrefix:
 
     Groups of one sequence and prefixes of no token are left out: nothing is shared.  The first call of every pair of head counts makes a plan of the work
     on the host, outside a stream capture, and has it on the device before it returns, so that calls on any stream find it there.  `update` says anew who shares what,
-    in place, so that a captured call goes by it; it takes up to `groups` groups of up to `largest` sequences (None: those given here)."""
+    in place, so that a captured call goes by it; it takes up to `groups` groups of up to `largest` sequences (None: those given here).  A captured call reads the plan
+    of this object: keep it as long as the graph."""
 
     def __init__(self, members: list, tokens: list, batch: int, device="cuda", groups: int | None = None, largest: int | None = None):
         if batch < 0 or batch > 65535:
@@ -151,9 +152,10 @@ class SharedPrefix:
             else:
                 if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("the plan of a shared prefix is made on the host: call once with these heads before the capture")
-                plan = self._made(n_q, n_kv)
-                if self.device.type == "cuda":              # on a stream of its own, waited for: the next call may be on any
-                    plan = _native.uploaded(plan, torch.cuda.current_device() if self.device.index is None else self.device.index)
+                with torch.inference_mode(False):           # `update` may be called outside the mode that this call is in
+                    plan = self._made(n_q, n_kv)
+                    if self.device.type == "cuda":          # on a stream of its own, waited for: the next call may be on any
+                        plan = _native.uploaded(plan, torch.cuda.current_device() if self.device.index is None else self.device.index)
             self._plans[n_q, n_kv] = plan
         return plan
 

@@ -182,3 +182,15 @@ def test_the_choice_goes_by_the_groups_too(b200, groups, per, tokens, codes, sha
     cache.grow([0 if b % per else tokens for b in range(n)])
     cache.fork([b - b % per for b in range(n)])
     assert cache._shares == shares
+
+
+def test_a_plan_made_in_inference_mode_can_be_updated(b200):
+    """A step in inference mode, the fork behind it outside."""
+    prefix = b200.SharedPrefix([[0, 1]], [16], 4, device="cpu")
+    with torch.inference_mode():
+        plan = prefix.plan(8, 2)
+    prefix.update([[2, 3]], [640])
+    assert prefix.plan(8, 2) is plan and plan.tolist() == make_plan([[2, 3]], [640], 4, 8, 2)[1]
+    with torch.inference_mode():
+        prefix.update([[0, 3]], [64])
+    assert plan.tolist() == make_plan([[0, 3]], [64], 4, 8, 2)[1]
