@@ -421,7 +421,7 @@ class PagedKvCache:
         for old in self._pages:
             self._give_back(old)
         self._pages, self._tokens = fresh, [min(keep, t) for t in self._tokens]
-        self._new = [0] * self.batch
+        self._new, self._rows = [0] * self.batch, 0      # `grow` comes before the next `append`
         self._share()
         return kept
 
@@ -464,7 +464,7 @@ class PagedKvCache:
         for b in moved:
             self._give_back(self._pages[b][same[b]:])
         self._released = {b for b, p in enumerate(parents) if p in self._released}
-        self._tokens, self._new, self._rows = [self._tokens[p] for p in parents], [0] * self.batch, 0      # `grow` comes before the next `append`
+        self._tokens, self._new, self._rows = [self._tokens[p] for p in parents], [0] * self.batch, 0
         for b, pages in held.items():
             self._pages[b] = pages
         width = self.table.shape[1]

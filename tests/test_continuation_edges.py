@@ -194,3 +194,15 @@ def test_a_plan_made_in_inference_mode_can_be_updated(b200):
     with torch.inference_mode():
         prefix.update([[0, 3]], [64])
     assert plan.tolist() == make_plan([[0, 3]], [64], 4, 8, 2)[1]
+
+
+def test_nothing_is_appended_behind_an_eviction_without_room(b200, monkeypatch):
+    import tensorrt_b200.kv_cache as kv
+
+    monkeypatch.setattr(kv, "paged_evict", lambda k, v, table, lens, weights, out, *, keep, recent, sinks: (torch.zeros(3, 2, keep, dtype=torch.int32), lens.clamp(max=keep), weights))
+    cache = b200.PagedKvCache(1, 3, 2, 16, pages=60, max_tokens=64, page_size=8, weights=True, device="cpu")
+    cache.grow([5, 4, 3])
+    cache.evict(2)
+    rows = torch.zeros(12, 2, 16, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="expected the rows of 0 new tokens"):
+        cache.append(0, rows, rows)
